@@ -47,6 +47,7 @@ from .dense_indexer_loss import (  # noqa: F401
     npu_dense_lightning_indexer_grad_kl_loss_triton,
     npu_dense_lightning_indexer_softmax_lse_triton,
 )
+from .flash_attention_paged import flash_attention_paged  # noqa: F401
 from .streaming import bind_host_to_device, host_outputs, sfa_fwd_bwd_from_host  # noqa: F401
 from .autograd import (  # noqa: F401
     IndexerKLLossFunction,

@@ -106,6 +106,21 @@ class DenseIndexerParams(ctypes.Structure):
     ]
 
 
+class AttnPagedParams(ctypes.Structure):
+    _fields_ = [
+        ("query", _p), ("query_rope", _p), ("key_cache", _p), ("key_rope_cache", _p),
+        ("block_table", _p), ("act_q", _p), ("act_k", _p), ("out", _p), ("softmax_max", _p),
+        ("softmax_sum", _p), ("error_flag", _p), ("workspace", _p), ("workspace_bytes", _i64),
+        ("batch", _i64), ("s1", _i64), ("n1", _i64), ("d", _i64), ("num_pages", _i64),
+        ("page_size", _i64), ("max_blocks", _i64),
+        ("q_batch_stride", _i64), ("q_token_stride", _i64), ("q_head_stride", _i64),
+        ("qr_batch_stride", _i64), ("qr_token_stride", _i64), ("qr_head_stride", _i64),
+        ("k_page_stride", _i64), ("k_row_stride", _i64),
+        ("kr_page_stride", _i64), ("kr_row_stride", _i64),
+        ("scale", ctypes.c_float), ("sparse_mode", ctypes.c_int32), ("dtype", ctypes.c_int32),
+    ]
+
+
 _lock = threading.Lock()
 _lib = None
 _err_bufs: dict = {}
@@ -152,6 +167,10 @@ def lib() -> ctypes.CDLL:
                     fn.restype = ctypes.c_int
                 l.dsa_dense_indexer_workspace_size.argtypes = [_i64] * 4
                 l.dsa_dense_indexer_workspace_size.restype = _i64
+                l.dsa_attn_paged.argtypes = [ctypes.POINTER(AttnPagedParams), _p]
+                l.dsa_attn_paged.restype = ctypes.c_int
+                l.dsa_attn_paged_workspace_size.argtypes = [_i64] * 4
+                l.dsa_attn_paged_workspace_size.restype = _i64
                 _lib = l
     return _lib
 
@@ -180,7 +199,8 @@ def check_device_errors(device=None) -> None:
     if v:
         buf.zero_()
         raise RuntimeError(f"dsa kernel reported device error bits 0x{v:x} "
-                           "(bit1: bounded wait timed out, bit3: misaligned shared memory)")
+                           "(bit1: bounded wait timed out, bit2: an index or position outside its "
+                           "tensor, bit3: misaligned shared memory)")
 
 
 def ptr(t) -> int:

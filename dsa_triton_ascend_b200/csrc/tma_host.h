@@ -67,6 +67,27 @@ inline bool make_tmap_3d_16b(CUtensorMap* map, const void* base, bool is_bf16, u
   return r == CUDA_SUCCESS;
 }
 
+// Map of `rank` dims over a 16-bit tensor: dims[0] is contiguous, strides[i] is the byte stride
+// of dims[i + 1]; 128-byte swizzle.
+inline bool make_tmap_16b(CUtensorMap* map, const void* base, bool is_bf16, uint32_t rank,
+                          const uint64_t* dims, const uint64_t* strides, const uint32_t* box) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (!fn || rank < 2 || rank > 5) return false;
+  cuuint64_t d[5], s[4];
+  cuuint32_t b[5], estr[5];
+  for (uint32_t i = 0; i < rank; ++i) {
+    d[i] = dims[i];
+    b[i] = box[i];
+    estr[i] = 1;
+    if (i + 1 < rank) s[i] = strides[i];
+  }
+  CUresult r = fn(map, is_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                  rank, const_cast<void*>(base), d, s, b, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS;
+}
+
 // 8-bit elements (fp8): the same 3-D tiled map with 1-byte elements
 inline bool make_tmap_3d_8b(CUtensorMap* map, const void* base, uint64_t d0, uint64_t d1,
                             uint64_t d2, uint64_t s1, uint64_t s2, uint32_t b0, uint32_t b1,

@@ -396,6 +396,58 @@ int dsa_dense_indexer_softmax_lse(const DsaDenseIndexerParams* params, void* str
 int dsa_dense_indexer_grad_kl_loss(const DsaDenseIndexerParams* params, void* stream);
 int64_t dsa_dense_indexer_workspace_size(int64_t batch, int64_t s1, int64_t s2, int64_t d_index);
 
+/*
+ * Attention of new tokens over the whole paged latent cache (MLA-absorb: value =
+ * key[..., :d], one key head), the dense counterpart of dsa_sfa_fwd's paged form.  No
+ * counterpart in the reference.
+ *   query [batch][s1][n1][d] (d 128 / 256 / 512, n1 1..128), query_rope [batch][s1][n1][64],
+ *   key_cache [num_pages][page_size][d], key_rope_cache [num_pages][page_size][64], bf16/fp16.
+ *   The last dim of each is contiguous; the other strides are given in elements and are
+ *   multiples of 8; bases are 16-byte aligned.  page_size is a multiple of 8.
+ *   block_table [batch][max_blocks] int32, act_k [batch]: key position t of batch b is row
+ *   t % page_size of page block_table[b][t / page_size]; a negative entry holds no keys, an
+ *   entry >= num_pages is treated so and reported in error_flag.
+ *   act_q [batch] (NULL: s1).  Row (b, s) sees key positions t < min(act_k, max_blocks *
+ *   page_size), in sparse_mode 3 also t < act_k - act_q + s + 1; rows s >= act_q see none.
+ * Rows of a page past the row's keys are not used, whatever they hold.
+ * Outputs: out [batch][s1][n1][d]; softmax_max / softmax_sum [batch][s1][n1] fp32 (both NULL
+ * to skip) as in dsa_sfa_fwd; rows without keys get zeros.  The result does not depend on
+ * timing: the parts of a split row are joined in one order.
+ * Workspace: dsa_attn_paged_workspace_size() bytes (for the current device), 16-byte aligned.
+ */
+typedef struct DsaAttnPagedParams {
+  const void* query;
+  const void* query_rope;
+  const void* key_cache;
+  const void* key_rope_cache;
+  const int32_t* block_table;
+  const int32_t* act_q;
+  const int32_t* act_k;
+  void* out;
+  float* softmax_max;
+  float* softmax_sum;
+  int* error_flag;
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t batch;
+  int64_t s1;
+  int64_t n1;
+  int64_t d;
+  int64_t num_pages;
+  int64_t page_size;
+  int64_t max_blocks;
+  int64_t q_batch_stride, q_token_stride, q_head_stride;
+  int64_t qr_batch_stride, qr_token_stride, qr_head_stride;
+  int64_t k_page_stride, k_row_stride;
+  int64_t kr_page_stride, kr_row_stride;
+  float scale;
+  int32_t sparse_mode;
+  int32_t dtype;
+} DsaAttnPagedParams;
+
+int dsa_attn_paged(const DsaAttnPagedParams* params, void* stream);
+int64_t dsa_attn_paged_workspace_size(int64_t batch, int64_t s1, int64_t n1, int64_t d);
+
 #ifdef __cplusplus
 }
 #endif
