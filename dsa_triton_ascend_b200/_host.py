@@ -97,3 +97,32 @@ def require_cuda(*ts) -> None:
 
 def is_pow2_block(bs: int) -> bool:
     return 1 <= bs <= 128 and (bs & (bs - 1)) == 0
+
+
+def _extent(t: torch.Tensor):
+    """First and last byte address that a (non-negatively strided) tensor covers, or None."""
+    if t.numel() == 0:
+        return None
+    last = sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + last * t.element_size() + t.element_size() - 1
+
+
+def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the address ranges of two tensors meet (interleaved views count as meeting),
+    unless they are one and the same view."""
+    ea, eb = _extent(a), _extent(b)
+    if ea is None or eb is None:
+        return False
+    if a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.stride() == b.stride():
+        return False
+    return ea[0] <= eb[1] and eb[0] <= ea[1]
+
+
+def self_overlap(t: torch.Tensor) -> bool:
+    """Whether two indices of a tensor may name one address (an expanded tensor, say)."""
+    reach = 0
+    for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n > 1):
+        if st <= reach:
+            return True
+        reach += st * (n - 1)
+    return False

@@ -121,6 +121,54 @@ class AttnPagedParams(ctypes.Structure):
     ]
 
 
+class RotaryParams(ctypes.Structure):
+    _fields_ = [
+        ("x", _p), ("out", _p), ("positions", _p), ("table", _p), ("error_flag", _p),
+        ("batch", _i64), ("s", _i64), ("heads", _i64), ("head_dim", _i64), ("offset", _i64),
+        ("dim", _i64), ("max_positions", _i64),
+        ("x_batch_stride", _i64), ("x_token_stride", _i64), ("x_head_stride", _i64),
+        ("out_batch_stride", _i64), ("out_token_stride", _i64), ("out_head_stride", _i64),
+        ("half_layout", ctypes.c_int32), ("inverse", ctypes.c_int32), ("dtype", ctypes.c_int32),
+    ]
+
+
+ROTARY_CODES = {None: 0, "interleaved": 1, "half": 2}   # DSA_ROTARY_*
+APPEND_MAX_ENTRIES = 4                                  # DSA_APPEND_MAX_ENTRIES
+PAGES_COPY, PAGES_FORK, PAGES_EXTEND, PAGES_FREE, PAGES_COMPACT = range(5)   # DSA_PAGES_*
+
+
+class CacheRows(ctypes.Structure):
+    _fields_ = [
+        ("src", _p), ("cache", _p), ("src_batch_stride", _i64), ("src_token_stride", _i64),
+        ("page_stride", _i64), ("row_stride", _i64), ("width_bytes", _i64), ("offset", _i64),
+        ("rotary", ctypes.c_int32), ("dtype", ctypes.c_int32),
+    ]
+
+
+class CacheAppendParams(ctypes.Structure):
+    _fields_ = [
+        ("rows", CacheRows * APPEND_MAX_ENTRIES), ("block_table", _p), ("starts", _p),
+        ("counts", _p), ("table", _p), ("error_flag", _p), ("batch", _i64), ("s", _i64),
+        ("num_pages", _i64), ("page_size", _i64), ("max_blocks", _i64), ("max_positions", _i64),
+        ("dim", _i64), ("entries", ctypes.c_int32),
+    ]
+
+
+class PageCache(ctypes.Structure):
+    _fields_ = [("data", _p), ("page_stride", _i64), ("row_stride", _i64), ("row_bytes", _i64)]
+
+
+class PagesParams(ctypes.Structure):
+    _fields_ = [
+        ("block_table", _p), ("seq_lengths", _p), ("ref_counts", _p), ("block_table_out", _p),
+        ("seq_lengths_out", _p), ("ref_counts_out", _p), ("first", _p), ("second", _p),
+        ("caches", ctypes.POINTER(PageCache)), ("error_flag", _p), ("workspace", _p),
+        ("workspace_bytes", _i64), ("n", _i64), ("slots", _i64), ("max_blocks", _i64),
+        ("num_pages", _i64), ("page_size", _i64), ("num_caches", ctypes.c_int32),
+        ("op", ctypes.c_int32),
+    ]
+
+
 _lock = threading.Lock()
 _lib = None
 _err_bufs: dict = {}
@@ -171,6 +219,17 @@ def lib() -> ctypes.CDLL:
                 l.dsa_attn_paged.restype = ctypes.c_int
                 l.dsa_attn_paged_workspace_size.argtypes = [_i64] * 4
                 l.dsa_attn_paged_workspace_size.restype = _i64
+                l.dsa_rotary.argtypes = [ctypes.POINTER(RotaryParams), _p]
+                l.dsa_rotary.restype = ctypes.c_int
+                l.dsa_rotary_table.argtypes = [_p, _i64, _i64, ctypes.POINTER(ctypes.c_double),
+                                               ctypes.c_double, _p]
+                l.dsa_rotary_table.restype = ctypes.c_int
+                l.dsa_cache_append.argtypes = [ctypes.POINTER(CacheAppendParams), _p]
+                l.dsa_cache_append.restype = ctypes.c_int
+                l.dsa_pages.argtypes = [ctypes.POINTER(PagesParams), _p]
+                l.dsa_pages.restype = ctypes.c_int
+                l.dsa_pages_workspace_size.argtypes = [ctypes.c_int32, _i64, _i64, _i64]
+                l.dsa_pages_workspace_size.restype = _i64
                 _lib = l
     return _lib
 
@@ -200,7 +259,7 @@ def check_device_errors(device=None) -> None:
         buf.zero_()
         raise RuntimeError(f"dsa kernel reported device error bits 0x{v:x} "
                            "(bit1: bounded wait timed out, bit2: an index or position outside its "
-                           "tensor, bit3: misaligned shared memory)")
+                           "tensor, bit3: misaligned shared memory, bit4: no free page left)")
 
 
 def ptr(t) -> int:

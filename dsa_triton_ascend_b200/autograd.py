@@ -14,6 +14,8 @@ torch:
 * :class:`SparseAttentionWithIndexer` -- lightning indexer (top-k, not differentiated)
   -> sparse attention -> indexer KL loss, the training-time composition of a DSA layer
   (cf. dsa_torch.py:111-151).
+* :class:`RotaryEmbeddingFunction` -- rotary positions on queries and keys; the gradient is
+  the inverse rotation.
 """
 from __future__ import annotations
 
@@ -22,6 +24,7 @@ import torch
 from . import _host as H
 
 from .lightning_indexer import lightning_indexer_triton
+from .rotary_embedding import rotary_embedding
 from .sparse_flash_attention import sparse_flash_attention_triton
 from .sparse_flash_attention_grad import sparse_flash_attention_grad_merged
 from .sparse_lightning_indexer_grad_kl_loss import sparse_lightning_indexer_grad_kl_loss_triton
@@ -167,3 +170,21 @@ class SparseAttentionWithIndexer(torch.nn.Module):
             query_index, key_index, weights, query.detach(), key.detach(), query_rope.detach(),
             key_rope.detach(), sparse_indices, smax, ssum, self.scale_value)
         return out, loss
+
+
+class RotaryEmbeddingFunction(torch.autograd.Function):
+    """out = rotary_embedding(x, table, positions, layout, offset); the gradient of ``x`` turns
+    back by the same table (amplitude kept), nothing of the forward but the positions is saved."""
+
+    @staticmethod
+    def forward(ctx, x, table, positions, layout="interleaved", offset=0):
+        ctx.save_for_backward(table, positions)
+        ctx.cfg = (layout, offset)
+        return rotary_embedding(x, table, positions, layout=layout, offset=offset)
+
+    @staticmethod
+    def backward(ctx, d_out):
+        table, positions = ctx.saved_tensors
+        layout, offset = ctx.cfg
+        return rotary_embedding(d_out, table, positions, layout=layout, offset=offset,
+                                inverse=True), None, None, None, None

@@ -1,0 +1,585 @@
+// The pages of a cache: appending new tokens, and copying, forking, growing, compacting and
+// freeing pages.
+//
+// A pool of num_pages pages is described by int32 state on the device: block_table
+// [slots][max_blocks] (page of each block of a sequence, -1 where there is none), seq_lengths
+// [slots], ref_counts [num_pages] (sequences that hold a page; 0: free).  One table serves
+// every cache of the pool (layers; latent, rotary and index keys).  The bookkeeping calls read
+// that state and write a new one, so nothing waits for the host and a call can be captured;
+// the page data is moved in place.  Pages are handed out lowest id first.
+//
+// A call is two launches: page_plan_kernel (one block) finds the pages with prefix sums over
+// ref_counts, page_apply_kernel (the whole GPU) writes the new table and moves the data.
+#include <cuda_runtime.h>
+
+#include "dsa_b200.h"
+#include "rotary.cuh"
+
+namespace dsa {
+namespace pages {
+
+// ---------------------------------------------------------------------------------------
+// append
+// ---------------------------------------------------------------------------------------
+constexpr int kAppendThreads = 256;
+
+struct AppendArgs {
+  DsaCacheRows e[DSA_APPEND_MAX_ENTRIES];
+  uint32_t first[DSA_APPEND_MAX_ENTRIES + 1];   // first piece of each entry
+  const int32_t* block_table;
+  const int32_t* starts;
+  const int32_t* counts;
+  const float* table;
+  int* error_flag;
+  int64_t token0;
+  uint32_t items, units;
+  int32_t entries, s, page_size, max_blocks, num_pages, max_positions, dim;
+};
+
+// One 16-byte piece of a token's rows (a pair of pieces in the half layout) per thread.
+template <typename T>
+__device__ __forceinline__ void append_piece(const AppendArgs& a, const DsaCacheRows& e, const char* src,
+                                             char* dst, int u, int pos) {
+  constexpr int kN = rotary::Vec<T>::kN;
+  const int half = a.dim / 2;
+  const float* row = a.table + (int64_t)pos * a.dim;
+  if (e.rotary == DSA_ROTARY_INTERLEAVED) {
+    const int at = u * kN, in = at - e.offset;
+    uint4 v = *reinterpret_cast<const uint4*>(src + at * sizeof(T));
+    if (in >= 0 && in < a.dim) {
+      float cs[kN / 2], sn[kN / 2];
+      rotary::load_angles<kN / 2>(row, half, in / 2, 1.0f, cs, sn);
+      v = rotary::turn_interleaved<T>(v, cs, sn);
+    }
+    *reinterpret_cast<uint4*>(dst + at * sizeof(T)) = v;
+    return;
+  }
+  const int pairs = half / kN;
+  if (u < pairs) {
+    const int at = e.offset + u * kN;
+    uint4 lo = *reinterpret_cast<const uint4*>(src + at * sizeof(T));
+    uint4 hi = *reinterpret_cast<const uint4*>(src + (at + half) * sizeof(T));
+    float cs[kN], sn[kN];
+    rotary::load_angles<kN>(row, half, u * kN, 1.0f, cs, sn);
+    rotary::turn_half<T>(lo, hi, cs, sn);
+    *reinterpret_cast<uint4*>(dst + at * sizeof(T)) = lo;
+    *reinterpret_cast<uint4*>(dst + (at + half) * sizeof(T)) = hi;
+    return;
+  }
+  int at = (u - pairs) * kN;
+  if (at >= e.offset) at += a.dim;
+  *reinterpret_cast<uint4*>(dst + at * sizeof(T)) = *reinterpret_cast<const uint4*>(src + at * sizeof(T));
+}
+
+__global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ AppendArgs a) {
+  const uint32_t item = blockIdx.x * kAppendThreads + threadIdx.x;
+  if (item >= a.items) return;
+  const uint32_t tok = item / a.units, u = item - tok * a.units;
+  const int64_t token = a.token0 + tok, b = token / a.s;
+  const int s = (int)(token - b * a.s);
+  if (a.counts && s >= a.counts[b]) return;
+  const int64_t pos = (int64_t)a.starts[b] + s;
+  int32_t page = -1;
+  if (pos >= 0 && pos < (int64_t)a.max_blocks * a.page_size)
+    page = a.block_table[b * a.max_blocks + pos / a.page_size];
+  if (page < 0 || page >= a.num_pages || (a.table && pos >= a.max_positions)) {
+    if (u == 0) report_error(a.error_flag, kErrBadIndex);
+    return;
+  }
+  int i = 0;
+  while (i + 1 < a.entries && u >= a.first[i + 1]) ++i;
+  const DsaCacheRows& e = a.e[i];
+  const int in = (int)(u - a.first[i]);
+  const char* src = static_cast<const char*>(e.src) + b * e.src_batch_stride + s * e.src_token_stride;
+  char* dst = static_cast<char*>(e.cache) + page * e.page_stride + (pos % a.page_size) * e.row_stride;
+  if (e.rotary == DSA_ROTARY_NONE)
+    reinterpret_cast<uint4*>(dst)[in] = reinterpret_cast<const uint4*>(src)[in];
+  else if (e.dtype == DSA_DTYPE_BF16)
+    append_piece<__nv_bfloat16>(a, e, src, dst, in, (int)pos);
+  else if (e.dtype == DSA_DTYPE_FP16)
+    append_piece<__half>(a, e, src, dst, in, (int)pos);
+  else
+    append_piece<float>(a, e, src, dst, in, (int)pos);
+}
+
+// ---------------------------------------------------------------------------------------
+// bookkeeping
+// ---------------------------------------------------------------------------------------
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanWarps = kPlanThreads / 32;
+constexpr int kApplyThreads = 256;
+constexpr int kMaxCaches = 32;              // caches of one apply launch
+constexpr int kSliceBytes = 16384;          // of a page, per block and turn
+
+struct PoolArgs {
+  const int32_t* table;
+  const int32_t* lens;
+  const int32_t* refs;
+  int32_t* table_out;
+  int32_t* lens_out;
+  int32_t* refs_out;
+  const int32_t* first;    // fork: parents, extend: counts, free: rows, copy: source pages
+  const int32_t* second;   // fork: children, copy: destination pages
+  int* error_flag;
+  int32_t* header;         // [0] page copies
+  int32_t* mark;           // [slots] fork: the fork that makes the row; free: 1; extend: first page
+  int32_t* list_a;         // source pages (compact, fork), free pages (extend)
+  int32_t* list_b;         // destination pages (compact, fork)
+  int32_t* list_c;         // rows of the page that a fork copies; compact: new id of each page
+  int32_t op, n, slots, max_blocks, num_pages, page_size;
+};
+
+__device__ __forceinline__ int plan_scan(int v, int* tmp, int* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();
+  if (lane == 31) tmp[warp] = x;
+  __syncthreads();
+  int t = tmp[lane];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, t, o);
+    if (lane >= o) t += y;
+  }
+  *total = __shfl_sync(0xffffffffu, t, 31);
+  const int before = __shfl_sync(0xffffffffu, t, warp) - tmp[warp];
+  return before + x - v;
+}
+
+// Calls f(page, rank) for the pages that `pick` takes, ranked by id, up to `limit` of them;
+// returns how many there are.  Each warp takes a run of ids.
+template <typename Pick, typename F>
+__device__ int rank_pages(int num_pages, int limit, int* tmp, Pick pick, F f) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int run = ((num_pages + kPlanWarps * 32 - 1) / (kPlanWarps * 32)) * 32;
+  const int from = min(num_pages, warp * run), to = min(num_pages, from + run);
+  int count = 0;
+#pragma unroll 8
+  for (int p = from + lane; p < to; p += 32) count += pick(p) ? 1 : 0;
+  count = __reduce_add_sync(0xffffffffu, count);
+  int total;
+  const int at = plan_scan(lane == 0 ? count : 0, tmp, &total);
+  int rank = __shfl_sync(0xffffffffu, at, 0);
+  for (int p0 = from; p0 < to && rank < limit; p0 += 32) {
+    const int p = p0 + lane;
+    const bool yes = p < to && pick(p);
+    const uint32_t m = __ballot_sync(0xffffffffu, yes);
+    const int r = rank + __popc(m & ((1u << lane) - 1u));
+    if (yes && r < limit) f(p, r);
+    rank += __popc(m);
+  }
+  return total;
+}
+
+__device__ __forceinline__ int blocks_of(int64_t tokens, int page_size) {
+  return (int)((tokens + page_size - 1) / page_size);
+}
+
+__global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PoolArgs a) {
+  __shared__ int tmp[kPlanWarps];
+  __shared__ int run_total;
+  const int tid = threadIdx.x;
+  griddep_launch_dependents();
+  if (tid == 0) a.header[0] = 0;
+  auto is_free = [&](int p) { return a.refs[p] <= 0; };
+  bool bad = false, full = false;
+
+  if (a.op == DSA_PAGES_COMPACT) {
+    // live pages beyond the first n_live ids move, in order, to the free ids among those
+    int live = 0;
+    for (int p = tid; p < a.num_pages; p += kPlanThreads) {
+      a.list_c[p] = p;
+      const int r = a.refs[p];
+      a.refs_out[p] = r;
+      live += r > 0 ? 1 : 0;
+    }
+    int total;
+    plan_scan(live, tmp, &total);
+    const int n_live = total;
+    __syncthreads();
+    const int moved = rank_pages(a.num_pages, a.num_pages, tmp,
+                                 [&](int p) { return p >= n_live && a.refs[p] > 0; },
+                                 [&](int p, int r) { a.list_a[r] = p; });
+    rank_pages(a.num_pages, a.num_pages, tmp, [&](int p) { return p < n_live && a.refs[p] <= 0; },
+               [&](int p, int r) { a.list_b[r] = p; });
+    __syncthreads();
+    for (int i = tid; i < moved; i += kPlanThreads) {
+      const int from = a.list_a[i], to = a.list_b[i];
+      a.list_c[from] = to;
+      a.refs_out[to] = a.refs[from];
+      a.refs_out[from] = 0;
+    }
+    if (tid == 0) a.header[0] = moved;
+    return;
+  }
+
+  for (int p = tid; p < a.num_pages; p += kPlanThreads) a.refs_out[p] = a.refs[p];
+  if (a.op == DSA_PAGES_FREE) {
+    for (int r = tid; r < a.slots; r += kPlanThreads) a.mark[r] = 0;
+    __syncthreads();
+    for (int i = tid; i < a.n; i += kPlanThreads) {
+      const int r = a.first[i];
+      if (r >= 0 && r < a.slots) a.mark[r] = 1;
+      else bad = true;
+    }
+  } else if (a.op == DSA_PAGES_EXTEND) {
+    // row r grows to lens + counts tokens; the pages it needs are a run of the free ones
+    if (tid == 0) run_total = 0;
+    __syncthreads();
+    const int free_pages = rank_pages(a.num_pages, a.num_pages, tmp, is_free,
+                                      [&](int p, int r) { a.list_a[r] = p; });
+    for (int r0 = 0; r0 < a.slots; r0 += kPlanThreads) {
+      const int r = r0 + tid;
+      int need = 0;
+      bool grows = false;
+      int64_t len = 0, more = 0;
+      if (r < a.slots) {
+        len = a.lens[r];
+        more = a.first[r];
+        grows = more >= 0 && len >= 0 && len + more <= (int64_t)a.max_blocks * a.page_size;
+        bad |= !grows;
+        if (grows) need = blocks_of(len + more, a.page_size) - blocks_of(len, a.page_size);
+      }
+      int sum;
+      const int at = run_total + plan_scan(need, tmp, &sum);
+      if (r < a.slots) {
+        const bool fits = need == 0 || at + need <= free_pages;
+        full |= !fits;
+        grows = grows && fits;
+        a.lens_out[r] = (int)(grows ? len + more : len);
+        a.mark[r] = at;
+        if (grows)
+          for (int j = 0; j < need; ++j) a.refs_out[a.list_a[at + j]] = 1;
+      }
+      __syncthreads();
+      if (tid == 0) run_total += sum;
+      __syncthreads();
+    }
+  } else {   // DSA_PAGES_FORK
+    for (int r = tid; r < a.slots; r += kPlanThreads) a.mark[r] = 0x7fffffff;
+    if (tid == 0) run_total = 0;
+    __syncthreads();
+    // the child must be an empty row; of forks into the same row the first counts
+    auto valid = [&](int i) {
+      const int p = a.first[i], c = a.second[i];
+      if (p < 0 || p >= a.slots || c < 0 || c >= a.slots) return false;
+      const int64_t len = a.lens[p];
+      if (a.lens[c] != 0 || len < 0 || len > (int64_t)a.max_blocks * a.page_size) return false;
+      if (len % a.page_size == 0) return true;
+      const int page = a.table[(int64_t)p * a.max_blocks + len / a.page_size];
+      return page >= 0 && page < a.num_pages;
+    };
+    for (int i = tid; i < a.n; i += kPlanThreads) {
+      if (valid(i)) atomicMin(&a.mark[a.second[i]], i);
+      else bad = true;
+    }
+    __syncthreads();
+    const int free_pages = rank_pages(a.num_pages, min(a.n, a.num_pages), tmp, is_free,
+                                      [&](int p, int r) { a.list_b[r] = p; });
+    __syncthreads();
+    for (int i0 = 0; i0 < a.n; i0 += kPlanThreads) {
+      const int i = i0 + tid;
+      int rest = 0, child = -1;
+      bool mine = false;
+      if (i < a.n) {
+        child = a.second[i];
+        mine = child >= 0 && child < a.slots && a.mark[child] == i;
+        bad |= !mine;
+        if (mine) rest = a.lens[a.first[i]] % a.page_size;
+      }
+      int sum;
+      const int at = run_total + plan_scan(rest > 0 ? 1 : 0, tmp, &sum);
+      if (mine && rest > 0) {
+        if (at < free_pages) {
+          const int parent = a.first[i];
+          a.list_a[at] = a.table[(int64_t)parent * a.max_blocks + a.lens[parent] / a.page_size];
+          a.list_c[at] = rest;
+          a.refs_out[a.list_b[at]] = 1;
+        } else {
+          full = true;
+          a.mark[child] = -1;   // no page left: the child stays empty
+        }
+      }
+      // where the apply kernel finds the child's own page
+      if (mine) a.header[8 + i] = at;
+      __syncthreads();
+      if (tid == 0) {
+        run_total += sum;
+        a.header[0] = min(run_total, free_pages);
+      }
+      __syncthreads();
+    }
+  }
+  if (bad) report_error(a.error_flag, kErrBadIndex);
+  if (full) report_error(a.error_flag, kErrNoPages);
+}
+
+struct Caches {
+  DsaPageCache c[kMaxCaches];
+  int32_t slices[kMaxCaches];   // of kSliceBytes, rounded up, of a whole page
+  int32_t count, total;
+};
+
+// Copy the first `rows` rows of page src to page dst: slice `sl` of cache `c`.
+__device__ __forceinline__ void copy_slice(const DsaPageCache& c, int sl, int64_t src, int64_t dst, int rows) {
+  constexpr int kPieces = kSliceBytes / 16;
+  const int row_pieces = (int)(c.row_bytes / 16);
+  const int64_t all = (int64_t)rows * row_pieces;
+  const char* from = static_cast<const char*>(c.data) + src * c.page_stride;
+  char* to = static_cast<char*>(c.data) + dst * c.page_stride;
+  const bool dense = c.row_stride == c.row_bytes;
+  uint4 v[kPieces / kApplyThreads];
+#pragma unroll
+  for (int k = 0; k < kPieces / kApplyThreads; ++k) {
+    const int64_t i = (int64_t)sl * kPieces + k * kApplyThreads + threadIdx.x;
+    if (i < all) {
+      const int64_t at = dense ? i * 16 : i / row_pieces * c.row_stride + i % row_pieces * 16;
+      v[k] = *reinterpret_cast<const uint4*>(from + at);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kPieces / kApplyThreads; ++k) {
+    const int64_t i = (int64_t)sl * kPieces + k * kApplyThreads + threadIdx.x;
+    if (i < all) {
+      const int64_t at = dense ? i * 16 : i / row_pieces * c.row_stride + i % row_pieces * 16;
+      *reinterpret_cast<uint4*>(to + at) = v[k];
+    }
+  }
+}
+
+__global__ void __launch_bounds__(kApplyThreads)
+    page_apply_kernel(const PoolArgs a, const __grid_constant__ Caches caches, int do_table) {
+  griddep_wait();
+  const int64_t stride = (int64_t)gridDim.x * kApplyThreads;
+  const int64_t me = (int64_t)blockIdx.x * kApplyThreads + threadIdx.x;
+  if (do_table && a.op != DSA_PAGES_COPY) {
+    const int64_t cells = (int64_t)a.slots * a.max_blocks;
+    for (int64_t i = me; i < cells; i += stride) {
+      const int row = (int)(i / a.max_blocks), j = (int)(i - (int64_t)row * a.max_blocks);
+      int v = a.table[i];
+      if (a.op == DSA_PAGES_COMPACT) {
+        if (v >= 0 && v < a.num_pages) v = a.list_c[v];
+      } else if (a.op == DSA_PAGES_FREE) {
+        if (a.mark[row]) {
+          if (v >= 0 && v < a.num_pages) {
+            // a page held more often than it is counted was free already: it stays at 0
+            if (atomicSub(&a.refs_out[v], 1) <= 0) {
+              atomicAdd(&a.refs_out[v], 1);
+              report_error(a.error_flag, kErrBadIndex);
+            }
+          } else if (v >= a.num_pages) {
+            report_error(a.error_flag, kErrBadIndex);
+          }
+          v = -1;
+        }
+        if (j == 0) a.lens_out[row] = a.mark[row] ? 0 : a.lens[row];
+      } else if (a.op == DSA_PAGES_EXTEND) {
+        const int had = blocks_of(a.lens[row], a.page_size), has = blocks_of(a.lens_out[row], a.page_size);
+        if (j >= had && j < has) v = a.list_a[a.mark[row] + j - had];
+      } else {   // fork
+        const int f = a.mark[row];
+        const bool child = f >= 0 && f < a.n;
+        const int len = child ? a.lens[a.first[f]] : a.lens[row];
+        if (child) {
+          const int full = len / a.page_size;
+          v = -1;
+          if (j < full) {
+            v = a.table[(int64_t)a.first[f] * a.max_blocks + j];
+            if (v >= 0 && v < a.num_pages) {
+              atomicAdd(&a.refs_out[v], 1);
+            } else {   // the parent has no such page: neither has the child
+              report_error(a.error_flag, kErrBadIndex);
+              v = -1;
+            }
+          } else if (j == full && len % a.page_size) {
+            v = a.list_b[a.header[8 + f]];
+          }
+        }
+        if (j == 0) a.lens_out[row] = len;
+      }
+      a.table_out[i] = v;
+    }
+  }
+  if (caches.count == 0) return;
+  const int copies = a.op == DSA_PAGES_COPY ? a.n
+                     : a.op == DSA_PAGES_COMPACT || a.op == DSA_PAGES_FORK ? a.header[0] : 0;
+  const int64_t jobs = (int64_t)copies * caches.total;
+  for (int64_t job = blockIdx.x; job < jobs; job += gridDim.x) {
+    const int item = (int)(job / caches.total);
+    int sl = (int)(job - (int64_t)item * caches.total), c = 0;
+    while (sl >= caches.slices[c]) sl -= caches.slices[c++];
+    int src, dst, rows = a.page_size;
+    if (a.op == DSA_PAGES_COPY) {
+      src = a.first[item];
+      dst = a.second[item];
+      if (src < 0 || dst < 0 || src >= a.num_pages || dst >= a.num_pages) {
+        // -1 skips an entry; an id past the pool is an error
+        if (threadIdx.x == 0 && (src >= a.num_pages || dst >= a.num_pages))
+          report_error(a.error_flag, kErrBadIndex);
+        continue;
+      }
+    } else {
+      src = a.list_a[item];
+      dst = a.list_b[item];
+      if (a.op == DSA_PAGES_FORK) rows = a.list_c[item];
+    }
+    if (src != dst) copy_slice(caches.c[c], sl, src, dst, rows);
+  }
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+int64_t align64(int64_t n) { return (n + 63) & ~(int64_t)63; }
+
+}  // namespace pages
+}  // namespace dsa
+
+extern "C" int dsa_cache_append(const DsaCacheAppendParams* p, void* stream_) {
+  using namespace dsa::pages;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  constexpr int64_t kMax = 0x7fffffff;
+  if (!p || p->batch < 0 || p->s < 0) return DSA_ERR_INVALID_ARG;
+  if (p->entries < 1 || p->entries > DSA_APPEND_MAX_ENTRIES || !p->block_table || !p->starts ||
+      p->page_size < 1 || p->page_size > kMax || p->max_blocks < 1 || p->max_blocks > kMax / p->page_size ||
+      p->num_pages < 1 || p->num_pages > kMax || p->batch > kMax || p->s > kMax)
+    return DSA_ERR_INVALID_ARG;
+  AppendArgs a = {};
+  uint32_t units = 0;
+  for (int i = 0; i < p->entries; ++i) {
+    const DsaCacheRows& e = p->rows[i];
+    if (!e.src || !e.cache || e.width_bytes < 16 || e.width_bytes > (1 << 24) || e.width_bytes % 16 ||
+        !aligned16(e.src) || !aligned16(e.cache) || e.src_batch_stride % 16 || e.src_token_stride % 16 ||
+        e.page_stride % 16 || e.row_stride % 16)
+      return DSA_ERR_INVALID_ARG;
+    uint32_t pieces = (uint32_t)(e.width_bytes / 16);
+    if (e.rotary != DSA_ROTARY_NONE) {
+      const int64_t size = e.dtype == DSA_DTYPE_FP32 ? 4 : 2, n = 16 / size;
+      if ((e.dtype != DSA_DTYPE_BF16 && e.dtype != DSA_DTYPE_FP16 && e.dtype != DSA_DTYPE_FP32) ||
+          (e.rotary != DSA_ROTARY_INTERLEAVED && e.rotary != DSA_ROTARY_HALF) || !p->table ||
+          !aligned16(p->table) || p->dim < 8 || p->dim > 256 || p->dim % 8 || e.offset < 0 ||
+          e.offset % n || p->dim % (e.rotary == DSA_ROTARY_HALF ? 2 * n : n) ||
+          (e.offset + p->dim) * size > e.width_bytes || p->max_positions < 1 || p->max_positions > kMax)
+        return DSA_ERR_INVALID_ARG;
+      if (e.rotary == DSA_ROTARY_HALF) pieces -= (uint32_t)(p->dim / 2 / n);
+    }
+    a.e[i] = e;
+    a.first[i] = units;
+    units += pieces;
+  }
+  a.first[p->entries] = units;
+  if (p->batch == 0 || p->s == 0) return DSA_OK;
+  a.block_table = p->block_table;
+  a.starts = p->starts;
+  a.counts = p->counts;
+  a.table = p->table;
+  a.error_flag = p->error_flag;
+  a.units = units;
+  a.entries = p->entries;
+  a.s = (int)p->s;
+  a.page_size = (int)p->page_size;
+  a.max_blocks = (int)p->max_blocks;
+  a.num_pages = (int)p->num_pages;
+  a.max_positions = (int)p->max_positions;
+  a.dim = (int)p->dim;
+  const int64_t tokens = p->batch * p->s, chunk = (1LL << 30) / units;
+  for (int64_t t0 = 0; t0 < tokens; t0 += chunk) {
+    const int64_t n = tokens - t0 < chunk ? tokens - t0 : chunk;
+    a.token0 = t0;
+    a.items = (uint32_t)(n * units);
+    append_kernel<<<(a.items + kAppendThreads - 1) / kAppendThreads, kAppendThreads, 0, stream>>>(a);
+    if (cudaGetLastError() != cudaSuccess) return DSA_ERR_CUDA;
+  }
+  return DSA_OK;
+}
+
+extern "C" int64_t dsa_pages_workspace_size(int32_t op, int64_t n, int64_t slots, int64_t num_pages) {
+  using namespace dsa::pages;
+  if (n < 0 || slots < 0 || num_pages < 0) return -1;
+  if (op == DSA_PAGES_COPY) return 0;
+  return 4 * (align64(8 + (op == DSA_PAGES_FORK ? n : 0)) + align64(slots) + 3 * align64(num_pages));
+}
+
+extern "C" int dsa_pages(const DsaPagesParams* p, void* stream_) {
+  using namespace dsa::pages;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  constexpr int64_t kMax = 0x7fffffff;
+  if (!p || p->op < DSA_PAGES_COPY || p->op > DSA_PAGES_COMPACT) return DSA_ERR_INVALID_ARG;
+  const bool copy = p->op == DSA_PAGES_COPY;
+  if (p->n < 0 || p->n > kMax || p->num_pages < 1 || p->num_pages > kMax || p->page_size < 1 ||
+      p->page_size > kMax || p->num_caches < 0 || (p->num_caches > 0 && !p->caches))
+    return DSA_ERR_INVALID_ARG;
+  if (!copy && (p->slots < 1 || p->slots > kMax || p->max_blocks < 1 ||
+                p->max_blocks > kMax / p->page_size || p->slots > kMax / p->max_blocks || !p->block_table || !p->block_table_out ||
+                !p->ref_counts || !p->ref_counts_out || !p->workspace ||
+                p->workspace_bytes < dsa_pages_workspace_size(p->op, p->n, p->slots, p->num_pages)))
+    return DSA_ERR_INVALID_ARG;
+  if (!copy && p->op != DSA_PAGES_COMPACT && (!p->seq_lengths || !p->seq_lengths_out)) return DSA_ERR_INVALID_ARG;
+  const bool two = copy || p->op == DSA_PAGES_FORK;
+  if (p->op != DSA_PAGES_COMPACT && ((p->n > 0 && !p->first) || (two && p->n > 0 && !p->second)))
+    return DSA_ERR_INVALID_ARG;
+  if (p->op == DSA_PAGES_EXTEND && p->n != p->slots) return DSA_ERR_INVALID_ARG;
+  for (int i = 0; i < p->num_caches; ++i) {
+    const DsaPageCache& c = p->caches[i];
+    if (!c.data || !aligned16(c.data) || c.row_bytes < 16 || c.row_bytes % 16 || c.row_stride % 16 ||
+        c.page_stride % 16 || c.row_bytes > kMax / p->page_size)
+      return DSA_ERR_INVALID_ARG;
+  }
+  if (copy && (p->n == 0 || p->num_caches == 0)) return DSA_OK;
+  PoolArgs a = {};
+  a.table = p->block_table, a.lens = p->seq_lengths, a.refs = p->ref_counts;
+  a.table_out = p->block_table_out, a.lens_out = p->seq_lengths_out, a.refs_out = p->ref_counts_out;
+  a.first = p->first, a.second = p->second;
+  a.error_flag = p->error_flag;
+  if (!copy) {
+    int32_t* ws = static_cast<int32_t*>(p->workspace);
+    a.header = ws;
+    ws += align64(8 + (p->op == DSA_PAGES_FORK ? p->n : 0));
+    a.mark = ws;
+    ws += align64(p->slots);
+    a.list_a = ws;
+    a.list_b = ws + align64(p->num_pages);
+    a.list_c = ws + 2 * align64(p->num_pages);
+  }
+  a.op = p->op;
+  a.n = (int)p->n;
+  a.slots = (int)p->slots;
+  a.max_blocks = (int)p->max_blocks;
+  a.num_pages = (int)p->num_pages;
+  a.page_size = (int)p->page_size;
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return DSA_ERR_CUDA;
+  if (!copy) {
+    page_plan_kernel<<<1, kPlanThreads, 0, stream>>>(a);
+    if (cudaGetLastError() != cudaSuccess) return DSA_ERR_CUDA;
+  }
+  cudaLaunchAttribute pdl[1];
+  pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  pdl[0].val.programmaticStreamSerializationAllowed = 1;
+  for (int i0 = 0; i0 == 0 || i0 < p->num_caches; i0 += kMaxCaches) {
+    Caches c = {};
+    for (int i = i0; i < p->num_caches && c.count < kMaxCaches; ++i) {
+      c.c[c.count] = p->caches[i];
+      c.slices[c.count] = (int)((p->caches[i].row_bytes * p->page_size + kSliceBytes - 1) / kSliceBytes);
+      c.total += c.slices[c.count++];
+    }
+    int64_t blocks = (int64_t)sms * 8;
+    if (c.count == 0) {
+      const int64_t need = (p->slots * p->max_blocks + kApplyThreads - 1) / kApplyThreads;
+      if (need < blocks) blocks = need;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3(kApplyThreads);
+    cfg.stream = stream;
+    cfg.attrs = pdl;
+    cfg.numAttrs = copy || i0 > 0 ? 0 : 1;
+    if (cudaLaunchKernelEx(&cfg, page_apply_kernel, a, c, i0 == 0 ? 1 : 0) != cudaSuccess) return DSA_ERR_CUDA;
+  }
+  return DSA_OK;
+}

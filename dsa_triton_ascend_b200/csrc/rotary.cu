@@ -1,0 +1,245 @@
+// Rotary positions of queries and keys, their gradient, and the table of cosines and sines.
+//
+// rotary_kernel is bound by memory: it reads and writes each value once.  A thread takes one
+// 16-byte piece (in the half layout the two pieces that turn together) of up to kHeads heads
+// of one token, so that the cosines and sines are fetched once for those heads and several
+// loads are in flight.  Neighbouring lanes take neighbouring pieces.
+#include <cuda_runtime.h>
+
+#include "dsa_b200.h"
+#include "rotary.cuh"
+
+namespace dsa {
+namespace rotary {
+
+constexpr int kThreads = 256;
+constexpr int kHeads = 4;
+constexpr int kMaxPairs = 128;
+
+struct Args {
+  const void* x;
+  void* out;
+  const int32_t* positions;
+  const float* table;
+  int* error_flag;
+  int64_t token0;                       // first token of this launch
+  int64_t x_batch, x_token, x_head;     // strides in elements
+  int64_t o_batch, o_token, o_head;
+  uint32_t items;                       // threads with work
+  uint32_t units, head_steps;           // pieces of a head; heads / kHeads, rounded up
+  int32_t s, heads, head_dim, offset, dim, half_layout, max_positions;
+  float sign;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) rotary_kernel(const Args a) {
+  using V = Vec<T>;
+  constexpr int kN = V::kN;
+  const uint32_t item = blockIdx.x * kThreads + threadIdx.x;
+  if (item >= a.items) return;
+  const uint32_t rest = item / a.units, u = item - rest * a.units;
+  const uint32_t tok = rest / a.head_steps, h0 = rest - tok * a.head_steps;
+  const int64_t token = a.token0 + tok, b = token / a.s, s = token - b * a.s;
+  const T* x = static_cast<const T*>(a.x) + b * a.x_batch + s * a.x_token;
+  T* out = static_cast<T*>(a.out) + b * a.o_batch + s * a.o_token;
+  const int32_t pos = a.positions[token];
+  const bool known = pos >= 0 && pos < a.max_positions;
+  if (!known && u == 0 && h0 == 0) report_error(a.error_flag, kErrBadIndex);
+  const int half = a.dim / 2;
+  const float* row = a.table + (int64_t)(known ? pos : 0) * a.dim;
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+
+  if (!a.half_layout) {
+    const int at = (int)u * kN, in = at - a.offset;
+    const bool turned = in >= 0 && in < a.dim;
+    uint4 v[kHeads];
+#pragma unroll
+    for (int j = 0; j < kHeads; ++j) {
+      const int h = h0 + j * a.head_steps;
+      if (h < a.heads) v[j] = *reinterpret_cast<const uint4*>(x + h * a.x_head + at);
+    }
+    float cs[kN / 2], sn[kN / 2];
+    if (turned) load_angles<kN / 2>(row, half, in / 2, a.sign, cs, sn);
+#pragma unroll
+    for (int j = 0; j < kHeads; ++j) {
+      const int h = h0 + j * a.head_steps;
+      if (h >= a.heads) continue;
+      if (turned) v[j] = turn_interleaved<T>(v[j], cs, sn);
+      *reinterpret_cast<uint4*>(out + h * a.o_head + at) = known ? v[j] : zero;
+    }
+    return;
+  }
+  // half layout: the first dim / (2 kN) pieces are pairs, the others are copied
+  const int pairs = half / kN;
+  if ((int)u < pairs) {
+    const int in = (int)u * kN, at = a.offset + in;
+    uint4 lo[kHeads], hi[kHeads];
+#pragma unroll
+    for (int j = 0; j < kHeads; ++j) {
+      const int h = h0 + j * a.head_steps;
+      if (h >= a.heads) continue;
+      lo[j] = *reinterpret_cast<const uint4*>(x + h * a.x_head + at);
+      hi[j] = *reinterpret_cast<const uint4*>(x + h * a.x_head + at + half);
+    }
+    float cs[kN], sn[kN];
+    load_angles<kN>(row, half, in, a.sign, cs, sn);
+#pragma unroll
+    for (int j = 0; j < kHeads; ++j) {
+      const int h = h0 + j * a.head_steps;
+      if (h >= a.heads) continue;
+      turn_half<T>(lo[j], hi[j], cs, sn);
+      *reinterpret_cast<uint4*>(out + h * a.o_head + at) = known ? lo[j] : zero;
+      *reinterpret_cast<uint4*>(out + h * a.o_head + at + half) = known ? hi[j] : zero;
+    }
+    return;
+  }
+  int at = ((int)u - pairs) * kN;
+  if (at >= a.offset) at += a.dim;
+#pragma unroll
+  for (int j = 0; j < kHeads; ++j) {
+    const int h = h0 + j * a.head_steps;
+    if (h >= a.heads) continue;
+    const uint4 v = *reinterpret_cast<const uint4*>(x + h * a.x_head + at);
+    *reinterpret_cast<uint4*>(out + h * a.o_head + at) = known ? v : zero;
+  }
+}
+
+// Any strides, offsets and even widths: one pair or one copied value per thread.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) rotary_any_kernel(const Args a) {
+  const uint32_t item = blockIdx.x * kThreads + threadIdx.x;
+  if (item >= a.items) return;
+  const uint32_t rest = item / a.units, u = item - rest * a.units;
+  const uint32_t tok = rest / a.heads, h = rest - tok * a.heads;
+  const int64_t token = a.token0 + tok, b = token / a.s, s = token - b * a.s;
+  const T* x = static_cast<const T*>(a.x) + b * a.x_batch + s * a.x_token + h * a.x_head;
+  T* out = static_cast<T*>(a.out) + b * a.o_batch + s * a.o_token + h * a.o_head;
+  const int32_t pos = a.positions[token];
+  const bool known = pos >= 0 && pos < a.max_positions;
+  if (!known && u == 0 && h == 0) report_error(a.error_flag, kErrBadIndex);
+  const int half = a.dim / 2;
+  auto get = [](const T& v) {
+    if constexpr (sizeof(T) == 4) return v;
+    else return ElemTraits<T>::to_f(v);
+  };
+  auto put = [](float v) {
+    if constexpr (sizeof(T) == 4) return v;
+    else return ElemTraits<T>::from_f(v);
+  };
+  if ((int)u < half) {
+    const float* row = a.table + (int64_t)(known ? pos : 0) * a.dim;
+    const int ia = a.offset + (a.half_layout ? (int)u : 2 * (int)u);
+    const int ib = ia + (a.half_layout ? half : 1);
+    float va = get(x[ia]), vb = get(x[ib]);
+    turn(va, vb, row[u], a.sign * row[half + u]);
+    out[ia] = put(known ? va : 0.0f);
+    out[ib] = put(known ? vb : 0.0f);
+  } else {
+    int at = (int)u - half;
+    if (at >= a.offset) at += a.dim;
+    out[at] = known ? x[at] : put(0.0f);
+  }
+}
+
+struct Frequencies {
+  double f[kMaxPairs];
+};
+
+// table[p][i] = amplitude cos(p f[i]), table[p][half + i] = amplitude sin(p f[i]): the angle in
+// 64 bits, since p f in 32 would be off by 2^-24 p radians (0.008 at p = 131072).
+__global__ void __launch_bounds__(kThreads) rotary_table_kernel(const __grid_constant__ Frequencies fr,
+                                                                float* table, int64_t n, int half,
+                                                                double amplitude) {
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n;
+       i += (int64_t)gridDim.x * kThreads) {
+    const int64_t p = i / half;
+    const int j = (int)(i - p * half);
+    double s, c;
+    sincos((double)p * fr.f[j], &s, &c);
+    table[p * 2 * half + j] = (float)(amplitude * c);
+    table[p * 2 * half + half + j] = (float)(amplitude * s);
+  }
+}
+
+template <typename T>
+int launch(const DsaRotaryParams* p, cudaStream_t stream) {
+  constexpr int kN = Vec<T>::kN;
+  Args a;
+  a.x = p->x;
+  a.out = p->out;
+  a.positions = p->positions;
+  a.table = p->table;
+  a.error_flag = p->error_flag;
+  a.x_batch = p->x_batch_stride, a.x_token = p->x_token_stride, a.x_head = p->x_head_stride;
+  a.o_batch = p->out_batch_stride, a.o_token = p->out_token_stride, a.o_head = p->out_head_stride;
+  a.s = (int)p->s;
+  a.heads = (int)p->heads;
+  a.head_dim = (int)p->head_dim;
+  a.offset = (int)p->offset;
+  a.dim = (int)p->dim;
+  a.half_layout = p->half_layout;
+  a.max_positions = (int)p->max_positions;
+  a.sign = p->inverse ? -1.0f : 1.0f;
+  bool vec = p->head_dim % kN == 0 && p->offset % kN == 0 &&
+             p->dim % (p->half_layout ? 2 * kN : kN) == 0 &&
+             reinterpret_cast<uintptr_t>(p->x) % 16 == 0 &&
+             reinterpret_cast<uintptr_t>(p->out) % 16 == 0 &&
+             reinterpret_cast<uintptr_t>(p->table) % 16 == 0 && p->dim % 8 == 0;
+  for (int64_t st : {a.x_batch, a.x_token, a.x_head, a.o_batch, a.o_token, a.o_head})
+    vec = vec && st % kN == 0;
+  if (vec) {
+    a.units = (uint32_t)((p->head_dim - (p->half_layout ? p->dim / 2 : 0)) / kN);
+    a.head_steps = (uint32_t)((p->heads + kHeads - 1) / kHeads);
+  } else {
+    a.units = (uint32_t)(p->head_dim - p->dim / 2);
+    a.head_steps = (uint32_t)p->heads;
+  }
+  const int64_t per_token = (int64_t)a.units * a.head_steps, tokens = p->batch * p->s;
+  const int64_t chunk = (1LL << 30) / per_token > 0 ? (1LL << 30) / per_token : 1;
+  if (per_token > (1LL << 30)) return DSA_ERR_INVALID_ARG;
+  for (int64_t t0 = 0; t0 < tokens; t0 += chunk) {
+    const int64_t n = tokens - t0 < chunk ? tokens - t0 : chunk;
+    a.token0 = t0;
+    a.items = (uint32_t)(n * per_token);
+    const unsigned grid = (unsigned)((a.items + kThreads - 1) / kThreads);
+    if (vec) rotary_kernel<T><<<grid, kThreads, 0, stream>>>(a);
+    else rotary_any_kernel<T><<<grid, kThreads, 0, stream>>>(a);
+    if (cudaGetLastError() != cudaSuccess) return DSA_ERR_CUDA;
+  }
+  return DSA_OK;
+}
+
+}  // namespace rotary
+}  // namespace dsa
+
+extern "C" int dsa_rotary(const DsaRotaryParams* p, void* stream_) {
+  using namespace dsa::rotary;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  if (!p || p->batch < 0 || p->s < 0 || p->heads < 0) return DSA_ERR_INVALID_ARG;
+  if (p->batch == 0 || p->s == 0 || p->heads == 0) return DSA_OK;
+  constexpr int64_t kMax = 0x7fffffff;
+  if (!p->x || !p->out || !p->positions || !p->table || p->dim < 2 || p->dim % 2 ||
+      p->dim > 2 * kMaxPairs || p->offset < 0 || p->head_dim > (1 << 20) ||
+      p->offset + p->dim > p->head_dim || p->max_positions < 1 || p->max_positions > kMax ||
+      p->heads > (1 << 20) || p->s > kMax || p->batch > kMax)
+    return DSA_ERR_INVALID_ARG;
+  if (p->dtype == DSA_DTYPE_BF16) return launch<__nv_bfloat16>(p, stream);
+  if (p->dtype == DSA_DTYPE_FP16) return launch<__half>(p, stream);
+  if (p->dtype == DSA_DTYPE_FP32) return launch<float>(p, stream);
+  return DSA_ERR_INVALID_ARG;
+}
+
+extern "C" int dsa_rotary_table(float* table, int64_t max_positions, int64_t dim,
+                                const double* frequencies, double amplitude, void* stream_) {
+  using namespace dsa::rotary;
+  if (!table || !frequencies || max_positions < 1 || max_positions > 0x7fffffff || dim < 2 ||
+      dim % 2 || dim > 2 * kMaxPairs)
+    return DSA_ERR_INVALID_ARG;
+  Frequencies fr = {};
+  const int half = (int)dim / 2;
+  for (int i = 0; i < half; ++i) fr.f[i] = frequencies[i];
+  const int64_t n = max_positions * half, blocks = (n + kThreads - 1) / kThreads;
+  rotary_table_kernel<<<(unsigned)(blocks < 65536 ? blocks : 65536), kThreads, 0,
+                        static_cast<cudaStream_t>(stream_)>>>(fr, table, n, half, amplitude);
+  return cudaGetLastError() == cudaSuccess ? DSA_OK : DSA_ERR_CUDA;
+}

@@ -19,6 +19,7 @@ enum : int {
   kErrTimeout = 1,      // a bounded wait gave up
   kErrBadIndex = 2,     // device-side index validation failed
   kErrMisaligned = 3,   // shared-memory window not 1 KiB aligned
+  kErrNoPages = 4,      // a page pool had no free page left
 };
 
 // Wall-clock budget for one wait (nanoseconds).  Kernels here finish in

@@ -448,6 +448,139 @@ typedef struct DsaAttnPagedParams {
 int dsa_attn_paged(const DsaAttnPagedParams* params, void* stream);
 int64_t dsa_attn_paged_workspace_size(int64_t batch, int64_t s1, int64_t n1, int64_t d);
 
+/*
+ * Rotary positions.  No counterpart in the reference, which takes rotated tensors.
+ *   x, out [batch][s][heads][head_dim] (bf16 / fp16 / fp32, last dim contiguous, strides in
+ *   elements; out may be x), positions [batch][s] int32, table [max_positions][dim] fp32
+ *   (dim / 2 cosines, then dim / 2 sines).  Values offset .. offset + dim of each head turn,
+ *   the others are copied; pairs are (2 i, 2 i + 1), or (i, i + dim / 2) with half_layout.
+ *   inverse turns by the negative angle (the gradient).  dim is even and at most 256.  A
+ *   position outside the table gives a zero row and a bit in error_flag.
+ */
+typedef struct DsaRotaryParams {
+  const void* x;
+  void* out;
+  const int32_t* positions;
+  const float* table;
+  int* error_flag;
+  int64_t batch;
+  int64_t s;
+  int64_t heads;
+  int64_t head_dim;
+  int64_t offset;
+  int64_t dim;
+  int64_t max_positions;
+  int64_t x_batch_stride, x_token_stride, x_head_stride;
+  int64_t out_batch_stride, out_token_stride, out_head_stride;
+  int32_t half_layout;
+  int32_t inverse;
+  int32_t dtype;
+} DsaRotaryParams;
+
+int dsa_rotary(const DsaRotaryParams* params, void* stream);
+
+/* table[p][i] = amplitude * cos(p * frequencies[i]), table[p][dim / 2 + i] = amplitude * sin(...)
+ * for p < max_positions, i < dim / 2; `frequencies` is a host array, read before the return. */
+int dsa_rotary_table(float* table, int64_t max_positions, int64_t dim, const double* frequencies,
+                     double amplitude, void* stream);
+
+/*
+ * Append new tokens to a paged cache: token s < counts[b] (counts NULL: every token) of batch b
+ * goes to position starts[b] + s, i.e. row pos % page_size of page block_table[b][pos /
+ * page_size], in up to four caches at once; rows with a rotary layout are rotated by their
+ * position on the way.  No counterpart in the reference.  All strides are in bytes and
+ * multiples of 16, as are bases and widths.  A token whose position is past the table or the
+ * block table, or whose page is not in the pool, is left out and reported in error_flag.
+ */
+#define DSA_ROTARY_NONE 0
+#define DSA_ROTARY_INTERLEAVED 1
+#define DSA_ROTARY_HALF 2
+#define DSA_APPEND_MAX_ENTRIES 4
+
+typedef struct DsaCacheRows {
+  const void* src;               /* [batch][s][width] */
+  void* cache;                   /* [num_pages][page_size][width] */
+  int64_t src_batch_stride, src_token_stride;
+  int64_t page_stride, row_stride;
+  int64_t width_bytes;
+  int64_t offset;                /* first rotated value */
+  int32_t rotary;                /* DSA_ROTARY_* */
+  int32_t dtype;                 /* read for rotated rows only */
+} DsaCacheRows;
+
+typedef struct DsaCacheAppendParams {
+  DsaCacheRows rows[DSA_APPEND_MAX_ENTRIES];
+  const int32_t* block_table;    /* [batch][max_blocks] */
+  const int32_t* starts;         /* [batch] */
+  const int32_t* counts;         /* [batch] or NULL */
+  const float* table;            /* [max_positions][dim], NULL when nothing is rotated */
+  int* error_flag;
+  int64_t batch;
+  int64_t s;
+  int64_t num_pages;
+  int64_t page_size;
+  int64_t max_blocks;
+  int64_t max_positions;
+  int64_t dim;
+  int32_t entries;
+} DsaCacheAppendParams;
+
+int dsa_cache_append(const DsaCacheAppendParams* params, void* stream);
+
+/*
+ * Upkeep of a page pool.  No counterpart in the reference.  State: block_table
+ * [slots][max_blocks] (-1: none), seq_lengths [slots], ref_counts [num_pages] (0: free).  The
+ * state is read and a new one written to the *_out arrays (which must not overlap the inputs);
+ * the data of `caches` (a host array) is moved in place.  Free pages are taken lowest id first.
+ *   COPY     n pairs first[i] -> second[i] of pages; a negative id skips the pair.  No page is
+ *            both written and read.  Only num_pages, page_size, caches and the pairs are read.
+ *   FORK     n pairs parent row first[i] -> empty row second[i]: the child shares the parent's
+ *            full pages and gets a page of its own with the rows of the partly filled one.
+ *   EXTEND   row r grows by first[r] tokens (n == slots), with the pages that takes.
+ *   FREE     n rows first[i] give their pages back and become empty.
+ *   COMPACT  live pages move to the lowest ids, n_live of them, in order; seq_lengths unused.
+ * A fork or row that asks for what cannot be (an id out of range, a child in use, a length past
+ * the block table) or for which no page is left stays as it was; error_flag tells.
+ * Workspace: dsa_pages_workspace_size() bytes (n as in the call).
+ */
+#define DSA_PAGES_COPY 0
+#define DSA_PAGES_FORK 1
+#define DSA_PAGES_EXTEND 2
+#define DSA_PAGES_FREE 3
+#define DSA_PAGES_COMPACT 4
+
+typedef struct DsaPageCache {
+  void* data;
+  int64_t page_stride;           /* bytes */
+  int64_t row_stride;
+  int64_t row_bytes;
+} DsaPageCache;
+
+typedef struct DsaPagesParams {
+  const int32_t* block_table;
+  const int32_t* seq_lengths;
+  const int32_t* ref_counts;
+  int32_t* block_table_out;
+  int32_t* seq_lengths_out;
+  int32_t* ref_counts_out;
+  const int32_t* first;
+  const int32_t* second;
+  const DsaPageCache* caches;
+  int* error_flag;
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t n;
+  int64_t slots;
+  int64_t max_blocks;
+  int64_t num_pages;
+  int64_t page_size;
+  int32_t num_caches;
+  int32_t op;
+} DsaPagesParams;
+
+int dsa_pages(const DsaPagesParams* params, void* stream);
+int64_t dsa_pages_workspace_size(int32_t op, int64_t n, int64_t slots, int64_t num_pages);
+
 #ifdef __cplusplus
 }
 #endif
