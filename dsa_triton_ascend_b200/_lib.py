@@ -239,22 +239,37 @@ def check(rc: int, what: str) -> None:
         raise RuntimeError(f"{what}: {_ERR_TEXT.get(rc, 'error')} (code {rc})")
 
 
-def error_flag(device: torch.device) -> torch.Tensor:
-    """Per-device int32 the kernels OR their error bits into."""
+def _flags(device) -> torch.Tensor:
+    """Per-device pair of int32: error_flag and report_flag."""
     key = torch.device(device).index
+    if key is None:   # "cuda" is the current device: one pair, whichever way it is named
+        key = torch.cuda.current_device()
     buf = _err_bufs.get(key)
     if buf is None:
-        buf = torch.zeros(1, dtype=torch.int32, device=device)
+        buf = torch.zeros(2, dtype=torch.int32, device=torch.device("cuda", key))
         _err_bufs[key] = buf
     return buf
+
+
+def error_flag(device: torch.device) -> torch.Tensor:
+    """Per-device int32 the kernels OR their error bits into.  Kernels of the sparse path give
+    up their work while a bit is set."""
+    return _flags(device)[:1]
+
+
+def report_flag(device: torch.device) -> torch.Tensor:
+    """Per-device int32 for operators that report a request they cannot meet (a page that is
+    not in the pool, no page left) and go on: such a bit stops no other kernel."""
+    return _flags(device)[1:]
 
 
 def check_device_errors(device=None) -> None:
     """Synchronise and raise if any kernel reported a device-side error."""
     dev = torch.device("cuda" if device is None else device)
-    buf = error_flag(dev)
+    buf = _flags(dev)
     torch.cuda.synchronize(dev)
-    v = int(buf.item())
+    error, report = buf.tolist()
+    v = error | report
     if v:
         buf.zero_()
         raise RuntimeError(f"dsa kernel reported device error bits 0x{v:x} "
