@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import _host as H
-from ._lib import AttnPagedParams, check, error_flag, lib, ptr, stream_ptr
+from ._lib import AttnPagedParams, check, lib, ptr, report_flag, stream_ptr
 
 _VALID_D = (128, 256, 512)
 _D_ROPE = 64
@@ -122,7 +122,7 @@ def flash_attention_paged(
         p.block_table, p.act_q, p.act_k, p.out = ptr(bt), ptr(act_q), ptr(act_k), ptr(out)
         if return_softmax_lse:
             p.softmax_max, p.softmax_sum = ptr(smax), ptr(ssum)
-        p.error_flag = ptr(error_flag(dev))
+        p.error_flag = ptr(report_flag(dev))
         p.workspace, p.workspace_bytes = ptr(ws), ws_bytes
         p.batch, p.s1, p.n1, p.d = B, S1, N1, D
         p.num_pages, p.page_size, p.max_blocks = num_pages, page, max_blocks

@@ -22,7 +22,7 @@ import torch
 from . import _host as H
 from ._lib import (APPEND_MAX_ENTRIES, DSA_DTYPE_BF16, DSA_DTYPE_FP16, DSA_DTYPE_FP32, PAGES_COMPACT, PAGES_COPY,
                    PAGES_EXTEND, PAGES_FORK, PAGES_FREE, ROTARY_CODES, CacheAppendParams, PageCache,
-                   PagesParams, check, error_flag, lib, ptr, stream_ptr)
+                   PagesParams, check, lib, ptr, report_flag, stream_ptr)
 
 _ROTATED = {torch.bfloat16: DSA_DTYPE_BF16, torch.float16: DSA_DTYPE_FP16, torch.float32: DSA_DTYPE_FP32}
 
@@ -156,7 +156,7 @@ def paged_cache_append(tokens, caches, block_table, starts, counts=None, table=N
                 table = table.clone()
             p.table, p.max_positions, p.dim = ptr(table), table.shape[0], dim
         p.block_table, p.starts, p.counts = ptr(bt), ptr(st), ptr(ct)
-        p.error_flag = ptr(error_flag(dev))
+        p.error_flag = ptr(report_flag(dev))
         p.batch, p.s, p.num_pages, p.page_size = B, S, num_pages, page_size
         p.max_blocks, p.entries = bt.shape[1], len(tokens)
         check(lib().dsa_cache_append(p, stream_ptr(dev)), "dsa_cache_append")
@@ -168,7 +168,7 @@ def _run(op, dev, caches, page_size, num_pages, table=None, lens=None, refs=None
     with torch.cuda.device(dev):
         p = PagesParams()
         p.op, p.n, p.num_pages, p.page_size = op, n, num_pages, page_size
-        p.error_flag = ptr(error_flag(dev))
+        p.error_flag = ptr(report_flag(dev))
         p.first, p.second = ptr(first), ptr(second)
         out = [None, None, None]
         if table is not None:

@@ -12,7 +12,7 @@ import math
 import torch
 
 from . import _host as H
-from ._lib import DSA_DTYPE_FP32, RotaryParams, check, error_flag, lib, ptr, stream_ptr
+from ._lib import DSA_DTYPE_FP32, RotaryParams, check, lib, ptr, report_flag, stream_ptr
 
 _MAX_DIM = 256
 LAYOUTS = ("interleaved", "half")
@@ -130,7 +130,7 @@ def rotary_embedding(x, table, positions, layout="interleaved", offset=0, invers
         table = table.contiguous()
         p = RotaryParams()
         p.x, p.out, p.positions, p.table = ptr(x), ptr(out), ptr(positions), ptr(table)
-        p.error_flag = ptr(error_flag(dev))
+        p.error_flag = ptr(report_flag(dev))
         p.batch, p.s = (1, x.shape[0]) if x.dim() == 3 else x.shape[:2]
         p.heads, p.head_dim, p.offset, p.dim = x.shape[-2], x.shape[-1], int(offset), dim
         p.max_positions = table.shape[0]
