@@ -27,10 +27,16 @@ namespace attn_paged {
 constexpr int kTile = 64;       // keys of a step
 constexpr int kRope = 64;
 constexpr int kSmemLimit = 232448;
-constexpr int kSoftmaxThreads = 128;   // warps 0-3
-constexpr int kThreads = 192;          // warp 4: loads, warp 5: MMA
+constexpr int kSoftmaxThreads = 128;   // of a warpgroup; there are two (warps 0-3, 4-7), each with
+                                       // half of the heads
+constexpr int kLoadWarp = 8;           // warps 8-11: loads (one warp issues a box in 160 cycles,
+                                       // so 16 boxes a tile from one warp took 2,600 of them)
+constexpr int kMmaWarp = 12;
+constexpr int kQueryWarp = 13;
+constexpr int kThreads = 448;
 constexpr int kMaxStages = 8;
 constexpr int kMinTiles = 2;    // tiles a CTA takes at least: fewer cost more in joining than they save
+constexpr int kAhead = 3;       // tiles that are brought into L2 before their load
 constexpr float kRescale = 8.0f;       // log2 units the running max may pass the reference
 
 template <int D, int NH>
@@ -42,12 +48,16 @@ struct Cfg {
   static constexpr int kRopeBytes = 64 * 128;
   static constexpr int kStageBytes = kKeyBytes + kRopeBytes;
   static constexpr int kQBytes = NH * (D + kRope) * 2;
+  static constexpr int kHeads = NH / 2;   // of a softmax warpgroup
   static constexpr int kPBytes = kTile * NH * 2;
   // row maxima of two tiles per warp, factors, barriers and the rest
   static constexpr int kSmallBytes = 2 * 4 * NH * 4 + NH * 4 + 512;
   static constexpr int kRoom = (kSmemLimit - kQBytes - kPBytes - kSmallBytes) / kStageBytes;
   static constexpr int kStages = kRoom < kMaxStages ? kRoom : kMaxStages;
-  static constexpr int kSmem = kStages * kStageBytes + kQBytes + kPBytes + kSmallBytes;
+  // the next segment's queries are loaded while this one's are in use, where they fit
+  static constexpr int kQBufs =
+      kStages * kStageBytes + 2 * kQBytes + kPBytes + kSmallBytes <= kSmemLimit ? 2 : 1;
+  static constexpr int kSmem = kStages * kStageBytes + kQBufs * kQBytes + kPBytes + kSmallBytes;
   static constexpr uint32_t kCols = (2 + kBlocks) * NH;
   static constexpr uint32_t kTmem = kCols <= 32 ? 32 : kCols <= 64 ? 64 : kCols <= 128 ? 128
                                     : kCols <= 256 ? 256 : 512;
@@ -68,7 +78,8 @@ struct Args {
   int* error_flag;
   int32_t* ws_prefix;   // [rows + 1] first tile of each row
   float* ws_o;          // [2 * CTAs][NH][D]
-  float4* ws_s;         // [2 * CTAs][NH]: reference, running max, sum
+  float4* ws_s;         // [2 * CTAs][NH]: reference and running maximum (log2 units), sum,
+                        // raw running maximum
   int32_t rows, s1, n1, groups;
   int32_t page_size, max_blocks, num_pages, mode;
   float scale;
@@ -167,12 +178,16 @@ __device__ __forceinline__ uint64_t p_desc(uint32_t saddr) {
 // every 8 columns the pair 2 (l % 4).  r[4 i + {0, 1}] is the first row, {2, 3} the second.
 template <int N>
 __device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, uint32_t (&r)[N / 2]) {
-  if constexpr (N == 16)
+  if constexpr (N == 8)
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x1.b32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(taddr));
+  else if constexpr (N == 16)
     asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
                    "=r"(r[6]), "=r"(r[7])
                  : "r"(taddr));
-  else if constexpr (N == 32)
+  else
     asm volatile(
         "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,"
         "%15}, [%16];"
@@ -180,20 +195,32 @@ __device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, uint32_t (&r)[N / 2
           "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
           "=r"(r[14]), "=r"(r[15])
         : "r"(taddr));
-  else
-    asm volatile(
-        "tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,"
-        "%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-          "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
-          "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
-          "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr));
 }
 
-__device__ __forceinline__ void softmax_bar() {
-  asm volatile("bar.sync 1, %0;" ::"n"(kSoftmaxThreads) : "memory");
+// 2^x, 2^-126 and below flushed to 0
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// The four warps of softmax warpgroup `wg` meet.
+__device__ __forceinline__ void softmax_bar(int wg) {
+  asm volatile("bar.sync %0, %1;" ::"r"(1 + wg), "n"(kSoftmaxThreads) : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld16(taddr, r); }
+__device__ __forceinline__ void tmem_st_cols(uint32_t taddr, const uint32_t (&r)[16]) { tmem_st16(taddr, r); }
+__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+                 "=r"(r[7])
+               : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st_cols(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr),
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 
 template <int D, int NH, typename T>
@@ -208,13 +235,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base = smem_u32(smem);
   const uint32_t s_q = base + C::kStages * C::kStageBytes;
-  const uint32_t s_p = s_q + C::kQBytes;
-  uint8_t* small = smem + C::kStages * C::kStageBytes + C::kQBytes + C::kPBytes;
+  const uint32_t s_p = s_q + C::kQBufs * C::kQBytes;
+  uint8_t* small = smem + C::kStages * C::kStageBytes + C::kQBufs * C::kQBytes + C::kPBytes;
   float* wmax = reinterpret_cast<float*>(small);          // [2][4][NH]
   float* factor = wmax + 2 * 4 * NH;                      // [NH]
   uint64_t* bars = reinterpret_cast<uint64_t*>(factor + NH);
-  int32_t* tmask = reinterpret_cast<int32_t*>(bars + 32);  // [kMaxStages]
-  int32_t* tmp = tmask + kMaxStages;                       // [16]
+  int32_t* tmask = reinterpret_cast<int32_t*>(bars + 32);  // [kMaxStages][4]
+  int32_t* tmp = tmask + 4 * kMaxStages;                   // [16]
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(tmp + 16);
   int32_t* start = reinterpret_cast<int32_t*>(tmem_ptr + 1);   // [3]
 
@@ -222,9 +249,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto full = [&](int s) { return b0 + 8u * s; };
   auto empty = [&](int s) { return b0 + 8u * (kMaxStages + s); };
   auto s_full = [&](int s) { return b0 + 8u * (2 * kMaxStages + s); };
-  auto s_empty = [&](int s) { return b0 + 8u * (2 * kMaxStages + 2 + s); };
-  const uint32_t p_full = b0 + 8u * (2 * kMaxStages + 4), p_empty = b0 + 8u * (2 * kMaxStages + 5);
-  const uint32_t q_full = b0 + 8u * (2 * kMaxStages + 6), q_empty = b0 + 8u * (2 * kMaxStages + 7);
+  const uint32_t p_full = b0 + 8u * (2 * kMaxStages + 2), p_empty = b0 + 8u * (2 * kMaxStages + 3);
+  auto q_full = [&](int s) { return b0 + 8u * (2 * kMaxStages + 4 + s); };
+  auto q_empty = [&](int s) { return b0 + 8u * (2 * kMaxStages + 6 + s); };
   const uint32_t o_empty = b0 + 8u * (2 * kMaxStages + 8);
   const uint32_t drained = b0 + 8u * (2 * kMaxStages + 9);
 
@@ -235,30 +262,30 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(full(s), 1);
+      mbar_init(full(s), 4);
       mbar_init(empty(s), 1);
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(s_full(s), 1);
-      mbar_init(s_empty(s), 4);
+      mbar_init(q_full(s), 1);
+      mbar_init(q_empty(s), 1);
     }
-    mbar_init(p_full, 4);
+    mbar_init(p_full, 8);
     mbar_init(p_empty, 1);
-    mbar_init(q_full, 1);
-    mbar_init(q_empty, 1);
-    mbar_init(o_empty, 4);
+    mbar_init(o_empty, 8);
     mbar_init(drained, 1);
     fence_mbarrier_init();
   }
-  if (warp == 5) tmem_alloc<1>(smem_u32(tmem_ptr), C::kTmem);
+  if (warp == kMmaWarp) tmem_alloc<1>(smem_u32(tmem_ptr), C::kTmem);
 
   // ---- this CTA's share of the tiles ----
   int64_t total = 0;
+  int mine = 0, before = 0;   // the tiles of the thread's last row and of the rows before it
   for (int r0 = 0; r0 < a.rows; r0 += kThreads) {
     const int r = r0 + threadIdx.x;
     int sum;
-    const int v = r < a.rows ? row_tiles(a, r) : 0;
-    const int before = block_scan(v, tmp, &sum);
+    mine = r < a.rows ? row_tiles(a, r) : 0;
+    before = block_scan(mine, tmp, &sum);
     if (blockIdx.x == 0 && r < a.rows) a.ws_prefix[r] = (int)total + before;
     total += sum;
   }
@@ -271,19 +298,20 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (blockIdx.x < ctas) {
     from = tiles * blockIdx.x / ctas;
     work.left = (int)(tiles * (blockIdx.x + 1) / ctas - from);
-  }
-  {
     int64_t seen = 0;
     for (int r0 = 0; r0 < a.rows; r0 += kThreads) {
       const int r = r0 + threadIdx.x;
-      int sum;
-      const int v = r < a.rows ? row_tiles(a, r) : 0;
-      const int64_t first = (seen + block_scan(v, tmp, &sum)) * a.groups;
-      if (v > 0 && first <= from && from < first + (int64_t)v * a.groups) {
+      int sum = (int)total;
+      if (a.rows > kThreads) {
+        mine = r < a.rows ? row_tiles(a, r) : 0;
+        before = block_scan(mine, tmp, &sum);
+      }
+      const int64_t first = (seen + before) * a.groups;
+      if (mine > 0 && first <= from && from < first + (int64_t)mine * a.groups) {
         const int in = (int)(from - first);
         start[0] = r;
-        start[1] = in / v;
-        start[2] = in - (in / v) * v;
+        start[1] = in / mine;
+        start[2] = in - (in / mine) * mine;
       }
       seen += sum;
       if (seen * a.groups > from) break;   // the same for every thread
@@ -301,77 +329,100 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   bool failed = false;
 
-  if (warp == 4) {
+  if (warp >= kLoadWarp && warp < kMmaWarp) {
     // -------------------------------------------------------------------- loads
-    if (lane == 0) {
-      tma_prefetch_desc(&maps.q);
-      tma_prefetch_desc(&maps.qr);
-      tma_prefetch_desc(&maps.k);
-      tma_prefetch_desc(&maps.kr);
-    }
+    const int w = warp - kLoadWarp;
+    // this warp loads groups 2 w and 2 w + 1 (of 8 keys) of every tile: lanes 0 and 1 their
+    // latent rows, lanes 2 and 3 the rotary ones; lanes 4 .. 7 bring the same of the tile kAhead
+    // further on into L2
+    const int grp = 2 * w + (lane & 1), ahead = lane < 4 ? 0 : kAhead;
+    const bool is_rope = lane & 2;
     Segment sg;
-    int g = 0, nseg = 0;
+    int g = 0;
     while (!failed && next_segment(a, work, sg)) {
-      const int b = sg.row / a.s1, s = sg.row - b * a.s1;
+      const int b = sg.row / a.s1;
       const int32_t* table = a.block_table + (int64_t)b * a.max_blocks;
-      // lane l < 8 takes keys 8 l .. 8 l + 7 of a tile; -1: no such page
-      auto page_of = [&](int tile) {
-        const int pos = tile * kTile + lane * 8;
-        if (lane >= 8 || pos >= sg.keys) return -1;
+      auto page_of = [&](int tile) {   // -1: no such page
+        const int pos = (tile + ahead) * kTile + grp * 8;
+        if (lane >= 8 || pos >= sg.keys || tile + ahead >= sg.first + sg.count) return -1;
         const int id = table[pos / a.page_size];
-        if (id >= a.num_pages) report_error(a.error_flag, kErrBadIndex);
+        if (id >= a.num_pages && lane < 2) report_error(a.error_flag, kErrBadIndex);
         return id < a.num_pages ? id : -1;
       };
       int page = page_of(sg.first);
-      if (nseg > 0) mbar_wait(q_empty, (nseg - 1) & 1, a.error_flag, &failed);
-      if ((failed = __any_sync(0xffffffffu, failed))) break;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(q_full, C::kQBytes);
-        tma_load_5d(s_q, &maps.q, q_full, 0, sg.group * NH, 0, s, b);
-        tma_load_5d(s_q + NH * D * 2, &maps.qr, q_full, 0, sg.group * NH, 0, s, b);
-      }
       for (int i = 0; i < sg.count; ++i, ++g) {
         const int st = g % C::kStages, tile = sg.first + i;
         const int now = page;
         if (i + 1 < sg.count) page = page_of(tile + 1);
         if (g >= C::kStages) mbar_wait(empty(st), (g / C::kStages - 1) & 1, a.error_flag, &failed);
-        if ((failed = __any_sync(0xffffffffu, failed))) break;
-        const uint32_t mask = __ballot_sync(0xffffffffu, now >= 0);
+        failed = __any_sync(0xffffffffu, failed);
+        if (failed) break;
+        const uint32_t mask = __ballot_sync(0xffffffffu, now >= 0) & 3u;
         const uint32_t dst = base + st * C::kStageBytes;
         if (lane == 0) {
-          tmask[st] = (int)mask;
+          tmask[4 * st + w] = (int)mask;
           const uint32_t bytes = __popc(mask) * (C::kGroupBytes + 1024);
           if (bytes) mbar_arrive_expect_tx(full(st), bytes);
           else mbar_arrive(full(st));
         }
         __syncwarp();
-        if (now >= 0) {
-          const int in_page = (tile * kTile + lane * 8) % a.page_size;
-          tma_load_4d(dst + lane * C::kGroupBytes, &maps.k, full(st), 0, in_page, 0, now);
-          tma_load_4d(dst + C::kKeyBytes + lane * 1024, &maps.kr, full(st), 0, in_page, 0, now);
-        }
+        const int in_page = ((tile + ahead) * kTile + grp * 8) % a.page_size;
+        const CUtensorMap* map = is_rope ? &maps.kr : &maps.k;
+        if (now >= 0 && lane < 4)
+          tma_load_4d(dst + (is_rope ? C::kKeyBytes + grp * 1024 : grp * C::kGroupBytes), map, full(st), 0,
+                      in_page, 0, now);
+        else if (now >= 0)
+          tma_prefetch_4d(map, 0, in_page, 0, now);
       }
-      ++nseg;
     }
     if (failed) {   // the copies in flight land before the CTA ends
       bool gave_up = false;
-      if (nseg > 0) mbar_wait(q_full, (nseg - 1) & 1, a.error_flag, &gave_up);
       for (int t = max(0, g - C::kStages); t < g; ++t)
         mbar_wait(full(t % C::kStages), (t / C::kStages) & 1, a.error_flag, &gave_up);
       __syncwarp();
     }
-  } else if (warp == 5) {
+  } else if (warp == kQueryWarp) {
+    // -------------------------------------------------------------------- queries
+    Segment sg;
+    int nseg = 0;
+    while (!failed && next_segment(a, work, sg)) {
+      const int b = sg.row / a.s1, s = sg.row - b * a.s1;
+      const int buf = nseg % C::kQBufs, use = nseg / C::kQBufs;
+      if (use > 0) mbar_wait(q_empty(buf), (use - 1) & 1, a.error_flag, &failed);
+      failed = __any_sync(0xffffffffu, failed);
+      if (failed) break;
+      if (lane == 0) {
+        const uint32_t dst = s_q + buf * C::kQBytes;
+        mbar_arrive_expect_tx(q_full(buf), C::kQBytes);
+        tma_load_5d(dst, &maps.q, q_full(buf), 0, sg.group * NH, 0, s, b);
+        tma_load_5d(dst + NH * D * 2, &maps.qr, q_full(buf), 0, sg.group * NH, 0, s, b);
+      }
+      __syncwarp();
+      ++nseg;
+    }
+    if (failed) {
+      bool gave_up = false;
+      for (int t = max(0, nseg - C::kQBufs); t < nseg; ++t)
+        mbar_wait(q_full(t % C::kQBufs), (t / C::kQBufs) & 1, a.error_flag, &gave_up);
+      __syncwarp();
+    }
+  } else if (warp == kMmaWarp) {
     // -------------------------------------------------------------------- MMA
     constexpr uint32_t kIdQk = idesc_f16(64, NH, kBf16, false, false);
     constexpr uint32_t kIdPv = idesc_f16(128, NH, kBf16, true, true);
+    // A look at a barrier takes some 100 cycles beside the tensor core's operand reads, so each
+    // is looked at once.  The buffer of scores needs no barrier of its own: QK(g) overwrites
+    // those of tile g - 2, which were read before the probabilities that PV(g - 2) waited for.
     bool pv_due = false, pv_first = false;
     int pv_tile = 0, pv_seg = 0;
-    auto issue_pv = [&]() {
+    auto all = [](bool v) { return __all_sync(0xffffffffu, v) != 0; };
+    auto issue_pv = [&](bool there) {
+      if (!there) mbar_wait_spin(p_full, pv_tile & 1, a.error_flag, &failed);
       if (pv_first && pv_seg > 0)
         mbar_wait_spin(o_empty, (pv_seg - 1) & 1, a.error_flag, &failed);
-      mbar_wait_spin(p_full, pv_tile & 1, a.error_flag, &failed);
       pv_due = false;
-      if ((failed = __any_sync(0xffffffffu, failed))) return;
+      failed = !all(!failed);
+      if (failed) return;
       tc_fence_after();
       const int st = pv_tile % C::kStages;
       if (elect_one()) {
@@ -391,25 +442,31 @@ __global__ void __launch_bounds__(kThreads, 1)
     Segment sg;
     int g = 0, nseg = 0;
     while (!failed && next_segment(a, work, sg)) {
+      const int buf = nseg % C::kQBufs;
+      const uint32_t q_par = (nseg / C::kQBufs) & 1;
       for (int i = 0; i < sg.count && !failed; ++i, ++g) {
         const int st = g % C::kStages;
-        // while this tile's keys (or the segment's queries) are on their way, the product
-        // of the tile before goes first
-        if (pv_due) {
-          const bool here = (i > 0 || mbar_try_wait(q_full, nseg & 1)) &&
-                            mbar_try_wait(full(st), (g / C::kStages) & 1);
-          if (!__all_sync(0xffffffffu, here)) issue_pv();
+        if (i == 0) {
+          if (pv_due && !all(mbar_test_wait(q_full(buf), q_par))) issue_pv(false);
+          mbar_wait_spin(q_full(buf), q_par, a.error_flag, &failed);
         }
-        if (i == 0) mbar_wait_spin(q_full, nseg & 1, a.error_flag, &failed);
-        mbar_wait_spin(full(st), (g / C::kStages) & 1, a.error_flag, &failed);
-        if (g >= 2) mbar_wait_spin(s_empty(g & 1), ((g >> 1) - 1) & 1, a.error_flag, &failed);
-        if ((failed = __any_sync(0xffffffffu, failed))) break;
+        // while this tile's keys are on their way, the product of the tile before goes first if
+        // its probabilities are there
+        const uint32_t par = (g / C::kStages) & 1;
+        bool here = all(mbar_test_wait(full(st), par));
+        for (int spin = 0; !here && pv_due && spin < (1 << 20); ++spin) {
+          if (all(mbar_test_wait(p_full, pv_tile & 1))) issue_pv(true);
+          here = all(mbar_test_wait(full(st), par));
+        }
+        if (!here) mbar_wait_spin(full(st), par, a.error_flag, &failed);
+        failed = !all(!failed);
+        if (failed) break;
         tc_fence_after();
         if (elect_one()) {
           const uint64_t ka = smem_desc_sw128(base + st * C::kStageBytes, 16, C::kGroupBytes);
           const uint64_t ra =
               smem_desc_sw128(base + st * C::kStageBytes + C::kKeyBytes, 16, 1024);
-          const uint64_t qb = smem_desc_sw128(s_q, 16, 1024);
+          const uint64_t qb = smem_desc_sw128(s_q + buf * C::kQBytes, 16, 1024);
           const uint32_t d = tmem + (g & 1) * NH;
 #pragma unroll
           for (int c = 0; c < C::kChunks; ++c)
@@ -422,10 +479,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             umma_f16<1>(d, ra + ((k * 32) >> 4), qb + ((C::kChunks * NH * 128 + k * 32) >> 4),
                         kIdQk, 1);
           umma_commit(s_full(g & 1));
-          if (i == sg.count - 1) umma_commit(q_empty);
+          if (i == sg.count - 1) umma_commit(q_empty(buf));
         }
         __syncwarp();
-        if (pv_due) issue_pv();
+        if (pv_due) issue_pv(false);
         pv_due = true;
         pv_first = i == 0;
         pv_tile = g;
@@ -433,7 +490,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       ++nseg;
     }
-    if (pv_due && !failed) issue_pv();
+    if (pv_due && !failed) issue_pv(false);
     if (failed) {   // the products in flight end before the tensor memory is given back
       bool gave_up = false;
       if (elect_one()) umma_commit(drained);
@@ -441,132 +498,150 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_wait(drained, 0, a.error_flag, &gave_up);
       __syncwarp();
     }
-  } else if (warp < 4) {
+  } else if (warp < kLoadWarp) {
     // -------------------------------------------------------------------- softmax
-    constexpr int kPairs = NH / 8;   // column pairs of a thread
-    const float c2 = a.scale * 1.4426950408889634f;
-    const uint32_t lane_base = (uint32_t)warp * 32u << 16;
+    constexpr int HW = C::kHeads;    // heads of this warpgroup, from `head0` on
+    constexpr int kPairs = HW / 8;   // column pairs of a thread
+    constexpr int kCols = HW < 16 ? 8 : 16;
+    const int wg = warp >> 2, quarter = warp & 3, head0 = wg * HW;
+    // scores in log2 units are raw * c2; a negative scale turns the raw scores over
+    const bool flip = a.scale < 0.0f;
+    // (a scale of 0 leaves masked keys, whose raw score is -inf, at -inf)
+    const float c2 = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-38f);
+    const uint32_t lane_base = (uint32_t)quarter * 32u << 16;
     // a failed wait is not a way out of this loop: the four warps meet at their barrier as often
     // as there are tiles, and only the waits are passed over
-    const int key0 = warp * 16 + (lane >> 2);   // and key0 + 8
-    const int col = 2 * (lane & 3);             // heads 8 i + col, 8 i + col + 1
-    float ref[2 * kPairs], run[2 * kPairs], sum[2 * kPairs];
+    const int key0 = quarter * 16 + (lane >> 2);   // and key0 + 8
+    const int col = head0 + 2 * (lane & 3);     // heads 8 i + col, 8 i + col + 1
+    // per column: the reference of the exponents in log2 units (one for all four warps), the raw
+    // score above which it has to be raised, this thread's running maximum (raw) and sum
+    float ref[2 * kPairs], lim[2 * kPairs], run[2 * kPairs], sum[2 * kPairs];
     Segment sg;
     int g = 0, nseg = 0;
     while (next_segment(a, work, sg)) {
 #pragma unroll
       for (int j = 0; j < 2 * kPairs; ++j) {
-        ref[j] = run[j] = -INFINITY;
+        ref[j] = run[j] = lim[j] = -INFINITY;
         sum[j] = 0.0f;
       }
       for (int i = 0; i < sg.count; ++i, ++g) {
         const int st = g % C::kStages;
-        mbar_wait_spin(s_full(g & 1), (g >> 1) & 1, a.error_flag, &failed);
         mbar_wait_spin(full(st), (g / C::kStages) & 1, a.error_flag, &failed);
+        const uint32_t mask = (uint32_t)tmask[4 * st + quarter];   // of this warp's 16 keys
+        const int valid = sg.keys - (sg.first + i) * kTile;        // keys of this tile, >= 1
+        const bool whole_tile = valid >= kTile && mask == 3u;
+        mbar_wait_spin(s_full(g & 1), (g >> 1) & 1, a.error_flag, &failed);
         tc_fence_after();
-        uint32_t raw[NH / 2];
-        tmem_ld_frag<NH>(tmem + (g & 1) * NH + lane_base, raw);
+        uint32_t raw[HW / 2];
+        tmem_ld_frag<HW>(tmem + (g & 1) * NH + head0 + lane_base, raw);
         tmem_ld_wait();
         tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(s_empty(g & 1));
 
-        const uint32_t mask = (uint32_t)tmask[st];
-        const int valid = sg.keys - (sg.first + i) * kTile;   // keys of this tile, >= 1
-        const bool ok0 = (mask >> (2 * warp) & 1u) && key0 < valid;
-        const bool ok1 = (mask >> (2 * warp + 1) & 1u) && key0 + 8 < valid;
-        float z[NH / 2], top[2 * kPairs];
+        float z[HW / 2];
 #pragma unroll
-        for (int j = 0; j < kPairs; ++j)
+        for (int j = 0; j < HW / 2; ++j) z[j] = __uint_as_float(raw[j]);
+        if (flip)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            z[4 * j + e] = ok0 ? __uint_as_float(raw[4 * j + e]) * c2 : -INFINITY;
-            z[4 * j + 2 + e] = ok1 ? __uint_as_float(raw[4 * j + 2 + e]) * c2 : -INFINITY;
-            top[2 * j + e] = fmaxf(z[4 * j + e], z[4 * j + 2 + e]);
-          }
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1)
-#pragma unroll
-          for (int j = 0; j < 2 * kPairs; ++j)
-            top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], o));
-        float* wm = wmax + (g & 1) * 4 * NH;
-        if (lane < 4)
+          for (int j = 0; j < HW / 2; ++j) z[j] = -z[j];
+        if (!whole_tile) {
+          const bool ok0 = (mask & 1u) && key0 < valid, ok1 = (mask & 2u) && key0 + 8 < valid;
 #pragma unroll
           for (int j = 0; j < kPairs; ++j)
-            *reinterpret_cast<float2*>(wm + warp * NH + 8 * j + col) =
-                make_float2(top[2 * j], top[2 * j + 1]);
-        softmax_bar();
-        bool raise = false;
 #pragma unroll
-        for (int j = 0; j < kPairs; ++j) {
-          float2 m = *reinterpret_cast<float2*>(wm + 8 * j + col);
-#pragma unroll
-          for (int w = 1; w < 4; ++w) {
-            const float2 y = *reinterpret_cast<float2*>(wm + w * NH + 8 * j + col);
-            m.x = fmaxf(m.x, y.x);
-            m.y = fmaxf(m.y, y.y);
-          }
-          run[2 * j] = fmaxf(run[2 * j], m.x);
-          run[2 * j + 1] = fmaxf(run[2 * j + 1], m.y);
-          raise |= run[2 * j] > ref[2 * j] + kRescale || run[2 * j + 1] > ref[2 * j + 1] + kRescale;
+            for (int e = 0; e < 2; ++e) {
+              if (!ok0) z[4 * j + e] = -INFINITY;
+              if (!ok1) z[4 * j + 2 + e] = -INFINITY;
+            }
         }
-        if (i == 0) {
+        bool raise = i == 0;
 #pragma unroll
-          for (int j = 0; j < 2 * kPairs; ++j) ref[j] = run[j];
-        } else if (__any_sync(0xffffffffu, raise)) {
-          // every warp sees the same maxima, so all four come here together
-          if (g > 0) mbar_wait_spin(p_empty, (g - 1) & 1, a.error_flag, &failed);
-            tc_fence_after();
+        for (int j = 0; j < 2 * kPairs; ++j) {
+          const float m = fmaxf(z[4 * (j >> 1) + (j & 1)], z[4 * (j >> 1) + 2 + (j & 1)]);
+          raise |= m > lim[j];
+          run[j] = fmaxf(run[j], m);
+        }
+        // The maxima of the columns are joined over the warpgroup only where the reference has
+        // to move: at the first tile, and when a score passes it by 2^8, which keeps the
+        // probabilities within range.  Otherwise one barrier per tile tells that nobody asks.
+        if (named_bar_or(1 + wg, kSoftmaxThreads, raise)) {
+          float top[2 * kPairs];
+#pragma unroll
+          for (int j = 0; j < 2 * kPairs; ++j) top[j] = run[j];
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1)
+#pragma unroll
+            for (int j = 0; j < 2 * kPairs; ++j)
+              top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], o));
+          if (lane < 4)
+#pragma unroll
+            for (int j = 0; j < kPairs; ++j)
+              *reinterpret_cast<float2*>(wmax + quarter * NH + 8 * j + col) =
+                  make_float2(top[2 * j], top[2 * j + 1]);
+          softmax_bar(wg);
+          float f[2 * kPairs];
 #pragma unroll
           for (int j = 0; j < 2 * kPairs; ++j) {
-            const float f = ref[j] == run[j] ? 1.0f : exp2f(ref[j] - run[j]);
-            sum[j] *= f;
-            ref[j] = run[j];
-            if (warp == 0 && lane < 4) factor[8 * (j >> 1) + col + (j & 1)] = f;
+            const int h = 8 * (j >> 1) + col + (j & 1);
+            const float m = fmaxf(fmaxf(wmax[h], wmax[NH + h]), fmaxf(wmax[2 * NH + h], wmax[3 * NH + h]));
+            const float now = m == -INFINITY ? -INFINITY : m * c2;   // no key so far: stays -inf
+            f[j] = ref[j] == now ? 1.0f : exp2f(ref[j] - now);
+            sum[j] *= f[j];
+            ref[j] = now;
+            lim[j] = (now + kRescale) / c2;
           }
-          softmax_bar();
-#pragma unroll 1
-          for (int cc = 0; cc < C::kBlocks * NH; cc += 16) {
-            uint32_t o[16];
-            tmem_ld16(t_o + cc + lane_base, o);
-            tmem_ld_wait();
+          if (quarter == 0 && lane < 4)
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-              o[j] = __float_as_uint(__uint_as_float(o[j]) * factor[(cc + j) % NH]);
-            tmem_st16(t_o + cc + lane_base, o);
+            for (int j = 0; j < 2 * kPairs; ++j) factor[8 * (j >> 1) + col + (j & 1)] = f[j];
+          softmax_bar(wg);   // the factors are there, the maxima read
+          if (i > 0) {
+            mbar_wait_spin(p_empty, (g - 1) & 1, a.error_flag, &failed);
+            tc_fence_after();
+#pragma unroll 1
+            for (int m = 0; m < C::kBlocks; ++m)
+#pragma unroll 1
+              for (int h0 = head0; h0 < head0 + HW; h0 += kCols) {
+                uint32_t o[kCols];
+                tmem_ld_cols(t_o + m * NH + h0 + lane_base, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < kCols; ++j)
+                  o[j] = __float_as_uint(__uint_as_float(o[j]) * factor[h0 + j]);
+                tmem_st_cols(t_o + m * NH + h0 + lane_base, o);
+              }
+            tmem_st_wait();
           }
-          tmem_st_wait();
+          softmax_bar(wg);   // the factors are read: the next tile may write its own
         }
+        const bool p_free = g == 0 || mbar_test_wait(p_empty, (g - 1) & 1);   // used below
         // probabilities; a column without any key so far has reference -inf and stays zero
-        uint32_t packed[NH / 4];
+        uint32_t packed[HW / 4];
 #pragma unroll
         for (int j = 0; j < kPairs; ++j) {
           float p[4];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float r = ref[2 * j + e] == -INFINITY ? 0.0f : ref[2 * j + e] - kShift;
-            p[e] = exp2f(z[4 * j + e] - r);
-            p[2 + e] = exp2f(z[4 * j + 2 + e] - r);
+            const float r = ref[2 * j + e] == -INFINITY ? 0.0f : kShift - ref[2 * j + e];
+            p[e] = exp2_approx(fmaf(z[4 * j + e], c2, r));
+            p[2 + e] = exp2_approx(fmaf(z[4 * j + 2 + e], c2, r));
             sum[2 * j + e] += p[e] + p[2 + e];
           }
           packed[2 * j] = E::pack2(p[0], p[1]);
           packed[2 * j + 1] = E::pack2(p[2], p[3]);
         }
-        if (g > 0) mbar_wait_spin(p_empty, (g - 1) & 1, a.error_flag, &failed);
+        if (!p_free) mbar_wait_spin(p_empty, (g - 1) & 1, a.error_flag, &failed);
         uint8_t* ps = smem + (s_p - base);
 #pragma unroll
         for (int j = 0; j < kPairs; ++j) {
-          *reinterpret_cast<uint32_t*>(ps + p_offset<NH>(key0, j) + 2 * col) = packed[2 * j];
-          *reinterpret_cast<uint32_t*>(ps + p_offset<NH>(key0 + 8, j) + 2 * col) = packed[2 * j + 1];
+          *reinterpret_cast<uint32_t*>(ps + p_offset<NH>(key0, head0 / 8 + j) + 4 * (lane & 3)) = packed[2 * j];
+          *reinterpret_cast<uint32_t*>(ps + p_offset<NH>(key0 + 8, head0 / 8 + j) + 4 * (lane & 3)) = packed[2 * j + 1];
         }
-        if (valid < kTile || mask != 0xffu) {
+        if (valid < kTile || mask != 3u) {
           // rows of this tile that no key stands in hold what was there before (or a page's
           // stale tail): cleared, so that 0 x NaN cannot enter the product
-          const int key = threadIdx.x >> 1;
-          if (key >= valid || !(mask >> (key >> 3) & 1u)) {
-            uint8_t* row = smem + st * C::kStageBytes + (key >> 3) * C::kGroupBytes + (key & 7) * 128 +
-                           (threadIdx.x & 1) * (C::kChunks / 2) * 1024;
-            for (int c = 0; c < C::kChunks / 2; ++c)
+          const int key = quarter * 16 + (lane >> 1);
+          if (key >= valid || !(mask >> (key >> 3 & 1) & 1u)) {
+            uint8_t* row = smem + st * C::kStageBytes + (key >> 3) * C::kGroupBytes + (key & 7) * 128;
+            for (int c = 2 * wg + (lane & 1); c < C::kChunks; c += 4)
 #pragma unroll
               for (int x = 0; x < 8; ++x)
                 *reinterpret_cast<uint4*>(row + c * 1024 + x * 16) = make_uint4(0, 0, 0, 0);
@@ -578,58 +653,66 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(p_full);
       }
 
-      // ---- the segment's result ----
+      // ---- the segment's result: maxima and sums over the warpgroup ----
 #pragma unroll
       for (int o = 4; o < 32; o <<= 1)
 #pragma unroll
-        for (int j = 0; j < 2 * kPairs; ++j) sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], o);
-      float* ws = wmax + (g & 1) * 4 * NH;   // the maxima of the tile after this one come later
+        for (int j = 0; j < 2 * kPairs; ++j) {
+          sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], o);
+          run[j] = fmaxf(run[j], __shfl_xor_sync(0xffffffffu, run[j], o));
+        }
+      float* wsum = wmax + 4 * NH;
       if (lane < 4)
 #pragma unroll
-        for (int j = 0; j < kPairs; ++j)
-          *reinterpret_cast<float2*>(ws + warp * NH + 8 * j + col) =
+        for (int j = 0; j < kPairs; ++j) {
+          *reinterpret_cast<float2*>(wsum + quarter * NH + 8 * j + col) =
               make_float2(sum[2 * j], sum[2 * j + 1]);
-      softmax_bar();
+          *reinterpret_cast<float2*>(wmax + quarter * NH + 8 * j + col) =
+              make_float2(run[2 * j], run[2 * j + 1]);
+        }
+      softmax_bar(wg);
       const bool whole = sg.count == sg.tiles;
       const int slot = 2 * blockIdx.x + (nseg == 0 ? 0 : 1);
-      if (warp == 0 && lane < 4)
+      if (quarter == 0 && lane < 4)
 #pragma unroll
         for (int j = 0; j < 2 * kPairs; ++j) {
           const int h = 8 * (j >> 1) + col + (j & 1), head = sg.group * NH + h;
-          const float l = ws[h] + ws[NH + h] + ws[2 * NH + h] + ws[3 * NH + h];
+          const float l = wsum[h] + wsum[NH + h] + wsum[2 * NH + h] + wsum[3 * NH + h];
+          const float m = fmaxf(fmaxf(wmax[h], wmax[NH + h]), fmaxf(wmax[2 * NH + h], wmax[3 * NH + h]));
+          const bool any = m != -INFINITY;
+          const float most = any ? m * c2 : -INFINITY;
           factor[h] = !whole ? 1.0f : l > 0.0f || l != l ? 1.0f / l : 0.0f;
           if (head >= a.n1) continue;
           if (!whole) {
-            a.ws_s[(int64_t)slot * NH + h] = make_float4(ref[j] - kShift, run[j], l, 0.0f);
+            a.ws_s[(int64_t)slot * NH + h] = make_float4(ref[j] - kShift, most, l, m);
           } else if (a.softmax_max) {
             const int64_t at = (int64_t)sg.row * a.n1 + head;
-            const bool any = run[j] != -INFINITY;
-            a.softmax_max[at] = any ? run[j] * 0.6931471805599453f : 0.0f;
-            a.softmax_sum[at] = any ? l * exp2f(ref[j] - kShift - run[j]) : 0.0f;
+            a.softmax_max[at] = any ? m * fabsf(a.scale) : 0.0f;
+            a.softmax_sum[at] = any ? l * exp2f(ref[j] - kShift - most) : 0.0f;
           }
         }
-      softmax_bar();
+      softmax_bar(wg);
       mbar_wait_spin(p_empty, (g - 1) & 1, a.error_flag, &failed);
       tc_fence_after();
-      const int heads = min(NH, a.n1 - sg.group * NH);
-      const int dim = warp * 32 + lane;
+      const int heads = min(head0 + HW, a.n1 - sg.group * NH);
+      const int dim = quarter * 32 + lane;
 #pragma unroll 1
       for (int m = 0; m < C::kBlocks; ++m)
 #pragma unroll 1
-        for (int h0 = 0; h0 < heads; h0 += 16) {
-          uint32_t o[16];
-          tmem_ld16(t_o + m * NH + h0 + lane_base, o);
+        for (int h0 = head0; h0 < heads; h0 += kCols) {
+          uint32_t o[kCols];
+          tmem_ld_cols(t_o + m * NH + h0 + lane_base, o);
           tmem_ld_wait();
           if (whole) {
             T* out = static_cast<T*>(a.out) +
                      ((int64_t)sg.row * a.n1 + sg.group * NH + h0) * D + m * 128 + dim;
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
+            for (int j = 0; j < kCols; ++j)
               if (h0 + j < heads) out[j * D] = E::from_f(__uint_as_float(o[j]) * factor[h0 + j]);
           } else {
             float* out = a.ws_o + ((int64_t)slot * NH + h0) * D + m * 128 + dim;
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
+            for (int j = 0; j < kCols; ++j)
               if (h0 + j < heads) out[j * D] = __uint_as_float(o[j]);
           }
         }
@@ -643,61 +726,84 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 5) {
+  if (warp == kMmaWarp) {
     tmem_relinquish<1>();
     tmem_dealloc<1>(tmem, C::kTmem);
   }
 }
 
-// One block per (row, head): join the parts that the row's CTAs left.
+// One block per (row, head): join the parts that the row's CTAs left.  D / 4 threads take a
+// part (one float4 each), kGroups of them go through the parts side by side.
+constexpr int kJoinThreads = 256;
+
 template <int D, int NH, typename T>
-__global__ void __launch_bounds__(128) attn_paged_combine_kernel(const Args a, int grid) {
+__global__ void __launch_bounds__(kJoinThreads) attn_paged_combine_kernel(const Args a, int grid) {
   using E = ElemTraits<T>;
-  constexpr int kPer = D / 128;
+  constexpr int kGroups = kJoinThreads / (D / 4);
+  __shared__ float4 part[kGroups][D / 4];
+  __shared__ float psum[kGroups];
   griddep_wait();
   const int row = blockIdx.x / a.n1, head = blockIdx.x - row * a.n1;
+  const int first = a.ws_prefix[row], next = a.ws_prefix[row + 1], all = a.ws_prefix[a.rows];
+  const int count = next - first;
   const int64_t at = blockIdx.x;
-  const int first = a.ws_prefix[row], count = a.ws_prefix[row + 1] - first;
-  T* out = static_cast<T*>(a.out) + at * D + threadIdx.x * kPer;
+  const int grp = threadIdx.x / (D / 4), col = threadIdx.x % (D / 4);
+  T* out = static_cast<T*>(a.out) + at * D + col * 4;
   if (count == 0) {
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) out[j] = E::from_f(0.0f);
+    if (grp == 0) *reinterpret_cast<uint2*>(out) = make_uint2(0, 0);
     if (threadIdx.x == 0 && a.softmax_max) a.softmax_max[at] = a.softmax_sum[at] = 0.0f;
     return;
   }
-  const int64_t tiles = (int64_t)a.ws_prefix[a.rows] * a.groups;
+  const int64_t tiles = (int64_t)all * a.groups;
   const int64_t ctas = ctas_used(tiles, grid);
   const int group = head / NH, h = head - group * NH;
   const int64_t x0 = (int64_t)first * a.groups + (int64_t)group * count, x1 = x0 + count;
   const int c0 = (int)(((x0 + 1) * ctas - 1) / tiles), c1 = (int)((x1 * ctas - 1) / tiles);
   if (c0 == c1) return;   // written whole
-  // the part of CTA c is its first one unless the row begins inside its share
-  auto slot = [&](int c) { return 2 * c + (tiles * c / ctas < x0 ? 1 : 0); };
-  float ref = -INFINITY, run = -INFINITY;
-  for (int c = c0; c <= c1; ++c) {
-    const float4 s = a.ws_s[(int64_t)slot(c) * NH + h];
+  // a CTA's part of this row is its first, but where the row begins inside the CTA's share
+  const int skip = tiles * c0 / ctas < x0 ? 1 : 0;
+  auto slot = [&](int c) { return (int64_t)(2 * c + (c == c0 ? skip : 0)) * NH + h; };
+  float ref = -INFINITY, run = -INFINITY, top = -INFINITY;
+  for (int c = c0 + (threadIdx.x & 31); c <= c1; c += 32) {
+    const float4 s = a.ws_s[slot(c)];
     ref = fmaxf(ref, s.x);
     run = fmaxf(run, s.y);
+    top = fmaxf(top, s.w);
   }
-  float acc[kPer] = {}, sum = 0.0f;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, o));
+    run = fmaxf(run, __shfl_xor_sync(0xffffffffu, run, o));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  }
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float sum = 0.0f;
   if (ref != -INFINITY) {
 #pragma unroll 4
-    for (int c = c0; c <= c1; ++c) {
-      const int64_t sl = (int64_t)slot(c) * NH + h;
-      const float4 s = a.ws_s[sl];
+    for (int c = c0 + grp; c <= c1; c += kGroups) {
+      const float4 s = a.ws_s[slot(c)];
+      const float4 o = *reinterpret_cast<const float4*>(a.ws_o + slot(c) * D + col * 4);
       const float w = s.x == ref ? 1.0f : exp2f(s.x - ref);
       sum += w * s.z;
-      const float* o = a.ws_o + sl * D + threadIdx.x * kPer;
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) acc[j] += w * o[j];
+      acc.x += w * o.x, acc.y += w * o.y, acc.z += w * o.z, acc.w += w * o.w;
     }
   }
-  const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+  part[grp][col] = acc;
+  if (col == 0) psum[grp] = sum;
+  __syncthreads();
+  if (grp > 0) return;
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) out[j] = E::from_f(acc[j] * inv);
+  for (int k = 1; k < kGroups; ++k) {
+    const float4 o = part[k][col];
+    sum += psum[k];
+    acc.x += o.x, acc.y += o.y, acc.z += o.z, acc.w += o.w;
+  }
+  const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+  *reinterpret_cast<uint2*>(out) =
+      make_uint2(E::pack2(acc.x * inv, acc.y * inv), E::pack2(acc.z * inv, acc.w * inv));
   if (threadIdx.x == 0 && a.softmax_max) {
     const bool any = run != -INFINITY;
-    a.softmax_max[at] = any ? run * 0.6931471805599453f : 0.0f;
+    a.softmax_max[at] = any ? top * fabsf(a.scale) : 0.0f;
     a.softmax_sum[at] = any ? sum * exp2f(ref - run) : 0.0f;
   }
 }
@@ -778,7 +884,7 @@ int launch(const DsaAttnPagedParams* p, cudaStream_t stream) {
   pdl[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(b * s1 * n1));
-  cfg.blockDim = dim3(128);
+  cfg.blockDim = dim3(kJoinThreads);
   cfg.stream = stream;
   cfg.attrs = pdl;
   cfg.numAttrs = 1;
