@@ -126,3 +126,37 @@ def self_overlap(t: torch.Tensor) -> bool:
             return True
         reach += st * (n - 1)
     return False
+
+
+# Host time is most of a small call, so the checks of a call's arguments and what follows from
+# their shapes (strides, sizes, output shapes) are kept per signature, and the raw device and
+# stream handles are asked for without torch's wrapper objects.
+class Plans(dict):
+    """What calls of one signature (shapes, strides, types, devices, options) have in common."""
+
+    def keep(self, key, plan):
+        if len(self) >= 1024:
+            self.clear()
+        self[key] = plan
+        return plan
+
+
+def signature(tensors) -> tuple:
+    return tuple([None if t is None else (t.shape, t.stride(), t.dtype, t.get_device()) for t in tensors])
+
+
+try:
+    from torch._C import _cuda_getCurrentRawStream as raw_stream   # device index -> cudaStream_t
+    from torch._C import _cuda_getDevice as current_device
+except ImportError:   # a torch without these names, or without CUDA
+    def raw_stream(index):
+        return torch.cuda.current_stream(index).cuda_stream
+
+    def current_device():
+        return torch.cuda.current_device()
+
+
+def is_i32_vector(t, n, index) -> bool:
+    """A tensor the kernels read as int32[n] on device `index` as it is."""
+    return torch.is_tensor(t) and t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] == n \
+        and t.get_device() == index and t.is_contiguous()

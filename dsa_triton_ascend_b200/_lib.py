@@ -172,6 +172,7 @@ class PagesParams(ctypes.Structure):
 _lock = threading.Lock()
 _lib = None
 _err_bufs: dict = {}
+_report_ptrs: dict = {}
 
 
 def lib() -> ctypes.CDLL:
@@ -261,6 +262,14 @@ def report_flag(device: torch.device) -> torch.Tensor:
     """Per-device int32 for operators that report a request they cannot meet (a page that is
     not in the pool, no page left) and go on: such a bit stops no other kernel."""
     return _flags(device)[1:]
+
+
+def report_ptr(index: int) -> int:
+    """Address of :func:`report_flag` of device `index`."""
+    p = _report_ptrs.get(index)
+    if p is None:
+        p = _report_ptrs[index] = report_flag(torch.device("cuda", index)).data_ptr()
+    return p
 
 
 def check_device_errors(device=None) -> None:

@@ -810,14 +810,6 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_combine_kernel(const 
 
 int heads_of(int64_t n1) { return n1 <= 16 ? 16 : n1 <= 32 ? 32 : 64; }
 
-int sm_count() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return 0;
-  return n;
-}
-
 int64_t align256(int64_t x) { return (x + 255) & ~(int64_t)255; }
 
 template <int D, int NH, typename T>
@@ -874,9 +866,8 @@ int launch(const DsaAttnPagedParams* p, cudaStream_t stream) {
   a.ws_prefix = reinterpret_cast<int32_t*>(ws);
 
   auto kern = attn_paged_kernel<D, NH, T>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) !=
-      cudaSuccess)
-    return DSA_ERR_CUDA;
+  static std::atomic<uint64_t> ready;   // devices on which the kernel may use its shared memory
+  if (!allow_smem(reinterpret_cast<const void*>(kern), C::kSmem, &ready)) return DSA_ERR_CUDA;
   kern<<<grid, kThreads, C::kSmem, stream>>>(maps, a);
   if (cudaGetLastError() != cudaSuccess) return DSA_ERR_CUDA;
   cudaLaunchAttribute pdl[1];
@@ -918,7 +909,7 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 extern "C" int64_t dsa_attn_paged_workspace_size(int64_t batch, int64_t s1, int64_t n1, int64_t d) {
   using namespace dsa::attn_paged;
   if (batch < 0 || s1 < 0 || n1 < 1 || n1 > 128 || d < 1) return -1;
-  const int64_t nh = heads_of(n1), grid = sm_count();
+  const int64_t nh = heads_of(n1), grid = dsa::sm_count();
   if (grid < 1) return -1;
   return align256(2 * grid * nh * (d * 4 + 16) + (batch * s1 + 1) * 4);
 }

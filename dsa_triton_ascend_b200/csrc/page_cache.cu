@@ -14,6 +14,7 @@
 
 #include "dsa_b200.h"
 #include "rotary.cuh"
+#include "tma_host.h"
 
 namespace dsa {
 namespace pages {
@@ -550,10 +551,8 @@ extern "C" int dsa_pages(const DsaPagesParams* p, void* stream_) {
   a.max_blocks = (int)p->max_blocks;
   a.num_pages = (int)p->num_pages;
   a.page_size = (int)p->page_size;
-  int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return DSA_ERR_CUDA;
+  const int sms = dsa::sm_count();
+  if (sms < 1) return DSA_ERR_CUDA;
   if (!copy) {
     page_plan_kernel<<<1, kPlanThreads, 0, stream>>>(a);
     if (cudaGetLastError() != cudaSuccess) return DSA_ERR_CUDA;

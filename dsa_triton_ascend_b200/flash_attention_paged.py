@@ -11,34 +11,80 @@ from __future__ import annotations
 import torch
 
 from . import _host as H
-from ._lib import AttnPagedParams, check, lib, ptr, report_flag, stream_ptr
+from ._lib import AttnPagedParams, check, lib, report_ptr
 
 _VALID_D = (128, 256, 512)
 _D_ROPE = 64
 
 
-def _strided(t: torch.Tensor, dims) -> tuple:
-    """``t`` with a contiguous last dim, 16-byte steps and a 16-byte base (copied if it has
-    none), and its strides over ``dims`` (a size-1 dim's own stride means nothing)."""
-    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(
-        t.shape[i] == 1 or t.stride(i) % 8 == 0 for i in dims)
-    if not ok:
-        t = t.contiguous()
-        if t.data_ptr() % 16:
-            t = t.clone()
-    width = -(-t.shape[-1] // 8) * 8
-    return t, [t.stride(i) if t.shape[i] > 1 else width for i in dims]
+_plans = H.Plans()
+
+
+def _tma_strides(t: torch.Tensor):
+    """Strides over (batch, token, head) if TMA can address the tensor (contiguous last dim,
+    16-byte steps), else None.  A size-1 dim's own stride means nothing."""
+    if t.stride(-1) != 1 or any(t.shape[i] > 1 and t.stride(i) % 8 for i in (0, 1, 2)):
+        return None
+    return [t.stride(i) if t.shape[i] > 1 else t.shape[-1] for i in (0, 1, 2)]
 
 
 def _cache_strides(t: torch.Tensor, what: str):
     """Strides over (page, row) of a cache [num_pages, page_size, 1, width]; a cache is never
     copied, so one that TMA cannot address is refused."""
-    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(
-            t.shape[i] > 1 and t.stride(i) % 8 for i in (0, 1)):
-        raise ValueError(f"{what} needs a contiguous last dim, 16-byte strides and a 16-byte base")
+    if t.stride(-1) != 1 or any(t.shape[i] > 1 and t.stride(i) % 8 for i in (0, 1)):
+        raise ValueError(f"{what} needs a contiguous last dim and 16-byte strides")
     width = t.shape[-1]
     row = t.stride(1) if t.shape[1] > 1 else width
     return (t.stride(0) if t.shape[0] > 1 else row * t.shape[1]), row
+
+
+def _plan(query, query_rope, key_cache, key_rope_cache, block_table, scale_value, sparse_mode):
+    """Check the arguments and fill in what their shapes decide: (parameters, strides fit,
+    statistics' shape, workspace bytes)."""
+    if sparse_mode not in (0, 3):
+        raise ValueError("Only sparse_mode 0 (full) / 3 (rightDownCausal) supported")
+    if query.dim() != 4 or query_rope.dim() != 4:
+        raise ValueError("query and query_rope must be [B, S1, N1, D]")
+    if key_cache.dim() != 4 or key_rope_cache.dim() != 4:
+        raise ValueError("key_cache and key_rope_cache must be [num_pages, page_size, 1, D]")
+    B, S1, N1, D = query.shape
+    num_pages, page, n2, dk = key_cache.shape
+    if D not in _VALID_D or dk != D:
+        raise ValueError(f"query and key_cache must share a D of {_VALID_D}, got {D} and {dk}")
+    if not 1 <= N1 <= 128:
+        raise ValueError(f"N1 must be 1..128, got {N1}")
+    if tuple(query_rope.shape) != (B, S1, N1, _D_ROPE):
+        raise ValueError(f"query_rope must be {(B, S1, N1, _D_ROPE)}, got {tuple(query_rope.shape)}")
+    if n2 != 1 or tuple(key_rope_cache.shape) != (num_pages, page, 1, _D_ROPE):
+        raise ValueError("Only N2=1 (MQA) is supported, with key_rope_cache "
+                         f"[num_pages, page_size, 1, {_D_ROPE}]")
+    if num_pages < 1 or page < 8 or page % 8:
+        raise ValueError(f"page_size ({page}) must be a multiple of 8 and the cache not empty")
+    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.shape[0] != B \
+            or block_table.shape[1] < 1:
+        raise ValueError("block_table must be an int32 [B, max_blocks] tensor")
+    dtype = H.dtype_code(query)
+    if not query.dtype == query_rope.dtype == key_cache.dtype == key_rope_cache.dtype:
+        raise ValueError("query, query_rope and the caches must share their dtype")
+    H.require_cuda(query, query_rope, key_cache, key_rope_cache, block_table)
+    if not all(t.device == query.device for t in (query_rope, key_cache, key_rope_cache, block_table)):
+        raise ValueError("all tensors must be on one device")
+    p = AttnPagedParams()
+    p.k_page_stride, p.k_row_stride = _cache_strides(key_cache, "key_cache")
+    p.kr_page_stride, p.kr_row_stride = _cache_strides(key_rope_cache, "key_rope_cache")
+    qs, qrs = _tma_strides(query), _tma_strides(query_rope)
+    contiguous = lambda w: (S1 * N1 * w, N1 * w, w)
+    p.q_batch_stride, p.q_token_stride, p.q_head_stride = qs or contiguous(D)
+    p.qr_batch_stride, p.qr_token_stride, p.qr_head_stride = qrs or contiguous(_D_ROPE)
+    p.batch, p.s1, p.n1, p.d = B, S1, N1, D
+    p.num_pages, p.page_size, p.max_blocks = num_pages, page, block_table.shape[1]
+    p.scale, p.sparse_mode, p.dtype = scale_value, int(sparse_mode), dtype
+    p.workspace_bytes = lib().dsa_attn_paged_workspace_size(B, S1, N1, D)
+    return bytes(p), qs is not None, qrs is not None, (B, 1, S1, N1), max(p.workspace_bytes, 16)
+
+
+def _copied(t: torch.Tensor) -> torch.Tensor:
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def flash_attention_paged(
@@ -68,70 +114,56 @@ def flash_attention_paged(
     zeros when ``return_softmax_lse`` is False.  Strided inputs (views of a joint projection or
     of a joint cache) are read in place.
     """
-    if sparse_mode not in (0, 3):
-        raise ValueError("Only sparse_mode 0 (full) / 3 (rightDownCausal) supported")
-    if query.dim() != 4 or query_rope.dim() != 4:
-        raise ValueError("query and query_rope must be [B, S1, N1, D]")
-    if key_cache.dim() != 4 or key_rope_cache.dim() != 4:
-        raise ValueError("key_cache and key_rope_cache must be [num_pages, page_size, 1, D]")
-    B, S1, N1, D = query.shape
-    num_pages, page, n2, dk = key_cache.shape
-    if D not in _VALID_D or dk != D:
-        raise ValueError(f"query and key_cache must share a D of {_VALID_D}, got {D} and {dk}")
-    if not 1 <= N1 <= 128:
-        raise ValueError(f"N1 must be 1..128, got {N1}")
-    if tuple(query_rope.shape) != (B, S1, N1, _D_ROPE):
-        raise ValueError(f"query_rope must be {(B, S1, N1, _D_ROPE)}, got {tuple(query_rope.shape)}")
-    if n2 != 1 or tuple(key_rope_cache.shape) != (num_pages, page, 1, _D_ROPE):
-        raise ValueError("Only N2=1 (MQA) is supported, with key_rope_cache "
-                         f"[num_pages, page_size, 1, {_D_ROPE}]")
-    if num_pages < 1 or page < 8 or page % 8:
-        raise ValueError(f"page_size ({page}) must be a multiple of 8 and the cache not empty")
-    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.shape[0] != B \
-            or block_table.shape[1] < 1:
-        raise ValueError("block_table must be an int32 [B, max_blocks] tensor")
-    dtype = H.dtype_code(query)
-    if not query.dtype == query_rope.dtype == key_cache.dtype == key_rope_cache.dtype:
-        raise ValueError("query, query_rope and the caches must share their dtype")
-    H.require_cuda(query, query_rope, key_cache, key_rope_cache, block_table)
+    scale_value = float(scale_value)
+    key = (H.signature((query, query_rope, key_cache, key_rope_cache, block_table)), scale_value, sparse_mode)
+    plan = _plans.get(key)
+    index = query.get_device()
+    if plan is None or H.current_device() != index:
+        if plan is None:
+            checked = lambda: _plan(query, query_rope, key_cache, key_rope_cache, block_table, scale_value, sparse_mode)
+            if query.is_cuda:
+                with torch.cuda.device(index):
+                    plan = _plans.keep(key, checked())
+            else:
+                checked()
+        if H.current_device() != index:
+            with torch.cuda.device(index):
+                return flash_attention_paged(query, query_rope, key_cache, key_rope_cache, block_table,
+                                             actual_seq_lengths_key, scale_value, actual_seq_lengths_query,
+                                             sparse_mode, return_softmax_lse)
+    template, q_fits, qr_fits, stat_shape, ws_bytes = plan
     dev = query.device
-    if not all(t.device == dev for t in (query_rope, key_cache, key_rope_cache, block_table)):
-        raise ValueError("all tensors must be on one device")
-    kp, kr = _cache_strides(key_cache, "key_cache")
-    rp, rr = _cache_strides(key_rope_cache, "key_rope_cache")
-
-    with torch.cuda.device(dev):
-        max_blocks = block_table.shape[1]
-        act_k = H.lens_tensor(actual_seq_lengths_key, B, max_blocks * page, dev).contiguous()
-        act_q = None
-        if actual_seq_lengths_query is not None:
-            act_q = H.lens_tensor(actual_seq_lengths_query, B, S1, dev).contiguous()
-        out = torch.empty((B, S1, N1, D), dtype=query.dtype, device=dev)
-        alloc = torch.empty if return_softmax_lse else torch.zeros
-        smax = alloc((B, 1, S1, N1), dtype=torch.float32, device=dev)
-        ssum = alloc((B, 1, S1, N1), dtype=torch.float32, device=dev)
-        if B == 0 or S1 == 0:
-            return out, smax, ssum
-        q, qs = _strided(query, (0, 1, 2))
-        qr, qrs = _strided(query_rope, (0, 1, 2))
-        bt = block_table.contiguous()
-        ws_bytes = lib().dsa_attn_paged_workspace_size(B, S1, N1, D)
-        ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=dev)
-        p = AttnPagedParams()
-        p.query, p.query_rope, p.key_cache, p.key_rope_cache = ptr(q), ptr(qr), ptr(key_cache), ptr(key_rope_cache)
-        p.block_table, p.act_q, p.act_k, p.out = ptr(bt), ptr(act_q), ptr(act_k), ptr(out)
-        if return_softmax_lse:
-            p.softmax_max, p.softmax_sum = ptr(smax), ptr(ssum)
-        p.error_flag = ptr(report_flag(dev))
-        p.workspace, p.workspace_bytes = ptr(ws), ws_bytes
-        p.batch, p.s1, p.n1, p.d = B, S1, N1, D
-        p.num_pages, p.page_size, p.max_blocks = num_pages, page, max_blocks
-        p.q_batch_stride, p.q_token_stride, p.q_head_stride = qs
-        p.qr_batch_stride, p.qr_token_stride, p.qr_head_stride = qrs
-        p.k_page_stride, p.k_row_stride = kp, kr
-        p.kr_page_stride, p.kr_row_stride = rp, rr
-        p.scale = float(scale_value)
-        p.sparse_mode = int(sparse_mode)
-        p.dtype = dtype
-        check(lib().dsa_attn_paged(p, stream_ptr(dev)), "dsa_attn_paged")
+    B, _, S1, _ = stat_shape
+    p = AttnPagedParams.from_buffer_copy(template)
+    act_k = actual_seq_lengths_key
+    if not H.is_i32_vector(act_k, B, index):
+        act_k = H.lens_tensor(act_k, B, p.max_blocks * p.page_size, dev).contiguous()
+    act_q = actual_seq_lengths_query
+    if act_q is not None and not H.is_i32_vector(act_q, B, index):
+        act_q = H.lens_tensor(act_q, B, S1, dev).contiguous()
+    out = torch.empty(query.shape, dtype=query.dtype, device=dev)
+    alloc = torch.empty if return_softmax_lse else torch.zeros
+    smax = alloc(stat_shape, dtype=torch.float32, device=dev)
+    ssum = alloc(stat_shape, dtype=torch.float32, device=dev)
+    if B == 0 or S1 == 0:
+        return out, smax, ssum
+    q = query if q_fits and query.data_ptr() % 16 == 0 else _copied(query)
+    qr = query_rope if qr_fits and query_rope.data_ptr() % 16 == 0 else _copied(query_rope)
+    if q is not query:
+        p.q_batch_stride, p.q_token_stride, p.q_head_stride = q.stride()[:3]
+    if qr is not query_rope:
+        p.qr_batch_stride, p.qr_token_stride, p.qr_head_stride = qr.stride()[:3]
+    kc, krc = key_cache.data_ptr(), key_rope_cache.data_ptr()
+    if (kc | krc) % 16:
+        raise ValueError("key_cache and key_rope_cache need 16-byte aligned bases")
+    bt = block_table.contiguous()
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    p.query, p.query_rope, p.key_cache, p.key_rope_cache = q.data_ptr(), qr.data_ptr(), kc, krc
+    p.block_table, p.act_k, p.out, p.workspace = bt.data_ptr(), act_k.data_ptr(), out.data_ptr(), ws.data_ptr()
+    if act_q is not None:
+        p.act_q = act_q.data_ptr()
+    if return_softmax_lse:
+        p.softmax_max, p.softmax_sum = smax.data_ptr(), ssum.data_ptr()
+    p.error_flag = report_ptr(index)
+    check(lib().dsa_attn_paged(p, H.raw_stream(index)), "dsa_attn_paged")
     return out, smax, ssum

@@ -12,7 +12,7 @@ import math
 import torch
 
 from . import _host as H
-from ._lib import DSA_DTYPE_FP32, RotaryParams, check, lib, ptr, report_flag, stream_ptr
+from ._lib import DSA_DTYPE_FP32, RotaryParams, check, lib, ptr, report_ptr, stream_ptr
 
 _MAX_DIM = 256
 LAYOUTS = ("interleaved", "half")
@@ -78,17 +78,11 @@ def _token_strides(t: torch.Tensor):
     return (0, *t.stride()[:2]) if t.dim() == 3 else tuple(t.stride()[:3])
 
 
-def rotary_embedding(x, table, positions, layout="interleaved", offset=0, inverse=False, out=None):
-    """Rotate ``x`` [B, S, N, H] (``positions`` [B, S]) or [T, N, H] (``positions`` [T]): of each
-    head the values ``offset`` .. ``offset + table.shape[1]`` turn by the angles of the token's
-    position, the others are copied.  ``layout`` "interleaved" pairs (2 i, 2 i + 1), "half"
-    pairs (i, i + dim / 2).  ``inverse`` turns back by the same table, amplitude kept: the
-    gradient with respect to ``x`` of a rotation is the inverse rotation of the gradient.
+_plans = H.Plans()
 
-    bf16, fp16 or fp32; any strides with a contiguous last dim.  ``out`` (same shape and type;
-    ``x`` itself for a rotation in place) receives the result, else a new tensor.  A position
-    outside the table gives a zero row and is reported by ``check_device_errors``.
-    """
+
+def _plan(x, table, positions, layout, offset, inverse, out):
+    """Check the arguments and fill in what their shapes decide."""
     if layout not in LAYOUTS:
         raise ValueError(f"layout must be one of {LAYOUTS}, got {layout!r}")
     if x.dim() not in (3, 4):
@@ -107,36 +101,60 @@ def rotary_embedding(x, table, positions, layout="interleaved", offset=0, invers
     if positions.dtype not in (torch.int32, torch.int64):
         raise ValueError("positions must be int32 or int64")
     H.require_cuda(x, table, positions, out)
-    dev = x.device
-    if table.device != dev or positions.device != dev:
+    if table.device != x.device or positions.device != x.device:
         raise ValueError("all tensors must be on one device")
-    with torch.cuda.device(dev):
-        if x.stride(-1) != 1:
-            if out is x:
-                raise ValueError("a rotation in place needs a contiguous last dim")
-            x = x.contiguous()
-        if out is None:
-            out = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        else:
-            if out.shape != x.shape or out.dtype != x.dtype or out.device != dev or out.stride(-1) != 1:
-                raise ValueError("out must have x's shape, dtype and device, and a contiguous last dim")
-            if H.self_overlap(out):
-                raise ValueError("out must not be an expanded tensor")
-            if H.overlap(out, x):
-                raise ValueError("out overlaps x (pass x itself to rotate in place)")
-        if positions.dtype != torch.int32:   # a position past 32 bits stays outside the table
-            positions = positions.clamp(-1, 0x7fffffff).to(torch.int32)
-        positions = positions.contiguous()
-        table = table.contiguous()
-        p = RotaryParams()
-        p.x, p.out, p.positions, p.table = ptr(x), ptr(out), ptr(positions), ptr(table)
-        p.error_flag = ptr(report_flag(dev))
-        p.batch, p.s = (1, x.shape[0]) if x.dim() == 3 else x.shape[:2]
-        p.heads, p.head_dim, p.offset, p.dim = x.shape[-2], x.shape[-1], int(offset), dim
-        p.max_positions = table.shape[0]
+    if out is not None:
+        if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or out.stride(-1) != 1:
+            raise ValueError("out must have x's shape, dtype and device, and a contiguous last dim")
+        if H.self_overlap(out):
+            raise ValueError("out must not be an expanded tensor")
+    p = RotaryParams()
+    p.batch, p.s = (1, x.shape[0]) if x.dim() == 3 else x.shape[:2]
+    p.heads, p.head_dim, p.offset, p.dim = x.shape[-2], x.shape[-1], int(offset), dim
+    p.max_positions = table.shape[0]
+    p.x_batch_stride, p.x_token_stride, p.x_head_stride = _token_strides(x)
+    o = torch.empty(x.shape, dtype=x.dtype, device="meta") if out is None else out
+    p.out_batch_stride, p.out_token_stride, p.out_head_stride = _token_strides(o)
+    p.half_layout, p.inverse = int(layout == "half"), int(bool(inverse))
+    p.dtype = DSA_DTYPE_FP32 if x.dtype == torch.float32 else H.dtype_code(x)
+    return bytes(p)
+
+
+def rotary_embedding(x, table, positions, layout="interleaved", offset=0, inverse=False, out=None):
+    """Rotate ``x`` [B, S, N, H] (``positions`` [B, S]) or [T, N, H] (``positions`` [T]): of each
+    head the values ``offset`` .. ``offset + table.shape[1]`` turn by the angles of the token's
+    position, the others are copied.  ``layout`` "interleaved" pairs (2 i, 2 i + 1), "half"
+    pairs (i, i + dim / 2).  ``inverse`` turns back by the same table, amplitude kept: the
+    gradient with respect to ``x`` of a rotation is the inverse rotation of the gradient.
+
+    bf16, fp16 or fp32; any strides with a contiguous last dim.  ``out`` (same shape and type;
+    ``x`` itself for a rotation in place) receives the result, else a new tensor.  A position
+    outside the table gives a zero row and is reported by ``check_device_errors``.
+    """
+    key = (H.signature((x, table, positions, out)), layout, offset, inverse)
+    template = _plans.get(key)
+    if template is None:
+        template = _plans.keep(key, _plan(x, table, positions, layout, offset, inverse, out))
+    index = x.get_device()
+    if H.current_device() != index:
+        with torch.cuda.device(index):
+            return rotary_embedding(x, table, positions, layout, offset, inverse, out)
+    p = RotaryParams.from_buffer_copy(template)
+    if x.stride(-1) != 1:
+        if out is x:
+            raise ValueError("a rotation in place needs a contiguous last dim")
+        x = x.contiguous()
         p.x_batch_stride, p.x_token_stride, p.x_head_stride = _token_strides(x)
-        p.out_batch_stride, p.out_token_stride, p.out_head_stride = _token_strides(out)
-        p.half_layout, p.inverse = int(layout == "half"), int(bool(inverse))
-        p.dtype = DSA_DTYPE_FP32 if x.dtype == torch.float32 else H.dtype_code(x)
-        check(lib().dsa_rotary(p, stream_ptr(dev)), "dsa_rotary")
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    elif out is not x and H.overlap(out, x):
+        raise ValueError("out overlaps x (pass x itself to rotate in place)")
+    if positions.dtype != torch.int32:   # a position past 32 bits stays outside the table
+        positions = positions.clamp(-1, 0x7fffffff).to(torch.int32)
+    positions = positions.contiguous()
+    table = table.contiguous()
+    p.x, p.out = x.data_ptr(), out.data_ptr()
+    p.positions, p.table = positions.data_ptr(), table.data_ptr()
+    p.error_flag = report_ptr(index)
+    check(lib().dsa_rotary(p, H.raw_stream(index)), "dsa_rotary")
     return out
