@@ -17,6 +17,8 @@
 // that see no key.
 #include <cuda_runtime.h>
 
+#include "attn_paged.cuh"
+#include "attn_paged_pair.cuh"
 #include "dsa_b200.h"
 #include "sm100.cuh"
 #include "tma_host.h"
@@ -25,8 +27,6 @@ namespace dsa {
 namespace attn_paged {
 
 constexpr int kTile = 64;       // keys of a step
-constexpr int kRope = 64;
-constexpr int kSmemLimit = 232448;
 constexpr int kSoftmaxThreads = 128;   // of a warpgroup; there are two (warps 0-3, 4-7), each with
                                        // half of the heads
 constexpr int kLoadWarp = 8;           // warps 8-11: loads (one warp issues a box in 160 cycles,
@@ -35,9 +35,6 @@ constexpr int kMmaWarp = 12;
 constexpr int kQueryWarp = 13;
 constexpr int kThreads = 448;
 constexpr int kMaxStages = 8;
-constexpr int kMinTiles = 2;    // tiles a CTA takes at least: fewer cost more in joining than they save
-constexpr int kAhead = 3;       // tiles that are brought into L2 before their load
-constexpr float kRescale = 8.0f;       // log2 units the running max may pass the reference
 
 template <int D, int NH>
 struct Cfg {
@@ -63,100 +60,6 @@ struct Cfg {
                                     : kCols <= 256 ? 256 : 512;
   static_assert(kStages >= 2, "two key tiles have to fit");
 };
-
-struct Maps {
-  CUtensorMap q, qr, k, kr;
-};
-
-struct Args {
-  const int32_t* act_q;
-  const int32_t* act_k;
-  const int32_t* block_table;
-  void* out;
-  float* softmax_max;
-  float* softmax_sum;
-  int* error_flag;
-  int32_t* ws_prefix;   // [rows + 1] first tile of each row
-  float* ws_o;          // [2 * CTAs][NH][D]
-  float4* ws_s;         // [2 * CTAs][NH]: reference and running maximum (log2 units), sum,
-                        // raw running maximum
-  int32_t rows, s1, n1, groups;
-  int32_t page_size, max_blocks, num_pages, mode;
-  float scale;
-};
-
-// Keys that query row `row` sees.
-__device__ __forceinline__ int row_keys(const Args& a, int row) {
-  const int b = row / a.s1, s = row - b * a.s1;
-  const int ak = a.act_k[b], aq = a.act_q ? a.act_q[b] : a.s1;
-  int64_t n = min((int64_t)ak, (int64_t)a.max_blocks * a.page_size);
-  if (a.mode == 3) n = min(n, (int64_t)ak - aq + s + 1);
-  if (s >= aq || n < 0) n = 0;
-  return (int)n;
-}
-__device__ __forceinline__ int row_tiles(const Args& a, int row) {
-  return (row_keys(a, row) + kTile - 1) / kTile;
-}
-
-// CTAs that share `tiles` tiles.
-__device__ __forceinline__ int64_t ctas_used(int64_t tiles, int grid) {
-  const int64_t c = (tiles + kMinTiles - 1) / kMinTiles;
-  return c < 1 ? 1 : c < grid ? c : grid;
-}
-
-// Exclusive prefix of v over the block (kThreads threads) and its total.
-__device__ __forceinline__ int block_scan(int v, int* tmp, int* total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int x = v;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
-  }
-  __syncthreads();
-  if (lane == 31) tmp[warp] = x;
-  __syncthreads();
-  int before = 0, sum = 0;
-#pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) {
-    if (w < warp) before += tmp[w];
-    sum += tmp[w];
-  }
-  *total = sum;
-  return before + x - v;
-}
-
-// One CTA's share: tiles from (row, head group, tile) on, `left` of them.
-struct Work {
-  int row, group, tile, left;
-};
-// A run of tiles of one (row, head group).
-struct Segment {
-  int row, group, first, count, keys, tiles;
-};
-// The next run of `w` (false when the share is done); `w` moves past it.
-__device__ __forceinline__ bool next_segment(const Args& a, Work& w, Segment& s) {
-  while (w.left > 0 && w.row < a.rows) {
-    s.keys = row_keys(a, w.row);
-    s.tiles = (s.keys + kTile - 1) / kTile;
-    if (s.tiles == 0) {
-      ++w.row;
-      continue;
-    }
-    s.row = w.row;
-    s.group = w.group;
-    s.first = w.tile;
-    s.count = min(s.tiles - w.tile, w.left);
-    w.left -= s.count;
-    w.tile = 0;
-    if (++w.group == a.groups) {
-      w.group = 0;
-      ++w.row;
-    }
-    return true;
-  }
-  return false;
-}
 
 // P^T as the MN-major operand: a key's NH heads are one row of NH * 2 bytes, with the swizzle
 // of that width (128, 64 or 32 bytes).  Byte offset of 16-byte chunk `c` of key row `key`.
@@ -195,13 +98,6 @@ __device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, uint32_t (&r)[N / 2
           "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
           "=r"(r[14]), "=r"(r[15])
         : "r"(taddr));
-}
-
-// 2^x, 2^-126 and below flushed to 0
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 
 // The four warps of softmax warpgroup `wg` meet.
@@ -278,55 +174,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   if (warp == kMmaWarp) tmem_alloc<1>(smem_u32(tmem_ptr), C::kTmem);
 
-  // ---- this CTA's share of the tiles ----
-  int64_t total = 0;
-  int mine = 0, before = 0;   // the tiles of the thread's last row and of the rows before it
-  for (int r0 = 0; r0 < a.rows; r0 += kThreads) {
-    const int r = r0 + threadIdx.x;
-    int sum;
-    mine = r < a.rows ? row_tiles(a, r) : 0;
-    before = block_scan(mine, tmp, &sum);
-    if (blockIdx.x == 0 && r < a.rows) a.ws_prefix[r] = (int)total + before;
-    total += sum;
-  }
-  if (blockIdx.x == 0 && threadIdx.x == 0) a.ws_prefix[a.rows] = (int)total;
+  Work work = share_of<kTile, kThreads>(a, blockIdx.x, gridDim.x, blockIdx.x == 0, tmp, start);
   griddep_launch_dependents();
-  const int64_t tiles = total * a.groups;
-  const int64_t ctas = ctas_used(tiles, gridDim.x);
-  Work work{0, 0, 0, 0};
-  int64_t from = 0;
-  if (blockIdx.x < ctas) {
-    from = tiles * blockIdx.x / ctas;
-    work.left = (int)(tiles * (blockIdx.x + 1) / ctas - from);
-    int64_t seen = 0;
-    for (int r0 = 0; r0 < a.rows; r0 += kThreads) {
-      const int r = r0 + threadIdx.x;
-      int sum = (int)total;
-      if (a.rows > kThreads) {
-        mine = r < a.rows ? row_tiles(a, r) : 0;
-        before = block_scan(mine, tmp, &sum);
-      }
-      const int64_t first = (seen + before) * a.groups;
-      if (mine > 0 && first <= from && from < first + (int64_t)mine * a.groups) {
-        const int in = (int)(from - first);
-        start[0] = r;
-        start[1] = in / mine;
-        start[2] = in - (in / mine) * mine;
-      }
-      seen += sum;
-      if (seen * a.groups > from) break;   // the same for every thread
-    }
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_ptr;
   const uint32_t t_o = tmem + 2 * NH;
-  if (work.left > 0) {
-    work.row = start[0];
-    work.group = start[1];
-    work.tile = start[2];
-  }
+  take_start(work, start);
   bool failed = false;
 
   if (warp >= kLoadWarp && warp < kMmaWarp) {
@@ -339,7 +194,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool is_rope = lane & 2;
     Segment sg;
     int g = 0;
-    while (!failed && next_segment(a, work, sg)) {
+    while (!failed && next_segment<kTile>(a, work, sg)) {
       const int b = sg.row / a.s1;
       const int32_t* table = a.block_table + (int64_t)b * a.max_blocks;
       auto page_of = [&](int tile) {   // -1: no such page
@@ -385,7 +240,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // -------------------------------------------------------------------- queries
     Segment sg;
     int nseg = 0;
-    while (!failed && next_segment(a, work, sg)) {
+    while (!failed && next_segment<kTile>(a, work, sg)) {
       const int b = sg.row / a.s1, s = sg.row - b * a.s1;
       const int buf = nseg % C::kQBufs, use = nseg / C::kQBufs;
       if (use > 0) mbar_wait(q_empty(buf), (use - 1) & 1, a.error_flag, &failed);
@@ -441,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     Segment sg;
     int g = 0, nseg = 0;
-    while (!failed && next_segment(a, work, sg)) {
+    while (!failed && next_segment<kTile>(a, work, sg)) {
       const int buf = nseg % C::kQBufs;
       const uint32_t q_par = (nseg / C::kQBufs) & 1;
       for (int i = 0; i < sg.count && !failed; ++i, ++g) {
@@ -518,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     float ref[2 * kPairs], lim[2 * kPairs], run[2 * kPairs], sum[2 * kPairs];
     Segment sg;
     int g = 0, nseg = 0;
-    while (next_segment(a, work, sg)) {
+    while (next_segment<kTile>(a, work, sg)) {
 #pragma unroll
       for (int j = 0; j < 2 * kPairs; ++j) {
         ref[j] = run[j] = lim[j] = -INFINITY;
@@ -808,39 +663,13 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_combine_kernel(const 
   }
 }
 
-int heads_of(int64_t n1) { return n1 <= 16 ? 16 : n1 <= 32 ? 32 : 64; }
+// Heads of a work item: the smallest operand that holds them, and the pair kernel past 64.
+int heads_of(int64_t n1) { return n1 <= 16 ? 16 : n1 <= 32 ? 32 : n1 <= 64 ? 64 : 128; }
 
 int64_t align256(int64_t x) { return (x + 255) & ~(int64_t)255; }
 
-template <int D, int NH, typename T>
-int launch(const DsaAttnPagedParams* p, cudaStream_t stream) {
-  using C = Cfg<D, NH>;
-  constexpr bool kBf16 = ElemTraits<T>::kIsBf16;
-  const int64_t b = p->batch, s1 = p->s1, n1 = p->n1;
-  const int grid = sm_count();
-  if (grid < 1) return DSA_ERR_CUDA;
-  Maps maps;
-  {
-    const uint64_t dims[5] = {64, (uint64_t)n1, D / 64, (uint64_t)s1, (uint64_t)b};
-    const uint64_t st[4] = {(uint64_t)p->q_head_stride * 2, 128, (uint64_t)p->q_token_stride * 2,
-                            (uint64_t)p->q_batch_stride * 2};
-    const uint32_t box[5] = {64, NH, D / 64, 1, 1};
-    const uint64_t rdims[5] = {64, (uint64_t)n1, 1, (uint64_t)s1, (uint64_t)b};
-    const uint64_t rst[4] = {(uint64_t)p->qr_head_stride * 2, 128, (uint64_t)p->qr_token_stride * 2,
-                             (uint64_t)p->qr_batch_stride * 2};
-    const uint32_t rbox[5] = {64, NH, 1, 1, 1};
-    const uint64_t kdims[4] = {64, (uint64_t)p->page_size, D / 64, (uint64_t)p->num_pages};
-    const uint64_t kst[3] = {(uint64_t)p->k_row_stride * 2, 128, (uint64_t)p->k_page_stride * 2};
-    const uint32_t kbox[4] = {64, 8, D / 64, 1};
-    const uint64_t krdims[4] = {64, (uint64_t)p->page_size, 1, (uint64_t)p->num_pages};
-    const uint64_t krst[3] = {(uint64_t)p->kr_row_stride * 2, 128, (uint64_t)p->kr_page_stride * 2};
-    const uint32_t krbox[4] = {64, 8, 1, 1};
-    if (!make_tmap_16b(&maps.q, p->query, kBf16, 5, dims, st, box) ||
-        !make_tmap_16b(&maps.qr, p->query_rope, kBf16, 5, rdims, rst, rbox) ||
-        !make_tmap_16b(&maps.k, p->key_cache, kBf16, 4, kdims, kst, kbox) ||
-        !make_tmap_16b(&maps.kr, p->key_rope_cache, kBf16, 4, krdims, krst, krbox))
-      return DSA_ERR_TMA_DESCRIPTOR;
-  }
+// What both kernels take; `nh` heads a work item, `shares` of the work.
+Args make_args(const DsaAttnPagedParams* p, int nh, int shares) {
   Args a;
   a.act_q = p->act_q;
   a.act_k = p->act_k;
@@ -849,10 +678,10 @@ int launch(const DsaAttnPagedParams* p, cudaStream_t stream) {
   a.softmax_max = p->softmax_max;
   a.softmax_sum = p->softmax_sum;
   a.error_flag = p->error_flag;
-  a.rows = (int)(b * s1);
-  a.s1 = (int)s1;
-  a.n1 = (int)n1;
-  a.groups = (int)((n1 + NH - 1) / NH);
+  a.rows = (int)(p->batch * p->s1);
+  a.s1 = (int)p->s1;
+  a.n1 = (int)p->n1;
+  a.groups = 1;
   a.page_size = (int)p->page_size;
   a.max_blocks = (int)p->max_blocks;
   a.num_pages = (int)p->num_pages;
@@ -860,28 +689,93 @@ int launch(const DsaAttnPagedParams* p, cudaStream_t stream) {
   a.scale = p->scale;
   uint8_t* ws = static_cast<uint8_t*>(p->workspace);
   a.ws_o = reinterpret_cast<float*>(ws);
-  ws += (int64_t)2 * grid * NH * D * 4;
+  ws += (int64_t)2 * shares * nh * p->d * 4;
   a.ws_s = reinterpret_cast<float4*>(ws);
-  ws += (int64_t)2 * grid * NH * 16;
+  ws += (int64_t)2 * shares * nh * 16;
   a.ws_prefix = reinterpret_cast<int32_t*>(ws);
+  return a;
+}
 
-  auto kern = attn_paged_kernel<D, NH, T>;
-  static std::atomic<uint64_t> ready;   // devices on which the kernel may use its shared memory
-  if (!allow_smem(reinterpret_cast<const void*>(kern), C::kSmem, &ready)) return DSA_ERR_CUDA;
-  kern<<<grid, kThreads, C::kSmem, stream>>>(maps, a);
-  if (cudaGetLastError() != cudaSuccess) return DSA_ERR_CUDA;
+// Tensor maps of the queries (boxes of `nh` heads) and keys (boxes of 8).
+template <int D>
+bool make_maps(Maps* maps, const DsaAttnPagedParams* p, bool bf16, uint32_t nh) {
+  const uint64_t n1 = p->n1, s1 = p->s1, b = p->batch, page = p->page_size, pages = p->num_pages;
+  const uint64_t dims[5] = {64, n1, D / 64, s1, b};
+  const uint64_t st[4] = {(uint64_t)p->q_head_stride * 2, 128, (uint64_t)p->q_token_stride * 2,
+                          (uint64_t)p->q_batch_stride * 2};
+  const uint32_t box[5] = {64, nh, D / 64, 1, 1};
+  const uint64_t rdims[5] = {64, n1, 1, s1, b};
+  const uint64_t rst[4] = {(uint64_t)p->qr_head_stride * 2, 128, (uint64_t)p->qr_token_stride * 2,
+                           (uint64_t)p->qr_batch_stride * 2};
+  const uint32_t rbox[5] = {64, nh, 1, 1, 1};
+  const uint64_t kdims[4] = {64, page, D / 64, pages};
+  const uint64_t kst[3] = {(uint64_t)p->k_row_stride * 2, 128, (uint64_t)p->k_page_stride * 2};
+  const uint32_t kbox[4] = {64, 8, D / 64, 1};
+  const uint64_t krdims[4] = {64, page, 1, pages};
+  const uint64_t krst[3] = {(uint64_t)p->kr_row_stride * 2, 128, (uint64_t)p->kr_page_stride * 2};
+  const uint32_t krbox[4] = {64, 8, 1, 1};
+  return make_tmap_16b(&maps->q, p->query, bf16, 5, dims, st, box) &&
+         make_tmap_16b(&maps->qr, p->query_rope, bf16, 5, rdims, rst, rbox) &&
+         make_tmap_16b(&maps->k, p->key_cache, bf16, 4, kdims, kst, kbox) &&
+         make_tmap_16b(&maps->kr, p->key_rope_cache, bf16, 4, krdims, krst, krbox);
+}
+
+template <int D, int NH, typename T>
+int launch_join(const DsaAttnPagedParams* p, const Args& a, int shares, cudaStream_t stream) {
   cudaLaunchAttribute pdl[1];
   pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   pdl[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(b * s1 * n1));
+  cfg.gridDim = dim3((unsigned)(p->batch * p->s1 * p->n1));
   cfg.blockDim = dim3(kJoinThreads);
   cfg.stream = stream;
   cfg.attrs = pdl;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, attn_paged_combine_kernel<D, NH, T>, a, grid) != cudaSuccess)
+  return cudaLaunchKernelEx(&cfg, attn_paged_combine_kernel<D, NH, T>, a, shares) == cudaSuccess
+             ? DSA_OK
+             : DSA_ERR_CUDA;
+}
+
+template <int D, int NH, typename T>
+int launch(const DsaAttnPagedParams* p, cudaStream_t stream) {
+  using C = Cfg<D, NH>;
+  const int grid = sm_count();
+  if (grid < 1) return DSA_ERR_CUDA;
+  Maps maps;
+  if (!make_maps<D>(&maps, p, ElemTraits<T>::kIsBf16, NH)) return DSA_ERR_TMA_DESCRIPTOR;
+  Args a = make_args(p, NH, grid);
+  a.groups = (int)((p->n1 + NH - 1) / NH);
+  auto kern = attn_paged_kernel<D, NH, T>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) !=
+      cudaSuccess)
     return DSA_ERR_CUDA;
-  return DSA_OK;
+  kern<<<grid, kThreads, C::kSmem, stream>>>(maps, a);
+  if (cudaGetLastError() != cudaSuccess) return DSA_ERR_CUDA;
+  return launch_join<D, NH, T>(p, a, grid, stream);
+}
+
+template <int D, typename T>
+int launch_pair(const DsaAttnPagedParams* p, cudaStream_t stream) {
+  using C = pair::Cfg<D>;
+  constexpr bool kBf16 = ElemTraits<T>::kIsBf16;
+  const int pairs = sm_count() / 2;
+  if (pairs < 1) return DSA_ERR_CUDA;
+  Maps maps;
+  CUtensorMap map_v;
+  const uint64_t dims[4] = {64, (uint64_t)p->page_size, D / 64, (uint64_t)p->num_pages};
+  const uint64_t st[3] = {(uint64_t)p->k_row_stride * 2, 128, (uint64_t)p->k_page_stride * 2};
+  const uint32_t box[4] = {64, 8, C::kVChunks, 1};
+  if (!make_maps<D>(&maps, p, kBf16, pair::kHeads) ||
+      !make_tmap_16b(&map_v, p->key_cache, kBf16, 4, dims, st, box))
+    return DSA_ERR_TMA_DESCRIPTOR;
+  const Args a = make_args(p, 2 * pair::kHeads, pairs);
+  auto kern = pair::attn_paged_pair_kernel<D, T>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) !=
+      cudaSuccess)
+    return DSA_ERR_CUDA;
+  kern<<<2 * pairs, pair::kThreads, C::kSmem, stream>>>(maps, map_v, a);
+  if (cudaGetLastError() != cudaSuccess) return DSA_ERR_CUDA;
+  return launch_join<D, 2 * pair::kHeads, T>(p, a, pairs, stream);
 }
 
 template <int D, typename T>
@@ -889,7 +783,8 @@ int launch_heads(const DsaAttnPagedParams* p, cudaStream_t stream) {
   switch (heads_of(p->n1)) {
     case 16: return launch<D, 16, T>(p, stream);
     case 32: return launch<D, 32, T>(p, stream);
-    default: return launch<D, 64, T>(p, stream);
+    case 64: return launch<D, 64, T>(p, stream);
+    default: return launch_pair<D, T>(p, stream);
   }
 }
 
@@ -909,9 +804,10 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 extern "C" int64_t dsa_attn_paged_workspace_size(int64_t batch, int64_t s1, int64_t n1, int64_t d) {
   using namespace dsa::attn_paged;
   if (batch < 0 || s1 < 0 || n1 < 1 || n1 > 128 || d < 1) return -1;
-  const int64_t nh = heads_of(n1), grid = dsa::sm_count();
-  if (grid < 1) return -1;
-  return align256(2 * grid * nh * (d * 4 + 16) + (batch * s1 + 1) * 4);
+  const int64_t nh = heads_of(n1), sms = dsa::sm_count();
+  if (sms < 1) return -1;
+  const int64_t shares = nh == 128 ? sms / 2 : sms;
+  return align256(2 * shares * nh * (d * 4 + 16) + (batch * s1 + 1) * 4);
 }
 
 extern "C" int dsa_attn_paged(const DsaAttnPagedParams* p, void* stream_) {

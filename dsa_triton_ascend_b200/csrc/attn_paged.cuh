@@ -1,0 +1,177 @@
+// What the kernels of attn_paged.cu share: arguments, and the division of the work.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include "dsa_b200.h"
+#include "sm100.cuh"
+
+namespace dsa {
+namespace attn_paged {
+
+constexpr int kRope = 64;
+constexpr int kSmemLimit = 232448;
+constexpr int kAhead = 3;           // tiles that are brought into L2 before their load
+constexpr float kRescale = 8.0f;    // log2 units a score may pass the reference
+
+struct Maps {
+  CUtensorMap q, qr, k, kr;
+};
+
+struct Args {
+  const int32_t* act_q;
+  const int32_t* act_k;
+  const int32_t* block_table;
+  void* out;
+  float* softmax_max;
+  float* softmax_sum;
+  int* error_flag;
+  int32_t* ws_prefix;   // [rows + 1] first tile of each row
+  float* ws_o;          // [2 * CTAs][NH][D]
+  float4* ws_s;         // [2 * CTAs][NH]: reference and running maximum (log2 units), sum,
+                        // raw running maximum
+  int32_t rows, s1, n1, groups;
+  int32_t page_size, max_blocks, num_pages, mode;
+  float scale;
+};
+
+// Keys that query row `row` sees.
+__device__ __forceinline__ int row_keys(const Args& a, int row) {
+  const int b = row / a.s1, s = row - b * a.s1;
+  const int ak = a.act_k[b], aq = a.act_q ? a.act_q[b] : a.s1;
+  int64_t n = min((int64_t)ak, (int64_t)a.max_blocks * a.page_size);
+  if (a.mode == 3) n = min(n, (int64_t)ak - aq + s + 1);
+  if (s >= aq || n < 0) n = 0;
+  return (int)n;
+}
+template <int kTile>
+__device__ __forceinline__ int row_tiles(const Args& a, int row) {
+  return (row_keys(a, row) + kTile - 1) / kTile;
+}
+
+// CTAs (pairs of them in the pair kernel) that share `tiles` tiles; each takes kMinTiles at
+// least, as fewer cost more in joining than they save.
+constexpr int kMinTiles = 2;
+__device__ __forceinline__ int64_t ctas_used(int64_t tiles, int grid) {
+  const int64_t c = (tiles + kMinTiles - 1) / kMinTiles;
+  return c < 1 ? 1 : c < grid ? c : grid;
+}
+
+// Exclusive prefix of v over the block (kThreads threads) and its total.
+template <int kThreads>
+__device__ __forceinline__ int block_scan(int v, int* tmp, int* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();
+  if (lane == 31) tmp[warp] = x;
+  __syncthreads();
+  int before = 0, sum = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before += tmp[w];
+    sum += tmp[w];
+  }
+  *total = sum;
+  return before + x - v;
+}
+
+// One CTA's share: tiles from (row, head group, tile) on, `left` of them.
+struct Work {
+  int row, group, tile, left;
+};
+// A run of tiles of one (row, head group).
+struct Segment {
+  int row, group, first, count, keys, tiles;
+};
+// The next run of `w` (false when the share is done); `w` moves past it.
+template <int kTile>
+__device__ __forceinline__ bool next_segment(const Args& a, Work& w, Segment& s) {
+  while (w.left > 0 && w.row < a.rows) {
+    s.keys = row_keys(a, w.row);
+    s.tiles = (s.keys + kTile - 1) / kTile;
+    if (s.tiles == 0) {
+      ++w.row;
+      continue;
+    }
+    s.row = w.row;
+    s.group = w.group;
+    s.first = w.tile;
+    s.count = min(s.tiles - w.tile, w.left);
+    w.left -= s.count;
+    w.tile = 0;
+    if (++w.group == a.groups) {
+      w.group = 0;
+      ++w.row;
+    }
+    return true;
+  }
+  return false;
+}
+
+// The share of CTA (or pair) `cta` of `ctas_max`: equal numbers of tiles, whatever rows they
+// are of.  All threads of the block call it; the place where the share begins is left in
+// `start` (shared memory), to be read after a barrier (take_start).  The first CTA also writes
+// the rows' prefix for the join.
+template <int kTile, int kThreads>
+__device__ __forceinline__ Work share_of(const Args& a, int cta, int ctas_max, bool first_cta, int* tmp,
+                                         int32_t* start) {
+  int64_t total = 0;
+  int mine = 0, before = 0;   // the tiles of the thread's last row and of the rows before it
+  for (int r0 = 0; r0 < a.rows; r0 += kThreads) {
+    const int r = r0 + threadIdx.x;
+    int sum;
+    mine = r < a.rows ? row_tiles<kTile>(a, r) : 0;
+    before = block_scan<kThreads>(mine, tmp, &sum);
+    if (first_cta && r < a.rows) a.ws_prefix[r] = (int)total + before;
+    total += sum;
+  }
+  if (first_cta && threadIdx.x == 0) a.ws_prefix[a.rows] = (int)total;
+  const int64_t tiles = total * a.groups;
+  const int64_t ctas = ctas_used(tiles, ctas_max);
+  Work work{0, 0, 0, 0};
+  int64_t from = 0;
+  if (cta < ctas) {
+    from = tiles * cta / ctas;
+    work.left = (int)(tiles * (cta + 1) / ctas - from);
+    int64_t seen = 0;
+    for (int r0 = 0; r0 < a.rows; r0 += kThreads) {
+      const int r = r0 + threadIdx.x;
+      int sum = (int)total;
+      if (a.rows > kThreads) {
+        mine = r < a.rows ? row_tiles<kTile>(a, r) : 0;
+        before = block_scan<kThreads>(mine, tmp, &sum);
+      }
+      const int64_t first = (seen + before) * a.groups;
+      if (mine > 0 && first <= from && from < first + (int64_t)mine * a.groups) {
+        const int in = (int)(from - first);
+        start[0] = r;
+        start[1] = in / mine;
+        start[2] = in - (in / mine) * mine;
+      }
+      seen += sum;
+      if (seen * a.groups > from) break;   // the same for every thread
+    }
+  }
+  return work;
+}
+__device__ __forceinline__ void take_start(Work& work, const int32_t* start) {
+  if (work.left <= 0) return;
+  work.row = start[0];
+  work.group = start[1];
+  work.tile = start[2];
+}
+
+// 2^x, 2^-126 and below flushed to 0
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+}  // namespace attn_paged
+}  // namespace dsa

@@ -1,0 +1,540 @@
+// Attention over the paged cache for more than 64 heads: a pair of CTAs per row.
+//
+// The product of 128 heads x 512 dims fills the tensor memory of one SM, so a pair shares it
+// (cta_group::2, M = 128: 64 heads in each CTA), as it shares the operands:
+//   S [128 heads x 128 keys] = Q K^T: each CTA holds its 64 heads' queries and 64 of the keys
+//   O [128 heads x D]       += P V:   each CTA holds its 64 heads' P and D / 2 of the dims of
+//                                     all 128 keys
+// so a CTA loads its keys whole (K-major) and its half of every key's value part (MN-major): the
+// pool is read once from HBM, 1.9 times from L2.  Against two CTAs that each take 64 heads and
+// all keys (the other kernel, twice) the tensor core's operand reads from shared memory fall
+// from 555 KB to 260 KB per 128 keys and CTA, which is what bounded that form.
+//
+// A tile of 128 keys and the queries leave room for one buffer each of K and V at D = 512.
+// That is enough: K(t + 1) arrives during softmax(t) and PV(t), V(t + 1) during QK(t + 1).
+#pragma once
+
+#include "attn_paged.cuh"
+#include "sm100.cuh"
+
+namespace dsa {
+namespace attn_paged {
+namespace pair {
+
+constexpr int kTile = 128;
+constexpr int kHeads = 64;          // of a CTA
+constexpr int kSoftmaxThreads = 256;
+constexpr int kKeyWarp = 8;         // warps 8-11 load K
+constexpr int kValueWarp = 12;      // warps 12, 13 load V
+constexpr int kMmaWarp = 14;
+constexpr int kQueryWarp = 15;
+constexpr int kThreads = 512;
+constexpr int kMaxStages = 4;
+
+template <int D>
+struct Cfg {
+  static constexpr int kChunks = D / 64;
+  static constexpr int kGroupBytes = kChunks * 1024;           // 8 keys of K: [chunk][8][128 B]
+  static constexpr int kKeyBytes = 8 * kGroupBytes;            // this CTA's 64 keys
+  static constexpr int kRopeBytes = 64 * 128;
+  static constexpr int kKBytes = kKeyBytes + kRopeBytes;
+  static constexpr int kVChunks = D / 128;                     // this CTA's dims
+  static constexpr int kVGroupBytes = kVChunks * 1024;
+  static constexpr int kVBytes = 16 * kVGroupBytes;            // 128 keys
+  static constexpr int kQBytes = kHeads * (D + kRope) * 2;
+  static constexpr int kPBytes = kHeads * kTile * 2;
+  static constexpr int kSmallBytes = 2 * 4 * kHeads * 4 + 640;
+  static constexpr int kRoom = (kSmemLimit - kQBytes - kPBytes - kSmallBytes) / (kKBytes + kVBytes);
+  static constexpr int kStages = kRoom < kMaxStages ? kRoom : kMaxStages;   // of K and of V
+  static constexpr int kQBufs =
+      kStages * (kKBytes + kVBytes) + 2 * kQBytes + kPBytes + kSmallBytes <= kSmemLimit ? 2 : 1;
+  static constexpr int kOffK = kQBufs * kQBytes;
+  static constexpr int kOffV = kOffK + kStages * kKBytes;
+  static constexpr int kOffP = kOffV + kStages * kVBytes;
+  static constexpr int kOffSmall = kOffP + kPBytes;
+  static constexpr int kSmem = kOffSmall + kSmallBytes;
+  static constexpr int kPvN = D < 256 ? D : 256;               // dims of one PV instruction
+  static constexpr int kPvs = D / kPvN;
+  static constexpr uint32_t kColsO = 128;                      // after two buffers of S
+  static constexpr uint32_t kTmem = D == 512 ? 512 : 256;
+  static_assert(kStages >= 1 && kOffK % 1024 == 0 && kOffV % 1024 == 0 && kOffP % 1024 == 0, "layout");
+};
+
+// The tiles of a share one by one.
+struct Tiles {
+  Work w;
+  Segment s;
+  int i, seg;
+  __device__ __forceinline__ bool next(const Args& a) {
+    if (seg >= 0 && i + 1 < s.count) {
+      ++i;
+      return true;
+    }
+    i = 0;
+    ++seg;
+    return next_segment<kTile>(a, w, s);
+  }
+};
+
+template <int D, typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    attn_paged_pair_kernel(const __grid_constant__ Maps maps, const __grid_constant__ CUtensorMap map_v,
+                           const Args a) {
+  using C = Cfg<D>;
+  using E = ElemTraits<T>;
+  constexpr bool kBf16 = E::kIsBf16;
+  constexpr float kShift = kBf16 ? 0.0f : 6.0f;   // half's probabilities are held 2^6 higher
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t base = smem_u32(smem);
+  float* wmax = reinterpret_cast<float*>(smem + C::kOffSmall);   // [4][kHeads]
+  float* wsum = wmax + 4 * kHeads;                               // [4][kHeads]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(wsum + 4 * kHeads);
+  int32_t* tmp = reinterpret_cast<int32_t*>(bars + 48);          // [16]
+  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(tmp + 16);
+  int32_t* start = reinterpret_cast<int32_t*>(tmem_ptr + 1);     // [3]
+
+  const uint32_t b0 = smem_u32(bars);
+  auto k_full = [&](int s) { return b0 + 8u * s; };                      // leader's
+  auto k_empty = [&](int s) { return b0 + 8u * (kMaxStages + s); };
+  auto v_full = [&](int s) { return b0 + 8u * (2 * kMaxStages + s); };   // leader's
+  auto v_empty = [&](int s) { return b0 + 8u * (3 * kMaxStages + s); };
+  auto s_full = [&](int s) { return b0 + 8u * (4 * kMaxStages + s); };
+  auto q_full = [&](int s) { return b0 + 8u * (4 * kMaxStages + 2 + s); };   // leader's
+  auto q_empty = [&](int s) { return b0 + 8u * (4 * kMaxStages + 4 + s); };
+  const uint32_t p_full = b0 + 8u * (4 * kMaxStages + 6);      // leader's
+  const uint32_t p_empty = b0 + 8u * (4 * kMaxStages + 7);
+  const uint32_t o_empty = b0 + 8u * (4 * kMaxStages + 8);     // leader's
+  const uint32_t drained = b0 + 8u * (4 * kMaxStages + 9);
+  auto v_tail = [&](int s) { return b0 + 8u * (4 * kMaxStages + 10 + s); };
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (base & 1023u) {   // the same in both CTAs
+    if (threadIdx.x == 0) report_error(a.error_flag, kErrMisaligned);
+    return;
+  }
+  const uint32_t rank = cluster_ctarank();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(k_full(s), 4);
+      mbar_init(k_empty(s), 1);
+      mbar_init(v_full(s), 2);
+      mbar_init(v_empty(s), 1);
+      mbar_init(v_tail(s), 2);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(s_full(s), 1);
+      mbar_init(q_full(s), 1);
+      mbar_init(q_empty(s), 1);
+    }
+    mbar_init(p_full, 16);
+    mbar_init(p_empty, 1);
+    mbar_init(o_empty, 16);
+    mbar_init(drained, 1);
+    fence_mbarrier_init();
+  }
+  if (warp == kMmaWarp) tmem_alloc<2>(smem_u32(tmem_ptr), C::kTmem);
+  Work work = share_of<kTile, kThreads>(a, blockIdx.x >> 1, gridDim.x >> 1, blockIdx.x == 0, tmp, start);
+  griddep_launch_dependents();
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_ptr;
+  take_start(work, start);
+  bool failed = false;
+
+  // Lane l < 16 looks up the page of keys 8 l .. 8 l + 7 of a tile, lanes 16 .. 31 that of the
+  // tile kAhead further on.  -1: no such page.  (Every role that has to know which keys are
+  // there looks for itself, one tile ahead, so that nobody waits for a message.)
+  auto page_of = [&](const Segment& sg, const int32_t* table, int tile, bool tell) {
+    const int t = tile + (lane < 16 ? 0 : kAhead), pos = t * kTile + (lane & 15) * 8;
+    if (pos >= sg.keys || t >= sg.first + sg.count) return -1;
+    const int id = table[pos / a.page_size];
+    if (tell && lane < 16 && id >= a.num_pages) report_error(a.error_flag, kErrBadIndex);
+    return id < a.num_pages ? id : -1;
+  };
+  auto table_of = [&](const Segment& sg) { return a.block_table + (int64_t)(sg.row / a.s1) * a.max_blocks; };
+
+  if (warp >= kKeyWarp && warp < kValueWarp) {
+    // -------------------------------------------------------------------- K
+    // This warp loads groups 2 w and 2 w + 1 (of 8 keys) of this CTA's 64 keys of every tile.
+    // The leader's barrier counts the bytes of both CTAs.
+    const int w = warp - kKeyWarp, g0 = 8 * (int)rank + 2 * w;
+    const bool mine = ((lane & 15) >> 1) == (g0 >> 1);
+    Tiles t{work, {}, 0, -1};
+    int g = 0, page = -1;
+    for (; t.next(a); ++g) {
+      const int32_t* table = table_of(t.s);
+      const int tile = t.s.first + t.i, st = g % C::kStages;
+      const int now = t.i == 0 ? page_of(t.s, table, tile, rank == 0 && w == 0) : page;
+      if (t.i + 1 < t.s.count) page = page_of(t.s, table, tile + 1, rank == 0 && w == 0);
+      if (g >= C::kStages) mbar_wait(k_empty(st), (g / C::kStages - 1) & 1, a.error_flag, &failed);
+      failed = __any_sync(0xffffffffu, failed);
+      if (failed) break;
+      const uint32_t mask = __ballot_sync(0xffffffffu, now >= 0);
+      if (rank == 0 && lane == 0) {
+        const uint32_t bytes = __popc(mask & (3u << (2 * w) | 3u << (8 + 2 * w))) * (C::kGroupBytes + 1024);
+        if (bytes) mbar_arrive_expect_tx(k_full(st), bytes);
+        else mbar_arrive(k_full(st));
+      }
+      __syncwarp();
+      const int in_page = ((tile + (lane < 16 ? 0 : kAhead)) * kTile + (lane & 15) * 8) % a.page_size;
+      const uint32_t dst = base + C::kOffK + st * C::kKBytes;
+      const int grp = (lane & 15) - 8 * (int)rank;
+      if (mine && now >= 0 && lane < 16) {
+        const uint32_t bar = mapa_shared(k_full(st), 0);
+        tma_load_4d_pair(dst + grp * C::kGroupBytes, &maps.k, bar, 0, in_page, 0, now);
+        tma_load_4d_pair(dst + C::kKeyBytes + grp * 1024, &maps.kr, bar, 0, in_page, 0, now);
+      } else if (mine && now >= 0) {
+        tma_prefetch_4d(&maps.k, 0, in_page, 0, now);
+        tma_prefetch_4d(&maps.kr, 0, in_page, 0, now);
+      }
+      __syncwarp();
+    }
+    if (failed && rank == 0) {   // the copies in flight, of both CTAs, land before the pair ends
+      bool gave_up = false;
+      for (int u = max(0, g - C::kStages); u < g; ++u)
+        mbar_wait(k_full(u % C::kStages), (u / C::kStages) & 1, a.error_flag, &gave_up, true);
+    }
+    __syncwarp();
+  } else if (warp >= kValueWarp && warp < kMmaWarp) {
+    // -------------------------------------------------------------------- V
+    // This warp loads 8 of the tile's 16 groups, this CTA's dims of them.  A tile with keys that
+    // are not there completes on a barrier of the CTA's own, since its softmax warps clear those
+    // rows before the product; their P then tells the leader.
+    const int w = warp - kValueWarp;
+    Tiles t{work, {}, 0, -1};
+    int g = 0, page = -1;
+    for (; t.next(a); ++g) {
+      const int32_t* table = table_of(t.s);
+      const int tile = t.s.first + t.i, st = g % C::kStages;
+      const int now = t.i == 0 ? page_of(t.s, table, tile, false) : page;
+      if (t.i + 1 < t.s.count) page = page_of(t.s, table, tile + 1, false);
+      if (g >= C::kStages) mbar_wait(v_empty(st), (g / C::kStages - 1) & 1, a.error_flag, &failed);
+      failed = __any_sync(0xffffffffu, failed);
+      if (failed) break;
+      const uint32_t mask = __ballot_sync(0xffffffffu, now >= 0) & 0xffffu;
+      const bool tail = mask != 0xffffu || t.s.keys - tile * kTile < kTile;
+      if (lane == 0) {
+        const uint32_t bytes = __popc(mask & (0xffu << (8 * w))) * C::kVGroupBytes;
+        if (tail) {
+          if (bytes) mbar_arrive_expect_tx(v_tail(st), bytes);
+          else mbar_arrive(v_tail(st));
+        }
+        if (rank == 0) {
+          if (tail) mbar_arrive(v_full(st));
+          else mbar_arrive_expect_tx(v_full(st), 2 * bytes);
+        }
+      }
+      __syncwarp();
+      if (now >= 0 && lane < 16 && (lane >> 3) == w) {
+        const int in_page = (tile * kTile + lane * 8) % a.page_size;
+        const uint32_t dst = base + C::kOffV + st * C::kVBytes + lane * C::kVGroupBytes;
+        if (tail)
+          tma_load_4d(dst, &map_v, v_tail(st), 0, in_page, C::kVChunks * (int)rank, now);
+        else
+          tma_load_4d_pair(dst, &map_v, mapa_shared(v_full(st), 0), 0, in_page, C::kVChunks * (int)rank, now);
+      }
+      __syncwarp();
+    }
+    if (failed) {
+      bool gave_up = false;
+      if (rank == 0)
+        for (int u = max(0, g - C::kStages); u < g; ++u)
+          mbar_wait(v_full(u % C::kStages), (u / C::kStages) & 1, a.error_flag, &gave_up, true);
+    }
+    __syncwarp();
+  } else if (warp == kQueryWarp) {
+    // -------------------------------------------------------------------- queries
+    Work w = work;
+    Segment sg;
+    int nseg = 0;
+    while (next_segment<kTile>(a, w, sg)) {
+      const int b = sg.row / a.s1, s = sg.row - b * a.s1;
+      const int buf = nseg % C::kQBufs, use = nseg / C::kQBufs;
+      if (use > 0) mbar_wait(q_empty(buf), (use - 1) & 1, a.error_flag, &failed);
+      failed = __any_sync(0xffffffffu, failed);
+      if (failed) break;
+      if (lane == 0) {
+        const uint32_t dst = base + buf * C::kQBytes, bar = mapa_shared(q_full(buf), 0);
+        if (rank == 0) mbar_arrive_expect_tx(q_full(buf), 2 * C::kQBytes);
+        tma_load_5d_pair(dst, &maps.q, bar, 0, kHeads * (int)rank, 0, s, b);
+        tma_load_5d_pair(dst + kHeads * D * 2, &maps.qr, bar, 0, kHeads * (int)rank, 0, s, b);
+      }
+      __syncwarp();
+      ++nseg;
+    }
+    if (failed && rank == 0) {
+      bool gave_up = false;
+      for (int u = max(0, nseg - C::kQBufs); u < nseg; ++u)
+        mbar_wait(q_full(u % C::kQBufs), (u / C::kQBufs) & 1, a.error_flag, &gave_up, true);
+    }
+    __syncwarp();
+  } else if (warp == kMmaWarp) {
+    // -------------------------------------------------------------------- MMA (leader)
+    if (rank == 0) {
+      constexpr uint32_t kIdQk = idesc_f16(128, kTile, kBf16, false, false);
+      constexpr uint32_t kIdPv = idesc_f16(128, C::kPvN, kBf16, false, true);
+      // Whichever product has its operands goes next: QK(a) at most two tiles ahead of PV, as
+      // there are two buffers of scores and PV(a - 2) waited for the probabilities made of S(a - 2).
+      Tiles q{work, {}, 0, -1}, v{work, {}, 0, -1};
+      bool more_q = q.next(a), more_v = v.next(a);
+      int na = 0, nb = 0;
+      uint64_t t0 = 0;
+      auto all = [](bool x) { return __all_sync(0xffffffffu, x) != 0; };
+      for (uint32_t idle = 0; more_v && !failed;) {
+        const int sa = na % C::kStages, sb = nb % C::kStages;
+        const int buf = q.seg % C::kQBufs;
+        if (more_q && na - nb < 2 &&
+            all((q.i > 0 || mbar_test_wait_cluster(q_full(buf), (q.seg / C::kQBufs) & 1)) &&
+                mbar_test_wait_cluster(k_full(sa), (na / C::kStages) & 1))) {
+          tc_fence_after();
+          if (elect_one()) {
+            const uint64_t qa = smem_desc_sw128(base + buf * C::kQBytes, 16, 1024);
+            const uint32_t ks = base + C::kOffK + sa * C::kKBytes;
+            const uint64_t kb = smem_desc_sw128(ks, 16, C::kGroupBytes);
+            const uint64_t rb = smem_desc_sw128(ks + C::kKeyBytes, 16, 1024);
+            const uint32_t d = tmem + 64 * (na & 1);
+#pragma unroll
+            for (int c = 0; c < C::kChunks; ++c)
+#pragma unroll
+              for (int u = 0; u < 4; ++u)
+                umma_f16<2>(d, qa + ((c * kHeads * 128 + u * 32) >> 4), kb + ((c * 1024 + u * 32) >> 4),
+                            kIdQk, c + u > 0);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              umma_f16<2>(d, qa + ((C::kChunks * kHeads * 128 + u * 32) >> 4), rb + ((u * 32) >> 4), kIdQk, 1);
+            umma_commit_pair(s_full(na & 1), 3);
+            umma_commit_pair(k_empty(sa), 3);
+            if (q.i == q.s.count - 1) umma_commit_pair(q_empty(buf), 3);
+          }
+          __syncwarp();
+          more_q = q.next(a);
+          ++na;
+          idle = 0;
+          continue;
+        }
+        if (nb < na && all(mbar_test_wait_cluster(p_full, nb & 1) &&
+                           mbar_test_wait_cluster(v_full(sb), (nb / C::kStages) & 1) &&
+                           (v.i > 0 || v.seg == 0 || mbar_test_wait_cluster(o_empty, (v.seg - 1) & 1)))) {
+          tc_fence_after();
+          if (elect_one()) {
+            const uint64_t pa = smem_desc_sw128(base + C::kOffP, 16, 1024);
+            const uint64_t vb = smem_desc_sw128(base + C::kOffV + sb * C::kVBytes, 1024, C::kVGroupBytes);
+#pragma unroll
+            for (int k = 0; k < kTile / 16; ++k)
+#pragma unroll
+              for (int n = 0; n < C::kPvs; ++n)
+                umma_f16<2>(tmem + C::kColsO + n * (C::kPvN / 2),
+                            pa + (((k >> 2) * kHeads * 128 + (k & 3) * 32) >> 4),
+                            vb + ((k * 2 * C::kVGroupBytes + n * 2048) >> 4), kIdPv, !(v.i == 0 && k == 0));
+            umma_commit_pair(v_empty(sb), 3);
+            umma_commit_pair(p_empty, 3);
+          }
+          __syncwarp();
+          more_v = v.next(a);
+          ++nb;
+          idle = 0;
+          continue;
+        }
+        if ((++idle & 1023u) == 0) {   // nothing for long: a bounded wait
+          const uint64_t now = globaltimer();
+          if (idle == 1024u) t0 = now;
+          else if (now - t0 > kWaitLimitNs) failed = true;
+          failed = __any_sync(0xffffffffu, failed);
+          if (failed && lane == 0) report_error(a.error_flag, kErrTimeout);
+        }
+      }
+      if (failed) {   // the products in flight end before the tensor memory is given back
+        bool gave_up = false;
+        if (elect_one()) umma_commit_pair(drained, 1);
+        __syncwarp();
+        mbar_wait(drained, 0, a.error_flag, &gave_up);
+      }
+    }
+    __syncwarp();
+  } else {
+    // -------------------------------------------------------------------- softmax
+    // Lanes 0-63 of the tensor memory hold this CTA's heads with the first half of the columns
+    // (keys, or dims of O), lanes 64-127 the same heads with the second half; warpgroup wg
+    // takes the wg-th half of those columns.  So four threads share a head.  No wait's failure is
+    // a way out of this loop: the warps meet at their barrier as often as there are tiles.
+    const int wg = warp >> 2, q = warp & 3, half = q >> 1;
+    const int h = 32 * (q & 1) + lane, part = 2 * half + wg;
+    const uint32_t lane_addr = (uint32_t)(32 * q) << 16;
+    const bool flip = a.scale < 0.0f;   // a negative scale turns the raw scores over
+    const float c2 = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-38f);
+    const uint32_t lead_p = mapa_shared(p_full, 0), lead_o = mapa_shared(o_empty, 0);
+    uint8_t* prow = smem + C::kOffP + half * (kHeads * 128) + h * 128;
+    constexpr int kDims = D / 4;   // of O, of one thread
+    Work w = work;
+    Segment sg;
+    int g = 0, nseg = 0;
+    uint32_t tails = 0;   // parity of each stage's tiles with keys that are not there
+    while (next_segment<kTile>(a, w, sg)) {
+      const int32_t* table = table_of(sg);
+      float ref = -INFINITY, lim = -INFINITY, run = -INFINITY, sum = 0.0f;
+      int page = page_of(sg, table, sg.first, false);
+      for (int i = 0; i < sg.count; ++i, ++g) {
+        const int tile = sg.first + i, st = g % C::kStages;
+        const uint32_t mask = __ballot_sync(0xffffffffu, page >= 0) & 0xffffu;
+        if (i + 1 < sg.count) page = page_of(sg, table, tile + 1, false);
+        const int valid = sg.keys - tile * kTile;
+        const bool tail = mask != 0xffffu || valid < kTile;
+        mbar_wait_spin(s_full(g & 1), (g >> 1) & 1, a.error_flag, &failed);
+        tc_fence_after();
+        uint32_t r[32];
+        tmem_ld32(tmem + 64 * (g & 1) + 32 * wg + lane_addr, r);
+        tmem_ld_wait_regs(r);
+        tc_fence_before();
+        float z[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) z[j] = __uint_as_float(r[j]);
+        if (flip)
+#pragma unroll
+          for (int j = 0; j < 32; ++j) z[j] = -z[j];
+        if (tail) {
+          const int k0 = 64 * half + 32 * wg;
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (k0 + j >= valid || !(mask >> ((k0 + j) >> 3) & 1u)) z[j] = -INFINITY;
+        }
+        float top = z[0];
+#pragma unroll
+        for (int j = 1; j < 32; ++j) top = fmaxf(top, z[j]);
+        run = fmaxf(run, top);
+        // the reference moves at the first tile, and when a score passes it by 2^8
+        if (named_bar_or(1, kSoftmaxThreads, i == 0 || top > lim)) {
+          wmax[part * kHeads + h] = run;
+          asm volatile("bar.sync 1, %0;" ::"n"(kSoftmaxThreads) : "memory");
+          const float m = fmaxf(fmaxf(wmax[h], wmax[kHeads + h]), fmaxf(wmax[2 * kHeads + h], wmax[3 * kHeads + h]));
+          const float now = m == -INFINITY ? -INFINITY : m * c2;
+          const float f = ref == now ? 1.0f : exp2f(ref - now);
+          sum *= f;
+          ref = now;
+          lim = (now + kRescale) / c2;
+          if (i > 0) {
+            mbar_wait_spin(p_empty, (g - 1) & 1, a.error_flag, &failed);
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < kDims; c += 16) {
+              uint32_t o[16];
+              tmem_ld16(tmem + C::kColsO + wg * kDims + c + lane_addr, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+              tmem_st16(tmem + C::kColsO + wg * kDims + c + lane_addr, o);
+            }
+            tmem_st_wait();
+          }
+          asm volatile("bar.sync 1, %0;" ::"n"(kSoftmaxThreads) : "memory");   // the maxima are read
+        }
+        const bool p_free = g == 0 || mbar_test_wait(p_empty, (g - 1) & 1);
+        // probabilities; a head without any key so far has reference -inf and stays zero
+        const float off = ref == -INFINITY ? 0.0f : kShift - ref;
+        uint32_t pk[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float p0 = exp2_approx(fmaf(z[2 * j], c2, off));
+          const float p1 = exp2_approx(fmaf(z[2 * j + 1], c2, off));
+          sum += p0 + p1;
+          pk[j] = E::pack2(p0, p1);
+        }
+        if (!p_free) mbar_wait_spin(p_empty, (g - 1) & 1, a.error_flag, &failed);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          *reinterpret_cast<uint4*>(prow + (((4 * wg + j) ^ (h & 7)) << 4)) =
+              make_uint4(pk[4 * j], pk[4 * j + 1], pk[4 * j + 2], pk[4 * j + 3]);
+        if (tail) {
+          // rows of this tile that no key stands in hold what was there before (or a page's
+          // stale tail): cleared, so that 0 x NaN cannot enter the product
+          mbar_wait_spin(v_tail(st), tails >> st & 1, a.error_flag, &failed);
+          tails ^= 1u << st;
+          const int key = threadIdx.x >> 1;
+          if (key >= valid || !(mask >> (key >> 3) & 1u)) {
+            uint8_t* row = smem + C::kOffV + st * C::kVBytes + (key >> 3) * C::kVGroupBytes + (key & 7) * 128;
+            for (int c = threadIdx.x & 1; c < C::kVChunks; c += 2)
+#pragma unroll
+              for (int x = 0; x < 8; ++x)
+                *reinterpret_cast<uint4*>(row + c * 1024 + x * 16) = make_uint4(0, 0, 0, 0);
+          }
+        }
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (rank == 0) mbar_arrive(p_full);
+          else mbar_arrive_cluster(lead_p);
+        }
+      }
+
+      // ---- the segment's result ----
+      wsum[part * kHeads + h] = sum;
+      wmax[part * kHeads + h] = run;
+      asm volatile("bar.sync 1, %0;" ::"n"(kSoftmaxThreads) : "memory");
+      const float l = wsum[h] + wsum[kHeads + h] + wsum[2 * kHeads + h] + wsum[3 * kHeads + h];
+      const float m = fmaxf(fmaxf(wmax[h], wmax[kHeads + h]), fmaxf(wmax[2 * kHeads + h], wmax[3 * kHeads + h]));
+      const bool any = m != -INFINITY;
+      const float most = any ? m * c2 : -INFINITY;
+      const bool whole = sg.count == sg.tiles;
+      const int64_t slot = 2 * (blockIdx.x >> 1) + (nseg == 0 ? 0 : 1);
+      const int head = kHeads * (int)rank + h;
+      const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+      if (part == 0 && head < a.n1) {
+        if (!whole) {
+          a.ws_s[slot * (2 * kHeads) + head] = make_float4(ref - kShift, most, l, m);
+        } else if (a.softmax_max) {
+          const int64_t at = (int64_t)sg.row * a.n1 + head;
+          a.softmax_max[at] = any ? m * fabsf(a.scale) : 0.0f;
+          a.softmax_sum[at] = any ? l * exp2f(ref - kShift - most) : 0.0f;
+        }
+      }
+      mbar_wait_spin(p_empty, (g - 1) & 1, a.error_flag, &failed);
+      tc_fence_after();
+      const int dim = half * (D / 2) + wg * kDims;
+#pragma unroll 1
+      for (int c = 0; c < kDims; c += 32) {
+        uint32_t o[32];
+        tmem_ld32(tmem + C::kColsO + wg * kDims + c + lane_addr, o);
+        tmem_ld_wait_regs(o);
+        if (head >= a.n1) {
+          // a padded head: nothing to write
+        } else if (whole) {
+          uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + ((int64_t)sg.row * a.n1 + head) * D + dim + c);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            auto two = [&](int k) {
+              return E::pack2(__uint_as_float(o[8 * j + k]) * inv, __uint_as_float(o[8 * j + k + 1]) * inv);
+            };
+            out[j] = make_uint4(two(0), two(2), two(4), two(6));
+          }
+        } else {
+          uint4* out = reinterpret_cast<uint4*>(a.ws_o + (slot * (2 * kHeads) + head) * D + dim + c);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) out[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+        }
+        __syncwarp();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (rank == 0) mbar_arrive(o_empty);
+        else mbar_arrive_cluster(lead_o);
+      }
+      ++nseg;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  if (warp == kMmaWarp) {
+    tmem_relinquish<2>();
+    tmem_dealloc<2>(tmem, C::kTmem);
+  }
+}
+
+}  // namespace pair
+}  // namespace attn_paged
+}  // namespace dsa
