@@ -27,13 +27,15 @@ namespace dsa {
 namespace attn_paged {
 
 constexpr int kTile = 64;       // keys of a step
+constexpr int kSegmentCost = 2; // of starting an item, in tiles
 constexpr int kSoftmaxThreads = 128;   // of a warpgroup; there are two (warps 0-3, 4-7), each with
                                        // half of the heads
 constexpr int kLoadWarp = 8;           // warps 8-11: loads (one warp issues a box in 160 cycles,
                                        // so 16 boxes a tile from one warp took 2,600 of them)
-constexpr int kMmaWarp = 12;
-constexpr int kQueryWarp = 13;
-constexpr int kThreads = 448;
+constexpr int kQkWarp = 12;
+constexpr int kPvWarp = 13;
+constexpr int kQueryWarp = 14;
+constexpr int kThreads = 480;
 constexpr int kMaxStages = 8;
 
 template <int D, int NH>
@@ -149,7 +151,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto q_full = [&](int s) { return b0 + 8u * (2 * kMaxStages + 4 + s); };
   auto q_empty = [&](int s) { return b0 + 8u * (2 * kMaxStages + 6 + s); };
   const uint32_t o_empty = b0 + 8u * (2 * kMaxStages + 8);
-  const uint32_t drained = b0 + 8u * (2 * kMaxStages + 9);
+  auto s_empty = [&](int s) { return b0 + 8u * (2 * kMaxStages + 9 + s); };
+  auto drained = [&](int s) { return b0 + 8u * (2 * kMaxStages + 11 + s); };
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (base & 1023u) {
@@ -165,16 +168,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(s_full(s), 1);
       mbar_init(q_full(s), 1);
       mbar_init(q_empty(s), 1);
+      mbar_init(s_empty(s), 8);
+      mbar_init(drained(s), 1);
     }
     mbar_init(p_full, 8);
     mbar_init(p_empty, 1);
     mbar_init(o_empty, 8);
-    mbar_init(drained, 1);
     fence_mbarrier_init();
   }
-  if (warp == kMmaWarp) tmem_alloc<1>(smem_u32(tmem_ptr), C::kTmem);
+  if (warp == kQkWarp) tmem_alloc<1>(smem_u32(tmem_ptr), C::kTmem);
 
-  Work work = share_of<kTile, kThreads>(a, blockIdx.x, gridDim.x, blockIdx.x == 0, tmp, start);
+  Work work = share_of<kTile, kSegmentCost, kThreads>(a, blockIdx.x, gridDim.x, blockIdx.x == 0, tmp, start);
   griddep_launch_dependents();
   tc_fence_before();
   __syncthreads();
@@ -184,24 +188,24 @@ __global__ void __launch_bounds__(kThreads, 1)
   take_start(work, start);
   bool failed = false;
 
-  if (warp >= kLoadWarp && warp < kMmaWarp) {
+  if (warp >= kLoadWarp && warp < kQkWarp) {
     // -------------------------------------------------------------------- loads
     const int w = warp - kLoadWarp;
     // this warp loads groups 2 w and 2 w + 1 (of 8 keys) of every tile: lanes 0 and 1 their
-    // latent rows, lanes 2 and 3 the rotary ones; lanes 4 .. 7 bring the same of the tile kAhead
-    // further on into L2
-    const int grp = 2 * w + (lane & 1), ahead = lane < 4 ? 0 : kAhead;
+    // latent rows, lanes 2 and 3 the rotary ones.  (Bringing tiles into L2 ahead of their load
+    // gained 1.6 % at 64 rows of up to 16411 keys and lost 3 % at D = 256 with 64 heads.)
+    const int grp = 2 * w + (lane & 1);
     const bool is_rope = lane & 2;
     Segment sg;
     int g = 0;
-    while (!failed && next_segment<kTile>(a, work, sg)) {
+    while (!failed && next_segment<kTile, kSegmentCost>(a, work, sg)) {
       const int b = sg.row / a.s1;
       const int32_t* table = a.block_table + (int64_t)b * a.max_blocks;
       auto page_of = [&](int tile) {   // -1: no such page
-        const int pos = (tile + ahead) * kTile + grp * 8;
-        if (lane >= 8 || pos >= sg.keys || tile + ahead >= sg.first + sg.count) return -1;
+        const int pos = tile * kTile + grp * 8;
+        if (lane >= 4 || pos >= sg.keys) return -1;
         const int id = table[pos / a.page_size];
-        if (id >= a.num_pages && lane < 2) report_error(a.error_flag, kErrBadIndex);
+        if (id >= a.num_pages && !is_rope) report_error(a.error_flag, kErrBadIndex);
         return id < a.num_pages ? id : -1;
       };
       int page = page_of(sg.first);
@@ -221,13 +225,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           else mbar_arrive(full(st));
         }
         __syncwarp();
-        const int in_page = ((tile + ahead) * kTile + grp * 8) % a.page_size;
-        const CUtensorMap* map = is_rope ? &maps.kr : &maps.k;
-        if (now >= 0 && lane < 4)
-          tma_load_4d(dst + (is_rope ? C::kKeyBytes + grp * 1024 : grp * C::kGroupBytes), map, full(st), 0,
-                      in_page, 0, now);
-        else if (now >= 0)
-          tma_prefetch_4d(map, 0, in_page, 0, now);
+        if (now >= 0)
+          tma_load_4d(dst + (is_rope ? C::kKeyBytes + grp * 1024 : grp * C::kGroupBytes),
+                      is_rope ? &maps.kr : &maps.k, full(st), 0, (tile * kTile + grp * 8) % a.page_size, 0, now);
       }
     }
     if (failed) {   // the copies in flight land before the CTA ends
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // -------------------------------------------------------------------- queries
     Segment sg;
     int nseg = 0;
-    while (!failed && next_segment<kTile>(a, work, sg)) {
+    while (!failed && next_segment<kTile, kSegmentCost>(a, work, sg)) {
       const int b = sg.row / a.s1, s = sg.row - b * a.s1;
       const int buf = nseg % C::kQBufs, use = nseg / C::kQBufs;
       if (use > 0) mbar_wait(q_empty(buf), (use - 1) & 1, a.error_flag, &failed);
@@ -261,96 +261,79 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_wait(q_full(t % C::kQBufs), (t / C::kQBufs) & 1, a.error_flag, &gave_up);
       __syncwarp();
     }
-  } else if (warp == kMmaWarp) {
+  } else if (warp == kQkWarp || warp == kPvWarp) {
     // -------------------------------------------------------------------- MMA
-    constexpr uint32_t kIdQk = idesc_f16(64, NH, kBf16, false, false);
-    constexpr uint32_t kIdPv = idesc_f16(128, NH, kBf16, true, true);
-    // A look at a barrier takes some 100 cycles beside the tensor core's operand reads, so each
-    // is looked at once.  The buffer of scores needs no barrier of its own: QK(g) overwrites
-    // those of tile g - 2, which were read before the probabilities that PV(g - 2) waited for.
-    bool pv_due = false, pv_first = false;
-    int pv_tile = 0, pv_seg = 0;
-    auto all = [](bool v) { return __all_sync(0xffffffffu, v) != 0; };
-    auto issue_pv = [&](bool there) {
-      if (!there) mbar_wait_spin(p_full, pv_tile & 1, a.error_flag, &failed);
-      if (pv_first && pv_seg > 0)
-        mbar_wait_spin(o_empty, (pv_seg - 1) & 1, a.error_flag, &failed);
-      pv_due = false;
-      failed = !all(!failed);
-      if (failed) return;
-      tc_fence_after();
-      const int st = pv_tile % C::kStages;
-      if (elect_one()) {
-        const uint64_t va = smem_desc_sw128(base + st * C::kStageBytes, 1024, C::kGroupBytes);
-        const uint64_t pb = p_desc<NH>(s_p);
-#pragma unroll
-        for (int k = 0; k < kTile / 16; ++k)
-#pragma unroll
-          for (int m = 0; m < C::kBlocks; ++m)
-            umma_f16<1>(t_o + m * NH, va + ((k * 2 * C::kGroupBytes + m * 2048) >> 4),
-                        pb + ((k * 16 * NH * 2) >> 4), kIdPv, !(pv_first && k == 0));
-        umma_commit(empty(st));
-        umma_commit(p_empty);
-      }
-      __syncwarp();
-    };
+    // S and O are made by a warp each: an issuing warp is held up while the tensor core is busy,
+    // and a look at a barrier takes some 100 cycles beside the core's operand reads, so one warp
+    // for both left gaps between them.
     Segment sg;
     int g = 0, nseg = 0;
-    while (!failed && next_segment<kTile>(a, work, sg)) {
-      const int buf = nseg % C::kQBufs;
-      const uint32_t q_par = (nseg / C::kQBufs) & 1;
-      for (int i = 0; i < sg.count && !failed; ++i, ++g) {
-        const int st = g % C::kStages;
-        if (i == 0) {
-          if (pv_due && !all(mbar_test_wait(q_full(buf), q_par))) issue_pv(false);
-          mbar_wait_spin(q_full(buf), q_par, a.error_flag, &failed);
-        }
-        // while this tile's keys are on their way, the product of the tile before goes first if
-        // its probabilities are there
-        const uint32_t par = (g / C::kStages) & 1;
-        bool here = all(mbar_test_wait(full(st), par));
-        for (int spin = 0; !here && pv_due && spin < (1 << 20); ++spin) {
-          if (all(mbar_test_wait(p_full, pv_tile & 1))) issue_pv(true);
-          here = all(mbar_test_wait(full(st), par));
-        }
-        if (!here) mbar_wait_spin(full(st), par, a.error_flag, &failed);
-        failed = !all(!failed);
-        if (failed) break;
-        tc_fence_after();
-        if (elect_one()) {
-          const uint64_t ka = smem_desc_sw128(base + st * C::kStageBytes, 16, C::kGroupBytes);
-          const uint64_t ra =
-              smem_desc_sw128(base + st * C::kStageBytes + C::kKeyBytes, 16, 1024);
-          const uint64_t qb = smem_desc_sw128(s_q + buf * C::kQBytes, 16, 1024);
-          const uint32_t d = tmem + (g & 1) * NH;
+    if (warp == kQkWarp) {
+      constexpr uint32_t kIdQk = idesc_f16(64, NH, kBf16, false, false);
+      while (!failed && next_segment<kTile, kSegmentCost>(a, work, sg)) {
+        const int buf = nseg % C::kQBufs;
+        mbar_wait_spin(q_full(buf), (nseg / C::kQBufs) & 1, a.error_flag, &failed);
+        for (int i = 0; i < sg.count; ++i, ++g) {
+          const int st = g % C::kStages;
+          if (g >= 2) mbar_wait_spin(s_empty(g & 1), ((g >> 1) - 1) & 1, a.error_flag, &failed);
+          mbar_wait_spin(full(st), (g / C::kStages) & 1, a.error_flag, &failed);
+          failed = __any_sync(0xffffffffu, failed);
+          if (failed) break;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint64_t ka = smem_desc_sw128(base + st * C::kStageBytes, 16, C::kGroupBytes);
+            const uint64_t ra = smem_desc_sw128(base + st * C::kStageBytes + C::kKeyBytes, 16, 1024);
+            const uint64_t qb = smem_desc_sw128(s_q + buf * C::kQBytes, 16, 1024);
+            const uint32_t d = tmem + (g & 1) * NH;
 #pragma unroll
-          for (int c = 0; c < C::kChunks; ++c)
+            for (int c = 0; c < C::kChunks; ++c)
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                umma_f16<1>(d, ka + ((c * 1024 + k * 32) >> 4), qb + ((c * NH * 128 + k * 32) >> 4),
+                            kIdQk, c + k > 0);
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              umma_f16<1>(d, ka + ((c * 1024 + k * 32) >> 4), qb + ((c * NH * 128 + k * 32) >> 4),
-                          kIdQk, c + k > 0);
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_f16<1>(d, ra + ((k * 32) >> 4), qb + ((C::kChunks * NH * 128 + k * 32) >> 4),
-                        kIdQk, 1);
-          umma_commit(s_full(g & 1));
-          if (i == sg.count - 1) umma_commit(q_empty(buf));
+              umma_f16<1>(d, ra + ((k * 32) >> 4), qb + ((C::kChunks * NH * 128 + k * 32) >> 4), kIdQk, 1);
+            umma_commit(s_full(g & 1));
+            if (i == sg.count - 1) umma_commit(q_empty(buf));
+          }
+          __syncwarp();
         }
-        __syncwarp();
-        if (pv_due) issue_pv(false);
-        pv_due = true;
-        pv_first = i == 0;
-        pv_tile = g;
-        pv_seg = nseg;
+        ++nseg;
       }
-      ++nseg;
+    } else {
+      constexpr uint32_t kIdPv = idesc_f16(128, NH, kBf16, true, true);
+      while (!failed && next_segment<kTile, kSegmentCost>(a, work, sg)) {
+        for (int i = 0; i < sg.count; ++i, ++g) {
+          const int st = g % C::kStages;
+          if (i == 0 && nseg > 0) mbar_wait_spin(o_empty, (nseg - 1) & 1, a.error_flag, &failed);
+          mbar_wait_spin(p_full, g & 1, a.error_flag, &failed);
+          failed = __any_sync(0xffffffffu, failed);
+          if (failed) break;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint64_t va = smem_desc_sw128(base + st * C::kStageBytes, 1024, C::kGroupBytes);
+            const uint64_t pb = p_desc<NH>(s_p);
+#pragma unroll
+            for (int k = 0; k < kTile / 16; ++k)
+#pragma unroll
+              for (int m = 0; m < C::kBlocks; ++m)
+                umma_f16<1>(t_o + m * NH, va + ((k * 2 * C::kGroupBytes + m * 2048) >> 4),
+                            pb + ((k * 16 * NH * 2) >> 4), kIdPv, (i > 0) | (k > 0));
+            umma_commit(empty(st));
+            umma_commit(p_empty);
+          }
+          __syncwarp();
+        }
+        ++nseg;
+      }
     }
-    if (pv_due && !failed) issue_pv(false);
     if (failed) {   // the products in flight end before the tensor memory is given back
       bool gave_up = false;
-      if (elect_one()) umma_commit(drained);
+      const uint32_t bar = drained(warp == kQkWarp ? 0 : 1);
+      if (elect_one()) umma_commit(bar);
       __syncwarp();
-      mbar_wait(drained, 0, a.error_flag, &gave_up);
+      mbar_wait(bar, 0, a.error_flag, &gave_up);
       __syncwarp();
     }
   } else if (warp < kLoadWarp) {
@@ -373,7 +356,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     float ref[2 * kPairs], lim[2 * kPairs], run[2 * kPairs], sum[2 * kPairs];
     Segment sg;
     int g = 0, nseg = 0;
-    while (next_segment<kTile>(a, work, sg)) {
+    while (next_segment<kTile, kSegmentCost>(a, work, sg)) {
 #pragma unroll
       for (int j = 0; j < 2 * kPairs; ++j) {
         ref[j] = run[j] = lim[j] = -INFINITY;
@@ -391,6 +374,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_ld_frag<HW>(tmem + (g & 1) * NH + head0 + lane_base, raw);
         tmem_ld_wait();
         tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(s_empty(g & 1));
 
         float z[HW / 2];
 #pragma unroll
@@ -581,46 +566,76 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == kMmaWarp) {
+  if (warp == kQkWarp) {
     tmem_relinquish<1>();
     tmem_dealloc<1>(tmem, C::kTmem);
   }
 }
 
-// One block per (row, head): join the parts that the row's CTAs left.  D / 4 threads take a
-// part (one float4 each), kGroups of them go through the parts side by side.
+// Where the parts of one (row, head) are: CTAs c0 .. c1, whose slot of a part is 2 c, but 2 c0 + 1
+// where the row begins inside the share of c0.
+struct Parts {
+  int c0, c1, skip;
+  template <int NH>
+  __device__ __forceinline__ int64_t at(int c, int h) const {
+    return (int64_t)(2 * c + (c == c0 ? skip : 0)) * NH + h;
+  }
+};
+
+template <int NH, int kCost>
+__device__ __forceinline__ bool parts_of(const Args& a, int grid, int row, int head, Parts* p, bool* empty) {
+  const int first = a.ws_prefix[row], next = a.ws_prefix[row + 1], all = a.ws_prefix[a.rows];
+  const int count = next - first;   // units
+  *empty = count == 0;
+  if (count == 0) return false;
+  const int64_t units = (int64_t)all * a.groups, ctas = ctas_used(units, grid);
+  const int64_t x0 = (int64_t)first * a.groups + (int64_t)(head / NH) * count;
+  const int64_t lo = (x0 + kCost + 1) * ctas - 1, hi = (x0 + count) * ctas - 1;
+  if (units * ctas < (1LL << 31)) {   // (a 64-bit division takes as long as a trip to L2)
+    const uint32_t u = (uint32_t)units;
+    p->c0 = (int)((uint32_t)lo / u);
+    p->c1 = (int)((uint32_t)hi / u);
+    p->skip = (uint32_t)(units * p->c0) / (uint32_t)ctas < x0 ? 1 : 0;
+  } else {
+    p->c0 = (int)(lo / units);
+    p->c1 = (int)(hi / units);
+    p->skip = units * p->c0 / ctas < x0 ? 1 : 0;
+  }
+  return p->c0 != p->c1;   // else written whole
+}
+
+// Join the parts that a row's CTAs left; zeros for a row without keys.  kJoinLanes threads go
+// through the parts of one (row, head), D / 4 of them taking a part's float4s side by side:
+// a whole block where there are few rows (and so many parts of each), else a warp.
 constexpr int kJoinThreads = 256;
 
-template <int D, int NH, typename T>
+template <int D, int NH, int kCost, int kLanes, typename T>
 __global__ void __launch_bounds__(kJoinThreads) attn_paged_combine_kernel(const Args a, int grid) {
   using E = ElemTraits<T>;
-  constexpr int kGroups = kJoinThreads / (D / 4);
-  __shared__ float4 part[kGroups][D / 4];
+  constexpr int kCols = kLanes < D / 4 ? kLanes : D / 4;   // threads of a part
+  constexpr int kPer = D / 4 / kCols;                      // float4s of each
+  constexpr int kGroups = kLanes / kCols;                  // parts at a time
+  __shared__ float4 part[kLanes == kJoinThreads ? kGroups : 1][kLanes == kJoinThreads ? D / 4 : 1];
   __shared__ float psum[kGroups];
   griddep_wait();
-  const int row = blockIdx.x / a.n1, head = blockIdx.x - row * a.n1;
-  const int first = a.ws_prefix[row], next = a.ws_prefix[row + 1], all = a.ws_prefix[a.rows];
-  const int count = next - first;
-  const int64_t at = blockIdx.x;
-  const int grp = threadIdx.x / (D / 4), col = threadIdx.x % (D / 4);
-  T* out = static_cast<T*>(a.out) + at * D + col * 4;
-  if (count == 0) {
-    if (grp == 0) *reinterpret_cast<uint2*>(out) = make_uint2(0, 0);
-    if (threadIdx.x == 0 && a.softmax_max) a.softmax_max[at] = a.softmax_sum[at] = 0.0f;
+  const int64_t at = (int64_t)blockIdx.x * (kJoinThreads / kLanes) + threadIdx.x / kLanes;
+  if (at >= (int64_t)a.rows * a.n1) return;
+  const int row = (int)(at / a.n1), head = (int)(at - (int64_t)row * a.n1), h = head % NH;
+  const int t = threadIdx.x % kLanes, grp = t / kCols, col = t % kCols;
+  T* out = static_cast<T*>(a.out) + at * D;
+  Parts p;
+  bool empty;
+  if (!parts_of<NH, kCost>(a, grid, row, head, &p, &empty)) {
+    if (!empty) return;
+    if (grp == 0)
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) *reinterpret_cast<uint2*>(out + (i * kCols + col) * 4) = make_uint2(0, 0);
+    if (t == 0 && a.softmax_max) a.softmax_max[at] = a.softmax_sum[at] = 0.0f;
     return;
   }
-  const int64_t tiles = (int64_t)all * a.groups;
-  const int64_t ctas = ctas_used(tiles, grid);
-  const int group = head / NH, h = head - group * NH;
-  const int64_t x0 = (int64_t)first * a.groups + (int64_t)group * count, x1 = x0 + count;
-  const int c0 = (int)(((x0 + 1) * ctas - 1) / tiles), c1 = (int)((x1 * ctas - 1) / tiles);
-  if (c0 == c1) return;   // written whole
-  // a CTA's part of this row is its first, but where the row begins inside the CTA's share
-  const int skip = tiles * c0 / ctas < x0 ? 1 : 0;
-  auto slot = [&](int c) { return (int64_t)(2 * c + (c == c0 ? skip : 0)) * NH + h; };
   float ref = -INFINITY, run = -INFINITY, top = -INFINITY;
-  for (int c = c0 + (threadIdx.x & 31); c <= c1; c += 32) {
-    const float4 s = a.ws_s[slot(c)];
+  for (int c = p.c0 + (threadIdx.x & 31); c <= p.c1; c += 32) {
+    const float4 s = a.ws_s[p.at<NH>(c, h)];
     ref = fmaxf(ref, s.x);
     run = fmaxf(run, s.y);
     top = fmaxf(top, s.w);
@@ -631,32 +646,42 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_combine_kernel(const 
     run = fmaxf(run, __shfl_xor_sync(0xffffffffu, run, o));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   }
-  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float4 acc[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float sum = 0.0f;
   if (ref != -INFINITY) {
 #pragma unroll 4
-    for (int c = c0 + grp; c <= c1; c += kGroups) {
-      const float4 s = a.ws_s[slot(c)];
-      const float4 o = *reinterpret_cast<const float4*>(a.ws_o + slot(c) * D + col * 4);
+    for (int c = p.c0 + grp; c <= p.c1; c += kGroups) {
+      const float4 s = a.ws_s[p.at<NH>(c, h)];
+      const float4* o = reinterpret_cast<const float4*>(a.ws_o + p.at<NH>(c, h) * D) + col;
       const float w = s.x == ref ? 1.0f : exp2f(s.x - ref);
       sum += w * s.z;
-      acc.x += w * o.x, acc.y += w * o.y, acc.z += w * o.z, acc.w += w * o.w;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const float4 x = o[i * kCols];
+        acc[i].x += w * x.x, acc[i].y += w * x.y, acc[i].z += w * x.z, acc[i].w += w * x.w;
+      }
     }
   }
-  part[grp][col] = acc;
-  if (col == 0) psum[grp] = sum;
-  __syncthreads();
-  if (grp > 0) return;
+  if constexpr (kLanes == kJoinThreads) {
+    part[grp][col] = acc[0];
+    if (col == 0) psum[grp] = sum;
+    __syncthreads();
+    if (grp > 0) return;
 #pragma unroll
-  for (int k = 1; k < kGroups; ++k) {
-    const float4 o = part[k][col];
-    sum += psum[k];
-    acc.x += o.x, acc.y += o.y, acc.z += o.z, acc.w += o.w;
+    for (int k = 1; k < kGroups; ++k) {
+      const float4 o = part[k][col];
+      sum += psum[k];
+      acc[0].x += o.x, acc[0].y += o.y, acc[0].z += o.z, acc[0].w += o.w;
+    }
   }
   const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
-  *reinterpret_cast<uint2*>(out) =
-      make_uint2(E::pack2(acc.x * inv, acc.y * inv), E::pack2(acc.z * inv, acc.w * inv));
-  if (threadIdx.x == 0 && a.softmax_max) {
+#pragma unroll
+  for (int i = 0; i < kPer; ++i)
+    *reinterpret_cast<uint2*>(out + (i * kCols + col) * 4) =
+        make_uint2(E::pack2(acc[i].x * inv, acc[i].y * inv), E::pack2(acc[i].z * inv, acc[i].w * inv));
+  if (t == 0 && a.softmax_max) {
     const bool any = run != -INFINITY;
     a.softmax_max[at] = any ? top * fabsf(a.scale) : 0.0f;
     a.softmax_sum[at] = any ? sum * exp2f(ref - run) : 0.0f;
@@ -720,20 +745,24 @@ bool make_maps(Maps* maps, const DsaAttnPagedParams* p, bool bf16, uint32_t nh) 
          make_tmap_16b(&maps->kr, p->key_rope_cache, bf16, 4, krdims, krst, krbox);
 }
 
-template <int D, int NH, typename T>
+template <int D, int NH, int kCost, typename T>
 int launch_join(const DsaAttnPagedParams* p, const Args& a, int shares, cudaStream_t stream) {
+  const int64_t items = p->batch * p->s1 * p->n1;
+  // a block each up to eight a multiprocessor (what runs at once), else a warp each
+  const bool wide = items <= 8LL * sm_count();
+  const int64_t blocks = wide ? items : (items + kJoinThreads / 32 - 1) / (kJoinThreads / 32);
   cudaLaunchAttribute pdl[1];
   pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   pdl[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(p->batch * p->s1 * p->n1));
+  cfg.gridDim = dim3((unsigned)blocks);
   cfg.blockDim = dim3(kJoinThreads);
   cfg.stream = stream;
   cfg.attrs = pdl;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, attn_paged_combine_kernel<D, NH, T>, a, shares) == cudaSuccess
-             ? DSA_OK
-             : DSA_ERR_CUDA;
+  auto kern = wide ? attn_paged_combine_kernel<D, NH, kCost, kJoinThreads, T>
+                   : attn_paged_combine_kernel<D, NH, kCost, 32, T>;
+  return cudaLaunchKernelEx(&cfg, kern, a, shares) == cudaSuccess ? DSA_OK : DSA_ERR_CUDA;
 }
 
 template <int D, int NH, typename T>
@@ -751,7 +780,7 @@ int launch(const DsaAttnPagedParams* p, cudaStream_t stream) {
     return DSA_ERR_CUDA;
   kern<<<grid, kThreads, C::kSmem, stream>>>(maps, a);
   if (cudaGetLastError() != cudaSuccess) return DSA_ERR_CUDA;
-  return launch_join<D, NH, T>(p, a, grid, stream);
+  return launch_join<D, NH, kSegmentCost, T>(p, a, grid, stream);
 }
 
 template <int D, typename T>
@@ -761,7 +790,7 @@ int launch_pair(const DsaAttnPagedParams* p, cudaStream_t stream) {
   const int pairs = sm_count() / 2;
   if (pairs < 1) return DSA_ERR_CUDA;
   Maps maps;
-  CUtensorMap map_v;
+  CUtensorMap map_v;   // boxes of 8 keys, a CTA's half of the dims
   const uint64_t dims[4] = {64, (uint64_t)p->page_size, D / 64, (uint64_t)p->num_pages};
   const uint64_t st[3] = {(uint64_t)p->k_row_stride * 2, 128, (uint64_t)p->k_page_stride * 2};
   const uint32_t box[4] = {64, 8, C::kVChunks, 1};
@@ -775,7 +804,7 @@ int launch_pair(const DsaAttnPagedParams* p, cudaStream_t stream) {
     return DSA_ERR_CUDA;
   kern<<<2 * pairs, pair::kThreads, C::kSmem, stream>>>(maps, map_v, a);
   if (cudaGetLastError() != cudaSuccess) return DSA_ERR_CUDA;
-  return launch_join<D, 2 * pair::kHeads, T>(p, a, pairs, stream);
+  return launch_join<D, 2 * pair::kHeads, pair::kSegmentCost, T>(p, a, pairs, stream);
 }
 
 template <int D, typename T>
@@ -796,7 +825,7 @@ int launch_dim(const DsaAttnPagedParams* p, cudaStream_t stream) {
   return DSA_ERR_INVALID_ARG;
 }
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+bool aligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
 }  // namespace attn_paged
 }  // namespace dsa
@@ -822,9 +851,10 @@ extern "C" int dsa_attn_paged(const DsaAttnPagedParams* p, void* stream_) {
     return DSA_ERR_INVALID_ARG;
   // sizes the kernels index with 32 bits: rows * n1 blocks, tiles, pages
   constexpr int64_t kMax = 0x7fffffff;
+  // (units are counted in 32 bits: a row's tiles and its start)
   if (p->batch > kMax || p->s1 > kMax || p->batch * p->s1 > kMax / p->n1 || p->num_pages > kMax ||
       p->page_size > (1 << 20) || p->max_blocks > (kMax - kTile) / p->page_size ||
-      p->batch * p->s1 > kMax / ((p->max_blocks * p->page_size + kTile - 1) / kTile))
+      p->batch * p->s1 > kMax / ((p->max_blocks * p->page_size + kTile - 1) / kTile + 8))
     return DSA_ERR_INVALID_ARG;
   if ((p->softmax_max == nullptr) != (p->softmax_sum == nullptr)) return DSA_ERR_INVALID_ARG;
   const int64_t strides[10] = {p->q_head_stride,  p->q_token_stride,  p->q_batch_stride,
@@ -833,8 +863,8 @@ extern "C" int dsa_attn_paged(const DsaAttnPagedParams* p, void* stream_) {
                                p->kr_page_stride};
   for (int64_t s : strides)
     if (s < 0 || s % 8) return DSA_ERR_INVALID_ARG;
-  if (!aligned16(p->query) || !aligned16(p->query_rope) || !aligned16(p->key_cache) ||
-      !aligned16(p->key_rope_cache) || !aligned16(p->workspace))
+  if (!aligned(p->query, 16) || !aligned(p->query_rope, 16) || !aligned(p->key_cache, 16) ||
+      !aligned(p->key_rope_cache, 16) || !aligned(p->workspace, 32) || !aligned(p->out, 32))
     return DSA_ERR_INVALID_ARG;
   if (p->workspace_bytes < dsa_attn_paged_workspace_size(p->batch, p->s1, p->n1, p->d))
     return DSA_ERR_INVALID_ARG;

@@ -11,7 +11,6 @@ namespace attn_paged {
 
 constexpr int kRope = 64;
 constexpr int kSmemLimit = 232448;
-constexpr int kAhead = 3;           // tiles that are brought into L2 before their load
 constexpr float kRescale = 8.0f;    // log2 units a score may pass the reference
 
 struct Maps {
@@ -26,7 +25,7 @@ struct Args {
   float* softmax_max;
   float* softmax_sum;
   int* error_flag;
-  int32_t* ws_prefix;   // [rows + 1] first tile of each row
+  int32_t* ws_prefix;   // [rows + 1] units of the rows before each (of one head group)
   float* ws_o;          // [2 * CTAs][NH][D]
   float4* ws_s;         // [2 * CTAs][NH]: reference and running maximum (log2 units), sum,
                         // raw running maximum
@@ -44,16 +43,21 @@ __device__ __forceinline__ int row_keys(const Args& a, int row) {
   if (s >= aq || n < 0) n = 0;
   return (int)n;
 }
-template <int kTile>
-__device__ __forceinline__ int row_tiles(const Args& a, int row) {
-  return (row_keys(a, row) + kTile - 1) / kTile;
+template <int kTile, int kCost>
+__device__ __forceinline__ int row_units(const Args& a, int row) {
+  const int tiles = (row_keys(a, row) + kTile - 1) / kTile;
+  return tiles > 0 ? tiles + kCost : 0;
 }
 
-// CTAs (pairs of them in the pair kernel) that share `tiles` tiles; each takes kMinTiles at
-// least, as fewer cost more in joining than they save.
-constexpr int kMinTiles = 2;
-__device__ __forceinline__ int64_t ctas_used(int64_t tiles, int grid) {
-  const int64_t c = (tiles + kMinTiles - 1) / kMinTiles;
+// Work is divided by units: an item (a row's head group) of T tiles has T + kCost of them, the
+// first kCost standing for what a CTA spends on starting an item (queries, filling the pipeline,
+// the result).  CTA c of n takes units [U c / n, U (c + 1) / n) of all U.
+
+// CTAs (pairs of them in the pair kernel) that share `units`; each takes kMinUnits at least, as
+// fewer cost more in joining than they save.
+constexpr int kMinUnits = 2;
+__device__ __forceinline__ int64_t ctas_used(int64_t units, int grid) {
+  const int64_t c = (units + kMinUnits - 1) / kMinUnits;
   return c < 1 ? 1 : c < grid ? c : grid;
 }
 
@@ -80,16 +84,16 @@ __device__ __forceinline__ int block_scan(int v, int* tmp, int* total) {
   return before + x - v;
 }
 
-// One CTA's share: tiles from (row, head group, tile) on, `left` of them.
+// One CTA's share: `left` units from unit `unit` of (row, head group) on.
 struct Work {
-  int row, group, tile, left;
+  int row, group, unit, left;
 };
 // A run of tiles of one (row, head group).
 struct Segment {
   int row, group, first, count, keys, tiles;
 };
 // The next run of `w` (false when the share is done); `w` moves past it.
-template <int kTile>
+template <int kTile, int kCost>
 __device__ __forceinline__ bool next_segment(const Args& a, Work& w, Segment& s) {
   while (w.left > 0 && w.row < a.rows) {
     s.keys = row_keys(a, w.row);
@@ -98,52 +102,52 @@ __device__ __forceinline__ bool next_segment(const Args& a, Work& w, Segment& s)
       ++w.row;
       continue;
     }
+    const int end = min(s.tiles + kCost, w.unit + w.left);
     s.row = w.row;
     s.group = w.group;
-    s.first = w.tile;
-    s.count = min(s.tiles - w.tile, w.left);
-    w.left -= s.count;
-    w.tile = 0;
+    s.first = max(0, w.unit - kCost);
+    s.count = max(0, end - kCost) - s.first;
+    w.left -= end - w.unit;
+    w.unit = 0;
     if (++w.group == a.groups) {
       w.group = 0;
       ++w.row;
     }
-    return true;
+    if (s.count > 0) return true;
   }
   return false;
 }
 
-// The share of CTA (or pair) `cta` of `ctas_max`: equal numbers of tiles, whatever rows they
-// are of.  All threads of the block call it; the place where the share begins is left in
+// The share of CTA (or pair) `cta` of `ctas_max`.  All threads of the block call it; the place where the share begins is left in
 // `start` (shared memory), to be read after a barrier (take_start).  The first CTA also writes
 // the rows' prefix for the join.
-template <int kTile, int kThreads>
+template <int kTile, int kCost, int kThreads>
 __device__ __forceinline__ Work share_of(const Args& a, int cta, int ctas_max, bool first_cta, int* tmp,
                                          int32_t* start) {
   int64_t total = 0;
-  int mine = 0, before = 0;   // the tiles of the thread's last row and of the rows before it
+  int mine = 0, before = 0;   // the units of the thread's last row and of the rows before it
   for (int r0 = 0; r0 < a.rows; r0 += kThreads) {
     const int r = r0 + threadIdx.x;
     int sum;
-    mine = r < a.rows ? row_tiles<kTile>(a, r) : 0;
+    mine = r < a.rows ? row_units<kTile, kCost>(a, r) : 0;
     before = block_scan<kThreads>(mine, tmp, &sum);
     if (first_cta && r < a.rows) a.ws_prefix[r] = (int)total + before;
     total += sum;
   }
   if (first_cta && threadIdx.x == 0) a.ws_prefix[a.rows] = (int)total;
-  const int64_t tiles = total * a.groups;
-  const int64_t ctas = ctas_used(tiles, ctas_max);
+  const int64_t units = total * a.groups;
+  const int64_t ctas = ctas_used(units, ctas_max);
   Work work{0, 0, 0, 0};
   int64_t from = 0;
   if (cta < ctas) {
-    from = tiles * cta / ctas;
-    work.left = (int)(tiles * (cta + 1) / ctas - from);
+    from = units * cta / ctas;
+    work.left = (int)(units * (cta + 1) / ctas - from);
     int64_t seen = 0;
     for (int r0 = 0; r0 < a.rows; r0 += kThreads) {
       const int r = r0 + threadIdx.x;
       int sum = (int)total;
       if (a.rows > kThreads) {
-        mine = r < a.rows ? row_tiles<kTile>(a, r) : 0;
+        mine = r < a.rows ? row_units<kTile, kCost>(a, r) : 0;
         before = block_scan<kThreads>(mine, tmp, &sum);
       }
       const int64_t first = (seen + before) * a.groups;
@@ -163,7 +167,7 @@ __device__ __forceinline__ void take_start(Work& work, const int32_t* start) {
   if (work.left <= 0) return;
   work.row = start[0];
   work.group = start[1];
-  work.tile = start[2];
+  work.unit = start[2];
 }
 
 // 2^x, 2^-126 and below flushed to 0

@@ -10,8 +10,12 @@
 // all keys (the other kernel, twice) the tensor core's operand reads from shared memory fall
 // from 555 KB to 260 KB per 128 keys and CTA, which is what bounded that form.
 //
-// A tile of 128 keys and the queries leave room for one buffer each of K and V at D = 512.
-// That is enough: K(t + 1) arrives during softmax(t) and PV(t), V(t + 1) during QK(t + 1).
+// A tile of 128 keys and the queries leave room for one buffer each of K and V at D = 512.  V is
+// held in halves of 64 keys with barriers of their own, so that the next tile's first half is on
+// its way while the second is in work.  (K in three parts of 192 dims, refilled one by one, took
+// 369 us against 347 for 32 rows of 8192 .. 65536 keys and 128 heads: the loads then meet QK's
+// operand reads, and shared memory, at 400 KB a tile and CTA, is what bounds this kernel.
+// Bringing tiles into L2 ahead of their load gained nothing here.)
 #pragma once
 
 #include "attn_paged.cuh"
@@ -22,30 +26,32 @@ namespace attn_paged {
 namespace pair {
 
 constexpr int kTile = 128;
+constexpr int kSegmentCost = 4;    // of starting a row, in tiles
 constexpr int kHeads = 64;          // of a CTA
 constexpr int kSoftmaxThreads = 256;
 constexpr int kKeyWarp = 8;         // warps 8-11 load K
-constexpr int kValueWarp = 12;      // warps 12, 13 load V
+constexpr int kValueWarp = 12;      // warps 12, 13 load V, warp 12 the queries too
 constexpr int kMmaWarp = 14;
-constexpr int kQueryWarp = 15;
-constexpr int kThreads = 512;
-constexpr int kMaxStages = 4;
+constexpr int kThreads = 480;
+constexpr int kMaxStages = 3;
+constexpr int kMaxSlots = 6;        // halves of V
 
 template <int D>
 struct Cfg {
   static constexpr int kChunks = D / 64;
   static constexpr int kGroupBytes = kChunks * 1024;           // 8 keys of K: [chunk][8][128 B]
   static constexpr int kKeyBytes = 8 * kGroupBytes;            // this CTA's 64 keys
-  static constexpr int kRopeBytes = 64 * 128;
-  static constexpr int kKBytes = kKeyBytes + kRopeBytes;
+  static constexpr int kKBytes = kKeyBytes + 64 * 128;         // and their rotary parts
   static constexpr int kVChunks = D / 128;                     // this CTA's dims
   static constexpr int kVGroupBytes = kVChunks * 1024;
-  static constexpr int kVBytes = 16 * kVGroupBytes;            // 128 keys
+  static constexpr int kHalfBytes = 8 * kVGroupBytes;          // 64 keys
+  static constexpr int kVBytes = 2 * kHalfBytes;
   static constexpr int kQBytes = kHeads * (D + kRope) * 2;
   static constexpr int kPBytes = kHeads * kTile * 2;
   static constexpr int kSmallBytes = 2 * 4 * kHeads * 4 + 640;
   static constexpr int kRoom = (kSmemLimit - kQBytes - kPBytes - kSmallBytes) / (kKBytes + kVBytes);
   static constexpr int kStages = kRoom < kMaxStages ? kRoom : kMaxStages;   // of K and of V
+  static constexpr int kVSlots = kStages * 2;
   static constexpr int kQBufs =
       kStages * (kKBytes + kVBytes) + 2 * kQBytes + kPBytes + kSmallBytes <= kSmemLimit ? 2 : 1;
   static constexpr int kOffK = kQBufs * kQBytes;
@@ -57,7 +63,7 @@ struct Cfg {
   static constexpr int kPvs = D / kPvN;
   static constexpr uint32_t kColsO = 128;                      // after two buffers of S
   static constexpr uint32_t kTmem = D == 512 ? 512 : 256;
-  static_assert(kStages >= 1 && kOffK % 1024 == 0 && kOffV % 1024 == 0 && kOffP % 1024 == 0, "layout");
+  static_assert(kStages >= 1 && kVSlots <= kMaxSlots && kOffK % 1024 == 0 && kOffV % 1024 == 0 && kOffP % 1024 == 0, "layout");
 };
 
 // The tiles of a share one by one.
@@ -72,7 +78,7 @@ struct Tiles {
     }
     i = 0;
     ++seg;
-    return next_segment<kTile>(a, w, s);
+    return next_segment<kTile, kSegmentCost>(a, w, s);
   }
 };
 
@@ -94,18 +100,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   int32_t* start = reinterpret_cast<int32_t*>(tmem_ptr + 1);     // [3]
 
   const uint32_t b0 = smem_u32(bars);
-  auto k_full = [&](int s) { return b0 + 8u * s; };                      // leader's
-  auto k_empty = [&](int s) { return b0 + 8u * (kMaxStages + s); };
-  auto v_full = [&](int s) { return b0 + 8u * (2 * kMaxStages + s); };   // leader's
-  auto v_empty = [&](int s) { return b0 + 8u * (3 * kMaxStages + s); };
-  auto s_full = [&](int s) { return b0 + 8u * (4 * kMaxStages + s); };
-  auto q_full = [&](int s) { return b0 + 8u * (4 * kMaxStages + 2 + s); };   // leader's
-  auto q_empty = [&](int s) { return b0 + 8u * (4 * kMaxStages + 4 + s); };
-  const uint32_t p_full = b0 + 8u * (4 * kMaxStages + 6);      // leader's
-  const uint32_t p_empty = b0 + 8u * (4 * kMaxStages + 7);
-  const uint32_t o_empty = b0 + 8u * (4 * kMaxStages + 8);     // leader's
-  const uint32_t drained = b0 + 8u * (4 * kMaxStages + 9);
-  auto v_tail = [&](int s) { return b0 + 8u * (4 * kMaxStages + 10 + s); };
+  auto k_full = [&](int s) { return b0 + 8u * s; };                     // leader's
+  auto k_empty = [&](int s) { return b0 + 8u * (kMaxSlots + s); };
+  auto v_full = [&](int s) { return b0 + 8u * (2 * kMaxSlots + s); };   // leader's
+  auto v_empty = [&](int s) { return b0 + 8u * (3 * kMaxSlots + s); };
+  auto v_tail = [&](int s) { return b0 + 8u * (4 * kMaxSlots + s); };
+  auto s_full = [&](int s) { return b0 + 8u * (5 * kMaxSlots + s); };
+  auto q_full = [&](int s) { return b0 + 8u * (5 * kMaxSlots + 2 + s); };   // leader's
+  auto q_empty = [&](int s) { return b0 + 8u * (5 * kMaxSlots + 4 + s); };
+  const uint32_t p_full = b0 + 8u * (5 * kMaxSlots + 6);       // leader's
+  const uint32_t p_empty = b0 + 8u * (5 * kMaxSlots + 7);
+  const uint32_t o_empty = b0 + 8u * (5 * kMaxSlots + 8);      // leader's
+  const uint32_t drained = b0 + 8u * (5 * kMaxSlots + 9);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (base & 1023u) {   // the same in both CTAs
@@ -117,6 +123,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(k_full(s), 4);
       mbar_init(k_empty(s), 1);
+    }
+    for (int s = 0; s < C::kVSlots; ++s) {
       mbar_init(v_full(s), 2);
       mbar_init(v_empty(s), 1);
       mbar_init(v_tail(s), 2);
@@ -127,13 +135,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       mbar_init(q_empty(s), 1);
     }
     mbar_init(p_full, 16);
+    mbar_init(drained, 1);
     mbar_init(p_empty, 1);
     mbar_init(o_empty, 16);
-    mbar_init(drained, 1);
     fence_mbarrier_init();
   }
   if (warp == kMmaWarp) tmem_alloc<2>(smem_u32(tmem_ptr), C::kTmem);
-  Work work = share_of<kTile, kThreads>(a, blockIdx.x >> 1, gridDim.x >> 1, blockIdx.x == 0, tmp, start);
+  Work work = share_of<kTile, kSegmentCost, kThreads>(a, blockIdx.x >> 1, gridDim.x >> 1, blockIdx.x == 0, tmp, start);
   griddep_launch_dependents();
   tc_fence_before();
   __syncthreads();
@@ -143,14 +151,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   take_start(work, start);
   bool failed = false;
 
-  // Lane l < 16 looks up the page of keys 8 l .. 8 l + 7 of a tile, lanes 16 .. 31 that of the
-  // tile kAhead further on.  -1: no such page.  (Every role that has to know which keys are
-  // there looks for itself, one tile ahead, so that nobody waits for a message.)
+  // Lane l < 16 looks up the page of keys 8 l .. 8 l + 7 of a tile.  -1: no such page.  (Every
+  // role that has to know which keys are there looks for itself, one tile ahead, so that nobody
+  // waits for a message.)
   auto page_of = [&](const Segment& sg, const int32_t* table, int tile, bool tell) {
-    const int t = tile + (lane < 16 ? 0 : kAhead), pos = t * kTile + (lane & 15) * 8;
-    if (pos >= sg.keys || t >= sg.first + sg.count) return -1;
+    const int pos = tile * kTile + lane * 8;
+    if (lane >= 16 || pos >= sg.keys) return -1;
     const int id = table[pos / a.page_size];
-    if (tell && lane < 16 && id >= a.num_pages) report_error(a.error_flag, kErrBadIndex);
+    if (tell && id >= a.num_pages) report_error(a.error_flag, kErrBadIndex);
     return id < a.num_pages ? id : -1;
   };
   auto table_of = [&](const Segment& sg) { return a.block_table + (int64_t)(sg.row / a.s1) * a.max_blocks; };
@@ -160,7 +168,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     // This warp loads groups 2 w and 2 w + 1 (of 8 keys) of this CTA's 64 keys of every tile.
     // The leader's barrier counts the bytes of both CTAs.
     const int w = warp - kKeyWarp, g0 = 8 * (int)rank + 2 * w;
-    const bool mine = ((lane & 15) >> 1) == (g0 >> 1);
+    const int grp = lane - 8 * (int)rank;
     Tiles t{work, {}, 0, -1};
     int g = 0, page = -1;
     for (; t.next(a); ++g) {
@@ -168,26 +176,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const int tile = t.s.first + t.i, st = g % C::kStages;
       const int now = t.i == 0 ? page_of(t.s, table, tile, rank == 0 && w == 0) : page;
       if (t.i + 1 < t.s.count) page = page_of(t.s, table, tile + 1, rank == 0 && w == 0);
+      const uint32_t mask = __ballot_sync(0xffffffffu, now >= 0);
+      const int in_page = (tile * kTile + lane * 8) % a.page_size;
       if (g >= C::kStages) mbar_wait(k_empty(st), (g / C::kStages - 1) & 1, a.error_flag, &failed);
       failed = __any_sync(0xffffffffu, failed);
       if (failed) break;
-      const uint32_t mask = __ballot_sync(0xffffffffu, now >= 0);
       if (rank == 0 && lane == 0) {
         const uint32_t bytes = __popc(mask & (3u << (2 * w) | 3u << (8 + 2 * w))) * (C::kGroupBytes + 1024);
         if (bytes) mbar_arrive_expect_tx(k_full(st), bytes);
         else mbar_arrive(k_full(st));
       }
       __syncwarp();
-      const int in_page = ((tile + (lane < 16 ? 0 : kAhead)) * kTile + (lane & 15) * 8) % a.page_size;
-      const uint32_t dst = base + C::kOffK + st * C::kKBytes;
-      const int grp = (lane & 15) - 8 * (int)rank;
-      if (mine && now >= 0 && lane < 16) {
-        const uint32_t bar = mapa_shared(k_full(st), 0);
+      if (now >= 0 && (lane == g0 || lane == g0 + 1)) {
+        const uint32_t bar = mapa_shared(k_full(st), 0), dst = base + C::kOffK + st * C::kKBytes;
         tma_load_4d_pair(dst + grp * C::kGroupBytes, &maps.k, bar, 0, in_page, 0, now);
         tma_load_4d_pair(dst + C::kKeyBytes + grp * 1024, &maps.kr, bar, 0, in_page, 0, now);
-      } else if (mine && now >= 0) {
-        tma_prefetch_4d(&maps.k, 0, in_page, 0, now);
-        tma_prefetch_4d(&maps.kr, 0, in_page, 0, now);
       }
       __syncwarp();
     }
@@ -198,76 +201,69 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
   } else if (warp >= kValueWarp && warp < kMmaWarp) {
-    // -------------------------------------------------------------------- V
-    // This warp loads 8 of the tile's 16 groups, this CTA's dims of them.  A tile with keys that
-    // are not there completes on a barrier of the CTA's own, since its softmax warps clear those
-    // rows before the product; their P then tells the leader.
+    // -------------------------------------------------------------------- V, queries
+    // This warp loads 4 groups (of 8 keys) of each half of the tile, this CTA's dims of them.
+    // A tile with keys that are not there completes on barriers of the CTA's own, since its
+    // softmax warps clear those rows before the product; their P then tells the leader.
     const int w = warp - kValueWarp;
     Tiles t{work, {}, 0, -1};
     int g = 0, page = -1;
     for (; t.next(a); ++g) {
       const int32_t* table = table_of(t.s);
-      const int tile = t.s.first + t.i, st = g % C::kStages;
+      const int tile = t.s.first + t.i;
       const int now = t.i == 0 ? page_of(t.s, table, tile, false) : page;
       if (t.i + 1 < t.s.count) page = page_of(t.s, table, tile + 1, false);
-      if (g >= C::kStages) mbar_wait(v_empty(st), (g / C::kStages - 1) & 1, a.error_flag, &failed);
-      failed = __any_sync(0xffffffffu, failed);
-      if (failed) break;
       const uint32_t mask = __ballot_sync(0xffffffffu, now >= 0) & 0xffffu;
       const bool tail = mask != 0xffffu || t.s.keys - tile * kTile < kTile;
-      if (lane == 0) {
-        const uint32_t bytes = __popc(mask & (0xffu << (8 * w))) * C::kVGroupBytes;
-        if (tail) {
-          if (bytes) mbar_arrive_expect_tx(v_tail(st), bytes);
-          else mbar_arrive(v_tail(st));
+      const int in_page = (tile * kTile + lane * 8) % a.page_size;
+      if (w == 0 && t.i == 0) {
+        const int b = t.s.row / a.s1, s = t.s.row - b * a.s1;
+        const int buf = t.seg % C::kQBufs, use = t.seg / C::kQBufs;
+        if (use > 0) mbar_wait(q_empty(buf), (use - 1) & 1, a.error_flag, &failed);
+        failed = __any_sync(0xffffffffu, failed);
+        if (failed) break;
+        if (lane == 0) {
+          const uint32_t dst = base + buf * C::kQBytes, bar = mapa_shared(q_full(buf), 0);
+          if (rank == 0) mbar_arrive_expect_tx(q_full(buf), 2 * C::kQBytes);
+          tma_load_5d_pair(dst, &maps.q, bar, 0, kHeads * (int)rank, 0, s, b);
+          tma_load_5d_pair(dst + kHeads * D * 2, &maps.qr, bar, 0, kHeads * (int)rank, 0, s, b);
         }
-        if (rank == 0) {
-          if (tail) mbar_arrive(v_full(st));
-          else mbar_arrive_expect_tx(v_full(st), 2 * bytes);
+        __syncwarp();
+      }
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const int u = 2 * g + hf, slot = u % C::kVSlots;
+        if (u >= C::kVSlots) mbar_wait(v_empty(slot), (u / C::kVSlots - 1) & 1, a.error_flag, &failed);
+        failed = __any_sync(0xffffffffu, failed);
+        if (failed) break;
+        if (lane == 0) {
+          const uint32_t bytes = __popc(mask & (0xfu << (8 * hf + 4 * w))) * C::kVGroupBytes;
+          if (tail) {
+            if (bytes) mbar_arrive_expect_tx(v_tail(slot), bytes);
+            else mbar_arrive(v_tail(slot));
+          }
+          if (rank == 0) {
+            if (tail) mbar_arrive(v_full(slot));
+            else mbar_arrive_expect_tx(v_full(slot), 2 * bytes);
+          }
         }
+        __syncwarp();
+        if (now >= 0 && lane < 16 && (lane >> 2) == 2 * hf + w) {
+          const uint32_t dst = base + C::kOffV + slot * C::kHalfBytes + (lane & 7) * C::kVGroupBytes;
+          if (tail)
+            tma_load_4d(dst, &map_v, v_tail(slot), 0, in_page, C::kVChunks * (int)rank, now);
+          else
+            tma_load_4d_pair(dst, &map_v, mapa_shared(v_full(slot), 0), 0, in_page,
+                             C::kVChunks * (int)rank, now);
+        }
+        __syncwarp();
       }
-      __syncwarp();
-      if (now >= 0 && lane < 16 && (lane >> 3) == w) {
-        const int in_page = (tile * kTile + lane * 8) % a.page_size;
-        const uint32_t dst = base + C::kOffV + st * C::kVBytes + lane * C::kVGroupBytes;
-        if (tail)
-          tma_load_4d(dst, &map_v, v_tail(st), 0, in_page, C::kVChunks * (int)rank, now);
-        else
-          tma_load_4d_pair(dst, &map_v, mapa_shared(v_full(st), 0), 0, in_page, C::kVChunks * (int)rank, now);
-      }
-      __syncwarp();
-    }
-    if (failed) {
-      bool gave_up = false;
-      if (rank == 0)
-        for (int u = max(0, g - C::kStages); u < g; ++u)
-          mbar_wait(v_full(u % C::kStages), (u / C::kStages) & 1, a.error_flag, &gave_up, true);
-    }
-    __syncwarp();
-  } else if (warp == kQueryWarp) {
-    // -------------------------------------------------------------------- queries
-    Work w = work;
-    Segment sg;
-    int nseg = 0;
-    while (next_segment<kTile>(a, w, sg)) {
-      const int b = sg.row / a.s1, s = sg.row - b * a.s1;
-      const int buf = nseg % C::kQBufs, use = nseg / C::kQBufs;
-      if (use > 0) mbar_wait(q_empty(buf), (use - 1) & 1, a.error_flag, &failed);
-      failed = __any_sync(0xffffffffu, failed);
       if (failed) break;
-      if (lane == 0) {
-        const uint32_t dst = base + buf * C::kQBytes, bar = mapa_shared(q_full(buf), 0);
-        if (rank == 0) mbar_arrive_expect_tx(q_full(buf), 2 * C::kQBytes);
-        tma_load_5d_pair(dst, &maps.q, bar, 0, kHeads * (int)rank, 0, s, b);
-        tma_load_5d_pair(dst + kHeads * D * 2, &maps.qr, bar, 0, kHeads * (int)rank, 0, s, b);
-      }
-      __syncwarp();
-      ++nseg;
     }
     if (failed && rank == 0) {
       bool gave_up = false;
-      for (int u = max(0, nseg - C::kQBufs); u < nseg; ++u)
-        mbar_wait(q_full(u % C::kQBufs), (u / C::kQBufs) & 1, a.error_flag, &gave_up, true);
+      for (int u = max(0, 2 * (g - C::kStages)); u < 2 * g; ++u)
+        mbar_wait(v_full(u % C::kVSlots), (u / C::kVSlots) & 1, a.error_flag, &gave_up, true);
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
@@ -275,15 +271,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     if (rank == 0) {
       constexpr uint32_t kIdQk = idesc_f16(128, kTile, kBf16, false, false);
       constexpr uint32_t kIdPv = idesc_f16(128, C::kPvN, kBf16, false, true);
-      // Whichever product has its operands goes next: QK(a) at most two tiles ahead of PV, as
-      // there are two buffers of scores and PV(a - 2) waited for the probabilities made of S(a - 2).
+      // Whichever product has its operands goes next: QK(na) at most two tiles ahead of PV(nb),
+      // which goes half by half, as there are two buffers of scores and PV(na - 2) waited for the
+      // probabilities made of S(na - 2).  One warp issues both whole: with a warp for each (as in
+      // the other kernel) their instructions alternate, and the same rows took 395 us for 349.
       Tiles q{work, {}, 0, -1}, v{work, {}, 0, -1};
       bool more_q = q.next(a), more_v = v.next(a);
-      int na = 0, nb = 0;
+      int na = 0, nb = 0, pb = 0;
       uint64_t t0 = 0;
       auto all = [](bool x) { return __all_sync(0xffffffffu, x) != 0; };
       for (uint32_t idle = 0; more_v && !failed;) {
-        const int sa = na % C::kStages, sb = nb % C::kStages;
+        const int sa = na % C::kStages;
+        const int ub = 2 * nb + pb, sb = ub % C::kVSlots;
         const int buf = q.seg % C::kQBufs;
         if (more_q && na - nb < 2 &&
             all((q.i > 0 || mbar_test_wait_cluster(q_full(buf), (q.seg / C::kQBufs) & 1)) &&
@@ -314,26 +313,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           idle = 0;
           continue;
         }
-        if (nb < na && all(mbar_test_wait_cluster(p_full, nb & 1) &&
-                           mbar_test_wait_cluster(v_full(sb), (nb / C::kStages) & 1) &&
-                           (v.i > 0 || v.seg == 0 || mbar_test_wait_cluster(o_empty, (v.seg - 1) & 1)))) {
+        if (nb < na && all((pb > 0 || mbar_test_wait_cluster(p_full, nb & 1)) &&
+                           mbar_test_wait_cluster(v_full(sb), (ub / C::kVSlots) & 1) &&
+                           (v.i + pb > 0 || v.seg == 0 || mbar_test_wait_cluster(o_empty, (v.seg - 1) & 1)))) {
           tc_fence_after();
           if (elect_one()) {
-            const uint64_t pa = smem_desc_sw128(base + C::kOffP, 16, 1024);
-            const uint64_t vb = smem_desc_sw128(base + C::kOffV + sb * C::kVBytes, 1024, C::kVGroupBytes);
+            const uint64_t pd = smem_desc_sw128(base + C::kOffP + pb * (kHeads * 128), 16, 1024);
+            const uint64_t vb = smem_desc_sw128(base + C::kOffV + sb * C::kHalfBytes, 1024, C::kVGroupBytes);
 #pragma unroll
-            for (int k = 0; k < kTile / 16; ++k)
+            for (int k = 0; k < 4; ++k)
 #pragma unroll
               for (int n = 0; n < C::kPvs; ++n)
-                umma_f16<2>(tmem + C::kColsO + n * (C::kPvN / 2),
-                            pa + (((k >> 2) * kHeads * 128 + (k & 3) * 32) >> 4),
-                            vb + ((k * 2 * C::kVGroupBytes + n * 2048) >> 4), kIdPv, !(v.i == 0 && k == 0));
+                umma_f16<2>(tmem + C::kColsO + n * (C::kPvN / 2), pd + ((k * 32) >> 4),
+                            vb + ((k * 2 * C::kVGroupBytes + n * 2048) >> 4), kIdPv, (v.i + pb > 0) | (k > 0));
             umma_commit_pair(v_empty(sb), 3);
-            umma_commit_pair(p_empty, 3);
+            if (pb == 1) umma_commit_pair(p_empty, 3);
           }
           __syncwarp();
-          more_v = v.next(a);
-          ++nb;
+          if (pb == 1) {
+            more_v = v.next(a);
+            ++nb;
+          }
+          pb ^= 1;
           idle = 0;
           continue;
         }
@@ -345,12 +346,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           if (failed && lane == 0) report_error(a.error_flag, kErrTimeout);
         }
       }
-      if (failed) {   // the products in flight end before the tensor memory is given back
-        bool gave_up = false;
-        if (elect_one()) umma_commit_pair(drained, 1);
-        __syncwarp();
-        mbar_wait(drained, 0, a.error_flag, &gave_up);
-      }
+    }
+    if (failed) {   // the products in flight end before the tensor memory is given back
+      bool gave_up = false;
+      if (elect_one()) umma_commit_pair(drained, 1);
+      __syncwarp();
+      mbar_wait(drained, 0, a.error_flag, &gave_up);
     }
     __syncwarp();
   } else {
@@ -370,13 +371,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     Work w = work;
     Segment sg;
     int g = 0, nseg = 0;
-    uint32_t tails = 0;   // parity of each stage's tiles with keys that are not there
-    while (next_segment<kTile>(a, w, sg)) {
+    uint32_t tails = 0;   // parity of each slot's halves of tiles with keys that are not there
+    while (next_segment<kTile, kSegmentCost>(a, w, sg)) {
       const int32_t* table = table_of(sg);
       float ref = -INFINITY, lim = -INFINITY, run = -INFINITY, sum = 0.0f;
       int page = page_of(sg, table, sg.first, false);
       for (int i = 0; i < sg.count; ++i, ++g) {
-        const int tile = sg.first + i, st = g % C::kStages;
+        const int tile = sg.first + i;
         const uint32_t mask = __ballot_sync(0xffffffffu, page >= 0) & 0xffffu;
         if (i + 1 < sg.count) page = page_of(sg, table, tile + 1, false);
         const int valid = sg.keys - tile * kTile;
@@ -448,11 +449,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (tail) {
           // rows of this tile that no key stands in hold what was there before (or a page's
           // stale tail): cleared, so that 0 x NaN cannot enter the product
-          mbar_wait_spin(v_tail(st), tails >> st & 1, a.error_flag, &failed);
-          tails ^= 1u << st;
           const int key = threadIdx.x >> 1;
+          const int s0 = 2 * g % C::kVSlots, slot = s0 + (key >> 6);   // of this thread's half
+          mbar_wait_spin(v_tail(slot), tails >> slot & 1, a.error_flag, &failed);
+          tails ^= 3u << s0;
           if (key >= valid || !(mask >> (key >> 3) & 1u)) {
-            uint8_t* row = smem + C::kOffV + st * C::kVBytes + (key >> 3) * C::kVGroupBytes + (key & 7) * 128;
+            uint8_t* row = smem + C::kOffV + slot * C::kHalfBytes + (key >> 3 & 7) * C::kVGroupBytes + (key & 7) * 128;
             for (int c = threadIdx.x & 1; c < C::kVChunks; c += 2)
 #pragma unroll
               for (int x = 0; x < 8; ++x)
@@ -499,19 +501,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         tmem_ld_wait_regs(o);
         if (head >= a.n1) {
           // a padded head: nothing to write
-        } else if (whole) {
-          uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + ((int64_t)sg.row * a.n1 + head) * D + dim + c);
+        } else if (whole) {   // whole 32-byte sectors, as a lane's neighbours write other rows
+          T* out = static_cast<T*>(a.out) + ((int64_t)sg.row * a.n1 + head) * D + dim + c;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            auto two = [&](int k) {
-              return E::pack2(__uint_as_float(o[8 * j + k]) * inv, __uint_as_float(o[8 * j + k + 1]) * inv);
-            };
-            out[j] = make_uint4(two(0), two(2), two(4), two(6));
+          for (int j = 0; j < 32; j += 16) {
+            uint32_t v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              v[k] = E::pack2(__uint_as_float(o[j + 2 * k]) * inv, __uint_as_float(o[j + 2 * k + 1]) * inv);
+            st_global_v8(out + j, v);
           }
         } else {
-          uint4* out = reinterpret_cast<uint4*>(a.ws_o + (slot * (2 * kHeads) + head) * D + dim + c);
+          float* out = a.ws_o + (slot * (2 * kHeads) + head) * D + dim + c;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) out[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+          for (int j = 0; j < 32; j += 8) {
+            const uint32_t v[8] = {o[j], o[j + 1], o[j + 2], o[j + 3], o[j + 4], o[j + 5], o[j + 6], o[j + 7]};
+            st_global_v8(out + j, v);
+          }
         }
         __syncwarp();
       }

@@ -353,15 +353,6 @@ __device__ __forceinline__ void tma_load_5d_pair(uint32_t dst, const CUtensorMap
       : "memory");
 }
 
-// Bring a 4-D tile into L2.
-__device__ __forceinline__ void tma_prefetch_4d(const CUtensorMap* map, int32_t x, int32_t y,
-                                                int32_t z, int32_t w) {
-  asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];" ::"l"(
-                   reinterpret_cast<uint64_t>(map)),
-               "r"(x), "r"(y), "r"(z), "r"(w)
-               : "memory");
-}
-
 // 2-D tile load into own smem whose completion is signalled on the barrier of the
 // pair-leader CTA (`leader_bar` is a cluster-window address).
 __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map,

@@ -413,7 +413,8 @@ int64_t dsa_dense_indexer_workspace_size(int64_t batch, int64_t s1, int64_t s2, 
  * Outputs: out [batch][s1][n1][d]; softmax_max / softmax_sum [batch][s1][n1] fp32 (both NULL
  * to skip) as in dsa_sfa_fwd; rows without keys get zeros.  The result does not depend on
  * timing: the parts of a split row are joined in one order.
- * Workspace: dsa_attn_paged_workspace_size() bytes (for the current device), 16-byte aligned.
+ * out and workspace (dsa_attn_paged_workspace_size() bytes for the current device) are 32-byte
+ * aligned.
  */
 typedef struct DsaAttnPagedParams {
   const void* query;
