@@ -8,8 +8,11 @@
 // that state and write a new one, so nothing waits for the host and a call can be captured;
 // the page data is moved in place.  Pages are handed out lowest id first.
 //
-// A call is two launches: page_plan_kernel (one block) finds the pages with prefix sums over
-// ref_counts, page_apply_kernel (the whole GPU) writes the new table and moves the data.
+// A call is two launches: page_plan_kernel finds the pages, page_apply_kernel writes the new table
+// and moves the data, both over the whole GPU.  What the plan needs in order (which free page is
+// the k-th) is one block's work: it makes a bit per page of ref_counts (read once, eight loads a
+// thread in flight) and ranks the pages by prefix sums over the bits' counts; the other blocks
+// copy the counts meanwhile.
 #include <cuda_runtime.h>
 
 #include "dsa_b200.h"
@@ -23,6 +26,7 @@ namespace pages {
 // append
 // ---------------------------------------------------------------------------------------
 constexpr int kAppendThreads = 256;
+constexpr int kInFlight = 4;   // pieces of a lane that are loaded before any is stored
 
 struct AppendArgs {
   DsaCacheRows e[DSA_APPEND_MAX_ENTRIES];
@@ -32,75 +36,92 @@ struct AppendArgs {
   const int32_t* counts;
   const float* table;
   int* error_flag;
-  int64_t token0;
-  uint32_t items, units;
-  int32_t entries, s, page_size, max_blocks, num_pages, max_positions, dim;
+  int64_t tokens;
+  rotary::FastDiv page;
+  uint32_t units;
+  int32_t entries, s, max_blocks, num_pages, max_positions, dim;
 };
 
-// One 16-byte piece of a token's rows (a pair of pieces in the half layout) per thread.
+// The rotation of one piece (in the half layout of a pair of pieces, `v` and `w`) at value `in`
+// of the rotated part.
 template <typename T>
-__device__ __forceinline__ void append_piece(const AppendArgs& a, const DsaCacheRows& e, const char* src,
-                                             char* dst, int u, int pos) {
+__device__ __forceinline__ void turn_piece(const AppendArgs& a, bool pair, int64_t pos, int in, uint4& v, uint4& w) {
   constexpr int kN = rotary::Vec<T>::kN;
-  const int half = a.dim / 2;
-  const float* row = a.table + (int64_t)pos * a.dim;
-  if (e.rotary == DSA_ROTARY_INTERLEAVED) {
-    const int at = u * kN, in = at - e.offset;
-    uint4 v = *reinterpret_cast<const uint4*>(src + at * sizeof(T));
-    if (in >= 0 && in < a.dim) {
-      float cs[kN / 2], sn[kN / 2];
-      rotary::load_angles<kN / 2>(row, half, in / 2, 1.0f, cs, sn);
-      v = rotary::turn_interleaved<T>(v, cs, sn);
-    }
-    *reinterpret_cast<uint4*>(dst + at * sizeof(T)) = v;
-    return;
-  }
-  const int pairs = half / kN;
-  if (u < pairs) {
-    const int at = e.offset + u * kN;
-    uint4 lo = *reinterpret_cast<const uint4*>(src + at * sizeof(T));
-    uint4 hi = *reinterpret_cast<const uint4*>(src + (at + half) * sizeof(T));
+  const float* row = a.table + pos * a.dim;
+  if (!pair) {
+    float cs[kN / 2], sn[kN / 2];
+    rotary::load_angles<kN / 2>(row, a.dim / 2, in / 2, 1.0f, cs, sn);
+    v = rotary::turn_interleaved<T>(v, cs, sn);
+  } else {
     float cs[kN], sn[kN];
-    rotary::load_angles<kN>(row, half, u * kN, 1.0f, cs, sn);
-    rotary::turn_half<T>(lo, hi, cs, sn);
-    *reinterpret_cast<uint4*>(dst + at * sizeof(T)) = lo;
-    *reinterpret_cast<uint4*>(dst + (at + half) * sizeof(T)) = hi;
-    return;
+    rotary::load_angles<kN>(row, a.dim / 2, in, 1.0f, cs, sn);
+    rotary::turn_half<T>(v, w, cs, sn);
   }
-  int at = (u - pairs) * kN;
-  if (at >= e.offset) at += a.dim;
-  *reinterpret_cast<uint4*>(dst + at * sizeof(T)) = *reinterpret_cast<const uint4*>(src + at * sizeof(T));
 }
 
+// A warp per token: its rows are read while its page is looked up, kInFlight pieces a lane.
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ AppendArgs a) {
-  const uint32_t item = blockIdx.x * kAppendThreads + threadIdx.x;
-  if (item >= a.items) return;
-  const uint32_t tok = item / a.units, u = item - tok * a.units;
-  const int64_t token = a.token0 + tok, b = token / a.s;
+  const int lane = threadIdx.x & 31;
+  const int64_t token = (int64_t)blockIdx.x * (kAppendThreads / 32) + (threadIdx.x >> 5);
+  if (token >= a.tokens) return;
+  const int64_t b = token / a.s;
   const int s = (int)(token - b * a.s);
+  const int32_t start = a.starts[b];
   if (a.counts && s >= a.counts[b]) return;
-  const int64_t pos = (int64_t)a.starts[b] + s;
+  const int64_t pos = (int64_t)start + s;
+  // (pages and positions are below 2^31, as the host has seen to)
+  const uint32_t block = pos >= 0 && pos < (1LL << 31) - 1 ? a.page.div((uint32_t)pos) : (uint32_t)a.max_blocks;
   int32_t page = -1;
-  if (pos >= 0 && pos < (int64_t)a.max_blocks * a.page_size)
-    page = a.block_table[b * a.max_blocks + pos / a.page_size];
-  if (page < 0 || page >= a.num_pages || (a.table && pos >= a.max_positions)) {
-    if (u == 0) report_error(a.error_flag, kErrBadIndex);
-    return;
+  if (block < (uint32_t)a.max_blocks) page = a.block_table[b * a.max_blocks + block];
+  for (uint32_t u0 = lane; u0 < a.units; u0 += 32 * kInFlight) {
+    uint4 v[kInFlight], w[kInFlight];
+    int at[kInFlight], entry[kInFlight];   // byte offset in the row; w is `half` bytes further
+#pragma unroll
+    for (int k = 0; k < kInFlight; ++k) {
+      const uint32_t u = u0 + 32 * k;
+      if (u >= a.units) break;
+      int i = 0;
+      while (i + 1 < a.entries && u >= a.first[i + 1]) ++i;
+      const DsaCacheRows& e = a.e[i];
+      entry[k] = i;
+      int in = (int)(u - a.first[i]) * 16;
+      const char* src = static_cast<const char*>(e.src) + b * e.src_batch_stride + s * e.src_token_stride;
+      if (e.rotary == DSA_ROTARY_HALF) {
+        const int size = e.dtype == DSA_DTYPE_FP32 ? 4 : 2, half = a.dim / 2 * size, off = (int)e.offset * size;
+        if (in < half) {   // the first pieces are pairs
+          in += off;
+          w[k] = *reinterpret_cast<const uint4*>(src + in + half);
+        } else {           // then come the copied ones, around the rotated part
+          in -= half;
+          if (in >= off) in += 2 * half;
+        }
+      }
+      at[k] = in;
+      v[k] = *reinterpret_cast<const uint4*>(src + in);
+    }
+    if (page < 0 || page >= a.num_pages || (a.table && pos >= a.max_positions)) {
+      if (lane == 0) report_error(a.error_flag, kErrBadIndex);
+      return;
+    }
+    const uint32_t row = (uint32_t)pos - block * a.page.d;
+#pragma unroll
+    for (int k = 0; k < kInFlight; ++k) {
+      if (u0 + 32 * k >= a.units) break;
+      const DsaCacheRows& e = a.e[entry[k]];
+      char* dst = static_cast<char*>(e.cache) + page * e.page_stride + row * e.row_stride + at[k];
+      if (e.rotary != DSA_ROTARY_NONE) {
+        const int size = e.dtype == DSA_DTYPE_FP32 ? 4 : 2, in = at[k] / size - (int)e.offset;
+        const bool pair = e.rotary == DSA_ROTARY_HALF;
+        if (in >= 0 && in < (pair ? a.dim / 2 : a.dim)) {
+          if (e.dtype == DSA_DTYPE_BF16) turn_piece<__nv_bfloat16>(a, pair, pos, in, v[k], w[k]);
+          else if (e.dtype == DSA_DTYPE_FP16) turn_piece<__half>(a, pair, pos, in, v[k], w[k]);
+          else turn_piece<float>(a, pair, pos, in, v[k], w[k]);
+          if (pair) *reinterpret_cast<uint4*>(dst + a.dim / 2 * size) = w[k];
+        }
+      }
+      *reinterpret_cast<uint4*>(dst) = v[k];
+    }
   }
-  int i = 0;
-  while (i + 1 < a.entries && u >= a.first[i + 1]) ++i;
-  const DsaCacheRows& e = a.e[i];
-  const int in = (int)(u - a.first[i]);
-  const char* src = static_cast<const char*>(e.src) + b * e.src_batch_stride + s * e.src_token_stride;
-  char* dst = static_cast<char*>(e.cache) + page * e.page_stride + (pos % a.page_size) * e.row_stride;
-  if (e.rotary == DSA_ROTARY_NONE)
-    reinterpret_cast<uint4*>(dst)[in] = reinterpret_cast<const uint4*>(src)[in];
-  else if (e.dtype == DSA_DTYPE_BF16)
-    append_piece<__nv_bfloat16>(a, e, src, dst, in, (int)pos);
-  else if (e.dtype == DSA_DTYPE_FP16)
-    append_piece<__half>(a, e, src, dst, in, (int)pos);
-  else
-    append_piece<float>(a, e, src, dst, in, (int)pos);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -126,7 +147,9 @@ struct PoolArgs {
   int32_t* mark;           // [slots] fork: the fork that makes the row; free: 1; extend: first page
   int32_t* list_a;         // source pages (compact, fork), free pages (extend)
   int32_t* list_b;         // destination pages (compact, fork)
-  int32_t* list_c;         // rows of the page that a fork copies; compact: new id of each page
+  int32_t* list_c;         // rows of the page that a fork copies; compact: new id of
+                           // each page that moves
+  uint32_t* bits;          // a bit per page, where they are too many for shared memory
   int32_t op, n, slots, max_blocks, num_pages, page_size;
 };
 
@@ -152,74 +175,91 @@ __device__ __forceinline__ int plan_scan(int v, int* tmp, int* total) {
   return before + x - v;
 }
 
-// Calls f(page, rank) for the pages that `pick` takes, ranked by id, up to `limit` of them;
-// returns how many there are.  Each warp takes a run of ids.
-template <typename Pick, typename F>
-__device__ int rank_pages(int num_pages, int limit, int* tmp, Pick pick, F f) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int run = ((num_pages + kPlanWarps * 32 - 1) / (kPlanWarps * 32)) * 32;
-  const int from = min(num_pages, warp * run), to = min(num_pages, from + run);
-  int count = 0;
-#pragma unroll 8
-  for (int p = from + lane; p < to; p += 32) count += pick(p) ? 1 : 0;
-  count = __reduce_add_sync(0xffffffffu, count);
-  int total;
-  const int at = plan_scan(lane == 0 ? count : 0, tmp, &total);
-  int rank = __shfl_sync(0xffffffffu, at, 0);
-  for (int p0 = from; p0 < to && rank < limit; p0 += 32) {
-    const int p = p0 + lane;
-    const bool yes = p < to && pick(p);
-    const uint32_t m = __ballot_sync(0xffffffffu, yes);
-    const int r = rank + __popc(m & ((1u << lane) - 1u));
-    if (yes && r < limit) f(p, r);
-    rank += __popc(m);
-  }
-  return total;
-}
-
 __device__ __forceinline__ int blocks_of(int64_t tokens, int page_size) {
   return (int)((tokens + page_size - 1) / page_size);
+}
+
+constexpr int kBitWords = 4096;   // pages / 32 that are held in shared memory; more in the workspace
+
+// A bit per page: whether it is free.
+__device__ __forceinline__ void free_bits(const int32_t* __restrict__ refs, int num_pages, uint32_t* bits) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int p0 = warp * 256; p0 < num_pages; p0 += kPlanWarps * 256) {
+    int r[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int p = p0 + 32 * k + lane;
+      r[k] = p < num_pages ? __ldg(refs + p) : 1;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t m = __ballot_sync(0xffffffffu, r[k] <= 0);
+      if (lane == 0 && p0 + 32 * k < num_pages) bits[p0 / 32 + k] = m;
+    }
+  }
+  __syncthreads();
+}
+
+// Calls f(page, rank) for the first `limit` of the pages whose bit of word(i) is set, ranked by
+// id; returns how many there are.
+template <typename Word, typename F>
+__device__ int rank_pages(int num_pages, int limit, int* tmp, Word word, F f) {
+  const int words = (num_pages + 31) / 32;
+  int before = 0;
+  for (int w0 = 0; w0 < words; w0 += kPlanThreads) {
+    const int w = w0 + threadIdx.x;
+    uint32_t m = w < words ? word(w) : 0u;
+    int sum;
+    int rank = before + plan_scan(__popc(m), tmp, &sum);
+    for (; m && rank < limit; ++rank, m &= m - 1) f(32 * w + __ffs(m) - 1, rank);
+    before += sum;
+  }
+  return before;
 }
 
 __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PoolArgs a) {
   __shared__ int tmp[kPlanWarps];
   __shared__ int run_total;
+  __shared__ uint32_t bit_room[kBitWords];
   const int tid = threadIdx.x;
   griddep_launch_dependents();
+  if (blockIdx.x > 0) {
+    // the counts go over as they are; what changes is counted in by the apply kernel
+    const int stride = (gridDim.x - 1) * kPlanThreads;
+    for (int p = (blockIdx.x - 1) * kPlanThreads + tid; p < a.num_pages; p += stride) a.refs_out[p] = a.refs[p];
+    return;
+  }
   if (tid == 0) a.header[0] = 0;
-  auto is_free = [&](int p) { return a.refs[p] <= 0; };
   bool bad = false, full = false;
+  uint32_t* bits = a.num_pages <= 32 * kBitWords ? bit_room : a.bits;
+  if (a.op != DSA_PAGES_FREE) free_bits(a.refs, a.num_pages, bits);
+  auto free_word = [&](int w) { return bits[w]; };
 
   if (a.op == DSA_PAGES_COMPACT) {
     // live pages beyond the first n_live ids move, in order, to the free ids among those
-    int live = 0;
-    for (int p = tid; p < a.num_pages; p += kPlanThreads) {
-      a.list_c[p] = p;
-      const int r = a.refs[p];
-      a.refs_out[p] = r;
-      live += r > 0 ? 1 : 0;
-    }
-    int total;
-    plan_scan(live, tmp, &total);
-    const int n_live = total;
-    __syncthreads();
+    const int n_live = a.num_pages - rank_pages(a.num_pages, 0, tmp, free_word, [](int, int) {});
+    auto below = [&](int w) {   // bits of word w whose id is below n_live
+      const int n = n_live - 32 * w;
+      return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
+    };
+    auto valid = [&](int w) {
+      const int n = a.num_pages - 32 * w;
+      return n >= 32 ? 0xffffffffu : (1u << n) - 1u;
+    };
     const int moved = rank_pages(a.num_pages, a.num_pages, tmp,
-                                 [&](int p) { return p >= n_live && a.refs[p] > 0; },
+                                 [&](int w) { return ~bits[w] & ~below(w) & valid(w); },
                                  [&](int p, int r) { a.list_a[r] = p; });
-    rank_pages(a.num_pages, a.num_pages, tmp, [&](int p) { return p < n_live && a.refs[p] <= 0; },
+    rank_pages(a.num_pages, a.num_pages, tmp, [&](int w) { return bits[w] & below(w); },
                [&](int p, int r) { a.list_b[r] = p; });
     __syncthreads();
-    for (int i = tid; i < moved; i += kPlanThreads) {
-      const int from = a.list_a[i], to = a.list_b[i];
-      a.list_c[from] = to;
-      a.refs_out[to] = a.refs[from];
-      a.refs_out[from] = 0;
+    for (int i = tid; i < moved; i += kPlanThreads) a.list_c[a.list_a[i]] = a.list_b[i];
+    if (tid == 0) {
+      a.header[0] = moved;
+      a.header[1] = n_live;
     }
-    if (tid == 0) a.header[0] = moved;
     return;
   }
 
-  for (int p = tid; p < a.num_pages; p += kPlanThreads) a.refs_out[p] = a.refs[p];
   if (a.op == DSA_PAGES_FREE) {
     for (int r = tid; r < a.slots; r += kPlanThreads) a.mark[r] = 0;
     __syncthreads();
@@ -232,7 +272,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PoolArgs 
     // row r grows to lens + counts tokens; the pages it needs are a run of the free ones
     if (tid == 0) run_total = 0;
     __syncthreads();
-    const int free_pages = rank_pages(a.num_pages, a.num_pages, tmp, is_free,
+    const int free_pages = rank_pages(a.num_pages, a.num_pages, tmp, free_word,
                                       [&](int p, int r) { a.list_a[r] = p; });
     for (int r0 = 0; r0 < a.slots; r0 += kPlanThreads) {
       const int r = r0 + tid;
@@ -254,8 +294,6 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PoolArgs 
         grows = grows && fits;
         a.lens_out[r] = (int)(grows ? len + more : len);
         a.mark[r] = at;
-        if (grows)
-          for (int j = 0; j < need; ++j) a.refs_out[a.list_a[at + j]] = 1;
       }
       __syncthreads();
       if (tid == 0) run_total += sum;
@@ -280,7 +318,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PoolArgs 
       else bad = true;
     }
     __syncthreads();
-    const int free_pages = rank_pages(a.num_pages, min(a.n, a.num_pages), tmp, is_free,
+    const int free_pages = rank_pages(a.num_pages, min(a.n, a.num_pages), tmp, free_word,
                                       [&](int p, int r) { a.list_b[r] = p; });
     __syncthreads();
     for (int i0 = 0; i0 < a.n; i0 += kPlanThreads) {
@@ -300,7 +338,6 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PoolArgs 
           const int parent = a.first[i];
           a.list_a[at] = a.table[(int64_t)parent * a.max_blocks + a.lens[parent] / a.page_size];
           a.list_c[at] = rest;
-          a.refs_out[a.list_b[at]] = 1;
         } else {
           full = true;
           a.mark[child] = -1;   // no page left: the child stays empty
@@ -356,54 +393,86 @@ __device__ __forceinline__ void copy_slice(const DsaPageCache& c, int sl, int64_
 __global__ void __launch_bounds__(kApplyThreads)
     page_apply_kernel(const PoolArgs a, const __grid_constant__ Caches caches, int do_table) {
   griddep_wait();
-  const int64_t stride = (int64_t)gridDim.x * kApplyThreads;
-  const int64_t me = (int64_t)blockIdx.x * kApplyThreads + threadIdx.x;
   if (do_table && a.op != DSA_PAGES_COPY) {
-    const int64_t cells = (int64_t)a.slots * a.max_blocks;
-    for (int64_t i = me; i < cells; i += stride) {
-      const int row = (int)(i / a.max_blocks), j = (int)(i - (int64_t)row * a.max_blocks);
-      int v = a.table[i];
+    // a warp per row, or per kRowPiece entries of it
+    constexpr int kRowPiece = 1024;
+    const int lane = threadIdx.x & 31;
+    const int warps = gridDim.x * (kApplyThreads / 32), me = blockIdx.x * (kApplyThreads / 32) + (threadIdx.x >> 5);
+    const int per_row = (a.max_blocks + kRowPiece - 1) / kRowPiece;
+    const int moved = a.op == DSA_PAGES_COMPACT ? a.header[0] : 0;
+    const int n_live = a.op == DSA_PAGES_COMPACT ? a.header[1] : 0;
+    for (int64_t i = me * 32 + lane; i < moved; i += (int64_t)warps * 32) {
+      const int from = a.list_a[i];
+      a.refs_out[a.list_b[i]] = a.refs[from];
+      a.refs_out[from] = 0;
+    }
+    for (int64_t task = me; task < (int64_t)a.slots * per_row; task += warps) {
+      const int row = (int)(task / per_row), j0 = (int)(task - (int64_t)row * per_row) * kRowPiece;
+      const int end = min(j0 + kRowPiece, a.max_blocks);
+      const int32_t* in = a.table + (int64_t)row * a.max_blocks;
+      int32_t* out = a.table_out + (int64_t)row * a.max_blocks;
       if (a.op == DSA_PAGES_COMPACT) {
-        if (v >= 0 && v < a.num_pages) v = a.list_c[v];
-      } else if (a.op == DSA_PAGES_FREE) {
-        if (a.mark[row]) {
-          if (v >= 0 && v < a.num_pages) {
-            // a page held more often than it is counted was free already: it stays at 0
-            if (atomicSub(&a.refs_out[v], 1) <= 0) {
-              atomicAdd(&a.refs_out[v], 1);
-              report_error(a.error_flag, kErrBadIndex);
-            }
-          } else if (v >= a.num_pages) {
-            report_error(a.error_flag, kErrBadIndex);
-          }
-          v = -1;
+#pragma unroll 4
+        for (int j = j0 + lane; j < end; j += 32) {
+          int v = in[j];
+          if (v >= n_live && v < a.num_pages && a.refs[v] > 0) v = a.list_c[v];
+          out[j] = v;
         }
-        if (j == 0) a.lens_out[row] = a.mark[row] ? 0 : a.lens[row];
+      } else if (a.op == DSA_PAGES_FREE) {
+        const bool gone = a.mark[row] != 0;
+        if (j0 == 0 && lane == 0) a.lens_out[row] = gone ? 0 : a.lens[row];
+#pragma unroll 4
+        for (int j = j0 + lane; j < end; j += 32) {
+          const int v = in[j];
+          out[j] = gone ? -1 : v;
+          if (!gone || v < 0) continue;
+          // a page held more often than it is counted was free already: it stays at 0
+          bool wrong = v >= a.num_pages;
+          if (!wrong && atomicSub(&a.refs_out[v], 1) <= 0) {
+            atomicAdd(&a.refs_out[v], 1);
+            wrong = true;
+          }
+          if (wrong) report_error(a.error_flag, kErrBadIndex);
+        }
       } else if (a.op == DSA_PAGES_EXTEND) {
         const int had = blocks_of(a.lens[row], a.page_size), has = blocks_of(a.lens_out[row], a.page_size);
-        if (j >= had && j < has) v = a.list_a[a.mark[row] + j - had];
+        const int32_t* fresh = a.list_a + a.mark[row] - had;
+#pragma unroll 4
+        for (int j = j0 + lane; j < end; j += 32) {
+          int v = in[j];
+          if (j >= had && j < has) {
+            v = fresh[j];
+            a.refs_out[v] = 1;
+          }
+          out[j] = v;
+        }
       } else {   // fork
         const int f = a.mark[row];
         const bool child = f >= 0 && f < a.n;
-        const int len = child ? a.lens[a.first[f]] : a.lens[row];
-        if (child) {
-          const int full = len / a.page_size;
-          v = -1;
-          if (j < full) {
-            v = a.table[(int64_t)a.first[f] * a.max_blocks + j];
+        const int parent = child ? a.first[f] : row, len = a.lens[parent];
+        const int full = len / a.page_size;
+        if (j0 == 0 && lane == 0) a.lens_out[row] = len;
+        const int32_t* from = a.table + (int64_t)parent * a.max_blocks;
+#pragma unroll 4
+        for (int j = j0 + lane; j < end; j += 32) {
+          int v = from[j];
+          if (child && j < full) {
             if (v >= 0 && v < a.num_pages) {
               atomicAdd(&a.refs_out[v], 1);
             } else {   // the parent has no such page: neither has the child
               report_error(a.error_flag, kErrBadIndex);
               v = -1;
             }
-          } else if (j == full && len % a.page_size) {
-            v = a.list_b[a.header[8 + f]];
+          } else if (child) {
+            v = -1;
+            if (j == full && len % a.page_size) {
+              v = a.list_b[a.header[8 + f]];
+              a.refs_out[v] = 1;
+            }
           }
+          out[j] = v;
         }
-        if (j == 0) a.lens_out[row] = len;
       }
-      a.table_out[i] = v;
     }
   }
   if (caches.count == 0) return;
@@ -479,29 +548,26 @@ extern "C" int dsa_cache_append(const DsaCacheAppendParams* p, void* stream_) {
   a.table = p->table;
   a.error_flag = p->error_flag;
   a.units = units;
+  a.tokens = p->batch * p->s;
+  a.page = dsa::rotary::FastDiv((uint32_t)p->page_size);
   a.entries = p->entries;
   a.s = (int)p->s;
-  a.page_size = (int)p->page_size;
   a.max_blocks = (int)p->max_blocks;
   a.num_pages = (int)p->num_pages;
   a.max_positions = (int)p->max_positions;
   a.dim = (int)p->dim;
-  const int64_t tokens = p->batch * p->s, chunk = (1LL << 30) / units;
-  for (int64_t t0 = 0; t0 < tokens; t0 += chunk) {
-    const int64_t n = tokens - t0 < chunk ? tokens - t0 : chunk;
-    a.token0 = t0;
-    a.items = (uint32_t)(n * units);
-    append_kernel<<<(a.items + kAppendThreads - 1) / kAppendThreads, kAppendThreads, 0, stream>>>(a);
-    if (cudaGetLastError() != cudaSuccess) return DSA_ERR_CUDA;
-  }
-  return DSA_OK;
+  const int64_t blocks = (a.tokens + kAppendThreads / 32 - 1) / (kAppendThreads / 32);
+  if (blocks > kMax) return DSA_ERR_INVALID_ARG;
+  append_kernel<<<(unsigned)blocks, kAppendThreads, 0, stream>>>(a);
+  return cudaGetLastError() == cudaSuccess ? DSA_OK : DSA_ERR_CUDA;
 }
 
 extern "C" int64_t dsa_pages_workspace_size(int32_t op, int64_t n, int64_t slots, int64_t num_pages) {
   using namespace dsa::pages;
   if (n < 0 || slots < 0 || num_pages < 0) return -1;
   if (op == DSA_PAGES_COPY) return 0;
-  return 4 * (align64(8 + (op == DSA_PAGES_FORK ? n : 0)) + align64(slots) + 3 * align64(num_pages));
+  return 4 * (align64(8 + (op == DSA_PAGES_FORK ? n : 0)) + align64(slots) + 3 * align64(num_pages) +
+              align64(num_pages / 32 + 1));
 }
 
 extern "C" int dsa_pages(const DsaPagesParams* p, void* stream_) {
@@ -544,6 +610,7 @@ extern "C" int dsa_pages(const DsaPagesParams* p, void* stream_) {
     a.list_a = ws;
     a.list_b = ws + align64(p->num_pages);
     a.list_c = ws + 2 * align64(p->num_pages);
+    a.bits = reinterpret_cast<uint32_t*>(ws + 3 * align64(p->num_pages));
   }
   a.op = p->op;
   a.n = (int)p->n;
@@ -554,7 +621,8 @@ extern "C" int dsa_pages(const DsaPagesParams* p, void* stream_) {
   const int sms = dsa::sm_count();
   if (sms < 1) return DSA_ERR_CUDA;
   if (!copy) {
-    page_plan_kernel<<<1, kPlanThreads, 0, stream>>>(a);
+    const int64_t copy_blocks = (p->num_pages + 4 * kPlanThreads - 1) / (4 * kPlanThreads);
+    page_plan_kernel<<<1 + (unsigned)(copy_blocks < 64 ? copy_blocks : 64), kPlanThreads, 0, stream>>>(a);
     if (cudaGetLastError() != cudaSuccess) return DSA_ERR_CUDA;
   }
   cudaLaunchAttribute pdl[1];
@@ -569,7 +637,7 @@ extern "C" int dsa_pages(const DsaPagesParams* p, void* stream_) {
     }
     int64_t blocks = (int64_t)sms * 8;
     if (c.count == 0) {
-      const int64_t need = (p->slots * p->max_blocks + kApplyThreads - 1) / kApplyThreads;
+      const int64_t need = p->slots * ((p->max_blocks + 1023) / 1024) / (kApplyThreads / 32) + 1;
       if (need < blocks) blocks = need;
     }
     cudaLaunchConfig_t cfg = {};

@@ -1,9 +1,10 @@
 // Rotary positions of queries and keys, their gradient, and the table of cosines and sines.
 //
 // rotary_kernel is bound by memory: it reads and writes each value once.  A thread takes one
-// 16-byte piece (in the half layout the two pieces that turn together) of up to kHeads heads
-// of one token, so that the cosines and sines are fetched once for those heads and several
-// loads are in flight.  Neighbouring lanes take neighbouring pieces.
+// 16-byte piece of up to kHeads heads of one token, so that the cosines and sines are fetched
+// once for those heads and several loads are in flight; neighbouring lanes take neighbouring
+// pieces.  In the half layout a piece needs its partner from the other half, which a lane of the
+// same warp holds where a head's pieces divide a warp; else one thread takes both pieces.
 #include <cuda_runtime.h>
 
 #include "dsa_b200.h"
@@ -26,20 +27,32 @@ struct Args {
   int64_t x_batch, x_token, x_head;     // strides in elements
   int64_t o_batch, o_token, o_head;
   uint32_t items;                       // threads with work
-  uint32_t units, head_steps;           // pieces of a head; heads / kHeads, rounded up
-  int32_t s, heads, head_dim, offset, dim, half_layout, max_positions;
+  FastDiv units, head_steps, s;         // pieces of a head; heads / kHeads, rounded up; tokens of a batch
+  int32_t heads, head_dim, offset, dim, half_layout, max_positions;
   float sign;
 };
 
-template <typename T>
+enum { kInterleaved, kHalfShuffle, kHalfBoth };
+
+template <typename T, int kMode>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const Args a) {
-  using V = Vec<T>;
-  constexpr int kN = V::kN;
+  constexpr int kN = Vec<T>::kN;
   const uint32_t item = blockIdx.x * kThreads + threadIdx.x;
-  if (item >= a.items) return;
-  const uint32_t rest = item / a.units, u = item - rest * a.units;
-  const uint32_t tok = rest / a.head_steps, h0 = rest - tok * a.head_steps;
-  const int64_t token = a.token0 + tok, b = token / a.s, s = token - b * a.s;
+  // (the shuffle needs whole warps: lanes past the end repeat the last item and store nothing)
+  const bool live = item < a.items;
+  if (kMode != kHalfShuffle && !live) return;
+  const uint32_t it = live ? item : a.items - 1;
+  const uint32_t rest = a.units.div(it), u = it - rest * a.units.d;
+  const uint32_t tok = a.head_steps.div(rest), h0 = rest - tok * a.head_steps.d;
+  const int64_t token = a.token0 + tok;
+  int64_t b, s;
+  if (token < (1LL << 31)) {
+    b = a.s.div((uint32_t)token);
+    s = token - b * a.s.d;
+  } else {
+    b = token / a.s.d;
+    s = token - b * a.s.d;
+  }
   const T* x = static_cast<const T*>(a.x) + b * a.x_batch + s * a.x_token;
   T* out = static_cast<T*>(a.out) + b * a.o_batch + s * a.o_token;
   const int32_t pos = a.positions[token];
@@ -48,59 +61,67 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const Args a) {
   const int half = a.dim / 2;
   const float* row = a.table + (int64_t)(known ? pos : 0) * a.dim;
   const uint4 zero = make_uint4(0, 0, 0, 0);
+  auto head = [&](int j) { return (int)(h0 + j * a.head_steps.d); };
 
-  if (!a.half_layout) {
-    const int at = (int)u * kN, in = at - a.offset;
-    const bool turned = in >= 0 && in < a.dim;
-    uint4 v[kHeads];
+  if constexpr (kMode == kHalfBoth) {
+    // the first dim / (2 kN) pieces are pairs, the others are copied
+    const int pairs = half / kN;
+    const bool pair = (int)u < pairs;
+    int at = pair ? a.offset + (int)u * kN : ((int)u - pairs) * kN;
+    if (!pair && at >= a.offset) at += a.dim;
+    uint4 lo[kHeads], hi[kHeads];
 #pragma unroll
     for (int j = 0; j < kHeads; ++j) {
-      const int h = h0 + j * a.head_steps;
-      if (h < a.heads) v[j] = *reinterpret_cast<const uint4*>(x + h * a.x_head + at);
+      if (head(j) >= a.heads) continue;
+      lo[j] = __ldcs(reinterpret_cast<const uint4*>(x + head(j) * a.x_head + at));
+      if (pair) hi[j] = __ldcs(reinterpret_cast<const uint4*>(x + head(j) * a.x_head + at + half));
     }
+    float cs[kN], sn[kN];
+    if (pair) load_angles<kN>(row, half, (int)u * kN, a.sign, cs, sn);
+#pragma unroll
+    for (int j = 0; j < kHeads; ++j) {
+      if (head(j) >= a.heads) continue;
+      if (pair) {
+        turn_half<T>(lo[j], hi[j], cs, sn);
+        __stcs(reinterpret_cast<uint4*>(out + head(j) * a.o_head + at + half), known ? hi[j] : zero);
+      }
+      __stcs(reinterpret_cast<uint4*>(out + head(j) * a.o_head + at), known ? lo[j] : zero);
+    }
+    return;
+  }
+
+  const int at = (int)u * kN, in = at - a.offset;
+  const bool turned = in >= 0 && in < a.dim;
+  uint4 v[kHeads];
+#pragma unroll
+  for (int j = 0; j < kHeads; ++j)
+    if (head(j) < a.heads) v[j] = __ldcs(reinterpret_cast<const uint4*>(x + head(j) * a.x_head + at));
+  if constexpr (kMode == kInterleaved) {
     float cs[kN / 2], sn[kN / 2];
     if (turned) load_angles<kN / 2>(row, half, in / 2, a.sign, cs, sn);
 #pragma unroll
     for (int j = 0; j < kHeads; ++j) {
-      const int h = h0 + j * a.head_steps;
-      if (h >= a.heads) continue;
+      if (head(j) >= a.heads) continue;
       if (turned) v[j] = turn_interleaved<T>(v[j], cs, sn);
-      *reinterpret_cast<uint4*>(out + h * a.o_head + at) = known ? v[j] : zero;
+      __stcs(reinterpret_cast<uint4*>(out + head(j) * a.o_head + at), known ? v[j] : zero);
     }
-    return;
-  }
-  // half layout: the first dim / (2 kN) pieces are pairs, the others are copied
-  const int pairs = half / kN;
-  if ((int)u < pairs) {
-    const int in = (int)u * kN, at = a.offset + in;
-    uint4 lo[kHeads], hi[kHeads];
-#pragma unroll
-    for (int j = 0; j < kHeads; ++j) {
-      const int h = h0 + j * a.head_steps;
-      if (h >= a.heads) continue;
-      lo[j] = *reinterpret_cast<const uint4*>(x + h * a.x_head + at);
-      hi[j] = *reinterpret_cast<const uint4*>(x + h * a.x_head + at + half);
-    }
+  } else {
+    const bool second = in >= half;
+    const int lane = threadIdx.x & 31, partner = turned ? (second ? lane - half / kN : lane + half / kN) : lane;
     float cs[kN], sn[kN];
-    load_angles<kN>(row, half, in, a.sign, cs, sn);
+    if (turned) load_angles<kN>(row, half, second ? in - half : in, a.sign, cs, sn);
 #pragma unroll
     for (int j = 0; j < kHeads; ++j) {
-      const int h = h0 + j * a.head_steps;
-      if (h >= a.heads) continue;
-      turn_half<T>(lo[j], hi[j], cs, sn);
-      *reinterpret_cast<uint4*>(out + h * a.o_head + at) = known ? lo[j] : zero;
-      *reinterpret_cast<uint4*>(out + h * a.o_head + at + half) = known ? hi[j] : zero;
+      // a warp's lanes are whole heads of up to 32 head steps, so all of a head's lanes have it
+      uint4 w;
+      w.x = __shfl_sync(0xffffffffu, v[j].x, partner);
+      w.y = __shfl_sync(0xffffffffu, v[j].y, partner);
+      w.z = __shfl_sync(0xffffffffu, v[j].z, partner);
+      w.w = __shfl_sync(0xffffffffu, v[j].w, partner);
+      if (!live || head(j) >= a.heads) continue;
+      if (turned) v[j] = turn_half_one<T>(v[j], w, second, cs, sn);
+      __stcs(reinterpret_cast<uint4*>(out + head(j) * a.o_head + at), known ? v[j] : zero);
     }
-    return;
-  }
-  int at = ((int)u - pairs) * kN;
-  if (at >= a.offset) at += a.dim;
-#pragma unroll
-  for (int j = 0; j < kHeads; ++j) {
-    const int h = h0 + j * a.head_steps;
-    if (h >= a.heads) continue;
-    const uint4 v = *reinterpret_cast<const uint4*>(x + h * a.x_head + at);
-    *reinterpret_cast<uint4*>(out + h * a.o_head + at) = known ? v : zero;
   }
 }
 
@@ -109,9 +130,9 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads) rotary_any_kernel(const Args a) {
   const uint32_t item = blockIdx.x * kThreads + threadIdx.x;
   if (item >= a.items) return;
-  const uint32_t rest = item / a.units, u = item - rest * a.units;
-  const uint32_t tok = rest / a.heads, h = rest - tok * a.heads;
-  const int64_t token = a.token0 + tok, b = token / a.s, s = token - b * a.s;
+  const uint32_t rest = a.units.div(item), u = item - rest * a.units.d;
+  const uint32_t tok = a.head_steps.div(rest), h = rest - tok * a.head_steps.d;
+  const int64_t token = a.token0 + tok, b = token / a.s.d, s = token - b * a.s.d;
   const T* x = static_cast<const T*>(a.x) + b * a.x_batch + s * a.x_token + h * a.x_head;
   T* out = static_cast<T*>(a.out) + b * a.o_batch + s * a.o_token + h * a.o_head;
   const int32_t pos = a.positions[token];
@@ -172,7 +193,7 @@ int launch(const DsaRotaryParams* p, cudaStream_t stream) {
   a.error_flag = p->error_flag;
   a.x_batch = p->x_batch_stride, a.x_token = p->x_token_stride, a.x_head = p->x_head_stride;
   a.o_batch = p->out_batch_stride, a.o_token = p->out_token_stride, a.o_head = p->out_head_stride;
-  a.s = (int)p->s;
+  a.s = FastDiv((uint32_t)p->s);
   a.heads = (int)p->heads;
   a.head_dim = (int)p->head_dim;
   a.offset = (int)p->offset;
@@ -187,23 +208,30 @@ int launch(const DsaRotaryParams* p, cudaStream_t stream) {
              reinterpret_cast<uintptr_t>(p->table) % 16 == 0 && p->dim % 8 == 0;
   for (int64_t st : {a.x_batch, a.x_token, a.x_head, a.o_batch, a.o_token, a.o_head})
     vec = vec && st % kN == 0;
+  uint32_t units, steps;
+  // a warp holds whole heads where a head's pieces divide it
+  const bool shuffle = vec && p->half_layout && 32 % (p->head_dim / kN) == 0;
   if (vec) {
-    a.units = (uint32_t)((p->head_dim - (p->half_layout ? p->dim / 2 : 0)) / kN);
-    a.head_steps = (uint32_t)((p->heads + kHeads - 1) / kHeads);
+    units = (uint32_t)((p->head_dim - (p->half_layout && !shuffle ? p->dim / 2 : 0)) / kN);
+    steps = (uint32_t)((p->heads + kHeads - 1) / kHeads);
   } else {
-    a.units = (uint32_t)(p->head_dim - p->dim / 2);
-    a.head_steps = (uint32_t)p->heads;
+    units = (uint32_t)(p->head_dim - p->dim / 2);
+    steps = (uint32_t)p->heads;
   }
-  const int64_t per_token = (int64_t)a.units * a.head_steps, tokens = p->batch * p->s;
-  const int64_t chunk = (1LL << 30) / per_token > 0 ? (1LL << 30) / per_token : 1;
+  a.units = FastDiv(units);
+  a.head_steps = FastDiv(steps);
+  const int64_t per_token = (int64_t)units * steps, tokens = p->batch * p->s;
   if (per_token > (1LL << 30)) return DSA_ERR_INVALID_ARG;
+  const int64_t chunk = (1LL << 30) / per_token;
   for (int64_t t0 = 0; t0 < tokens; t0 += chunk) {
     const int64_t n = tokens - t0 < chunk ? tokens - t0 : chunk;
     a.token0 = t0;
     a.items = (uint32_t)(n * per_token);
     const unsigned grid = (unsigned)((a.items + kThreads - 1) / kThreads);
-    if (vec) rotary_kernel<T><<<grid, kThreads, 0, stream>>>(a);
-    else rotary_any_kernel<T><<<grid, kThreads, 0, stream>>>(a);
+    if (!vec) rotary_any_kernel<T><<<grid, kThreads, 0, stream>>>(a);
+    else if (!p->half_layout) rotary_kernel<T, kInterleaved><<<grid, kThreads, 0, stream>>>(a);
+    else if (shuffle) rotary_kernel<T, kHalfShuffle><<<grid, kThreads, 0, stream>>>(a);
+    else rotary_kernel<T, kHalfBoth><<<grid, kThreads, 0, stream>>>(a);
     if (cudaGetLastError() != cudaSuccess) return DSA_ERR_CUDA;
   }
   return DSA_OK;

@@ -13,6 +13,21 @@
 namespace dsa {
 namespace rotary {
 
+// n / d for n < 2^31 by a multiplication (Granlund and Montgomery, "Division by invariant
+// integers using multiplication", 1994): with l = ceil(log2 d) and m = floor(2^32 (2^l - d) / d) + 1,
+// n / d = (hi(m n) + n) >> l.
+struct FastDiv {
+  uint32_t d, m, l;
+  FastDiv() = default;
+  explicit FastDiv(uint32_t div) : d(div), m(0), l(0) {
+    while ((1ull << l) < d) ++l;
+    m = (uint32_t)(((1ull << 32) * ((1ull << l) - d)) / d + 1);
+  }
+#ifdef __CUDACC__
+  __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(m, n) + n) >> l; }
+#endif
+};
+
 template <typename T>
 struct Vec {   // 16 bytes of T as fp32 values
   static constexpr int kN = 16 / sizeof(T);
@@ -61,6 +76,22 @@ __device__ __forceinline__ void turn_half(uint4& lo, uint4& hi, const float* cs,
   for (int i = 0; i < Vec<T>::kN; ++i) turn(a[i], b[i], cs[i], sn[i]);
   lo = Vec<T>::pack(a);
   hi = Vec<T>::pack(b);
+}
+
+// kN values of one half (`second`: of the second) given the partners of the other.
+template <typename T>
+__device__ __forceinline__ uint4 turn_half_one(const uint4& own, const uint4& other, bool second,
+                                               const float* cs, const float* sn) {
+  float a[Vec<T>::kN], b[Vec<T>::kN];
+  Vec<T>::unpack(own, a);
+  Vec<T>::unpack(other, b);
+#pragma unroll
+  for (int i = 0; i < Vec<T>::kN; ++i) {
+    float x = second ? b[i] : a[i], y = second ? a[i] : b[i];
+    turn(x, y, cs[i], sn[i]);
+    a[i] = second ? y : x;
+  }
+  return Vec<T>::pack(a);
 }
 
 // `n` (2, 4 or 8) cosines and sines of a table row from pair `i` on, 4-float aligned when n >= 4.
