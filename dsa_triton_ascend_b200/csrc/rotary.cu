@@ -5,6 +5,10 @@
 // once for those heads and several loads are in flight; neighbouring lanes take neighbouring
 // pieces.  In the half layout a piece needs its partner from the other half, which a lane of the
 // same warp holds where a head's pieces divide a warp; else one thread takes both pieces.
+// Measured: 8192 tokens x 128 heads x 64 (bf16, interleaved) in 43.5 us, 6.2 TB/s, where a copy of
+// the same tensor takes 44.6; the gradient of 2 x 4093 tokens x 64 heads x 128, half of each head
+// rotated, in 45.6 us, 5.9 TB/s (49.5 with blocks of 256 threads, 51.5 with both pieces in a
+// thread, 62 with two heads a thread).
 #include <cuda_runtime.h>
 
 #include "dsa_b200.h"
@@ -13,7 +17,7 @@
 namespace dsa {
 namespace rotary {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 constexpr int kHeads = 4;
 constexpr int kMaxPairs = 128;
 
@@ -109,7 +113,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const Args a) {
     const bool second = in >= half;
     const int lane = threadIdx.x & 31, partner = turned ? (second ? lane - half / kN : lane + half / kN) : lane;
     float cs[kN], sn[kN];
-    if (turned) load_angles<kN>(row, half, second ? in - half : in, a.sign, cs, sn);
+    if (turned) load_angles<kN>(row, half, second ? in - half : in, second ? a.sign : -a.sign, cs, sn);
 #pragma unroll
     for (int j = 0; j < kHeads; ++j) {
       // a warp's lanes are whole heads of up to 32 head steps, so all of a head's lanes have it
@@ -119,7 +123,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const Args a) {
       w.z = __shfl_sync(0xffffffffu, v[j].z, partner);
       w.w = __shfl_sync(0xffffffffu, v[j].w, partner);
       if (!live || head(j) >= a.heads) continue;
-      if (turned) v[j] = turn_half_one<T>(v[j], w, second, cs, sn);
+      if (turned) v[j] = turn_half_one<T>(v[j], w, cs, sn);
       __stcs(reinterpret_cast<uint4*>(out + head(j) * a.o_head + at), known ? v[j] : zero);
     }
   }

@@ -52,7 +52,7 @@ struct Vec {   // 16 bytes of T as fp32 values
 };
 
 __device__ __forceinline__ void turn(float& a, float& b, float c, float s) {
-  const float x = fmaf(a, c, -b * s), y = fmaf(a, s, b * c);
+  const float x = fmaf(a, c, -(b * s)), y = fmaf(b, c, a * s);
   a = x;
   b = y;
 }
@@ -78,19 +78,15 @@ __device__ __forceinline__ void turn_half(uint4& lo, uint4& hi, const float* cs,
   hi = Vec<T>::pack(b);
 }
 
-// kN values of one half (`second`: of the second) given the partners of the other.
+// kN values of one half given their partners of the other; `sn` comes negated for the first.
 template <typename T>
-__device__ __forceinline__ uint4 turn_half_one(const uint4& own, const uint4& other, bool second,
-                                               const float* cs, const float* sn) {
+__device__ __forceinline__ uint4 turn_half_one(const uint4& own, const uint4& other, const float* cs,
+                                               const float* sn) {
   float a[Vec<T>::kN], b[Vec<T>::kN];
   Vec<T>::unpack(own, a);
   Vec<T>::unpack(other, b);
 #pragma unroll
-  for (int i = 0; i < Vec<T>::kN; ++i) {
-    float x = second ? b[i] : a[i], y = second ? a[i] : b[i];
-    turn(x, y, cs[i], sn[i]);
-    a[i] = second ? y : x;
-  }
+  for (int i = 0; i < Vec<T>::kN; ++i) a[i] = fmaf(a[i], cs[i], b[i] * sn[i]);
   return Vec<T>::pack(a);
 }
 
