@@ -128,23 +128,7 @@ def self_overlap(t: torch.Tensor) -> bool:
     return False
 
 
-# Host time is most of a small call, so the checks of a call's arguments and what follows from
-# their shapes (strides, sizes, output shapes) are kept per signature, and the raw device and
-# stream handles are asked for without torch's wrapper objects.
-class Plans(dict):
-    """What calls of one signature (shapes, strides, types, devices, options) have in common."""
-
-    def keep(self, key, plan):
-        if len(self) >= 1024:
-            self.clear()
-        self[key] = plan
-        return plan
-
-
-def signature(tensors) -> tuple:
-    return tuple([None if t is None else (t.shape, t.stride(), t.dtype, t.get_device()) for t in tensors])
-
-
+# raw device and stream handles, without torch's wrapper objects
 try:
     from torch._C import _cuda_getCurrentRawStream as raw_stream   # device index -> cudaStream_t
     from torch._C import _cuda_getDevice as current_device

@@ -235,6 +235,29 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+_binding = None
+
+
+def binding():
+    """The compiled path of the serving operators' repeated calls (csrc/binding.cpp), or None
+    where it is not built; the operators' own Python path calls the same entries."""
+    global _binding
+    if _binding is None:
+        _binding = False
+        try:
+            from . import _binding as module
+        except ImportError:
+            return None
+        entries = [ctypes.cast(getattr(lib(), name), ctypes.c_void_p).value
+                   for name in ("dsa_attn_paged", "dsa_rotary", "dsa_cache_append", "dsa_pages")]
+        module.connect(*entries, check)
+        _binding = module
+    return _binding or None
+
+
+BIND_ATTN, BIND_ROTARY, BIND_APPEND, BIND_UPKEEP = range(4)   # Op of csrc/binding.cpp
+
+
 def check(rc: int, what: str) -> None:
     if rc != DSA_OK:
         raise RuntimeError(f"{what}: {_ERR_TEXT.get(rc, 'error')} (code {rc})")
@@ -269,6 +292,8 @@ def report_ptr(index: int) -> int:
     p = _report_ptrs.get(index)
     if p is None:
         p = _report_ptrs[index] = report_flag(torch.device("cuda", index)).data_ptr()
+        if binding() is not None:
+            binding().set_report(index, p)
     return p
 
 

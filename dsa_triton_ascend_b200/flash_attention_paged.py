@@ -11,13 +11,10 @@ from __future__ import annotations
 import torch
 
 from . import _host as H
-from ._lib import AttnPagedParams, check, lib, report_ptr
+from ._lib import BIND_ATTN, AttnPagedParams, binding, check, lib, report_ptr
 
 _VALID_D = (128, 256, 512)
 _D_ROPE = 64
-
-
-_plans = H.Plans()
 
 
 def _tma_strides(t: torch.Tensor):
@@ -114,23 +111,20 @@ def flash_attention_paged(
     zeros when ``return_softmax_lse`` is False.  Strided inputs (views of a joint projection or
     of a joint cache) are read in place.
     """
-    scale_value = float(scale_value)
-    key = (H.signature((query, query_rope, key_cache, key_rope_cache, block_table)), scale_value, sparse_mode)
-    plan = _plans.get(key)
+    args = (query, query_rope, key_cache, key_rope_cache, block_table, actual_seq_lengths_key,
+            actual_seq_lengths_query, float(scale_value), sparse_mode, bool(return_softmax_lse))
+    fast = binding()
+    if fast is not None:
+        done = fast.attn(*args)
+        if done is not None:
+            return done
     index = query.get_device()
-    if plan is None or H.current_device() != index:
-        if plan is None:
-            checked = lambda: _plan(query, query_rope, key_cache, key_rope_cache, block_table, scale_value, sparse_mode)
-            if query.is_cuda:
-                with torch.cuda.device(index):
-                    plan = _plans.keep(key, checked())
-            else:
-                checked()
-        if H.current_device() != index:
-            with torch.cuda.device(index):
-                return flash_attention_paged(query, query_rope, key_cache, key_rope_cache, block_table,
-                                             actual_seq_lengths_key, scale_value, actual_seq_lengths_query,
-                                             sparse_mode, return_softmax_lse)
+    if index >= 0 and H.current_device() != index:
+        with torch.cuda.device(index):
+            return flash_attention_paged(query, query_rope, key_cache, key_rope_cache, block_table,
+                                         actual_seq_lengths_key, scale_value, actual_seq_lengths_query,
+                                         sparse_mode, return_softmax_lse)
+    plan = _plan(query, query_rope, key_cache, key_rope_cache, block_table, float(scale_value), sparse_mode)
     template, q_fits, qr_fits, stat_shape, ws_bytes = plan
     dev = query.device
     B, _, S1, _ = stat_shape
@@ -166,4 +160,7 @@ def flash_attention_paged(
         p.softmax_max, p.softmax_sum = smax.data_ptr(), ssum.data_ptr()
     p.error_flag = report_ptr(index)
     check(lib().dsa_attn_paged(p, H.raw_stream(index)), "dsa_attn_paged")
+    if fast is not None and q is query and qr is query_rope and bt is block_table \
+            and act_k is actual_seq_lengths_key and act_q is actual_seq_lengths_query:
+        fast.keep(BIND_ATTN, *args, template, b"", ws_bytes)
     return out, smax, ssum

@@ -20,9 +20,9 @@ from __future__ import annotations
 import torch
 
 from . import _host as H
-from ._lib import (APPEND_MAX_ENTRIES, DSA_DTYPE_BF16, DSA_DTYPE_FP16, DSA_DTYPE_FP32, PAGES_COMPACT, PAGES_COPY,
+from ._lib import (APPEND_MAX_ENTRIES, BIND_APPEND, BIND_UPKEEP, DSA_DTYPE_BF16, DSA_DTYPE_FP16, DSA_DTYPE_FP32, PAGES_COMPACT, PAGES_COPY,
                    PAGES_EXTEND, PAGES_FORK, PAGES_FREE, ROTARY_CODES, CacheAppendParams, PageCache,
-                   PagesParams, check, lib, ptr, report_ptr)
+                   PagesParams, binding, check, lib, ptr, report_ptr)
 
 _ROTATED = {torch.bfloat16: DSA_DTYPE_BF16, torch.float16: DSA_DTYPE_FP16, torch.float32: DSA_DTYPE_FP32}
 
@@ -75,10 +75,6 @@ def _check_caches(caches, dev, num_pages=None):
     if num_pages is not None and num_pages < 1 or page_size is not None and page_size < 1:
         raise ValueError("the caches must not be empty")
     return num_pages, page_size
-
-
-_append_plans = H.Plans()
-_pool_plans = H.Plans()
 
 
 def _append_plan(tokens, caches, block_table, starts, counts, table, rotary):
@@ -159,13 +155,12 @@ def paged_cache_append(tokens, caches, block_table, starts, counts=None, table=N
     reported.  Rows are whole 16-byte pieces.
     """
     tokens, caches = list(tokens), list(caches)
+    args = (tokens, caches, block_table, starts, counts, table, rotary)
+    fast = binding()
+    if fast is not None and fast.append(*args):
+        return caches
     rotary = [None] * len(tokens) if rotary is None else list(rotary)
-    key = (H.signature(tokens), H.signature(caches), H.signature((block_table, starts, counts, table)),
-           tuple([None if r is None else tuple(r) for r in rotary]))
-    plan = _append_plans.get(key)
-    if plan is None:
-        plan = _append_plans.keep(key, _append_plan(tokens, caches, block_table, starts, counts, table, rotary))
-    template, copy = plan
+    template, copy = _append_plan(tokens, caches, block_table, starts, counts, table, rotary)
     index = caches[0].get_device()
     if H.current_device() != index:
         with torch.cuda.device(index):
@@ -192,6 +187,9 @@ def paged_cache_append(tokens, caches, block_table, starts, counts=None, table=N
     p.block_table, p.starts, p.counts = bt.data_ptr(), st.data_ptr(), ptr(ct)
     p.error_flag = report_ptr(index)
     check(lib().dsa_cache_append(p, H.raw_stream(index)), "dsa_cache_append")
+    if fast is not None and not keep and bt is block_table and st is starts and ct is counts \
+            and (table is args[5] or not p.dim):
+        fast.keep(BIND_APPEND, *args, template, b"", 0)
     return caches
 
 
@@ -248,12 +246,13 @@ def _upkeep(op, caches, block_table=None, seq_lengths=None, ref_counts=None, fir
     """Run one call of ``dsa_pages``; returns the new (block_table, seq_lengths, ref_counts)."""
     page_size = None if page_size is None else int(page_size)
     state = (block_table, seq_lengths, ref_counts)
-    key = (op, H.signature(caches), H.signature(t if torch.is_tensor(t) else None for t in (*state, first, second)),
-           page_size)
-    plan = _pool_plans.get(key)
-    if plan is None:
-        plan = _pool_plans.keep(key, _pool_plan(op, caches, *state, first, second, page_size))
-    template, cache_template, ws_bytes = plan
+    args = (op, caches, *state, first, second, page_size)
+    fast = binding()
+    if fast is not None:
+        done = fast.upkeep(*args)
+        if done is not None:
+            return done
+    template, cache_template, ws_bytes = _pool_plan(op, caches, *state, first, second, page_size)
     lead = caches[0] if block_table is None else block_table
     index = lead.get_device()
     if H.current_device() != index:
@@ -283,7 +282,9 @@ def _upkeep(op, caches, block_table=None, seq_lengths=None, ref_counts=None, fir
         p.caches = array
     p.error_flag = report_ptr(index)
     check(lib().dsa_pages(p, H.raw_stream(index)), "dsa_pages")
-    return out
+    if fast is not None and all(a is b for a, b in zip(args[2:7], (*state, first, second))):
+        fast.keep(BIND_UPKEEP, *args, template, cache_template, ws_bytes)
+    return tuple(out)
 
 
 def paged_cache_copy(caches, src_pages, dst_pages):
@@ -297,7 +298,7 @@ def paged_cache_copy(caches, src_pages, dst_pages):
 def paged_cache_extend(block_table, seq_lengths, ref_counts, counts, page_size):
     """Grow sequence r by ``counts[r]`` [slots] tokens, with the pages that takes.  Returns the new
     (block_table, seq_lengths, ref_counts)."""
-    return tuple(_upkeep(PAGES_EXTEND, [], block_table, seq_lengths, ref_counts, counts, page_size=page_size))
+    return _upkeep(PAGES_EXTEND, [], block_table, seq_lengths, ref_counts, counts, page_size=page_size)
 
 
 def paged_cache_fork(caches, block_table, seq_lengths, ref_counts, parents, children, page_size=None):
@@ -305,14 +306,14 @@ def paged_cache_fork(caches, block_table, seq_lengths, ref_counts, parents, chil
     the parents' full pages, and a partly filled last page is copied (its filled rows, in every
     cache) to a page of the child's own.  Returns the new (block_table, seq_lengths, ref_counts).
     ``page_size`` is needed where ``caches`` is empty."""
-    return tuple(_upkeep(PAGES_FORK, list(caches), block_table, seq_lengths, ref_counts, parents, children,
-                         page_size))
+    return _upkeep(PAGES_FORK, list(caches), block_table, seq_lengths, ref_counts, parents, children,
+                   page_size)
 
 
 def paged_cache_free(block_table, seq_lengths, ref_counts, rows):
     """Empty the slots ``rows`` [n]: their pages lose one holder each.  Returns the new
     (block_table, seq_lengths, ref_counts)."""
-    return tuple(_upkeep(PAGES_FREE, [], block_table, seq_lengths, ref_counts, rows))
+    return _upkeep(PAGES_FREE, [], block_table, seq_lengths, ref_counts, rows)
 
 
 def paged_cache_compact(caches, block_table, ref_counts):

@@ -12,7 +12,8 @@ import math
 import torch
 
 from . import _host as H
-from ._lib import DSA_DTYPE_FP32, RotaryParams, check, lib, ptr, report_ptr, stream_ptr
+from ._lib import (BIND_ROTARY, DSA_DTYPE_FP32, RotaryParams, binding, check, lib, ptr, report_ptr,
+                   stream_ptr)
 
 _MAX_DIM = 256
 LAYOUTS = ("interleaved", "half")
@@ -78,9 +79,6 @@ def _token_strides(t: torch.Tensor):
     return (0, *t.stride()[:2]) if t.dim() == 3 else tuple(t.stride()[:3])
 
 
-_plans = H.Plans()
-
-
 def _plan(x, table, positions, layout, offset, inverse, out):
     """Check the arguments and fill in what their shapes decide."""
     if layout not in LAYOUTS:
@@ -131,10 +129,13 @@ def rotary_embedding(x, table, positions, layout="interleaved", offset=0, invers
     ``x`` itself for a rotation in place) receives the result, else a new tensor.  A position
     outside the table gives a zero row and is reported by ``check_device_errors``.
     """
-    key = (H.signature((x, table, positions, out)), layout, offset, inverse)
-    template = _plans.get(key)
-    if template is None:
-        template = _plans.keep(key, _plan(x, table, positions, layout, offset, inverse, out))
+    args = (x, table, positions, layout, offset, bool(inverse), out)
+    fast = binding()
+    if fast is not None:
+        done = fast.rotary(*args)
+        if done is not None:
+            return done
+    template = _plan(x, table, positions, layout, offset, inverse, out)
     index = x.get_device()
     if H.current_device() != index:
         with torch.cuda.device(index):
@@ -157,4 +158,6 @@ def rotary_embedding(x, table, positions, layout="interleaved", offset=0, invers
     p.positions, p.table = positions.data_ptr(), table.data_ptr()
     p.error_flag = report_ptr(index)
     check(lib().dsa_rotary(p, H.raw_stream(index)), "dsa_rotary")
+    if fast is not None and x is args[0] and table is args[1] and positions is args[2]:
+        fast.keep(BIND_ROTARY, *args, template, b"", 0)
     return out
