@@ -255,6 +255,15 @@ def binding():
     return _binding or None
 
 
+def remember(op: int, index: int, *call) -> None:
+    """Keep the plan of a call's signature for the compiled path: the operator's arguments, its
+    parameters, extra bytes and workspace bytes."""
+    module = binding()
+    if module is not None:
+        module.set_report(index, report_ptr(index))
+        module.keep(op, *call)
+
+
 BIND_ATTN, BIND_ROTARY, BIND_APPEND, BIND_UPKEEP = range(4)   # Op of csrc/binding.cpp
 
 
@@ -292,8 +301,6 @@ def report_ptr(index: int) -> int:
     p = _report_ptrs.get(index)
     if p is None:
         p = _report_ptrs[index] = report_flag(torch.device("cuda", index)).data_ptr()
-        if binding() is not None:
-            binding().set_report(index, p)
     return p
 
 

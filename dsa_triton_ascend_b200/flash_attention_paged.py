@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import _host as H
-from ._lib import BIND_ATTN, AttnPagedParams, binding, check, lib, report_ptr
+from ._lib import BIND_ATTN, AttnPagedParams, binding, check, lib, remember, report_ptr
 
 _VALID_D = (128, 256, 512)
 _D_ROPE = 64
@@ -160,7 +160,7 @@ def flash_attention_paged(
         p.softmax_max, p.softmax_sum = smax.data_ptr(), ssum.data_ptr()
     p.error_flag = report_ptr(index)
     check(lib().dsa_attn_paged(p, H.raw_stream(index)), "dsa_attn_paged")
-    if fast is not None and q is query and qr is query_rope and bt is block_table \
+    if q is query and qr is query_rope and bt is block_table \
             and act_k is actual_seq_lengths_key and act_q is actual_seq_lengths_query:
-        fast.keep(BIND_ATTN, *args, template, b"", ws_bytes)
+        remember(BIND_ATTN, index, *args, template, b"", ws_bytes)
     return out, smax, ssum

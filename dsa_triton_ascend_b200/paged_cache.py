@@ -22,7 +22,7 @@ import torch
 from . import _host as H
 from ._lib import (APPEND_MAX_ENTRIES, BIND_APPEND, BIND_UPKEEP, DSA_DTYPE_BF16, DSA_DTYPE_FP16, DSA_DTYPE_FP32, PAGES_COMPACT, PAGES_COPY,
                    PAGES_EXTEND, PAGES_FORK, PAGES_FREE, ROTARY_CODES, CacheAppendParams, PageCache,
-                   PagesParams, binding, check, lib, ptr, report_ptr)
+                   PagesParams, binding, check, lib, ptr, remember, report_ptr)
 
 _ROTATED = {torch.bfloat16: DSA_DTYPE_BF16, torch.float16: DSA_DTYPE_FP16, torch.float32: DSA_DTYPE_FP32}
 
@@ -187,9 +187,9 @@ def paged_cache_append(tokens, caches, block_table, starts, counts=None, table=N
     p.block_table, p.starts, p.counts = bt.data_ptr(), st.data_ptr(), ptr(ct)
     p.error_flag = report_ptr(index)
     check(lib().dsa_cache_append(p, H.raw_stream(index)), "dsa_cache_append")
-    if fast is not None and not keep and bt is block_table and st is starts and ct is counts \
+    if not keep and bt is block_table and st is starts and ct is counts \
             and (table is args[5] or not p.dim):
-        fast.keep(BIND_APPEND, *args, template, b"", 0)
+        remember(BIND_APPEND, index, *args, template, b"", 0)
     return caches
 
 
@@ -282,8 +282,8 @@ def _upkeep(op, caches, block_table=None, seq_lengths=None, ref_counts=None, fir
         p.caches = array
     p.error_flag = report_ptr(index)
     check(lib().dsa_pages(p, H.raw_stream(index)), "dsa_pages")
-    if fast is not None and all(a is b for a, b in zip(args[2:7], (*state, first, second))):
-        fast.keep(BIND_UPKEEP, *args, template, cache_template, ws_bytes)
+    if all(a is b for a, b in zip(args[2:7], (*state, first, second))):
+        remember(BIND_UPKEEP, index, *args, template, cache_template, ws_bytes)
     return tuple(out)
 
 

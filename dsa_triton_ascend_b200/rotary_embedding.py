@@ -12,8 +12,8 @@ import math
 import torch
 
 from . import _host as H
-from ._lib import (BIND_ROTARY, DSA_DTYPE_FP32, RotaryParams, binding, check, lib, ptr, report_ptr,
-                   stream_ptr)
+from ._lib import (BIND_ROTARY, DSA_DTYPE_FP32, RotaryParams, binding, check, lib, ptr, remember,
+                   report_ptr, stream_ptr)
 
 _MAX_DIM = 256
 LAYOUTS = ("interleaved", "half")
@@ -158,6 +158,6 @@ def rotary_embedding(x, table, positions, layout="interleaved", offset=0, invers
     p.positions, p.table = positions.data_ptr(), table.data_ptr()
     p.error_flag = report_ptr(index)
     check(lib().dsa_rotary(p, H.raw_stream(index)), "dsa_rotary")
-    if fast is not None and x is args[0] and table is args[1] and positions is args[2]:
-        fast.keep(BIND_ROTARY, *args, template, b"", 0)
+    if x is args[0] and table is args[1] and positions is args[2]:
+        remember(BIND_ROTARY, index, *args, template, b"", 0)
     return out
