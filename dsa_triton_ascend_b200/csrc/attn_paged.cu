@@ -177,7 +177,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     fence_mbarrier_init();
   }
   if (warp == kQkWarp) tmem_alloc<1>(smem_u32(tmem_ptr), C::kTmem);
+  griddep_wait();   // what the stream's kernels before this one wrote may be read from here on
 
+  if (threadIdx.x == kLoadWarp * 32) {
+    tma_prefetch_desc(&maps.k);
+    tma_prefetch_desc(&maps.kr);
+    tma_prefetch_desc(&maps.q);
+    tma_prefetch_desc(&maps.qr);
+  }
   Work work = share_of<kTile, kSegmentCost, kThreads>(a, blockIdx.x, gridDim.x, blockIdx.x == 0, tmp, start);
   griddep_launch_dependents();
   tc_fence_before();
@@ -185,7 +192,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_ptr;
   const uint32_t t_o = tmem + 2 * NH;
-  take_start(work, start);
   bool failed = false;
 
   if (warp >= kLoadWarp && warp < kQkWarp) {
@@ -213,7 +219,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int st = g % C::kStages, tile = sg.first + i;
         const int now = page;
         if (i + 1 < sg.count) page = page_of(tile + 1);
-        if (g >= C::kStages) mbar_wait(empty(st), (g / C::kStages - 1) & 1, a.error_flag, &failed);
+        if (g >= C::kStages) mbar_wait_hot(empty(st), (g / C::kStages - 1) & 1, a.error_flag, &failed);
         failed = __any_sync(0xffffffffu, failed);
         if (failed) break;
         const uint32_t mask = __ballot_sync(0xffffffffu, now >= 0) & 3u;
@@ -243,7 +249,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     while (!failed && next_segment<kTile, kSegmentCost>(a, work, sg)) {
       const int b = sg.row / a.s1, s = sg.row - b * a.s1;
       const int buf = nseg % C::kQBufs, use = nseg / C::kQBufs;
-      if (use > 0) mbar_wait(q_empty(buf), (use - 1) & 1, a.error_flag, &failed);
+      if (use > 0) mbar_wait_hot(q_empty(buf), (use - 1) & 1, a.error_flag, &failed);
       failed = __any_sync(0xffffffffu, failed);
       if (failed) break;
       if (lane == 0) {
@@ -272,11 +278,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr uint32_t kIdQk = idesc_f16(64, NH, kBf16, false, false);
       while (!failed && next_segment<kTile, kSegmentCost>(a, work, sg)) {
         const int buf = nseg % C::kQBufs;
-        mbar_wait_spin(q_full(buf), (nseg / C::kQBufs) & 1, a.error_flag, &failed);
+        mbar_wait_hot(q_full(buf), (nseg / C::kQBufs) & 1, a.error_flag, &failed);
         for (int i = 0; i < sg.count; ++i, ++g) {
           const int st = g % C::kStages;
-          if (g >= 2) mbar_wait_spin(s_empty(g & 1), ((g >> 1) - 1) & 1, a.error_flag, &failed);
-          mbar_wait_spin(full(st), (g / C::kStages) & 1, a.error_flag, &failed);
+          if (g >= 2) mbar_wait_hot(s_empty(g & 1), ((g >> 1) - 1) & 1, a.error_flag, &failed);
+          mbar_wait_hot(full(st), (g / C::kStages) & 1, a.error_flag, &failed);
           failed = __any_sync(0xffffffffu, failed);
           if (failed) break;
           tc_fence_after();
@@ -306,8 +312,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       while (!failed && next_segment<kTile, kSegmentCost>(a, work, sg)) {
         for (int i = 0; i < sg.count; ++i, ++g) {
           const int st = g % C::kStages;
-          if (i == 0 && nseg > 0) mbar_wait_spin(o_empty, (nseg - 1) & 1, a.error_flag, &failed);
-          mbar_wait_spin(p_full, g & 1, a.error_flag, &failed);
+          if (i == 0 && nseg > 0) mbar_wait_hot(o_empty, (nseg - 1) & 1, a.error_flag, &failed);
+          mbar_wait_hot(p_full, g & 1, a.error_flag, &failed);
           failed = __any_sync(0xffffffffu, failed);
           if (failed) break;
           tc_fence_after();
@@ -364,11 +370,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       for (int i = 0; i < sg.count; ++i, ++g) {
         const int st = g % C::kStages;
-        mbar_wait_spin(full(st), (g / C::kStages) & 1, a.error_flag, &failed);
+        mbar_wait_hot(full(st), (g / C::kStages) & 1, a.error_flag, &failed);
         const uint32_t mask = (uint32_t)tmask[4 * st + quarter];   // of this warp's 16 keys
         const int valid = sg.keys - (sg.first + i) * kTile;        // keys of this tile, >= 1
         const bool whole_tile = valid >= kTile && mask == 3u;
-        mbar_wait_spin(s_full(g & 1), (g >> 1) & 1, a.error_flag, &failed);
+        mbar_wait_hot(s_full(g & 1), (g >> 1) & 1, a.error_flag, &failed);
         tc_fence_after();
         uint32_t raw[HW / 2];
         tmem_ld_frag<HW>(tmem + (g & 1) * NH + head0 + lane_base, raw);
@@ -434,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int j = 0; j < 2 * kPairs; ++j) factor[8 * (j >> 1) + col + (j & 1)] = f[j];
           softmax_bar(wg);   // the factors are there, the maxima read
           if (i > 0) {
-            mbar_wait_spin(p_empty, (g - 1) & 1, a.error_flag, &failed);
+            mbar_wait_hot(p_empty, (g - 1) & 1, a.error_flag, &failed);
             tc_fence_after();
 #pragma unroll 1
             for (int m = 0; m < C::kBlocks; ++m)
@@ -468,7 +474,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           packed[2 * j] = E::pack2(p[0], p[1]);
           packed[2 * j + 1] = E::pack2(p[2], p[3]);
         }
-        if (!p_free) mbar_wait_spin(p_empty, (g - 1) & 1, a.error_flag, &failed);
+        if (!p_free) mbar_wait_hot(p_empty, (g - 1) & 1, a.error_flag, &failed);
         uint8_t* ps = smem + (s_p - base);
 #pragma unroll
         for (int j = 0; j < kPairs; ++j) {
@@ -532,7 +538,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       softmax_bar(wg);
-      mbar_wait_spin(p_empty, (g - 1) & 1, a.error_flag, &failed);
+      mbar_wait_hot(p_empty, (g - 1) & 1, a.error_flag, &failed);
       tc_fence_after();
       const int heads = min(head0 + HW, a.n1 - sg.group * NH);
       const int dim = quarter * 32 + lane;
@@ -591,16 +597,15 @@ __device__ __forceinline__ bool parts_of(const Args& a, int grid, int row, int h
   const int64_t units = (int64_t)all * a.groups, ctas = ctas_used(units, grid);
   const int64_t x0 = (int64_t)first * a.groups + (int64_t)(head / NH) * count;
   const int64_t lo = (x0 + kCost + 1) * ctas - 1, hi = (x0 + count) * ctas - 1;
-  if (units * ctas < (1LL << 31)) {   // (a 64-bit division takes as long as a trip to L2)
+  if (units * ctas < (1LL << 32)) {
     const uint32_t u = (uint32_t)units;
     p->c0 = (int)((uint32_t)lo / u);
     p->c1 = (int)((uint32_t)hi / u);
-    p->skip = (uint32_t)(units * p->c0) / (uint32_t)ctas < x0 ? 1 : 0;
   } else {
     p->c0 = (int)(lo / units);
     p->c1 = (int)(hi / units);
-    p->skip = units * p->c0 / ctas < x0 ? 1 : 0;
   }
+  p->skip = share_begin(units, p->c0, ctas) < x0 ? 1 : 0;
   return p->c0 != p->c1;   // else written whole
 }
 
@@ -618,6 +623,7 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_combine_kernel(const 
   __shared__ float4 part[kLanes == kJoinThreads ? kGroups : 1][kLanes == kJoinThreads ? D / 4 : 1];
   __shared__ float psum[kGroups];
   griddep_wait();
+  griddep_launch_dependents();
   const int64_t at = (int64_t)blockIdx.x * (kJoinThreads / kLanes) + threadIdx.x / kLanes;
   if (at >= (int64_t)a.rows * a.n1) return;
   const int row = (int)(at / a.n1), head = (int)(at - (int64_t)row * a.n1), h = head % NH;
@@ -745,24 +751,32 @@ bool make_maps(Maps* maps, const DsaAttnPagedParams* p, bool bf16, uint32_t nh) 
          make_tmap_16b(&maps->kr, p->key_rope_cache, bf16, 4, krdims, krst, krbox);
 }
 
+// A launch that may begin before the stream's kernel before it has ended: the kernels here wait
+// for that one's results (griddep_wait) once they are set up.
+template <typename... P, typename... A>
+bool launch_early(void (*kern)(P...), int64_t blocks, int threads, int smem, cudaStream_t stream, const A&... args) {
+  cudaLaunchAttribute pdl[1];
+  pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  pdl[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = pdl;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess;
+}
+
 template <int D, int NH, int kCost, typename T>
 int launch_join(const DsaAttnPagedParams* p, const Args& a, int shares, cudaStream_t stream) {
   const int64_t items = p->batch * p->s1 * p->n1;
   // a block each up to eight a multiprocessor (what runs at once), else a warp each
   const bool wide = items <= 8LL * sm_count();
   const int64_t blocks = wide ? items : (items + kJoinThreads / 32 - 1) / (kJoinThreads / 32);
-  cudaLaunchAttribute pdl[1];
-  pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  pdl[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)blocks);
-  cfg.blockDim = dim3(kJoinThreads);
-  cfg.stream = stream;
-  cfg.attrs = pdl;
-  cfg.numAttrs = 1;
   auto kern = wide ? attn_paged_combine_kernel<D, NH, kCost, kJoinThreads, T>
                    : attn_paged_combine_kernel<D, NH, kCost, 32, T>;
-  return cudaLaunchKernelEx(&cfg, kern, a, shares) == cudaSuccess ? DSA_OK : DSA_ERR_CUDA;
+  return launch_early(kern, blocks, kJoinThreads, 0, stream, a, shares) ? DSA_OK : DSA_ERR_CUDA;
 }
 
 template <int D, int NH, typename T>
@@ -778,8 +792,7 @@ int launch(const DsaAttnPagedParams* p, cudaStream_t stream) {
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) !=
       cudaSuccess)
     return DSA_ERR_CUDA;
-  kern<<<grid, kThreads, C::kSmem, stream>>>(maps, a);
-  if (cudaGetLastError() != cudaSuccess) return DSA_ERR_CUDA;
+  if (!launch_early(kern, grid, kThreads, C::kSmem, stream, maps, a)) return DSA_ERR_CUDA;
   return launch_join<D, NH, kSegmentCost, T>(p, a, grid, stream);
 }
 
@@ -802,8 +815,7 @@ int launch_pair(const DsaAttnPagedParams* p, cudaStream_t stream) {
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) !=
       cudaSuccess)
     return DSA_ERR_CUDA;
-  kern<<<2 * pairs, pair::kThreads, C::kSmem, stream>>>(maps, map_v, a);
-  if (cudaGetLastError() != cudaSuccess) return DSA_ERR_CUDA;
+  if (!launch_early(kern, 2 * pairs, pair::kThreads, C::kSmem, stream, maps, map_v, a)) return DSA_ERR_CUDA;
   return launch_join<D, 2 * pair::kHeads, pair::kSegmentCost, T>(p, a, pairs, stream);
 }
 

@@ -118,12 +118,51 @@ __device__ __forceinline__ bool next_segment(const Args& a, Work& w, Segment& s)
   return false;
 }
 
-// The share of CTA (or pair) `cta` of `ctas_max`.  All threads of the block call it; the place where the share begins is left in
-// `start` (shared memory), to be read after a barrier (take_start).  The first CTA also writes
-// the rows' prefix for the join.
+// units * c / ctas, by 32-bit numbers where they hold it (a 64-bit division takes as long as a
+// trip to L2).
+__device__ __forceinline__ int64_t share_begin(int64_t units, int64_t c, int64_t ctas) {
+  if (units * ctas < (1LL << 32)) return (uint32_t)(units * c) / (uint32_t)ctas;
+  return units * c / ctas;
+}
+
+// The share of CTA (or pair) `cta` of `ctas_max`.  All threads of the block call it.  The first CTA
+// also writes the rows' prefix for the join.
 template <int kTile, int kCost, int kThreads>
 __device__ __forceinline__ Work share_of(const Args& a, int cta, int ctas_max, bool first_cta, int* tmp,
                                          int32_t* start) {
+  Work work{0, 0, 0, 0};
+  if (a.rows <= 32) {
+    // each warp for itself, without a barrier
+    const int lane = threadIdx.x & 31;
+    const int mine = lane < a.rows ? row_units<kTile, kCost>(a, lane) : 0;
+    int x = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    const int total = __shfl_sync(0xffffffffu, x, 31);
+    if (first_cta && threadIdx.x < 32) {
+      if (lane < a.rows) a.ws_prefix[lane] = x - mine;
+      if (lane == 0) a.ws_prefix[a.rows] = total;
+    }
+    const int64_t units = (int64_t)total * a.groups, ctas = ctas_used(units, ctas_max);
+    if (cta >= ctas) return work;
+    const int64_t from = share_begin(units, cta, ctas);
+    work.left = (int)(share_begin(units, cta + 1, ctas) - from);
+    const int64_t first = (int64_t)(x - mine) * a.groups;
+    const uint32_t here = __ballot_sync(0xffffffffu, mine > 0 && first <= from && from < first + (int64_t)mine * a.groups);
+    if (here == 0) {   // no unit at all
+      work.left = 0;
+      return work;
+    }
+    const int row = __ffs(here) - 1;
+    const int in = (int)(from - __shfl_sync(0xffffffffu, first, row)), per = __shfl_sync(0xffffffffu, mine, row);
+    work.row = row;
+    work.group = in / per;
+    work.unit = in - work.group * per;
+    return work;
+  }
   int64_t total = 0;
   int mine = 0, before = 0;   // the units of the thread's last row and of the rows before it
   for (int r0 = 0; r0 < a.rows; r0 += kThreads) {
@@ -137,37 +176,32 @@ __device__ __forceinline__ Work share_of(const Args& a, int cta, int ctas_max, b
   if (first_cta && threadIdx.x == 0) a.ws_prefix[a.rows] = (int)total;
   const int64_t units = total * a.groups;
   const int64_t ctas = ctas_used(units, ctas_max);
-  Work work{0, 0, 0, 0};
-  int64_t from = 0;
-  if (cta < ctas) {
-    from = units * cta / ctas;
-    work.left = (int)(units * (cta + 1) / ctas - from);
-    int64_t seen = 0;
-    for (int r0 = 0; r0 < a.rows; r0 += kThreads) {
-      const int r = r0 + threadIdx.x;
-      int sum = (int)total;
-      if (a.rows > kThreads) {
-        mine = r < a.rows ? row_units<kTile, kCost>(a, r) : 0;
-        before = block_scan<kThreads>(mine, tmp, &sum);
-      }
-      const int64_t first = (seen + before) * a.groups;
-      if (mine > 0 && first <= from && from < first + (int64_t)mine * a.groups) {
-        const int in = (int)(from - first);
-        start[0] = r;
-        start[1] = in / mine;
-        start[2] = in - (in / mine) * mine;
-      }
-      seen += sum;
-      if (seen * a.groups > from) break;   // the same for every thread
+  if (units == 0 || cta >= ctas) return work;
+  const int64_t from = share_begin(units, cta, ctas);
+  work.left = (int)(share_begin(units, cta + 1, ctas) - from);
+  int64_t seen = 0;
+  for (int r0 = 0; r0 < a.rows; r0 += kThreads) {
+    const int r = r0 + threadIdx.x;
+    int sum = (int)total;
+    if (a.rows > kThreads) {
+      mine = r < a.rows ? row_units<kTile, kCost>(a, r) : 0;
+      before = block_scan<kThreads>(mine, tmp, &sum);
     }
+    const int64_t first = (seen + before) * a.groups;
+    if (mine > 0 && first <= from && from < first + (int64_t)mine * a.groups) {
+      const int in = (int)(from - first);
+      start[0] = r;
+      start[1] = in / mine;
+      start[2] = in - (in / mine) * mine;
+    }
+    seen += sum;
+    if (seen * a.groups > from) break;   // the same for every thread
   }
-  return work;
-}
-__device__ __forceinline__ void take_start(Work& work, const int32_t* start) {
-  if (work.left <= 0) return;
+  __syncthreads();
   work.row = start[0];
   work.group = start[1];
   work.unit = start[2];
+  return work;
 }
 
 // 2^x, 2^-126 and below flushed to 0

@@ -141,6 +141,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     fence_mbarrier_init();
   }
   if (warp == kMmaWarp) tmem_alloc<2>(smem_u32(tmem_ptr), C::kTmem);
+  griddep_wait();
+  if (threadIdx.x == kKeyWarp * 32) {
+    tma_prefetch_desc(&maps.k);
+    tma_prefetch_desc(&maps.kr);
+    tma_prefetch_desc(&map_v);
+    tma_prefetch_desc(&maps.q);
+    tma_prefetch_desc(&maps.qr);
+  }
   Work work = share_of<kTile, kSegmentCost, kThreads>(a, blockIdx.x >> 1, gridDim.x >> 1, blockIdx.x == 0, tmp, start);
   griddep_launch_dependents();
   tc_fence_before();
@@ -148,7 +156,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   cluster_sync();
   tc_fence_after();
   const uint32_t tmem = *tmem_ptr;
-  take_start(work, start);
   bool failed = false;
 
   // Lane l < 16 looks up the page of keys 8 l .. 8 l + 7 of a tile.  -1: no such page.  (Every
@@ -178,7 +185,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (t.i + 1 < t.s.count) page = page_of(t.s, table, tile + 1, rank == 0 && w == 0);
       const uint32_t mask = __ballot_sync(0xffffffffu, now >= 0);
       const int in_page = (tile * kTile + lane * 8) % a.page_size;
-      if (g >= C::kStages) mbar_wait(k_empty(st), (g / C::kStages - 1) & 1, a.error_flag, &failed);
+      if (g >= C::kStages) mbar_wait_hot(k_empty(st), (g / C::kStages - 1) & 1, a.error_flag, &failed);
       failed = __any_sync(0xffffffffu, failed);
       if (failed) break;
       if (rank == 0 && lane == 0) {
@@ -219,7 +226,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (w == 0 && t.i == 0) {
         const int b = t.s.row / a.s1, s = t.s.row - b * a.s1;
         const int buf = t.seg % C::kQBufs, use = t.seg / C::kQBufs;
-        if (use > 0) mbar_wait(q_empty(buf), (use - 1) & 1, a.error_flag, &failed);
+        if (use > 0) mbar_wait_hot(q_empty(buf), (use - 1) & 1, a.error_flag, &failed);
         failed = __any_sync(0xffffffffu, failed);
         if (failed) break;
         if (lane == 0) {
@@ -233,7 +240,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
         const int u = 2 * g + hf, slot = u % C::kVSlots;
-        if (u >= C::kVSlots) mbar_wait(v_empty(slot), (u / C::kVSlots - 1) & 1, a.error_flag, &failed);
+        if (u >= C::kVSlots) mbar_wait_hot(v_empty(slot), (u / C::kVSlots - 1) & 1, a.error_flag, &failed);
         failed = __any_sync(0xffffffffu, failed);
         if (failed) break;
         if (lane == 0) {
@@ -382,7 +389,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (i + 1 < sg.count) page = page_of(sg, table, tile + 1, false);
         const int valid = sg.keys - tile * kTile;
         const bool tail = mask != 0xffffu || valid < kTile;
-        mbar_wait_spin(s_full(g & 1), (g >> 1) & 1, a.error_flag, &failed);
+        mbar_wait_hot(s_full(g & 1), (g >> 1) & 1, a.error_flag, &failed);
         tc_fence_after();
         uint32_t r[32];
         tmem_ld32(tmem + 64 * (g & 1) + 32 * wg + lane_addr, r);
@@ -415,7 +422,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           ref = now;
           lim = (now + kRescale) / c2;
           if (i > 0) {
-            mbar_wait_spin(p_empty, (g - 1) & 1, a.error_flag, &failed);
+            mbar_wait_hot(p_empty, (g - 1) & 1, a.error_flag, &failed);
             tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < kDims; c += 16) {
@@ -441,7 +448,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           sum += p0 + p1;
           pk[j] = E::pack2(p0, p1);
         }
-        if (!p_free) mbar_wait_spin(p_empty, (g - 1) & 1, a.error_flag, &failed);
+        if (!p_free) mbar_wait_hot(p_empty, (g - 1) & 1, a.error_flag, &failed);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           *reinterpret_cast<uint4*>(prow + (((4 * wg + j) ^ (h & 7)) << 4)) =
@@ -451,7 +458,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           // stale tail): cleared, so that 0 x NaN cannot enter the product
           const int key = threadIdx.x >> 1;
           const int s0 = 2 * g % C::kVSlots, slot = s0 + (key >> 6);   // of this thread's half
-          mbar_wait_spin(v_tail(slot), tails >> slot & 1, a.error_flag, &failed);
+          mbar_wait_hot(v_tail(slot), tails >> slot & 1, a.error_flag, &failed);
           tails ^= 3u << s0;
           if (key >= valid || !(mask >> (key >> 3) & 1u)) {
             uint8_t* row = smem + C::kOffV + slot * C::kHalfBytes + (key >> 3 & 7) * C::kVGroupBytes + (key & 7) * 128;
@@ -491,7 +498,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           a.softmax_sum[at] = any ? l * exp2f(ref - kShift - most) : 0.0f;
         }
       }
-      mbar_wait_spin(p_empty, (g - 1) & 1, a.error_flag, &failed);
+      mbar_wait_hot(p_empty, (g - 1) & 1, a.error_flag, &failed);
       tc_fence_after();
       const int dim = half * (D / 2) + wg * kDims;
 #pragma unroll 1

@@ -200,6 +200,20 @@ __device__ __forceinline__ bool mbar_wait_spin(uint32_t bar, uint32_t parity, in
   return false;
 }
 
+// Bounded wait of a pipeline whose every hand-over counts: as mbar_wait_spin, but the global
+// timer (whose reading takes long enough to miss the phase's end) is not looked at before some
+// ten thousand polls.
+__device__ __forceinline__ bool mbar_wait_hot(uint32_t bar, uint32_t parity, int* err, bool* failed,
+                                              bool cluster_scope = false) {
+  if (*failed) return false;
+#pragma unroll 1
+  for (int i = 0; i < 16384; ++i)
+    if (cluster_scope ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity)) return true;
+  if (mbar_wait_timed(bar, parity, err, cluster_scope)) return true;
+  *failed = true;
+  return false;
+}
+
 // Bounded wait with a sleep between polls, for a role thread that waits long (a producer
 // for a free slot, an MMA issuer for a drained buffer): polling at full rate would take
 // issue slots from the warps that do the work on the same scheduler.
