@@ -517,8 +517,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               make_float2(run[2 * j], run[2 * j + 1]);
         }
       softmax_bar(wg);
-      const bool whole = sg.count == sg.tiles;
-      const int slot = 2 * blockIdx.x + (nseg == 0 ? 0 : 1);
+      const bool all = sg.count == sg.tiles, whole = all && a.diag == 0;
+      const int64_t slot = all ? (int64_t)2 * gridDim.x + sg.row : 2 * blockIdx.x + (nseg == 0 ? 0 : 1);
       if (quarter == 0 && lane < 4)
 #pragma unroll
         for (int j = 0; j < 2 * kPairs; ++j) {
@@ -530,7 +530,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           factor[h] = !whole ? 1.0f : l > 0.0f || l != l ? 1.0f / l : 0.0f;
           if (head >= a.n1) continue;
           if (!whole) {
-            a.ws_s[(int64_t)slot * NH + h] = make_float4(ref[j] - kShift, most, l, m);
+            a.ws_s[slot * NH + h] = make_float4(ref[j] - kShift, most, l, m);
           } else if (a.softmax_max) {
             const int64_t at = (int64_t)sg.row * a.n1 + head;
             a.softmax_max[at] = any ? m * fabsf(a.scale) : 0.0f;
@@ -556,7 +556,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int j = 0; j < kCols; ++j)
               if (h0 + j < heads) out[j * D] = E::from_f(__uint_as_float(o[j]) * factor[h0 + j]);
           } else {
-            float* out = a.ws_o + ((int64_t)slot * NH + h0) * D + m * 128 + dim;
+            float* out = a.ws_o + (slot * NH + h0) * D + m * 128 + dim;
 #pragma unroll
             for (int j = 0; j < kCols; ++j)
               if (h0 + j < heads) out[j * D] = __uint_as_float(o[j]);
@@ -579,20 +579,24 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // Where the parts of one (row, head) are: CTAs c0 .. c1, whose slot of a part is 2 c, but 2 c0 + 1
-// where the row begins inside the share of c0.
+// where the row begins inside the share of c0; or the row's own slot (c0 == c1).
 struct Parts {
-  int c0, c1, skip;
+  int c0, c1, skip, own;
   template <int NH>
   __device__ __forceinline__ int64_t at(int c, int h) const {
-    return (int64_t)(2 * c + (c == c0 ? skip : 0)) * NH + h;
+    return (int64_t)(c0 == c1 ? own : 2 * c + (c == c0 ? skip : 0)) * NH + h;
   }
 };
 
+// False for a row without a part (c1 < c0).
 template <int NH, int kCost>
-__device__ __forceinline__ bool parts_of(const Args& a, int grid, int row, int head, Parts* p, bool* empty) {
+__device__ __forceinline__ bool parts_of(const Args& a, int grid, int row, int head, Parts* p) {
   const int first = a.ws_prefix[row], next = a.ws_prefix[row + 1], all = a.ws_prefix[a.rows];
   const int count = next - first;   // units
-  *empty = count == 0;
+  p->own = 2 * grid + row;
+  p->skip = 0;
+  p->c0 = 1;
+  p->c1 = 0;
   if (count == 0) return false;
   const int64_t units = (int64_t)all * a.groups, ctas = ctas_used(units, grid);
   const int64_t x0 = (int64_t)first * a.groups + (int64_t)(head / NH) * count;
@@ -606,41 +610,91 @@ __device__ __forceinline__ bool parts_of(const Args& a, int grid, int row, int h
     p->c1 = (int)(hi / units);
   }
   p->skip = share_begin(units, p->c0, ctas) < x0 ? 1 : 0;
-  return p->c0 != p->c1;   // else written whole
+  return true;
 }
 
-// Join the parts that a row's CTAs left; zeros for a row without keys.  kJoinLanes threads go
-// through the parts of one (row, head), D / 4 of them taking a part's float4s side by side:
-// a whole block where there are few rows (and so many parts of each), else a warp.
+// q . k + qr . kr of packed head `head` of batch `b` and the key at position `pos`, by a warp; false
+// if there is no such page.
+template <int D, typename T>
+__device__ __forceinline__ bool warp_dot(const Args& a, int b, int head, int pos, int lane, float* dot,
+                                         const T** key) {
+  const int page = a.block_table[(int64_t)b * a.max_blocks + pos / a.page_size], row = pos % a.page_size;
+  if (page >= a.num_pages && lane == 0) report_error(a.error_flag, kErrBadIndex);
+  if (page < 0 || page >= a.num_pages) return false;
+  const T* k = static_cast<const T*>(a.k) + page * a.k_page + row * a.k_row;
+  const T* kr = static_cast<const T*>(a.kr) + page * a.kr_page + row * a.kr_row;
+  const T* q = static_cast<const T*>(a.q) + b * a.q_batch + head * a.q_head;
+  const T* qr = static_cast<const T*>(a.qr) + b * a.qr_batch + head * a.qr_head;
+  float sum = 0.0f;
+  for (int i = lane; i < (D + kRope) / 8; i += 32) {
+    const bool rope = i >= D / 8;
+    const uint4 x = *reinterpret_cast<const uint4*>(rope ? qr + (i - D / 8) * 8 : q + i * 8);
+    const uint4 y = *reinterpret_cast<const uint4*>(rope ? kr + (i - D / 8) * 8 : k + i * 8);
+    const T *xe = reinterpret_cast<const T*>(&x), *ye = reinterpret_cast<const T*>(&y);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      sum = fmaf(ElemTraits<T>::to_f(xe[e]), ElemTraits<T>::to_f(ye[e]), sum);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  *dot = sum;
+  *key = k;
+  return true;
+}
+
+constexpr int kMaxDiag = 7;
+
+// Join the parts that a row's CTAs left, and the keys that only its later tokens see; zeros for a
+// row without keys.  kLanes threads go through the parts of one (row, head), D / 4 of them taking
+// a part's float4s side by side: a whole block where there are few rows (and so many parts of
+// each), else a warp.
 constexpr int kJoinThreads = 256;
 
 template <int D, int NH, int kCost, int kLanes, typename T>
 __global__ void __launch_bounds__(kJoinThreads) attn_paged_combine_kernel(const Args a, int grid) {
   using E = ElemTraits<T>;
+  constexpr bool kWide = kLanes == kJoinThreads;
   constexpr int kCols = kLanes < D / 4 ? kLanes : D / 4;   // threads of a part
   constexpr int kPer = D / 4 / kCols;                      // float4s of each
   constexpr int kGroups = kLanes / kCols;                  // parts at a time
-  __shared__ float4 part[kLanes == kJoinThreads ? kGroups : 1][kLanes == kJoinThreads ? D / 4 : 1];
+  __shared__ float4 part[kWide ? kGroups : 1][kWide ? D / 4 : 1];
   __shared__ float psum[kGroups];
+  __shared__ float late_dot[kWide ? 8 : 1];
+  __shared__ const T* late_key[kWide ? 8 : 1];
   griddep_wait();
   griddep_launch_dependents();
   const int64_t at = (int64_t)blockIdx.x * (kJoinThreads / kLanes) + threadIdx.x / kLanes;
   if (at >= (int64_t)a.rows * a.n1) return;
   const int row = (int)(at / a.n1), head = (int)(at - (int64_t)row * a.n1), h = head % NH;
-  const int t = threadIdx.x % kLanes, grp = t / kCols, col = t % kCols;
+  const int t = threadIdx.x % kLanes, grp = t / kCols, col = t % kCols, lane = threadIdx.x & 31;
   T* out = static_cast<T*>(a.out) + at * D;
   Parts p;
-  bool empty;
-  if (!parts_of<NH, kCost>(a, grid, row, head, &p, &empty)) {
-    if (!empty) return;
+  const bool some = parts_of<NH, kCost>(a, grid, row, head, &p);
+  // keys from `common` on that this token sees beside the row's common ones
+  int late = 0, common = 0;
+  if (a.diag > 0) {
+    const int64_t cap = (int64_t)a.max_blocks * a.page_size, ak = a.act_k[row];
+    common = (int)max((int64_t)0, min(cap, ak - a.diag));
+    late = (int)(max((int64_t)common, min(cap, ak - a.diag + head / a.heads)) - common);
+  } else if (some && p.c0 == p.c1) {
+    return;   // written whole
+  }
+  if (!some && late == 0) {
     if (grp == 0)
 #pragma unroll
       for (int i = 0; i < kPer; ++i) *reinterpret_cast<uint2*>(out + (i * kCols + col) * 4) = make_uint2(0, 0);
     if (t == 0 && a.softmax_max) a.softmax_max[at] = a.softmax_sum[at] = 0.0f;
     return;
   }
+  if (kWide && (threadIdx.x >> 5) < late) {   // a warp per late key
+    float dot = 0.0f;
+    const T* key = nullptr;
+    if (!warp_dot<D, T>(a, row, head, common + (threadIdx.x >> 5), lane, &dot, &key)) key = nullptr;
+    late_dot[threadIdx.x >> 5] = dot;
+    late_key[threadIdx.x >> 5] = key;
+  }
   float ref = -INFINITY, run = -INFINITY, top = -INFINITY;
-  for (int c = p.c0 + (threadIdx.x & 31); c <= p.c1; c += 32) {
+  for (int c = p.c0 + lane; c <= p.c1; c += 32) {
     const float4 s = a.ws_s[p.at<NH>(c, h)];
     ref = fmaxf(ref, s.x);
     run = fmaxf(run, s.y);
@@ -670,7 +724,7 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_combine_kernel(const 
       }
     }
   }
-  if constexpr (kLanes == kJoinThreads) {
+  if constexpr (kWide) {
     part[grp][col] = acc[0];
     if (col == 0) psum[grp] = sum;
     __syncthreads();
@@ -680,6 +734,30 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_combine_kernel(const 
       const float4 o = part[k][col];
       sum += psum[k];
       acc[0].x += o.x, acc[0].y += o.y, acc[0].z += o.z, acc[0].w += o.w;
+    }
+  }
+  for (int i = 0; i < late; ++i) {
+    float dot = 0.0f;
+    const T* key = nullptr;
+    if constexpr (kWide) {
+      dot = late_dot[i];
+      key = late_key[i];
+    } else {
+      if (!warp_dot<D, T>(a, row, head, common + i, lane, &dot, &key)) key = nullptr;
+    }
+    if (!key) continue;
+    const float raw = a.scale < 0.0f ? -dot : dot, z = dot * a.scale * 1.4426950408889634f;
+    const float now = fmaxf(ref, z), f = ref == now ? 1.0f : exp2f(ref - now), w = exp2f(z - now);
+    ref = now;
+    run = fmaxf(run, z);
+    top = fmaxf(top, raw);
+    sum = sum * f + w;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const uint2 v = *reinterpret_cast<const uint2*>(key + (k * kCols + col) * 4);
+      const T* e = reinterpret_cast<const T*>(&v);
+      acc[k].x = fmaf(w, E::to_f(e[0]), acc[k].x * f), acc[k].y = fmaf(w, E::to_f(e[1]), acc[k].y * f);
+      acc[k].z = fmaf(w, E::to_f(e[2]), acc[k].z * f), acc[k].w = fmaf(w, E::to_f(e[3]), acc[k].w * f);
     }
   }
   const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
@@ -694,13 +772,16 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_combine_kernel(const 
   }
 }
 
-// Heads of a work item: the smallest operand that holds them, and the pair kernel past 64.
-int heads_of(int64_t n1) { return n1 <= 16 ? 16 : n1 <= 32 ? 32 : n1 <= 64 ? 64 : 128; }
+// Heads of a work item: the smallest operand that holds them.  Past 64 the pair kernel takes them
+// all at D = 512 (32 rows of 8192 .. 65536 keys, 128 heads: 348 us against 478 for two items of 64);
+// below, where a result of 64 heads leaves room for several key tiles, two items are faster (the
+// same rows at D = 256: 252 us against 314 with a pair).
+int heads_of(int64_t n1, int64_t d) { return n1 <= 16 ? 16 : n1 <= 32 ? 32 : n1 <= 64 || d < 512 ? 64 : 128; }
 
 int64_t align256(int64_t x) { return (x + 255) & ~(int64_t)255; }
 
 // What both kernels take; `nh` heads a work item, `shares` of the work.
-Args make_args(const DsaAttnPagedParams* p, int nh, int shares) {
+Args make_args(const DsaAttnPagedParams* p, int nh, int shares, int diag, int heads) {
   Args a;
   a.act_q = p->act_q;
   a.act_k = p->act_k;
@@ -718,11 +799,19 @@ Args make_args(const DsaAttnPagedParams* p, int nh, int shares) {
   a.num_pages = (int)p->num_pages;
   a.mode = p->sparse_mode;
   a.scale = p->scale;
+  a.diag = diag;
+  a.heads = heads;
+  a.q = p->query, a.qr = p->query_rope, a.k = p->key_cache, a.kr = p->key_rope_cache;
+  a.q_batch = p->q_batch_stride, a.q_head = p->q_head_stride;
+  a.qr_batch = p->qr_batch_stride, a.qr_head = p->qr_head_stride;
+  a.k_page = p->k_page_stride, a.k_row = p->k_row_stride;
+  a.kr_page = p->kr_page_stride, a.kr_row = p->kr_row_stride;
+  const int64_t slots = (int64_t)2 * shares + (diag > 0 ? a.rows : 0);
   uint8_t* ws = static_cast<uint8_t*>(p->workspace);
   a.ws_o = reinterpret_cast<float*>(ws);
-  ws += (int64_t)2 * shares * nh * p->d * 4;
+  ws += slots * nh * p->d * 4;
   a.ws_s = reinterpret_cast<float4*>(ws);
-  ws += (int64_t)2 * shares * nh * 16;
+  ws += slots * nh * 16;
   a.ws_prefix = reinterpret_cast<int32_t*>(ws);
   return a;
 }
@@ -780,13 +869,13 @@ int launch_join(const DsaAttnPagedParams* p, const Args& a, int shares, cudaStre
 }
 
 template <int D, int NH, typename T>
-int launch(const DsaAttnPagedParams* p, cudaStream_t stream) {
+int launch(const DsaAttnPagedParams* p, int diag, int heads, cudaStream_t stream) {
   using C = Cfg<D, NH>;
   const int grid = sm_count();
   if (grid < 1) return DSA_ERR_CUDA;
   Maps maps;
   if (!make_maps<D>(&maps, p, ElemTraits<T>::kIsBf16, NH)) return DSA_ERR_TMA_DESCRIPTOR;
-  Args a = make_args(p, NH, grid);
+  Args a = make_args(p, NH, grid, diag, heads);
   a.groups = (int)((p->n1 + NH - 1) / NH);
   auto kern = attn_paged_kernel<D, NH, T>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) !=
@@ -796,8 +885,9 @@ int launch(const DsaAttnPagedParams* p, cudaStream_t stream) {
   return launch_join<D, NH, kSegmentCost, T>(p, a, grid, stream);
 }
 
-template <int D, typename T>
-int launch_pair(const DsaAttnPagedParams* p, cudaStream_t stream) {
+template <typename T>
+int launch_pair(const DsaAttnPagedParams* p, int diag, int heads, cudaStream_t stream) {
+  constexpr int D = 512;
   using C = pair::Cfg<D>;
   constexpr bool kBf16 = ElemTraits<T>::kIsBf16;
   const int pairs = sm_count() / 2;
@@ -810,7 +900,7 @@ int launch_pair(const DsaAttnPagedParams* p, cudaStream_t stream) {
   if (!make_maps<D>(&maps, p, kBf16, pair::kHeads) ||
       !make_tmap_16b(&map_v, p->key_cache, kBf16, 4, dims, st, box))
     return DSA_ERR_TMA_DESCRIPTOR;
-  const Args a = make_args(p, 2 * pair::kHeads, pairs);
+  const Args a = make_args(p, 2 * pair::kHeads, pairs, diag, heads);
   auto kern = pair::attn_paged_pair_kernel<D, T>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) !=
       cudaSuccess)
@@ -820,20 +910,40 @@ int launch_pair(const DsaAttnPagedParams* p, cudaStream_t stream) {
 }
 
 template <int D, typename T>
-int launch_heads(const DsaAttnPagedParams* p, cudaStream_t stream) {
-  switch (heads_of(p->n1)) {
-    case 16: return launch<D, 16, T>(p, stream);
-    case 32: return launch<D, 32, T>(p, stream);
-    case 64: return launch<D, 64, T>(p, stream);
-    default: return launch_pair<D, T>(p, stream);
+int launch_heads(const DsaAttnPagedParams* p, int diag, int heads, cudaStream_t stream) {
+  switch (heads_of(p->n1, D)) {
+    case 16: return launch<D, 16, T>(p, diag, heads, stream);
+    case 32: return launch<D, 32, T>(p, diag, heads, stream);
+    case 64: return launch<D, 64, T>(p, diag, heads, stream);
+    default:
+      if constexpr (D == 512) return launch_pair<T>(p, diag, heads, stream);
+      return DSA_ERR_INVALID_ARG;
   }
+}
+
+// Whether several new tokens of a batch can be taken as one row of s1 * n1 heads, so that their
+// keys are read once: up to 8 tokens, all of them valid, whose heads fit one work item.
+bool packs(int64_t s1, int64_t n1, int64_t d) {
+  return s1 > 1 && s1 <= kMaxDiag + 1 && s1 * n1 <= (d == 512 ? 128 : 64);
 }
 
 template <typename T>
 int launch_dim(const DsaAttnPagedParams* p, cudaStream_t stream) {
-  if (p->d == 512) return launch_heads<512, T>(p, stream);
-  if (p->d == 256) return launch_heads<256, T>(p, stream);
-  if (p->d == 128) return launch_heads<128, T>(p, stream);
+  DsaAttnPagedParams q = *p;
+  int diag = 0;
+  // (the heads of a token and the next token's have to be one step apart)
+  if (packs(p->s1, p->n1, p->d) && !p->act_q &&
+      (p->n1 == 1 || (p->q_token_stride == p->n1 * p->q_head_stride &&
+                      p->qr_token_stride == p->n1 * p->qr_head_stride))) {
+    if (p->n1 == 1) q.q_head_stride = p->q_token_stride, q.qr_head_stride = p->qr_token_stride;
+    q.n1 = p->s1 * p->n1;
+    q.s1 = 1;
+    diag = p->sparse_mode == 3 ? (int)p->s1 - 1 : 0;
+  }
+  const int heads = (int)p->n1;
+  if (p->d == 512) return launch_heads<512, T>(&q, diag, heads, stream);
+  if (p->d == 256) return launch_heads<256, T>(&q, diag, heads, stream);
+  if (p->d == 128) return launch_heads<128, T>(&q, diag, heads, stream);
   return DSA_ERR_INVALID_ARG;
 }
 
@@ -845,10 +955,14 @@ bool aligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p)
 extern "C" int64_t dsa_attn_paged_workspace_size(int64_t batch, int64_t s1, int64_t n1, int64_t d) {
   using namespace dsa::attn_paged;
   if (batch < 0 || s1 < 0 || n1 < 1 || n1 > 128 || d < 1) return -1;
-  const int64_t nh = heads_of(n1), sms = dsa::sm_count();
+  const int64_t sms = dsa::sm_count();
   if (sms < 1) return -1;
-  const int64_t shares = nh == 128 ? sms / 2 : sms;
-  return align256(2 * shares * nh * (d * 4 + 16) + (batch * s1 + 1) * 4);
+  auto size = [&](int64_t rows, int64_t heads, int64_t own) {
+    const int64_t nh = heads_of(heads, d), shares = nh == 128 ? sms / 2 : sms;
+    return align256((2 * shares + own) * nh * (d * 4 + 16) + (rows + 1) * 4);
+  };
+  const int64_t plain = size(batch * s1, n1, 0), packed = packs(s1, n1, d) ? size(batch, s1 * n1, batch) : 0;
+  return plain > packed ? plain : packed;
 }
 
 extern "C" int dsa_attn_paged(const DsaAttnPagedParams* p, void* stream_) {

@@ -26,10 +26,16 @@ struct Args {
   float* softmax_sum;
   int* error_flag;
   int32_t* ws_prefix;   // [rows + 1] units of the rows before each (of one head group)
-  float* ws_o;          // [2 * CTAs][NH][D]
-  float4* ws_s;         // [2 * CTAs][NH]: reference and running maximum (log2 units), sum,
-                        // raw running maximum
+  float* ws_o;          // [slots][NH][D], slots: two of each CTA, then one of each row (diag > 0)
+  float4* ws_s;         // [slots][NH]: reference and running maximum (log2 units), sum, raw
+                        // running maximum
   int32_t rows, s1, n1, groups;
+  // Several new tokens of a batch as one row of s1 * heads heads (s1 is 1 then): the kernels take
+  // the keys that all of them see; the last `diag` ones, which only the later tokens see, are
+  // taken in by the join.
+  int32_t diag, heads;
+  const void *q, *qr, *k, *kr;   // for the join's own products; strides in elements
+  int64_t q_batch, q_head, qr_batch, qr_head, k_page, k_row, kr_page, kr_row;
   int32_t page_size, max_blocks, num_pages, mode;
   float scale;
 };
@@ -39,7 +45,7 @@ __device__ __forceinline__ int row_keys(const Args& a, int row) {
   const int b = row / a.s1, s = row - b * a.s1;
   const int ak = a.act_k[b], aq = a.act_q ? a.act_q[b] : a.s1;
   int64_t n = min((int64_t)ak, (int64_t)a.max_blocks * a.page_size);
-  if (a.mode == 3) n = min(n, (int64_t)ak - aq + s + 1);
+  if (a.mode == 3) n = min(n, (int64_t)ak - aq + s + 1 - a.diag);
   if (s >= aq || n < 0) n = 0;
   return (int)n;
 }

@@ -1,4 +1,4 @@
-// Attention over the paged cache for more than 64 heads: a pair of CTAs per row.
+// Attention over the paged cache for more than 64 heads at D = 512: a pair of CTAs per row.
 //
 // The product of 128 heads x 512 dims fills the tensor memory of one SM, so a pair shares it
 // (cta_group::2, M = 128: 64 heads in each CTA), as it shares the operands:
@@ -485,8 +485,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const float m = fmaxf(fmaxf(wmax[h], wmax[kHeads + h]), fmaxf(wmax[2 * kHeads + h], wmax[3 * kHeads + h]));
       const bool any = m != -INFINITY;
       const float most = any ? m * c2 : -INFINITY;
-      const bool whole = sg.count == sg.tiles;
-      const int64_t slot = 2 * (blockIdx.x >> 1) + (nseg == 0 ? 0 : 1);
+      const bool all = sg.count == sg.tiles, whole = all && a.diag == 0;
+      const int64_t slot = all ? (int64_t)gridDim.x + sg.row : 2 * (blockIdx.x >> 1) + (nseg == 0 ? 0 : 1);
       const int head = kHeads * (int)rank + h;
       const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
       if (part == 0 && head < a.n1) {

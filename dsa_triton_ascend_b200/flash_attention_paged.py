@@ -70,6 +70,10 @@ def _plan(query, query_rope, key_cache, key_rope_cache, block_table, scale_value
     p.k_page_stride, p.k_row_stride = _cache_strides(key_cache, "key_cache")
     p.kr_page_stride, p.kr_row_stride = _cache_strides(key_rope_cache, "key_rope_cache")
     qs, qrs = _tma_strides(query), _tma_strides(query_rope)
+    # up to 8 tokens whose heads fit one work item share their keys, if their heads lie one step
+    # apart; queries that lie otherwise are copied rather than read token by token
+    if 1 < S1 <= 8 and 1 < N1 and S1 * N1 <= (128 if D == 512 else 64):
+        qs, qrs = [None if st is None or st[1] != N1 * st[2] else st for st in (qs, qrs)]
     contiguous = lambda w: (S1 * N1 * w, N1 * w, w)
     p.q_batch_stride, p.q_token_stride, p.q_head_stride = qs or contiguous(D)
     p.qr_batch_stride, p.qr_token_stride, p.qr_head_stride = qrs or contiguous(_D_ROPE)

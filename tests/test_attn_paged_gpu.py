@@ -277,3 +277,49 @@ def test_agrees_with_the_sparse_operator_over_every_key():
     dsa.check_device_errors()
     assert torch.allclose(out.float(), ref.float(), rtol=2e-2, atol=2e-3)
     assert torch.allclose(top, rt, rtol=1e-4, atol=1e-5) and torch.allclose(total, rl, rtol=1e-4, atol=1e-5)
+
+
+@pytest.mark.parametrize("heads,s1", [(16, 2), (1, 8), (17, 3), (64, 2), (5, 7), (32, 4), (16, 9), (100, 2)])
+@pytest.mark.parametrize("d", [128, 512])
+@pytest.mark.parametrize("mode", [0, 3])
+def test_new_tokens_that_share_their_keys(heads, s1, d, mode):
+    """Tokens of a batch are taken together where their heads fit; lengths below, at and above the
+    number of tokens, and long ones that are split."""
+    Case([0, 1, 2, s1 - 1, s1, s1 + 1, 63, 64, 65, 129, 700, 5000], heads, d, 16, s1=s1, seed=heads + s1).run(mode)
+    Case([64] * 40 + [3], heads, d, 64, s1=s1, seed=s1).run(mode)
+
+
+def test_a_later_token_leaves_the_earlier_ones_alone():
+    """NaN and infinite keys that only the last token sees."""
+    for s1, heads in ((3, 16), (2, 128), (4, 32)):
+        c = Case([200, 64, 65, s1], heads, 256, 16, s1=s1, seed=18)
+        for b, n in enumerate(c.lens):
+            c.kc[int(c.table[b, (n - 1) // 16]), (n - 1) % 16] = float("nan") if b % 2 else float("inf")
+        got = c.run(3, check=False)
+        q, qr, lens = c.q, c.qr, c.lens
+        assert not got[0][:, -1].isfinite().all()
+        # the tokens before it, against the same cache without that key
+        c.q, c.qr, c.lens = q[:, :-1].contiguous(), qr[:, :-1].contiguous(), [n - 1 for n in lens]
+        c.check([got[0][:, :-1], got[1][:, :, :-1], got[2][:, :, :-1]], 3)
+
+
+def test_shared_keys_of_a_page_that_is_not_there():
+    c = Case([35, 18], 16, 128, 8, s1=3, seed=19)
+    c.table[0, 4], c.table[1, 2] = -1, c.kc.shape[0]      # pages of the last keys
+    got = dsa.flash_attention_paged(c.q, c.qr, c.kc, c.krc, c.table, actual_seq_lengths_key=i32(c.lens),
+                                    scale_value=c.scale, sparse_mode=3, return_softmax_lse=True)
+    with pytest.raises(RuntimeError, match="bits 0x4"):
+        dsa.check_device_errors()
+    c.check(got, 3, skip={(0, 4), (1, 2)})
+
+
+def test_tokens_of_strided_queries_share_their_keys():
+    c = Case([333, 65], 20, 512, 64, s1=3, seed=20)
+    ref = c.run(3)
+    for wide in (torch.empty(2, 3, 20, 640, device="cuda", dtype=torch.bfloat16),
+                 torch.empty(3, 2, 20, 640, device="cuda", dtype=torch.bfloat16).transpose(0, 1)):
+        q, qr = wide[..., :512], wide[..., 576:]
+        q.copy_(c.q)
+        qr.copy_(c.qr)
+        c.q, c.qr = q, qr
+        assert all(torch.equal(x, y) for x, y in zip(ref, c.run(3)))
