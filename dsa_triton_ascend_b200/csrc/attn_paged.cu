@@ -198,10 +198,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     // -------------------------------------------------------------------- loads
     const int w = warp - kLoadWarp;
     // this warp loads groups 2 w and 2 w + 1 (of 8 keys) of every tile: lanes 0 and 1 their
-    // latent rows, lanes 2 and 3 the rotary ones.  (Bringing tiles into L2 ahead of their load
-    // gained 1.6 % at 64 rows of up to 16411 keys and lost 3 % at D = 256 with 64 heads.)
+    // latent rows, lanes 2 and 3 the rotary ones (lane 2 both, in boxes of 16).  (Bringing tiles
+    // into L2 ahead of their load gained 1.6 % at 64 rows of up to 16411 keys and lost 3 % at
+    // D = 256 with 64 heads.)
     const int grp = 2 * w + (lane & 1);
-    const bool is_rope = lane & 2;
+    const bool is_rope = lane & 2, loads = !is_rope || (a.box_mask >> grp & 1u);
     Segment sg;
     int g = 0;
     while (!failed && next_segment<kTile, kSegmentCost>(a, work, sg)) {
@@ -226,12 +227,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t dst = base + st * C::kStageBytes;
         if (lane == 0) {
           tmask[4 * st + w] = (int)mask;
-          const uint32_t bytes = __popc(mask) * (C::kGroupBytes + 1024);
+          const uint32_t bytes = __popc(mask) * C::kGroupBytes + __popc(mask & a.box_mask) * (a.box_rows * 128);
           if (bytes) mbar_arrive_expect_tx(full(st), bytes);
           else mbar_arrive(full(st));
         }
         __syncwarp();
-        if (now >= 0)
+        if (now >= 0 && loads)
           tma_load_4d(dst + (is_rope ? C::kKeyBytes + grp * 1024 : grp * C::kGroupBytes),
                       is_rope ? &maps.kr : &maps.k, full(st), 0, (tile * kTile + grp * 8) % a.page_size, 0, now);
       }
@@ -799,6 +800,8 @@ Args make_args(const DsaAttnPagedParams* p, int nh, int shares, int diag, int he
   a.num_pages = (int)p->num_pages;
   a.mode = p->sparse_mode;
   a.scale = p->scale;
+  a.box_rows = p->page_size % 16 ? 8 : 16;
+  a.box_mask = p->page_size % 16 ? 0xffffu : 0x5555u;
   a.diag = diag;
   a.heads = heads;
   a.q = p->query, a.qr = p->query_rope, a.k = p->key_cache, a.kr = p->key_rope_cache;
@@ -816,7 +819,8 @@ Args make_args(const DsaAttnPagedParams* p, int nh, int shares, int diag, int he
   return a;
 }
 
-// Tensor maps of the queries (boxes of `nh` heads) and keys (boxes of 8).
+// Tensor maps of the queries (boxes of `nh` heads) and keys (boxes of 8 keys; of their rotary
+// parts 16 where the page size allows).
 template <int D>
 bool make_maps(Maps* maps, const DsaAttnPagedParams* p, bool bf16, uint32_t nh) {
   const uint64_t n1 = p->n1, s1 = p->s1, b = p->batch, page = p->page_size, pages = p->num_pages;
@@ -833,7 +837,7 @@ bool make_maps(Maps* maps, const DsaAttnPagedParams* p, bool bf16, uint32_t nh) 
   const uint32_t kbox[4] = {64, 8, D / 64, 1};
   const uint64_t krdims[4] = {64, page, 1, pages};
   const uint64_t krst[3] = {(uint64_t)p->kr_row_stride * 2, 128, (uint64_t)p->kr_page_stride * 2};
-  const uint32_t krbox[4] = {64, 8, 1, 1};
+  const uint32_t krbox[4] = {64, page % 16 ? 8u : 16u, 1, 1};
   return make_tmap_16b(&maps->q, p->query, bf16, 5, dims, st, box) &&
          make_tmap_16b(&maps->qr, p->query_rope, bf16, 5, rdims, rst, rbox) &&
          make_tmap_16b(&maps->k, p->key_cache, bf16, 4, kdims, kst, kbox) &&
@@ -893,10 +897,10 @@ int launch_pair(const DsaAttnPagedParams* p, int diag, int heads, cudaStream_t s
   const int pairs = sm_count() / 2;
   if (pairs < 1) return DSA_ERR_CUDA;
   Maps maps;
-  CUtensorMap map_v;   // boxes of 8 keys, a CTA's half of the dims
+  CUtensorMap map_v;   // boxes of 8 or 16 keys, a CTA's half of the dims
   const uint64_t dims[4] = {64, (uint64_t)p->page_size, D / 64, (uint64_t)p->num_pages};
   const uint64_t st[3] = {(uint64_t)p->k_row_stride * 2, 128, (uint64_t)p->k_page_stride * 2};
-  const uint32_t box[4] = {64, 8, C::kVChunks, 1};
+  const uint32_t box[4] = {64, p->page_size % 16 ? 8u : 16u, C::kVChunks, 1};
   if (!make_maps<D>(&maps, p, kBf16, pair::kHeads) ||
       !make_tmap_16b(&map_v, p->key_cache, kBf16, 4, dims, st, box))
     return DSA_ERR_TMA_DESCRIPTOR;

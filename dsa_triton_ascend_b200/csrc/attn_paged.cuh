@@ -37,6 +37,10 @@ struct Args {
   const void *q, *qr, *k, *kr;   // for the join's own products; strides in elements
   int64_t q_batch, q_head, qr_batch, qr_head, k_page, k_row, kr_page, kr_row;
   int32_t page_size, max_blocks, num_pages, mode;
+  // keys of a box of rotary parts or (pair kernel) of values, 8 or 16, and the groups of 8 of a
+  // tile at which one begins
+  int32_t box_rows;
+  uint32_t box_mask;
   float scale;
 };
 

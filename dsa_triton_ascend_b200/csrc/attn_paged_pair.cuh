@@ -33,8 +33,6 @@ constexpr int kKeyWarp = 8;         // warps 8-11 load K
 constexpr int kValueWarp = 12;      // warps 12, 13 load V, warp 12 the queries too
 constexpr int kMmaWarp = 14;
 constexpr int kThreads = 480;
-constexpr int kMaxStages = 3;
-constexpr int kMaxSlots = 6;        // halves of V
 
 template <int D>
 struct Cfg {
@@ -43,27 +41,20 @@ struct Cfg {
   static constexpr int kKeyBytes = 8 * kGroupBytes;            // this CTA's 64 keys
   static constexpr int kKBytes = kKeyBytes + 64 * 128;         // and their rotary parts
   static constexpr int kVChunks = D / 128;                     // this CTA's dims
-  static constexpr int kVGroupBytes = kVChunks * 1024;
-  static constexpr int kHalfBytes = 8 * kVGroupBytes;          // 64 keys
-  static constexpr int kVBytes = 2 * kHalfBytes;
+  static constexpr int kHalfBytes = kVChunks * 64 * 128;       // of V: 64 keys
   static constexpr int kQBytes = kHeads * (D + kRope) * 2;
   static constexpr int kPBytes = kHeads * kTile * 2;
-  static constexpr int kSmallBytes = 2 * 4 * kHeads * 4 + 640;
-  static constexpr int kRoom = (kSmemLimit - kQBytes - kPBytes - kSmallBytes) / (kKBytes + kVBytes);
-  static constexpr int kStages = kRoom < kMaxStages ? kRoom : kMaxStages;   // of K and of V
-  static constexpr int kVSlots = kStages * 2;
-  static constexpr int kQBufs =
-      kStages * (kKBytes + kVBytes) + 2 * kQBytes + kPBytes + kSmallBytes <= kSmemLimit ? 2 : 1;
-  static constexpr int kOffK = kQBufs * kQBytes;
-  static constexpr int kOffV = kOffK + kStages * kKBytes;
-  static constexpr int kOffP = kOffV + kStages * kVBytes;
+  static constexpr int kSmallBytes = 2 * 4 * kHeads * 4 + 384;
+  static constexpr int kOffK = kQBytes;
+  static constexpr int kOffV = kOffK + kKBytes;
+  static constexpr int kOffP = kOffV + 2 * kHalfBytes;
   static constexpr int kOffSmall = kOffP + kPBytes;
   static constexpr int kSmem = kOffSmall + kSmallBytes;
-  static constexpr int kPvN = D < 256 ? D : 256;               // dims of one PV instruction
+  static constexpr int kPvN = 256;                             // dims of one PV instruction
   static constexpr int kPvs = D / kPvN;
   static constexpr uint32_t kColsO = 128;                      // after two buffers of S
-  static constexpr uint32_t kTmem = D == 512 ? 512 : 256;
-  static_assert(kStages >= 1 && kVSlots <= kMaxSlots && kOffK % 1024 == 0 && kOffV % 1024 == 0 && kOffP % 1024 == 0, "layout");
+  static constexpr uint32_t kTmem = 512;
+  static_assert(D == 512 && kSmem <= kSmemLimit, "one buffer of each operand has to fit");
 };
 
 // The tiles of a share one by one.
@@ -95,23 +86,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   float* wmax = reinterpret_cast<float*>(smem + C::kOffSmall);   // [4][kHeads]
   float* wsum = wmax + 4 * kHeads;                               // [4][kHeads]
   uint64_t* bars = reinterpret_cast<uint64_t*>(wsum + 4 * kHeads);
-  int32_t* tmp = reinterpret_cast<int32_t*>(bars + 48);          // [16]
+  int32_t* tmp = reinterpret_cast<int32_t*>(bars + 16);          // [16]
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(tmp + 16);
   int32_t* start = reinterpret_cast<int32_t*>(tmem_ptr + 1);     // [3]
 
   const uint32_t b0 = smem_u32(bars);
-  auto k_full = [&](int s) { return b0 + 8u * s; };                     // leader's
-  auto k_empty = [&](int s) { return b0 + 8u * (kMaxSlots + s); };
-  auto v_full = [&](int s) { return b0 + 8u * (2 * kMaxSlots + s); };   // leader's
-  auto v_empty = [&](int s) { return b0 + 8u * (3 * kMaxSlots + s); };
-  auto v_tail = [&](int s) { return b0 + 8u * (4 * kMaxSlots + s); };
-  auto s_full = [&](int s) { return b0 + 8u * (5 * kMaxSlots + s); };
-  auto q_full = [&](int s) { return b0 + 8u * (5 * kMaxSlots + 2 + s); };   // leader's
-  auto q_empty = [&](int s) { return b0 + 8u * (5 * kMaxSlots + 4 + s); };
-  const uint32_t p_full = b0 + 8u * (5 * kMaxSlots + 6);       // leader's
-  const uint32_t p_empty = b0 + 8u * (5 * kMaxSlots + 7);
-  const uint32_t o_empty = b0 + 8u * (5 * kMaxSlots + 8);      // leader's
-  const uint32_t drained = b0 + 8u * (5 * kMaxSlots + 9);
+  const uint32_t k_full = b0, k_empty = b0 + 8;                // the leader's; each CTA's
+  auto v_full = [&](int s) { return b0 + 16u + 8u * s; };      // leader's
+  auto v_empty = [&](int s) { return b0 + 32u + 8u * s; };
+  auto v_tail = [&](int s) { return b0 + 48u + 8u * s; };
+  auto s_full = [&](int s) { return b0 + 64u + 8u * s; };
+  const uint32_t q_full = b0 + 80, q_empty = b0 + 88;          // leader's; each CTA's
+  const uint32_t p_full = b0 + 96, p_empty = b0 + 104;         // leader's; each CTA's
+  const uint32_t o_empty = b0 + 112, drained = b0 + 120;       // leader's
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (base & 1023u) {   // the same in both CTAs
@@ -120,19 +107,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   }
   const uint32_t rank = cluster_ctarank();
   if (threadIdx.x == 0) {
-    for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(k_full(s), 4);
-      mbar_init(k_empty(s), 1);
-    }
-    for (int s = 0; s < C::kVSlots; ++s) {
+    mbar_init(k_full, 4);
+    mbar_init(k_empty, 1);
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int s = 0; s < 2; ++s) {
       mbar_init(v_full(s), 2);
       mbar_init(v_empty(s), 1);
       mbar_init(v_tail(s), 2);
-    }
-    for (int s = 0; s < 2; ++s) {
       mbar_init(s_full(s), 1);
-      mbar_init(q_full(s), 1);
-      mbar_init(q_empty(s), 1);
     }
     mbar_init(p_full, 16);
     mbar_init(drained, 1);
@@ -180,36 +163,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     int g = 0, page = -1;
     for (; t.next(a); ++g) {
       const int32_t* table = table_of(t.s);
-      const int tile = t.s.first + t.i, st = g % C::kStages;
+      const int tile = t.s.first + t.i;
       const int now = t.i == 0 ? page_of(t.s, table, tile, rank == 0 && w == 0) : page;
       if (t.i + 1 < t.s.count) page = page_of(t.s, table, tile + 1, rank == 0 && w == 0);
       const uint32_t mask = __ballot_sync(0xffffffffu, now >= 0);
       const int in_page = (tile * kTile + lane * 8) % a.page_size;
-      if (g >= C::kStages) mbar_wait_hot(k_empty(st), (g / C::kStages - 1) & 1, a.error_flag, &failed);
+      if (g > 0) mbar_wait_hot(k_empty, (g - 1) & 1, a.error_flag, &failed);
       failed = __any_sync(0xffffffffu, failed);
       if (failed) break;
       if (rank == 0 && lane == 0) {
-        const uint32_t bytes = __popc(mask & (3u << (2 * w) | 3u << (8 + 2 * w))) * (C::kGroupBytes + 1024);
-        if (bytes) mbar_arrive_expect_tx(k_full(st), bytes);
-        else mbar_arrive(k_full(st));
+        // (of a rotary box of 16 keys the first half has to be there)
+        const uint32_t both = mask & (3u << (2 * w) | 3u << (8 + 2 * w));
+        const uint32_t bytes = __popc(both) * C::kGroupBytes + __popc(both & a.box_mask) * (a.box_rows * 128);
+        if (bytes) mbar_arrive_expect_tx(k_full, bytes);
+        else mbar_arrive(k_full);
       }
       __syncwarp();
       if (now >= 0 && (lane == g0 || lane == g0 + 1)) {
-        const uint32_t bar = mapa_shared(k_full(st), 0), dst = base + C::kOffK + st * C::kKBytes;
+        const uint32_t bar = mapa_shared(k_full, 0), dst = base + C::kOffK;
         tma_load_4d_pair(dst + grp * C::kGroupBytes, &maps.k, bar, 0, in_page, 0, now);
-        tma_load_4d_pair(dst + C::kKeyBytes + grp * 1024, &maps.kr, bar, 0, in_page, 0, now);
+        if (a.box_mask >> lane & 1u)
+          tma_load_4d_pair(dst + C::kKeyBytes + grp * 1024, &maps.kr, bar, 0, in_page, 0, now);
       }
       __syncwarp();
     }
     if (failed && rank == 0) {   // the copies in flight, of both CTAs, land before the pair ends
       bool gave_up = false;
-      for (int u = max(0, g - C::kStages); u < g; ++u)
-        mbar_wait(k_full(u % C::kStages), (u / C::kStages) & 1, a.error_flag, &gave_up, true);
+      if (g > 0) mbar_wait(k_full, (g - 1) & 1, a.error_flag, &gave_up, true);
     }
     __syncwarp();
   } else if (warp >= kValueWarp && warp < kMmaWarp) {
     // -------------------------------------------------------------------- V, queries
-    // This warp loads 4 groups (of 8 keys) of each half of the tile, this CTA's dims of them.
+    // This warp loads half of each half of the tile, this CTA's dims of it, in boxes of box_rows keys,
+    // [box][chunk][box_rows][128 B]; 16 where the page size allows, as a box takes a warp 160 cycles.
     // A tile with keys that are not there completes on barriers of the CTA's own, since its
     // softmax warps clear those rows before the product; their P then tells the leader.
     const int w = warp - kValueWarp;
@@ -225,43 +211,40 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const int in_page = (tile * kTile + lane * 8) % a.page_size;
       if (w == 0 && t.i == 0) {
         const int b = t.s.row / a.s1, s = t.s.row - b * a.s1;
-        const int buf = t.seg % C::kQBufs, use = t.seg / C::kQBufs;
-        if (use > 0) mbar_wait_hot(q_empty(buf), (use - 1) & 1, a.error_flag, &failed);
+        if (t.seg > 0) mbar_wait_hot(q_empty, (t.seg - 1) & 1, a.error_flag, &failed);
         failed = __any_sync(0xffffffffu, failed);
         if (failed) break;
         if (lane == 0) {
-          const uint32_t dst = base + buf * C::kQBytes, bar = mapa_shared(q_full(buf), 0);
-          if (rank == 0) mbar_arrive_expect_tx(q_full(buf), 2 * C::kQBytes);
-          tma_load_5d_pair(dst, &maps.q, bar, 0, kHeads * (int)rank, 0, s, b);
-          tma_load_5d_pair(dst + kHeads * D * 2, &maps.qr, bar, 0, kHeads * (int)rank, 0, s, b);
+          const uint32_t bar = mapa_shared(q_full, 0);
+          if (rank == 0) mbar_arrive_expect_tx(q_full, 2 * C::kQBytes);
+          tma_load_5d_pair(base, &maps.q, bar, 0, kHeads * (int)rank, 0, s, b);
+          tma_load_5d_pair(base + kHeads * D * 2, &maps.qr, bar, 0, kHeads * (int)rank, 0, s, b);
         }
         __syncwarp();
       }
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
-        const int u = 2 * g + hf, slot = u % C::kVSlots;
-        if (u >= C::kVSlots) mbar_wait_hot(v_empty(slot), (u / C::kVSlots - 1) & 1, a.error_flag, &failed);
+        if (g > 0) mbar_wait_hot(v_empty(hf), (g - 1) & 1, a.error_flag, &failed);
         failed = __any_sync(0xffffffffu, failed);
         if (failed) break;
         if (lane == 0) {
-          const uint32_t bytes = __popc(mask & (0xfu << (8 * hf + 4 * w))) * C::kVGroupBytes;
+          const uint32_t bytes = __popc(mask & a.box_mask & (0xfu << (8 * hf + 4 * w))) * (a.box_rows * C::kVChunks * 128);
           if (tail) {
-            if (bytes) mbar_arrive_expect_tx(v_tail(slot), bytes);
-            else mbar_arrive(v_tail(slot));
+            if (bytes) mbar_arrive_expect_tx(v_tail(hf), bytes);
+            else mbar_arrive(v_tail(hf));
           }
           if (rank == 0) {
-            if (tail) mbar_arrive(v_full(slot));
-            else mbar_arrive_expect_tx(v_full(slot), 2 * bytes);
+            if (tail) mbar_arrive(v_full(hf));
+            else mbar_arrive_expect_tx(v_full(hf), 2 * bytes);
           }
         }
         __syncwarp();
-        if (now >= 0 && lane < 16 && (lane >> 2) == 2 * hf + w) {
-          const uint32_t dst = base + C::kOffV + slot * C::kHalfBytes + (lane & 7) * C::kVGroupBytes;
+        if (now >= 0 && lane < 16 && (lane >> 2) == 2 * hf + w && (a.box_mask >> lane & 1u)) {
+          const uint32_t dst = base + C::kOffV + lane * (C::kVChunks * 1024);
           if (tail)
-            tma_load_4d(dst, &map_v, v_tail(slot), 0, in_page, C::kVChunks * (int)rank, now);
+            tma_load_4d(dst, &map_v, v_tail(hf), 0, in_page, C::kVChunks * (int)rank, now);
           else
-            tma_load_4d_pair(dst, &map_v, mapa_shared(v_full(slot), 0), 0, in_page,
-                             C::kVChunks * (int)rank, now);
+            tma_load_4d_pair(dst, &map_v, mapa_shared(v_full(hf), 0), 0, in_page, C::kVChunks * (int)rank, now);
         }
         __syncwarp();
       }
@@ -269,8 +252,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
     if (failed && rank == 0) {
       bool gave_up = false;
-      for (int u = max(0, 2 * (g - C::kStages)); u < 2 * g; ++u)
-        mbar_wait(v_full(u % C::kVSlots), (u / C::kVSlots) & 1, a.error_flag, &gave_up, true);
+      for (int hf = 0; hf < 2 && g > 0; ++hf)
+        mbar_wait(v_full(hf), (g - 1) & 1, a.error_flag, &gave_up, true);
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
@@ -282,22 +265,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       // which goes half by half, as there are two buffers of scores and PV(na - 2) waited for the
       // probabilities made of S(na - 2).  One warp issues both whole: with a warp for each (as in
       // the other kernel) their instructions alternate, and the same rows took 395 us for 349.
+      // bytes between V's groups of 8 keys, and between its 128 dims of one instruction and the next
+      const uint32_t v_group = a.box_rows == 16 ? 1024 : C::kVChunks * 1024;
+      const uint32_t v_next = (2 * a.box_rows * 128) >> 4;
       Tiles q{work, {}, 0, -1}, v{work, {}, 0, -1};
       bool more_q = q.next(a), more_v = v.next(a);
       int na = 0, nb = 0, pb = 0;
       uint64_t t0 = 0;
       auto all = [](bool x) { return __all_sync(0xffffffffu, x) != 0; };
       for (uint32_t idle = 0; more_v && !failed;) {
-        const int sa = na % C::kStages;
-        const int ub = 2 * nb + pb, sb = ub % C::kVSlots;
-        const int buf = q.seg % C::kQBufs;
         if (more_q && na - nb < 2 &&
-            all((q.i > 0 || mbar_test_wait_cluster(q_full(buf), (q.seg / C::kQBufs) & 1)) &&
-                mbar_test_wait_cluster(k_full(sa), (na / C::kStages) & 1))) {
+            all((q.i > 0 || mbar_test_wait_cluster(q_full, q.seg & 1)) && mbar_test_wait_cluster(k_full, na & 1))) {
           tc_fence_after();
           if (elect_one()) {
-            const uint64_t qa = smem_desc_sw128(base + buf * C::kQBytes, 16, 1024);
-            const uint32_t ks = base + C::kOffK + sa * C::kKBytes;
+            const uint64_t qa = smem_desc_sw128(base, 16, 1024);
+            const uint32_t ks = base + C::kOffK;
             const uint64_t kb = smem_desc_sw128(ks, 16, C::kGroupBytes);
             const uint64_t rb = smem_desc_sw128(ks + C::kKeyBytes, 16, 1024);
             const uint32_t d = tmem + 64 * (na & 1);
@@ -311,8 +293,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             for (int u = 0; u < 4; ++u)
               umma_f16<2>(d, qa + ((C::kChunks * kHeads * 128 + u * 32) >> 4), rb + ((u * 32) >> 4), kIdQk, 1);
             umma_commit_pair(s_full(na & 1), 3);
-            umma_commit_pair(k_empty(sa), 3);
-            if (q.i == q.s.count - 1) umma_commit_pair(q_empty(buf), 3);
+            umma_commit_pair(k_empty, 3);
+            if (q.i == q.s.count - 1) umma_commit_pair(q_empty, 3);
           }
           __syncwarp();
           more_q = q.next(a);
@@ -321,19 +303,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           continue;
         }
         if (nb < na && all((pb > 0 || mbar_test_wait_cluster(p_full, nb & 1)) &&
-                           mbar_test_wait_cluster(v_full(sb), (ub / C::kVSlots) & 1) &&
+                           mbar_test_wait_cluster(v_full(pb), nb & 1) &&
                            (v.i + pb > 0 || v.seg == 0 || mbar_test_wait_cluster(o_empty, (v.seg - 1) & 1)))) {
           tc_fence_after();
           if (elect_one()) {
             const uint64_t pd = smem_desc_sw128(base + C::kOffP + pb * (kHeads * 128), 16, 1024);
-            const uint64_t vb = smem_desc_sw128(base + C::kOffV + sb * C::kHalfBytes, 1024, C::kVGroupBytes);
+            const uint64_t vb = smem_desc_sw128(base + C::kOffV + pb * C::kHalfBytes, a.box_rows * 128, v_group);
 #pragma unroll
             for (int k = 0; k < 4; ++k)
 #pragma unroll
               for (int n = 0; n < C::kPvs; ++n)
                 umma_f16<2>(tmem + C::kColsO + n * (C::kPvN / 2), pd + ((k * 32) >> 4),
-                            vb + ((k * 2 * C::kVGroupBytes + n * 2048) >> 4), kIdPv, (v.i + pb > 0) | (k > 0));
-            umma_commit_pair(v_empty(sb), 3);
+                            vb + ((k * 16 * C::kVChunks * 128) >> 4) + n * v_next, kIdPv, (v.i + pb > 0) | (k > 0));
+            umma_commit_pair(v_empty(pb), 3);
             if (pb == 1) umma_commit_pair(p_empty, 3);
           }
           __syncwarp();
@@ -378,7 +360,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     Work w = work;
     Segment sg;
     int g = 0, nseg = 0;
-    uint32_t tails = 0;   // parity of each slot's halves of tiles with keys that are not there
+    int tails = 0;   // tiles with keys that are not there
     while (next_segment<kTile, kSegmentCost>(a, w, sg)) {
       const int32_t* table = table_of(sg);
       float ref = -INFINITY, lim = -INFINITY, run = -INFINITY, sum = 0.0f;
@@ -457,15 +439,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           // rows of this tile that no key stands in hold what was there before (or a page's
           // stale tail): cleared, so that 0 x NaN cannot enter the product
           const int key = threadIdx.x >> 1;
-          const int s0 = 2 * g % C::kVSlots, slot = s0 + (key >> 6);   // of this thread's half
-          mbar_wait_hot(v_tail(slot), tails >> slot & 1, a.error_flag, &failed);
-          tails ^= 3u << s0;
+          mbar_wait_hot(v_tail(key >> 6), tails & 1, a.error_flag, &failed);
+          ++tails;
           if (key >= valid || !(mask >> (key >> 3) & 1u)) {
-            uint8_t* row = smem + C::kOffV + slot * C::kHalfBytes + (key >> 3 & 7) * C::kVGroupBytes + (key & 7) * 128;
+            const int box = key / a.box_rows;
+            uint8_t* row = smem + C::kOffV + box * (a.box_rows * C::kVChunks * 128) + (key - box * a.box_rows) * 128;
             for (int c = threadIdx.x & 1; c < C::kVChunks; c += 2)
 #pragma unroll
               for (int x = 0; x < 8; ++x)
-                *reinterpret_cast<uint4*>(row + c * 1024 + x * 16) = make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4*>(row + c * (a.box_rows * 128) + x * 16) = make_uint4(0, 0, 0, 0);
           }
         }
         fence_proxy_async_smem();
