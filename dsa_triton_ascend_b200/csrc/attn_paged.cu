@@ -534,8 +534,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             a.ws_s[slot * NH + h] = make_float4(ref[j] - kShift, most, l, m);
           } else if (a.softmax_max) {
             const int64_t at = (int64_t)sg.row * a.n1 + head;
-            a.softmax_max[at] = any ? m * fabsf(a.scale) : 0.0f;
-            a.softmax_sum[at] = any ? l * exp2f(ref[j] - kShift - most) : 0.0f;
+            put_stats(a, at, m, ref[j] - kShift, most, l);
           }
         }
       softmax_bar(wg);
@@ -711,18 +710,16 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_combine_kernel(const 
 #pragma unroll
   for (int i = 0; i < kPer; ++i) acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float sum = 0.0f;
-  if (ref != -INFINITY) {
 #pragma unroll 4
-    for (int c = p.c0 + grp; c <= p.c1; c += kGroups) {
-      const float4 s = a.ws_s[p.at<NH>(c, h)];
-      const float4* o = reinterpret_cast<const float4*>(a.ws_o + p.at<NH>(c, h) * D) + col;
-      const float w = s.x == ref ? 1.0f : exp2f(s.x - ref);
-      sum += w * s.z;
+  for (int c = p.c0 + grp; c <= p.c1; c += kGroups) {
+    const float4 s = a.ws_s[p.at<NH>(c, h)];
+    const float4* o = reinterpret_cast<const float4*>(a.ws_o + p.at<NH>(c, h) * D) + col;
+    const float w = s.x == ref ? 1.0f : exp2f(s.x - ref);
+    sum += w * s.z;
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const float4 x = o[i * kCols];
-        acc[i].x += w * x.x, acc[i].y += w * x.y, acc[i].z += w * x.z, acc[i].w += w * x.w;
-      }
+    for (int i = 0; i < kPer; ++i) {
+      const float4 x = o[i * kCols];
+      acc[i].x += w * x.x, acc[i].y += w * x.y, acc[i].z += w * x.z, acc[i].w += w * x.w;
     }
   }
   if constexpr (kWide) {
@@ -766,11 +763,7 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_combine_kernel(const 
   for (int i = 0; i < kPer; ++i)
     *reinterpret_cast<uint2*>(out + (i * kCols + col) * 4) =
         make_uint2(E::pack2(acc[i].x * inv, acc[i].y * inv), E::pack2(acc[i].z * inv, acc[i].w * inv));
-  if (t == 0 && a.softmax_max) {
-    const bool any = run != -INFINITY;
-    a.softmax_max[at] = any ? top * fabsf(a.scale) : 0.0f;
-    a.softmax_sum[at] = any ? sum * exp2f(ref - run) : 0.0f;
-  }
+  if (t == 0 && a.softmax_max) put_stats(a, at, top, ref, run, sum);
 }
 
 // Heads of a work item: the smallest operand that holds them.  Past 64 the pair kernel takes them

@@ -214,6 +214,15 @@ __device__ __forceinline__ Work share_of(const Args& a, int cta, int ctas_max, b
   return work;
 }
 
+// The statistics of one (row, head): raw maximum `top`, sum over the exponents' reference `ref`,
+// whose running maximum is `run` (log2 units).  A sum that is NaN (a NaN or infinite score) makes
+// both NaN.
+__device__ __forceinline__ void put_stats(const Args& a, int64_t at, float top, float ref, float run, float sum) {
+  const bool any = run != -INFINITY, bad = sum != sum;
+  a.softmax_max[at] = bad ? sum : any ? top * fabsf(a.scale) : 0.0f;
+  a.softmax_sum[at] = bad ? sum : any ? sum * exp2f(ref - run) : 0.0f;
+}
+
 // 2^x, 2^-126 and below flushed to 0
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;

@@ -476,8 +476,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           a.ws_s[slot * (2 * kHeads) + head] = make_float4(ref - kShift, most, l, m);
         } else if (a.softmax_max) {
           const int64_t at = (int64_t)sg.row * a.n1 + head;
-          a.softmax_max[at] = any ? m * fabsf(a.scale) : 0.0f;
-          a.softmax_sum[at] = any ? l * exp2f(ref - kShift - most) : 0.0f;
+          put_stats(a, at, m, ref - kShift, most, l);
         }
       }
       mbar_wait_hot(p_empty, (g - 1) & 1, a.error_flag, &failed);

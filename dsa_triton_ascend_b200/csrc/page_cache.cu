@@ -395,7 +395,7 @@ __global__ void __launch_bounds__(kApplyThreads)
   griddep_wait();
   if (do_table && a.op != DSA_PAGES_COPY) {
     // a warp per row, or per kRowPiece entries of it
-    constexpr int kRowPiece = 1024;
+    constexpr int kRowPiece = 128;
     const int lane = threadIdx.x & 31;
     const int warps = gridDim.x * (kApplyThreads / 32), me = blockIdx.x * (kApplyThreads / 32) + (threadIdx.x >> 5);
     const int per_row = (a.max_blocks + kRowPiece - 1) / kRowPiece;
@@ -637,7 +637,7 @@ extern "C" int dsa_pages(const DsaPagesParams* p, void* stream_) {
     }
     int64_t blocks = (int64_t)sms * 8;
     if (c.count == 0) {
-      const int64_t need = p->slots * ((p->max_blocks + 1023) / 1024) / (kApplyThreads / 32) + 1;
+      const int64_t need = p->slots * ((p->max_blocks + 127) / 128) / (kApplyThreads / 32) + 1;
       if (need < blocks) blocks = need;
     }
     cudaLaunchConfig_t cfg = {};

@@ -323,3 +323,21 @@ def test_tokens_of_strided_queries_share_their_keys():
         qr.copy_(c.qr)
         c.q, c.qr = q, qr
         assert all(torch.equal(x, y) for x, y in zip(ref, c.run(3)))
+
+
+@pytest.mark.parametrize("heads,d", [(16, 512), (128, 512), (100, 256)])
+@pytest.mark.parametrize("lens", [[100, 40], [9000, 3000]])    # whole rows, split rows
+def test_nan_where_it_is_seen(heads, d, lens):
+    """A NaN query makes its own head's row NaN, a NaN key its sequence's; nothing else."""
+    c = Case(lens, heads, d, 64, seed=21)
+    ref = c.run()
+    c.q[0, 0, 3] = float("nan")
+    got = c.run(check=False)
+    rest = [h for h in range(heads) if h != 3]
+    assert got[0][0, 0, 3].isnan().all() and got[1][0, 0, 0, 3].isnan() and got[2][0, 0, 0, 3].isnan()
+    assert torch.equal(got[0][:, :, rest], ref[0][:, :, rest]) and torch.equal(got[0][1], ref[0][1])
+    c.q[0, 0, 3] = 0.0
+    c.krc[int(c.table[1, 0]), 5, 0, 7] = float("nan")
+    got = c.run(check=False)
+    assert got[0][1].isnan().all() and got[1][1].isnan().all() and got[2][1].isnan().all()
+    assert torch.equal(got[0][0][:, rest], ref[0][0][:, rest]) and got[0][0].isfinite().all()
