@@ -25,12 +25,12 @@ namespace pages {
 // ---------------------------------------------------------------------------------------
 // append
 // ---------------------------------------------------------------------------------------
-constexpr int kAppendThreads = 256;
-constexpr int kInFlight = 4;   // pieces of a lane that are loaded before any is stored
+constexpr int kAppendThreads = 128;
+constexpr int kInFlight = 4;   // copied pieces of a lane that are loaded before any is stored
 
 struct AppendArgs {
-  DsaCacheRows e[DSA_APPEND_MAX_ENTRIES];
-  uint32_t first[DSA_APPEND_MAX_ENTRIES + 1];   // first piece of each entry
+  DsaCacheRows e[DSA_APPEND_MAX_ENTRIES];       // copied rows first, then the rotated ones
+  uint32_t first[DSA_APPEND_MAX_ENTRIES + 1];   // first piece of each entry, of its kind
   const int32_t* block_table;
   const int32_t* starts;
   const int32_t* counts;
@@ -38,28 +38,58 @@ struct AppendArgs {
   int* error_flag;
   int64_t tokens;
   rotary::FastDiv page;
-  uint32_t units;
-  int32_t entries, s, max_blocks, num_pages, max_positions, dim;
+  uint32_t copied, turned;   // pieces
+  int32_t plain, entries, s, max_blocks, num_pages, max_positions, dim;
 };
 
-// The rotation of one piece (in the half layout of a pair of pieces, `v` and `w`) at value `in`
-// of the rotated part.
+// A piece of a rotated row: an interleaved one, a pair of the half layout, or one that is copied.
 template <typename T>
-__device__ __forceinline__ void turn_piece(const AppendArgs& a, bool pair, int64_t pos, int in, uint4& v, uint4& w) {
-  constexpr int kN = rotary::Vec<T>::kN;
-  const float* row = a.table + pos * a.dim;
-  if (!pair) {
-    float cs[kN / 2], sn[kN / 2];
-    rotary::load_angles<kN / 2>(row, a.dim / 2, in / 2, 1.0f, cs, sn);
-    v = rotary::turn_interleaved<T>(v, cs, sn);
-  } else {
-    float cs[kN], sn[kN];
-    rotary::load_angles<kN>(row, a.dim / 2, in, 1.0f, cs, sn);
-    rotary::turn_half<T>(v, w, cs, sn);
+struct Piece {
+  static constexpr int kN = rotary::Vec<T>::kN;
+  uint4 v, w;
+  int entry, at;   // byte offset in the row
+  bool pair, turned;
+  __device__ __forceinline__ void load(const AppendArgs& a, uint32_t u, int64_t b, int s) {
+    int i = a.plain;
+    while (i + 1 < a.entries && u >= a.first[i + 1]) ++i;
+    const DsaCacheRows& e = a.e[i];
+    entry = i;
+    const int half = a.dim / 2, piece = (int)(u - a.first[i]) * kN;
+    int in = piece;   // value in the row
+    pair = e.rotary == DSA_ROTARY_HALF && piece < half;
+    if (pair) {
+      in = (int)e.offset + piece;
+    } else if (e.rotary == DSA_ROTARY_HALF) {   // the copied ones, around the rotated part
+      in = piece - half;
+      if (in >= e.offset) in += a.dim;
+    }
+    turned = pair || (e.rotary == DSA_ROTARY_INTERLEAVED && in >= e.offset && in < e.offset + a.dim);
+    at = in * (int)sizeof(T);
+    const char* src = static_cast<const char*>(e.src) + b * e.src_batch_stride + s * e.src_token_stride + at;
+    v = *reinterpret_cast<const uint4*>(src);
+    if (pair) w = *reinterpret_cast<const uint4*>(src + half * sizeof(T));
   }
-}
+  __device__ __forceinline__ void store(const AppendArgs& a, int64_t pos, int32_t page, uint32_t row) {
+    const DsaCacheRows& e = a.e[entry];
+    char* dst = static_cast<char*>(e.cache) + page * e.page_stride + row * e.row_stride + at;
+    const float* angles = a.table + pos * a.dim;
+    const int half = a.dim / 2, in = at / (int)sizeof(T) - (int)e.offset;
+    if (pair) {
+      float cs[kN], sn[kN];
+      rotary::load_angles<kN>(angles, half, in, 1.0f, cs, sn);
+      rotary::turn_half<T>(v, w, cs, sn);
+      *reinterpret_cast<uint4*>(dst + half * sizeof(T)) = w;
+    } else if (turned) {
+      float cs[kN / 2], sn[kN / 2];
+      rotary::load_angles<kN / 2>(angles, half, in / 2, 1.0f, cs, sn);
+      v = rotary::turn_interleaved<T>(v, cs, sn);
+    }
+    *reinterpret_cast<uint4*>(dst) = v;
+  }
+};
 
-// A warp per token: its rows are read while its page is looked up, kInFlight pieces a lane.
+// A warp per token: its rows are read while its page is looked up.  Rotated rows hold values of T.
+template <typename T>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ AppendArgs a) {
   const int lane = threadIdx.x & 31;
   const int64_t token = (int64_t)blockIdx.x * (kAppendThreads / 32) + (threadIdx.x >> 5);
@@ -73,54 +103,43 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
   const uint32_t block = pos >= 0 && pos < (1LL << 31) - 1 ? a.page.div((uint32_t)pos) : (uint32_t)a.max_blocks;
   int32_t page = -1;
   if (block < (uint32_t)a.max_blocks) page = a.block_table[b * a.max_blocks + block];
-  for (uint32_t u0 = lane; u0 < a.units; u0 += 32 * kInFlight) {
-    uint4 v[kInFlight], w[kInFlight];
-    int at[kInFlight], entry[kInFlight];   // byte offset in the row; w is `half` bytes further
+  Piece<T> piece;
+  if ((uint32_t)lane < a.turned) piece.load(a, lane, b, s);
+  bool known = false;
+  auto look = [&]() {   // first looked at with loads in flight
+    known = page >= 0 && page < a.num_pages && !(a.table && pos >= a.max_positions);
+    if (!known && lane == 0) report_error(a.error_flag, kErrBadIndex);
+  };
+  const uint32_t row = (uint32_t)pos - block * a.page.d;
+  for (uint32_t u0 = lane; u0 < a.copied; u0 += 32 * kInFlight) {
+    uint4 v[kInFlight];
+    int at[kInFlight], entry[kInFlight];
 #pragma unroll
     for (int k = 0; k < kInFlight; ++k) {
       const uint32_t u = u0 + 32 * k;
-      if (u >= a.units) break;
+      if (u >= a.copied) break;
       int i = 0;
-      while (i + 1 < a.entries && u >= a.first[i + 1]) ++i;
+      while (i + 1 < a.plain && u >= a.first[i + 1]) ++i;
       const DsaCacheRows& e = a.e[i];
       entry[k] = i;
-      int in = (int)(u - a.first[i]) * 16;
-      const char* src = static_cast<const char*>(e.src) + b * e.src_batch_stride + s * e.src_token_stride;
-      if (e.rotary == DSA_ROTARY_HALF) {
-        const int size = e.dtype == DSA_DTYPE_FP32 ? 4 : 2, half = a.dim / 2 * size, off = (int)e.offset * size;
-        if (in < half) {   // the first pieces are pairs
-          in += off;
-          w[k] = *reinterpret_cast<const uint4*>(src + in + half);
-        } else {           // then come the copied ones, around the rotated part
-          in -= half;
-          if (in >= off) in += 2 * half;
-        }
-      }
-      at[k] = in;
-      v[k] = *reinterpret_cast<const uint4*>(src + in);
+      at[k] = (int)(u - a.first[i]) * 16;
+      v[k] = *reinterpret_cast<const uint4*>(static_cast<const char*>(e.src) + b * e.src_batch_stride +
+                                             s * e.src_token_stride + at[k]);
     }
-    if (page < 0 || page >= a.num_pages || (a.table && pos >= a.max_positions)) {
-      if (lane == 0) report_error(a.error_flag, kErrBadIndex);
-      return;
-    }
-    const uint32_t row = (uint32_t)pos - block * a.page.d;
+    if (u0 == (uint32_t)lane) look();
+    if (!known) return;
 #pragma unroll
     for (int k = 0; k < kInFlight; ++k) {
-      if (u0 + 32 * k >= a.units) break;
+      if (u0 + 32 * k >= a.copied) break;
       const DsaCacheRows& e = a.e[entry[k]];
-      char* dst = static_cast<char*>(e.cache) + page * e.page_stride + row * e.row_stride + at[k];
-      if (e.rotary != DSA_ROTARY_NONE) {
-        const int size = e.dtype == DSA_DTYPE_FP32 ? 4 : 2, in = at[k] / size - (int)e.offset;
-        const bool pair = e.rotary == DSA_ROTARY_HALF;
-        if (in >= 0 && in < (pair ? a.dim / 2 : a.dim)) {
-          if (e.dtype == DSA_DTYPE_BF16) turn_piece<__nv_bfloat16>(a, pair, pos, in, v[k], w[k]);
-          else if (e.dtype == DSA_DTYPE_FP16) turn_piece<__half>(a, pair, pos, in, v[k], w[k]);
-          else turn_piece<float>(a, pair, pos, in, v[k], w[k]);
-          if (pair) *reinterpret_cast<uint4*>(dst + a.dim / 2 * size) = w[k];
-        }
-      }
-      *reinterpret_cast<uint4*>(dst) = v[k];
+      *reinterpret_cast<uint4*>(static_cast<char*>(e.cache) + page * e.page_stride + row * e.row_stride + at[k]) = v[k];
     }
+  }
+  if (a.copied <= (uint32_t)lane) look();
+  if (!known) return;
+  for (uint32_t u = lane; u < a.turned; u += 32) {
+    if (u != (uint32_t)lane) piece.load(a, u, b, s);
+    piece.store(a, pos, page, row);
   }
 }
 
@@ -517,40 +536,31 @@ extern "C" int dsa_cache_append(const DsaCacheAppendParams* p, void* stream_) {
       p->page_size < 1 || p->page_size > kMax || p->max_blocks < 1 || p->max_blocks > kMax / p->page_size ||
       p->num_pages < 1 || p->num_pages > kMax || p->batch > kMax || p->s > kMax)
     return DSA_ERR_INVALID_ARG;
-  AppendArgs a = {};
-  uint32_t units = 0;
+  // copied rows and the rotated rows of each type, one launch for each type there is (one, as a rule)
   for (int i = 0; i < p->entries; ++i) {
     const DsaCacheRows& e = p->rows[i];
     if (!e.src || !e.cache || e.width_bytes < 16 || e.width_bytes > (1 << 24) || e.width_bytes % 16 ||
         !aligned16(e.src) || !aligned16(e.cache) || e.src_batch_stride % 16 || e.src_token_stride % 16 ||
         e.page_stride % 16 || e.row_stride % 16)
       return DSA_ERR_INVALID_ARG;
-    uint32_t pieces = (uint32_t)(e.width_bytes / 16);
-    if (e.rotary != DSA_ROTARY_NONE) {
-      const int64_t size = e.dtype == DSA_DTYPE_FP32 ? 4 : 2, n = 16 / size;
-      if ((e.dtype != DSA_DTYPE_BF16 && e.dtype != DSA_DTYPE_FP16 && e.dtype != DSA_DTYPE_FP32) ||
-          (e.rotary != DSA_ROTARY_INTERLEAVED && e.rotary != DSA_ROTARY_HALF) || !p->table ||
-          !aligned16(p->table) || p->dim < 8 || p->dim > 256 || p->dim % 8 || e.offset < 0 ||
-          e.offset % n || p->dim % (e.rotary == DSA_ROTARY_HALF ? 2 * n : n) ||
-          (e.offset + p->dim) * size > e.width_bytes || p->max_positions < 1 || p->max_positions > kMax)
-        return DSA_ERR_INVALID_ARG;
-      if (e.rotary == DSA_ROTARY_HALF) pieces -= (uint32_t)(p->dim / 2 / n);
-    }
-    a.e[i] = e;
-    a.first[i] = units;
-    units += pieces;
+    if (e.rotary == DSA_ROTARY_NONE) continue;
+    const int64_t size = e.dtype == DSA_DTYPE_FP32 ? 4 : 2, n = 16 / size;
+    if ((e.dtype != DSA_DTYPE_BF16 && e.dtype != DSA_DTYPE_FP16 && e.dtype != DSA_DTYPE_FP32) ||
+        (e.rotary != DSA_ROTARY_INTERLEAVED && e.rotary != DSA_ROTARY_HALF) || !p->table ||
+        !aligned16(p->table) || p->dim < 8 || p->dim > 256 || p->dim % 8 || e.offset < 0 ||
+        e.offset % n || p->dim % (e.rotary == DSA_ROTARY_HALF ? 2 * n : n) ||
+        (e.offset + p->dim) * size > e.width_bytes || p->max_positions < 1 || p->max_positions > kMax)
+      return DSA_ERR_INVALID_ARG;
   }
-  a.first[p->entries] = units;
   if (p->batch == 0 || p->s == 0) return DSA_OK;
+  AppendArgs a = {};
   a.block_table = p->block_table;
   a.starts = p->starts;
   a.counts = p->counts;
   a.table = p->table;
   a.error_flag = p->error_flag;
-  a.units = units;
   a.tokens = p->batch * p->s;
   a.page = dsa::rotary::FastDiv((uint32_t)p->page_size);
-  a.entries = p->entries;
   a.s = (int)p->s;
   a.max_blocks = (int)p->max_blocks;
   a.num_pages = (int)p->num_pages;
@@ -558,8 +568,34 @@ extern "C" int dsa_cache_append(const DsaCacheAppendParams* p, void* stream_) {
   a.dim = (int)p->dim;
   const int64_t blocks = (a.tokens + kAppendThreads / 32 - 1) / (kAppendThreads / 32);
   if (blocks > kMax) return DSA_ERR_INVALID_ARG;
-  append_kernel<<<(unsigned)blocks, kAppendThreads, 0, stream>>>(a);
-  return cudaGetLastError() == cudaSuccess ? DSA_OK : DSA_ERR_CUDA;
+  bool copies = true;   // not launched yet
+  for (int32_t type : {DSA_DTYPE_BF16, DSA_DTYPE_FP16, DSA_DTYPE_FP32}) {
+    a.entries = 0;
+    a.copied = a.turned = 0;
+    for (int i = 0; i < p->entries && copies; ++i)
+      if (p->rows[i].rotary == DSA_ROTARY_NONE) {
+        a.first[a.entries] = a.copied;
+        a.e[a.entries++] = p->rows[i];
+        a.copied += (uint32_t)(p->rows[i].width_bytes / 16);
+      }
+    a.plain = a.entries;
+    for (int i = 0; i < p->entries; ++i) {
+      const DsaCacheRows& e = p->rows[i];
+      if (e.rotary == DSA_ROTARY_NONE || e.dtype != type) continue;
+      a.first[a.entries] = a.turned;
+      a.e[a.entries++] = e;
+      const int64_t pairs = e.rotary == DSA_ROTARY_HALF ? p->dim / 2 * (type == DSA_DTYPE_FP32 ? 4 : 2) / 16 : 0;
+      a.turned += (uint32_t)(e.width_bytes / 16 - pairs);
+    }
+    // (copied rows go with the first rotated type; alone if there is none)
+    if (a.turned == 0 && (type != DSA_DTYPE_FP32 || a.copied == 0)) continue;
+    copies = false;
+    if (type == DSA_DTYPE_BF16) append_kernel<__nv_bfloat16><<<(unsigned)blocks, kAppendThreads, 0, stream>>>(a);
+    else if (type == DSA_DTYPE_FP16) append_kernel<__half><<<(unsigned)blocks, kAppendThreads, 0, stream>>>(a);
+    else append_kernel<float><<<(unsigned)blocks, kAppendThreads, 0, stream>>>(a);
+    if (cudaGetLastError() != cudaSuccess) return DSA_ERR_CUDA;
+  }
+  return DSA_OK;
 }
 
 extern "C" int64_t dsa_pages_workspace_size(int32_t op, int64_t n, int64_t slots, int64_t num_pages) {
