@@ -57,7 +57,7 @@ struct Cfg {
   static constexpr int kQBufs =
       kStages * kStageBytes + 2 * kQBytes + kPBytes + kSmallBytes <= kSmemLimit ? 2 : 1;
   static constexpr int kSmem = kStages * kStageBytes + kQBufs * kQBytes + kPBytes + kSmallBytes;
-  static constexpr uint32_t kCols = (2 + kBlocks) * NH;
+  static constexpr uint32_t kCols = (4 + kBlocks) * NH;   // S of two tiles in two parts each, O
   static constexpr uint32_t kTmem = kCols <= 32 ? 32 : kCols <= 64 ? 64 : kCols <= 128 ? 128
                                     : kCols <= 256 ? 256 : 512;
   static_assert(kStages >= 2, "two key tiles have to fit");
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_ptr;
-  const uint32_t t_o = tmem + 2 * NH;
+  const uint32_t t_o = tmem + 4 * NH;
   bool failed = false;
 
   if (warp >= kLoadWarp && warp < kQkWarp) {
@@ -291,16 +291,18 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint64_t ka = smem_desc_sw128(base + st * C::kStageBytes, 16, C::kGroupBytes);
             const uint64_t ra = smem_desc_sw128(base + st * C::kStageBytes + C::kKeyBytes, 16, 1024);
             const uint64_t qb = smem_desc_sw128(s_q + buf * C::kQBytes, 16, 1024);
-            const uint32_t d = tmem + (g & 1) * NH;
+            // in two sums over half of the k-steps each, added by the softmax warps: the core cuts
+            // off what a sum's fp32 does not hold, and half as many, half as large cuts leave half
+            // the error (softmax_max 1.8e-6 too low in one sum)
+            const uint32_t d = tmem + (g & 1) * 2 * NH;
+            constexpr int kSteps = 4 * C::kChunks + 4;
 #pragma unroll
-            for (int c = 0; c < C::kChunks; ++c)
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                umma_f16<1>(d, ka + ((c * 1024 + k * 32) >> 4), qb + ((c * NH * 128 + k * 32) >> 4),
-                            kIdQk, c + k > 0);
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              umma_f16<1>(d, ra + ((k * 32) >> 4), qb + ((C::kChunks * NH * 128 + k * 32) >> 4), kIdQk, 1);
+            for (int u = 0; u < kSteps; ++u) {
+              const int c = u / 4, k = u % 4;
+              umma_f16<1>(d + (u < kSteps / 2 ? 0 : NH),
+                          c < C::kChunks ? ka + ((c * 1024 + k * 32) >> 4) : ra + ((k * 32) >> 4),
+                          qb + ((c * NH * 128 + k * 32) >> 4), kIdQk, u % (kSteps / 2) > 0);
+            }
             umma_commit(s_full(g & 1));
             if (i == sg.count - 1) umma_commit(q_empty(buf));
           }
@@ -377,8 +379,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool whole_tile = valid >= kTile && mask == 3u;
         mbar_wait_hot(s_full(g & 1), (g >> 1) & 1, a.error_flag, &failed);
         tc_fence_after();
-        uint32_t raw[HW / 2];
-        tmem_ld_frag<HW>(tmem + (g & 1) * NH + head0 + lane_base, raw);
+        uint32_t raw[HW / 2], more[HW / 2];
+        tmem_ld_frag<HW>(tmem + (g & 1) * 2 * NH + head0 + lane_base, raw);
+        tmem_ld_frag<HW>(tmem + (g & 1) * 2 * NH + NH + head0 + lane_base, more);
         tmem_ld_wait();
         tc_fence_before();
         __syncwarp();
@@ -386,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
         float z[HW / 2];
 #pragma unroll
-        for (int j = 0; j < HW / 2; ++j) z[j] = __uint_as_float(raw[j]);
+        for (int j = 0; j < HW / 2; ++j) z[j] = __uint_as_float(raw[j]) + __uint_as_float(more[j]);
         if (flip)
 #pragma unroll
           for (int j = 0; j < HW / 2; ++j) z[j] = -z[j];
@@ -767,9 +770,9 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_combine_kernel(const 
 }
 
 // Heads of a work item: the smallest operand that holds them.  Past 64 the pair kernel takes them
-// all at D = 512 (32 rows of 8192 .. 65536 keys, 128 heads: 348 us against 478 for two items of 64);
+// all at D = 512 (32 rows of 8192 .. 65536 keys, 128 heads: 356 us against 502 for two items of 64);
 // below, where a result of 64 heads leaves room for several key tiles, two items are faster (the
-// same rows at D = 256: 252 us against 314 with a pair).
+// same rows at D = 256: 271 us against 314 with a pair).
 int heads_of(int64_t n1, int64_t d) { return n1 <= 16 ? 16 : n1 <= 32 ? 32 : n1 <= 64 || d < 512 ? 64 : 128; }
 
 int64_t align256(int64_t x) { return (x + 255) & ~(int64_t)255; }

@@ -12,10 +12,11 @@
 //
 // A tile of 128 keys and the queries leave room for one buffer each of K and V at D = 512.  V is
 // held in halves of 64 keys with barriers of their own, so that the next tile's first half is on
-// its way while the second is in work.  (K in three parts of 192 dims, refilled one by one, took
-// 369 us against 347 for 32 rows of 8192 .. 65536 keys and 128 heads: the loads then meet QK's
-// operand reads, and shared memory, at 400 KB a tile and CTA, is what bounds this kernel.
-// Bringing tiles into L2 ahead of their load gained nothing here.)
+// its way while the second is in work.  32 rows of 8192 .. 65536 keys and 128 heads take
+// 351 us in a burst and 385 under the power cap.  (Not kept, as slower at those rows: K in three
+// parts of 192 dims, refilled one by one, 369 us against 347, since the loads then meet QK's
+// operand reads, and shared memory, at 400 KB a tile and CTA, is what bounds this kernel; P in
+// halves, 366 against 351; tiles brought into L2 ahead of their load, 364 against 356.)
 #pragma once
 
 #include "attn_paged.cuh"
@@ -52,7 +53,7 @@ struct Cfg {
   static constexpr int kSmem = kOffSmall + kSmallBytes;
   static constexpr int kPvN = 256;                             // dims of one PV instruction
   static constexpr int kPvs = D / kPvN;
-  static constexpr uint32_t kColsO = 128;                      // after two buffers of S
+  static constexpr uint32_t kColsO = 256;                      // after S of two tiles in two parts each
   static constexpr uint32_t kTmem = 512;
   static_assert(D == 512 && kSmem <= kSmemLimit, "one buffer of each operand has to fit");
 };
@@ -201,6 +202,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int w = warp - kValueWarp;
     Tiles t{work, {}, 0, -1};
     int g = 0, page = -1;
+    int sent = 0, tails = 0, queries = 0;   // halves, halves on the CTA's own barriers, segments' queries
     for (; t.next(a); ++g) {
       const int32_t* table = table_of(t.s);
       const int tile = t.s.first + t.i;
@@ -220,6 +222,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           tma_load_5d_pair(base, &maps.q, bar, 0, kHeads * (int)rank, 0, s, b);
           tma_load_5d_pair(base + kHeads * D * 2, &maps.qr, bar, 0, kHeads * (int)rank, 0, s, b);
         }
+        ++queries;
         __syncwarp();
       }
 #pragma unroll
@@ -246,14 +249,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           else
             tma_load_4d_pair(dst, &map_v, mapa_shared(v_full(hf), 0), 0, in_page, C::kVChunks * (int)rank, now);
         }
+        ++sent;
+        tails += tail;
         __syncwarp();
       }
       if (failed) break;
     }
-    if (failed && rank == 0) {
+    if (failed) {   // half x is the x / 2-th use of its barrier
       bool gave_up = false;
-      for (int hf = 0; hf < 2 && g > 0; ++hf)
-        mbar_wait(v_full(hf), (g - 1) & 1, a.error_flag, &gave_up, true);
+      for (int x = max(0, tails - 2); x < tails; ++x)
+        mbar_wait(v_tail(x & 1), (x >> 1) & 1, a.error_flag, &gave_up);
+      for (int x = max(0, sent - 2); x < sent && rank == 0; ++x)
+        mbar_wait(v_full(x & 1), (x >> 1) & 1, a.error_flag, &gave_up, true);
+      if (queries > 0 && rank == 0) mbar_wait(q_full, (queries - 1) & 1, a.error_flag, &gave_up, true);
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
@@ -282,16 +290,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const uint32_t ks = base + C::kOffK;
             const uint64_t kb = smem_desc_sw128(ks, 16, C::kGroupBytes);
             const uint64_t rb = smem_desc_sw128(ks + C::kKeyBytes, 16, 1024);
-            const uint32_t d = tmem + 64 * (na & 1);
+            // in two sums over half of the k-steps each, as in the other kernel
+            const uint32_t d = tmem + 128 * (na & 1);
+            constexpr int kSteps = 4 * C::kChunks + 4;
 #pragma unroll
-            for (int c = 0; c < C::kChunks; ++c)
-#pragma unroll
-              for (int u = 0; u < 4; ++u)
-                umma_f16<2>(d, qa + ((c * kHeads * 128 + u * 32) >> 4), kb + ((c * 1024 + u * 32) >> 4),
-                            kIdQk, c + u > 0);
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-              umma_f16<2>(d, qa + ((C::kChunks * kHeads * 128 + u * 32) >> 4), rb + ((u * 32) >> 4), kIdQk, 1);
+            for (int i = 0; i < kSteps; ++i) {
+              const int c = i / 4, u = i % 4;
+              umma_f16<2>(d + (i < kSteps / 2 ? 0 : 64), qa + ((c * kHeads * 128 + u * 32) >> 4),
+                          c < C::kChunks ? kb + ((c * 1024 + u * 32) >> 4) : rb + ((u * 32) >> 4), kIdQk,
+                          i % (kSteps / 2) > 0);
+            }
             umma_commit_pair(s_full(na & 1), 3);
             umma_commit_pair(k_empty, 3);
             if (q.i == q.s.count - 1) umma_commit_pair(q_empty, 3);
@@ -373,13 +381,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const bool tail = mask != 0xffffu || valid < kTile;
         mbar_wait_hot(s_full(g & 1), (g >> 1) & 1, a.error_flag, &failed);
         tc_fence_after();
-        uint32_t r[32];
-        tmem_ld32(tmem + 64 * (g & 1) + 32 * wg + lane_addr, r);
+        uint32_t r[32], more[32];
+        const uint32_t s_at = tmem + 128 * (g & 1) + 32 * wg + lane_addr;
+        tmem_ld32(s_at, r);
+        tmem_ld32(s_at + 64, more);
         tmem_ld_wait_regs(r);
-        tc_fence_before();
+        tmem_ld_wait_regs(more);
         float z[32];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) z[j] = __uint_as_float(r[j]);
+        for (int j = 0; j < 32; ++j) z[j] = __uint_as_float(r[j]) + __uint_as_float(more[j]);
+        tc_fence_before();
         if (flip)
 #pragma unroll
           for (int j = 0; j < 32; ++j) z[j] = -z[j];

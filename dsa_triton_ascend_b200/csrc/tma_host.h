@@ -20,19 +20,6 @@ inline int sm_count() {
   return n;
 }
 
-// Let `kernel` use `bytes` of dynamic shared memory on the current device; asked for once per
-// device (`ready`, a bit for each).
-inline bool allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>* ready) {
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return false;
-  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
-  if (ready->load(std::memory_order_acquire) & bit) return true;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
-    return false;
-  ready->fetch_or(bit, std::memory_order_release);
-  return true;
-}
-
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
