@@ -19,6 +19,7 @@
 
 #include "attn_paged.cuh"
 #include "attn_paged_pair.cuh"
+#include "attn_paged_wide.cuh"
 #include "dsa_b200.h"
 #include "sm100.cuh"
 #include "tma_host.h"
@@ -773,7 +774,7 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_combine_kernel(const 
 // all at D = 512 (32 rows of 8192 .. 65536 keys, 128 heads: 356 us against 502 for two items of 64);
 // below, where a result of 64 heads leaves room for several key tiles, two items are faster (the
 // same rows at D = 256: 271 us against 314 with a pair).
-int heads_of(int64_t n1, int64_t d) { return n1 <= 16 ? 16 : n1 <= 32 ? 32 : n1 <= 64 || d < 512 ? 64 : 128; }
+int heads_of(int64_t n1) { return n1 <= 16 ? 16 : n1 <= 32 ? 32 : n1 <= 64 ? 64 : 128; }
 
 int64_t align256(int64_t x) { return (x + 255) & ~(int64_t)255; }
 
@@ -910,21 +911,37 @@ int launch_pair(const DsaAttnPagedParams* p, int diag, int heads, cudaStream_t s
 }
 
 template <int D, typename T>
+int launch_wide(const DsaAttnPagedParams* p, int diag, int heads, cudaStream_t stream) {
+  using C = wide::Cfg<D>;
+  const int grid = sm_count();
+  if (grid < 1) return DSA_ERR_CUDA;
+  Maps maps;
+  if (!make_maps<D>(&maps, p, ElemTraits<T>::kIsBf16, wide::kHeads)) return DSA_ERR_TMA_DESCRIPTOR;
+  const Args a = make_args(p, wide::kHeads, grid, diag, heads);
+  auto kern = wide::attn_paged_wide_kernel<D, T>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) !=
+      cudaSuccess)
+    return DSA_ERR_CUDA;
+  if (!launch_early(kern, grid, wide::kThreads, C::kSmem, stream, maps, a)) return DSA_ERR_CUDA;
+  return launch_join<D, wide::kHeads, wide::kSegmentCost, T>(p, a, grid, stream);
+}
+
+template <int D, typename T>
 int launch_heads(const DsaAttnPagedParams* p, int diag, int heads, cudaStream_t stream) {
-  switch (heads_of(p->n1, D)) {
+  switch (heads_of(p->n1)) {
     case 16: return launch<D, 16, T>(p, diag, heads, stream);
     case 32: return launch<D, 32, T>(p, diag, heads, stream);
     case 64: return launch<D, 64, T>(p, diag, heads, stream);
     default:
       if constexpr (D == 512) return launch_pair<T>(p, diag, heads, stream);
-      return DSA_ERR_INVALID_ARG;
+      else return launch_wide<D, T>(p, diag, heads, stream);
   }
 }
 
 // Whether several new tokens of a batch can be taken as one row of s1 * n1 heads, so that their
 // keys are read once: up to 8 tokens, all of them valid, whose heads fit one work item.
-bool packs(int64_t s1, int64_t n1, int64_t d) {
-  return s1 > 1 && s1 <= kMaxDiag + 1 && s1 * n1 <= (d == 512 ? 128 : 64);
+bool packs(int64_t s1, int64_t n1) {
+  return s1 > 1 && s1 <= kMaxDiag + 1 && s1 * n1 <= 128;
 }
 
 template <typename T>
@@ -932,7 +949,7 @@ int launch_dim(const DsaAttnPagedParams* p, cudaStream_t stream) {
   DsaAttnPagedParams q = *p;
   int diag = 0;
   // (the heads of a token and the next token's have to be one step apart)
-  if (packs(p->s1, p->n1, p->d) && !p->act_q &&
+  if (packs(p->s1, p->n1) && !p->act_q &&
       (p->n1 == 1 || (p->q_token_stride == p->n1 * p->q_head_stride &&
                       p->qr_token_stride == p->n1 * p->qr_head_stride))) {
     if (p->n1 == 1) q.q_head_stride = p->q_token_stride, q.qr_head_stride = p->qr_token_stride;
@@ -958,10 +975,10 @@ extern "C" int64_t dsa_attn_paged_workspace_size(int64_t batch, int64_t s1, int6
   const int64_t sms = dsa::sm_count();
   if (sms < 1) return -1;
   auto size = [&](int64_t rows, int64_t heads, int64_t own) {
-    const int64_t nh = heads_of(heads, d), shares = nh == 128 ? sms / 2 : sms;
+    const int64_t nh = heads_of(heads), shares = nh == 128 && d == 512 ? sms / 2 : sms;
     return align256((2 * shares + own) * nh * (d * 4 + 16) + (rows + 1) * 4);
   };
-  const int64_t plain = size(batch * s1, n1, 0), packed = packs(s1, n1, d) ? size(batch, s1 * n1, batch) : 0;
+  const int64_t plain = size(batch * s1, n1, 0), packed = packs(s1, n1) ? size(batch, s1 * n1, batch) : 0;
   return plain > packed ? plain : packed;
 }
 
