@@ -770,10 +770,10 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_combine_kernel(const 
   if (t == 0 && a.softmax_max) put_stats(a, at, top, ref, run, sum);
 }
 
-// Heads of a work item: the smallest operand that holds them.  Past 64 the pair kernel takes them
-// all at D = 512 (32 rows of 8192 .. 65536 keys, 128 heads: 356 us against 502 for two items of 64);
-// below, where a result of 64 heads leaves room for several key tiles, two items are faster (the
-// same rows at D = 256: 271 us against 314 with a pair).
+// Heads of a work item: the smallest operand that holds them.  Past 64 they are taken whole: at
+// D = 512 by the pair kernel (32 rows of 8192 .. 65536 keys, 128 heads: 356 us against 502 for two
+// items of 64), below by the wide one (the same rows at D = 256: 185 us against 266; a pair there
+// took 314).
 int heads_of(int64_t n1) { return n1 <= 16 ? 16 : n1 <= 32 ? 32 : n1 <= 64 ? 64 : 128; }
 
 int64_t align256(int64_t x) { return (x + 255) & ~(int64_t)255; }

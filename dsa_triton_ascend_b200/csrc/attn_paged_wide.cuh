@@ -4,12 +4,19 @@
 //   O [128 heads x D]      += P V       (M = 128, N = D)
 // One copy of a key tile is the K-major operand K and, as the same bytes, the MN-major operand V.
 // An instruction takes 32 B x (rows of A + rows of B) / 128 B cycles, so at D = 256 a tile costs
-// 20 x 48 + 4 x 96 = 1,344 of them, where two items of 64 heads with the keys on the M side
-// cost 2 x (20 x 32 + 8 x 48) = 2,048, load every key twice, and pass through twice the softmax
-// barriers.  The result and two tiles of scores (in two sums each) fill the tensor memory.
+// 20 x 48 + 4 x 128 = 1,472 of them, where two items of 64 heads with the keys on the M side
+// cost 2 x (20 x 32 + 8 x 48) = 2,048 and load every key twice.  The result and scores of two
+// tiles (three at D = 128; in two sums each) fill the tensor memory; the probabilities take the place of their
+// scores, as the operand A from tensor memory, which leaves shared memory for a fourth tile.
 //
 // A lane of tensor memory is a head, so the two warps that share 32 heads (one for each half of
 // a tile's keys, and of the dims) need only each other: their barrier has 64 threads.
+//
+// 32 rows of 8192 .. 65536 keys, 128 heads: 185 us at D = 256 and 147 at D = 128, against 266 and
+// 243 as two items of 64 heads.  A tile takes 2,200 and 1,850 cycles there: with two (three)
+// buffers the way from S over the softmax (1,250) to the end of PV is what is waited for.
+// (Probabilities through shared memory, and so three tiles at D = 256, took 191 and 156 us; the
+// softmax warps' own look at the page table for the loads' barrier, 163 at D = 128.)
 #pragma once
 
 #include "attn_paged.cuh"
@@ -20,7 +27,8 @@ namespace attn_paged {
 namespace wide {
 
 constexpr int kTile = 64;
-constexpr int kSegmentCost = 2;    // of starting a row, in tiles
+constexpr int kSegmentCost = 4;    // of starting a row, in tiles (8 rows of 4000 .. 32768 keys: 45 us
+                                   // against 47 with 2)
 constexpr int kHeads = 128;
 constexpr int kLoadWarp = 8;       // warps 0-7: softmax; 8-11: loads
 constexpr int kQkWarp = 12;
@@ -29,24 +37,28 @@ constexpr int kQueryWarp = 14;
 constexpr int kThreads = 480;
 constexpr int kMaxStages = 8;
 
+constexpr int imin(int a, int b) { return a < b ? a : b; }
+
 template <int D>
 struct Cfg {
   static constexpr int kChunks = D / 64;
   static constexpr int kGroupBytes = kChunks * 1024;   // 8 keys: [chunk][8][128 B]
   static constexpr int kKeyBytes = 8 * kGroupBytes;
-  static constexpr int kStageBytes = kKeyBytes + kTile * 128;
+  static constexpr int kRopeBytes = kTile * 128;
   static constexpr int kQBytes = kHeads * (D + kRope) * 2;
-  static constexpr int kPBytes = kHeads * kTile * 2;
-  static constexpr int kSmallBytes = 2 * 2 * kHeads * 4 + 512;
-  static constexpr int kRoom = (kSmemLimit - kQBytes - kPBytes - kSmallBytes) / kStageBytes;
-  static constexpr int kStages = kRoom < kMaxStages ? kRoom : kMaxStages;
-  static constexpr int kOffQ = kStages * kStageBytes;
-  static constexpr int kOffP = kOffQ + kQBytes;
-  static constexpr int kOffSmall = kOffP + kPBytes;
+  static constexpr int kSmallBytes = 2 * 2 * kHeads * 4 + 576;
+  // latent and rotary parts in rings of their own, as the rotary ones are free after S
+  static constexpr int kRoom = kSmemLimit - kQBytes - kSmallBytes;
+  static constexpr int kStages = imin((kRoom - 2 * kRopeBytes) / kKeyBytes, kMaxStages);
+  static constexpr int kRopes = imin((kRoom - kStages * kKeyBytes) / kRopeBytes, kStages);
+  static constexpr int kOffRope = kStages * kKeyBytes;
+  static constexpr int kOffQ = kOffRope + kRopes * kRopeBytes;
+  static constexpr int kOffSmall = kOffQ + kQBytes;
   static constexpr int kSmem = kOffSmall + kSmallBytes;
-  static constexpr uint32_t kColsO = 4 * kTile;   // after S of two tiles in two sums each
+  static constexpr int kBufs = (512 - D) / (2 * kTile);   // of S (in two sums) and P: 2 or 3
+  static constexpr uint32_t kColsO = kBufs * 2 * kTile;
   static constexpr uint32_t kTmem = 512;
-  static_assert(D <= 256 && kStages >= 3, "a result of 128 heads has to leave room for the scores");
+  static_assert(D <= 256 && kStages >= 4 && kRopes >= 2 && kSmem <= kSmemLimit, "a result of 128 heads has to leave room for the scores");
 };
 
 template <int D, typename T>
@@ -58,11 +70,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr float kShift = kBf16 ? 0.0f : 6.0f;   // half's probabilities are held 2^6 higher
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base = smem_u32(smem);
-  const uint32_t s_q = base + C::kOffQ, s_p = base + C::kOffP;
+  const uint32_t s_q = base + C::kOffQ;
   float* wmax = reinterpret_cast<float*>(smem + C::kOffSmall);   // [2][kHeads]
   float* wsum = wmax + 2 * kHeads;                               // [2][kHeads]
   uint64_t* bars = reinterpret_cast<uint64_t*>(wsum + 2 * kHeads);
-  int32_t* tmask = reinterpret_cast<int32_t*>(bars + 32);        // [kMaxStages][4]
+  int32_t* tmask = reinterpret_cast<int32_t*>(bars + 46);        // [kMaxStages][4]
   int32_t* tmp = tmask + 4 * kMaxStages;                         // [16]
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(tmp + 16);
   int32_t* start = reinterpret_cast<int32_t*>(tmem_ptr + 1);     // [3]
@@ -70,12 +82,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t b0 = smem_u32(bars);
   auto full = [&](int s) { return b0 + 8u * s; };
   auto empty = [&](int s) { return b0 + 8u * (kMaxStages + s); };
-  auto s_full = [&](int s) { return b0 + 8u * (2 * kMaxStages + s); };
-  auto s_empty = [&](int s) { return b0 + 8u * (2 * kMaxStages + 2 + s); };
-  auto drained = [&](int s) { return b0 + 8u * (2 * kMaxStages + 4 + s); };
-  const uint32_t p_full = b0 + 8u * (2 * kMaxStages + 6), p_empty = b0 + 8u * (2 * kMaxStages + 7);
-  const uint32_t q_full = b0 + 8u * (2 * kMaxStages + 8), q_empty = b0 + 8u * (2 * kMaxStages + 9);
-  const uint32_t o_empty = b0 + 8u * (2 * kMaxStages + 10);
+  auto r_full = [&](int s) { return b0 + 8u * (2 * kMaxStages + s); };
+  auto r_empty = [&](int s) { return b0 + 8u * (3 * kMaxStages + s); };
+  auto s_full = [&](int s) { return b0 + 8u * (4 * kMaxStages + s); };
+  auto p_full = [&](int s) { return b0 + 8u * (4 * kMaxStages + 3 + s); };
+  auto p_empty = [&](int s) { return b0 + 8u * (4 * kMaxStages + 6 + s); };
+  auto drained = [&](int s) { return b0 + 8u * (4 * kMaxStages + 9 + s); };
+  const uint32_t q_full = b0 + 8u * (4 * kMaxStages + 11), q_empty = b0 + 8u * (4 * kMaxStages + 12);
+  const uint32_t o_empty = b0 + 8u * (4 * kMaxStages + 13);
+  constexpr int kBufs = C::kBufs;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (base & 1023u) {
@@ -87,13 +102,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(full(s), 4);
       mbar_init(empty(s), 1);
     }
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(s_full(s), 1);
-      mbar_init(s_empty(s), 8);
-      mbar_init(drained(s), 1);
+    for (int s = 0; s < C::kRopes; ++s) {
+      mbar_init(r_full(s), 4);
+      mbar_init(r_empty(s), 1);
     }
-    mbar_init(p_full, 8);
-    mbar_init(p_empty, 1);
+    for (int s = 0; s < kBufs; ++s) {
+      mbar_init(s_full(s), 1);
+      mbar_init(p_full(s), 8);
+      mbar_init(p_empty(s), 1);
+    }
+    mbar_init(drained(0), 1);
+    mbar_init(drained(1), 1);
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
     mbar_init(o_empty, 8);
@@ -123,7 +142,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     // every tile, lanes 0 and 1 their latent rows, lanes 2 and 3 the rotary ones.
     const int w = warp - kLoadWarp;
     const int grp = 2 * w + (lane & 1);
-    const bool is_rope = lane & 2, loads = !is_rope || (a.box_mask >> grp & 1u);
+    const bool is_rope = lane & 2;
+    int sent = 0;   // tiles of latent rows
     while (!failed && next_segment<kTile, kSegmentCost>(a, work, sg)) {
       const int32_t* table = a.block_table + (int64_t)(sg.row / a.s1) * a.max_blocks;
       auto page_of = [&](int tile) {   // -1: no such page
@@ -135,30 +155,42 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       int page = page_of(sg.first);
       for (int i = 0; i < sg.count; ++i, ++g) {
-        const int st = g % C::kStages, tile = sg.first + i;
-        const int now = page;
+        const int st = g % C::kStages, rs = g % C::kRopes, tile = sg.first + i;
+        const int now = page, in_page = (tile * kTile + grp * 8) % a.page_size;
         if (i + 1 < sg.count) page = page_of(tile + 1);
+        const uint32_t mask = __ballot_sync(0xffffffffu, now >= 0) & 3u;
         if (g >= C::kStages) mbar_wait_hot(empty(st), (g / C::kStages - 1) & 1, a.error_flag, &failed);
         failed = __any_sync(0xffffffffu, failed);
         if (failed) break;
-        const uint32_t mask = __ballot_sync(0xffffffffu, now >= 0) & 3u;
-        const uint32_t dst = base + st * C::kStageBytes;
         if (lane == 0) {
           tmask[4 * st + w] = (int)mask;
-          const uint32_t bytes = __popc(mask) * C::kGroupBytes + __popc(mask & a.box_mask) * (a.box_rows * 128);
+          const uint32_t bytes = __popc(mask) * C::kGroupBytes;
           if (bytes) mbar_arrive_expect_tx(full(st), bytes);
           else mbar_arrive(full(st));
         }
         __syncwarp();
-        if (now >= 0 && loads)
-          tma_load_4d(dst + (is_rope ? C::kKeyBytes + grp * 1024 : grp * C::kGroupBytes),
-                      is_rope ? &maps.kr : &maps.k, full(st), 0, (tile * kTile + grp * 8) % a.page_size, 0, now);
+        if (now >= 0 && !is_rope)
+          tma_load_4d(base + st * C::kKeyBytes + grp * C::kGroupBytes, &maps.k, full(st), 0, in_page, 0, now);
+        ++sent;
+        if (g >= C::kRopes) mbar_wait_hot(r_empty(rs), (g / C::kRopes - 1) & 1, a.error_flag, &failed);
+        failed = __any_sync(0xffffffffu, failed);
+        if (failed) break;
+        if (lane == 0) {
+          const uint32_t bytes = __popc(mask & a.box_mask) * (a.box_rows * 128);
+          if (bytes) mbar_arrive_expect_tx(r_full(rs), bytes);
+          else mbar_arrive(r_full(rs));
+        }
+        __syncwarp();
+        if (now >= 0 && is_rope && (a.box_mask >> grp & 1u))
+          tma_load_4d(base + C::kOffRope + rs * C::kRopeBytes + grp * 1024, &maps.kr, r_full(rs), 0, in_page, 0, now);
       }
     }
     if (failed) {   // the copies in flight land before the CTA ends
       bool gave_up = false;
-      for (int t = max(0, g - C::kStages); t < g; ++t)
+      for (int t = max(0, sent - C::kStages); t < sent; ++t)
         mbar_wait(full(t % C::kStages), (t / C::kStages) & 1, a.error_flag, &gave_up);
+      for (int t = max(0, g - C::kRopes); t < g; ++t)
+        mbar_wait(r_full(t % C::kRopes), (t / C::kRopes) & 1, a.error_flag, &gave_up);
       __syncwarp();
     }
   } else if (warp == kQueryWarp) {
@@ -189,17 +221,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       while (!failed && next_segment<kTile, kSegmentCost>(a, work, sg)) {
         mbar_wait_hot(q_full, nseg & 1, a.error_flag, &failed);
         for (int i = 0; i < sg.count; ++i, ++g) {
-          const int st = g % C::kStages;
-          if (g >= 2) mbar_wait_hot(s_empty(g & 1), ((g >> 1) - 1) & 1, a.error_flag, &failed);
+          const int st = g % C::kStages, rs = g % C::kRopes;
           mbar_wait_hot(full(st), (g / C::kStages) & 1, a.error_flag, &failed);
+          mbar_wait_hot(r_full(rs), (g / C::kRopes) & 1, a.error_flag, &failed);
+          // last what comes last: the probabilities stand in the scores' place until their product
+          // is done (and a look at a barrier takes 200 cycles here)
+          if (g >= kBufs) mbar_wait_hot(p_empty(g % kBufs), (g / kBufs - 1) & 1, a.error_flag, &failed);
           failed = __any_sync(0xffffffffu, failed);
           if (failed) break;
           tc_fence_after();
           if (elect_one()) {
-            const uint64_t kb = smem_desc_sw128(base + st * C::kStageBytes, 16, C::kGroupBytes);
-            const uint64_t rb = smem_desc_sw128(base + st * C::kStageBytes + C::kKeyBytes, 16, 1024);
+            const uint64_t kb = smem_desc_sw128(base + st * C::kKeyBytes, 16, C::kGroupBytes);
+            const uint64_t rb = smem_desc_sw128(base + C::kOffRope + rs * C::kRopeBytes, 16, 1024);
             // in two sums over half of the k-steps each, as in the kernel for fewer heads
-            const uint32_t d = tmem + (g & 1) * 2 * kTile;
+            const uint32_t d = tmem + (g % kBufs) * 2 * kTile;
             constexpr int kSteps = 4 * C::kChunks + 4;
 #pragma unroll
             for (int u = 0; u < kSteps; ++u) {
@@ -208,7 +243,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                           c < C::kChunks ? kb + ((c * 1024 + k * 32) >> 4) : rb + ((k * 32) >> 4), kIdQk,
                           u % (kSteps / 2) > 0);
             }
-            umma_commit(s_full(g & 1));
+            umma_commit(s_full(g % kBufs));
+            umma_commit(r_empty(rs));
             if (i == sg.count - 1) umma_commit(q_empty);
           }
           __syncwarp();
@@ -217,23 +253,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     } else {
       constexpr uint32_t kIdPv = idesc_f16(kHeads, D, kBf16, false, true);
-      const uint64_t pa = smem_desc_sw128(s_p, 16, 1024);
       while (!failed && next_segment<kTile, kSegmentCost>(a, work, sg)) {
         for (int i = 0; i < sg.count; ++i, ++g) {
           const int st = g % C::kStages;
           if (i == 0 && nseg > 0) mbar_wait_hot(o_empty, (nseg - 1) & 1, a.error_flag, &failed);
-          mbar_wait_hot(p_full, g & 1, a.error_flag, &failed);
+          mbar_wait_hot(p_full(g % kBufs), (g / kBufs) & 1, a.error_flag, &failed);
           failed = __any_sync(0xffffffffu, failed);
           if (failed) break;
           tc_fence_after();
           if (elect_one()) {
-            const uint64_t vb = smem_desc_sw128(base + st * C::kStageBytes, 1024, C::kGroupBytes);
+            const uint64_t vb = smem_desc_sw128(base + st * C::kKeyBytes, 1024, C::kGroupBytes);
 #pragma unroll
-            for (int k = 0; k < kTile / 16; ++k)
-              umma_f16<1>(tmem + C::kColsO, pa + ((k * 32) >> 4), vb + ((k * 2 * C::kGroupBytes) >> 4), kIdPv,
-                          (i > 0) | (k > 0));
+            for (int k = 0; k < kTile / 16; ++k)   // 16 keys of P are 8 columns
+              umma_f16_ts(tmem + C::kColsO, tmem + (g % kBufs) * 2 * kTile + 8 * k, vb + ((k * 2 * C::kGroupBytes) >> 4),
+                          kIdPv, (i > 0) | (k > 0));
             umma_commit(empty(st));
-            umma_commit(p_empty);
+            umma_commit(p_empty(g % kBufs));
           }
           __syncwarp();
         }
@@ -257,7 +292,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lane_addr = (uint32_t)(32 * q) << 16;
     const bool flip = a.scale < 0.0f;   // a negative scale turns the raw scores over
     const float c2 = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-38f);
-    uint8_t* prow = smem + C::kOffP + h * 128;
     constexpr int kDims = D / 2;   // of O, of one thread
     const uint32_t o_at = tmem + C::kColsO + wg * kDims + lane_addr;
     auto meet = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + q) : "memory"); };
@@ -270,17 +304,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t mask = m4.x | m4.y << 2 | m4.z << 4 | m4.w << 6;   // a bit per 8 keys
         const int valid = sg.keys - (sg.first + i) * kTile;               // keys of this tile, >= 1
         const bool tail = mask != 0xffu || valid < kTile;
-        mbar_wait_hot(s_full(g & 1), (g >> 1) & 1, a.error_flag, &failed);
+        mbar_wait_hot(s_full(g % kBufs), (g / kBufs) & 1, a.error_flag, &failed);
         tc_fence_after();
         uint32_t r[32], more[32];
-        const uint32_t s_at = tmem + (g & 1) * 2 * kTile + 32 * wg + lane_addr;
+        const uint32_t s_at = tmem + (g % kBufs) * 2 * kTile + 32 * wg + lane_addr;
         tmem_ld32(s_at, r);
         tmem_ld32(s_at + kTile, more);
         tmem_ld_wait_regs(r);
         tmem_ld_wait_regs(more);
         tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(s_empty(g & 1));
         float z[32];
 #pragma unroll
         for (int j = 0; j < 32; ++j) z[j] = __uint_as_float(r[j]) + __uint_as_float(more[j]);
@@ -306,7 +338,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ref = now;
           lim = (now + kRescale) / c2;
           if (i > 0) {
-            mbar_wait_hot(p_empty, (g - 1) & 1, a.error_flag, &failed);
+            mbar_wait_hot(p_empty((g - 1) % kBufs), (g - 1) / kBufs & 1, a.error_flag, &failed);
             tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < kDims; c += 16) {
@@ -321,7 +353,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           meet();   // the maxima are read
         }
-        const bool p_free = g == 0 || mbar_test_wait(p_empty, (g - 1) & 1);
         // probabilities; a head without any key so far has reference -inf and stays zero
         const float off = ref == -INFINITY ? 0.0f : kShift - ref;
         uint32_t pk[16];
@@ -332,27 +363,26 @@ __global__ void __launch_bounds__(kThreads, 1)
           sum += p0 + p1;
           pk[j] = E::pack2(p0, p1);
         }
-        if (!p_free) mbar_wait_hot(p_empty, (g - 1) & 1, a.error_flag, &failed);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          *reinterpret_cast<uint4*>(prow + (((4 * wg + j) ^ (h & 7)) << 4)) =
-              make_uint4(pk[4 * j], pk[4 * j + 1], pk[4 * j + 2], pk[4 * j + 3]);
+        // in the place of the scores, which both warps have read before they met
+        tc_fence_after();
+        tmem_st16(tmem + (g % kBufs) * 2 * kTile + 16 * wg + lane_addr, pk);
         if (tail) {
           // rows of this tile that no key stands in hold what was there before (or a page's
           // stale tail): cleared, so that 0 x NaN cannot enter the product; 8 keys a warp
           const int key = 8 * warp + (lane >> 2);
           if (key >= valid || !(mask >> warp & 1u)) {
-            uint8_t* row = smem + st * C::kStageBytes + warp * C::kGroupBytes + (lane >> 2) * 128;
+            uint8_t* row = smem + st * C::kKeyBytes + warp * C::kGroupBytes + (lane >> 2) * 128;
             for (int c = lane & 3; c < C::kChunks; c += 4)
 #pragma unroll
               for (int x = 0; x < 8; ++x)
                 *reinterpret_cast<uint4*>(row + c * 1024 + x * 16) = make_uint4(0, 0, 0, 0);
           }
+          fence_proxy_async_smem();
         }
-        fence_proxy_async_smem();
+        tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_full);
+        if (lane == 0) mbar_arrive(p_full(g % kBufs));
       }
 
       // ---- the segment's result ----
@@ -371,7 +401,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         else if (a.softmax_max)
           put_stats(a, (int64_t)sg.row * a.n1 + h, m, ref - kShift, most, l);
       }
-      mbar_wait_hot(p_empty, (g - 1) & 1, a.error_flag, &failed);
+      mbar_wait_hot(p_empty((g - 1) % kBufs), (g - 1) / kBufs & 1, a.error_flag, &failed);
       tc_fence_after();
 #pragma unroll 1
       for (int c = 0; c < kDims; c += 32) {
