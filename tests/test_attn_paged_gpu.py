@@ -341,3 +341,21 @@ def test_nan_where_it_is_seen(heads, d, lens):
     got = c.run(check=False)
     assert got[0][1].isnan().all() and got[1][1].isnan().all() and got[2][1].isnan().all()
     assert torch.equal(got[0][0][:, rest], ref[0][0][:, rest]) and got[0][0].isfinite().all()
+
+
+@pytest.mark.parametrize("d", [128, 256])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_many_heads_of_a_narrow_latent(d, dtype):
+    """More than 64 heads at D <= 256: lengths around tile and page ends, rows that are split, pages
+    that are missing inside a row, keys that raise the running maximum, several new tokens."""
+    c = Case([0, 1, 63, 64, 65, 130, 700, 20001], 100, d, 24, dtype=dtype, seed=31)
+    c.run()
+    c.table[6, 3] = c.table[7, 40] = -1   # the keys of those pages are not seen
+    for b, n in enumerate(c.lens):
+        for t0 in range(0, n, 96):
+            page = int(c.table[b, t0 // 24])
+            if page >= 0:
+                c.krc[page] = (c.krc[page].float().clamp(-2, 2) * min(1.5 ** (t0 // 96 % 9), 20.0)).to(dtype)
+    c.check(c.run(check=False), skip={(6, 3), (7, 40)})
+    for s1, heads in ((2, 64), (8, 16), (3, 128)):
+        Case([0, 1, s1, 64, 5000, 200], heads, d, 16, s1=s1, dtype=dtype, seed=s1).run(3)
