@@ -13,6 +13,8 @@
 // bytes as the MN-major operand V^T.  The pool is read once, by TMA boxes of 8 keys (which
 // never straddle a page, as page_size is a multiple of 8).
 //
+// More than 64 heads: attn_paged_pair.cuh (D = 512) and attn_paged_wide.cuh.
+//
 // attn_paged_combine_kernel joins the parts of rows that were split and writes zeros for rows
 // that see no key.
 #include <cuda_runtime.h>
@@ -778,7 +780,7 @@ int heads_of(int64_t n1) { return n1 <= 16 ? 16 : n1 <= 32 ? 32 : n1 <= 64 ? 64 
 
 int64_t align256(int64_t x) { return (x + 255) & ~(int64_t)255; }
 
-// What both kernels take; `nh` heads a work item, `shares` of the work.
+// What the kernels take; `nh` heads a work item, `shares` of the work.
 Args make_args(const DsaAttnPagedParams* p, int nh, int shares, int diag, int heads) {
   Args a;
   a.act_q = p->act_q;
@@ -939,7 +941,8 @@ int launch_heads(const DsaAttnPagedParams* p, int diag, int heads, cudaStream_t 
 }
 
 // Whether several new tokens of a batch can be taken as one row of s1 * n1 heads, so that their
-// keys are read once: up to 8 tokens, all of them valid, whose heads fit one work item.
+// keys are read once: up to 8 tokens, all of them valid, whose heads fit one work item (4 x 8 tokens,
+// 16 heads, D = 256, up to 65536 keys: 53 us against 115 token by token).
 bool packs(int64_t s1, int64_t n1) {
   return s1 > 1 && s1 <= kMaxDiag + 1 && s1 * n1 <= 128;
 }
