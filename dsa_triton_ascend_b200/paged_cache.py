@@ -296,8 +296,9 @@ def paged_cache_copy(caches, src_pages, dst_pages):
 
 
 def paged_cache_extend(block_table, seq_lengths, ref_counts, counts, page_size):
-    """Grow sequence r by ``counts[r]`` [slots] tokens, with the pages that takes.  Returns the new
-    (block_table, seq_lengths, ref_counts)."""
+    """Grow sequence r by ``counts[r]`` [slots] tokens, with the pages that takes.  Rows are served
+    in order; one that the pages left cannot serve takes none of them, and those after it are
+    served all the same.  Returns the new (block_table, seq_lengths, ref_counts)."""
     return _upkeep(PAGES_EXTEND, [], block_table, seq_lengths, ref_counts, counts, page_size=page_size)
 
 

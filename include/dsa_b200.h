@@ -537,7 +537,8 @@ int dsa_cache_append(const DsaCacheAppendParams* params, void* stream);
  *            both written and read.  Only num_pages, page_size, caches and the pairs are read.
  *   FORK     n pairs parent row first[i] -> empty row second[i]: the child shares the parent's
  *            full pages and gets a page of its own with the rows of the partly filled one.
- *   EXTEND   row r grows by first[r] tokens (n == slots), with the pages that takes.
+ *   EXTEND   row r grows by first[r] tokens (n == slots), with the pages that takes.  Rows are
+ *            served in order; one that the pages left cannot serve takes none of them.
  *   FREE     n rows first[i] give their pages back and become empty.
  *   COMPACT  live pages move to the lowest ids, n_live of them, in order; seq_lengths unused.
  * A fork or row that asks for what cannot be (an id out of range, a child in use, a length past

@@ -12,3 +12,13 @@ for p in (ROOT, os.path.join(ROOT, "tests", "golden"), os.path.join(ROOT, "tests
 def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a CUDA B200 (run with -m gpu)")
     config.addinivalue_line("markers", "slow: larger CPU cases")
+
+
+# Kept as written, though the value it holds is not the contract's: it expects its last row, which
+# asks for one page, to be refused while a page is free (its own ref_counts [1, 1, 0] show it).  It
+# runs after the others, so that a run that stops at the first failure has seen them all.
+HOLDS_ANOTHER_VALUE = ("test_paged_cache_gpu.py::test_extend_when_the_pool_runs_out",)
+
+
+def pytest_collection_modifyitems(config, items):
+    items.sort(key=lambda item: item.nodeid.endswith(HOLDS_ANOTHER_VALUE))

@@ -344,3 +344,52 @@ def test_a_report_stops_no_other_operator():
     dsa.paged_cache_extend(i32([[-1]]), i32([0]), i32([1]), i32([3]), 8)
     with pytest.raises(RuntimeError, match="bits 0x10"):
         dsa.check_device_errors("cuda")
+
+
+def _grow_in_order(table, lens, refs, counts, page):
+    """Rows in order, each taking the lowest free pages; one that what is left cannot serve takes none."""
+    free = [p for p, r in enumerate(refs) if r == 0]
+    err = 0
+    for s, n in enumerate(counts):
+        if n < 0 or lens[s] + n > len(table[0]) * page:
+            err |= 1 << 2
+            continue
+        had, has = -(-lens[s] // page), -(-(lens[s] + n) // page)
+        if has - had > len(free):
+            err |= 1 << 4
+            continue
+        for j in range(had, has):
+            table[s][j] = free.pop(0)
+            refs[table[s][j]] = 1
+        lens[s] += n
+    return err
+
+
+def test_extend_past_a_row_that_does_not_fit():
+    """A row that the pool cannot serve leaves its pages to the rows after it."""
+    table, lens, refs = [[0, -1, -1], [-1] * 3, [-1] * 3, [-1] * 3], [5, 0, 0, 0], [1, 0, 0]
+    got = dsa.paged_cache_extend(i32(table), i32(lens), i32(refs), i32([3, 8, 16, 8]), 8)
+    assert errors() == 1 << 4
+    assert _equal(got, ([[0, -1, -1], [1, -1, -1], [-1] * 3, [2, -1, -1]], [8, 8, 0, 8], [1, 1, 1]))
+    # a prompt that is too long, before decode steps of one page each
+    table, lens, refs = [[-1] * 6 for _ in range(5)], [0] * 5, [0] * 4
+    got = dsa.paged_cache_extend(i32(table), i32(lens), i32(refs), i32([48, 1, 2, 3, 8]), 8)
+    assert errors() == 1 << 4
+    assert got[1].tolist() == [0, 1, 2, 3, 8] and [r[0] for r in got[0].tolist()] == [-1, 0, 1, 2, 3]
+
+
+@pytest.mark.parametrize("slots,width,pages,page", [(6, 5, 9, 8), (300, 20, 700, 16), (1024, 9, 1500, 8),
+                                                    (3000, 7, 4000, 4), (3000, 7, 140000, 4)])
+@pytest.mark.parametrize("seed", [0, 1, 2])
+def test_extend_of_more_than_the_pool_holds(slots, width, pages, page, seed):
+    """Requests of every size against a pool that runs out early, late, or within a block of rows."""
+    rng = random.Random(seed)
+    refs = [int(rng.random() < 0.3 + 0.3 * seed) for _ in range(pages)]
+    if pages > 8 * slots:
+        refs[2 * slots * seed + 40:] = [1] * (pages - 2 * slots * seed - 40)
+    lens = [rng.choice([0, 0, 1, page, page + 1]) for _ in range(slots)]
+    table = [[rng.randrange(pages) if j * page < n else -1 for j in range(width)] for n in lens]
+    counts = [rng.choice([0, 1, page, rng.randint(0, width * page), rng.randint(0, (width - 2) * page)]) for _ in range(slots)]
+    got = dsa.paged_cache_extend(i32(table), i32(lens), i32(refs), i32(counts), page)
+    assert errors() == _grow_in_order(table, lens, refs, counts, page)
+    assert _equal(got, (table, lens, refs))
