@@ -220,6 +220,8 @@ def lib() -> ctypes.CDLL:
                 l.dsa_attn_paged.restype = ctypes.c_int
                 l.dsa_attn_paged_workspace_size.argtypes = [_i64] * 4
                 l.dsa_attn_paged_workspace_size.restype = _i64
+                l.dsa_attn_paged_shares_keys.argtypes = [_i64] * 2
+                l.dsa_attn_paged_shares_keys.restype = ctypes.c_int
                 l.dsa_rotary.argtypes = [ctypes.POINTER(RotaryParams), _p]
                 l.dsa_rotary.restype = ctypes.c_int
                 l.dsa_rotary_table.argtypes = [_p, _i64, _i64, ctypes.POINTER(ctypes.c_double),

@@ -972,6 +972,10 @@ bool aligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p)
 }  // namespace attn_paged
 }  // namespace dsa
 
+extern "C" int dsa_attn_paged_shares_keys(int64_t s1, int64_t n1) {
+  return s1 >= 1 && n1 >= 1 && n1 <= 128 && dsa::attn_paged::packs(s1, n1);
+}
+
 extern "C" int64_t dsa_attn_paged_workspace_size(int64_t batch, int64_t s1, int64_t n1, int64_t d) {
   using namespace dsa::attn_paged;
   if (batch < 0 || s1 < 0 || n1 < 1 || n1 > 128 || d < 1) return -1;

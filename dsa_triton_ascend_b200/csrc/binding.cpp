@@ -31,7 +31,8 @@ PyObject* g_check;                        // raises for a code that is not DSA_O
 std::unordered_map<int, int*> g_report;   // report flag of each device
 
 struct Plan {
-  std::string params, extra;   // the struct; upkeep: the array of caches
+  std::string params, extra;   // the struct; upkeep: the array of caches, attention: which of
+                               // query and query_rope are copied first
   int64_t ws_bytes;
 };
 std::unordered_map<std::string, Plan> g_plans[kOps];
@@ -215,7 +216,11 @@ PyObject* attn(PyObject*, PyObject* const* argv, Py_ssize_t n) {
     int* report;
     if (n != 10 || !a.read(argv)) Py_RETURN_NONE;
     const Plan* plan = find(kAttn, a.key, *a.q, &report);
-    if (!plan || (at_of(a.q) | at_of(a.qr) | at_of(a.k) | at_of(a.kr)) % 16) Py_RETURN_NONE;
+    if (!plan) Py_RETURN_NONE;
+    const bool copy_q = plan->extra[0], copy_qr = plan->extra[1];
+    if (((copy_q ? 0 : at_of(a.q)) | (copy_qr ? 0 : at_of(a.qr)) | at_of(a.k) | at_of(a.kr)) % 16) Py_RETURN_NONE;
+    const at::Tensor q = copy_q ? a.q->clone(at::MemoryFormat::Contiguous) : *a.q;
+    const at::Tensor qr = copy_qr ? a.qr->clone(at::MemoryFormat::Contiguous) : *a.qr;
     DsaAttnPagedParams p;
     std::memcpy(&p, plan->params.data(), sizeof p);
     const auto f32 = a.q->options().dtype(at::kFloat);
@@ -224,8 +229,8 @@ PyObject* attn(PyObject*, PyObject* const* argv, Py_ssize_t n) {
     at::Tensor top = a.stats ? at::empty(shape, f32) : at::zeros(shape, f32);
     at::Tensor sum = a.stats ? at::empty(shape, f32) : at::zeros(shape, f32);
     at::Tensor ws = at::empty({plan->ws_bytes}, a.q->options().dtype(at::kByte));
-    p.query = a.q->data_ptr();
-    p.query_rope = a.qr->data_ptr();
+    p.query = q.data_ptr();
+    p.query_rope = qr.data_ptr();
     p.key_cache = a.k->data_ptr();
     p.key_rope_cache = a.kr->data_ptr();
     p.block_table = ptr<const int32_t>(a.table);
@@ -354,12 +359,12 @@ PyObject* keep(PyObject*, PyObject* const* argv, Py_ssize_t n) {
     if (n != kArgs[op] + 4 || (size_t)PyBytes_GET_SIZE(params) != kSize[op]) Py_RETURN_FALSE;
     Key key;
     bool ok = false;
-    size_t caches = 0;
-    if (op == kAttn) { AttnArgs a; ok = a.read(argv + 1); key = a.key; }
+    size_t more = 0;   // extra bytes
+    if (op == kAttn) { AttnArgs a; ok = a.read(argv + 1); key = a.key; more = 2; }
     if (op == kRotary) { RotaryArgs a; ok = a.read(argv + 1); key = a.key; }
     if (op == kAppend) { AppendArgs a; ok = a.read(argv + 1); key = a.key; }
-    if (op == kUpkeep) { UpkeepArgs a; ok = a.read(argv + 1); key = a.key; caches = a.caches.size(); }
-    if (!ok || (size_t)PyBytes_GET_SIZE(extra) != caches * sizeof(DsaPageCache)) Py_RETURN_FALSE;
+    if (op == kUpkeep) { UpkeepArgs a; ok = a.read(argv + 1); key = a.key; more = a.caches.size() * sizeof(DsaPageCache); }
+    if (!ok || (size_t)PyBytes_GET_SIZE(extra) != more) Py_RETURN_FALSE;
     Plan plan;
     plan.params.assign(PyBytes_AS_STRING(params), PyBytes_GET_SIZE(params));
     plan.extra.assign(PyBytes_AS_STRING(extra), PyBytes_GET_SIZE(extra));

@@ -35,9 +35,9 @@ def _cache_strides(t: torch.Tensor, what: str):
     return (t.stride(0) if t.shape[0] > 1 else row * t.shape[1]), row
 
 
-def _plan(query, query_rope, key_cache, key_rope_cache, block_table, scale_value, sparse_mode):
+def _plan(query, query_rope, key_cache, key_rope_cache, block_table, scale_value, sparse_mode, counted):
     """Check the arguments and fill in what their shapes decide: (parameters, strides fit,
-    statistics' shape, workspace bytes)."""
+    statistics' shape, workspace bytes).  `counted`: with a count of queries per sequence."""
     if sparse_mode not in (0, 3):
         raise ValueError("Only sparse_mode 0 (full) / 3 (rightDownCausal) supported")
     if query.dim() != 4 or query_rope.dim() != 4:
@@ -70,9 +70,11 @@ def _plan(query, query_rope, key_cache, key_rope_cache, block_table, scale_value
     p.k_page_stride, p.k_row_stride = _cache_strides(key_cache, "key_cache")
     p.kr_page_stride, p.kr_row_stride = _cache_strides(key_rope_cache, "key_rope_cache")
     qs, qrs = _tma_strides(query), _tma_strides(query_rope)
-    # up to 8 tokens whose heads fit one work item share their keys, if their heads lie one step
-    # apart; queries that lie otherwise are copied rather than read token by token
-    if 1 < S1 <= 8 and 1 < N1 and S1 * N1 <= (128 if D == 512 else 64):
+    # a few tokens share their keys if their heads lie one step apart; queries that lie otherwise
+    # are copied rather than each token's keys read anew (with counts per sequence none share):
+    # 32 x 2 tokens of 64 heads, D 256, 8192 .. 65536 keys: 194 us against 290 token by token
+    # (178 without a copy); 8 x 2 of them over 500 .. 4000 keys: 39 against 28
+    if N1 > 1 and not counted and lib().dsa_attn_paged_shares_keys(S1, N1):
         qs, qrs = [None if st is None or st[1] != N1 * st[2] else st for st in (qs, qrs)]
     contiguous = lambda w: (S1 * N1 * w, N1 * w, w)
     p.q_batch_stride, p.q_token_stride, p.q_head_stride = qs or contiguous(D)
@@ -128,7 +130,8 @@ def flash_attention_paged(
             return flash_attention_paged(query, query_rope, key_cache, key_rope_cache, block_table,
                                          actual_seq_lengths_key, scale_value, actual_seq_lengths_query,
                                          sparse_mode, return_softmax_lse)
-    plan = _plan(query, query_rope, key_cache, key_rope_cache, block_table, float(scale_value), sparse_mode)
+    plan = _plan(query, query_rope, key_cache, key_rope_cache, block_table, float(scale_value), sparse_mode,
+                 actual_seq_lengths_query is not None)
     template, q_fits, qr_fits, stat_shape, ws_bytes = plan
     dev = query.device
     B, _, S1, _ = stat_shape
@@ -164,7 +167,6 @@ def flash_attention_paged(
         p.softmax_max, p.softmax_sum = smax.data_ptr(), ssum.data_ptr()
     p.error_flag = report_ptr(index)
     check(lib().dsa_attn_paged(p, H.raw_stream(index)), "dsa_attn_paged")
-    if q is query and qr is query_rope and bt is block_table \
-            and act_k is actual_seq_lengths_key and act_q is actual_seq_lengths_query:
-        remember(BIND_ATTN, index, *args, template, b"", ws_bytes)
+    if bt is block_table and act_k is actual_seq_lengths_key and act_q is actual_seq_lengths_query:
+        remember(BIND_ATTN, index, *args, template, bytes((not q_fits, not qr_fits)), ws_bytes)
     return out, smax, ssum

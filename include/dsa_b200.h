@@ -448,6 +448,10 @@ typedef struct DsaAttnPagedParams {
 
 int dsa_attn_paged(const DsaAttnPagedParams* params, void* stream);
 int64_t dsa_attn_paged_workspace_size(int64_t batch, int64_t s1, int64_t n1, int64_t d);
+/* 1 where the s1 tokens of a batch share their keys' loads, given that act_q is NULL and that heads
+ * lie one step apart across tokens (q_token_stride == n1 * q_head_stride, and so for query_rope;
+ * any strides where n1 is 1); 0 where each token reads its keys for itself. */
+int dsa_attn_paged_shares_keys(int64_t s1, int64_t n1);
 
 /*
  * Rotary positions.  No counterpart in the reference, which takes rotated tensors.

@@ -359,3 +359,17 @@ def test_many_heads_of_a_narrow_latent(d, dtype):
     c.check(c.run(check=False), skip={(6, 3), (7, 40)})
     for s1, heads in ((2, 64), (8, 16), (3, 128)):
         Case([0, 1, s1, 64, 5000, 200], heads, d, 16, s1=s1, dtype=dtype, seed=s1).run(3)
+
+
+@pytest.mark.parametrize("d,s1,heads", [(256, 2, 64), (128, 2, 64), (256, 5, 20), (128, 8, 16), (512, 4, 32)])
+def test_heads_first_queries_share_their_keys(d, s1, heads):
+    """Queries laid out heads-first, or as a slice of more heads, take the path that contiguous ones
+    take: the same bits, where reading the keys token by token would split and round differently."""
+    c = Case([3333, 900, s1, 1], heads, d, 64, s1=s1, seed=s1 + d)
+    ref = c.run(3)
+    q, qr = c.q, c.qr
+    for view in (lambda t: t.transpose(1, 2).contiguous().transpose(1, 2),
+                 lambda t: torch.cat([t, t, t], 2)[:, :, heads:2 * heads]):
+        c.q, c.qr = view(q), view(qr)
+        assert not c.q.is_contiguous()
+        assert all(torch.equal(x, y) for x, y in zip(ref, c.run(3)))

@@ -143,3 +143,39 @@ def test_append_and_upkeep(paths):
     dsa.paged_cache_extend(table, lens, refs, i32(1, 90, 0), 8)     # the compiled path reports as well
     with pytest.raises(RuntimeError, match="bits 0x4"):
         dsa.check_device_errors()
+
+
+def test_counted_queries_are_read_where_they_are(paths):
+    """With counts per sequence no keys are shared, so heads-first queries are not copied, and the
+    call is one that the compiled path takes."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(2)
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda").bfloat16()
+    kc, krc = rnd(9, 16, 1, 512), rnd(9, 16, 1, 64)
+    table, lens = i32(0, 1, 2, 3, 4, 5, 6, 7).view(2, 4), i32(50, 64)
+    q, qr = [rnd(2, 8, 3, w).transpose(1, 2) for w in (512, 64)]
+    call = lambda a, b: dsa.flash_attention_paged(a, b, kc, krc, table, lens, 0.05, actual_seq_lengths_query=i32(1, 3),
+                                                  sparse_mode=3, return_softmax_lse=True)
+    plain, fast = paths(lambda: call(q, qr))
+    same(plain, fast)
+    same(fast, call(q.contiguous(), qr.contiguous()))
+    dsa.check_device_errors()
+
+
+def test_copied_queries(paths):
+    """Queries that are copied first (heads-first ones that share their keys, odd strides), one or both."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(3)
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda").bfloat16()
+    kc, krc = rnd(9, 16, 1, 256), rnd(9, 16, 1, 64)
+    table, lens = i32(0, 1, 2, 3, 4, 5, 6, 7).view(2, 4), i32(50, 64)
+    q, qr = rnd(2, 3, 8, 256), rnd(2, 3, 8, 64)
+    call = lambda a, b: dsa.flash_attention_paged(a, b, kc, krc, table, lens, 0.05, sparse_mode=3, return_softmax_lse=True)
+    ref = call(q, qr)
+    heads_first = lambda t: t.transpose(1, 2).contiguous().transpose(1, 2)
+    odd = lambda t: torch.cat([t, t[..., :3]], -1)[..., :t.shape[-1]]
+    for a, b in ((heads_first(q), heads_first(qr)), (odd(q), qr), (q, odd(qr)), (heads_first(q), odd(qr))):
+        plain, fast = paths(lambda: call(a, b))
+        same(plain, fast)
+        same(ref, fast)
+    dsa.check_device_errors()
