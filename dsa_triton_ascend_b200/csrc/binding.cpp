@@ -38,17 +38,33 @@ struct Plan {
 std::unordered_map<std::string, Plan> g_plans[kOps];
 constexpr size_t kMostPlans = 1024;
 
-// A signature, appended to piece by piece.
+// A signature, appended to piece by piece.  What an argument may be (None, a number, a tensor, a
+// text, a list) is written before it, so that no two kinds give the same bytes.
 struct Key {
   std::string s;
-  void num(int64_t v) { s.append(reinterpret_cast<const char*>(&v), sizeof v); }
-  void real(double v) { s.append(reinterpret_cast<const char*>(&v), sizeof v); }
-  void none() { num(-1); }
+  void raw(const void* p, size_t n) { s.append(static_cast<const char*>(p), n); }
+  void num(int64_t v) { raw(&v, sizeof v); }
+  void real(double v) { raw(&v, sizeof v); }
+  void none() { s.push_back('n'); }
+  void number(int64_t v) {
+    s.push_back('i');
+    num(v);
+  }
+  void text(const char* p, int64_t n) {
+    s.push_back('s');
+    num(n);
+    raw(p, n);
+  }
+  void list(int64_t n) {
+    s.push_back('l');
+    num(n);
+  }
   void tensor(const at::Tensor& t) {
     const auto sizes = t.sizes(), strides = t.strides();
+    s.push_back('t');
     num(((int64_t)t.scalar_type() << 40) | ((int64_t)(t.get_device() + 1) << 8) | (int64_t)sizes.size());
-    s.append(reinterpret_cast<const char*>(sizes.data()), sizes.size() * 8);
-    s.append(reinterpret_cast<const char*>(strides.data()), strides.size() * 8);
+    raw(sizes.data(), sizes.size() * 8);
+    raw(strides.data(), strides.size() * 8);
   }
 };
 
@@ -71,7 +87,7 @@ bool tensors_of(PyObject* list, Key& key, std::vector<const at::Tensor*>& out) {
   if (!PyList_Check(list) && !PyTuple_Check(list)) return false;
   PyObject** items = PySequence_Fast_ITEMS(list);
   const Py_ssize_t n = PySequence_Fast_GET_SIZE(list);
-  key.num(n);
+  key.list(n);
   out.resize(n);
   for (Py_ssize_t i = 0; i < n; ++i)
     if (!maybe_tensor(items[i], key, &out[i]) || !out[i]) return false;
@@ -85,7 +101,7 @@ bool number(PyObject* o, Key& key) {
   }
   if (!PyLong_Check(o)) return false;
   int over = 0;
-  key.num(PyLong_AsLongLongAndOverflow(o, &over));
+  key.number(PyLong_AsLongLongAndOverflow(o, &over));
   return !over;
 }
 
@@ -122,9 +138,8 @@ struct RotaryArgs {
       PyErr_Clear();
       return false;
     }
-    key.num(n);
-    key.s.append(layout, n);
-    key.num((a[5] == Py_True ? 1 : 0) + (a[6] == a[0] ? 2 : 0));
+    key.text(layout, n);
+    key.number((a[5] == Py_True ? 1 : 0) + (a[6] == a[0] ? 2 : 0));
     return (a[5] == Py_True || a[5] == Py_False) && (a[6] == Py_None || a[6] == a[0]);
   }
 };
@@ -144,6 +159,7 @@ struct AppendArgs {
     }
     if (!PyList_Check(a[6]) && !PyTuple_Check(a[6])) return false;
     PyObject** items = PySequence_Fast_ITEMS(a[6]);
+    key.list(PySequence_Fast_GET_SIZE(a[6]));
     for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(a[6]); ++i) {
       if (items[i] == Py_None) {
         key.none();
@@ -157,8 +173,7 @@ struct AppendArgs {
         PyErr_Clear();
         return false;
       }
-      key.num(n);
-      key.s.append(s, n);
+      key.text(s, n);
       if (!number(PyTuple_GET_ITEM(items[i], 1), key)) return false;
     }
     return true;

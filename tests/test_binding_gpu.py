@@ -179,3 +179,34 @@ def test_copied_queries(paths):
         same(plain, fast)
         same(ref, fast)
     dsa.check_device_errors()
+
+
+def test_refused_calls_stay_refused():
+    """A call that the checks refuse is refused after a valid call of nearly the same signature too."""
+    caches = [torch.randn(6, 8, 1, w, device="cuda").bfloat16() for w in (64, 128)]
+    keep = [c.clone() for c in caches]
+    tokens = [torch.randn(2, 1, 1, w, device="cuda").bfloat16() for w in (64, 128)]
+    table, lens, refs = i32(0, 1, -1, -1).view(2, 2), i32(9, 0), i32(1, 1, 0, 0, 0, 0)
+    append = lambda rotary, n=2: dsa.paged_cache_append(tokens[:n], caches[:n], table, i32(3, 0), counts=i32(0, 0), rotary=rotary)
+    for n, good, bad in ((2, None, ([None], [], [None] * 3, ())), (2, [None, None], ([None], [None] * 3)),
+                         (1, None, ([], [None] * 2)), (1, [None], ([], [None] * 2))):
+        for _ in range(3):
+            append(good, n)
+        for r in bad:
+            with pytest.raises(ValueError, match="one entry"):
+                append(r, n)
+    assert all(torch.equal(a, b) for a, b in zip(caches, keep))
+    fork = lambda size: dsa.paged_cache_fork(caches, table, lens, refs, i32(0), i32(1), page_size=size)
+    for good in (None, 8):
+        for _ in range(3):
+            fork(good)
+        for size in (-1, 0, 7):
+            with pytest.raises(ValueError, match="page_size"):
+                fork(size)
+    x, rot, pos = torch.randn(1, 2, 4, 64, device="cuda"), dsa.rotary_table(8, 64), i32(0, 1).view(1, 2)
+    for _ in range(3):
+        dsa.rotary_embedding(x, rot, pos)
+    for offset in (-1, 1):
+        with pytest.raises(ValueError, match="exceed"):
+            dsa.rotary_embedding(x, rot, pos, offset=offset)
+    dsa.check_device_errors()
