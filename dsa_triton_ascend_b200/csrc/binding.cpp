@@ -12,6 +12,7 @@
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstring>
@@ -215,14 +216,13 @@ bool call(Op op, const void* params, const at::Tensor& lead, const char* what) {
   return false;
 }
 
+// f(), its C++ exceptions turned into the Python ones that torch's own functions raise (its
+// OutOfMemoryError, which callers look for, among them).
 template <typename F>
 PyObject* guarded(F f) {
-  try {
-    return f();
-  } catch (const std::exception& e) {
-    if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, e.what());
-    return nullptr;
-  }
+  HANDLE_TH_ERRORS
+  return f();
+  END_HANDLE_TH_ERRORS
 }
 
 PyObject* attn(PyObject*, PyObject* const* argv, Py_ssize_t n) {

@@ -210,3 +210,21 @@ def test_refused_calls_stay_refused():
         with pytest.raises(ValueError, match="exceed"):
             dsa.rotary_embedding(x, rot, pos, offset=offset)
     dsa.check_device_errors()
+
+
+def test_out_of_memory_is_what_torch_raises():
+    """The compiled path raises torch's own exceptions, as the Python path does: a caller that makes
+    room and tries again asks for this one.  (The allocator's limit is what runs out here, not the
+    card.)"""
+    x = torch.randn(1, 4096, 64, 64, device="cuda").bfloat16()
+    table = dsa.rotary_table(4096, 64)
+    pos = torch.arange(4096, device="cuda", dtype=torch.int32)[None]
+    ref = [dsa.rotary_embedding(x, table, pos) for _ in range(2)]     # of a known signature from here on
+    torch.cuda.empty_cache()
+    torch.cuda.set_per_process_memory_fraction(1e-6)
+    try:
+        with pytest.raises(torch.OutOfMemoryError):
+            dsa.rotary_embedding(x, table, pos)
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    assert torch.equal(dsa.rotary_embedding(x, table, pos), ref[0])
