@@ -751,7 +751,9 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_combine_kernel(const 
     }
     if (!key) continue;
     const float raw = a.scale < 0.0f ? -dot : dot, z = dot * a.scale * 1.4426950408889634f;
-    const float now = fmaxf(ref, z), f = ref == now ? 1.0f : exp2f(ref - now), w = exp2f(z - now);
+    // (a score of -inf with none above it weighs nothing, as in the kernels)
+    const float now = fmaxf(ref, z), f = ref == now ? 1.0f : exp2f(ref - now);
+    const float w = z == -INFINITY ? 0.0f : exp2f(z - now);
     ref = now;
     run = fmaxf(run, z);
     top = fmaxf(top, raw);

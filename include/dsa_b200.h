@@ -411,8 +411,8 @@ int64_t dsa_dense_indexer_workspace_size(int64_t batch, int64_t s1, int64_t s2, 
  *   page_size), in sparse_mode 3 also t < act_k - act_q + s + 1; rows s >= act_q see none.
  * Rows of a page past the row's keys are not used, whatever they hold.
  * Outputs: out [batch][s1][n1][d]; softmax_max / softmax_sum [batch][s1][n1] fp32 (both NULL
- * to skip) as in dsa_sfa_fwd; rows without keys get zeros.  The result does not depend on
- * timing: the parts of a split row are joined in one order.
+ * to skip) as in dsa_sfa_fwd; rows without keys, or whose scores are all -inf, get zeros.  The
+ * result does not depend on timing: the parts of a split row are joined in one order.
  * out and workspace (dsa_attn_paged_workspace_size() bytes for the current device) are 32-byte
  * aligned.
  */

@@ -373,3 +373,29 @@ def test_heads_first_queries_share_their_keys(d, s1, heads):
         c.q, c.qr = view(q), view(qr)
         assert not c.q.is_contiguous()
         assert all(torch.equal(x, y) for x, y in zip(ref, c.run(3)))
+
+
+@pytest.mark.parametrize("heads", [4, 16, 64])
+def test_a_score_of_minus_infinity_alone(heads):
+    """A row whose only score is -inf has no weight to give and is left at zeros, whether its token
+    is taken by itself or with others (whose last keys the join takes in)."""
+    c = Case([1, 2], heads, 128, 16, s1=2, seed=41)
+    c.qr[..., 0] = c.qr[..., 0].abs() + 1
+    for b in range(2):
+        c.krc[int(c.table[b, 0]), :2, 0, 0] = float("-inf")
+    both = c.run(3, check=False)
+    assert not any(t.any() for t in both)               # (NaN counts as any)
+    q, qr = c.q, c.qr
+    for s in range(2):
+        c.q, c.qr, c.lens = q[:, s:s + 1].contiguous(), qr[:, s:s + 1].contiguous(), [s, 1 + s]
+        assert all(torch.equal(a.flatten(), b.flatten()) for a, b in
+                   zip(c.run(check=False), (both[0][:, s:s + 1], both[1][:, :, s:s + 1], both[2][:, :, s:s + 1])))
+    # beside a finite score it weighs nothing
+    c = Case([200, 2], heads, 128, 16, s1=2, seed=42)
+    c.qr[..., 0] = c.qr[..., 0].abs() + 1
+    for b, n in enumerate(c.lens):
+        c.krc[int(c.table[b, (n - 1) // 16]), (n - 1) % 16, 0, 0] = float("-inf")
+    got = c.run(3, check=False)
+    q, qr = c.q, c.qr
+    c.q, c.qr, c.lens = q[:, 1:].contiguous(), qr[:, 1:].contiguous(), [199, 1]
+    c.check([got[0][:, 1:], got[1][:, :, 1:], got[2][:, :, 1:]])
