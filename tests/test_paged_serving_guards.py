@@ -225,3 +225,17 @@ def test_rotary_frequencies_in_python():
     assert dsa.rotary_frequencies(64, scaling="linear", factor=4.0)[5] == pytest.approx(f[5] / 4)
     ntk = dsa.rotary_frequencies(64, scaling="ntk", factor=4.0)
     assert ntk[0] == 1.0 and ntk[31] == pytest.approx(f[31] / 4)   # the slowest pair by the whole factor
+
+
+def test_error_flag_is_kept(monkeypatch):
+    """Every call of every operator asks for its flag: one tensor per device, made once, not a new view
+    a call; the report flag stands beside it in the pair that check_device_errors reads."""
+    pair = torch.zeros(2, dtype=torch.int32)
+    monkeypatch.setattr(_lib, "_err_bufs", {3: pair})
+    monkeypatch.setattr(_lib, "_error_views", {}, raising=False)
+    dev = torch.device("cuda", 3)
+    flag = _lib.error_flag(dev)
+    assert _lib.error_flag(dev) is flag and _lib.error_flag("cuda:3") is flag
+    flag.fill_(7)
+    _lib.report_flag(dev).fill_(9)
+    assert pair.tolist() == [7, 9] and flag.shape == (1,)
