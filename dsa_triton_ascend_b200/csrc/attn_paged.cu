@@ -980,7 +980,10 @@ extern "C" int dsa_attn_paged_shares_keys(int64_t s1, int64_t n1) {
 
 extern "C" int64_t dsa_attn_paged_workspace_size(int64_t batch, int64_t s1, int64_t n1, int64_t d) {
   using namespace dsa::attn_paged;
-  if (batch < 0 || s1 < 0 || n1 < 1 || n1 > 128 || d < 1) return -1;
+  constexpr int64_t kMax = 0x7fffffff;   // of rows * n1, as in dsa_attn_paged
+  if (batch < 0 || s1 < 0 || n1 < 1 || n1 > 128 || d < 1 || d > 512 || batch > kMax || s1 > kMax ||
+      batch * s1 > kMax / n1)
+    return -1;
   const int64_t sms = dsa::sm_count();
   if (sms < 1) return -1;
   auto size = [&](int64_t rows, int64_t heads, int64_t own) {

@@ -574,7 +574,7 @@ extern "C" int dsa_cache_append(const DsaCacheAppendParams* p, void* stream_) {
     if ((e.dtype != DSA_DTYPE_BF16 && e.dtype != DSA_DTYPE_FP16 && e.dtype != DSA_DTYPE_FP32) ||
         (e.rotary != DSA_ROTARY_INTERLEAVED && e.rotary != DSA_ROTARY_HALF) || !p->table ||
         !aligned16(p->table) || p->dim < 8 || p->dim > 256 || p->dim % 8 || e.offset < 0 ||
-        e.offset % n || p->dim % (e.rotary == DSA_ROTARY_HALF ? 2 * n : n) ||
+        e.offset > e.width_bytes || e.offset % n || p->dim % (e.rotary == DSA_ROTARY_HALF ? 2 * n : n) ||
         (e.offset + p->dim) * size > e.width_bytes || p->max_positions < 1 || p->max_positions > kMax)
       return DSA_ERR_INVALID_ARG;
   }
@@ -626,7 +626,8 @@ extern "C" int dsa_cache_append(const DsaCacheAppendParams* p, void* stream_) {
 
 extern "C" int64_t dsa_pages_workspace_size(int32_t op, int64_t n, int64_t slots, int64_t num_pages) {
   using namespace dsa::pages;
-  if (n < 0 || slots < 0 || num_pages < 0) return -1;
+  constexpr int64_t kMax = 0x7fffffff;
+  if (n < 0 || slots < 0 || num_pages < 0 || n > kMax || slots > kMax || num_pages > kMax) return -1;
   if (op == DSA_PAGES_COPY) return 0;
   return 4 * (align64(8 + (op == DSA_PAGES_FORK ? n : 0)) + align64(slots) + 3 * align64(num_pages) +
               align64(num_pages / 32 + 1));

@@ -252,7 +252,7 @@ extern "C" int dsa_rotary(const DsaRotaryParams* p, void* stream_) {
   constexpr int64_t kMax = 0x7fffffff;
   if (!p->x || !p->out || !p->positions || !p->table || p->dim < 2 || p->dim % 2 ||
       p->dim > 2 * kMaxPairs || p->offset < 0 || p->head_dim > (1 << 20) ||
-      p->offset + p->dim > p->head_dim || p->max_positions < 1 || p->max_positions > kMax ||
+      p->head_dim < p->dim || p->offset > p->head_dim - p->dim || p->max_positions < 1 || p->max_positions > kMax ||
       p->heads > (1 << 20) || p->s > kMax || p->batch > kMax)
     return DSA_ERR_INVALID_ARG;
   if (p->dtype == DSA_DTYPE_BF16) return launch<__nv_bfloat16>(p, stream);

@@ -239,3 +239,31 @@ def test_error_flag_is_kept(monkeypatch):
     flag.fill_(7)
     _lib.report_flag(dev).fill_(9)
     assert pair.tolist() == [7, 9] and flag.shape == (1,)
+
+
+def test_c_entries_refuse_sizes_that_would_wrap(lib):
+    """Offsets and sizes near the end of 64 bits are refused, not added up past it."""
+    fake, huge = 1 << 20, (1 << 63) - 8
+    p = _lib.RotaryParams()
+    p.x = p.out = p.positions = p.table = fake
+    p.batch, p.s, p.heads, p.head_dim, p.dim, p.max_positions = 1, 2, 4, 64, 64, 8
+    for offset in (huge, huge - 64, 1 << 40):
+        p.offset = offset
+        assert _call(lib, "dsa_rotary", p) == 1
+    p = _lib.CacheAppendParams()
+    p.block_table = p.starts = p.table = fake
+    p.batch, p.s, p.num_pages, p.page_size, p.max_blocks, p.entries, p.dim, p.max_positions = 1, 2, 4, 8, 2, 1, 64, 8
+    e = p.rows[0]
+    e.src = e.cache = fake
+    e.width_bytes, e.row_stride, e.page_stride, e.rotary = 128, 128, 1024, 1
+    for offset in (huge, huge - 64, (1 << 62) - 64, 1 << 62, 1 << 40):
+        e.offset = offset
+        assert _call(lib, "dsa_cache_append", p) == 1
+    size = lib.dsa_attn_paged_workspace_size
+    size.restype, size.argtypes = ctypes.c_int64, [ctypes.c_int64] * 4
+    for args in ((1 << 40, 1 << 40, 16, 512), (1 << 31, 1, 16, 512), (1, 1 << 31, 16, 512), (1 << 30, 1 << 10, 16, 512), (1, 1, 16, 1 << 60)):
+        assert size(*args) == -1
+    size = lib.dsa_pages_workspace_size
+    size.restype, size.argtypes = ctypes.c_int64, [ctypes.c_int32] + [ctypes.c_int64] * 3
+    for args in ((1, huge, 4, 4), (1, 4, huge, 4), (1, 4, 4, huge), (1, 1 << 31, 4, 4)):
+        assert size(*args) == -1
