@@ -243,13 +243,16 @@ _binding = None
 
 def binding():
     """The compiled path of the serving operators' repeated calls (csrc/binding.cpp), or None
-    where it is not built; the operators' own Python path calls the same entries."""
+    where it is not built, or was built for another torch; the operators' own Python path calls the
+    same entries."""
     global _binding
     if _binding is None:
         _binding = False
         try:
             from . import _binding as module
         except ImportError:
+            return None
+        if getattr(module, "TORCH_VERSION", None) != torch.__version__:
             return None
         entries = [ctypes.cast(getattr(lib(), name), ctypes.c_void_p).value
                    for name in ("dsa_attn_paged", "dsa_rotary", "dsa_cache_append", "dsa_pages")]

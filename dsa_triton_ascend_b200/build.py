@@ -39,19 +39,27 @@ def _stale() -> bool:
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def _built_for(version: str) -> bool:
+    """Whether the binding carries the stamp of this torch (csrc/binding.cpp)."""
+    with open(BINDING, "rb") as f:
+        return b"dsa binding for torch " + version.encode() + b"\0" in f.read()
+
+
 def build_binding(force: bool = False) -> str:
-    """The CPython module that calls the serving operators' C entries (see csrc/binding.cpp)."""
+    """The CPython module that calls the serving operators' C entries (see csrc/binding.cpp), built
+    anew where its sources are newer or another torch is installed."""
+    import torch
     src, header = os.path.join(CSRC, "binding.cpp"), os.path.join(ROOT, "include", "dsa_b200.h")
     if not force and os.path.exists(BINDING) and os.path.getmtime(BINDING) > max(
-            os.path.getmtime(src), os.path.getmtime(header)):
+            os.path.getmtime(src), os.path.getmtime(header)) and _built_for(torch.__version__):
         return BINDING
-    import torch
     from torch.utils import cpp_extension
     inc = [ROOT + "/include", sysconfig.get_paths()["include"], *cpp_extension.include_paths(),
            os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include")]
     libs = cpp_extension.library_paths()
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f'-DDSA_TORCH_VERSION="{torch.__version__}"',
            *[f for i in inc for f in ("-isystem", i)], src, *[f"-L{p}" for p in libs],
            "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-o", BINDING + ".tmp"]
     subprocess.run(cmd, check=True)

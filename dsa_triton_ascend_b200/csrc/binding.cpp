@@ -425,4 +425,16 @@ PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, g_method
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__binding(void) { return PyModule_Create(&g_module); }
+// What the module was compiled against: another torch may have another ABI, whose symbols resolve all
+// the same.  The text is what build.py looks for in the built file.
+#define DSA_TORCH_STAMP "dsa binding for torch "
+static const char g_stamp[] = DSA_TORCH_STAMP DSA_TORCH_VERSION;
+
+PyMODINIT_FUNC PyInit__binding(void) {
+  PyObject* m = PyModule_Create(&g_module);
+  if (m && PyModule_AddStringConstant(m, "TORCH_VERSION", g_stamp + sizeof(DSA_TORCH_STAMP) - 1) < 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}

@@ -267,3 +267,39 @@ def test_c_entries_refuse_sizes_that_would_wrap(lib):
     size.restype, size.argtypes = ctypes.c_int64, [ctypes.c_int32] + [ctypes.c_int64] * 3
     for args in ((1, huge, 4, 4), (1, 4, huge, 4), (1, 4, 4, huge), (1, 1 << 31, 4, 4)):
         assert size(*args) == -1
+
+
+def test_binding_of_another_torch(tmp_path, monkeypatch):
+    """A compiled path that was built for another torch is not used, and is built again."""
+    import types
+    from dsa_triton_ascend_b200 import build
+    calls = []
+    other = types.SimpleNamespace(TORCH_VERSION="0.0.1", connect=lambda *a: calls.append(a))
+    monkeypatch.setattr(dsa, "_binding", other, raising=False)
+    monkeypatch.setitem(__import__("sys").modules, "dsa_triton_ascend_b200._binding", other)
+    monkeypatch.setattr(_lib, "_binding", None)
+    assert _lib.binding() is None and not calls
+
+    made = []
+
+    def compile_it(cmd, check):
+        made.append(cmd)
+        with open(cmd[cmd.index("-o") + 1], "wb") as f:
+            f.write(b"new")
+    monkeypatch.setattr(build.subprocess, "run", compile_it)
+    path = tmp_path / "_binding.so"
+    monkeypatch.setattr(build, "BINDING", str(path))
+    path.write_bytes(b"\0dsa binding for torch 0.0.1\0")      # newer than its source
+    build.build_binding()
+    assert len(made) == 1 and path.read_bytes() == b"new"
+    path.write_bytes(b"\0dsa binding for torch " + torch.__version__.encode() + b"\0")
+    build.build_binding()
+    assert len(made) == 1
+
+
+def test_binding_is_of_this_torch():
+    from dsa_triton_ascend_b200 import build
+    if not os.path.exists(build.BINDING):
+        pytest.skip("binding not built")
+    from dsa_triton_ascend_b200 import _binding
+    assert _binding.TORCH_VERSION == torch.__version__
