@@ -393,3 +393,30 @@ def test_extend_of_more_than_the_pool_holds(slots, width, pages, page, seed):
     got = dsa.paged_cache_extend(i32(table), i32(lens), i32(refs), i32(counts), page)
     assert errors() == _grow_in_order(table, lens, refs, counts, page)
     assert _equal(got, (table, lens, refs))
+
+
+def test_append_rotates_rows_of_several_types():
+    """Rotated rows of two and three types, with and without copied ones beside them."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(9)
+    types = [torch.bfloat16, torch.float16, torch.float32, torch.bfloat16]
+    B, S, page = 3, 21, 16
+    starts, counts = [5, 0, 40], [21, 0, 13]
+    table = [[4, 1, 9, 7], [2, 3, 0, 5], [6, 8, 10, 11]]
+    rot = dsa.rotary_table(64, 64)
+    pos = i32(starts)[:, None] + torch.arange(S, device="cuda", dtype=torch.int32)
+    for rotary in ([("interleaved", 0), ("half", 64), None, None], [("half", 0), ("half", 32), ("interleaved", 4), None],
+                   [None, ("interleaved", 8), ("half", 64), ("interleaved", 0)]):
+        caches = [torch.randn(12, page, 1, 128, generator=g, device="cuda").to(t) for t in types]
+        tokens = [torch.randn(B, S, 1, 128, generator=g, device="cuda").to(t) for t in types]
+        ref = [c.clone() for c in caches]
+        for c, t, r in zip(ref, tokens, rotary):
+            if r is not None:
+                t = dsa.rotary_embedding(t, rot, pos, layout=r[0], offset=r[1])
+            for b in range(B):
+                for s in range(counts[b]):
+                    at = starts[b] + s
+                    c[table[b][at // page], at % page] = t[b, s]
+        dsa.paged_cache_append(tokens, caches, i32(table), i32(starts), counts=i32(counts), table=rot, rotary=rotary)
+        assert errors() == 0
+        assert all(torch.equal(x, y) for x, y in zip(caches, ref))

@@ -146,3 +146,51 @@ def test_step_in_a_captured_graph():
         mirror.check(session, [1, 0], out, t[0], t[1])
     dsa.check_device_errors()
     assert state[1].tolist() == [35, 35] and int(state[2].sum()) == 6
+
+
+def test_step_over_the_picked_keys():
+    """A step with ``top_k`` after prompts, a fork, a free and a compaction: the indexer's picks are the
+    highest of the 64-bit scores, and the output is attention over just those keys.
+
+    An index score is sum_h w_h relu(qi_h . ki) over keys and queries that are rotated and rounded to
+    bf16 (2^-8 each), formed in fp32; so it is off by at most 2^-7 + 2^-9 of sum_h |w_h| |qi_h| . |ki|,
+    the second part for the products' sum and second-order terms, and two keys may change places only
+    where their scores are nearer than twice that."""
+    import dsa_triton_ascend_b200 as dsa
+    from paged_serving import PagedSession
+    heads, top_k = 16, 32
+    g = torch.Generator(device="cuda")
+    g.manual_seed(5)
+    rnd = lambda *shape: torch.randn(*shape, generator=g, device="cuda").bfloat16()
+    session, mirror = PagedSession(slots=6, num_pages=40, page_size=16, heads=heads), Mirror()
+    tokens = lambda n, s: [rnd(n, s, heads, 512), rnd(n, s, heads, 64), rnd(n, s, 1, 512), rnd(n, s, 1, 64), rnd(n, s, 1, 128)]
+    t = tokens(3, 90)
+    mirror.add([0, 4, 2], [90, 50, 77], *t[2:])
+    session.prompt(i32(0, 4, 2), i32(90, 50, 77), *t)
+    session.fork(i32(2), i32(5))
+    mirror.rows[5] = mirror.rows[2]
+    session.free(i32(0))
+    session.compact()
+    slots = [5, 4, 2]
+    t = tokens(3, 1)
+    mirror.add(slots, [1] * 3, *t[2:])
+    qi, w = rnd(3, 1, 64, 128), torch.rand(3, 1, 64, generator=g, device="cuda")
+    out = session.step(i32(*slots), *t, query_index=qi, weights=w, top_k=top_k)
+    at = session.lengths[i32(*slots)][:, None] - 1
+    picked, _ = dsa.lightning_indexer_paged(
+        dsa.rotary_embedding(qi, session.table, at, layout="half"), session.caches[2], w, session.block_table[i32(*slots)],
+        actual_seq_lengths_key=session.lengths[i32(*slots)], sparse_count=top_k)
+    dsa.check_device_errors()
+    picked = picked.reshape(3, top_k).long()
+    for n, s in enumerate(slots):
+        total = mirror.rows[s][2].shape[0]
+        mine = picked[n].tolist()
+        assert len(set(mine)) == top_k and 0 <= min(mine) and max(mine) < total
+        k = _rotated(mirror.rows[s][2][:, None], torch.arange(total, device="cuda"), "half")[:, 0]
+        q = _rotated(qi[n, 0][None], i32(total - 1), "half")[0]
+        score = w[n, 0].double() @ (q @ k.t()).relu()
+        slack = (2.0 ** -7 + 2.0 ** -9) * (w[n, 0].double() @ (q.abs() @ k.abs().t()))
+        rest = torch.ones(total, dtype=torch.bool, device="cuda")
+        rest[picked[n]] = False
+        assert bool((score[picked[n]] + slack[picked[n]]).min() >= (score[rest] - slack[rest]).max())
+    mirror.check(session, slots, out, t[0], t[1], picked=picked)
