@@ -558,6 +558,7 @@ extern "C" int dsa_cache_append(const DsaCacheAppendParams* p, void* stream_) {
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   constexpr int64_t kMax = 0x7fffffff;
   if (!p || p->batch < 0 || p->s < 0) return DSA_ERR_INVALID_ARG;
+  if (p->batch == 0 || p->s == 0) return DSA_OK;   // (empty tensors have no address)
   if (p->entries < 1 || p->entries > DSA_APPEND_MAX_ENTRIES || !p->block_table || !p->starts ||
       p->page_size < 1 || p->page_size > kMax || p->max_blocks < 1 || p->max_blocks > kMax / p->page_size ||
       p->num_pages < 1 || p->num_pages > kMax || p->batch > kMax || p->s > kMax)
@@ -578,7 +579,6 @@ extern "C" int dsa_cache_append(const DsaCacheAppendParams* p, void* stream_) {
         (e.offset + p->dim) * size > e.width_bytes || p->max_positions < 1 || p->max_positions > kMax)
       return DSA_ERR_INVALID_ARG;
   }
-  if (p->batch == 0 || p->s == 0) return DSA_OK;
   AppendArgs a = {};
   a.block_table = p->block_table;
   a.starts = p->starts;

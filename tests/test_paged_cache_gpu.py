@@ -420,3 +420,29 @@ def test_append_rotates_rows_of_several_types():
         dsa.paged_cache_append(tokens, caches, i32(table), i32(starts), counts=i32(counts), table=rot, rotary=rotary)
         assert errors() == 0
         assert all(torch.equal(x, y) for x, y in zip(caches, ref))
+
+
+@pytest.mark.parametrize("B,S", [(0, 1), (0, 5), (3, 0), (0, 0)])
+def test_nothing_to_append(B, S):
+    """A step without sequences or without tokens writes nothing, as the other operators take it."""
+    caches = _pool(4, 8, (64, 128))
+    ref = [c.clone() for c in caches]
+    tokens = [torch.empty(B, S, 1, w, device="cuda", dtype=torch.bfloat16) for w in (64, 128)]
+    table, starts = torch.zeros(B, 2, device="cuda", dtype=torch.int32), torch.zeros(B, device="cuda", dtype=torch.int32)
+    rot = dsa.rotary_table(16, 64)
+    for _ in range(2):
+        for kw in (dict(), dict(counts=starts), dict(table=rot, rotary=[("half", 0), None])):
+            back = dsa.paged_cache_append(tokens, caches, table, starts, **kw)
+            assert all(x is y for x, y in zip(back, caches))
+    assert errors() == 0 and all(torch.equal(a, b) for a, b in zip(caches, ref))
+
+
+def test_upkeep_of_no_rows():
+    table, lens, refs, none = i32([[0, -1], [-1, -1]]), i32([5, 0]), i32([1, 0]), i32([])
+    caches = _pool(2, 8, (64,))
+    keep = caches[0].clone()
+    for _ in range(2):
+        assert _equal(dsa.paged_cache_fork(caches, table, lens, refs, none, none), ([[0, -1], [-1, -1]], [5, 0], [1, 0]))
+        assert _equal(dsa.paged_cache_free(table, lens, refs, none), ([[0, -1], [-1, -1]], [5, 0], [1, 0]))
+        assert _equal(dsa.paged_cache_extend(table, lens, refs, i32([0, 0]), 8), ([[0, -1], [-1, -1]], [5, 0], [1, 0]))
+    assert errors() == 0 and torch.equal(caches[0], keep)

@@ -303,3 +303,13 @@ def test_binding_is_of_this_torch():
         pytest.skip("binding not built")
     from dsa_triton_ascend_b200 import _binding
     assert _binding.TORCH_VERSION == torch.__version__
+
+
+def test_c_append_of_nothing(lib):
+    """Empty tensors have no address: a call without batches or tokens is no error, as in the others."""
+    p = _lib.CacheAppendParams()
+    p.num_pages, p.page_size, p.max_blocks, p.entries = 4, 8, 2, 1
+    for p.batch, p.s in ((0, 1), (3, 0), (0, 0)):
+        assert _call(lib, "dsa_cache_append", p) == 0
+    p.batch = p.s = 1
+    assert _call(lib, "dsa_cache_append", p) == 1
