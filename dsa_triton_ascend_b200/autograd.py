@@ -173,18 +173,19 @@ class SparseAttentionWithIndexer(torch.nn.Module):
 
 
 class RotaryEmbeddingFunction(torch.autograd.Function):
-    """out = rotary_embedding(x, table, positions, layout, offset); the gradient of ``x`` turns
-    back by the same table (amplitude kept), nothing of the forward but the positions is saved."""
+    """out = rotary_embedding(x, table, positions, layout, offset, inverse); the gradient of ``x`` turns
+    the other way by the same table (amplitude kept) and has a gradient of its own.  Nothing of the
+    forward but the table and positions is saved."""
 
     @staticmethod
-    def forward(ctx, x, table, positions, layout="interleaved", offset=0):
+    def forward(ctx, x, table, positions, layout="interleaved", offset=0, inverse=False):
         ctx.save_for_backward(table, positions)
-        ctx.cfg = (layout, offset)
-        return rotary_embedding(x, table, positions, layout=layout, offset=offset)
+        ctx.cfg = (layout, offset, inverse)
+        return rotary_embedding(x, table, positions, layout=layout, offset=offset, inverse=inverse)
 
     @staticmethod
     def backward(ctx, d_out):
         table, positions = ctx.saved_tensors
-        layout, offset = ctx.cfg
-        return rotary_embedding(d_out, table, positions, layout=layout, offset=offset,
-                                inverse=True), None, None, None, None
+        layout, offset, inverse = ctx.cfg
+        turn = RotaryEmbeddingFunction.apply if d_out.requires_grad else rotary_embedding
+        return turn(d_out, table, positions, layout, offset, not inverse), None, None, None, None, None

@@ -184,3 +184,19 @@ def test_on_another_stream():
         got = dsa.rotary_embedding(x, table, pos)
     side.synchronize()
     assert torch.equal(got, ref)
+
+
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+def test_gradient_of_the_gradient(layout):
+    """The gradient is linear in d(out), so it has a gradient of its own: the rotation again.  With
+    g = R^T w, the sum of g v has the derivative R v in w."""
+    x = torch.randn(1, 3, 2, 12, generator=_gen(8), device="cuda", requires_grad=True)
+    w = torch.randn(x.shape, generator=_gen(9), device="cuda", requires_grad=True)
+    v = torch.randn(x.shape, generator=_gen(10), device="cuda")
+    pos = torch.tensor([[0, 5, 1000]], device="cuda", dtype=torch.int32)
+    table = dsa.rotary_table(1001, 8)
+    y = dsa.RotaryEmbeddingFunction.apply(x, table, pos, layout, 2)
+    g, = torch.autograd.grad(y, x, w, create_graph=True)
+    for got, arg, inverse in ((g, w, True), (torch.autograd.grad(g, w, v)[0], v, False)):
+        ref, bound = _expect(arg.detach(), pos, dsa.rotary_frequencies(8), 1.0, layout, 2, inverse)
+        assert bool(((got.detach().double() - ref).abs() <= bound).all())
