@@ -19,6 +19,8 @@
 // that see no key.
 #include <cuda_runtime.h>
 
+#include <cmath>
+
 #include "attn_paged.cuh"
 #include "attn_paged_pair.cuh"
 #include "attn_paged_wide.cuh"
@@ -1000,7 +1002,7 @@ extern "C" int dsa_attn_paged(const DsaAttnPagedParams* p, void* stream_) {
   if (!p || p->batch < 0 || p->s1 < 0) return DSA_ERR_INVALID_ARG;
   if (p->batch == 0 || p->s1 == 0) return DSA_OK;
   if (p->n1 < 1 || p->n1 > 128 || p->page_size < 8 || p->page_size % 8 || p->max_blocks < 1 ||
-      p->num_pages < 1 || (p->sparse_mode != 0 && p->sparse_mode != 3) || !p->query ||
+      p->num_pages < 1 || (p->sparse_mode != 0 && p->sparse_mode != 3) || !std::isfinite(p->scale) || !p->query ||
       !p->query_rope || !p->key_cache || !p->key_rope_cache || !p->act_k || !p->block_table ||
       !p->out || !p->workspace)
     return DSA_ERR_INVALID_ARG;

@@ -15,6 +15,7 @@ from ._lib import BIND_ATTN, AttnPagedParams, binding, check, lib, remember, rep
 
 _VALID_D = (128, 256, 512)
 _D_ROPE = 64
+_MAX_SCALE = torch.finfo(torch.float32).max
 
 
 def _tma_strides(t: torch.Tensor):
@@ -40,6 +41,8 @@ def _plan(query, query_rope, key_cache, key_rope_cache, block_table, scale_value
     statistics' shape, workspace bytes).  `counted`: with a count of queries per sequence."""
     if sparse_mode not in (0, 3):
         raise ValueError("Only sparse_mode 0 (full) / 3 (rightDownCausal) supported")
+    if not abs(scale_value) <= _MAX_SCALE:
+        raise ValueError(f"scale_value must be finite in float32, got {scale_value}")
     if query.dim() != 4 or query_rope.dim() != 4:
         raise ValueError("query and query_rope must be [B, S1, N1, D]")
     if key_cache.dim() != 4 or key_rope_cache.dim() != 4:

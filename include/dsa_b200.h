@@ -409,7 +409,7 @@ int64_t dsa_dense_indexer_workspace_size(int64_t batch, int64_t s1, int64_t s2, 
  *   entry >= num_pages is treated so and reported in error_flag.
  *   act_q [batch] (NULL: s1).  Row (b, s) sees key positions t < min(act_k, max_blocks *
  *   page_size), in sparse_mode 3 also t < act_k - act_q + s + 1; rows s >= act_q see none.
- * Rows of a page past the row's keys are not used, whatever they hold.
+ * Rows of a page past the row's keys are not used, whatever they hold.  scale is finite.
  * Outputs: out [batch][s1][n1][d]; softmax_max / softmax_sum [batch][s1][n1] fp32 (both NULL
  * to skip) as in dsa_sfa_fwd; rows without keys, or whose scores are all -inf, get zeros.  The
  * result does not depend on timing: the parts of a split row are joined in one order.

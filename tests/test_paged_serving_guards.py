@@ -313,3 +313,16 @@ def test_c_append_of_nothing(lib):
         assert _call(lib, "dsa_cache_append", p) == 0
     p.batch = p.s = 1
     assert _call(lib, "dsa_cache_append", p) == 1
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf"), 1e39])
+def test_scale_that_no_fp32_holds(lib, scale):
+    """The kernels keep the scale above 0 by a maximum, which a NaN would pass unseen."""
+    with pytest.raises(ValueError, match="scale_value"):
+        attn(scale_value=scale)
+    p = _lib.AttnPagedParams()
+    for f in ("query", "query_rope", "key_cache", "key_rope_cache", "block_table", "act_k", "out", "workspace"):
+        setattr(p, f, 1 << 20)
+    p.batch, p.s1, p.n1, p.d, p.num_pages, p.page_size, p.max_blocks, p.scale = 2, 1, 16, 512, 4, 16, 2, scale
+    p.workspace_bytes = 1 << 40
+    assert _call(lib, "dsa_attn_paged", p) == 1
