@@ -4,8 +4,8 @@
 //   z[h][t] = scale * (q[h] . k[t] + qr[h] . kr[t]),  m = max_t z,  p = exp(z - m),
 //   l = sum_t p,  out[h] = (sum_t p k[t][0:D]) / l.
 //
-// attn_paged_kernel: a persistent CTA per SM takes an equal share of all (row, head group)
-// tiles of 64 keys, so a long row is split over several CTAs and short rows share one.  The
+// attn_paged_kernel: a persistent CTA per SM takes an equal share of all rows' tiles of 64 keys,
+// so a long row is split over several CTAs and short rows share one.  The
 // products are formed with the keys on the M side of the tensor core:
 //   S^T [64 keys x NH heads]  = K [64 x (D + 64)] Q^T       (M = 64)
 //   O^T [D x NH heads]       += V^T [D x 64] P^T            (M = 128, D / 128 blocks)
@@ -32,7 +32,7 @@ namespace dsa {
 namespace attn_paged {
 
 constexpr int kTile = 64;       // keys of a step
-constexpr int kSegmentCost = 2; // of starting an item, in tiles
+constexpr int kSegmentCost = 2; // of starting a row, in tiles
 constexpr int kSoftmaxThreads = 128;   // of a warpgroup; there are two (warps 0-3, 4-7), each with
                                        // half of the heads
 constexpr int kLoadWarp = 8;           // warps 8-11: loads (one warp issues a box in 160 cycles,
@@ -54,7 +54,7 @@ struct Cfg {
   static constexpr int kQBytes = NH * (D + kRope) * 2;
   static constexpr int kHeads = NH / 2;   // of a softmax warpgroup
   static constexpr int kPBytes = kTile * NH * 2;
-  // row maxima of two tiles per warp, factors, barriers and the rest
+  // per warp row maxima and sums, then factors, barriers and the rest
   static constexpr int kSmallBytes = 2 * 4 * NH * 4 + NH * 4 + 512;
   static constexpr int kRoom = (kSmemLimit - kQBytes - kPBytes - kSmallBytes) / kStageBytes;
   static constexpr int kStages = kRoom < kMaxStages ? kRoom : kMaxStages;
@@ -140,13 +140,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t s_q = base + C::kStages * C::kStageBytes;
   const uint32_t s_p = s_q + C::kQBufs * C::kQBytes;
   uint8_t* small = smem + C::kStages * C::kStageBytes + C::kQBufs * C::kQBytes + C::kPBytes;
-  float* wmax = reinterpret_cast<float*>(small);          // [2][4][NH]
+  float* wmax = reinterpret_cast<float*>(small);          // [4][NH], then the sums, [4][NH]
   float* factor = wmax + 2 * 4 * NH;                      // [NH]
   uint64_t* bars = reinterpret_cast<uint64_t*>(factor + NH);
   int32_t* tmask = reinterpret_cast<int32_t*>(bars + 32);  // [kMaxStages][4]
   int32_t* tmp = tmask + 4 * kMaxStages;                   // [16]
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(tmp + 16);
-  int32_t* start = reinterpret_cast<int32_t*>(tmem_ptr + 1);   // [3]
+  int32_t* start = reinterpret_cast<int32_t*>(tmem_ptr + 1);   // [2]
 
   const uint32_t b0 = smem_u32(bars);
   auto full = [&](int s) { return b0 + 8u * s; };
@@ -261,8 +261,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) {
         const uint32_t dst = s_q + buf * C::kQBytes;
         mbar_arrive_expect_tx(q_full(buf), C::kQBytes);
-        tma_load_5d(dst, &maps.q, q_full(buf), 0, sg.group * NH, 0, s, b);
-        tma_load_5d(dst + NH * D * 2, &maps.qr, q_full(buf), 0, sg.group * NH, 0, s, b);
+        tma_load_5d(dst, &maps.q, q_full(buf), 0, 0, 0, s, b);
+        tma_load_5d(dst + NH * D * 2, &maps.qr, q_full(buf), 0, 0, 0, s, b);
       }
       __syncwarp();
       ++nseg;
@@ -526,29 +526,32 @@ __global__ void __launch_bounds__(kThreads, 1)
               make_float2(run[2 * j], run[2 * j + 1]);
         }
       softmax_bar(wg);
+      // opaque, so that what hangs on it (a test per head) is not made before the loop and held in
+      // registers through it: 28 bytes of spills at 64 heads, 140 us against 138 at D = 256
+      int n1 = a.n1;
+      asm volatile("" : "+r"(n1));
       const bool all = sg.count == sg.tiles, whole = all && a.diag == 0;
       const int64_t slot = all ? (int64_t)2 * gridDim.x + sg.row : 2 * blockIdx.x + (nseg == 0 ? 0 : 1);
       if (quarter == 0 && lane < 4)
 #pragma unroll
         for (int j = 0; j < 2 * kPairs; ++j) {
-          const int h = 8 * (j >> 1) + col + (j & 1), head = sg.group * NH + h;
+          const int h = 8 * (j >> 1) + col + (j & 1);
           const float l = wsum[h] + wsum[NH + h] + wsum[2 * NH + h] + wsum[3 * NH + h];
           const float m = fmaxf(fmaxf(wmax[h], wmax[NH + h]), fmaxf(wmax[2 * NH + h], wmax[3 * NH + h]));
           const bool any = m != -INFINITY;
           const float most = any ? m * c2 : -INFINITY;
           factor[h] = !whole ? 1.0f : l > 0.0f || l != l ? 1.0f / l : 0.0f;
-          if (head >= a.n1) continue;
+          if (h >= n1) continue;
           if (!whole) {
             a.ws_s[slot * NH + h] = make_float4(ref[j] - kShift, most, l, m);
           } else if (a.softmax_max) {
-            const int64_t at = (int64_t)sg.row * a.n1 + head;
-            put_stats(a, at, m, ref[j] - kShift, most, l);
+            put_stats(a, (int64_t)sg.row * n1 + h, m, ref[j] - kShift, most, l);
           }
         }
       softmax_bar(wg);
       mbar_wait_hot(p_empty, (g - 1) & 1, a.error_flag, &failed);
       tc_fence_after();
-      const int heads = min(head0 + HW, a.n1 - sg.group * NH);
+      const int heads = min(head0 + HW, n1);
       const int dim = quarter * 32 + lane;
 #pragma unroll 1
       for (int m = 0; m < C::kBlocks; ++m)
@@ -559,7 +562,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_ld_wait();
           if (whole) {
             T* out = static_cast<T*>(a.out) +
-                     ((int64_t)sg.row * a.n1 + sg.group * NH + h0) * D + m * 128 + dim;
+                     ((int64_t)sg.row * n1 + h0) * D + m * 128 + dim;
 #pragma unroll
             for (int j = 0; j < kCols; ++j)
               if (h0 + j < heads) out[j * D] = E::from_f(__uint_as_float(o[j]) * factor[h0 + j]);
@@ -597,8 +600,8 @@ struct Parts {
 };
 
 // False for a row without a part (c1 < c0).
-template <int NH, int kCost>
-__device__ __forceinline__ bool parts_of(const Args& a, int grid, int row, int head, Parts* p) {
+template <int kCost>
+__device__ __forceinline__ bool parts_of(const Args& a, int grid, int row, Parts* p) {
   const int first = a.ws_prefix[row], next = a.ws_prefix[row + 1], all = a.ws_prefix[a.rows];
   const int count = next - first;   // units
   p->own = 2 * grid + row;
@@ -606,8 +609,7 @@ __device__ __forceinline__ bool parts_of(const Args& a, int grid, int row, int h
   p->c0 = 1;
   p->c1 = 0;
   if (count == 0) return false;
-  const int64_t units = (int64_t)all * a.groups, ctas = ctas_used(units, grid);
-  const int64_t x0 = (int64_t)first * a.groups + (int64_t)(head / NH) * count;
+  const int64_t units = all, ctas = ctas_used(units, grid), x0 = first;
   const int64_t lo = (x0 + kCost + 1) * ctas - 1, hi = (x0 + count) * ctas - 1;
   if (units * ctas < (1LL << 32)) {
     const uint32_t u = (uint32_t)units;
@@ -673,11 +675,11 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_combine_kernel(const 
   griddep_launch_dependents();
   const int64_t at = (int64_t)blockIdx.x * (kJoinThreads / kLanes) + threadIdx.x / kLanes;
   if (at >= (int64_t)a.rows * a.n1) return;
-  const int row = (int)(at / a.n1), head = (int)(at - (int64_t)row * a.n1), h = head % NH;
+  const int row = (int)(at / a.n1), head = (int)(at - (int64_t)row * a.n1);
   const int t = threadIdx.x % kLanes, grp = t / kCols, col = t % kCols, lane = threadIdx.x & 31;
   T* out = static_cast<T*>(a.out) + at * D;
   Parts p;
-  const bool some = parts_of<NH, kCost>(a, grid, row, head, &p);
+  const bool some = parts_of<kCost>(a, grid, row, &p);
   // keys from `common` on that this token sees beside the row's common ones
   int late = 0, common = 0;
   if (a.diag > 0) {
@@ -703,7 +705,7 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_combine_kernel(const 
   }
   float ref = -INFINITY, run = -INFINITY, top = -INFINITY;
   for (int c = p.c0 + lane; c <= p.c1; c += 32) {
-    const float4 s = a.ws_s[p.at<NH>(c, h)];
+    const float4 s = a.ws_s[p.at<NH>(c, head)];
     ref = fmaxf(ref, s.x);
     run = fmaxf(run, s.y);
     top = fmaxf(top, s.w);
@@ -720,8 +722,8 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_combine_kernel(const 
   float sum = 0.0f;
 #pragma unroll 4
   for (int c = p.c0 + grp; c <= p.c1; c += kGroups) {
-    const float4 s = a.ws_s[p.at<NH>(c, h)];
-    const float4* o = reinterpret_cast<const float4*>(a.ws_o + p.at<NH>(c, h) * D) + col;
+    const float4 s = a.ws_s[p.at<NH>(c, head)];
+    const float4* o = reinterpret_cast<const float4*>(a.ws_o + p.at<NH>(c, head) * D) + col;
     const float w = s.x == ref ? 1.0f : exp2f(s.x - ref);
     sum += w * s.z;
 #pragma unroll
@@ -776,7 +778,7 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_combine_kernel(const 
   if (t == 0 && a.softmax_max) put_stats(a, at, top, ref, run, sum);
 }
 
-// Heads of a work item: the smallest operand that holds them.  Past 64 they are taken whole: at
+// Heads of a row as the kernels hold them: the smallest size that they fit.  Past 64 they are taken whole: at
 // D = 512 by the pair kernel (32 rows of 8192 .. 65536 keys, 128 heads: 356 us against 502 for two
 // items of 64), below by the wide one (the same rows at D = 256: 185 us against 266; a pair there
 // took 314).
@@ -784,7 +786,7 @@ int heads_of(int64_t n1) { return n1 <= 16 ? 16 : n1 <= 32 ? 32 : n1 <= 64 ? 64 
 
 int64_t align256(int64_t x) { return (x + 255) & ~(int64_t)255; }
 
-// What the kernels take; `nh` heads a work item, `shares` of the work.
+// What the kernels take; `nh` heads a row, `shares` of the work.
 Args make_args(const DsaAttnPagedParams* p, int nh, int shares, int diag, int heads) {
   Args a;
   a.act_q = p->act_q;
@@ -797,7 +799,6 @@ Args make_args(const DsaAttnPagedParams* p, int nh, int shares, int diag, int he
   a.rows = (int)(p->batch * p->s1);
   a.s1 = (int)p->s1;
   a.n1 = (int)p->n1;
-  a.groups = 1;
   a.page_size = (int)p->page_size;
   a.max_blocks = (int)p->max_blocks;
   a.num_pages = (int)p->num_pages;
@@ -882,8 +883,7 @@ int launch(const DsaAttnPagedParams* p, int diag, int heads, cudaStream_t stream
   if (grid < 1) return DSA_ERR_CUDA;
   Maps maps;
   if (!make_maps<D>(&maps, p, ElemTraits<T>::kIsBf16, NH)) return DSA_ERR_TMA_DESCRIPTOR;
-  Args a = make_args(p, NH, grid, diag, heads);
-  a.groups = (int)((p->n1 + NH - 1) / NH);
+  const Args a = make_args(p, NH, grid, diag, heads);
   auto kern = attn_paged_kernel<D, NH, T>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) !=
       cudaSuccess)
@@ -945,7 +945,7 @@ int launch_heads(const DsaAttnPagedParams* p, int diag, int heads, cudaStream_t 
 }
 
 // Whether several new tokens of a batch can be taken as one row of s1 * n1 heads, so that their
-// keys are read once: up to 8 tokens, all of them valid, whose heads fit one work item (4 x 8 tokens,
+// keys are read once: up to 8 tokens, all of them valid, with 128 heads in all at most (4 x 8 tokens,
 // 16 heads, D = 256, up to 65536 keys: 53 us against 115 token by token).
 bool packs(int64_t s1, int64_t n1) {
   return s1 > 1 && s1 <= kMaxDiag + 1 && s1 * n1 <= 128;

@@ -25,11 +25,11 @@ struct Args {
   float* softmax_max;
   float* softmax_sum;
   int* error_flag;
-  int32_t* ws_prefix;   // [rows + 1] units of the rows before each (of one head group)
+  int32_t* ws_prefix;   // [rows + 1] units of the rows before each
   float* ws_o;          // [slots][NH][D], slots: two of each CTA, then one of each row (diag > 0)
   float4* ws_s;         // [slots][NH]: reference and running maximum (log2 units), sum, raw
                         // running maximum
-  int32_t rows, s1, n1, groups;
+  int32_t rows, s1, n1;
   // Several new tokens of a batch as one row of s1 * heads heads (s1 is 1 then): the kernels take
   // the keys that all of them see; the last `diag` ones, which only the later tokens see, are
   // taken in by the join.
@@ -59,8 +59,8 @@ __device__ __forceinline__ int row_units(const Args& a, int row) {
   return tiles > 0 ? tiles + kCost : 0;
 }
 
-// Work is divided by units: an item (a row's head group) of T tiles has T + kCost of them, the
-// first kCost standing for what a CTA spends on starting an item (queries, filling the pipeline,
+// Work is divided by units: a row of T tiles (with all of its heads) has T + kCost of them, the
+// first kCost standing for what a CTA spends on starting a row (queries, filling the pipeline,
 // the result).  CTA c of n takes units [U c / n, U (c + 1) / n) of all U.
 
 // CTAs (pairs of them in the pair kernel) that share `units`; each takes kMinUnits at least, as
@@ -94,35 +94,27 @@ __device__ __forceinline__ int block_scan(int v, int* tmp, int* total) {
   return before + x - v;
 }
 
-// One CTA's share: `left` units from unit `unit` of (row, head group) on.
+// One CTA's share: `left` units from unit `unit` of a row on.
 struct Work {
-  int row, group, unit, left;
+  int row, unit, left;
 };
-// A run of tiles of one (row, head group).
+// A run of tiles of one row.
 struct Segment {
-  int row, group, first, count, keys, tiles;
+  int row, first, count, keys, tiles;
 };
 // The next run of `w` (false when the share is done); `w` moves past it.
 template <int kTile, int kCost>
 __device__ __forceinline__ bool next_segment(const Args& a, Work& w, Segment& s) {
   while (w.left > 0 && w.row < a.rows) {
-    s.keys = row_keys(a, w.row);
+    s.row = w.row++;
+    s.keys = row_keys(a, s.row);
     s.tiles = (s.keys + kTile - 1) / kTile;
-    if (s.tiles == 0) {
-      ++w.row;
-      continue;
-    }
+    if (s.tiles == 0) continue;
     const int end = min(s.tiles + kCost, w.unit + w.left);
-    s.row = w.row;
-    s.group = w.group;
     s.first = max(0, w.unit - kCost);
     s.count = max(0, end - kCost) - s.first;
     w.left -= end - w.unit;
     w.unit = 0;
-    if (++w.group == a.groups) {
-      w.group = 0;
-      ++w.row;
-    }
     if (s.count > 0) return true;
   }
   return false;
@@ -140,7 +132,7 @@ __device__ __forceinline__ int64_t share_begin(int64_t units, int64_t c, int64_t
 template <int kTile, int kCost, int kThreads>
 __device__ __forceinline__ Work share_of(const Args& a, int cta, int ctas_max, bool first_cta, int* tmp,
                                          int32_t* start) {
-  Work work{0, 0, 0, 0};
+  Work work{0, 0, 0};
   if (a.rows <= 32) {
     // each warp for itself, without a barrier
     const int lane = threadIdx.x & 31;
@@ -156,21 +148,18 @@ __device__ __forceinline__ Work share_of(const Args& a, int cta, int ctas_max, b
       if (lane < a.rows) a.ws_prefix[lane] = x - mine;
       if (lane == 0) a.ws_prefix[a.rows] = total;
     }
-    const int64_t units = (int64_t)total * a.groups, ctas = ctas_used(units, ctas_max);
+    const int64_t units = total, ctas = ctas_used(units, ctas_max);
     if (cta >= ctas) return work;
     const int64_t from = share_begin(units, cta, ctas);
     work.left = (int)(share_begin(units, cta + 1, ctas) - from);
-    const int64_t first = (int64_t)(x - mine) * a.groups;
-    const uint32_t here = __ballot_sync(0xffffffffu, mine > 0 && first <= from && from < first + (int64_t)mine * a.groups);
+    const int first = x - mine;
+    const uint32_t here = __ballot_sync(0xffffffffu, mine > 0 && first <= from && from < (int64_t)first + mine);
     if (here == 0) {   // no unit at all
       work.left = 0;
       return work;
     }
-    const int row = __ffs(here) - 1;
-    const int in = (int)(from - __shfl_sync(0xffffffffu, first, row)), per = __shfl_sync(0xffffffffu, mine, row);
-    work.row = row;
-    work.group = in / per;
-    work.unit = in - work.group * per;
+    work.row = __ffs(here) - 1;
+    work.unit = (int)(from - __shfl_sync(0xffffffffu, first, work.row));
     return work;
   }
   int64_t total = 0;
@@ -184,8 +173,7 @@ __device__ __forceinline__ Work share_of(const Args& a, int cta, int ctas_max, b
     total += sum;
   }
   if (first_cta && threadIdx.x == 0) a.ws_prefix[a.rows] = (int)total;
-  const int64_t units = total * a.groups;
-  const int64_t ctas = ctas_used(units, ctas_max);
+  const int64_t units = total, ctas = ctas_used(units, ctas_max);
   if (units == 0 || cta >= ctas) return work;
   const int64_t from = share_begin(units, cta, ctas);
   work.left = (int)(share_begin(units, cta + 1, ctas) - from);
@@ -197,20 +185,17 @@ __device__ __forceinline__ Work share_of(const Args& a, int cta, int ctas_max, b
       mine = r < a.rows ? row_units<kTile, kCost>(a, r) : 0;
       before = block_scan<kThreads>(mine, tmp, &sum);
     }
-    const int64_t first = (seen + before) * a.groups;
-    if (mine > 0 && first <= from && from < first + (int64_t)mine * a.groups) {
-      const int in = (int)(from - first);
+    const int64_t first = seen + before;
+    if (mine > 0 && first <= from && from < first + mine) {
       start[0] = r;
-      start[1] = in / mine;
-      start[2] = in - (in / mine) * mine;
+      start[1] = (int)(from - first);
     }
     seen += sum;
-    if (seen * a.groups > from) break;   // the same for every thread
+    if (seen > from) break;   // the same for every thread
   }
   __syncthreads();
   work.row = start[0];
-  work.group = start[1];
-  work.unit = start[2];
+  work.unit = start[1];
   return work;
 }
 

@@ -89,7 +89,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(wsum + 4 * kHeads);
   int32_t* tmp = reinterpret_cast<int32_t*>(bars + 16);          // [16]
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(tmp + 16);
-  int32_t* start = reinterpret_cast<int32_t*>(tmem_ptr + 1);     // [3]
+  int32_t* start = reinterpret_cast<int32_t*>(tmem_ptr + 1);     // [2]
 
   const uint32_t b0 = smem_u32(bars);
   const uint32_t k_full = b0, k_empty = b0 + 8;                // the leader's; each CTA's

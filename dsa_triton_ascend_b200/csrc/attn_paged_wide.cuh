@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   int32_t* tmask = reinterpret_cast<int32_t*>(bars + 46);        // [kMaxStages][4]
   int32_t* tmp = tmask + 4 * kMaxStages;                         // [16]
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(tmp + 16);
-  int32_t* start = reinterpret_cast<int32_t*>(tmem_ptr + 1);     // [3]
+  int32_t* start = reinterpret_cast<int32_t*>(tmem_ptr + 1);     // [2]
 
   const uint32_t b0 = smem_u32(bars);
   auto full = [&](int s) { return b0 + 8u * s; };
