@@ -3,6 +3,11 @@
 // For a query row r (one token) with n visible keys, head h and t < n:
 //   z[h][t] = scale * (q[h] . k[t] + qr[h] . kr[t]),  m = max_t z,  p = exp(z - m),
 //   l = sum_t p,  out[h] = (sum_t p k[t][0:D]) / l.
+// Scores, maxima, sums, the products' results and the join are fp32.  p alone is rounded to the
+// key type, as the operand of the second product that the tensor core takes (by up to 2^-8 of p in
+// bf16, 2^-11 in fp16; l is the sum of the unrounded ones).  In bf16 the result's relative error is
+// 2.0e-3 on 1021 keys, where fp32 probabilities with one rounding of the result leave 1.7e-3, and
+// 1.7e-3 for both on 8192 .. 65536 keys.
 //
 // attn_paged_kernel: a persistent CTA per SM takes an equal share of all rows' tiles of 64 keys,
 // so a long row is split over several CTAs and short rows share one.  The
@@ -468,7 +473,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           softmax_bar(wg);   // the factors are read: the next tile may write its own
         }
         const bool p_free = g == 0 || mbar_test_wait(p_empty, (g - 1) & 1);   // used below
-        // probabilities; a column without any key so far has reference -inf and stays zero
+        // probabilities, summed in fp32 and rounded for the product; a column without any key so
+        // far has reference -inf and stays zero
         uint32_t packed[HW / 4];
 #pragma unroll
         for (int j = 0; j < kPairs; ++j) {
@@ -778,10 +784,10 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_combine_kernel(const 
   if (t == 0 && a.softmax_max) put_stats(a, at, top, ref, run, sum);
 }
 
-// Heads of a row as the kernels hold them: the smallest size that they fit.  Past 64 they are taken whole: at
-// D = 512 by the pair kernel (32 rows of 8192 .. 65536 keys, 128 heads: 356 us against 502 for two
-// items of 64), below by the wide one (the same rows at D = 256: 185 us against 266; a pair there
-// took 314).
+// Heads of a row as the kernels hold them: the smallest size that they fit.  Past 64 they are
+// taken whole: at D = 512 by the pair kernel (32 rows of 8192 .. 65536 keys, 128 heads, in a burst:
+// 356 us against 502 for two items of 64), below by the wide one (the same rows at D = 256: 185 us
+// against 266; a pair there took 314).
 int heads_of(int64_t n1) { return n1 <= 16 ? 16 : n1 <= 32 ? 32 : n1 <= 64 ? 64 : 128; }
 
 int64_t align256(int64_t x) { return (x + 255) & ~(int64_t)255; }
@@ -945,8 +951,9 @@ int launch_heads(const DsaAttnPagedParams* p, int diag, int heads, cudaStream_t 
 }
 
 // Whether several new tokens of a batch can be taken as one row of s1 * n1 heads, so that their
-// keys are read once: up to 8 tokens, all of them valid, with 128 heads in all at most (4 x 8 tokens,
-// 16 heads, D = 256, up to 65536 keys: 53 us against 115 token by token).
+// keys are read once: up to 8 tokens, all of them valid (with act_q each is a row of its own), with
+// 128 heads in all at most (4 x 8 tokens, 16 heads, D = 256, up to 65536 keys: 53 us against 115
+// token by token; short rows lose, 8 x 2 tokens of 64 heads over 500 .. 4000 keys 31 against 28).
 bool packs(int64_t s1, int64_t n1) {
   return s1 > 1 && s1 <= kMaxDiag + 1 && s1 * n1 <= 128;
 }

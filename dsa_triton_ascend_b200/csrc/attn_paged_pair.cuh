@@ -13,7 +13,8 @@
 // A tile of 128 keys and the queries leave room for one buffer each of K and V at D = 512.  V is
 // held in halves of 64 keys with barriers of their own, so that the next tile's first half is on
 // its way while the second is in work.  32 rows of 8192 .. 65536 keys and 128 heads take
-// 351 us in a burst and 385 under the power cap.  (Not kept, as slower at those rows: K in three
+// 342 to 355 us in a burst (1,965 MHz) and 385 to 425 under the power cap, by the card (400 at
+// 985 W and 1,470 to 1,530 MHz).  (Not kept, as slower at those rows: K in three
 // parts of 192 dims, refilled one by one, 369 us against 347, since the loads then meet QK's
 // operand reads, and shared memory, at 400 KB a tile and CTA, is what bounds this kernel; P in
 // halves, 366 against 351; tiles brought into L2 ahead of their load, 364 against 356.)
@@ -431,7 +432,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           asm volatile("bar.sync 1, %0;" ::"n"(kSoftmaxThreads) : "memory");   // the maxima are read
         }
         const bool p_free = g == 0 || mbar_test_wait(p_empty, (g - 1) & 1);
-        // probabilities; a head without any key so far has reference -inf and stays zero
+        // probabilities, summed in fp32 and rounded for the product (see attn_paged.cu); a head
+        // without any key so far has reference -inf and stays zero
         const float off = ref == -INFINITY ? 0.0f : kShift - ref;
         uint32_t pk[16];
 #pragma unroll

@@ -353,7 +353,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           meet();   // the maxima are read
         }
-        // probabilities; a head without any key so far has reference -inf and stays zero
+        // probabilities, summed in fp32 and rounded for the product (see attn_paged.cu); a head
+        // without any key so far has reference -inf and stays zero
         const float off = ref == -INFINITY ? 0.0f : kShift - ref;
         uint32_t pk[16];
 #pragma unroll

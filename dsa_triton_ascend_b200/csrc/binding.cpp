@@ -3,9 +3,10 @@
 // Arguments are checked in Python (the operators' modules), once for each signature: shapes,
 // strides, types, devices and options.  What they decide, the filled-in parameter struct, is
 // then kept here under that signature, and a call whose signature is known allocates its
-// outputs, puts in the addresses and calls the library: some 5 us instead of 10 to 25.  Any other
-// call (a new signature, another current device, an address that is not aligned) is answered
-// with None and takes the Python path.  Nothing is kept by address.
+// outputs, puts in the addresses and calls the library: 5 us for a rotation or an append, 11 for
+// upkeep, 13 for attention, instead of 17 to 70 (attention 39).  Any other call (a new signature,
+// another current device, an address that is not aligned) is answered with None and takes the
+// Python path.  Nothing is kept by address.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 

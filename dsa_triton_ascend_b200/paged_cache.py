@@ -152,7 +152,8 @@ def paged_cache_append(tokens, caches, block_table, starts, counts=None, table=N
     ``block_table`` [B, max_blocks].  ``rotary[i]`` is None or (layout, offset): those rows are
     rotated on the way by ``table`` (:func:`rotary_table`) at their position, as
     ``rotary_embedding`` would.  A token without a page, or past the table, is left out and
-    reported.  Rows are whole 16-byte pieces.
+    reported.  Rows are whole 16-byte pieces; neither the tokens nor two caches share memory with
+    rows that are written.
     """
     tokens, caches = list(tokens), list(caches)
     args = (tokens, caches, block_table, starts, counts, table, rotary)
@@ -305,8 +306,9 @@ def paged_cache_extend(block_table, seq_lengths, ref_counts, counts, page_size):
 def paged_cache_fork(caches, block_table, seq_lengths, ref_counts, parents, children, page_size=None):
     """Make the empty slots ``children[i]`` [n] copies of the sequences ``parents[i]``: they share
     the parents' full pages, and a partly filled last page is copied (its filled rows, in every
-    cache) to a page of the child's own.  Returns the new (block_table, seq_lengths, ref_counts).
-    ``page_size`` is needed where ``caches`` is empty."""
+    cache) to a page of the child's own.  A full block without a page in the parent has none in the
+    child and is reported.  Returns the new (block_table, seq_lengths, ref_counts).  ``page_size`` is
+    needed where ``caches`` is empty."""
     return _upkeep(PAGES_FORK, list(caches), block_table, seq_lengths, ref_counts, parents, children,
                    page_size)
 

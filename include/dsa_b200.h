@@ -494,8 +494,9 @@ int dsa_rotary_table(float* table, int64_t max_positions, int64_t dim, const dou
  * goes to position starts[b] + s, i.e. row pos % page_size of page block_table[b][pos /
  * page_size], in up to four caches at once; rows with a rotary layout are rotated by their
  * position on the way.  No counterpart in the reference.  All strides are in bytes and
- * multiples of 16, as are bases and widths.  A token whose position is past the table or the
- * block table, or whose page is not in the pool, is left out and reported in error_flag.
+ * multiples of 16, as are bases and widths.  Rows of src and of the caches do not overlap.
+ * A token whose position is past the table or the block table, or whose page is not in the pool,
+ * is left out and reported in error_flag.
  */
 #define DSA_ROTARY_NONE 0
 #define DSA_ROTARY_INTERLEAVED 1
@@ -540,7 +541,9 @@ int dsa_cache_append(const DsaCacheAppendParams* params, void* stream);
  *   COPY     n pairs first[i] -> second[i] of pages; a negative id skips the pair.  No page is
  *            both written and read.  Only num_pages, page_size, caches and the pairs are read.
  *   FORK     n pairs parent row first[i] -> empty row second[i]: the child shares the parent's
- *            full pages and gets a page of its own with the rows of the partly filled one.
+ *            full pages and gets a page of its own with the rows of the partly filled one.  A full
+ *            block for which the parent's table names no page of the pool has none in the child
+ *            either and is reported; the fork is made.
  *   EXTEND   row r grows by first[r] tokens (n == slots), with the pages that takes.  Rows are
  *            served in order; one that the pages left cannot serve takes none of them.
  *   FREE     n rows first[i] give their pages back and become empty.
