@@ -51,7 +51,10 @@ from .dense_indexer_loss import (  # noqa: F401
     npu_dense_lightning_indexer_grad_kl_loss_triton,
     npu_dense_lightning_indexer_softmax_lse_triton,
 )
-from .flash_attention_paged import flash_attention_paged  # noqa: F401
+from .flash_attention_paged import (  # noqa: F401
+    flash_attention_paged,
+    flash_attention_shared_prefix,
+)
 from .paged_cache import (  # noqa: F401
     paged_cache_append,
     paged_cache_compact,
@@ -83,6 +86,7 @@ __all__ = [
     "sparse_lightning_indexer_grad_kl_loss_triton",
     "SparseLightningIndexerGradKLLossTriton",
     "flash_attention_paged",
+    "flash_attention_shared_prefix",
     "rotary_embedding",
     "rotary_table",
     "paged_cache_append",

@@ -121,6 +121,10 @@ class AttnPagedParams(ctypes.Structure):
     ]
 
 
+class AttnSharedParams(ctypes.Structure):
+    _fields_ = [("attn", AttnPagedParams), ("group_starts", _p), ("prefix_lengths", _p), ("groups", _i64)]
+
+
 class RotaryParams(ctypes.Structure):
     _fields_ = [
         ("x", _p), ("out", _p), ("positions", _p), ("table", _p), ("error_flag", _p),
@@ -223,6 +227,10 @@ def lib() -> ctypes.CDLL:
                 l.dsa_attn_paged_workspace_size.restype = _i64
                 l.dsa_attn_paged_shares_keys.argtypes = [_i64] * 2
                 l.dsa_attn_paged_shares_keys.restype = ctypes.c_int
+                l.dsa_attn_shared.argtypes = [ctypes.POINTER(AttnSharedParams), _p]
+                l.dsa_attn_shared.restype = ctypes.c_int
+                l.dsa_attn_shared_workspace_size.argtypes = [_i64] * 5
+                l.dsa_attn_shared_workspace_size.restype = _i64
                 l.dsa_rotary.argtypes = [ctypes.POINTER(RotaryParams), _p]
                 l.dsa_rotary.restype = ctypes.c_int
                 l.dsa_rotary_table.argtypes = [_p, _i64, _i64, ctypes.POINTER(ctypes.c_double),

@@ -45,7 +45,7 @@ struct Args {
 };
 
 // Keys that query row `row` sees.
-__device__ __forceinline__ int row_keys(const Args& a, int row) {
+__device__ __forceinline__ int token_keys(const Args& a, int row) {
   const int b = row / a.s1, s = row - b * a.s1;
   const int ak = a.act_k[b], aq = a.act_q ? a.act_q[b] : a.s1;
   int64_t n = min((int64_t)ak, (int64_t)a.max_blocks * a.page_size);
@@ -53,8 +53,60 @@ __device__ __forceinline__ int row_keys(const Args& a, int row) {
   if (s >= aq || n < 0) n = 0;
   return (int)n;
 }
-template <int kTile, int kCost>
-__device__ __forceinline__ int row_units(const Args& a, int row) {
+__device__ __forceinline__ int row_keys(const Args& a, int row) { return token_keys(a, row); }
+
+// What a call is made of in which rows share keys (attn_shared.cu): its pieces take the place of the
+// rows above.  The first `shared_items` are runs of neighbouring tokens over the keys that they have in
+// common, the others rows (or, packed, the tokens of a batch) over the rest of theirs.
+struct Item {
+  int32_t keys;     // 0: nothing to do
+  int32_t first;    // position of its first key, at the start of a page
+  int32_t table;    // row of the block table
+  int32_t head0;    // its first row of all batch * s1 * n1 rows of queries, and how many
+  int32_t heads;
+  int32_t part;     // whether its result is a part in any case
+  int32_t unused[2];
+};
+struct ItemArgs : Args {
+  const Item* items;      // [rows]
+  const int4* groups;     // [batch]: shared keys (0: none), first item, first token of the row's group
+  int32_t shared_items, per_item;   // tokens of a shared item
+};
+
+__device__ __forceinline__ int row_keys(const ItemArgs& a, int row) { return a.items[row].keys; }
+// Row of the block table, position of the first key, heads, where a row's results go among all
+// rows * n1, whether they are a part in any case.
+__device__ __forceinline__ int row_table(const Args& a, int row) { return row / a.s1; }
+__device__ __forceinline__ int row_table(const ItemArgs& a, int row) { return a.items[row].table; }
+__device__ __forceinline__ int row_first(const Args&, int) { return 0; }
+__device__ __forceinline__ int row_first(const ItemArgs& a, int row) { return a.items[row].first; }
+__device__ __forceinline__ int row_heads(const Args& a, int) { return a.n1; }
+__device__ __forceinline__ int row_heads(const ItemArgs& a, int row) { return a.items[row].heads; }
+__device__ __forceinline__ int64_t row_result(const Args&, int row, int heads) { return (int64_t)row * heads; }
+__device__ __forceinline__ int64_t row_result(const ItemArgs& a, int row, int) { return a.items[row].head0; }
+__device__ __forceinline__ bool row_is_part(const Args& a, int) { return a.diag > 0; }
+__device__ __forceinline__ bool row_is_part(const ItemArgs& a, int row) { return a.items[row].part; }
+// Coordinates of a row's queries in their tensor map.
+struct QueryAt {
+  int head, s, b;
+};
+__device__ __forceinline__ QueryAt row_query(const Args& a, int row) {
+  const int b = row / a.s1;
+  return {0, row - b * a.s1, b};
+}
+__device__ __forceinline__ QueryAt row_query(const ItemArgs& a, int row) { return {a.items[row].head0, 0, 0}; }
+// First of the workspace's places (of a head each) for a row that one CTA takes all of, behind the
+// two slots of each share; an item's rest has as many as it has heads.
+template <int NH>
+__device__ __forceinline__ int64_t own_place(const Args&, int shares, int row) { return ((int64_t)2 * shares + row) * NH; }
+template <int NH>
+__device__ __forceinline__ int64_t own_place(const ItemArgs& a, int shares, int row) {
+  if (row < a.shared_items) return ((int64_t)2 * shares + row) * NH;
+  return ((int64_t)2 * shares + a.shared_items) * NH + a.items[row].head0;
+}
+
+template <int kTile, int kCost, typename A>
+__device__ __forceinline__ int row_units(const A& a, int row) {
   const int tiles = (row_keys(a, row) + kTile - 1) / kTile;
   return tiles > 0 ? tiles + kCost : 0;
 }
@@ -103,8 +155,8 @@ struct Segment {
   int row, first, count, keys, tiles;
 };
 // The next run of `w` (false when the share is done); `w` moves past it.
-template <int kTile, int kCost>
-__device__ __forceinline__ bool next_segment(const Args& a, Work& w, Segment& s) {
+template <int kTile, int kCost, typename A>
+__device__ __forceinline__ bool next_segment(const A& a, Work& w, Segment& s) {
   while (w.left > 0 && w.row < a.rows) {
     s.row = w.row++;
     s.keys = row_keys(a, s.row);
@@ -129,8 +181,8 @@ __device__ __forceinline__ int64_t share_begin(int64_t units, int64_t c, int64_t
 
 // The share of CTA (or pair) `cta` of `ctas_max`.  All threads of the block call it.  The first CTA
 // also writes the rows' prefix for the join.
-template <int kTile, int kCost, int kThreads>
-__device__ __forceinline__ Work share_of(const Args& a, int cta, int ctas_max, bool first_cta, int* tmp,
+template <int kTile, int kCost, int kThreads, typename A>
+__device__ __forceinline__ Work share_of(const A& a, int cta, int ctas_max, bool first_cta, int* tmp,
                                          int32_t* start) {
   Work work{0, 0, 0};
   if (a.rows <= 32) {

@@ -64,7 +64,8 @@ struct Tiles {
   Work w;
   Segment s;
   int i, seg;
-  __device__ __forceinline__ bool next(const Args& a) {
+  template <typename A>
+  __device__ __forceinline__ bool next(const A& a) {
     if (seg >= 0 && i + 1 < s.count) {
       ++i;
       return true;
@@ -75,10 +76,10 @@ struct Tiles {
   }
 };
 
-template <int D, typename T>
+template <int D, typename T, typename A = Args>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     attn_paged_pair_kernel(const __grid_constant__ Maps maps, const __grid_constant__ CUtensorMap map_v,
-                           const Args a) {
+                           const A a) {
   using C = Cfg<D>;
   using E = ElemTraits<T>;
   constexpr bool kBf16 = E::kIsBf16;
@@ -149,11 +150,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   auto page_of = [&](const Segment& sg, const int32_t* table, int tile, bool tell) {
     const int pos = tile * kTile + lane * 8;
     if (lane >= 16 || pos >= sg.keys) return -1;
-    const int id = table[pos / a.page_size];
+    const int id = table[(row_first(a, sg.row) + pos) / a.page_size];
     if (tell && id >= a.num_pages) report_error(a.error_flag, kErrBadIndex);
     return id < a.num_pages ? id : -1;
   };
-  auto table_of = [&](const Segment& sg) { return a.block_table + (int64_t)(sg.row / a.s1) * a.max_blocks; };
+  auto table_of = [&](const Segment& sg) { return a.block_table + (int64_t)row_table(a, sg.row) * a.max_blocks; };
 
   if (warp >= kKeyWarp && warp < kValueWarp) {
     // -------------------------------------------------------------------- K
@@ -169,7 +170,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const int now = t.i == 0 ? page_of(t.s, table, tile, rank == 0 && w == 0) : page;
       if (t.i + 1 < t.s.count) page = page_of(t.s, table, tile + 1, rank == 0 && w == 0);
       const uint32_t mask = __ballot_sync(0xffffffffu, now >= 0);
-      const int in_page = (tile * kTile + lane * 8) % a.page_size;
+      const int in_page = (row_first(a, t.s.row) + tile * kTile + lane * 8) % a.page_size;
       if (g > 0) mbar_wait_hot(k_empty, (g - 1) & 1, a.error_flag, &failed);
       failed = __any_sync(0xffffffffu, failed);
       if (failed) break;
@@ -211,17 +212,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (t.i + 1 < t.s.count) page = page_of(t.s, table, tile + 1, false);
       const uint32_t mask = __ballot_sync(0xffffffffu, now >= 0) & 0xffffu;
       const bool tail = mask != 0xffffu || t.s.keys - tile * kTile < kTile;
-      const int in_page = (tile * kTile + lane * 8) % a.page_size;
+      const int in_page = (row_first(a, t.s.row) + tile * kTile + lane * 8) % a.page_size;
       if (w == 0 && t.i == 0) {
-        const int b = t.s.row / a.s1, s = t.s.row - b * a.s1;
+        const QueryAt at = row_query(a, t.s.row);
         if (t.seg > 0) mbar_wait_hot(q_empty, (t.seg - 1) & 1, a.error_flag, &failed);
         failed = __any_sync(0xffffffffu, failed);
         if (failed) break;
         if (lane == 0) {
           const uint32_t bar = mapa_shared(q_full, 0);
           if (rank == 0) mbar_arrive_expect_tx(q_full, 2 * C::kQBytes);
-          tma_load_5d_pair(base, &maps.q, bar, 0, kHeads * (int)rank, 0, s, b);
-          tma_load_5d_pair(base + kHeads * D * 2, &maps.qr, bar, 0, kHeads * (int)rank, 0, s, b);
+          tma_load_5d_pair(base, &maps.q, bar, 0, at.head + kHeads * (int)rank, 0, at.s, at.b);
+          tma_load_5d_pair(base + kHeads * D * 2, &maps.qr, bar, 0, at.head + kHeads * (int)rank, 0, at.s, at.b);
         }
         ++queries;
         __syncwarp();
@@ -480,16 +481,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const float m = fmaxf(fmaxf(wmax[h], wmax[kHeads + h]), fmaxf(wmax[2 * kHeads + h], wmax[3 * kHeads + h]));
       const bool any = m != -INFINITY;
       const float most = any ? m * c2 : -INFINITY;
-      const bool all = sg.count == sg.tiles, whole = all && a.diag == 0;
-      const int64_t slot = all ? (int64_t)gridDim.x + sg.row : 2 * (blockIdx.x >> 1) + (nseg == 0 ? 0 : 1);
-      const int head = kHeads * (int)rank + h;
+      const bool all = sg.count == sg.tiles, whole = all && !row_is_part(a, sg.row);
+      const int64_t place = all ? own_place<2 * kHeads>(a, gridDim.x >> 1, sg.row)
+                                : (int64_t)(2 * (blockIdx.x >> 1) + (nseg == 0 ? 0 : 1)) * (2 * kHeads);
+      const int head = kHeads * (int)rank + h, heads = row_heads(a, sg.row);
+      const int64_t result = row_result(a, sg.row, heads);
       const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-      if (part == 0 && head < a.n1) {
+      if (part == 0 && head < heads) {
         if (!whole) {
-          a.ws_s[slot * (2 * kHeads) + head] = make_float4(ref - kShift, most, l, m);
+          a.ws_s[place + head] = make_float4(ref - kShift, most, l, m);
         } else if (a.softmax_max) {
-          const int64_t at = (int64_t)sg.row * a.n1 + head;
-          put_stats(a, at, m, ref - kShift, most, l);
+          put_stats(a, result + head, m, ref - kShift, most, l);
         }
       }
       mbar_wait_hot(p_empty, (g - 1) & 1, a.error_flag, &failed);
@@ -500,10 +502,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         uint32_t o[32];
         tmem_ld32(tmem + C::kColsO + wg * kDims + c + lane_addr, o);
         tmem_ld_wait_regs(o);
-        if (head >= a.n1) {
+        if (head >= heads) {
           // a padded head: nothing to write
         } else if (whole) {   // whole 32-byte sectors, as a lane's neighbours write other rows
-          T* out = static_cast<T*>(a.out) + ((int64_t)sg.row * a.n1 + head) * D + dim + c;
+          T* out = static_cast<T*>(a.out) + (result + head) * D + dim + c;
 #pragma unroll
           for (int j = 0; j < 32; j += 16) {
             uint32_t v[8];
@@ -513,7 +515,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             st_global_v8(out + j, v);
           }
         } else {
-          float* out = a.ws_o + (slot * (2 * kHeads) + head) * D + dim + c;
+          float* out = a.ws_o + (place + head) * D + dim + c;
 #pragma unroll
           for (int j = 0; j < 32; j += 8) {
             const uint32_t v[8] = {o[j], o[j + 1], o[j + 2], o[j + 3], o[j + 4], o[j + 5], o[j + 6], o[j + 7]};

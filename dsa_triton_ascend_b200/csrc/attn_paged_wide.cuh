@@ -61,9 +61,9 @@ struct Cfg {
   static_assert(D <= 256 && kStages >= 4 && kRopes >= 2 && kSmem <= kSmemLimit, "a result of 128 heads has to leave room for the scores");
 };
 
-template <int D, typename T>
+template <int D, typename T, typename A = Args>
 __global__ void __launch_bounds__(kThreads, 1)
-    attn_paged_wide_kernel(const __grid_constant__ Maps maps, const Args a) {
+    attn_paged_wide_kernel(const __grid_constant__ Maps maps, const A a) {
   using C = Cfg<D>;
   using E = ElemTraits<T>;
   constexpr bool kBf16 = E::kIsBf16;
@@ -145,18 +145,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool is_rope = lane & 2;
     int sent = 0;   // tiles of latent rows
     while (!failed && next_segment<kTile, kSegmentCost>(a, work, sg)) {
-      const int32_t* table = a.block_table + (int64_t)(sg.row / a.s1) * a.max_blocks;
+      const int32_t* table = a.block_table + (int64_t)row_table(a, sg.row) * a.max_blocks;
+      const int key0 = row_first(a, sg.row);
       auto page_of = [&](int tile) {   // -1: no such page
         const int pos = tile * kTile + grp * 8;
         if (lane >= 4 || pos >= sg.keys) return -1;
-        const int id = table[pos / a.page_size];
+        const int id = table[(key0 + pos) / a.page_size];
         if (id >= a.num_pages && !is_rope) report_error(a.error_flag, kErrBadIndex);
         return id < a.num_pages ? id : -1;
       };
       int page = page_of(sg.first);
       for (int i = 0; i < sg.count; ++i, ++g) {
         const int st = g % C::kStages, rs = g % C::kRopes, tile = sg.first + i;
-        const int now = page, in_page = (tile * kTile + grp * 8) % a.page_size;
+        const int now = page, in_page = (key0 + tile * kTile + grp * 8) % a.page_size;
         if (i + 1 < sg.count) page = page_of(tile + 1);
         const uint32_t mask = __ballot_sync(0xffffffffu, now >= 0) & 3u;
         if (g >= C::kStages) mbar_wait_hot(empty(st), (g / C::kStages - 1) & 1, a.error_flag, &failed);
@@ -196,14 +197,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == kQueryWarp) {
     // -------------------------------------------------------------------- queries
     while (!failed && next_segment<kTile, kSegmentCost>(a, work, sg)) {
-      const int b = sg.row / a.s1, s = sg.row - b * a.s1;
+      const QueryAt at = row_query(a, sg.row);
       if (nseg > 0) mbar_wait_hot(q_empty, (nseg - 1) & 1, a.error_flag, &failed);
       failed = __any_sync(0xffffffffu, failed);
       if (failed) break;
       if (lane == 0) {
         mbar_arrive_expect_tx(q_full, C::kQBytes);
-        tma_load_5d(s_q, &maps.q, q_full, 0, 0, 0, s, b);
-        tma_load_5d(s_q + kHeads * D * 2, &maps.qr, q_full, 0, 0, 0, s, b);
+        tma_load_5d(s_q, &maps.q, q_full, 0, at.head, 0, at.s, at.b);
+        tma_load_5d(s_q + kHeads * D * 2, &maps.qr, q_full, 0, at.head, 0, at.s, at.b);
       }
       __syncwarp();
       ++nseg;
@@ -393,14 +394,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float l = wsum[h] + wsum[kHeads + h], m = fmaxf(wmax[h], wmax[kHeads + h]);
       meet();   // both are read: the next segment may write its own
       const float most = m != -INFINITY ? m * c2 : -INFINITY;
-      const bool all = sg.count == sg.tiles, whole = all && a.diag == 0;
-      const int64_t slot = all ? (int64_t)2 * gridDim.x + sg.row : 2 * blockIdx.x + (nseg == 0 ? 0 : 1);
+      const bool all = sg.count == sg.tiles, whole = all && !row_is_part(a, sg.row);
+      const int64_t place = all ? own_place<kHeads>(a, gridDim.x, sg.row) : (int64_t)(2 * blockIdx.x + (nseg == 0 ? 0 : 1)) * kHeads;
+      const int heads = row_heads(a, sg.row);
+      const int64_t result = row_result(a, sg.row, heads);
       const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-      if (wg == 0 && h < a.n1) {
+      if (wg == 0 && h < heads) {
         if (!whole)
-          a.ws_s[slot * kHeads + h] = make_float4(ref - kShift, most, l, m);
+          a.ws_s[place + h] = make_float4(ref - kShift, most, l, m);
         else if (a.softmax_max)
-          put_stats(a, (int64_t)sg.row * a.n1 + h, m, ref - kShift, most, l);
+          put_stats(a, result + h, m, ref - kShift, most, l);
       }
       mbar_wait_hot(p_empty((g - 1) % kBufs), (g - 1) / kBufs & 1, a.error_flag, &failed);
       tc_fence_after();
@@ -409,10 +412,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t o[32];
         tmem_ld32(o_at + c, o);
         tmem_ld_wait_regs(o);
-        if (h >= a.n1) {
+        if (h >= heads) {
           // a padded head: nothing to write
         } else if (whole) {   // whole 32-byte sectors, as a lane's neighbours write other rows
-          T* out = static_cast<T*>(a.out) + ((int64_t)sg.row * a.n1 + h) * D + wg * kDims + c;
+          T* out = static_cast<T*>(a.out) + (result + h) * D + wg * kDims + c;
 #pragma unroll
           for (int j = 0; j < 32; j += 16) {
             uint32_t v[8];
@@ -422,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             st_global_v8(out + j, v);
           }
         } else {
-          float* out = a.ws_o + (slot * kHeads + h) * D + wg * kDims + c;
+          float* out = a.ws_o + (place + h) * D + wg * kDims + c;
 #pragma unroll
           for (int j = 0; j < 32; j += 8) {
             const uint32_t v[8] = {o[j], o[j + 1], o[j + 2], o[j + 3], o[j + 4], o[j + 5], o[j + 6], o[j + 7]};

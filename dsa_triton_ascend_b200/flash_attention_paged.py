@@ -1,4 +1,5 @@
-"""flash_attention_paged: attention of new tokens over the whole paged latent cache.
+"""flash_attention_paged: attention of new tokens over the whole paged latent cache, and
+flash_attention_shared_prefix: the same for a batch whose rows share their first pages.
 
 The dense counterpart of ``sparse_flash_attention_triton`` with ``layout_kv="PA_BSND"``
 (sparse_flash_attention_triton.py:483-641): every visible key of a sequence is attended, so
@@ -11,7 +12,8 @@ from __future__ import annotations
 import torch
 
 from . import _host as H
-from ._lib import BIND_ATTN, AttnPagedParams, binding, check, lib, remember, report_ptr
+from ._lib import (BIND_ATTN, AttnPagedParams, AttnSharedParams, binding, check, lib, remember,
+                   report_ptr)
 
 _VALID_D = (128, 256, 512)
 _D_ROPE = 64
@@ -93,6 +95,45 @@ def _copied(t: torch.Tensor) -> torch.Tensor:
     return t.clone(memory_format=torch.contiguous_format)
 
 
+def _call(params, p, entry, name, tensors, stats, index, q_fits, qr_fits, stat_shape, ws_bytes):
+    """Fill `p`, the attention's part of `params`, in and call the entry: (results, whether the tables
+    and lengths went in as they were given)."""
+    query, query_rope, key_cache, key_rope_cache, block_table, act_k_given, act_q_given = tensors
+    dev = query.device
+    B, _, S1, _ = stat_shape
+    act_k, act_q = act_k_given, act_q_given
+    if not H.is_i32_vector(act_k, B, index):
+        act_k = H.lens_tensor(act_k, B, p.max_blocks * p.page_size, dev).contiguous()
+    if act_q is not None and not H.is_i32_vector(act_q, B, index):
+        act_q = H.lens_tensor(act_q, B, S1, dev).contiguous()
+    out = torch.empty(query.shape, dtype=query.dtype, device=dev)
+    alloc = torch.empty if stats else torch.zeros
+    smax = alloc(stat_shape, dtype=torch.float32, device=dev)
+    ssum = alloc(stat_shape, dtype=torch.float32, device=dev)
+    if B == 0 or S1 == 0:
+        return (out, smax, ssum), False
+    q = query if q_fits and query.data_ptr() % 16 == 0 else _copied(query)
+    qr = query_rope if qr_fits and query_rope.data_ptr() % 16 == 0 else _copied(query_rope)
+    if q is not query:
+        p.q_batch_stride, p.q_token_stride, p.q_head_stride = q.stride()[:3]
+    if qr is not query_rope:
+        p.qr_batch_stride, p.qr_token_stride, p.qr_head_stride = qr.stride()[:3]
+    kc, krc = key_cache.data_ptr(), key_rope_cache.data_ptr()
+    if (kc | krc) % 16:
+        raise ValueError("key_cache and key_rope_cache need 16-byte aligned bases")
+    bt = block_table.contiguous()
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    p.query, p.query_rope, p.key_cache, p.key_rope_cache = q.data_ptr(), qr.data_ptr(), kc, krc
+    p.block_table, p.act_k, p.out, p.workspace = bt.data_ptr(), act_k.data_ptr(), out.data_ptr(), ws.data_ptr()
+    if act_q is not None:
+        p.act_q = act_q.data_ptr()
+    if stats:
+        p.softmax_max, p.softmax_sum = smax.data_ptr(), ssum.data_ptr()
+    p.error_flag = report_ptr(index)
+    check(entry(params, H.raw_stream(index)), name)
+    return (out, smax, ssum), bt is block_table and act_k is act_k_given and act_q is act_q_given
+
+
 def flash_attention_paged(
     query: torch.Tensor,
     query_rope: torch.Tensor,
@@ -136,40 +177,96 @@ def flash_attention_paged(
     plan = _plan(query, query_rope, key_cache, key_rope_cache, block_table, float(scale_value), sparse_mode,
                  actual_seq_lengths_query is not None)
     template, q_fits, qr_fits, stat_shape, ws_bytes = plan
-    dev = query.device
-    B, _, S1, _ = stat_shape
     p = AttnPagedParams.from_buffer_copy(template)
-    act_k = actual_seq_lengths_key
-    if not H.is_i32_vector(act_k, B, index):
-        act_k = H.lens_tensor(act_k, B, p.max_blocks * p.page_size, dev).contiguous()
-    act_q = actual_seq_lengths_query
-    if act_q is not None and not H.is_i32_vector(act_q, B, index):
-        act_q = H.lens_tensor(act_q, B, S1, dev).contiguous()
-    out = torch.empty(query.shape, dtype=query.dtype, device=dev)
-    alloc = torch.empty if return_softmax_lse else torch.zeros
-    smax = alloc(stat_shape, dtype=torch.float32, device=dev)
-    ssum = alloc(stat_shape, dtype=torch.float32, device=dev)
-    if B == 0 or S1 == 0:
-        return out, smax, ssum
-    q = query if q_fits and query.data_ptr() % 16 == 0 else _copied(query)
-    qr = query_rope if qr_fits and query_rope.data_ptr() % 16 == 0 else _copied(query_rope)
-    if q is not query:
-        p.q_batch_stride, p.q_token_stride, p.q_head_stride = q.stride()[:3]
-    if qr is not query_rope:
-        p.qr_batch_stride, p.qr_token_stride, p.qr_head_stride = qr.stride()[:3]
-    kc, krc = key_cache.data_ptr(), key_rope_cache.data_ptr()
-    if (kc | krc) % 16:
-        raise ValueError("key_cache and key_rope_cache need 16-byte aligned bases")
-    bt = block_table.contiguous()
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-    p.query, p.query_rope, p.key_cache, p.key_rope_cache = q.data_ptr(), qr.data_ptr(), kc, krc
-    p.block_table, p.act_k, p.out, p.workspace = bt.data_ptr(), act_k.data_ptr(), out.data_ptr(), ws.data_ptr()
-    if act_q is not None:
-        p.act_q = act_q.data_ptr()
-    if return_softmax_lse:
-        p.softmax_max, p.softmax_sum = smax.data_ptr(), ssum.data_ptr()
-    p.error_flag = report_ptr(index)
-    check(lib().dsa_attn_paged(p, H.raw_stream(index)), "dsa_attn_paged")
-    if bt is block_table and act_k is actual_seq_lengths_key and act_q is actual_seq_lengths_query:
+    done, as_given = _call(p, p, lib().dsa_attn_paged, "dsa_attn_paged", args[:7], bool(return_softmax_lse), index, *plan[1:])
+    if as_given:
         remember(BIND_ATTN, index, *args, template, bytes((not q_fits, not qr_fits)), ws_bytes)
-    return out, smax, ssum
+    return done
+
+
+def _one_matrix(t: torch.Tensor, strides):
+    """Whether all heads of a [B, S1, N1, D] tensor lie one step apart, across tokens and rows."""
+    b, s, n, d = t.shape
+    step = strides[2] if n > 1 else strides[1] if s > 1 else strides[0] if b > 1 else d
+    return (s == 1 or strides[1] == n * step) and (b == 1 or strides[0] == s * n * step)
+
+
+def _shared_plan(query, query_rope, key_cache, key_rope_cache, block_table, group_starts, prefix_lengths,
+                 scale_value, sparse_mode):
+    """As _plan, for flash_attention_shared_prefix."""
+    template, _, _, stat_shape, _ = _plan(query, query_rope, key_cache, key_rope_cache, block_table, scale_value,
+                                          sparse_mode, True)
+    for t, what in ((group_starts, "group_starts"), (prefix_lengths, "prefix_lengths")):
+        if not torch.is_tensor(t) or t.dtype != torch.int32 or t.dim() != 1:
+            raise ValueError(f"{what} must be an int32 tensor of 1 dim")
+        H.require_cuda(t)
+        if t.device != query.device:
+            raise ValueError("all tensors must be on one device")
+    groups = prefix_lengths.numel()
+    if group_starts.numel() != groups + 1:
+        raise ValueError(f"group_starts must have {groups + 1} entries (one more than prefix_lengths), "
+                         f"got {group_starts.numel()}")
+    p = AttnSharedParams()
+    p.attn = AttnPagedParams.from_buffer_copy(template)
+    p.groups = groups
+    B, S1, N1, D = query.shape
+    # pieces of a prefix are runs of heads of neighbouring tokens; queries that lie otherwise are copied
+    fits = []
+    for t, name, width in ((query, "q", D), (query_rope, "qr", _D_ROPE)):
+        st = _tma_strides(t)
+        fits.append(st is not None and (N1 > 64 or _one_matrix(t, st)))
+        if not fits[-1]:
+            p_strides = (S1 * N1 * width, N1 * width, width)
+            for dim, v in zip(("batch", "token", "head"), p_strides):
+                setattr(p.attn, f"{name}_{dim}_stride", v)
+    p.attn.workspace_bytes = lib().dsa_attn_shared_workspace_size(B, S1, N1, D, groups)
+    return bytes(p), fits[0], fits[1], stat_shape, max(p.attn.workspace_bytes, 16)
+
+
+def flash_attention_shared_prefix(
+    query: torch.Tensor,
+    query_rope: torch.Tensor,
+    key_cache: torch.Tensor,
+    key_rope_cache: torch.Tensor,
+    block_table: torch.Tensor,
+    group_starts: torch.Tensor,
+    prefix_lengths: torch.Tensor,
+    actual_seq_lengths_key=None,
+    scale_value: float = 1.0,
+    actual_seq_lengths_query=None,
+    sparse_mode: int = 0,
+    return_softmax_lse: bool = False,
+):
+    """:func:`flash_attention_paged` for a batch whose rows share their first pages in groups (forks
+    of a sequence, requests with one system prompt): the keys that a group shares are read and
+    multiplied once for as many of its tokens as 64 or 128 heads hold.
+
+    ``group_starts`` [G + 1] int32, not decreasing, within 0 .. B: group g is the rows
+    ``group_starts[g]`` .. ``group_starts[g + 1]`` - 1.  ``prefix_lengths`` [G] int32: the first
+    tokens that all rows of the group have in common, for which their rows of ``block_table`` name
+    the same pages (those of the group's first row with keys are read); whole pages are shared, at
+    most as many as every row of the group with keys sees.  Rows outside all groups share
+    nothing.  ``paged_batch_plan`` makes both.  Starts that divide no batch of B rows are reported by
+    ``check_device_errors``, and nothing is shared.
+
+    The other arguments and the results are those of :func:`flash_attention_paged`.  With more than
+    64 heads a token fills a piece by itself and nothing is gained by sharing.  G should be near the
+    number of groups: the pieces are of 128 heads where B * S1 * N1 / G exceeds 64.
+    """
+    args = (query, query_rope, key_cache, key_rope_cache, block_table, group_starts, prefix_lengths,
+            actual_seq_lengths_key, actual_seq_lengths_query, float(scale_value), sparse_mode, bool(return_softmax_lse))
+    index = query.get_device()
+    if index >= 0 and H.current_device() != index:
+        with torch.cuda.device(index):
+            return flash_attention_shared_prefix(query, query_rope, key_cache, key_rope_cache, block_table,
+                                                 group_starts, prefix_lengths, actual_seq_lengths_key, scale_value,
+                                                 actual_seq_lengths_query, sparse_mode, return_softmax_lse)
+    plan = _shared_plan(query, query_rope, key_cache, key_rope_cache, block_table, group_starts, prefix_lengths,
+                        float(scale_value), sparse_mode)
+    template, q_fits, qr_fits, _, ws_bytes = plan
+    p = AttnSharedParams.from_buffer_copy(template)
+    starts, prefixes = group_starts.contiguous(), prefix_lengths.contiguous()
+    p.group_starts, p.prefix_lengths = starts.data_ptr(), prefixes.data_ptr()
+    done, as_given = _call(p, p.attn, lib().dsa_attn_shared, "dsa_attn_shared", (*args[:5], *args[7:9]),
+                           bool(return_softmax_lse), index, *plan[1:])
+    return done

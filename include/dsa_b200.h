@@ -454,6 +454,29 @@ int64_t dsa_attn_paged_workspace_size(int64_t batch, int64_t s1, int64_t n1, int
 int dsa_attn_paged_shares_keys(int64_t s1, int64_t n1);
 
 /*
+ * The same attention for a batch whose rows share their first pages in groups, whose keys are
+ * read and multiplied once for several tokens of a group.  No counterpart in the reference.
+ *   attn: as for dsa_attn_paged.  group_starts [groups + 1] int32, not decreasing, within
+ *   0 .. batch: group g is the batch rows group_starts[g] .. group_starts[g + 1] - 1, whose first
+ *   prefix_lengths[g] tokens are the same: their block_table rows name the same pages there, of
+ *   which the whole ones that all rows with keys see are shared.  Rows outside all groups share nothing.
+ * Group starts that are no such division are reported in error_flag, and nothing is shared.
+ * n1 * (tokens that share a row's keys) heads of more than 64, or of a group all told, are taken 128
+ * at a time; where a token has more than 64 heads nothing is shared.  Where something can be
+ * (n1 <= 64), all heads of query and of query_rope lie one step apart, across tokens and rows.
+ * Workspace: dsa_attn_shared_workspace_size() bytes.
+ */
+typedef struct DsaAttnSharedParams {
+  DsaAttnPagedParams attn;
+  const int32_t* group_starts;
+  const int32_t* prefix_lengths;
+  int64_t groups;
+} DsaAttnSharedParams;
+
+int dsa_attn_shared(const DsaAttnSharedParams* params, void* stream);
+int64_t dsa_attn_shared_workspace_size(int64_t batch, int64_t s1, int64_t n1, int64_t d, int64_t groups);
+
+/*
  * Rotary positions.  No counterpart in the reference, which takes rotated tensors.
  *   x, out [batch][s][heads][head_dim] (bf16 / fp16 / fp32, last dim contiguous, strides in
  *   elements; out may be x), positions [batch][s] int32, table [max_positions][dim] fp32
