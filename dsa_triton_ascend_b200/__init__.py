@@ -15,7 +15,10 @@ FP8 indexer), the dense indexer KL loss of
 :mod:`.dense_indexer_loss` (``dense_loss_backward_triton`` and its softmax-LSE helper) and
 the autograd functions of :mod:`.autograd`.  For serving from a paged cache:
 :func:`flash_attention_paged` (attention of new tokens over every cached key),
-:func:`rotary_embedding` with :func:`rotary_table`, :func:`paged_cache_append`, and the upkeep
+:func:`flash_attention_shared_prefix` (the same for rows that share their first pages),
+:func:`rotary_embedding` and :func:`rotary_embedding_axes` (positions on several axes) with
+:func:`rotary_table`, :func:`paged_cache_append`, :func:`paged_batch_plan` (a step's tables and slots from
+its requests' lengths) with :func:`paged_cache_store`, and the upkeep
 of the pages, :func:`paged_cache_extend`, :func:`paged_cache_fork`, :func:`paged_cache_free`,
 :func:`paged_cache_compact` and :func:`paged_cache_copy`.
 """
@@ -56,21 +59,27 @@ from .flash_attention_paged import (  # noqa: F401
     flash_attention_shared_prefix,
 )
 from .paged_cache import (  # noqa: F401
+    PagedBatchPlan,
+    paged_batch_plan,
     paged_cache_append,
     paged_cache_compact,
     paged_cache_copy,
     paged_cache_extend,
     paged_cache_fork,
     paged_cache_free,
+    paged_cache_store,
 )
 from .rotary_embedding import (  # noqa: F401
+    rotary_axes,
     rotary_embedding,
+    rotary_embedding_axes,
     rotary_frequencies,
     rotary_table,
 )
 from .streaming import bind_host_to_device, host_outputs, sfa_fwd_bwd_from_host  # noqa: F401
 from .autograd import (  # noqa: F401
     IndexerKLLossFunction,
+    RotaryEmbeddingAxesFunction,
     RotaryEmbeddingFunction,
     SparseAttentionWithIndexer,
     SparseFlashAttentionFunction,
@@ -88,12 +97,17 @@ __all__ = [
     "flash_attention_paged",
     "flash_attention_shared_prefix",
     "rotary_embedding",
+    "rotary_embedding_axes",
+    "rotary_axes",
     "rotary_table",
+    "PagedBatchPlan",
+    "paged_batch_plan",
     "paged_cache_append",
     "paged_cache_compact",
     "paged_cache_copy",
     "paged_cache_extend",
     "paged_cache_fork",
     "paged_cache_free",
+    "paged_cache_store",
     "check_device_errors",
 ]

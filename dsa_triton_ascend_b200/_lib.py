@@ -136,6 +136,11 @@ class RotaryParams(ctypes.Structure):
     ]
 
 
+class RotaryAxesParams(ctypes.Structure):
+    _fields_ = [("rotary", RotaryParams), ("axes", ctypes.c_int32), ("axis_of", ctypes.c_uint8 * 128)]
+
+
+ROTARY_MAX_AXES = 4                                     # DSA_ROTARY_MAX_AXES
 ROTARY_CODES = {None: 0, "interleaved": 1, "half": 2}   # DSA_ROTARY_*
 APPEND_MAX_ENTRIES = 4                                  # DSA_APPEND_MAX_ENTRIES
 PAGES_COPY, PAGES_FORK, PAGES_EXTEND, PAGES_FREE, PAGES_COMPACT = range(5)   # DSA_PAGES_*
@@ -170,6 +175,24 @@ class PagesParams(ctypes.Structure):
         ("workspace_bytes", _i64), ("n", _i64), ("slots", _i64), ("max_blocks", _i64),
         ("num_pages", _i64), ("page_size", _i64), ("num_caches", ctypes.c_int32),
         ("op", ctypes.c_int32),
+    ]
+
+
+class BatchPlanParams(ctypes.Structure):
+    _fields_ = [
+        ("block_table", _p), ("seq_lengths", _p), ("rows", _p), ("counts", _p), ("block_table_out", _p),
+        ("key_lengths", _p), ("query_ends", _p), ("token_rows", _p), ("positions", _p),
+        ("slot_map", _p), ("group_starts", _p), ("prefix_lengths", _p), ("error_flag", _p),
+        ("workspace", _p), ("workspace_bytes", _i64), ("batch", _i64), ("slots", _i64),
+        ("max_blocks", _i64), ("page_size", _i64), ("num_tokens", _i64), ("max_groups", _i64),
+        ("min_prefix", _i64),
+    ]
+
+
+class CacheStoreParams(ctypes.Structure):
+    _fields_ = [
+        ("rows", CacheRows * APPEND_MAX_ENTRIES), ("slots", _p), ("error_flag", _p), ("tokens", _i64),
+        ("num_pages", _i64), ("page_size", _i64), ("entries", ctypes.c_int32),
     ]
 
 
@@ -233,6 +256,8 @@ def lib() -> ctypes.CDLL:
                 l.dsa_attn_shared_workspace_size.restype = _i64
                 l.dsa_rotary.argtypes = [ctypes.POINTER(RotaryParams), _p]
                 l.dsa_rotary.restype = ctypes.c_int
+                l.dsa_rotary_axes.argtypes = [ctypes.POINTER(RotaryAxesParams), _p]
+                l.dsa_rotary_axes.restype = ctypes.c_int
                 l.dsa_rotary_table.argtypes = [_p, _i64, _i64, ctypes.POINTER(ctypes.c_double),
                                                ctypes.c_double, _p]
                 l.dsa_rotary_table.restype = ctypes.c_int
@@ -242,6 +267,12 @@ def lib() -> ctypes.CDLL:
                 l.dsa_pages.restype = ctypes.c_int
                 l.dsa_pages_workspace_size.argtypes = [ctypes.c_int32, _i64, _i64, _i64]
                 l.dsa_pages_workspace_size.restype = _i64
+                l.dsa_batch_plan.argtypes = [ctypes.POINTER(BatchPlanParams), _p]
+                l.dsa_batch_plan.restype = ctypes.c_int
+                l.dsa_batch_plan_workspace_size.argtypes = [_i64]
+                l.dsa_batch_plan_workspace_size.restype = _i64
+                l.dsa_cache_store.argtypes = [ctypes.POINTER(CacheStoreParams), _p]
+                l.dsa_cache_store.restype = ctypes.c_int
                 _lib = l
     return _lib
 

@@ -24,7 +24,7 @@ import torch
 from . import _host as H
 
 from .lightning_indexer import lightning_indexer_triton
-from .rotary_embedding import rotary_embedding
+from .rotary_embedding import rotary_embedding, rotary_embedding_axes
 from .sparse_flash_attention import sparse_flash_attention_triton
 from .sparse_flash_attention_grad import sparse_flash_attention_grad_merged
 from .sparse_lightning_indexer_grad_kl_loss import sparse_lightning_indexer_grad_kl_loss_triton
@@ -189,3 +189,21 @@ class RotaryEmbeddingFunction(torch.autograd.Function):
         layout, offset, inverse = ctx.cfg
         turn = RotaryEmbeddingFunction.apply if d_out.requires_grad else rotary_embedding
         return turn(d_out, table, positions, layout, offset, not inverse), None, None, None, None, None
+
+
+class RotaryEmbeddingAxesFunction(torch.autograd.Function):
+    """out = rotary_embedding_axes(x, table, positions, sections, layout, order, offset, inverse); the
+    gradient of ``x`` turns the other way, as for :class:`RotaryEmbeddingFunction`."""
+
+    @staticmethod
+    def forward(ctx, x, table, positions, sections, layout="interleaved", order="blocks", offset=0, inverse=False):
+        ctx.save_for_backward(table, positions)
+        ctx.cfg = (sections, layout, order, offset, inverse)
+        return rotary_embedding_axes(x, table, positions, *ctx.cfg)
+
+    @staticmethod
+    def backward(ctx, d_out):
+        table, positions = ctx.saved_tensors
+        sections, layout, order, offset, inverse = ctx.cfg
+        turn = RotaryEmbeddingAxesFunction.apply if d_out.requires_grad else rotary_embedding_axes
+        return (turn(d_out, table, positions, sections, layout, order, offset, not inverse), *[None] * 7)

@@ -18,7 +18,7 @@ CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libdsa_b200.so")
 BINDING = os.path.join(PKG, "_binding" + sysconfig.get_config_var("EXT_SUFFIX"))
 SOURCES = ["capi.cu", "sfa_fwd.cu", "sfa_bwd.cu", "li.cu", "sli.cu", "dense.cu", "attn_paged.cu",
-           "attn_shared.cu", "rotary.cu", "page_cache.cu"]
+           "attn_shared.cu", "rotary.cu", "page_cache.cu", "batch_plan.cu"]
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-lineinfo",
          "-Xcompiler", "-fPIC", "-shared", "--expt-relaxed-constexpr"]
 

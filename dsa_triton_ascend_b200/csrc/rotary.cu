@@ -36,10 +36,75 @@ struct Args {
   float sign;
 };
 
+// Positions of several axes: each pair turns by the position of its own axis.
+constexpr int kMaxAxes = DSA_ROTARY_MAX_AXES;
+struct AxesArgs : Args {
+  int64_t axis_stride;                  // positions of an axis
+  uint64_t codes[2 * kMaxPairs / 64];   // the axis of each pair, in two bits
+  int32_t axes;
+};
+
+// Where a token's angles are: a row of the table, or one for each axis.
+struct TableRow {
+  const float* row;
+  bool known;
+  __device__ __forceinline__ TableRow(const Args& a, int64_t token) {
+    const int32_t pos = a.positions[token];
+    known = pos >= 0 && pos < a.max_positions;
+    row = a.table + (int64_t)(known ? pos : 0) * a.dim;
+  }
+  // cosines and sines of N neighbouring pairs from `pair` (a multiple of N) on
+  template <int N>
+  __device__ __forceinline__ void angles(const Args& a, int pair, float sign, float (&cs)[N], float (&sn)[N]) const {
+    load_angles<N>(row, a.dim / 2, pair, sign, cs, sn);
+  }
+  __device__ __forceinline__ const float* of(const Args&, int) const { return row; }
+};
+struct TableRows {
+  const float* rows[kMaxAxes];
+  bool known;
+  __device__ __forceinline__ TableRows(const AxesArgs& a, int64_t token) {
+    int32_t pos[kMaxAxes];
+#pragma unroll
+    for (int i = 0; i < kMaxAxes; ++i) pos[i] = i < a.axes ? a.positions[i * a.axis_stride + token] : 0;
+    known = true;
+#pragma unroll
+    for (int i = 0; i < kMaxAxes; ++i) {
+      const bool inside = pos[i] >= 0 && pos[i] < a.max_positions;
+      known = known && inside;
+      rows[i] = a.table + (int64_t)(inside ? pos[i] : 0) * a.dim;
+    }
+  }
+  __device__ __forceinline__ const float* at(uint32_t axis) const {
+    const float *lo = axis & 1 ? rows[1] : rows[0], *hi = axis & 1 ? rows[3] : rows[2];
+    return axis & 2 ? hi : lo;
+  }
+  __device__ __forceinline__ const float* of(const AxesArgs& a, int pair) const {
+    return at((uint32_t)(a.codes[pair >> 5] >> (2 * (pair & 31))) & 3u);
+  }
+  template <int N>
+  __device__ __forceinline__ void angles(const AxesArgs& a, int pair, float sign, float (&cs)[N], float (&sn)[N]) const {
+    const uint32_t bits = (uint32_t)(a.codes[pair >> 5] >> (2 * (pair & 31))) & ((1u << 2 * N) - 1);
+    const int half = a.dim / 2;
+    if (bits == (bits & 3u) * (0x5555u & ((1u << 2 * N) - 1))) {   // one axis, as a rule
+      load_angles<N>(at(bits & 3u), half, pair, sign, cs, sn);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float* row = at(bits >> 2 * i & 3u);
+      cs[i] = row[pair + i];
+      sn[i] = sign * row[half + pair + i];
+    }
+  }
+};
+__device__ __forceinline__ TableRow rows_of(const Args& a, int64_t token) { return TableRow(a, token); }
+__device__ __forceinline__ TableRows rows_of(const AxesArgs& a, int64_t token) { return TableRows(a, token); }
+
 enum { kInterleaved, kHalfShuffle, kHalfBoth };
 
-template <typename T, int kMode>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const Args a) {
+template <typename T, int kMode, typename A>
+__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ A a) {
   constexpr int kN = Vec<T>::kN;
   const uint32_t item = blockIdx.x * kThreads + threadIdx.x;
   // (the shuffle needs whole warps: lanes past the end repeat the last item and store nothing)
@@ -59,11 +124,10 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const Args a) {
   }
   const T* x = static_cast<const T*>(a.x) + b * a.x_batch + s * a.x_token;
   T* out = static_cast<T*>(a.out) + b * a.o_batch + s * a.o_token;
-  const int32_t pos = a.positions[token];
-  const bool known = pos >= 0 && pos < a.max_positions;
+  const auto rows = rows_of(a, token);
+  const bool known = rows.known;
   if (!known && u == 0 && h0 == 0) report_error(a.error_flag, kErrBadIndex);
   const int half = a.dim / 2;
-  const float* row = a.table + (int64_t)(known ? pos : 0) * a.dim;
   const uint4 zero = make_uint4(0, 0, 0, 0);
   auto head = [&](int j) { return (int)(h0 + j * a.head_steps.d); };
 
@@ -81,7 +145,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const Args a) {
       if (pair) hi[j] = __ldcs(reinterpret_cast<const uint4*>(x + head(j) * a.x_head + at + half));
     }
     float cs[kN], sn[kN];
-    if (pair) load_angles<kN>(row, half, (int)u * kN, a.sign, cs, sn);
+    if (pair) rows.template angles<kN>(a, (int)u * kN, a.sign, cs, sn);
 #pragma unroll
     for (int j = 0; j < kHeads; ++j) {
       if (head(j) >= a.heads) continue;
@@ -102,7 +166,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const Args a) {
     if (head(j) < a.heads) v[j] = __ldcs(reinterpret_cast<const uint4*>(x + head(j) * a.x_head + at));
   if constexpr (kMode == kInterleaved) {
     float cs[kN / 2], sn[kN / 2];
-    if (turned) load_angles<kN / 2>(row, half, in / 2, a.sign, cs, sn);
+    if (turned) rows.template angles<kN / 2>(a, in / 2, a.sign, cs, sn);
 #pragma unroll
     for (int j = 0; j < kHeads; ++j) {
       if (head(j) >= a.heads) continue;
@@ -113,7 +177,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const Args a) {
     const bool second = in >= half;
     const int lane = threadIdx.x & 31, partner = turned ? (second ? lane - half / kN : lane + half / kN) : lane;
     float cs[kN], sn[kN];
-    if (turned) load_angles<kN>(row, half, second ? in - half : in, second ? a.sign : -a.sign, cs, sn);
+    if (turned) rows.template angles<kN>(a, second ? in - half : in, second ? a.sign : -a.sign, cs, sn);
 #pragma unroll
     for (int j = 0; j < kHeads; ++j) {
       // a warp's lanes are whole heads of up to 32 head steps, so all of a head's lanes have it
@@ -130,8 +194,8 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const Args a) {
 }
 
 // Any strides, offsets and even widths: one pair or one copied value per thread.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) rotary_any_kernel(const Args a) {
+template <typename T, typename A>
+__global__ void __launch_bounds__(kThreads) rotary_any_kernel(const __grid_constant__ A a) {
   const uint32_t item = blockIdx.x * kThreads + threadIdx.x;
   if (item >= a.items) return;
   const uint32_t rest = a.units.div(item), u = item - rest * a.units.d;
@@ -139,8 +203,8 @@ __global__ void __launch_bounds__(kThreads) rotary_any_kernel(const Args a) {
   const int64_t token = a.token0 + tok, b = token / a.s.d, s = token - b * a.s.d;
   const T* x = static_cast<const T*>(a.x) + b * a.x_batch + s * a.x_token + h * a.x_head;
   T* out = static_cast<T*>(a.out) + b * a.o_batch + s * a.o_token + h * a.o_head;
-  const int32_t pos = a.positions[token];
-  const bool known = pos >= 0 && pos < a.max_positions;
+  const auto rows = rows_of(a, token);
+  const bool known = rows.known;
   if (!known && u == 0 && h == 0) report_error(a.error_flag, kErrBadIndex);
   const int half = a.dim / 2;
   auto get = [](const T& v) {
@@ -152,7 +216,7 @@ __global__ void __launch_bounds__(kThreads) rotary_any_kernel(const Args a) {
     else return ElemTraits<T>::from_f(v);
   };
   if ((int)u < half) {
-    const float* row = a.table + (int64_t)(known ? pos : 0) * a.dim;
+    const float* row = rows.of(a, (int)u);
     const int ia = a.offset + (a.half_layout ? (int)u : 2 * (int)u);
     const int ib = ia + (a.half_layout ? half : 1);
     float va = get(x[ia]), vb = get(x[ib]);
@@ -186,10 +250,9 @@ __global__ void __launch_bounds__(kThreads) rotary_table_kernel(const __grid_con
   }
 }
 
-template <typename T>
-int launch(const DsaRotaryParams* p, cudaStream_t stream) {
+template <typename T, typename A>
+int launch(const DsaRotaryParams* p, A a, cudaStream_t stream) {
   constexpr int kN = Vec<T>::kN;
-  Args a;
   a.x = p->x;
   a.out = p->out;
   a.positions = p->positions;
@@ -210,8 +273,8 @@ int launch(const DsaRotaryParams* p, cudaStream_t stream) {
              reinterpret_cast<uintptr_t>(p->x) % 16 == 0 &&
              reinterpret_cast<uintptr_t>(p->out) % 16 == 0 &&
              reinterpret_cast<uintptr_t>(p->table) % 16 == 0 && p->dim % 8 == 0;
-  for (int64_t st : {a.x_batch, a.x_token, a.x_head, a.o_batch, a.o_token, a.o_head})
-    vec = vec && st % kN == 0;
+  const int64_t strides[6] = {a.x_batch, a.x_token, a.x_head, a.o_batch, a.o_token, a.o_head};
+  for (int64_t st : strides) vec = vec && st % kN == 0;
   uint32_t units, steps;
   // a warp holds whole heads where a head's pieces divide it
   const bool shuffle = vec && p->half_layout && 32 % (p->head_dim / kN) == 0;
@@ -232,10 +295,10 @@ int launch(const DsaRotaryParams* p, cudaStream_t stream) {
     a.token0 = t0;
     a.items = (uint32_t)(n * per_token);
     const unsigned grid = (unsigned)((a.items + kThreads - 1) / kThreads);
-    if (!vec) rotary_any_kernel<T><<<grid, kThreads, 0, stream>>>(a);
-    else if (!p->half_layout) rotary_kernel<T, kInterleaved><<<grid, kThreads, 0, stream>>>(a);
-    else if (shuffle) rotary_kernel<T, kHalfShuffle><<<grid, kThreads, 0, stream>>>(a);
-    else rotary_kernel<T, kHalfBoth><<<grid, kThreads, 0, stream>>>(a);
+    if (!vec) rotary_any_kernel<T, A><<<grid, kThreads, 0, stream>>>(a);
+    else if (!p->half_layout) rotary_kernel<T, kInterleaved, A><<<grid, kThreads, 0, stream>>>(a);
+    else if (shuffle) rotary_kernel<T, kHalfShuffle, A><<<grid, kThreads, 0, stream>>>(a);
+    else rotary_kernel<T, kHalfBoth, A><<<grid, kThreads, 0, stream>>>(a);
     if (cudaGetLastError() != cudaSuccess) return DSA_ERR_CUDA;
   }
   return DSA_OK;
@@ -244,21 +307,51 @@ int launch(const DsaRotaryParams* p, cudaStream_t stream) {
 }  // namespace rotary
 }  // namespace dsa
 
-extern "C" int dsa_rotary(const DsaRotaryParams* p, void* stream_) {
+namespace dsa {
+namespace rotary {
+
+// The checks of a call; nothing is launched for one without values.
+bool valid_params(const DsaRotaryParams* p) {
+  constexpr int64_t kMax = 0x7fffffff;
+  return p->x && p->out && p->positions && p->table && p->dim >= 2 && p->dim % 2 == 0 && p->dim <= 2 * kMaxPairs &&
+         p->offset >= 0 && p->head_dim <= (1 << 20) && p->head_dim >= p->dim && p->offset <= p->head_dim - p->dim &&
+         p->max_positions >= 1 && p->max_positions <= kMax && p->heads <= (1 << 20) && p->s <= kMax && p->batch <= kMax;
+}
+
+template <typename A>
+int launch_type(const DsaRotaryParams* p, const A& a, cudaStream_t stream) {
+  if (p->dtype == DSA_DTYPE_BF16) return launch<__nv_bfloat16>(p, a, stream);
+  if (p->dtype == DSA_DTYPE_FP16) return launch<__half>(p, a, stream);
+  if (p->dtype == DSA_DTYPE_FP32) return launch<float>(p, a, stream);
+  return DSA_ERR_INVALID_ARG;
+}
+
+}  // namespace rotary
+}  // namespace dsa
+
+extern "C" int dsa_rotary(const DsaRotaryParams* p, void* stream) {
   using namespace dsa::rotary;
-  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   if (!p || p->batch < 0 || p->s < 0 || p->heads < 0) return DSA_ERR_INVALID_ARG;
   if (p->batch == 0 || p->s == 0 || p->heads == 0) return DSA_OK;
-  constexpr int64_t kMax = 0x7fffffff;
-  if (!p->x || !p->out || !p->positions || !p->table || p->dim < 2 || p->dim % 2 ||
-      p->dim > 2 * kMaxPairs || p->offset < 0 || p->head_dim > (1 << 20) ||
-      p->head_dim < p->dim || p->offset > p->head_dim - p->dim || p->max_positions < 1 || p->max_positions > kMax ||
-      p->heads > (1 << 20) || p->s > kMax || p->batch > kMax)
-    return DSA_ERR_INVALID_ARG;
-  if (p->dtype == DSA_DTYPE_BF16) return launch<__nv_bfloat16>(p, stream);
-  if (p->dtype == DSA_DTYPE_FP16) return launch<__half>(p, stream);
-  if (p->dtype == DSA_DTYPE_FP32) return launch<float>(p, stream);
-  return DSA_ERR_INVALID_ARG;
+  if (!valid_params(p)) return DSA_ERR_INVALID_ARG;
+  return launch_type(p, Args{}, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int dsa_rotary_axes(const DsaRotaryAxesParams* ap, void* stream) {
+  using namespace dsa::rotary;
+  if (!ap) return DSA_ERR_INVALID_ARG;
+  const DsaRotaryParams* p = &ap->rotary;
+  if (p->batch < 0 || p->s < 0 || p->heads < 0) return DSA_ERR_INVALID_ARG;
+  if (p->batch == 0 || p->s == 0 || p->heads == 0) return DSA_OK;
+  if (!valid_params(p) || ap->axes < 1 || ap->axes > kMaxAxes) return DSA_ERR_INVALID_ARG;
+  AxesArgs a = {};
+  a.axes = ap->axes;
+  a.axis_stride = p->batch * p->s;
+  for (int i = 0; i < p->dim / 2; ++i) {
+    if (ap->axis_of[i] >= ap->axes) return DSA_ERR_INVALID_ARG;
+    a.codes[i / 32] |= (uint64_t)ap->axis_of[i] << (2 * (i % 32));
+  }
+  return launch_type(p, a, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int dsa_rotary_table(float* table, int64_t max_positions, int64_t dim,

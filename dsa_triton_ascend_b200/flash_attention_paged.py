@@ -194,14 +194,14 @@ def _one_matrix(t: torch.Tensor, strides):
 def _shared_plan(query, query_rope, key_cache, key_rope_cache, block_table, group_starts, prefix_lengths,
                  scale_value, sparse_mode):
     """As _plan, for flash_attention_shared_prefix."""
-    template, _, _, stat_shape, _ = _plan(query, query_rope, key_cache, key_rope_cache, block_table, scale_value,
-                                          sparse_mode, True)
     for t, what in ((group_starts, "group_starts"), (prefix_lengths, "prefix_lengths")):
         if not torch.is_tensor(t) or t.dtype != torch.int32 or t.dim() != 1:
             raise ValueError(f"{what} must be an int32 tensor of 1 dim")
-        H.require_cuda(t)
-        if t.device != query.device:
-            raise ValueError("all tensors must be on one device")
+    template, _, _, stat_shape, _ = _plan(query, query_rope, key_cache, key_rope_cache, block_table, scale_value,
+                                          sparse_mode, True)
+    H.require_cuda(group_starts, prefix_lengths)
+    if group_starts.device != query.device or prefix_lengths.device != query.device:
+        raise ValueError("all tensors must be on one device")
     groups = prefix_lengths.numel()
     if group_starts.numel() != groups + 1:
         raise ValueError(f"group_starts must have {groups + 1} entries (one more than prefix_lengths), "

@@ -1,4 +1,5 @@
-"""The pages of a latent cache: append, extend, fork, free, compact and copy.
+"""The pages of a latent cache: append, store, extend, fork, free, compact and copy, and the plan of
+a step over them.
 
 A pool is one or more caches [num_pages, page_size, ...] that share their page ids (latent,
 rotary and index keys; the layers of a model), and int32 state on the device:
@@ -17,10 +18,12 @@ whose paged layout takes the table as given (sparse_flash_attention_triton.py:39
 """
 from __future__ import annotations
 
+from typing import NamedTuple
+
 import torch
 
 from . import _host as H
-from ._lib import (APPEND_MAX_ENTRIES, BIND_APPEND, BIND_UPKEEP, DSA_DTYPE_BF16, DSA_DTYPE_FP16, DSA_DTYPE_FP32, PAGES_COMPACT, PAGES_COPY,
+from ._lib import (APPEND_MAX_ENTRIES, BIND_APPEND, BIND_UPKEEP, BatchPlanParams, CacheStoreParams, DSA_DTYPE_BF16, DSA_DTYPE_FP16, DSA_DTYPE_FP32, PAGES_COMPACT, PAGES_COPY,
                    PAGES_EXTEND, PAGES_FORK, PAGES_FREE, ROTARY_CODES, CacheAppendParams, PageCache,
                    PagesParams, binding, check, lib, ptr, remember, report_ptr)
 
@@ -325,3 +328,148 @@ def paged_cache_compact(caches, block_table, ref_counts):
     new (block_table, ref_counts)."""
     out = _upkeep(PAGES_COMPACT, list(caches), block_table, None, ref_counts)
     return out[0], out[2]
+
+
+def _store_plan(tokens, caches, slot_map):
+    """Check the arguments and fill in what their shapes decide: (parameters, which tokens have to be
+    copied first)."""
+    if not 1 <= len(tokens) <= APPEND_MAX_ENTRIES or len(tokens) != len(caches):
+        raise ValueError(f"tokens and caches must be lists of equal length, 1..{APPEND_MAX_ENTRIES}")
+    if not torch.is_tensor(slot_map) or slot_map.dtype not in (torch.int64, torch.int32) or slot_map.dim() != 1:
+        raise ValueError("slot_map must be an int64 or int32 tensor of 1 dim")
+    H.require_cuda(*tokens, *caches, slot_map)
+    dev, T = caches[0].device, slot_map.numel()
+    if slot_map.device != dev:
+        raise ValueError("all tensors must be on one device")
+    p = CacheStoreParams()
+    p.num_pages, p.page_size = _check_caches(caches, dev)
+    p.tokens, p.entries = T, len(tokens)
+    copy = []
+    for i, (t, c) in enumerate(zip(tokens, caches)):
+        if t.dim() != 3 or c.dim() != 4 or c.shape[2] != 1 or tuple(t.shape) != (T, 1, c.shape[3]):
+            raise ValueError(f"tokens {i} must be {(T, 1, c.shape[-1])}, got {tuple(t.shape)}")
+        if t.dtype != c.dtype or t.device != dev:
+            raise ValueError(f"tokens {i} must have its cache's dtype and device")
+        row, size = _row_bytes(c, 2, f"cache {i}"), c.element_size()
+        e = p.rows[i]
+        e.page_stride, e.row_stride = _page_strides(c, row, f"cache {i}")
+        e.width_bytes = row
+        copy.append(c.shape[3] > 1 and t.stride(2) != 1 or T > 1 and t.stride(0) * size % 16 != 0)
+        e.src_token_stride = row if copy[-1] or T == 1 else t.stride(0) * size
+    return bytes(p), copy
+
+
+def paged_cache_store(tokens, caches, slot_map):
+    """Write packed tokens to their slots, in up to four caches at once; returns ``caches``.
+
+    ``tokens[i]`` [T, 1, width] goes into ``caches[i]`` [num_pages, page_size, 1, width] of the same
+    dtype: token t to row ``slot_map[t]`` (int64 or int32) % page_size of page ``slot_map[t]`` //
+    page_size, as ``paged_batch_plan`` makes them.  A negative slot leaves its token out; so does one
+    past the pool, which is reported.  No two tokens have one slot; rows are whole 16-byte pieces, and
+    neither the tokens nor two caches share memory with rows that are written.
+    """
+    tokens, caches = list(tokens), list(caches)
+    template, copy = _store_plan(tokens, caches, slot_map)
+    index = caches[0].get_device()
+    if H.current_device() != index:
+        with torch.cuda.device(index):
+            return paged_cache_store(tokens, caches, slot_map)
+    p = CacheStoreParams.from_buffer_copy(template)
+    keep = []
+    for e, t, c, again in zip(p.rows, tokens, caches, copy):
+        if again or t.data_ptr() % 16:
+            t = t.clone(memory_format=torch.contiguous_format)
+            keep.append(t)
+            e.src_token_stride = e.width_bytes
+        if c.data_ptr() % 16:
+            raise ValueError("caches need 16-byte aligned bases")
+        e.src, e.cache = t.data_ptr(), c.data_ptr()
+    slots = slot_map.to(torch.int64).contiguous()
+    p.slots = slots.data_ptr()
+    p.error_flag = report_ptr(index)
+    check(lib().dsa_cache_store(p, H.raw_stream(index)), "dsa_cache_store")
+    return caches
+
+
+class PagedBatchPlan(NamedTuple):
+    """What :func:`paged_batch_plan` makes; int32, but for ``slot_map``."""
+    block_table: torch.Tensor      # [B, max_blocks]
+    key_lengths: torch.Tensor      # [B]
+    query_ends: torch.Tensor       # [B] new tokens up to the request's last (TND lengths)
+    token_rows: torch.Tensor       # [T] request of each token, -1 behind the last
+    positions: torch.Tensor        # [T], 0 behind the last
+    slot_map: torch.Tensor         # [T] int64, -1 behind the last
+    group_starts: torch.Tensor     # [max_groups + 1]
+    prefix_lengths: torch.Tensor   # [max_groups]
+
+
+def _batch_plan(block_table, seq_lengths, rows, counts, page_size, num_tokens, max_groups, min_prefix):
+    """Check the arguments and fill in what their shapes decide."""
+    H.require_cuda(block_table)
+    dev = block_table.device
+    bt = _int32(block_table, "block_table", 2, dev)
+    if bt.numel() == 0:
+        raise ValueError("block_table must not be empty")
+    if _int32(seq_lengths, "seq_lengths", 1, dev).numel() != bt.shape[0]:
+        raise ValueError(f"seq_lengths must have {bt.shape[0]} entries, got {seq_lengths.numel()}")
+    batch = _int32(rows, "rows", 1, dev).numel()
+    if _int32(counts, "counts", 1, dev).numel() != batch:
+        raise ValueError(f"counts must have {batch} entries (as rows has), got {counts.numel()}")
+    for value, name, least in ((page_size, "page_size", 1), (num_tokens, "num_tokens", 0), (max_groups, "max_groups", 0),
+                               (min_prefix, "min_prefix", 0)):
+        if not least <= value <= 0x7fffffff:
+            raise ValueError(f"{name} must be {least}..{0x7fffffff}, got {value}")
+    if bt.shape[1] * page_size > 0x7fffffff:
+        raise ValueError(f"{bt.shape[1]} blocks of {page_size} tokens pass 32 bits")
+    p = BatchPlanParams()
+    p.batch, p.page_size, p.num_tokens = batch, page_size, num_tokens
+    p.slots, p.max_blocks = bt.shape
+    p.max_groups, p.min_prefix = max_groups, min_prefix
+    p.workspace_bytes = lib().dsa_batch_plan_workspace_size(batch)
+    return bytes(p)
+
+
+def paged_batch_plan(block_table, seq_lengths, rows, counts, page_size, num_tokens, max_groups=None, min_prefix=1):
+    """The plan of a step, from the lengths of its requests, without waiting for them: request b is slot
+    ``rows[b]`` [B] of the pool's state with ``counts[b]`` new tokens, which ``seq_lengths`` counts
+    already (``paged_cache_extend``).  Returns a :class:`PagedBatchPlan`:
+
+    * ``block_table``, ``key_lengths``: the requests' pages (-1 behind their lengths) and lengths, for
+      attention and the indexer;
+    * ``query_ends``: the new tokens up to each request's last, the cumulative lengths of TND calls;
+    * ``token_rows``, ``positions``, ``slot_map``: of the ``num_tokens`` places of the packed new tokens,
+      one request behind another, the request, the position (for ``rotary_embedding``) and the slot, page *
+      page_size + row (for ``paged_cache_store``); -1, 0 and -1 behind the last token;
+    * ``group_starts``, ``prefix_lengths``: groups of neighbouring requests with at least
+      max(``min_prefix``, page_size) tokens in common, in whole pages that both had before this step (for
+      ``flash_attention_shared_prefix``); a request that shares less with the one before it begins a
+      group.  The first ``max_groups`` (default B) are listed.
+
+    A request that cannot be (a slot out of range, a count past its length) is taken as an empty one,
+    a token without a page has slot -1, and tokens past ``num_tokens`` are left out; all are reported
+    by ``check_device_errors``.
+    """
+    page_size, num_tokens, min_prefix = int(page_size), int(num_tokens), int(min_prefix)
+    if max_groups is None:
+        max_groups = rows.numel()
+    max_groups = int(max_groups)
+    template = _batch_plan(block_table, seq_lengths, rows, counts, page_size, num_tokens, max_groups, min_prefix)
+    index = block_table.get_device()
+    if H.current_device() != index:
+        with torch.cuda.device(index):
+            return paged_batch_plan(block_table, seq_lengths, rows, counts, page_size, num_tokens, max_groups, min_prefix)
+    p = BatchPlanParams.from_buffer_copy(template)
+    given = [t.contiguous() for t in (block_table, seq_lengths, rows, counts)]
+    p.block_table, p.seq_lengths, p.rows, p.counts = [t.data_ptr() for t in given]
+    batch = p.batch
+    make = lambda *shape, dtype=torch.int32: torch.empty(shape, dtype=dtype, device=block_table.device)
+    plan = PagedBatchPlan(make(batch, block_table.shape[1]), make(batch), make(batch), make(num_tokens), make(num_tokens),
+                          make(num_tokens, dtype=torch.int64), make(max_groups + 1), make(max_groups))
+    ws = make(max(batch, 1))
+    p.block_table_out, p.key_lengths, p.query_ends = [t.data_ptr() for t in plan[:3]]
+    p.token_rows, p.positions, p.slot_map = [t.data_ptr() for t in plan[3:6]]
+    p.group_starts, p.prefix_lengths = [t.data_ptr() for t in plan[6:]]
+    p.workspace = ws.data_ptr()
+    p.error_flag = report_ptr(index)
+    check(lib().dsa_batch_plan(p, H.raw_stream(index)), "dsa_batch_plan")
+    return plan

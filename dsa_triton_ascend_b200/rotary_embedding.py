@@ -1,4 +1,5 @@
-"""rotary_embedding: rotary positions on queries and keys, and their gradient.
+"""rotary_embedding, rotary_embedding_axes: rotary positions on queries and keys, on one axis or
+several, and their gradient.
 
 What produces the ``query_rope`` / ``key_rope`` arguments of the attention operators
 (interleaved pairs, 64 wide) and the rotated part of the index queries and keys (half layout,
@@ -12,11 +13,12 @@ import math
 import torch
 
 from . import _host as H
-from ._lib import (BIND_ROTARY, DSA_DTYPE_FP32, RotaryParams, binding, check, lib, ptr, remember,
-                   report_ptr, stream_ptr)
+from ._lib import (BIND_ROTARY, DSA_DTYPE_FP32, ROTARY_MAX_AXES, RotaryAxesParams, RotaryParams, binding,
+                   check, lib, ptr, remember, report_ptr, stream_ptr)
 
 _MAX_DIM = 256
 LAYOUTS = ("interleaved", "half")
+ORDERS = ("blocks", "cycled")
 
 
 def rotary_frequencies(dim, base=10000.0, scaling=None, factor=1.0, original_positions=4096,
@@ -79,8 +81,9 @@ def _token_strides(t: torch.Tensor):
     return (0, *t.stride()[:2]) if t.dim() == 3 else tuple(t.stride()[:3])
 
 
-def _plan(x, table, positions, layout, offset, inverse, out):
-    """Check the arguments and fill in what their shapes decide."""
+def _plan(x, table, positions, layout, offset, inverse, out, axes=None):
+    """Check the arguments and fill in what their shapes decide; `axes`: how many axes the positions
+    have, in a dim of their own."""
     if layout not in LAYOUTS:
         raise ValueError(f"layout must be one of {LAYOUTS}, got {layout!r}")
     if x.dim() not in (3, 4):
@@ -94,8 +97,9 @@ def _plan(x, table, positions, layout, offset, inverse, out):
         raise ValueError(f"the table's dim must be even, 2..{_MAX_DIM}, got {dim}")
     if offset < 0 or offset + dim > x.shape[-1]:
         raise ValueError(f"offset {offset} + dim {dim} exceed the head's {x.shape[-1]} values")
-    if positions.shape != x.shape[:-2]:
-        raise ValueError(f"positions must be {tuple(x.shape[:-2])}, got {tuple(positions.shape)}")
+    shape = (*(() if axes is None else (axes,)), *x.shape[:-2])
+    if tuple(positions.shape) != shape:
+        raise ValueError(f"positions must be {shape}, got {tuple(positions.shape)}")
     if positions.dtype not in (torch.int32, torch.int64):
         raise ValueError("positions must be int32 or int64")
     H.require_cuda(x, table, positions, out)
@@ -116,6 +120,28 @@ def _plan(x, table, positions, layout, offset, inverse, out):
     p.half_layout, p.inverse = int(layout == "half"), int(bool(inverse))
     p.dtype = DSA_DTYPE_FP32 if x.dtype == torch.float32 else H.dtype_code(x)
     return bytes(p)
+
+
+def _fill(p, x, table, positions, out):
+    """Put the addresses in: (out, whether x, table and positions went in as they were given, what has to
+    live until the launch)."""
+    given = (x, table, positions)
+    if x.stride(-1) != 1:
+        if out is x:
+            raise ValueError("a rotation in place needs a contiguous last dim")
+        x = x.contiguous()
+        p.x_batch_stride, p.x_token_stride, p.x_head_stride = _token_strides(x)
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    elif out is not x and H.overlap(out, x):
+        raise ValueError("out overlaps x (pass x itself to rotate in place)")
+    if positions.dtype != torch.int32:   # a position past 32 bits stays outside the table
+        positions = positions.clamp(-1, 0x7fffffff).to(torch.int32)
+    positions = positions.contiguous()
+    table = table.contiguous()
+    p.x, p.out = x.data_ptr(), out.data_ptr()
+    p.positions, p.table = positions.data_ptr(), table.data_ptr()
+    return out, all(a is b for a, b in zip(given, (x, table, positions))), (x, table, positions)
 
 
 def rotary_embedding(x, table, positions, layout="interleaved", offset=0, inverse=False, out=None):
@@ -141,23 +167,68 @@ def rotary_embedding(x, table, positions, layout="interleaved", offset=0, invers
         with torch.cuda.device(index):
             return rotary_embedding(x, table, positions, layout, offset, inverse, out)
     p = RotaryParams.from_buffer_copy(template)
-    if x.stride(-1) != 1:
-        if out is x:
-            raise ValueError("a rotation in place needs a contiguous last dim")
-        x = x.contiguous()
-        p.x_batch_stride, p.x_token_stride, p.x_head_stride = _token_strides(x)
-    if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    elif out is not x and H.overlap(out, x):
-        raise ValueError("out overlaps x (pass x itself to rotate in place)")
-    if positions.dtype != torch.int32:   # a position past 32 bits stays outside the table
-        positions = positions.clamp(-1, 0x7fffffff).to(torch.int32)
-    positions = positions.contiguous()
-    table = table.contiguous()
-    p.x, p.out = x.data_ptr(), out.data_ptr()
-    p.positions, p.table = positions.data_ptr(), table.data_ptr()
+    out, as_given, keep = _fill(p, x, table, positions, out)
     p.error_flag = report_ptr(index)
     check(lib().dsa_rotary(p, H.raw_stream(index)), "dsa_rotary")
-    if x is args[0] and table is args[1] and positions is args[2]:
+    if as_given:
         remember(BIND_ROTARY, index, *args, template, b"", 0)
+    return out
+
+
+def rotary_axes(sections, order="blocks"):
+    """The axis of each of the sum(sections) pairs, of which ``sections[a]`` turn by axis a.  "blocks":
+    the first ``sections[0]`` pairs by axis 0, the next by axis 1, and so on.  "cycled": pair i by axis
+    i % len(sections) as long as that axis has pairs left, by axis 0 from then on, so that each axis
+    has fast and slow pairs; it needs ``sections[a]`` turns of every axis but the first."""
+    try:
+        sections = tuple(int(n) for n in sections)
+    except TypeError:
+        raise ValueError(f"sections must be a sequence of numbers, got {sections!r}") from None
+    axes, half = len(sections), sum(sections)
+    if not 1 <= axes <= ROTARY_MAX_AXES or min(sections) < 1:
+        raise ValueError(f"sections must be 1..{ROTARY_MAX_AXES} positive numbers, got {sections}")
+    if order not in ORDERS:
+        raise ValueError(f"order must be one of {ORDERS}, got {order!r}")
+    if order == "blocks":
+        return [a for a, n in enumerate(sections) for _ in range(n)]
+    if any(axes * (n - 1) + a >= half for a, n in enumerate(sections) if a):
+        raise ValueError(f"sections {sections} cannot take turns: an axis has more pairs than turns")
+    return [i % axes if i < axes * sections[i % axes] else 0 for i in range(half)]
+
+
+def _axes_plan(x, table, positions, sections, layout, order, offset, inverse, out):
+    axis_of = rotary_axes(sections, order)
+    if table.dim() == 2 and 2 * len(axis_of) != table.shape[1]:
+        raise ValueError(f"sections {tuple(sections)} must add up to the table's {table.shape[1] // 2} pairs")
+    p = RotaryAxesParams()
+    p.rotary = RotaryParams.from_buffer_copy(_plan(x, table, positions, layout, offset, inverse, out, len(sections)))
+    p.axes = len(sections)
+    for i, a in enumerate(axis_of):
+        p.axis_of[i] = a
+    return bytes(p)
+
+
+def rotary_embedding_axes(x, table, positions, sections, layout="interleaved", order="blocks", offset=0,
+                          inverse=False, out=None):
+    """:func:`rotary_embedding` with positions on several axes (time, height and width of pictures and
+    films): ``positions`` is [A, B, S] for ``x`` [B, S, N, H] or [A, T] for [T, N, H], A up to 4, and of
+    the pairs of each head ``sections[a]`` turn by axis a's position, pair i by column i of the table
+    as there.  ``order`` says which, see :func:`rotary_axes`; ``sections`` add up to
+    ``table.shape[1] / 2``.  Text has the same position on every axis, and gives what
+    ``rotary_embedding`` gives.
+
+    A position outside the table on any axis gives a zero row and is reported by
+    ``check_device_errors``.
+    """
+    sections = tuple(sections) if isinstance(sections, (list, tuple)) else sections
+    args = (x, table, positions, sections, layout, order, offset, bool(inverse), out)
+    template = _axes_plan(*args)
+    index = x.get_device()
+    if H.current_device() != index:
+        with torch.cuda.device(index):
+            return rotary_embedding_axes(x, table, positions, sections, layout, order, offset, inverse, out)
+    p = RotaryAxesParams.from_buffer_copy(template)
+    out, as_given, keep = _fill(p.rotary, x, table, positions, out)
+    p.rotary.error_flag = report_ptr(index)
+    check(lib().dsa_rotary_axes(p, H.raw_stream(index)), "dsa_rotary_axes")
     return out

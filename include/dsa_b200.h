@@ -507,6 +507,22 @@ typedef struct DsaRotaryParams {
 
 int dsa_rotary(const DsaRotaryParams* params, void* stream);
 
+/*
+ * The same with positions on several axes (time, height and width of pictures and films):
+ * rotary.positions is [axes][batch][s], and pair i of each head turns by the position of axis
+ * axis_of[i] < axes (a host array's first dim / 2 entries), by column i of the table.  A token with
+ * a position outside the table on any axis becomes a zero row and is reported in error_flag.
+ */
+#define DSA_ROTARY_MAX_AXES 4
+
+typedef struct DsaRotaryAxesParams {
+  DsaRotaryParams rotary;
+  int32_t axes;
+  uint8_t axis_of[128];
+} DsaRotaryAxesParams;
+
+int dsa_rotary_axes(const DsaRotaryAxesParams* params, void* stream);
+
 /* table[p][i] = amplitude * cos(p * frequencies[i]), table[p][dim / 2 + i] = amplitude * sin(...)
  * for p < max_positions, i < dim / 2; `frequencies` is a host array, read before the return. */
 int dsa_rotary_table(float* table, int64_t max_positions, int64_t dim, const double* frequencies,
@@ -612,6 +628,70 @@ typedef struct DsaPagesParams {
 
 int dsa_pages(const DsaPagesParams* params, void* stream);
 int64_t dsa_pages_workspace_size(int32_t op, int64_t n, int64_t slots, int64_t num_pages);
+
+/*
+ * The plan of a step over a paged cache, from the lengths of its requests.  No counterpart in the
+ * reference.  Request b < batch is slot rows[b] of a pool's state (block_table [slots][max_blocks],
+ * seq_lengths [slots]) with counts[b] new tokens, which its length n counts already.
+ *   block_table_out [batch][max_blocks]  the request's pages, -1 behind its length
+ *   key_lengths [batch], query_ends [batch]  n, and the new tokens up to the request's last
+ *   token_rows, positions, slot_map [num_tokens]  of each new token, one request behind another:
+ *       its request, its position (n - counts[b] + i) and its slot, page * page_size + row; -1, 0
+ *       and -1 behind the last
+ *   group_starts [max_groups + 1], prefix_lengths [max_groups]  groups of neighbouring requests that
+ *       have at least max(min_prefix, page_size) tokens in whole pages in common, and how many; a
+ *       request of its own is a group with 0.  Of more groups the first max_groups are listed;
+ *       behind the last one starts are batch and lengths 0.
+ * A request that asks for what cannot be (a slot out of range, a count below 0 or past the length, a
+ * length past the table) is taken as an empty one, a token without a page has slot -1, tokens past
+ * num_tokens are not listed; error_flag tells.
+ * Workspace: dsa_batch_plan_workspace_size() bytes.
+ */
+typedef struct DsaBatchPlanParams {
+  const int32_t* block_table;
+  const int32_t* seq_lengths;
+  const int32_t* rows;
+  const int32_t* counts;
+  int32_t* block_table_out;
+  int32_t* key_lengths;
+  int32_t* query_ends;
+  int32_t* token_rows;
+  int32_t* positions;
+  int64_t* slot_map;
+  int32_t* group_starts;
+  int32_t* prefix_lengths;
+  int* error_flag;
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t batch;
+  int64_t slots;
+  int64_t max_blocks;
+  int64_t page_size;
+  int64_t num_tokens;
+  int64_t max_groups;
+  int64_t min_prefix;
+} DsaBatchPlanParams;
+
+int dsa_batch_plan(const DsaBatchPlanParams* params, void* stream);
+int64_t dsa_batch_plan_workspace_size(int64_t batch);
+
+/*
+ * Store packed tokens in a paged cache: token t goes to slot slots[t] (page * page_size + row) of up
+ * to four caches at once.  No counterpart in the reference.  Entries as for dsa_cache_append, without
+ * rotation; src_batch_stride is not read.  A negative slot leaves the token out; so does one past the
+ * pool, which is reported in error_flag.  No two tokens have one slot.
+ */
+typedef struct DsaCacheStoreParams {
+  DsaCacheRows rows[DSA_APPEND_MAX_ENTRIES];
+  const int64_t* slots;
+  int* error_flag;
+  int64_t tokens;
+  int64_t num_pages;
+  int64_t page_size;
+  int32_t entries;
+} DsaCacheStoreParams;
+
+int dsa_cache_store(const DsaCacheStoreParams* params, void* stream);
 
 #ifdef __cplusplus
 }
