@@ -122,7 +122,8 @@ class AttnPagedParams(ctypes.Structure):
 
 
 class AttnSharedParams(ctypes.Structure):
-    _fields_ = [("attn", AttnPagedParams), ("group_starts", _p), ("prefix_lengths", _p), ("groups", _i64)]
+    _fields_ = [("attn", AttnPagedParams), ("group_starts", _p), ("prefix_lengths", _p), ("groups", _i64),
+                ("least_saving", _i64)]
 
 
 class RotaryParams(ctypes.Structure):
@@ -293,9 +294,10 @@ def binding():
             return None
         if getattr(module, "TORCH_VERSION", None) != torch.__version__:
             return None
-        entries = [ctypes.cast(getattr(lib(), name), ctypes.c_void_p).value
-                   for name in ("dsa_attn_paged", "dsa_rotary", "dsa_cache_append", "dsa_pages")]
-        module.connect(*entries, check)
+        entries = tuple(ctypes.cast(getattr(lib(), name), ctypes.c_void_p).value for name in (
+            "dsa_attn_paged", "dsa_rotary", "dsa_cache_append", "dsa_pages", "dsa_attn_shared", "dsa_rotary_axes",
+            "dsa_batch_plan", "dsa_cache_store"))
+        module.connect(entries, check)
         _binding = module
     return _binding or None
 
@@ -309,7 +311,8 @@ def remember(op: int, index: int, *call) -> None:
         module.keep(op, *call)
 
 
-BIND_ATTN, BIND_ROTARY, BIND_APPEND, BIND_UPKEEP = range(4)   # Op of csrc/binding.cpp
+# Op of csrc/binding.cpp
+BIND_ATTN, BIND_ROTARY, BIND_APPEND, BIND_UPKEEP, BIND_SHARED, BIND_AXES, BIND_PLAN, BIND_STORE = range(8)
 
 
 def check(rc: int, what: str) -> None:

@@ -63,7 +63,7 @@ int launch(const DsaAttnPagedParams* p, int diag, int heads, cudaStream_t stream
       cudaSuccess)
     return DSA_ERR_CUDA;
   if (!launch_early(kern, grid, kThreads, C::kSmem, stream, maps, a)) return DSA_ERR_CUDA;
-  return launch_join<D, NH, kSegmentCost, T>(p, a, grid, stream);
+  return launch_join<D, NH, kSegmentCost, T>(a, grid, stream);
 }
 
 template <typename T>
@@ -75,7 +75,7 @@ int launch_pair(const DsaAttnPagedParams* p, int diag, int heads, cudaStream_t s
   if (pairs < 1) return DSA_ERR_CUDA;
   Maps maps;
   CUtensorMap map_v;
-  if (!make_maps<D>(&maps, p, kBf16, pair::kHeads) || !make_value_map<D>(&map_v, p, kBf16, C::kVChunks))
+  if (!make_pair_maps<D>(&maps, &map_v, p, kBf16, pair::kHeads))
     return DSA_ERR_TMA_DESCRIPTOR;
   const Args a = make_args(p, 2 * pair::kHeads, pairs, diag, heads);
   auto kern = pair::attn_paged_pair_kernel<D, T>;
@@ -83,7 +83,7 @@ int launch_pair(const DsaAttnPagedParams* p, int diag, int heads, cudaStream_t s
       cudaSuccess)
     return DSA_ERR_CUDA;
   if (!launch_early(kern, 2 * pairs, pair::kThreads, C::kSmem, stream, maps, map_v, a)) return DSA_ERR_CUDA;
-  return launch_join<D, 2 * pair::kHeads, pair::kSegmentCost, T>(p, a, pairs, stream);
+  return launch_join<D, 2 * pair::kHeads, pair::kSegmentCost, T>(a, pairs, stream);
 }
 
 template <int D, typename T>
@@ -99,7 +99,7 @@ int launch_wide(const DsaAttnPagedParams* p, int diag, int heads, cudaStream_t s
       cudaSuccess)
     return DSA_ERR_CUDA;
   if (!launch_early(kern, grid, wide::kThreads, C::kSmem, stream, maps, a)) return DSA_ERR_CUDA;
-  return launch_join<D, wide::kHeads, wide::kSegmentCost, T>(p, a, grid, stream);
+  return launch_join<D, wide::kHeads, wide::kSegmentCost, T>(a, grid, stream);
 }
 
 template <int D, typename T>

@@ -55,9 +55,9 @@ __device__ __forceinline__ int token_keys(const Args& a, int row) {
 }
 __device__ __forceinline__ int row_keys(const Args& a, int row) { return token_keys(a, row); }
 
-// What a call is made of in which rows share keys (attn_shared.cu): its pieces take the place of the
-// rows above.  The first `shared_items` are runs of neighbouring tokens over the keys that they have in
-// common, the others rows (or, packed, the tokens of a batch) over the rest of theirs.
+// Where rows share keys (attn_shared.cu), a call is two launches, whose pieces take the place of the rows
+// above: prefixes, for runs of neighbouring tokens each, and the rest, rows (or the tokens of a batch,
+// packed) over the other keys of theirs.
 struct Item {
   int32_t keys;     // 0: nothing to do
   int32_t first;    // position of its first key, at the start of a page
@@ -65,12 +65,15 @@ struct Item {
   int32_t head0;    // its first row of all batch * s1 * n1 rows of queries, and how many
   int32_t heads;
   int32_t part;     // whether its result is a part in any case
-  int32_t unused[2];
+  int32_t place;    // of its heads' results, behind the shares' slots, where one CTA takes all of it
+  int32_t unused;
 };
 struct ItemArgs : Args {
   const Item* items;      // [rows]
-  const int4* groups;     // [batch]: shared keys (0: none), first item, first token of the row's group
-  int32_t shared_items, per_item;   // tokens of a shared item
+  const int32_t* limit;   // CTAs (or pairs) that take part
+  // The second launch may run beside the first: that one lets it start once the plan is there, and it
+  // ends after that one, so that what follows it has both.
+  bool second;
 };
 
 __device__ __forceinline__ int row_keys(const ItemArgs& a, int row) { return a.items[row].keys; }
@@ -96,13 +99,23 @@ __device__ __forceinline__ QueryAt row_query(const Args& a, int row) {
 }
 __device__ __forceinline__ QueryAt row_query(const ItemArgs& a, int row) { return {a.items[row].head0, 0, 0}; }
 // First of the workspace's places (of a head each) for a row that one CTA takes all of, behind the
-// two slots of each share; an item's rest has as many as it has heads.
+// two slots of each share.
 template <int NH>
 __device__ __forceinline__ int64_t own_place(const Args&, int shares, int row) { return ((int64_t)2 * shares + row) * NH; }
 template <int NH>
 __device__ __forceinline__ int64_t own_place(const ItemArgs& a, int shares, int row) {
-  if (row < a.shared_items) return ((int64_t)2 * shares + row) * NH;
-  return ((int64_t)2 * shares + a.shared_items) * NH + a.items[row].head0;
+  return (int64_t)2 * shares * NH + a.items[row].place;
+}
+// The stream's kernels before this one have ended: before anything of theirs is read, and before the end.
+// The next kernel may start once that is so (where pieces wait for it, at once, else after the division).
+__device__ __forceinline__ void wait_first(const Args&) { griddep_wait(); }
+__device__ __forceinline__ void wait_first(const ItemArgs& a) {
+  if (!a.second) griddep_wait();
+  griddep_launch_dependents();
+}
+__device__ __forceinline__ void wait_last(const Args&) {}
+__device__ __forceinline__ void wait_last(const ItemArgs& a) {
+  if (a.second) griddep_wait();
 }
 
 template <int kTile, int kCost, typename A>
@@ -249,6 +262,20 @@ __device__ __forceinline__ Work share_of(const A& a, int cta, int ctas_max, bool
   work.row = start[0];
   work.unit = start[1];
   return work;
+}
+
+// The same, of as many CTAs as take part, and the next kernel let start.
+template <int kTile, int kCost, int kThreads>
+__device__ __forceinline__ Work take_share(const Args& a, int cta, int grid, bool first_cta, int* tmp, int32_t* start) {
+  const Work work = share_of<kTile, kCost, kThreads>(a, cta, grid, first_cta, tmp, start);
+  griddep_launch_dependents();
+  return work;
+}
+template <int kTile, int kCost, int kThreads>
+__device__ __forceinline__ Work take_share(const ItemArgs& a, int cta, int grid, bool first_cta, int* tmp, int32_t* start) {
+  const int limit = min(grid, *a.limit);
+  if (cta >= limit) return Work{0, 0, 0};
+  return share_of<kTile, kCost, kThreads>(a, cta, limit, first_cta, tmp, start);
 }
 
 // The statistics of one (row, head): raw maximum `top`, sum over the exponents' reference `ref`,

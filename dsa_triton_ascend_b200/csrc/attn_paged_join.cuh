@@ -2,7 +2,6 @@
 #pragma once
 
 #include <cmath>
-#include <type_traits>
 
 #include "attn_paged.cuh"
 #include "dsa_b200.h"
@@ -13,28 +12,19 @@ namespace dsa {
 namespace attn_paged {
 
 // Where the parts of one (row, head) are: CTAs c0 .. c1, whose slot of a part is 2 c, but 2 c0 + 1
-// where the row begins inside the share of c0; or the row's own slot (c0 == c1).
+// where the row begins inside the share of c0; or the row's own place (c0 == c1).
 struct Parts {
   int c0, c1, skip;
   int64_t own;
-  template <int NH>
-  __device__ __forceinline__ int64_t at(int c, int h) const {
-    return (c0 == c1 ? own : (int64_t)(2 * c + (c == c0 ? skip : 0)) * NH) + h;
+  __device__ __forceinline__ int64_t at(int c, int h, int nh) const {
+    return (c0 == c1 ? own : (int64_t)(2 * c + (c == c0 ? skip : 0)) * nh) + h;
   }
 };
 
-// False for a row without a part (c1 < c0).
-template <int NH, int kCost, typename A>
-__device__ __forceinline__ bool parts_of(const A& a, int grid, int row, Parts* p) {
-  const int first = a.ws_prefix[row], next = a.ws_prefix[row + 1], all = a.ws_prefix[a.rows];
-  const int count = next - first;   // units
-  p->own = own_place<NH>(a, grid, row);
-  p->skip = 0;
-  p->c0 = 1;
-  p->c1 = 0;
-  if (count == 0) return false;
-  const int64_t units = all, ctas = ctas_used(units, grid), x0 = first;
-  const int64_t lo = (x0 + kCost + 1) * ctas - 1, hi = (x0 + count) * ctas - 1;
+// Of a row with `count` units behind the first `first` of all `total`, `cost` of them for its start.
+__device__ __forceinline__ void find_parts(int first, int count, int64_t total, int cost, int grid, Parts* p) {
+  const int64_t units = total, ctas = ctas_used(units, grid), x0 = first;
+  const int64_t lo = (x0 + cost + 1) * ctas - 1, hi = (x0 + count) * ctas - 1;
   if (units * ctas < (1LL << 32)) {
     const uint32_t u = (uint32_t)units;
     p->c0 = (int)((uint32_t)lo / u);
@@ -44,17 +34,25 @@ __device__ __forceinline__ bool parts_of(const A& a, int grid, int row, Parts* p
     p->c1 = (int)(hi / units);
   }
   p->skip = share_begin(units, p->c0, ctas) < x0 ? 1 : 0;
+}
+
+// False for a row without a part (c1 < c0).
+template <int NH, int kCost>
+__device__ __forceinline__ bool parts_of(const Args& a, int grid, int row, Parts* p) {
+  const int first = a.ws_prefix[row], next = a.ws_prefix[row + 1], all = a.ws_prefix[a.rows];
+  const int count = next - first;   // units
+  p->own = own_place<NH>(a, grid, row);
+  p->skip = 0;
+  p->c0 = 1;
+  p->c1 = 0;
+  if (count == 0) return false;
+  find_parts(first, count, all, kCost, grid, p);
   return true;
 }
 
-// q . k + qr . kr of packed head `head` of batch `b` and the key at position `pos`, by a warp; false
-// if there is no such page.
+// q . k + qr . kr of packed head `head` of batch `b` and the key in row `row` of page `page`, by a warp.
 template <int D, typename T>
-__device__ __forceinline__ bool warp_dot(const Args& a, int b, int head, int pos, int lane, float* dot,
-                                         const T** key) {
-  const int page = a.block_table[(int64_t)b * a.max_blocks + pos / a.page_size], row = pos % a.page_size;
-  if (page >= a.num_pages && lane == 0) report_error(a.error_flag, kErrBadIndex);
-  if (page < 0 || page >= a.num_pages) return false;
+__device__ __forceinline__ float late_dot(const Args& a, int b, int head, int page, int row, int lane, const T** key) {
   const T* k = static_cast<const T*>(a.k) + page * a.k_page + row * a.k_row;
   const T* kr = static_cast<const T*>(a.kr) + page * a.kr_page + row * a.kr_row;
   const T* q = static_cast<const T*>(a.q) + b * a.q_batch + head * a.q_head;
@@ -71,8 +69,18 @@ __device__ __forceinline__ bool warp_dot(const Args& a, int b, int head, int pos
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  *dot = sum;
   *key = k;
+  return sum;
+}
+
+// The same of the key at position `pos`; false if there is no such page.
+template <int D, typename T>
+__device__ __forceinline__ bool warp_dot(const Args& a, int b, int head, int pos, int lane, float* dot,
+                                         const T** key) {
+  const int page = a.block_table[(int64_t)b * a.max_blocks + pos / a.page_size], row = pos % a.page_size;
+  if (page >= a.num_pages && lane == 0) report_error(a.error_flag, kErrBadIndex);
+  if (page < 0 || page >= a.num_pages) return false;
+  *dot = late_dot<D, T>(a, b, head, page, row, lane, key);
   return true;
 }
 
@@ -84,10 +92,9 @@ constexpr int kMaxDiag = 7;
 // each), else a warp.
 constexpr int kJoinThreads = 256;
 
-template <int D, int NH, int kCost, int kLanes, typename T, typename A = Args>
-__global__ void __launch_bounds__(kJoinThreads) attn_paged_combine_kernel(const A a, int grid) {
+template <int D, int NH, int kCost, int kLanes, typename T>
+__global__ void __launch_bounds__(kJoinThreads) attn_paged_combine_kernel(const Args a, int grid) {
   using E = ElemTraits<T>;
-  constexpr bool kItems = std::is_same<A, ItemArgs>::value;
   constexpr bool kWide = kLanes == kJoinThreads;
   constexpr int kCols = kLanes < D / 4 ? kLanes : D / 4;   // threads of a part
   constexpr int kPer = D / 4 / kCols;                      // float4s of each
@@ -99,42 +106,22 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_combine_kernel(const 
   griddep_wait();
   griddep_launch_dependents();
   const int64_t at = (int64_t)blockIdx.x * (kJoinThreads / kLanes) + threadIdx.x / kLanes;
-  int rows = a.rows, shared_items = 0;
-  if constexpr (kItems) {
-    shared_items = a.shared_items;
-    rows -= shared_items;
-  }
-  if (at >= (int64_t)rows * a.n1) return;
+  if (at >= (int64_t)a.rows * a.n1) return;
   const int row = (int)(at / a.n1), head = (int)(at - (int64_t)row * a.n1);
   const int t = threadIdx.x % kLanes, grp = t / kCols, col = t % kCols, lane = threadIdx.x & 31;
   T* out = static_cast<T*>(a.out) + at * D;
   Parts p;
-  const bool some = parts_of<NH, kCost>(a, grid, shared_items + row, &p);
-  // parts of the keys that the token's group shares, of which it is head `head2`
-  Parts p2{0, -1, 0, 0};
-  int head2 = 0;
-  if constexpr (kItems) {
-    const int b = row / a.s1;
-    const int4 g = a.groups[b];
-    const int tokens = a.n1 / a.heads, s = head / a.heads;   // of a packed row, and the one of this head
-    const int seen = tokens > 1 ? min(a.act_k[b], (int)min((int64_t)0x7fffffff, (int64_t)a.max_blocks * a.page_size)) - a.diag + (a.diag > 0 ? s : 0)
-                                : token_keys(a, row);
-    if (g.x > 0 && seen > 0) {
-      const int t = row * tokens + s - g.z, item = t / a.per_item;
-      head2 = (t - item * a.per_item) * a.heads + head - s * a.heads;
-      parts_of<NH, kCost>(a, grid, g.y + item, &p2);
-    }
-  }
+  const bool some = parts_of<NH, kCost>(a, grid, row, &p);
   // keys from `common` on that this token sees beside the row's common ones
   int late = 0, common = 0;
   if (a.diag > 0) {
     const int64_t cap = (int64_t)a.max_blocks * a.page_size, ak = a.act_k[row];
     common = (int)max((int64_t)0, min(cap, ak - a.diag));
     late = (int)(max((int64_t)common, min(cap, ak - a.diag + head / a.heads)) - common);
-  } else if (some && p.c0 == p.c1 && p2.c1 < p2.c0) {
+  } else if (some && p.c0 == p.c1) {
     return;   // written whole
   }
-  if (!some && late == 0 && p2.c1 < p2.c0) {
+  if (!some && late == 0) {
     if (grp == 0)
 #pragma unroll
       for (int i = 0; i < kPer; ++i) *reinterpret_cast<uint2*>(out + (i * kCols + col) * 4) = make_uint2(0, 0);
@@ -150,18 +137,10 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_combine_kernel(const 
   }
   float ref = -INFINITY, run = -INFINITY, top = -INFINITY;
   for (int c = p.c0 + lane; c <= p.c1; c += 32) {
-    const float4 s = a.ws_s[p.at<NH>(c, head)];
+    const float4 s = a.ws_s[p.at(c, head, NH)];
     ref = fmaxf(ref, s.x);
     run = fmaxf(run, s.y);
     top = fmaxf(top, s.w);
-  }
-  if constexpr (kItems) {
-    for (int c = p2.c0 + lane; c <= p2.c1; c += 32) {
-      const float4 s = a.ws_s[p2.at<NH>(c, head2)];
-      ref = fmaxf(ref, s.x);
-      run = fmaxf(run, s.y);
-      top = fmaxf(top, s.w);
-    }
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -173,9 +152,10 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_combine_kernel(const 
 #pragma unroll
   for (int i = 0; i < kPer; ++i) acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float sum = 0.0f;
-  auto take = [&](int64_t place) {
-    const float4 s = a.ws_s[place];
-    const float4* o = reinterpret_cast<const float4*>(a.ws_o + place * D) + col;
+#pragma unroll 4
+  for (int c = p.c0 + grp; c <= p.c1; c += kGroups) {
+    const float4 s = a.ws_s[p.at(c, head, NH)];
+    const float4* o = reinterpret_cast<const float4*>(a.ws_o + p.at(c, head, NH) * D) + col;
     const float w = s.x == ref ? 1.0f : exp2f(s.x - ref);
     sum += w * s.z;
 #pragma unroll
@@ -183,12 +163,6 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_combine_kernel(const 
       const float4 x = o[i * kCols];
       acc[i].x += w * x.x, acc[i].y += w * x.y, acc[i].z += w * x.z, acc[i].w += w * x.w;
     }
-  };
-#pragma unroll 4
-  for (int c = p.c0 + grp; c <= p.c1; c += kGroups) take(p.at<NH>(c, head));
-  if constexpr (kItems) {
-#pragma unroll 4
-    for (int c = p2.c0 + grp; c <= p2.c1; c += kGroups) take(p2.at<NH>(c, head2));
   }
   if constexpr (kWide) {
     part[grp][col] = acc[0];
@@ -299,13 +273,13 @@ bool make_maps(Maps* maps, const DsaAttnPagedParams* p, bool bf16, uint32_t nh) 
          make_tmap_16b(&maps->kr, p->key_rope_cache, bf16, 4, krdims, krst, krbox);
 }
 
-// Tensor map of values: boxes of 8 or 16 keys, `chunks` times 64 dims.
+// Tensor maps of the pair kernel: the others', and one of values, boxes of 8 or 16 keys, a CTA's half of the dims.
 template <int D>
-bool make_value_map(CUtensorMap* map, const DsaAttnPagedParams* p, bool bf16, uint32_t chunks) {
+bool make_pair_maps(Maps* maps, CUtensorMap* values, const DsaAttnPagedParams* p, bool bf16, uint32_t nh) {
   const uint64_t dims[4] = {64, (uint64_t)p->page_size, D / 64, (uint64_t)p->num_pages};
   const uint64_t st[3] = {(uint64_t)p->k_row_stride * 2, 128, (uint64_t)p->k_page_stride * 2};
-  const uint32_t box[4] = {64, p->page_size % 16 ? 8u : 16u, chunks, 1};
-  return make_tmap_16b(map, p->key_cache, bf16, 4, dims, st, box);
+  const uint32_t box[4] = {64, p->page_size % 16 ? 8u : 16u, D / 128, 1};
+  return make_maps<D>(maps, p, bf16, nh) && make_tmap_16b(values, p->key_cache, bf16, 4, dims, st, box);
 }
 
 // A launch that may begin before the stream's kernel before it has ended: the kernels here wait
@@ -325,14 +299,14 @@ bool launch_early(void (*kern)(P...), int64_t blocks, int threads, int smem, cud
   return cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess;
 }
 
-template <int D, int NH, int kCost, typename T, typename A>
-int launch_join(const DsaAttnPagedParams* p, const A& a, int shares, cudaStream_t stream) {
-  const int64_t items = p->batch * p->s1 * p->n1;
+template <int D, int NH, int kCost, typename T>
+int launch_join(const Args& a, int shares, cudaStream_t stream) {
+  const int64_t items = (int64_t)a.rows * a.n1;
   // a block each up to eight a multiprocessor (what runs at once), else a warp each
   const bool wide = items <= 8LL * sm_count();
   const int64_t blocks = wide ? items : (items + kJoinThreads / 32 - 1) / (kJoinThreads / 32);
-  auto kern = wide ? attn_paged_combine_kernel<D, NH, kCost, kJoinThreads, T, A>
-                   : attn_paged_combine_kernel<D, NH, kCost, 32, T, A>;
+  auto kern = wide ? attn_paged_combine_kernel<D, NH, kCost, kJoinThreads, T>
+                   : attn_paged_combine_kernel<D, NH, kCost, 32, T>;
   return launch_early(kern, blocks, kJoinThreads, 0, stream, a, shares) ? DSA_OK : DSA_ERR_CUDA;
 }
 

@@ -127,7 +127,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     fence_mbarrier_init();
   }
   if (warp == kMmaWarp) tmem_alloc<2>(smem_u32(tmem_ptr), C::kTmem);
-  griddep_wait();
+  wait_first(a);
   if (threadIdx.x == kKeyWarp * 32) {
     tma_prefetch_desc(&maps.k);
     tma_prefetch_desc(&maps.kr);
@@ -135,8 +135,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&maps.q);
     tma_prefetch_desc(&maps.qr);
   }
-  Work work = share_of<kTile, kSegmentCost, kThreads>(a, blockIdx.x >> 1, gridDim.x >> 1, blockIdx.x == 0, tmp, start);
-  griddep_launch_dependents();
+  Work work = take_share<kTile, kSegmentCost, kThreads>(a, blockIdx.x >> 1, gridDim.x >> 1, blockIdx.x == 0, tmp, start);
   tc_fence_before();
   __syncthreads();
   cluster_sync();
@@ -542,6 +541,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     tmem_relinquish<2>();
     tmem_dealloc<2>(tmem, C::kTmem);
   }
+  wait_last(a);
 }
 
 }  // namespace pair

@@ -119,15 +119,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     fence_mbarrier_init();
   }
   if (warp == kQkWarp) tmem_alloc<1>(smem_u32(tmem_ptr), C::kTmem);
-  griddep_wait();
+  wait_first(a);
   if (threadIdx.x == kLoadWarp * 32) {
     tma_prefetch_desc(&maps.k);
     tma_prefetch_desc(&maps.kr);
     tma_prefetch_desc(&maps.q);
     tma_prefetch_desc(&maps.qr);
   }
-  Work work = share_of<kTile, kSegmentCost, kThreads>(a, blockIdx.x, gridDim.x, blockIdx.x == 0, tmp, start);
-  griddep_launch_dependents();
+  Work work = take_share<kTile, kSegmentCost, kThreads>(a, blockIdx.x, gridDim.x, blockIdx.x == 0, tmp, start);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -448,6 +447,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_relinquish<1>();
     tmem_dealloc<1>(tmem, C::kTmem);
   }
+  wait_last(a);
 }
 
 }  // namespace wide

@@ -5,14 +5,18 @@
 //   m_i = max z,  l_i = sum exp(z - m_i),  o_i = sum exp(z - m_i) v,
 // the result is sum_i e^(m_i - M) o_i / sum_i e^(m_i - M) l_i, M = max_i m_i.  So the prefix is taken
 // by pieces of several tokens of the group (their heads side by side, as many as the kernel holds),
-// which read its keys once, the rest by rows of their own; the join of attn_paged.cu, which puts a
-// row's parts together in a fixed order, takes the prefix's parts among them.
+// which read its keys once, the rest by rows of their own, and the join puts a row's parts of both
+// together, in a fixed order.
 //
-// The pieces are made on the device, from the lengths, by one block (shared_plan_kernel), so that a
-// captured call follows the lengths; then the kernels of attn_paged.cu take prefixes and rests in one
-// launch, by equal shares.  A group shares the whole pages of its prefix, at most as many as all of
-// its rows see.
+// Four launches: shared_plan_kernel makes the pieces from the lengths, in one block, so that a captured call
+// follows them; a kernel of attn_paged.cu takes the prefixes' pieces, 64 or 128 heads each, bound by
+// products; another one, of the size that a row's own heads need, the rests, bound by memory.  The two
+// run side by side: the plan divides the multiprocessors between them by what they cost, and the
+// second starts where the first leaves some.  A group shares the whole pages of its prefix, at most as
+// many as all of its rows see, where that costs less than its rows by themselves.
 #include <cuda_runtime.h>
+
+#include <type_traits>
 
 #include "attn_paged.cuh"
 #include "attn_paged_heads.cuh"
@@ -20,57 +24,109 @@
 #include "attn_paged_pair.cuh"
 #include "attn_paged_wide.cuh"
 #include "dsa_b200.h"
+#include "rotary.cuh"
 #include "sm100.cuh"
 
 namespace dsa {
 namespace attn_paged {
 
-constexpr int kPlanThreads = 1024;
+constexpr int kPlanThreads = 512;
+constexpr int kPlanRows = 2048;     // batch rows and groups whose lists fit into shared memory
+constexpr int kPlanGroups = 1024;
+
+// What a launch of either kind is made of: keys of a tile (1 << shift), units of starting a piece,
+// multiprocessors of a share, a unit's cost and that of a share's start and end, in cycles.
+struct Kind {
+  int32_t shift, start, sms, cost, fixed;
+};
+
+// What the plan tells the join: shares of either launch, units of all pieces.
+struct Limits {
+  int32_t shares, rest_shares, units, unused;
+};
 
 struct PlanArgs {
-  ItemArgs a;
-  Item* items;
-  int4* by_row;      // [batch], what ItemArgs::groups points to
-  int4* by_group;    // [groups]: shared keys, items, first row with keys, first item
+  Args a;            // of the rest
+  Item* pieces;      // [most]
+  Item* rest;        // [rows]
+  Limits* limits;
+  int4* by_row;      // [batch]: shared keys (0: none), first piece, first token of the row's group, first unit
+  int4* by_group;    // [groups]: shared keys, pieces, first row with keys, first piece
+  int32_t* by_units; // [groups]: first unit
   const int32_t* starts;
   const int32_t* prefixes;
   int32_t groups, batch, s1, packed;   // packed: tokens of a row of the rest
+  int32_t most, per_item, nh, sms;     // pieces at most; tokens and places of each
+  Kind prefix, own;
+  int32_t own_rows;                    // rows of the rest of a batch row
+  int64_t least_saving;
 };
 
 // Keys that the first token of batch row b with any sees (0: no token of the row sees one).
 __device__ __forceinline__ int least_seen(const PlanArgs& p, int b) {
-  const int64_t ak = p.a.act_k[b], aq = p.a.act_q ? p.a.act_q[b] : p.s1;
-  const int64_t cap = (int64_t)p.a.max_blocks * p.a.page_size;
+  const int ak = p.a.act_k[b], aq = p.a.act_q ? p.a.act_q[b] : p.s1;
+  const int cap = p.a.max_blocks * p.a.page_size;   // (below 2^31, as the host has seen to)
   if (ak <= 0 || aq <= 0) return 0;
   int64_t n = ak;
   if (p.a.mode == 3) {
-    n = ak - aq + 1 > 1 ? ak - aq + 1 : 1;
-    if (ak - aq + min((int64_t)p.s1, aq) < 1) return 0;   // (more queries counted than there are)
+    n = (int64_t)ak - aq + 1;
+    if (n - 1 + min(p.s1, aq) < 1) return 0;   // (more queries counted than there are)
+    if (n < 1) n = 1;
   }
   return (int)(n < cap ? n : cap);
 }
+__device__ __forceinline__ int tiles_of(const Kind& k, int keys) { return (keys + (1 << k.shift) - 1) >> k.shift; }
+__device__ __forceinline__ int units_of(const Kind& k, int keys) { return keys > 0 ? tiles_of(k, keys) + k.start : 0; }
 
+// One block: what the inputs hold is fetched at once and held in shared memory where it fits, since each
+// trip to memory, each barrier and each line of code takes its time here, and nothing else does.
+// (Sums are of whole numbers, so that the division of the work does not depend on their order.)
 __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const __grid_constant__ PlanArgs p) {
-  __shared__ int tmp[kPlanThreads / 32];
+  __shared__ int4 group_room[kPlanGroups];
+  __shared__ int unit_room[kPlanGroups], start_room[kPlanGroups + 1];
+  __shared__ int seen_room[kPlanRows], shared_room[kPlanRows];
+  __shared__ unsigned long long saved;
+  __shared__ int units[2];   // of the pieces and of the rest
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   constexpr int kWarps = kPlanThreads / 32;
   griddep_wait();
   griddep_launch_dependents();
+  const bool groups_here = p.groups <= kPlanGroups, rows_here = p.batch <= kPlanRows;
+  int4* by_group = groups_here ? group_room : p.by_group;
+  int* by_units = groups_here ? unit_room : p.by_units;
+  const int32_t* starts = groups_here ? start_room : p.starts;
+  if (tid == 0) {
+    saved = 0;
+    units[0] = units[1] = 0;
+  }
   bool bad = false;
-  for (int g = tid; g < p.groups; g += kPlanThreads) {
-    const int from = p.starts[g], to = p.starts[g + 1];
+#pragma unroll 1
+  for (int g = tid; g <= p.groups; g += kPlanThreads) {
+    const int from = p.starts[g], to = g < p.groups ? p.starts[g + 1] : from;
+    if (groups_here) start_room[g] = from;
     bad |= from < 0 || to < from || to > p.batch;
   }
-  for (int b = tid; b < p.batch; b += kPlanThreads) p.by_row[b] = make_int4(0, 0, 0, 0);
-  for (int i = tid; i < p.a.shared_items; i += kPlanThreads) p.items[i] = Item{};
+#pragma unroll 1
+  for (int b = tid; b < p.batch; b += kPlanThreads) {
+    if (rows_here) {
+      seen_room[b] = least_seen(p, b);
+      shared_room[b] = 0;
+    }
+    p.by_row[b] = make_int4(0, 0, 0, 0);
+  }
+#pragma unroll 1
+  for (int i = tid; i < p.most; i += kPlanThreads) p.pieces[i].keys = 0;
   const bool none = __syncthreads_or(bad);   // groups that are no division of the batch are not used
   if (none && tid == 0) report_error(p.a.error_flag, kErrBadIndex);
   const int groups = none ? 0 : p.groups;
+
+#pragma unroll 1
   for (int g = warp; g < groups; g += kWarps) {
-    const int from = p.starts[g], to = p.starts[g + 1];
+    const int from = starts[g], to = starts[g + 1], prefix = p.prefixes[g];
     int least = 0x7fffffff, rows = 0, lead = 0x7fffffff;
+#pragma unroll 1
     for (int b = from + lane; b < to; b += 32) {
-      const int n = least_seen(p, b);
+      const int n = rows_here ? seen_room[b] : least_seen(p, b);
       if (n == 0) continue;
       least = min(least, n);
       lead = min(lead, b);
@@ -80,70 +136,274 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const __grid_
     lead = __reduce_min_sync(0xffffffffu, lead);
     rows = __reduce_add_sync(0xffffffffu, rows);
     if (lane == 0) {
-      int keys = min(p.prefixes[g], least);
-      keys -= keys % p.a.page_size;
-      const int64_t tokens = (int64_t)(to - from) * p.s1;
-      const int items = (int)((tokens + p.a.per_item - 1) / p.a.per_item);
-      // (a row of the rest holds `packed` tokens; without fewer pieces than rows nothing is saved)
-      const bool shares = keys > 0 && rows > 1 && items < (int64_t)rows * (p.s1 / p.packed);
-      p.by_group[g] = shares ? make_int4(keys, items, lead, 0) : make_int4(0, 0, 0, 0);
+      const uint32_t some = max(min(prefix, least), 0);
+      const int keys = (int)(some - some % (uint32_t)p.a.page_size);
+      const uint32_t tokens = (uint32_t)(to - from) * p.s1, own = (uint32_t)rows * p.own_rows;
+      const int items = (int)((tokens + p.per_item - 1) / (uint32_t)p.per_item);
+      // shared where its pieces cost less than its keys do in its rows
+      const long long less = (long long)own * tiles_of(p.own, keys) * p.own.cost -
+                             (long long)items * units_of(p.prefix, keys) * (p.prefix.cost * p.prefix.sms);
+      by_group[g] = less > 0 ? make_int4(keys, items, lead, 0) : make_int4(0, 0, 0, 0);
+      if (less > 0) atomicAdd(&saved, (unsigned long long)less);
     }
   }
   __syncthreads();
-  int before = 0;
-  for (int g0 = 0; g0 < groups; g0 += kPlanThreads) {
-    const int g = g0 + tid, items = g < groups ? p.by_group[g].y : 0;
-    int sum;
-    const int at = before + block_scan<kPlanThreads>(items, tmp, &sum);
-    if (g < groups) p.by_group[g].w = at;
-    before += sum;
-    __syncthreads();
+  const int sharing = (long long)saved > p.least_saving ? groups : 0;
+  if (warp == 0) {
+    int pieces = 0, all = 0;
+#pragma unroll 1
+    for (int g0 = 0; g0 < sharing; g0 += 32) {
+      const int g = g0 + lane;
+      const int4 group = g < groups ? by_group[g] : make_int4(0, 0, 0, 0);
+      int n = group.y, u = n * units_of(p.prefix, group.x);
+      const int own_n = n, own_u = u;
+#pragma unroll 1
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, n, o), y = __shfl_up_sync(0xffffffffu, u, o);
+        if (lane >= o) n += x, u += y;
+      }
+      if (g < groups) {
+        by_group[g].w = pieces + n - own_n;
+        by_units[g] = all + u - own_u;
+      }
+      pieces += __shfl_sync(0xffffffffu, n, 31);
+      all += __shfl_sync(0xffffffffu, u, 31);
+    }
+    if (lane == 0) units[0] = all;
   }
-  for (int g = warp; g < groups; g += kWarps) {
-    const int4 group = p.by_group[g];
-    const int from = p.starts[g], to = p.starts[g + 1];
-    if (group.x == 0 || group.w + group.y > p.a.shared_items) continue;
+  __syncthreads();
+#pragma unroll 1
+  for (int g = warp; g < sharing; g += kWarps) {
+    const int4 group = by_group[g];
+    const int from = starts[g], to = starts[g + 1];
+    if (group.x == 0) continue;
     const int first = from * p.s1, tokens = (to - from) * p.s1;
+#pragma unroll 1
     for (int i = lane; i < group.y; i += 32) {
-      const int t = i * p.a.per_item;
-      p.items[group.w + i] = Item{group.x, 0, group.z, (first + t) * p.a.heads, min(p.a.per_item, tokens - t) * p.a.heads, 1};
+      const int t = i * p.per_item, at = group.w + i;
+      p.pieces[at] = Item{group.x, 0, group.z, (first + t) * p.a.heads, min(p.per_item, tokens - t) * p.a.heads, 1,
+                          at * p.nh, 0};
     }
-    for (int b = from + lane; b < to; b += 32) p.by_row[b] = make_int4(group.x, group.w, first, 0);
+#pragma unroll 1
+    for (int b = from + lane; b < to; b += 32) {
+      p.by_row[b] = make_int4(group.x, group.w, first, by_units[g]);
+      if (rows_here) shared_room[b] = group.x;
+    }
   }
   __syncthreads();
-  for (int r = tid; r < p.a.rows - p.a.shared_items; r += kPlanThreads) {
-    const int b = r / p.a.s1, n = token_keys(p.a, r), shared = n > 0 ? p.by_row[b].x : 0;
-    p.items[p.a.shared_items + r] = Item{n - shared, shared, b, r * p.a.n1, p.a.n1, shared > 0 || p.a.diag > 0};
+  int rest = 0;
+#pragma unroll 1
+  for (int r = tid; r < p.a.rows; r += kPlanThreads) {
+    const int b = r / p.a.s1, n = row_keys(p.a, r), shared = n > 0 ? rows_here ? shared_room[b] : p.by_row[b].x : 0;
+    p.rest[r] = Item{n - shared, shared, b, r * p.a.n1, p.a.n1, shared > 0 || p.a.diag > 0, r * p.a.n1, 0};
+    rest += units_of(p.own, n - shared);
+  }
+  rest = __reduce_add_sync(0xffffffffu, rest);
+  if (lane == 0 && rest) atomicAdd(&units[1], rest);
+  __syncthreads();
+  if (warp == 0) {
+    // so many multiprocessors for the pieces that both launches end as early as may be
+    const float a = (float)units[0] * p.prefix.cost, b = (float)units[1] * p.own.cost;
+    const int all = p.sms / p.prefix.sms;
+    float best = INFINITY;
+    int n = 0;
+#pragma unroll 1
+    for (int k = lane + 1; k <= all && a > 0.0f; k += 32) {
+      const int m = (p.sms - k * p.prefix.sms) / p.own.sms;
+      const float t = fmaxf(p.prefix.fixed + a / k, b > 0.0f ? p.own.fixed + b / max(m, 1) + (m < 1 ? a : 0.0f) : 0.0f);
+      if (t < best) best = t, n = k;
+    }
+#pragma unroll 1
+    for (int o = 16; o > 0; o >>= 1) {
+      const float t = __shfl_xor_sync(0xffffffffu, best, o);
+      const int k = __shfl_xor_sync(0xffffffffu, n, o);
+      if (t < best || (t == best && k < n)) best = t, n = k;
+    }
+    if (lane == 0) *p.limits = Limits{max(n, 1), max((p.sms - n * p.prefix.sms) / p.own.sms, 1), units[0], 0};
   }
 }
 
-// How a call is divided: heads that the kernel holds, tokens of a piece of a prefix, such pieces at
-// most, rows of the rest, and the workspace.
+// What the join takes of the pieces' launch: its parts, and which of them are a row's.
+struct SharedParts {
+  const float* ws_o;
+  const float4* ws_s;
+  const Limits* limits;
+  const int4* by_row;
+  int32_t shares, nh;   // shares of the launch, heads of a piece
+  Kind kind;
+  rotary::FastDiv n1, s1, heads, per_item;   // heads and tokens of a row, heads of a token, tokens of a piece
+};
+
+// Join a row's own parts, its group's, and the keys that only its later tokens see; zeros for a row
+// without keys.  As attn_paged_combine_kernel, but the statistics of 32 parts are fetched at a time, by
+// a lane each, and the first values with them.  kLanes threads take a (row, head): a block, in groups
+// that take parts of their own, or one such group.
+template <int D, int NH, int kCost, int kLanes, typename T>
+__global__ void __launch_bounds__(kJoinThreads)
+    attn_shared_join_kernel(const __grid_constant__ Args a, int grid, const __grid_constant__ SharedParts sp) {
+  using E = ElemTraits<T>;
+  constexpr bool kWide = kLanes == kJoinThreads;
+  constexpr int kCols = D / 4;                // threads of a part, a float4 each
+  constexpr int kGroups = kLanes / kCols;     // parts at a time
+  constexpr int kAhead = 4;                   // of a thread
+  __shared__ float4 part[kWide ? kGroups : 1][kWide ? D / 4 : 1];
+  griddep_wait();
+  griddep_launch_dependents();
+  const int64_t at = (int64_t)blockIdx.x * (kJoinThreads / kLanes) + threadIdx.x / kLanes;
+  if (at >= (int64_t)a.rows * a.n1) return;
+  const int row = (int)sp.n1.div((uint32_t)at), head = (int)at - row * a.n1, b = (int)sp.s1.div(row);
+  const int t = threadIdx.x % kLanes, grp = t / kCols, col = t % kCols, lane = threadIdx.x & 31;
+  T* out = static_cast<T*>(a.out) + at * D;
+  const int4 g = sp.by_row[b];
+  const Limits limits = *sp.limits;
+  const int first = a.ws_prefix[row], count = a.ws_prefix[row + 1] - first, all = a.ws_prefix[a.rows];
+  const int64_t cap = (int64_t)a.max_blocks * a.page_size, ak = a.act_k[b];
+  const int tokens = (int)sp.heads.div(a.n1), s = (int)sp.heads.div(head);   // of a packed row, and the one of this head
+  // keys from `common` on that this token sees beside the row's common ones; lane i looks up the i-th's page
+  const int common = (int)max((int64_t)0, min(cap, ak - a.diag));
+  const int late = a.diag > 0 ? (int)max((int64_t)common, min(cap, ak - a.diag + s)) - common : 0;
+  int late_page = -1;
+  if (lane < late) late_page = a.block_table[(int64_t)b * a.max_blocks + (common + lane) / a.page_size];
+  const int64_t seen = tokens == 1 ? token_keys(a, row) : min(cap, ak - a.diag + (a.diag > 0 ? s : 0));
+  // the row's own parts, then those of the piece of which it is head `head2`
+  Parts p{1, 0, 0, (int64_t)2 * grid * NH + (int64_t)row * a.n1}, p2{1, 0, 0, 0};
+  int head2 = 0;
+  if (count > 0) find_parts(first, count, all, kCost, min(grid, limits.rest_shares), &p);
+  if (g.x > 0 && seen > 0) {
+    const int token = row * tokens + s - g.z, item = (int)sp.per_item.div(token), units = units_of(sp.kind, g.x);
+    head2 = (token - item * (int)sp.per_item.d) * a.heads + head - s * a.heads;
+    p2.own = (int64_t)(2 * sp.shares + g.y + item) * sp.nh;
+    find_parts(g.w + item * units, units, limits.units, sp.kind.start, min(sp.shares, limits.shares), &p2);
+  }
+  const int n1 = p.c1 - p.c0 + 1, n = n1 + p2.c1 - p2.c0 + 1;
+  if (a.diag == 0 && n == 1 && n1 == 1 && p.c0 == p.c1 && g.x == 0) return;   // written whole
+  if (n == 0 && late == 0) {
+    if (grp == 0) *reinterpret_cast<uint2*>(out + col * 4) = make_uint2(0, 0);
+    if (t == 0 && a.softmax_max) a.softmax_max[at] = a.softmax_sum[at] = 0.0f;
+    return;
+  }
+  float ref = -INFINITY, run = -INFINITY, top = -INFINITY, sum = 0.0f;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+  for (int k0 = 0; k0 < n; k0 += 32) {
+    const int m = min(32, n - k0);
+    auto place = [&](int k) { return k < n1 ? p.at(p.c0 + k, head, NH) : p2.at(p2.c0 + k - n1, head2, sp.nh); };
+    auto value = [&](int k) {
+      return reinterpret_cast<const float4*>((k < n1 ? a.ws_o : sp.ws_o) + place(k) * D)[col];
+    };
+    float4 st = make_float4(-INFINITY, -INFINITY, 0.0f, -INFINITY);
+    if (lane < m) st = (k0 + lane < n1 ? a.ws_s : sp.ws_s)[place(k0 + lane)];
+    float4 v[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (grp + j * kGroups < m) v[j] = value(k0 + grp + j * kGroups);
+    float now = st.x, all_run = st.y, all_top = st.w;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, o));
+      all_run = fmaxf(all_run, __shfl_xor_sync(0xffffffffu, all_run, o));
+      all_top = fmaxf(all_top, __shfl_xor_sync(0xffffffffu, all_top, o));
+    }
+    now = fmaxf(now, ref);
+    run = fmaxf(run, all_run);
+    top = fmaxf(top, all_top);
+    const float f = ref == now ? 1.0f : exp2f(ref - now), w = st.x == now ? 1.0f : exp2f(st.x - now);
+    ref = now;
+    float more = lane < m ? w * st.z : 0.0f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) more += __shfl_xor_sync(0xffffffffu, more, o);
+    sum = sum * f + more;
+    acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
+#pragma unroll 1
+    for (int j0 = 0; j0 < m; j0 += kAhead * kGroups) {   // (the same turns for every lane)
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const int k = j0 + grp + j * kGroups;
+        const float wk = __shfl_sync(0xffffffffu, w, k & 31);
+        if (k >= m) continue;
+        acc.x += wk * v[j].x, acc.y += wk * v[j].y, acc.z += wk * v[j].z, acc.w += wk * v[j].w;
+        if (k + kAhead * kGroups < m) v[j] = value(k0 + k + kAhead * kGroups);
+      }
+    }
+  }
+  if constexpr (kWide) {
+    part[grp][col] = acc;
+    __syncthreads();
+    if (grp > 0) return;   // (whole warps)
+#pragma unroll
+    for (int k = 1; k < kGroups; ++k) {
+      const float4 o = part[k][col];
+      acc.x += o.x, acc.y += o.y, acc.z += o.z, acc.w += o.w;
+    }
+  }
+#pragma unroll 1
+  for (int i = 0; i < late; ++i) {
+    const int page = __shfl_sync(0xffffffffu, late_page, i);
+    if (page >= a.num_pages && lane == 0) report_error(a.error_flag, kErrBadIndex);
+    if (page < 0 || page >= a.num_pages) continue;
+    const T* key;
+    const float dot = late_dot<D, T>(a, b, head, page, (common + i) % a.page_size, lane, &key);
+    const uint2 x = *reinterpret_cast<const uint2*>(key + col * 4);
+    const float raw = a.scale < 0.0f ? -dot : dot, z = dot * a.scale * 1.4426950408889634f;
+    // (a score of -inf with none above it weighs nothing, as in the kernels)
+    const float now = fmaxf(ref, z), f = ref == now ? 1.0f : exp2f(ref - now);
+    const float w = z == -INFINITY ? 0.0f : exp2f(z - now);
+    ref = now;
+    run = fmaxf(run, z);
+    top = fmaxf(top, raw);
+    sum = sum * f + w;
+    const T* e = reinterpret_cast<const T*>(&x);
+    acc.x = fmaf(w, E::to_f(e[0]), acc.x * f), acc.y = fmaf(w, E::to_f(e[1]), acc.y * f);
+    acc.z = fmaf(w, E::to_f(e[2]), acc.z * f), acc.w = fmaf(w, E::to_f(e[3]), acc.w * f);
+  }
+  const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+  *reinterpret_cast<uint2*>(out + col * 4) = make_uint2(E::pack2(acc.x * inv, acc.y * inv), E::pack2(acc.z * inv, acc.w * inv));
+  if (t == 0 && a.softmax_max) put_stats(a, at, top, ref, run, sum);
+}
+
+// How a call is divided: heads that either launch's kernel holds, tokens of a piece of a prefix, such
+// pieces at most, rows of the rest, and the workspace.
 struct Layout {
-  int nh, packed;
-  int64_t per_item, shared_items, rest, shares, places;
+  int nh, own_nh, packed;
+  int64_t per_item, most, rest, shares, own_shares, places, own_places;
+  int64_t lists(int64_t batch, int64_t groups) const {   // bytes of what the plan makes
+    return align256((most + rest) * (int64_t)sizeof(Item)) + align256((batch + groups) * 16 + groups * 4) + 256;
+  }
   int64_t bytes(int64_t d, int64_t batch, int64_t groups) const {
-    return align256(places * (d * 4 + 16) + (shared_items + rest + 1) * 4) +
-           align256((shared_items + rest) * (int64_t)sizeof(Item)) + align256((batch + groups) * 16);
+    return align256((places + own_places) * (d * 4 + 16) + (most + rest + 2) * 4) + lists(batch, groups);
   }
 };
 
 Layout layout_of(int64_t batch, int64_t s1, int64_t n1, int64_t d, int64_t groups, bool packed) {
   Layout l;
   l.packed = packed ? (int)s1 : 1;
-  // as many heads as a group has on the average: 64 of them, or 128
+  // pieces of 128 heads where a group has more than 64 on the average
   const int64_t own = n1 * l.packed, mean = (batch + groups - 1) / groups * s1 * n1;
-  l.nh = heads_of(mean > 128 ? 128 : mean > own ? mean : own);
+  l.nh = mean > 64 || own > 32 ? 128 : 64;
+  l.own_nh = heads_of(own);
   l.per_item = l.nh / n1;
   l.rest = packed ? batch : batch * s1;
-  l.shared_items = batch * s1 / l.per_item + (groups < batch / 2 ? groups : batch / 2);
-  l.shares = l.nh == 128 && d == 512 ? sm_count() / 2 : sm_count();
-  l.places = (2 * l.shares + l.shared_items) * l.nh + batch * s1 * n1;
+  l.most = batch * s1 / l.per_item + (groups < batch ? groups : batch);
+  auto shares = [&](int nh) { return nh == 128 && d == 512 ? sm_count() / 2 : sm_count(); };
+  l.shares = shares(l.nh);
+  l.own_shares = shares(l.own_nh);
+  l.places = (2 * l.shares + l.most) * l.nh;
+  l.own_places = 2 * l.own_shares * l.own_nh + batch * s1 * n1;
   return l;
 }
 
 // Whether pieces of a prefix can hold more tokens than a row of the rest does.
 bool can_share(const Layout& l) { return l.per_item > l.packed; }
+
+// The kernel for `nh` heads: a unit's cost (a tile's) and that of a share's start and end, in cycles, as
+// measured with keys that lie in L2.
+Kind kind_of(int nh, int64_t d) {
+  if (nh == 128 && d == 512) return {7, pair::kSegmentCost, 2, 4200, 15000};
+  if (nh == 128) return {6, wide::kSegmentCost, 1, d == 256 ? 2200 : 1850, 12000};
+  const int cost = d == 512 ? (nh == 64 ? 3800 : nh == 32 ? 3000 : 2600) : d == 256 ? (nh == 64 ? 3000 : 2300) : 1900;
+  return {6, kSegmentCost, 1, cost, 14000};
+}
+static_assert(pair::kTile == 128 && wide::kTile == 64 && kTile == 64, "kind_of has the tiles' sizes");
 
 // The step from one head to the next of all tokens' (a dim of size 1 has none of its own), and whether
 // they lie as rows of one matrix.
@@ -155,49 +415,31 @@ bool one_matrix(const DsaAttnPagedParams* p, int64_t head, int64_t token, int64_
   return (p->s1 == 1 || token == p->n1 * step) && (p->batch == 1 || batch == p->s1 * p->n1 * step);
 }
 
+// The kernel for `nh` heads over the pieces of `a`; `flat`: the queries as one matrix of rows.
 template <int D, typename T>
-int launch_items(const DsaAttnPagedParams* p, const Layout& l, const ItemArgs& a, const DsaAttnPagedParams* rest,
-                 cudaStream_t stream) {
+int launch_pieces(const DsaAttnPagedParams* flat, int nh, int shares, const ItemArgs& a, cudaStream_t stream) {
   constexpr bool kBf16 = ElemTraits<T>::kIsBf16;
-  // every token's heads as one matrix of rows
-  DsaAttnPagedParams flat = *p;
-  flat.n1 = p->batch * p->s1 * p->n1;
-  flat.s1 = flat.batch = 1;
-  flat.q_head_stride = flat.q_token_stride = flat.q_batch_stride =
-      row_step(p, p->q_head_stride, p->q_token_stride, p->q_batch_stride);
-  flat.qr_head_stride = flat.qr_token_stride = flat.qr_batch_stride =
-      row_step(p, p->qr_head_stride, p->qr_token_stride, p->qr_batch_stride);
   Maps maps;
-  auto go = [&](auto kern, int blocks, int threads, int smem, const auto&... more) {
+  auto go = [&](auto kern, int blocks, int threads, int smem, const auto&... more) -> int {
     return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess &&
-           launch_early(kern, blocks, threads, smem, stream, maps, more..., a);
+                   launch_early(kern, blocks, threads, smem, stream, maps, more..., a)
+               ? DSA_OK : DSA_ERR_CUDA;
   };
-  auto small = [&](auto nh) {
-    constexpr int NH = decltype(nh)::value;
-    if (!make_maps<D>(&maps, &flat, kBf16, NH)) return DSA_ERR_TMA_DESCRIPTOR;
-    if (!go(attn_paged_kernel<D, NH, T, ItemArgs>, (int)l.shares, kThreads, Cfg<D, NH>::kSmem)) return DSA_ERR_CUDA;
-    return launch_join<D, NH, kSegmentCost, T>(rest, a, (int)l.shares, stream);
-  };
-  if (l.nh == 16) return small(std::integral_constant<int, 16>());
-  if (l.nh == 32) return small(std::integral_constant<int, 32>());
-  if (l.nh == 64) return small(std::integral_constant<int, 64>());
+  if (!(nh == 128 && D == 512) && !make_maps<D>(&maps, flat, kBf16, nh)) return DSA_ERR_TMA_DESCRIPTOR;
+  if (nh == 16) return go(attn_paged_kernel<D, 16, T, ItemArgs>, shares, kThreads, Cfg<D, 16>::kSmem);
+  if (nh == 32) return go(attn_paged_kernel<D, 32, T, ItemArgs>, shares, kThreads, Cfg<D, 32>::kSmem);
+  if (nh == 64) return go(attn_paged_kernel<D, 64, T, ItemArgs>, shares, kThreads, Cfg<D, 64>::kSmem);
   if constexpr (D == 512) {
     using C = pair::Cfg<D>;
     CUtensorMap map_v;
-    if (!make_maps<D>(&maps, &flat, kBf16, pair::kHeads) || !make_value_map<D>(&map_v, p, kBf16, C::kVChunks))
-      return DSA_ERR_TMA_DESCRIPTOR;
-    if (!go(pair::attn_paged_pair_kernel<D, T, ItemArgs>, 2 * (int)l.shares, pair::kThreads, C::kSmem, map_v))
-      return DSA_ERR_CUDA;
-    return launch_join<D, 2 * pair::kHeads, pair::kSegmentCost, T>(rest, a, (int)l.shares, stream);
+    if (!make_pair_maps<D>(&maps, &map_v, flat, kBf16, pair::kHeads)) return DSA_ERR_TMA_DESCRIPTOR;
+    return go(pair::attn_paged_pair_kernel<D, T, ItemArgs>, 2 * shares, pair::kThreads, C::kSmem, map_v);
   } else {
-    if (!make_maps<D>(&maps, &flat, kBf16, wide::kHeads)) return DSA_ERR_TMA_DESCRIPTOR;
-    if (!go(wide::attn_paged_wide_kernel<D, T, ItemArgs>, (int)l.shares, wide::kThreads, wide::Cfg<D>::kSmem))
-      return DSA_ERR_CUDA;
-    return launch_join<D, wide::kHeads, wide::kSegmentCost, T>(rest, a, (int)l.shares, stream);
+    return go(wide::attn_paged_wide_kernel<D, T, ItemArgs>, shares, wide::kThreads, wide::Cfg<D>::kSmem);
   }
 }
 
-template <typename T>
+template <int D, typename T>
 int launch_shared(const DsaAttnSharedParams* sp, const Layout& l, cudaStream_t stream) {
   const DsaAttnPagedParams* p = &sp->attn;
   // the rest, as dsa_attn_paged would take it
@@ -209,33 +451,78 @@ int launch_shared(const DsaAttnSharedParams* sp, const Layout& l, cudaStream_t s
     rest.s1 = 1;
     diag = p->sparse_mode == 3 ? (int)p->s1 - 1 : 0;
   }
+  DsaAttnPagedParams flat = *p;
+  flat.n1 = p->batch * p->s1 * p->n1;
+  flat.s1 = flat.batch = 1;
+  flat.q_head_stride = flat.q_token_stride = flat.q_batch_stride =
+      row_step(p, p->q_head_stride, p->q_token_stride, p->q_batch_stride);
+  flat.qr_head_stride = flat.qr_token_stride = flat.qr_batch_stride =
+      row_step(p, p->qr_head_stride, p->qr_token_stride, p->qr_batch_stride);
+
+  ItemArgs own, pre;
+  static_cast<Args&>(own) = static_cast<Args&>(pre) = make_args(&rest, diag, (int)p->n1);
+  own.rows = (int)l.rest;
+  pre.rows = (int)l.most;
+  float* o = static_cast<float*>(p->workspace);
+  pre.ws_o = o, own.ws_o = o + l.places * D;
+  float4* st = reinterpret_cast<float4*>(o + (l.places + l.own_places) * D);
+  pre.ws_s = st, own.ws_s = st + l.places;
+  pre.ws_prefix = reinterpret_cast<int32_t*>(st + l.places + l.own_places);
+  own.ws_prefix = pre.ws_prefix + l.most + 1;
+  uint8_t* ws = static_cast<uint8_t*>(p->workspace) + align256((l.places + l.own_places) * (D * 4 + 16) + (l.most + l.rest + 2) * 4);
   PlanArgs plan;
-  static_cast<Args&>(plan.a) = make_args(&rest, diag, (int)p->n1);
-  ItemArgs& a = plan.a;
-  a.shared_items = (int)l.shared_items;
-  a.per_item = (int)l.per_item;
-  a.rows = (int)(l.shared_items + l.rest);
-  uint8_t* ws = static_cast<uint8_t*>(p->workspace);
-  a.ws_o = reinterpret_cast<float*>(ws);
-  a.ws_s = reinterpret_cast<float4*>(ws + l.places * p->d * 4);
-  a.ws_prefix = reinterpret_cast<int32_t*>(ws + l.places * (p->d * 4 + 16));
-  ws += align256(l.places * (p->d * 4 + 16) + (l.shared_items + l.rest + 1) * 4);
-  plan.items = reinterpret_cast<Item*>(ws);
-  a.items = plan.items;
-  ws += align256((l.shared_items + l.rest) * (int64_t)sizeof(Item));
-  plan.by_row = reinterpret_cast<int4*>(ws);
-  a.groups = plan.by_row;
+  plan.limits = reinterpret_cast<Limits*>(ws);
+  plan.pieces = reinterpret_cast<Item*>(ws + 256);
+  plan.rest = plan.pieces + l.most;
+  plan.by_row = reinterpret_cast<int4*>(ws + 256 + align256((l.most + l.rest) * (int64_t)sizeof(Item)));
   plan.by_group = plan.by_row + p->batch;
+  plan.by_units = reinterpret_cast<int32_t*>(plan.by_group + sp->groups);
+  pre.items = plan.pieces, pre.limit = &plan.limits->shares, pre.second = false;
+  own.items = plan.rest, own.limit = &plan.limits->rest_shares, own.second = true;
+  plan.a = own;
   plan.starts = sp->group_starts;
   plan.prefixes = sp->prefix_lengths;
   plan.groups = (int)sp->groups;
   plan.batch = (int)p->batch;
   plan.s1 = (int)p->s1;
   plan.packed = l.packed;
+  plan.own_rows = (int)p->s1 / l.packed;
+  plan.most = (int)l.most;
+  plan.per_item = (int)l.per_item;
+  plan.nh = l.nh;
+  plan.sms = sm_count();
+  plan.prefix = kind_of(l.nh, D);
+  plan.own = kind_of(l.own_nh, D);
+  plan.least_saving = sp->least_saving;
   if (!launch_early(shared_plan_kernel, 1, kPlanThreads, 0, stream, plan)) return DSA_ERR_CUDA;
-  if (p->d == 512) return launch_items<512, T>(p, l, a, &rest, stream);
-  if (p->d == 256) return launch_items<256, T>(p, l, a, &rest, stream);
-  if (p->d == 128) return launch_items<128, T>(p, l, a, &rest, stream);
+  int rc = launch_pieces<D, T>(&flat, l.nh, (int)l.shares, pre, stream);
+  if (rc == DSA_OK) rc = launch_pieces<D, T>(&flat, l.own_nh, (int)l.own_shares, own, stream);
+  if (rc != DSA_OK) return rc;
+  const SharedParts parts{pre.ws_o, pre.ws_s, plan.limits, plan.by_row, (int)l.shares, l.nh, plan.prefix,
+                          rotary::FastDiv((uint32_t)own.n1), rotary::FastDiv((uint32_t)own.s1),
+                          rotary::FastDiv((uint32_t)own.heads), rotary::FastDiv((uint32_t)l.per_item)};
+  auto join = [&](auto nh, auto cost) -> int {
+    constexpr int NH = decltype(nh)::value, kCost = decltype(cost)::value;
+    const int64_t items = (int64_t)own.rows * own.n1;
+    const bool block = items <= 2LL * sm_count();   // (few rows are split into many parts each)
+    const int each = block ? kJoinThreads : D / 4;
+    auto kern = block ? attn_shared_join_kernel<D, NH, kCost, kJoinThreads, T> : attn_shared_join_kernel<D, NH, kCost, D / 4, T>;
+    return launch_early(kern, (items * each + kJoinThreads - 1) / kJoinThreads, kJoinThreads, 0, stream,
+                        static_cast<const Args&>(own), (int)l.own_shares, parts) ? DSA_OK : DSA_ERR_CUDA;
+  };
+  using std::integral_constant;
+  if (l.own_nh == 16) return join(integral_constant<int, 16>(), integral_constant<int, kSegmentCost>());
+  if (l.own_nh == 32) return join(integral_constant<int, 32>(), integral_constant<int, kSegmentCost>());
+  if (l.own_nh == 64) return join(integral_constant<int, 64>(), integral_constant<int, kSegmentCost>());
+  static_assert(pair::kSegmentCost == wide::kSegmentCost, "a join for both");
+  return join(integral_constant<int, 128>(), integral_constant<int, pair::kSegmentCost>());
+}
+
+template <typename T>
+int launch_shared_dim(const DsaAttnSharedParams* sp, const Layout& l, cudaStream_t stream) {
+  if (sp->attn.d == 512) return launch_shared<512, T>(sp, l, stream);
+  if (sp->attn.d == 256) return launch_shared<256, T>(sp, l, stream);
+  if (sp->attn.d == 128) return launch_shared<128, T>(sp, l, stream);
   return DSA_ERR_INVALID_ARG;
 }
 
@@ -264,21 +551,25 @@ extern "C" int dsa_attn_shared(const DsaAttnSharedParams* sp, void* stream_) {
   const DsaAttnPagedParams* p = &sp->attn;
   if (p->batch == 0 || p->s1 == 0) return DSA_OK;
   constexpr int64_t kMax = 0x7fffffff;
-  if (!valid_params(p, kTile) || sp->groups > kMax || (sp->groups > 0 && (!sp->group_starts || !sp->prefix_lengths)) ||
+  if (!valid_params(p, kTile) || sp->groups > kMax || sp->least_saving < 0 || (sp->groups > 0 && (!sp->group_starts || !sp->prefix_lengths)) ||
       p->workspace_bytes < dsa_attn_shared_workspace_size(p->batch, p->s1, p->n1, p->d, sp->groups))
     return DSA_ERR_INVALID_ARG;
   if (sp->groups > 0) {
     const Layout l = layout_of(p->batch, p->s1, p->n1, p->d, sp->groups, packs(p->s1, p->n1) && !p->act_q);
-    if (can_share(l)) {
+    const Kind own = kind_of(l.own_nh, p->d);
+    const double all = (double)l.rest * ((p->max_blocks * p->page_size >> own.shift) + 1) * own.cost * own.sms;
+    if (can_share(l) && all > (double)sp->least_saving) {   // (what the tables can hold costs more than that)
       const int64_t tiles = (p->max_blocks * p->page_size + kTile - 1) / kTile + 8;
       if (!one_matrix(p, p->q_head_stride, p->q_token_stride, p->q_batch_stride) ||
           !one_matrix(p, p->qr_head_stride, p->qr_token_stride, p->qr_batch_stride) ||
-          l.shared_items + l.rest > kMax / tiles || l.shares < 1)
+          l.most + l.rest > kMax / tiles || l.shares < 1 ||
+          l.most * l.nh > kMax)
         return DSA_ERR_INVALID_ARG;
-      if (p->dtype == DSA_DTYPE_BF16) return launch_shared<__nv_bfloat16>(sp, l, static_cast<cudaStream_t>(stream_));
-      if (p->dtype == DSA_DTYPE_FP16) return launch_shared<__half>(sp, l, static_cast<cudaStream_t>(stream_));
+      if (p->dtype == DSA_DTYPE_BF16) return launch_shared_dim<__nv_bfloat16>(sp, l, static_cast<cudaStream_t>(stream_));
+      if (p->dtype == DSA_DTYPE_FP16) return launch_shared_dim<__half>(sp, l, static_cast<cudaStream_t>(stream_));
       return DSA_ERR_INVALID_ARG;
     }
   }
-  return dsa_attn_paged(p, stream_);   // a token's heads fill a piece, or there is no group: nothing to share
+  // a token's heads fill a piece, there is no group, or the call is too small: nothing to share
+  return dsa_attn_paged(p, stream_);
 }

@@ -25,7 +25,7 @@
 
 namespace {
 
-enum Op { kAttn, kRotary, kAppend, kUpkeep, kOps };
+enum Op { kAttn, kRotary, kAppend, kUpkeep, kShared, kAxes, kPlan, kStore, kOps };
 
 typedef int (*Entry)(const void*, void*);
 Entry g_entry[kOps];
@@ -33,8 +33,8 @@ PyObject* g_check;                        // raises for a code that is not DSA_O
 std::unordered_map<int, int*> g_report;   // report flag of each device
 
 struct Plan {
-  std::string params, extra;   // the struct; upkeep: the array of caches, attention: which of
-                               // query and query_rope are copied first
+  std::string params, extra;   // the struct; upkeep: the array of caches, attention (with a shared
+                               // prefix, too): which of query and query_rope are copied first
   int64_t ws_bytes;
 };
 std::unordered_map<std::string, Plan> g_plans[kOps];
@@ -111,7 +111,7 @@ uint64_t at_of(const at::Tensor* t) { return reinterpret_cast<uint64_t>(t->data_
 template <typename T>
 T* ptr(const at::Tensor* t) { return t ? static_cast<T*>(t->data_ptr()) : nullptr; }
 
-// What the signatures of the four operators are made of; false when the Python path has to look.
+// What the signatures of the operators are made of; false when the Python path has to look.
 struct AttnArgs {
   Key key;
   const at::Tensor *q, *qr, *k, *kr, *table, *act_k, *act_q;
@@ -125,6 +125,13 @@ struct AttnArgs {
     key.real(PyFloat_AS_DOUBLE(a[7]));
     stats = a[9] == Py_True;
     return true;
+  }
+};
+struct SharedArgs : AttnArgs {
+  const at::Tensor *starts, *prefixes;
+  bool read(PyObject* const* a) {
+    return AttnArgs::read(a) && maybe_tensor(a[10], key, &starts) && maybe_tensor(a[11], key, &prefixes) && starts &&
+           prefixes;
   }
 };
 struct RotaryArgs {
@@ -143,6 +150,52 @@ struct RotaryArgs {
     key.text(layout, n);
     key.number((a[5] == Py_True ? 1 : 0) + (a[6] == a[0] ? 2 : 0));
     return (a[5] == Py_True || a[5] == Py_False) && (a[6] == Py_None || a[6] == a[0]);
+  }
+};
+struct AxesArgs {
+  Key key;
+  const at::Tensor *x, *table, *positions;
+  bool read(PyObject* const* a) {
+    if (!maybe_tensor(a[0], key, &x) || !maybe_tensor(a[1], key, &table) || !maybe_tensor(a[2], key, &positions) ||
+        !x || !table || !positions || !PyTuple_Check(a[3]) || !number(a[6], key))
+      return false;
+    const Py_ssize_t axes = PyTuple_GET_SIZE(a[3]);
+    key.list(axes);
+    for (Py_ssize_t i = 0; i < axes; ++i)
+      if (!number(PyTuple_GET_ITEM(a[3], i), key)) return false;
+    for (int i = 4; i < 6; ++i) {   // layout, order
+      Py_ssize_t n;
+      const char* s = PyUnicode_Check(a[i]) ? PyUnicode_AsUTF8AndSize(a[i], &n) : nullptr;
+      if (!s) {
+        PyErr_Clear();
+        return false;
+      }
+      key.text(s, n);
+    }
+    key.number((a[7] == Py_True ? 1 : 0) + (a[8] == a[0] ? 2 : 0));
+    return (a[7] == Py_True || a[7] == Py_False) && (a[8] == Py_None || a[8] == a[0]);
+  }
+};
+struct PlanArgs {
+  Key key;
+  const at::Tensor* in[4];   // block_table, seq_lengths, rows, counts
+  int64_t num_tokens;        // another one each step: not a part of the signature
+  bool read(PyObject* const* a) {
+    for (int i = 0; i < 4; ++i)
+      if (!maybe_tensor(a[i], key, &in[i]) || !in[i]) return false;
+    if (!number(a[4], key) || !number(a[6], key) || !number(a[7], key) || !PyLong_Check(a[5])) return false;
+    int over = 0;
+    num_tokens = PyLong_AsLongLongAndOverflow(a[5], &over);
+    return !over && num_tokens >= 0 && num_tokens <= 0x7fffffff;
+  }
+};
+struct StoreArgs {
+  Key key;
+  std::vector<const at::Tensor*> tokens, caches;
+  const at::Tensor* slots;
+  bool read(PyObject* const* a) {
+    return tensors_of(a[0], key, tokens) && tensors_of(a[1], key, caches) && maybe_tensor(a[2], key, &slots) && slots &&
+           tokens.size() == caches.size() && tokens.size() <= DSA_APPEND_MAX_ENTRIES && !tokens.empty();
   }
 };
 struct AppendArgs {
@@ -226,6 +279,46 @@ PyObject* guarded(F f) {
   END_HANDLE_TH_ERRORS
 }
 
+// A call of an attention operator, whose own parameters `fill` puts in; `p` is the attention's part of
+// them.  None where the Python path has to look.
+template <typename P, typename F>
+PyObject* attend(Op op, const char* name, const AttnArgs& a, const Plan& plan, int* report, P& params, DsaAttnPagedParams& p,
+                 F fill) {
+  const bool copy_q = plan.extra[0], copy_qr = plan.extra[1];
+  if (((copy_q ? 0 : at_of(a.q)) | (copy_qr ? 0 : at_of(a.qr)) | at_of(a.k) | at_of(a.kr)) % 16) Py_RETURN_NONE;
+  const at::Tensor q = copy_q ? a.q->clone(at::MemoryFormat::Contiguous) : *a.q;
+  const at::Tensor qr = copy_qr ? a.qr->clone(at::MemoryFormat::Contiguous) : *a.qr;
+  std::memcpy(&params, plan.params.data(), sizeof params);
+  fill();
+  const auto f32 = a.q->options().dtype(at::kFloat);
+  at::Tensor out = at::empty(a.q->sizes(), a.q->options());
+  const int64_t shape[4] = {p.batch, 1, p.s1, p.n1};
+  at::Tensor top = a.stats ? at::empty(shape, f32) : at::zeros(shape, f32);
+  at::Tensor sum = a.stats ? at::empty(shape, f32) : at::zeros(shape, f32);
+  at::Tensor ws = at::empty({plan.ws_bytes}, a.q->options().dtype(at::kByte));
+  p.query = q.data_ptr();
+  p.query_rope = qr.data_ptr();
+  p.key_cache = a.k->data_ptr();
+  p.key_rope_cache = a.kr->data_ptr();
+  p.block_table = ptr<const int32_t>(a.table);
+  p.act_k = ptr<const int32_t>(a.act_k);
+  p.act_q = ptr<const int32_t>(a.act_q);
+  p.out = out.data_ptr();
+  if (a.stats) {
+    p.softmax_max = ptr<float>(&top);
+    p.softmax_sum = ptr<float>(&sum);
+  }
+  p.error_flag = report;
+  p.workspace = ws.data_ptr();
+  if (!call(op, &params, *a.q, name)) return nullptr;
+  PyObject* r = PyTuple_New(3);
+  if (!r) return nullptr;
+  PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(out));
+  PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(top));
+  PyTuple_SET_ITEM(r, 2, THPVariable_Wrap(sum));
+  return r;
+}
+
 PyObject* attn(PyObject*, PyObject* const* argv, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     AttnArgs a;
@@ -233,39 +326,23 @@ PyObject* attn(PyObject*, PyObject* const* argv, Py_ssize_t n) {
     if (n != 10 || !a.read(argv)) Py_RETURN_NONE;
     const Plan* plan = find(kAttn, a.key, *a.q, &report);
     if (!plan) Py_RETURN_NONE;
-    const bool copy_q = plan->extra[0], copy_qr = plan->extra[1];
-    if (((copy_q ? 0 : at_of(a.q)) | (copy_qr ? 0 : at_of(a.qr)) | at_of(a.k) | at_of(a.kr)) % 16) Py_RETURN_NONE;
-    const at::Tensor q = copy_q ? a.q->clone(at::MemoryFormat::Contiguous) : *a.q;
-    const at::Tensor qr = copy_qr ? a.qr->clone(at::MemoryFormat::Contiguous) : *a.qr;
     DsaAttnPagedParams p;
-    std::memcpy(&p, plan->params.data(), sizeof p);
-    const auto f32 = a.q->options().dtype(at::kFloat);
-    at::Tensor out = at::empty(a.q->sizes(), a.q->options());
-    const int64_t shape[4] = {p.batch, 1, p.s1, p.n1};
-    at::Tensor top = a.stats ? at::empty(shape, f32) : at::zeros(shape, f32);
-    at::Tensor sum = a.stats ? at::empty(shape, f32) : at::zeros(shape, f32);
-    at::Tensor ws = at::empty({plan->ws_bytes}, a.q->options().dtype(at::kByte));
-    p.query = q.data_ptr();
-    p.query_rope = qr.data_ptr();
-    p.key_cache = a.k->data_ptr();
-    p.key_rope_cache = a.kr->data_ptr();
-    p.block_table = ptr<const int32_t>(a.table);
-    p.act_k = ptr<const int32_t>(a.act_k);
-    p.act_q = ptr<const int32_t>(a.act_q);
-    p.out = out.data_ptr();
-    if (a.stats) {
-      p.softmax_max = ptr<float>(&top);
-      p.softmax_sum = ptr<float>(&sum);
-    }
-    p.error_flag = report;
-    p.workspace = ws.data_ptr();
-    if (!call(kAttn, &p, *a.q, "dsa_attn_paged")) return nullptr;
-    PyObject* r = PyTuple_New(3);
-    if (!r) return nullptr;
-    PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(out));
-    PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(top));
-    PyTuple_SET_ITEM(r, 2, THPVariable_Wrap(sum));
-    return r;
+    return attend(kAttn, "dsa_attn_paged", a, *plan, report, p, p, [] {});
+  });
+}
+
+PyObject* shared(PyObject*, PyObject* const* argv, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    SharedArgs a;
+    int* report;
+    if (n != 12 || !a.read(argv)) Py_RETURN_NONE;
+    const Plan* plan = find(kShared, a.key, *a.q, &report);
+    if (!plan) Py_RETURN_NONE;
+    DsaAttnSharedParams p;
+    return attend(kShared, "dsa_attn_shared", a, *plan, report, p, p.attn, [&] {
+      p.group_starts = ptr<const int32_t>(a.starts);
+      p.prefix_lengths = ptr<const int32_t>(a.prefixes);
+    });
   });
 }
 
@@ -288,6 +365,89 @@ PyObject* rotary(PyObject*, PyObject* const* argv, Py_ssize_t n) {
     if (argv[6] == Py_None) return THPVariable_Wrap(out);
     Py_INCREF(argv[6]);
     return argv[6];
+  });
+}
+
+PyObject* axes(PyObject*, PyObject* const* argv, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    AxesArgs a;
+    int* report;
+    if (n != 9 || !a.read(argv)) Py_RETURN_NONE;
+    const Plan* plan = find(kAxes, a.key, *a.x, &report);
+    if (!plan) Py_RETURN_NONE;
+    DsaRotaryAxesParams p;
+    std::memcpy(&p, plan->params.data(), sizeof p);
+    at::Tensor out = argv[8] == Py_None ? at::empty(a.x->sizes(), a.x->options()) : *a.x;   // or in place
+    p.rotary.x = a.x->data_ptr();
+    p.rotary.out = out.data_ptr();
+    p.rotary.positions = ptr<const int32_t>(a.positions);
+    p.rotary.table = ptr<const float>(a.table);
+    p.rotary.error_flag = report;
+    if (!call(kAxes, &p, *a.x, "dsa_rotary_axes")) return nullptr;
+    if (argv[8] == Py_None) return THPVariable_Wrap(out);
+    Py_INCREF(argv[8]);
+    return argv[8];
+  });
+}
+
+// The eight tensors of a plan, as a tuple.
+PyObject* plan(PyObject*, PyObject* const* argv, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    PlanArgs a;
+    int* report;
+    if (n != 8 || !a.read(argv)) Py_RETURN_NONE;
+    const Plan* plan = find(kPlan, a.key, *a.in[0], &report);
+    if (!plan) Py_RETURN_NONE;
+    DsaBatchPlanParams p;
+    std::memcpy(&p, plan->params.data(), sizeof p);
+    p.num_tokens = a.num_tokens;
+    const auto i32 = a.in[0]->options(), i64 = i32.dtype(at::kLong);
+    at::Tensor out[8] = {at::empty({p.batch, p.max_blocks}, i32), at::empty({p.batch}, i32), at::empty({p.batch}, i32),
+                         at::empty({p.num_tokens}, i32), at::empty({p.num_tokens}, i32), at::empty({p.num_tokens}, i64),
+                         at::empty({p.max_groups + 1}, i32), at::empty({p.max_groups}, i32)};
+    at::Tensor ws = at::empty({plan->ws_bytes}, i32.dtype(at::kByte));
+    p.block_table = ptr<const int32_t>(a.in[0]);
+    p.seq_lengths = ptr<const int32_t>(a.in[1]);
+    p.rows = ptr<const int32_t>(a.in[2]);
+    p.counts = ptr<const int32_t>(a.in[3]);
+    p.block_table_out = ptr<int32_t>(&out[0]);
+    p.key_lengths = ptr<int32_t>(&out[1]);
+    p.query_ends = ptr<int32_t>(&out[2]);
+    p.token_rows = ptr<int32_t>(&out[3]);
+    p.positions = ptr<int32_t>(&out[4]);
+    p.slot_map = ptr<int64_t>(&out[5]);
+    p.group_starts = ptr<int32_t>(&out[6]);
+    p.prefix_lengths = ptr<int32_t>(&out[7]);
+    p.error_flag = report;
+    p.workspace = ws.data_ptr();
+    if (!call(kPlan, &p, *a.in[0], "dsa_batch_plan")) return nullptr;
+    PyObject* r = PyTuple_New(8);
+    if (!r) return nullptr;
+    for (int i = 0; i < 8; ++i) PyTuple_SET_ITEM(r, i, THPVariable_Wrap(out[i]));
+    return r;
+  });
+}
+
+PyObject* store(PyObject*, PyObject* const* argv, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    StoreArgs a;
+    int* report;
+    if (n != 3 || !a.read(argv)) Py_RETURN_NONE;
+    const Plan* plan = find(kStore, a.key, *a.caches[0], &report);
+    if (!plan) Py_RETURN_NONE;
+    DsaCacheStoreParams p;
+    std::memcpy(&p, plan->params.data(), sizeof p);
+    uint64_t low = 0;
+    for (size_t i = 0; i < a.tokens.size(); ++i) {
+      low |= at_of(a.tokens[i]) | at_of(a.caches[i]);
+      p.rows[i].src = a.tokens[i]->data_ptr();
+      p.rows[i].cache = a.caches[i]->data_ptr();
+    }
+    if (low % 16) Py_RETURN_NONE;
+    p.slots = ptr<const int64_t>(a.slots);
+    p.error_flag = report;
+    if (!call(kStore, &p, *a.caches[0], "dsa_cache_store")) return nullptr;
+    Py_RETURN_TRUE;
   });
 }
 
@@ -369,9 +529,11 @@ PyObject* keep(PyObject*, PyObject* const* argv, Py_ssize_t n) {
     if (PyErr_Occurred()) return nullptr;
     PyObject *params = argv[n - 3], *extra = argv[n - 2];
     if (op < 0 || op >= kOps || !PyBytes_Check(params) || !PyBytes_Check(extra)) Py_RETURN_FALSE;
-    static const Py_ssize_t kArgs[kOps] = {10, 7, 7, 8};
-    static const size_t kSize[kOps] = {sizeof(DsaAttnPagedParams), sizeof(DsaRotaryParams),
-                                       sizeof(DsaCacheAppendParams), sizeof(DsaPagesParams)};
+    static const Py_ssize_t kArgs[kOps] = {10, 7, 7, 8, 12, 9, 8, 3};
+    static const size_t kSize[kOps] = {sizeof(DsaAttnPagedParams),  sizeof(DsaRotaryParams),
+                                       sizeof(DsaCacheAppendParams), sizeof(DsaPagesParams),
+                                       sizeof(DsaAttnSharedParams), sizeof(DsaRotaryAxesParams),
+                                       sizeof(DsaBatchPlanParams),  sizeof(DsaCacheStoreParams)};
     if (n != kArgs[op] + 4 || (size_t)PyBytes_GET_SIZE(params) != kSize[op]) Py_RETURN_FALSE;
     Key key;
     bool ok = false;
@@ -379,6 +541,10 @@ PyObject* keep(PyObject*, PyObject* const* argv, Py_ssize_t n) {
     if (op == kAttn) { AttnArgs a; ok = a.read(argv + 1); key = a.key; more = 2; }
     if (op == kRotary) { RotaryArgs a; ok = a.read(argv + 1); key = a.key; }
     if (op == kAppend) { AppendArgs a; ok = a.read(argv + 1); key = a.key; }
+    if (op == kShared) { SharedArgs a; ok = a.read(argv + 1); key = a.key; more = 2; }
+    if (op == kAxes) { AxesArgs a; ok = a.read(argv + 1); key = a.key; }
+    if (op == kPlan) { PlanArgs a; ok = a.read(argv + 1); key = a.key; }
+    if (op == kStore) { StoreArgs a; ok = a.read(argv + 1); key = a.key; }
     if (op == kUpkeep) { UpkeepArgs a; ok = a.read(argv + 1); key = a.key; more = a.caches.size() * sizeof(DsaPageCache); }
     if (!ok || (size_t)PyBytes_GET_SIZE(extra) != more) Py_RETURN_FALSE;
     Plan plan;
@@ -392,12 +558,18 @@ PyObject* keep(PyObject*, PyObject* const* argv, Py_ssize_t n) {
   });
 }
 
-// connect(entry addresses of the four operators, check): called once
+// connect(entry addresses of the operators, in a tuple, check): called once
 PyObject* connect(PyObject*, PyObject* args) {
-  unsigned long long e[kOps];
-  PyObject* check;
-  if (!PyArg_ParseTuple(args, "KKKKO", &e[0], &e[1], &e[2], &e[3], &check)) return nullptr;
-  for (int i = 0; i < kOps; ++i) g_entry[i] = reinterpret_cast<Entry>(e[i]);
+  PyObject *entries, *check;
+  if (!PyArg_ParseTuple(args, "O!O", &PyTuple_Type, &entries, &check)) return nullptr;
+  if (PyTuple_GET_SIZE(entries) != kOps) {
+    PyErr_SetString(PyExc_ValueError, "connect: another number of entries");
+    return nullptr;
+  }
+  for (int i = 0; i < kOps; ++i) {
+    g_entry[i] = reinterpret_cast<Entry>(PyLong_AsUnsignedLongLong(PyTuple_GET_ITEM(entries, i)));
+    if (PyErr_Occurred()) return nullptr;
+  }
   Py_INCREF(check);
   g_check = check;
   Py_RETURN_NONE;
@@ -417,6 +589,10 @@ PyMethodDef g_methods[] = {
     {"rotary", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rotary)), METH_FASTCALL, nullptr},
     {"append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(append)), METH_FASTCALL, nullptr},
     {"upkeep", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(upkeep)), METH_FASTCALL, nullptr},
+    {"shared", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(shared)), METH_FASTCALL, nullptr},
+    {"axes", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(axes)), METH_FASTCALL, nullptr},
+    {"plan", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(plan)), METH_FASTCALL, nullptr},
+    {"store", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(store)), METH_FASTCALL, nullptr},
     {"keep", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(keep)), METH_FASTCALL, nullptr},
     {"connect", connect, METH_VARARGS, nullptr},
     {"set_report", set_report, METH_VARARGS, nullptr},

@@ -12,11 +12,13 @@ from __future__ import annotations
 import torch
 
 from . import _host as H
-from ._lib import (BIND_ATTN, AttnPagedParams, AttnSharedParams, binding, check, lib, remember,
+from ._lib import (BIND_ATTN, BIND_SHARED, AttnPagedParams, AttnSharedParams, binding, check, lib, remember,
                    report_ptr)
 
 _VALID_D = (128, 256, 512)
 _D_ROPE = 64
+# Cycles of one multiprocessor that sharing has to save, as it takes two launches more
+_LEAST_SAVING = 1500000
 _MAX_SCALE = torch.finfo(torch.float32).max
 
 
@@ -208,7 +210,7 @@ def _shared_plan(query, query_rope, key_cache, key_rope_cache, block_table, grou
                          f"got {group_starts.numel()}")
     p = AttnSharedParams()
     p.attn = AttnPagedParams.from_buffer_copy(template)
-    p.groups = groups
+    p.groups, p.least_saving = groups, _LEAST_SAVING
     B, S1, N1, D = query.shape
     # pieces of a prefix are runs of heads of neighbouring tokens; queries that lie otherwise are copied
     fits = []
@@ -253,8 +255,13 @@ def flash_attention_shared_prefix(
     64 heads a token fills a piece by itself and nothing is gained by sharing.  G should be near the
     number of groups: the pieces are of 128 heads where B * S1 * N1 / G exceeds 64.
     """
-    args = (query, query_rope, key_cache, key_rope_cache, block_table, group_starts, prefix_lengths,
-            actual_seq_lengths_key, actual_seq_lengths_query, float(scale_value), sparse_mode, bool(return_softmax_lse))
+    args = (query, query_rope, key_cache, key_rope_cache, block_table, actual_seq_lengths_key, actual_seq_lengths_query,
+            float(scale_value), sparse_mode, bool(return_softmax_lse), group_starts, prefix_lengths)
+    fast = binding()
+    if fast is not None:
+        done = fast.shared(*args)
+        if done is not None:
+            return done
     index = query.get_device()
     if index >= 0 and H.current_device() != index:
         with torch.cuda.device(index):
@@ -267,6 +274,8 @@ def flash_attention_shared_prefix(
     p = AttnSharedParams.from_buffer_copy(template)
     starts, prefixes = group_starts.contiguous(), prefix_lengths.contiguous()
     p.group_starts, p.prefix_lengths = starts.data_ptr(), prefixes.data_ptr()
-    done, as_given = _call(p, p.attn, lib().dsa_attn_shared, "dsa_attn_shared", (*args[:5], *args[7:9]),
-                           bool(return_softmax_lse), index, *plan[1:])
+    done, as_given = _call(p, p.attn, lib().dsa_attn_shared, "dsa_attn_shared", args[:7], bool(return_softmax_lse),
+                           index, *plan[1:])
+    if as_given and starts is group_starts and prefixes is prefix_lengths:
+        remember(BIND_SHARED, index, *args, template, bytes((not q_fits, not qr_fits)), ws_bytes)
     return done

@@ -23,7 +23,7 @@ from typing import NamedTuple
 import torch
 
 from . import _host as H
-from ._lib import (APPEND_MAX_ENTRIES, BIND_APPEND, BIND_UPKEEP, BatchPlanParams, CacheStoreParams, DSA_DTYPE_BF16, DSA_DTYPE_FP16, DSA_DTYPE_FP32, PAGES_COMPACT, PAGES_COPY,
+from ._lib import (APPEND_MAX_ENTRIES, BIND_APPEND, BIND_PLAN, BIND_STORE, BIND_UPKEEP, BatchPlanParams, CacheStoreParams, DSA_DTYPE_BF16, DSA_DTYPE_FP16, DSA_DTYPE_FP32, PAGES_COMPACT, PAGES_COPY,
                    PAGES_EXTEND, PAGES_FORK, PAGES_FREE, ROTARY_CODES, CacheAppendParams, PageCache,
                    PagesParams, binding, check, lib, ptr, remember, report_ptr)
 
@@ -369,6 +369,10 @@ def paged_cache_store(tokens, caches, slot_map):
     neither the tokens nor two caches share memory with rows that are written.
     """
     tokens, caches = list(tokens), list(caches)
+    args = (tokens, caches, slot_map)
+    fast = binding()
+    if fast is not None and fast.store(*args):
+        return caches
     template, copy = _store_plan(tokens, caches, slot_map)
     index = caches[0].get_device()
     if H.current_device() != index:
@@ -388,6 +392,8 @@ def paged_cache_store(tokens, caches, slot_map):
     p.slots = slots.data_ptr()
     p.error_flag = report_ptr(index)
     check(lib().dsa_cache_store(p, H.raw_stream(index)), "dsa_cache_store")
+    if not keep and slots is slot_map:
+        remember(BIND_STORE, index, *args, template, b"", 0)
     return caches
 
 
@@ -453,11 +459,17 @@ def paged_batch_plan(block_table, seq_lengths, rows, counts, page_size, num_toke
     if max_groups is None:
         max_groups = rows.numel()
     max_groups = int(max_groups)
-    template = _batch_plan(block_table, seq_lengths, rows, counts, page_size, num_tokens, max_groups, min_prefix)
+    args = (block_table, seq_lengths, rows, counts, page_size, num_tokens, max_groups, min_prefix)
+    fast = binding()
+    if fast is not None:
+        done = fast.plan(*args)
+        if done is not None:
+            return PagedBatchPlan(*done)
+    template = _batch_plan(*args)
     index = block_table.get_device()
     if H.current_device() != index:
         with torch.cuda.device(index):
-            return paged_batch_plan(block_table, seq_lengths, rows, counts, page_size, num_tokens, max_groups, min_prefix)
+            return paged_batch_plan(*args)
     p = BatchPlanParams.from_buffer_copy(template)
     given = [t.contiguous() for t in (block_table, seq_lengths, rows, counts)]
     p.block_table, p.seq_lengths, p.rows, p.counts = [t.data_ptr() for t in given]
@@ -465,11 +477,14 @@ def paged_batch_plan(block_table, seq_lengths, rows, counts, page_size, num_toke
     make = lambda *shape, dtype=torch.int32: torch.empty(shape, dtype=dtype, device=block_table.device)
     plan = PagedBatchPlan(make(batch, block_table.shape[1]), make(batch), make(batch), make(num_tokens), make(num_tokens),
                           make(num_tokens, dtype=torch.int64), make(max_groups + 1), make(max_groups))
-    ws = make(max(batch, 1))
+    ws_bytes = max(p.workspace_bytes, 4)
+    ws = make(ws_bytes, dtype=torch.uint8)
     p.block_table_out, p.key_lengths, p.query_ends = [t.data_ptr() for t in plan[:3]]
     p.token_rows, p.positions, p.slot_map = [t.data_ptr() for t in plan[3:6]]
     p.group_starts, p.prefix_lengths = [t.data_ptr() for t in plan[6:]]
     p.workspace = ws.data_ptr()
     p.error_flag = report_ptr(index)
     check(lib().dsa_batch_plan(p, H.raw_stream(index)), "dsa_batch_plan")
+    if all(a is b for a, b in zip(args, given)):
+        remember(BIND_PLAN, index, *args, template, b"", ws_bytes)
     return plan

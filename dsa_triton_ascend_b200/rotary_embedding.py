@@ -13,7 +13,7 @@ import math
 import torch
 
 from . import _host as H
-from ._lib import (BIND_ROTARY, DSA_DTYPE_FP32, ROTARY_MAX_AXES, RotaryAxesParams, RotaryParams, binding,
+from ._lib import (BIND_AXES, BIND_ROTARY, DSA_DTYPE_FP32, ROTARY_MAX_AXES, RotaryAxesParams, RotaryParams, binding,
                    check, lib, ptr, remember, report_ptr, stream_ptr)
 
 _MAX_DIM = 256
@@ -222,6 +222,11 @@ def rotary_embedding_axes(x, table, positions, sections, layout="interleaved", o
     """
     sections = tuple(sections) if isinstance(sections, (list, tuple)) else sections
     args = (x, table, positions, sections, layout, order, offset, bool(inverse), out)
+    fast = binding()
+    if fast is not None:
+        done = fast.axes(*args)
+        if done is not None:
+            return done
     template = _axes_plan(*args)
     index = x.get_device()
     if H.current_device() != index:
@@ -231,4 +236,6 @@ def rotary_embedding_axes(x, table, positions, sections, layout="interleaved", o
     out, as_given, keep = _fill(p.rotary, x, table, positions, out)
     p.rotary.error_flag = report_ptr(index)
     check(lib().dsa_rotary_axes(p, H.raw_stream(index)), "dsa_rotary_axes")
+    if as_given:
+        remember(BIND_AXES, index, *args, template, b"", 0)
     return out

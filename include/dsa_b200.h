@@ -461,9 +461,10 @@ int dsa_attn_paged_shares_keys(int64_t s1, int64_t n1);
  *   prefix_lengths[g] tokens are the same: their block_table rows name the same pages there, of
  *   which the whole ones that all rows with keys see are shared.  Rows outside all groups share nothing.
  * Group starts that are no such division are reported in error_flag, and nothing is shared.
- * n1 * (tokens that share a row's keys) heads of more than 64, or of a group all told, are taken 128
- * at a time; where a token has more than 64 heads nothing is shared.  Where something can be
- * (n1 <= 64), all heads of query and of query_rope lie one step apart, across tokens and rows.
+ * Where a token has more than 64 heads nothing is shared; where something can be, all heads of query
+ * and of query_rope lie one step apart, across tokens and rows.  A prefix is shared where that takes
+ * fewer cycles than its rows by themselves, and anything only where it saves more than least_saving
+ * (cycles of one multiprocessor, >= 0) altogether.
  * Workspace: dsa_attn_shared_workspace_size() bytes.
  */
 typedef struct DsaAttnSharedParams {
@@ -471,6 +472,7 @@ typedef struct DsaAttnSharedParams {
   const int32_t* group_starts;
   const int32_t* prefix_lengths;
   int64_t groups;
+  int64_t least_saving;
 } DsaAttnSharedParams;
 
 int dsa_attn_shared(const DsaAttnSharedParams* params, void* stream);

@@ -3,6 +3,7 @@
 The reference and its tolerances are those of flash_attention_paged (test_attn_paged_gpu.py): the
 join of a prefix's parts with a row's own is one more fp32 sum of the few that the 2^-18 there allows.
 """
+import importlib
 import math
 import random
 
@@ -10,9 +11,20 @@ import pytest
 import torch
 
 import dsa_triton_ascend_b200 as dsa
+from dsa_triton_ascend_b200 import _lib
 from test_attn_paged_gpu import Case, i32
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def small_calls_share(monkeypatch):
+    """Prefixes are shared however little that saves."""
+    module = importlib.import_module("dsa_triton_ascend_b200.flash_attention_paged")
+    monkeypatch.setattr(module, "_LEAST_SAVING", 0)
+    if _lib.binding() is not None:   # which keeps what a signature's first call decided
+        monkeypatch.setattr(module, "binding", lambda: None)
+        monkeypatch.setattr(module, "remember", lambda *a: None)
 
 
 class Shared(Case):
