@@ -9,8 +9,8 @@
 // Two launches.  plan_rows_kernel, over the whole GPU: some blocks write the tokens' lists (each
 // finds its tokens' requests by a scan of the counts of its own, up to the last it needs), the others
 // the block table's rows and how many pages each has in common with the row before it.
-// plan_groups_kernel, one block: lengths, ends and groups.  Bound by latency: a chain of dependent
-// loads (slot, length, page) and the second launch.
+// plan_groups_kernel, one block beside it: lengths and ends, then the groups.  Bound by latency: a chain of
+// dependent loads (slot, length, page) and the second launch.
 #include <cuda_runtime.h>
 
 #include "dsa_b200.h"
@@ -26,12 +26,13 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kTokens = 4 * kThreads;   // of a block
 constexpr int kRows = 1024;             // requests scanned at a time
 constexpr int kSpan = 256;              // table entries of a warp's turn
-constexpr int kGroupThreads = 1024;
+constexpr int kGroupThreads = 512;
 
 struct Args {
   DsaBatchPlanParams p;
   int32_t* common;   // [batch] pages shared with the row before
   int32_t token_blocks, spans;
+  bool alone;        // plan_groups_kernel, without plan_rows_kernel before it
 };
 
 struct Request {
@@ -190,42 +191,56 @@ __global__ void __launch_bounds__(kThreads) plan_rows_kernel(const __grid_consta
   }
 }
 
+// What does not hang on the comparisons is done while they are made: plan_rows_kernel has let this
+// kernel start after its own wait, so the inputs are there.
 __global__ void __launch_bounds__(kGroupThreads) plan_groups_kernel(const __grid_constant__ Args a) {
   const DsaBatchPlanParams& p = a.p;
   __shared__ int64_t tmp[kGroupThreads / 32];
+  __shared__ int32_t least_room[kGroupThreads];
   const int tid = threadIdx.x;
   constexpr int32_t kNone = 0x7fffffff;
-  griddep_wait();
-  for (int64_t g = tid; g < p.max_groups; g += kGroupThreads) p.prefix_lengths[g] = kNone;
   const int64_t least = p.min_prefix > p.page_size ? p.min_prefix : p.page_size;
-  int64_t tokens = 0, groups = 0;
+  // smallest prefix of each group, in shared memory where all requests are looked at together
+  const bool together = p.batch <= kGroupThreads;
+  int32_t* smallest = together ? least_room : p.prefix_lengths;
+  const int64_t listed = together ? kGroupThreads : p.max_groups;
+  if (a.alone) griddep_wait();
+  int64_t tokens = 0, groups = 0, total;
   bool bad = false;
+#pragma unroll 1
   for (int64_t b0 = 0; b0 < p.batch; b0 += kGroupThreads) {
     const int64_t b = b0 + tid;
-    const bool there = b < p.batch;
     Request q{0, 0, 0};
-    int64_t common = 0;
-    if (there) {
-      q = request_of(p, b, &bad);
-      common = a.common[b] * p.page_size;
-      p.key_lengths[b] = q.tokens;
-    }
-    int64_t total;
+    if (b < p.batch) q = request_of(p, b, &bad);
     const int64_t end = tokens + block_prefix<kGroupThreads>(q.count, tmp, &total);
-    if (there) p.query_ends[b] = (int32_t)end;
+    if (b < p.batch) {
+      p.key_lengths[b] = q.tokens;
+      p.query_ends[b] = (int32_t)end;
+    }
     tokens += total;
-    const bool first = there && (b == 0 || common < least);
-    const int64_t group = groups + block_prefix<kGroupThreads>(first, tmp, &total) - 1;
-    groups += total;
-    if (there && first && group <= p.max_groups) p.group_starts[group] = (int32_t)b;
-    if (there && !first && group < p.max_groups) atomicMin(p.prefix_lengths + group, (int32_t)common);
   }
+#pragma unroll 1
+  for (int64_t g = tid; g < listed; g += kGroupThreads) smallest[g] = kNone;
   if (tokens > p.num_tokens) bad = true;   // the last ones are not listed
   if (bad) report_error(p.error_flag, kErrBadIndex);
+  if (!a.alone) griddep_wait();
+#pragma unroll 1
+  for (int64_t b0 = 0; b0 < p.batch; b0 += kGroupThreads) {
+    const int64_t b = b0 + tid, common = b < p.batch ? a.common[b] * p.page_size : 0;
+    const bool first = b < p.batch && (b == 0 || common < least);
+    const int64_t group = groups + block_prefix<kGroupThreads>(first, tmp, &total) - 1;
+    groups += total;
+    if (first && group <= p.max_groups) p.group_starts[group] = (int32_t)b;
+    if (b < p.batch && !first && group < listed) atomicMin(smallest + group, (int32_t)common);
+  }
+#pragma unroll 1
   for (int64_t g = groups + tid; g <= p.max_groups; g += kGroupThreads) p.group_starts[g] = (int32_t)p.batch;
   __syncthreads();
-  for (int64_t g = tid; g < p.max_groups; g += kGroupThreads)
-    if (*const_cast<volatile int32_t*>(p.prefix_lengths + g) == kNone) p.prefix_lengths[g] = 0;
+#pragma unroll 1
+  for (int64_t g = tid; g < p.max_groups; g += kGroupThreads) {
+    const int32_t v = g < listed ? *const_cast<volatile int32_t*>(smallest + g) : kNone;
+    p.prefix_lengths[g] = v == kNone ? 0 : v;
+  }
 }
 
 // ---------------------------------------------------------------------------------------
@@ -319,7 +334,8 @@ extern "C" int dsa_batch_plan(const DsaBatchPlanParams* p, void* stream_) {
   const int64_t jobs = (p->batch * (a.spans + 1) + kWarps - 1) / kWarps, most = 8LL * sms;
   cfg.gridDim = dim3((unsigned)(a.token_blocks + (jobs < most ? jobs : most)));
   cfg.blockDim = dim3(kThreads);
-  if (cfg.gridDim.x > 0 && cudaLaunchKernelEx(&cfg, plan_rows_kernel, a) != cudaSuccess) return DSA_ERR_CUDA;
+  a.alone = cfg.gridDim.x == 0;
+  if (!a.alone && cudaLaunchKernelEx(&cfg, plan_rows_kernel, a) != cudaSuccess) return DSA_ERR_CUDA;
   cfg.gridDim = dim3(1);
   cfg.blockDim = dim3(kGroupThreads);
   return cudaLaunchKernelEx(&cfg, plan_groups_kernel, a) == cudaSuccess ? DSA_OK : DSA_ERR_CUDA;
