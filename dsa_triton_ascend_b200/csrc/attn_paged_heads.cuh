@@ -139,6 +139,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (base & 1023u) {
     if (threadIdx.x == 0) report_error(a.error_flag, kErrMisaligned);
+    wait_first(a);
+    wait_last(a);
     return;
   }
   if (threadIdx.x == 0) {

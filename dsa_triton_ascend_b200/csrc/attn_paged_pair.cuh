@@ -106,6 +106,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (base & 1023u) {   // the same in both CTAs
     if (threadIdx.x == 0) report_error(a.error_flag, kErrMisaligned);
+    wait_first(a);
+    wait_last(a);
     return;
   }
   const uint32_t rank = cluster_ctarank();

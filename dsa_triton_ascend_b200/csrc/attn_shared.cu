@@ -35,9 +35,9 @@ constexpr int kPlanRows = 2048;     // batch rows and groups whose lists fit int
 constexpr int kPlanGroups = 1024;
 
 // What a launch of either kind is made of: keys of a tile (1 << shift), units of starting a piece,
-// multiprocessors of a share, a unit's cost and that of a share's start and end, in cycles.
+// multiprocessors of a share; and in cycles what a tile takes, a piece's start and end, and a launch's.
 struct Kind {
-  int32_t shift, start, sms, cost, fixed;
+  int32_t shift, start, sms, cost, piece, fixed;
 };
 
 // What the plan tells the join: shares of either launch, units of all pieces.
@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const __grid_
   __shared__ int unit_room[kPlanGroups], start_room[kPlanGroups + 1];
   __shared__ int seen_room[kPlanRows], shared_room[kPlanRows];
   __shared__ unsigned long long saved;
-  __shared__ int units[2];   // of the pieces and of the rest
+  __shared__ int tiles[2], count[2];   // of the pieces and of the rest
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   constexpr int kWarps = kPlanThreads / 32;
   griddep_wait();
@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const __grid_
   const int32_t* starts = groups_here ? start_room : p.starts;
   if (tid == 0) {
     saved = 0;
-    units[0] = units[1] = 0;
+    tiles[0] = tiles[1] = count[0] = count[1] = 0;
   }
   bool bad = false;
 #pragma unroll 1
@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const __grid_
       const int items = (int)((tokens + p.per_item - 1) / (uint32_t)p.per_item);
       // shared where its pieces cost less than its keys do in its rows
       const long long less = (long long)own * tiles_of(p.own, keys) * p.own.cost -
-                             (long long)items * units_of(p.prefix, keys) * (p.prefix.cost * p.prefix.sms);
+                             (long long)items * (tiles_of(p.prefix, keys) * p.prefix.cost + p.prefix.piece) * p.prefix.sms;
       by_group[g] = less > 0 ? make_int4(keys, items, lead, 0) : make_int4(0, 0, 0, 0);
       if (less > 0) atomicAdd(&saved, (unsigned long long)less);
     }
@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const __grid_
       pieces += __shfl_sync(0xffffffffu, n, 31);
       all += __shfl_sync(0xffffffffu, u, 31);
     }
-    if (lane == 0) units[0] = all;
+    if (lane == 0) count[0] = pieces, tiles[0] = all - pieces * p.prefix.start;
   }
   __syncthreads();
 #pragma unroll 1
@@ -191,19 +191,25 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const __grid_
     }
   }
   __syncthreads();
-  int rest = 0;
+  int rest = 0, rows = 0;
 #pragma unroll 1
   for (int r = tid; r < p.a.rows; r += kPlanThreads) {
     const int b = r / p.a.s1, n = row_keys(p.a, r), shared = n > 0 ? rows_here ? shared_room[b] : p.by_row[b].x : 0;
     p.rest[r] = Item{n - shared, shared, b, r * p.a.n1, p.a.n1, shared > 0 || p.a.diag > 0, r * p.a.n1, 0};
-    rest += units_of(p.own, n - shared);
+    rest += tiles_of(p.own, n - shared);
+    rows += n > shared;
   }
   rest = __reduce_add_sync(0xffffffffu, rest);
-  if (lane == 0 && rest) atomicAdd(&units[1], rest);
+  rows = __reduce_add_sync(0xffffffffu, rows);
+  if (lane == 0 && rest) {
+    atomicAdd(&tiles[1], rest);
+    atomicAdd(&count[1], rows);
+  }
   __syncthreads();
   if (warp == 0) {
     // so many multiprocessors for the pieces that both launches end as early as may be
-    const float a = (float)units[0] * p.prefix.cost, b = (float)units[1] * p.own.cost;
+    const float a = (float)tiles[0] * p.prefix.cost + (float)count[0] * p.prefix.piece;
+    const float b = (float)tiles[1] * p.own.cost + (float)count[1] * p.own.piece;
     const int all = p.sms / p.prefix.sms;
     float best = INFINITY;
     int n = 0;
@@ -219,7 +225,8 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const __grid_
       const int k = __shfl_xor_sync(0xffffffffu, n, o);
       if (t < best || (t == best && k < n)) best = t, n = k;
     }
-    if (lane == 0) *p.limits = Limits{max(n, 1), max((p.sms - n * p.prefix.sms) / p.own.sms, 1), units[0], 0};
+    if (lane == 0) *p.limits = Limits{max(n, 1), max((p.sms - n * p.prefix.sms) / p.own.sms, 1),
+                                        tiles[0] + count[0] * p.prefix.start, 0};
   }
 }
 
@@ -395,13 +402,14 @@ Layout layout_of(int64_t batch, int64_t s1, int64_t n1, int64_t d, int64_t group
 // Whether pieces of a prefix can hold more tokens than a row of the rest does.
 bool can_share(const Layout& l) { return l.per_item > l.packed; }
 
-// The kernel for `nh` heads: a unit's cost (a tile's) and that of a share's start and end, in cycles, as
-// measured with keys that lie in L2.
+// The kernel for `nh` heads, in cycles: a tile (the slope over rows of 4096 and 12288 keys, or prefixes of
+// 16384 and 49152, that lie in L2), the start and end of a piece (what rows of 400 and 1100 keys take
+// beyond their tiles) and of a launch.
 Kind kind_of(int nh, int64_t d) {
-  if (nh == 128 && d == 512) return {7, pair::kSegmentCost, 2, 4200, 15000};
-  if (nh == 128) return {6, wide::kSegmentCost, 1, d == 256 ? 2200 : 1850, 12000};
-  const int cost = d == 512 ? (nh == 64 ? 3800 : nh == 32 ? 3000 : 2600) : d == 256 ? (nh == 64 ? 3000 : 2300) : 1900;
-  return {6, kSegmentCost, 1, cost, 14000};
+  if (nh == 128 && d == 512) return {7, pair::kSegmentCost, 2, 4350, 17000, 15000};
+  if (nh == 128) return {6, wide::kSegmentCost, 1, 1850, 12000, 13000};
+  const int tile = d == 512 ? (nh == 64 ? 3000 : nh == 32 ? 2600 : 2400) : d == 256 ? (nh == 64 ? 1650 : 1450) : (nh == 64 ? 1600 : 1400);
+  return {6, kSegmentCost, 1, tile, 12000, 14000};
 }
 static_assert(pair::kTile == 128 && wide::kTile == 64 && kTile == 64, "kind_of has the tiles' sizes");
 

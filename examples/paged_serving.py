@@ -6,8 +6,10 @@ A session owns a pool of pages (latent, rotary and index keys) and the device-re
 its slots.  ``prompt`` grows empty slots, appends the prompts' keys (rotated on the way) and
 attends causally; ``fork`` makes further slots continue a sequence; ``step`` decodes one token
 per slot, over every key of the cache, or, with ``top_k``, over the keys that the lightning
-indexer picks; ``free`` and ``compact`` give pages back and close up the pool.  Nothing here waits
-for the GPU, so a step can be captured into a CUDA graph.
+indexer picks; ``extend_packed`` takes any number of new tokens per slot, packed, with positions on
+one axis or several (pictures and films), and attends with the keys that neighbouring slots share
+computed once; ``free`` and ``compact`` give pages back and close up the pool.  Nothing here waits for
+the GPU, so a step can be captured into a CUDA graph.
 
 The layer's projections are left out: a caller passes what they would produce (absorbed queries,
 the latent key, index queries and weights), before rotary positions.
@@ -74,6 +76,26 @@ class PagedSession:
             query, self.caches[0], self.caches[0], picked, self.scale, block_table=table,
             actual_seq_lengths_kv=lengths, query_rope=query_rope, key_rope=self.caches[1], layout_kv="PA_BSND")[0]
 
+    def extend_packed(self, rows, counts, query, query_rope, key, key_rope, key_index, sections=None, axes=None):
+        """``counts[i]`` [n] new tokens for slot ``rows[i]``, one slot's behind another's in
+        ``key`` [T, 1, ...], ``key_rope`` and ``key_index`` (T at least their sum), with ``query`` [n, S, ...] and
+        ``query_rope`` padded to S tokens a slot.  Neighbouring slots that are forks of a sequence share its
+        keys.  With ``sections``, ``axes(positions)`` [A, ...] are the positions on A axes."""
+        grow = torch.zeros_like(self.lengths).index_copy_(0, rows.long(), counts)
+        self.block_table, self.lengths, self.refs = dsa.paged_cache_extend(
+            self.block_table, self.lengths, self.refs, grow, self.page_size)
+        plan = dsa.paged_batch_plan(self.block_table, self.lengths, rows, counts, self.page_size, key.shape[0])
+        turn = lambda x, at: dsa.rotary_embedding(x, self.table, at) if sections is None else \
+            dsa.rotary_embedding_axes(x, self.table, axes(at), sections)
+        key_index = dsa.rotary_embedding(key_index, self.table, plan.positions, layout="half")
+        dsa.paged_cache_store([key, turn(key_rope, plan.positions), key_index], self.caches, plan.slot_map)
+        start = plan.key_lengths - counts
+        at = start[:, None] + torch.arange(query.shape[1], dtype=torch.int32, device=query.device).clamp(max=counts[:, None] - 1)
+        return dsa.flash_attention_shared_prefix(
+            query, turn(query_rope, at.clamp(min=0)), self.caches[0], self.caches[1], plan.block_table, plan.group_starts,
+            plan.prefix_lengths, actual_seq_lengths_key=plan.key_lengths, scale_value=self.scale,
+            actual_seq_lengths_query=counts, sparse_mode=3)[0]
+
     def fork(self, parents, children):
         self.block_table, self.lengths, self.refs = dsa.paged_cache_fork(
             self.caches, self.block_table, self.lengths, self.refs, parents, children)
@@ -103,6 +125,10 @@ def main():
         session.step(i32(0, 1, 2, 3, 4), *tokens(5, 1))
     session.step(i32(0, 2), *tokens(2, 1), query_index=rnd(2, 1, 64, 128),
                  weights=torch.rand(2, 1, 64, generator=g, device="cuda"), top_k=128)
+    counts = [1, 3, 2, 1, 5]                              # rows 0, 2 and 3 share a prompt, 1 and 4 another
+    packed = sum(counts)
+    session.extend_packed(i32(0, 2, 3, 1, 4), i32(*counts), *tokens(5, max(counts))[:2], *[t[0] for t in tokens(1, packed)[2:]],
+                          sections=(8, 12, 12), axes=lambda at: at.expand(3, *at.shape))
     session.free(i32(0, 3))
     session.compact()
     out = session.step(i32(1, 2, 4), *tokens(3, 1))
