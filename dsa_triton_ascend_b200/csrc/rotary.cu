@@ -18,10 +18,12 @@ namespace dsa {
 namespace rotary {
 
 constexpr int kThreads = 128;
-constexpr int kHeads = 4;
 constexpr int kMaxPairs = 128;
 
+// Heads of a thread: 4, or 8 where a thread fetches the angles of several axes (8186 tokens x 64 heads x
+// 128, half layout, axes in turn: 44.0 us against 49.7 with 4; with one axis both take 45.5).
 struct Args {
+  static constexpr int kHeads = 4;
   const void* x;
   void* out;
   const int32_t* positions;
@@ -39,6 +41,7 @@ struct Args {
 // Positions of several axes: each pair turns by the position of its own axis.
 constexpr int kMaxAxes = DSA_ROTARY_MAX_AXES;
 struct AxesArgs : Args {
+  static constexpr int kHeads = 8;
   int64_t axis_stride;                  // positions of an axis
   uint64_t codes[2 * kMaxPairs / 64];   // the axis of each pair, in two bits
   int32_t axes;
@@ -105,7 +108,7 @@ enum { kInterleaved, kHalfShuffle, kHalfBoth };
 
 template <typename T, int kMode, typename A>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ A a) {
-  constexpr int kN = Vec<T>::kN;
+  constexpr int kN = Vec<T>::kN, kHeads = A::kHeads;
   const uint32_t item = blockIdx.x * kThreads + threadIdx.x;
   // (the shuffle needs whole warps: lanes past the end repeat the last item and store nothing)
   const bool live = item < a.items;
@@ -252,7 +255,7 @@ __global__ void __launch_bounds__(kThreads) rotary_table_kernel(const __grid_con
 
 template <typename T, typename A>
 int launch(const DsaRotaryParams* p, A a, cudaStream_t stream) {
-  constexpr int kN = Vec<T>::kN;
+  constexpr int kN = Vec<T>::kN, kHeads = A::kHeads;
   a.x = p->x;
   a.out = p->out;
   a.positions = p->positions;
