@@ -248,12 +248,14 @@ def flash_attention_shared_prefix(
     tokens that all rows of the group have in common, for which their rows of ``block_table`` name
     the same pages (those of the group's first row with keys are read); whole pages are shared, at
     most as many as every row of the group with keys sees.  Rows outside all groups share
-    nothing.  ``paged_batch_plan`` makes both.  Starts that divide no batch of B rows are reported by
-    ``check_device_errors``, and nothing is shared.
+    nothing.  ``paged_batch_plan`` makes both.
 
-    The other arguments and the results are those of :func:`flash_attention_paged`.  With more than
-    64 heads a token fills a piece by itself and nothing is gained by sharing.  G should be near the
-    number of groups: the pieces are of 128 heads where B * S1 * N1 / G exceeds 64.
+    The other arguments and the results are those of :func:`flash_attention_paged`.  Whether a group's
+    prefix is shared is decided on the GPU, by what that saves: nothing is where a token has more
+    than 64 heads (it fills a piece by itself), or in calls that are small or whose tables are.  G
+    should be near the number of groups: the pieces are of 128 heads where B * S1 * N1 / G exceeds 64.
+    Starts that divide no batch of B rows share nothing; where they are looked at they are
+    reported by ``check_device_errors``.
     """
     args = (query, query_rope, key_cache, key_rope_cache, block_table, actual_seq_lengths_key, actual_seq_lengths_query,
             float(scale_value), sparse_mode, bool(return_softmax_lse), group_starts, prefix_lengths)

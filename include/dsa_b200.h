@@ -460,7 +460,8 @@ int dsa_attn_paged_shares_keys(int64_t s1, int64_t n1);
  *   0 .. batch: group g is the batch rows group_starts[g] .. group_starts[g + 1] - 1, whose first
  *   prefix_lengths[g] tokens are the same: their block_table rows name the same pages there, of
  *   which the whole ones that all rows with keys see are shared.  Rows outside all groups share nothing.
- * Group starts that are no such division are reported in error_flag, and nothing is shared.
+ * Group starts that are no such division share nothing and, where they are looked at, are reported
+ * in error_flag.
  * Where a token has more than 64 heads nothing is shared; where something can be, all heads of query
  * and of query_rope lie one step apart, across tokens and rows.  A prefix is shared where that takes
  * fewer cycles than its rows by themselves, and anything only where it saves more than least_saving

@@ -17,6 +17,13 @@ from test_attn_paged_gpu import Case, i32
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(autouse=True, scope="module")
+def give_memory_back():
+    """Large blocks that stay in torch's cache would serve a later test that counts on its being empty."""
+    yield
+    torch.cuda.empty_cache()
+
+
 @pytest.fixture(autouse=True)
 def small_calls_share(monkeypatch):
     """Prefixes are shared however little that saves."""

@@ -9,6 +9,13 @@ import dsa_triton_ascend_b200 as dsa
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(autouse=True, scope="module")
+def give_memory_back():
+    """Large blocks that stay in torch's cache would serve a later test that counts on its being empty."""
+    yield
+    torch.cuda.empty_cache()
+
+
 def i32(v):
     return torch.tensor(v, dtype=torch.int32, device="cuda")
 

@@ -10,6 +10,13 @@ import dsa_triton_ascend_b200 as dsa
 
 pytestmark = pytest.mark.gpu
 
+
+@pytest.fixture(autouse=True, scope="module")
+def give_memory_back():
+    """Large blocks that stay in torch's cache would serve a later test that counts on its being empty."""
+    yield
+    torch.cuda.empty_cache()
+
 UNIT = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
 
 

@@ -17,6 +17,13 @@ from dsa_triton_ascend_b200 import _lib
 
 pytestmark = pytest.mark.gpu
 
+
+@pytest.fixture(autouse=True, scope="module")
+def give_memory_back():
+    """Large blocks that stay in torch's cache would serve a later test that counts on its being empty."""
+    yield
+    torch.cuda.empty_cache()
+
 sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples"))
 
 
