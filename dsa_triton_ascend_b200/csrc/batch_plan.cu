@@ -264,6 +264,8 @@ struct StoreArgs {
 __global__ void __launch_bounds__(kStoreThreads) store_kernel(const __grid_constant__ StoreArgs a) {
   const int lane = threadIdx.x & 31;
   const int64_t token = (int64_t)blockIdx.x * (kStoreThreads / 32) + (threadIdx.x >> 5);
+  griddep_wait();
+  griddep_launch_dependents();
   if (token >= a.tokens) return;
   const int64_t slot = a.slots[token];
   bool known = false;
@@ -298,6 +300,18 @@ __global__ void __launch_bounds__(kStoreThreads) store_kernel(const __grid_const
   }
 }
 
+// A launch that may begin before the stream's kernel before it has ended; the kernels here wait for it.
+cudaLaunchConfig_t early_launch(cudaLaunchAttribute* attr, int threads, cudaStream_t stream) {
+  attr->id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr->val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(threads);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cfg;
+}
+
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 }  // namespace plan
@@ -324,16 +338,10 @@ extern "C" int dsa_batch_plan(const DsaBatchPlanParams* p, void* stream_) {
   a.spans = (int)((p->max_blocks + kSpan - 1) / kSpan);
   const int sms = dsa::sm_count();
   if (sms < 1) return DSA_ERR_CUDA;
-  cudaLaunchAttribute pdl[1];
-  pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  pdl[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.stream = stream;
-  cfg.attrs = pdl;
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute early[1];
+  cudaLaunchConfig_t cfg = early_launch(early, kThreads, stream);
   const int64_t jobs = (p->batch * (a.spans + 1) + kWarps - 1) / kWarps, most = 8LL * sms;
   cfg.gridDim = dim3((unsigned)(a.token_blocks + (jobs < most ? jobs : most)));
-  cfg.blockDim = dim3(kThreads);
   a.alone = cfg.gridDim.x == 0;
   if (!a.alone && cudaLaunchKernelEx(&cfg, plan_rows_kernel, a) != cudaSuccess) return DSA_ERR_CUDA;
   cfg.gridDim = dim3(1);
@@ -367,6 +375,8 @@ extern "C" int dsa_cache_store(const DsaCacheStoreParams* p, void* stream_) {
   a.num_slots = p->num_pages * p->page_size;
   a.page = dsa::rotary::FastDiv((uint32_t)p->page_size);
   const int64_t blocks = (a.tokens + kStoreThreads / 32 - 1) / (kStoreThreads / 32);
-  store_kernel<<<(unsigned)blocks, kStoreThreads, 0, static_cast<cudaStream_t>(stream_)>>>(a);
-  return cudaGetLastError() == cudaSuccess ? DSA_OK : DSA_ERR_CUDA;
+  cudaLaunchAttribute early[1];
+  cudaLaunchConfig_t cfg = early_launch(early, kStoreThreads, static_cast<cudaStream_t>(stream_));
+  cfg.gridDim = dim3((unsigned)blocks);
+  return cudaLaunchKernelEx(&cfg, store_kernel, a) == cudaSuccess ? DSA_OK : DSA_ERR_CUDA;
 }

@@ -11,6 +11,8 @@
 // thread, 62 with two heads a thread).
 #include <cuda_runtime.h>
 
+#include <type_traits>
+
 #include "dsa_b200.h"
 #include "rotary.cuh"
 
@@ -104,11 +106,19 @@ struct TableRows {
 __device__ __forceinline__ TableRow rows_of(const Args& a, int64_t token) { return TableRow(a, token); }
 __device__ __forceinline__ TableRows rows_of(const AxesArgs& a, int64_t token) { return TableRows(a, token); }
 
+// With several axes the kernels may begin before the stream's kernel before them has ended.
+__device__ __forceinline__ void wait_first(const Args&) {}
+__device__ __forceinline__ void wait_first(const AxesArgs&) {
+  griddep_wait();
+  griddep_launch_dependents();
+}
+
 enum { kInterleaved, kHalfShuffle, kHalfBoth };
 
 template <typename T, int kMode, typename A>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ A a) {
   constexpr int kN = Vec<T>::kN, kHeads = A::kHeads;
+  wait_first(a);
   const uint32_t item = blockIdx.x * kThreads + threadIdx.x;
   // (the shuffle needs whole warps: lanes past the end repeat the last item and store nothing)
   const bool live = item < a.items;
@@ -199,6 +209,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
 // Any strides, offsets and even widths: one pair or one copied value per thread.
 template <typename T, typename A>
 __global__ void __launch_bounds__(kThreads) rotary_any_kernel(const __grid_constant__ A a) {
+  wait_first(a);
   const uint32_t item = blockIdx.x * kThreads + threadIdx.x;
   if (item >= a.items) return;
   const uint32_t rest = a.units.div(item), u = item - rest * a.units.d;
@@ -298,11 +309,18 @@ int launch(const DsaRotaryParams* p, A a, cudaStream_t stream) {
     a.token0 = t0;
     a.items = (uint32_t)(n * per_token);
     const unsigned grid = (unsigned)((a.items + kThreads - 1) / kThreads);
-    if (!vec) rotary_any_kernel<T, A><<<grid, kThreads, 0, stream>>>(a);
-    else if (!p->half_layout) rotary_kernel<T, kInterleaved, A><<<grid, kThreads, 0, stream>>>(a);
-    else if (shuffle) rotary_kernel<T, kHalfShuffle, A><<<grid, kThreads, 0, stream>>>(a);
-    else rotary_kernel<T, kHalfBoth, A><<<grid, kThreads, 0, stream>>>(a);
-    if (cudaGetLastError() != cudaSuccess) return DSA_ERR_CUDA;
+    auto kern = !vec ? rotary_any_kernel<T, A> : !p->half_layout ? rotary_kernel<T, kInterleaved, A>
+                : shuffle ? rotary_kernel<T, kHalfShuffle, A> : rotary_kernel<T, kHalfBoth, A>;
+    cudaLaunchAttribute early[1];
+    early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = stream;
+    cfg.attrs = early;
+    cfg.numAttrs = std::is_same<A, AxesArgs>::value ? 1 : 0;
+    if (cudaLaunchKernelEx(&cfg, kern, a) != cudaSuccess) return DSA_ERR_CUDA;
   }
   return DSA_OK;
 }
