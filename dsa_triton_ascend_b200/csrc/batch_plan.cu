@@ -6,7 +6,7 @@
 // Neighbouring requests whose first pages are the same form a group (for attention that takes a
 // shared prefix once).
 //
-// Two launches.  plan_rows_kernel, over the whole GPU: some blocks write the tokens' lists (each
+// Two launches, or, for a small step, one cluster that does the same.  plan_rows_kernel, over the whole GPU: some blocks write the tokens' lists (each
 // finds its tokens' requests by a scan of the counts of its own, up to the last it needs), the others
 // the block table's rows and how many pages each has in common with the row before it.
 // plan_groups_kernel, one block beside it: lengths and ends, then the groups.  Bound by latency: a chain of
@@ -27,6 +27,7 @@ constexpr int kTokens = 4 * kThreads;   // of a block
 constexpr int kRows = 1024;             // requests scanned at a time
 constexpr int kSpan = 256;              // table entries of a warp's turn
 constexpr int kGroupThreads = 512;
+constexpr int kCluster = 8;             // CTAs that plan a small step
 
 struct Args {
   DsaBatchPlanParams p;
@@ -73,13 +74,13 @@ __device__ __forceinline__ int64_t block_prefix(int64_t v, int64_t* tmp, int64_t
   return v + before;
 }
 
-__device__ void plan_tokens(const Args& a) {
+__device__ __forceinline__ void plan_tokens(const Args& a, int64_t block) {
   const DsaBatchPlanParams& p = a.p;
   __shared__ int64_t tmp[kWarps];
   __shared__ int64_t ends[kRows];
   __shared__ int32_t slot[kRows], tokens[kRows];
   constexpr int kPer = kRows / kThreads;
-  const int64_t t0 = (int64_t)blockIdx.x * kTokens, t1 = min(t0 + kTokens, p.num_tokens);
+  const int64_t t0 = block * kTokens, t1 = min(t0 + kTokens, p.num_tokens);
   int64_t before = 0;   // tokens of the requests before these
   bool bad = false;
   for (int64_t b0 = 0; b0 < p.batch && before < t1; b0 += kRows) {
@@ -126,18 +127,11 @@ __device__ void plan_tokens(const Args& a) {
   if (bad) report_error(p.error_flag, kErrBadIndex);
 }
 
-__global__ void __launch_bounds__(kThreads) plan_rows_kernel(const __grid_constant__ Args a) {
-  griddep_wait();
-  griddep_launch_dependents();
-  if ((int)blockIdx.x < a.token_blocks) {
-    plan_tokens(a);
-    return;
-  }
+// The block table's rows and the comparisons, those of warp `warp` of `warps`.
+__device__ __forceinline__ void plan_rows(const Args& a, int64_t warp, int64_t warps) {
   const DsaBatchPlanParams& p = a.p;
   const int lane = threadIdx.x & 31;
-  const int64_t warp = (int64_t)(blockIdx.x - a.token_blocks) * kWarps + (threadIdx.x >> 5);
-  const int64_t warps = (int64_t)(gridDim.x - a.token_blocks) * kWarps;
-  bool bad = false;   // (told by plan_groups_kernel)
+  bool bad = false;   // (told by plan_groups)
   for (int64_t job = warp; job < p.batch * (a.spans + 1); job += warps) {
     // the comparisons, which are the longest, first
     const int64_t b = job < p.batch ? job : (job - p.batch) / a.spans;
@@ -191,28 +185,39 @@ __global__ void __launch_bounds__(kThreads) plan_rows_kernel(const __grid_consta
   }
 }
 
-// What does not hang on the comparisons is done while they are made: plan_rows_kernel has let this
-// kernel start after its own wait, so the inputs are there.
-__global__ void __launch_bounds__(kGroupThreads) plan_groups_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(kThreads) plan_rows_kernel(const __grid_constant__ Args a) {
+  griddep_wait();
+  griddep_launch_dependents();
+  if ((int)blockIdx.x < a.token_blocks) {
+    plan_tokens(a, blockIdx.x);
+    return;
+  }
+  plan_rows(a, (int64_t)(blockIdx.x - a.token_blocks) * kWarps + (threadIdx.x >> 5),
+            (int64_t)(gridDim.x - a.token_blocks) * kWarps);
+}
+
+// Lengths, ends and groups, by one block of kBlock threads.  What does not hang on the comparisons is done
+// before `wait`, which returns when they are made.
+template <int kBlock, typename Wait>
+__device__ __forceinline__ void plan_groups(const Args& a, Wait wait) {
   const DsaBatchPlanParams& p = a.p;
-  __shared__ int64_t tmp[kGroupThreads / 32];
-  __shared__ int32_t least_room[kGroupThreads];
+  __shared__ int64_t tmp[kBlock / 32];
+  __shared__ int32_t least_room[kBlock];
   const int tid = threadIdx.x;
   constexpr int32_t kNone = 0x7fffffff;
   const int64_t least = p.min_prefix > p.page_size ? p.min_prefix : p.page_size;
   // smallest prefix of each group, in shared memory where all requests are looked at together
-  const bool together = p.batch <= kGroupThreads;
+  const bool together = p.batch <= kBlock;
   int32_t* smallest = together ? least_room : p.prefix_lengths;
-  const int64_t listed = together ? kGroupThreads : p.max_groups;
-  if (a.alone) griddep_wait();
+  const int64_t listed = together ? kBlock : p.max_groups;
   int64_t tokens = 0, groups = 0, total;
   bool bad = false;
 #pragma unroll 1
-  for (int64_t b0 = 0; b0 < p.batch; b0 += kGroupThreads) {
+  for (int64_t b0 = 0; b0 < p.batch; b0 += kBlock) {
     const int64_t b = b0 + tid;
     Request q{0, 0, 0};
     if (b < p.batch) q = request_of(p, b, &bad);
-    const int64_t end = tokens + block_prefix<kGroupThreads>(q.count, tmp, &total);
+    const int64_t end = tokens + block_prefix<kBlock>(q.count, tmp, &total);
     if (b < p.batch) {
       p.key_lengths[b] = q.tokens;
       p.query_ends[b] = (int32_t)end;
@@ -220,27 +225,49 @@ __global__ void __launch_bounds__(kGroupThreads) plan_groups_kernel(const __grid
     tokens += total;
   }
 #pragma unroll 1
-  for (int64_t g = tid; g < listed; g += kGroupThreads) smallest[g] = kNone;
+  for (int64_t g = tid; g < listed; g += kBlock) smallest[g] = kNone;
   if (tokens > p.num_tokens) bad = true;   // the last ones are not listed
   if (bad) report_error(p.error_flag, kErrBadIndex);
-  if (!a.alone) griddep_wait();
+  wait();
 #pragma unroll 1
-  for (int64_t b0 = 0; b0 < p.batch; b0 += kGroupThreads) {
+  for (int64_t b0 = 0; b0 < p.batch; b0 += kBlock) {
     const int64_t b = b0 + tid, common = b < p.batch ? a.common[b] * p.page_size : 0;
     const bool first = b < p.batch && (b == 0 || common < least);
-    const int64_t group = groups + block_prefix<kGroupThreads>(first, tmp, &total) - 1;
+    const int64_t group = groups + block_prefix<kBlock>(first, tmp, &total) - 1;
     groups += total;
     if (first && group <= p.max_groups) p.group_starts[group] = (int32_t)b;
     if (b < p.batch && !first && group < listed) atomicMin(smallest + group, (int32_t)common);
   }
 #pragma unroll 1
-  for (int64_t g = groups + tid; g <= p.max_groups; g += kGroupThreads) p.group_starts[g] = (int32_t)p.batch;
+  for (int64_t g = groups + tid; g <= p.max_groups; g += kBlock) p.group_starts[g] = (int32_t)p.batch;
   __syncthreads();
 #pragma unroll 1
-  for (int64_t g = tid; g < p.max_groups; g += kGroupThreads) {
+  for (int64_t g = tid; g < p.max_groups; g += kBlock) {
     const int32_t v = g < listed ? *const_cast<volatile int32_t*>(smallest + g) : kNone;
     p.prefix_lengths[g] = v == kNone ? 0 : v;
   }
+}
+
+// (The kernel above has let this one start after its own wait, so the inputs are there.)
+__global__ void __launch_bounds__(kGroupThreads) plan_groups_kernel(const __grid_constant__ Args a) {
+  if (a.alone) griddep_wait();
+  plan_groups<kGroupThreads>(a, [&] {
+    if (!a.alone) griddep_wait();
+  });
+}
+
+// All of a small step by one cluster: the groups by its first CTA, tokens by the last ones.
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) plan_step_kernel(const __grid_constant__ Args a) {
+  griddep_wait();
+  griddep_launch_dependents();
+  const int rows = kCluster - 1 - a.token_blocks;   // CTAs
+  if (blockIdx.x == 0) {
+    plan_groups<kThreads>(a, [] { cluster_sync(); });
+    return;
+  }
+  if ((int)blockIdx.x <= rows) plan_rows(a, ((int)blockIdx.x - 1) * kWarps + (threadIdx.x >> 5), rows * kWarps);
+  else plan_tokens(a, blockIdx.x - 1 - rows);
+  cluster_sync();
 }
 
 // ---------------------------------------------------------------------------------------
@@ -340,7 +367,12 @@ extern "C" int dsa_batch_plan(const DsaBatchPlanParams* p, void* stream_) {
   if (sms < 1) return DSA_ERR_CUDA;
   cudaLaunchAttribute early[1];
   cudaLaunchConfig_t cfg = early_launch(early, kThreads, stream);
-  const int64_t jobs = (p->batch * (a.spans + 1) + kWarps - 1) / kWarps, most = 8LL * sms;
+  const int64_t warps = p->batch * (a.spans + 1), jobs = (warps + kWarps - 1) / kWarps, most = 8LL * sms;
+  // up to two turns of a warp: one launch
+  if (a.token_blocks < kCluster - 1 && warps <= 2 * (kCluster - 1 - a.token_blocks) * kWarps) {
+    cfg.gridDim = dim3(kCluster);
+    return cudaLaunchKernelEx(&cfg, plan_step_kernel, a) == cudaSuccess ? DSA_OK : DSA_ERR_CUDA;
+  }
   cfg.gridDim = dim3((unsigned)(a.token_blocks + (jobs < most ? jobs : most)));
   a.alone = cfg.gridDim.x == 0;
   if (!a.alone && cudaLaunchKernelEx(&cfg, plan_rows_kernel, a) != cudaSuccess) return DSA_ERR_CUDA;

@@ -124,6 +124,17 @@ def test_long_prompts_and_tables():
     _check(table, lens, [0, 6, 6, 0, 1, 1], [0, 1, 1, 0, 0, 0], page, 3)
 
 
+@pytest.mark.parametrize("batch", [1, 2, 8, 16, 24, 48, 56, 57])
+@pytest.mark.parametrize("T", [0, 1, 1023, 1024, 1025, 5000, 6144, 6145, 9000])
+def test_small_steps_of_any_number_of_tokens(batch, T):
+    """One launch or two, by requests and blocks of tokens; the last tokens behind the requests' or left out."""
+    rng = random.Random(batch * T)
+    table, lens = _pool(rng, 60, 40, 16, 0.7)
+    rows = rng.sample(range(60), batch)
+    counts = [rng.randint(0, lens[r]) for r in rows]
+    _check(table, lens, rows, counts, 16, T)
+
+
 def test_requests_that_cannot_be():
     table, lens = [[0, 1, 2], [3, 4, -1], [5, -1, -1]], [20, 16, 99]
     _check(table, lens, [0, 1, -1, 3, 1, 0, 2], [1, 2, 1, 1, -1, 21, 1], 8, 4)
