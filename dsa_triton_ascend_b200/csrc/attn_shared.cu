@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const __grid_
       const int items = (int)((tokens + p.per_item - 1) / (uint32_t)p.per_item);
       // shared where its pieces cost less than its keys do in its rows
       const long long less = (long long)own * tiles_of(p.own, keys) * p.own.cost -
-                             (long long)items * (tiles_of(p.prefix, keys) * p.prefix.cost + p.prefix.piece) * p.prefix.sms;
+                             (long long)items * ((long long)tiles_of(p.prefix, keys) * p.prefix.cost + p.prefix.piece) * p.prefix.sms;
       by_group[g] = less > 0 ? make_int4(keys, items, lead, 0) : make_int4(0, 0, 0, 0);
       if (less > 0) atomicAdd(&saved, (unsigned long long)less);
     }
