@@ -33,6 +33,7 @@ namespace attn_paged {
 constexpr int kPlanThreads = 512;
 constexpr int kPlanRows = 2048;     // batch rows and groups whose lists fit into shared memory
 constexpr int kPlanGroups = 1024;
+constexpr int64_t kMaxGroups = 1 << 30;
 
 // What a launch of either kind is made of: keys of a tile (1 << shift), units of starting a piece,
 // multiprocessors of a share; and in cycles what a tile takes, a piece's start and end, and a launch's.
@@ -75,7 +76,9 @@ __device__ __forceinline__ int least_seen(const PlanArgs& p, int b) {
   }
   return (int)(n < cap ? n : cap);
 }
-__device__ __forceinline__ int tiles_of(const Kind& k, int keys) { return (keys + (1 << k.shift) - 1) >> k.shift; }
+__device__ __forceinline__ int tiles_of(const Kind& k, int keys) {
+  return (int)(((uint32_t)keys + (1u << k.shift) - 1) >> k.shift);
+}
 __device__ __forceinline__ int units_of(const Kind& k, int keys) { return keys > 0 ? tiles_of(k, keys) + k.start : 0; }
 
 // One block: what the inputs hold is fetched at once and held in shared memory where it fits, since each
@@ -136,7 +139,7 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const __grid_
     lead = __reduce_min_sync(0xffffffffu, lead);
     rows = __reduce_add_sync(0xffffffffu, rows);
     if (lane == 0) {
-      const uint32_t some = max(min(prefix, least), 0);
+      const uint32_t some = rows > 0 ? max(min(prefix, least), 0) : 0;   // (idle rows have no page to read)
       const int keys = (int)(some - some % (uint32_t)p.a.page_size);
       const uint32_t tokens = (uint32_t)(to - from) * p.s1, own = (uint32_t)rows * p.own_rows;
       const int items = (int)((tokens + p.per_item - 1) / (uint32_t)p.per_item);
@@ -539,9 +542,8 @@ int launch_shared_dim(const DsaAttnSharedParams* sp, const Layout& l, cudaStream
 
 extern "C" int64_t dsa_attn_shared_workspace_size(int64_t batch, int64_t s1, int64_t n1, int64_t d, int64_t groups) {
   using namespace dsa::attn_paged;
-  constexpr int64_t kMax = 0x7fffffff;
   const int64_t plain = dsa_attn_paged_workspace_size(batch, s1, n1, d);
-  if (plain < 0 || groups < 0 || groups > kMax) return -1;
+  if (plain < 0 || groups < 0 || groups > kMaxGroups) return -1;
   int64_t most = plain;
   if (groups == 0 || batch == 0 || s1 == 0) return most;
   for (const bool packed : {false, true}) {
@@ -559,7 +561,7 @@ extern "C" int dsa_attn_shared(const DsaAttnSharedParams* sp, void* stream_) {
   const DsaAttnPagedParams* p = &sp->attn;
   if (p->batch == 0 || p->s1 == 0) return DSA_OK;
   constexpr int64_t kMax = 0x7fffffff;
-  if (!valid_params(p, kTile) || sp->groups > kMax || sp->least_saving < 0 || (sp->groups > 0 && (!sp->group_starts || !sp->prefix_lengths)) ||
+  if (!valid_params(p, kTile) || sp->groups > kMaxGroups || sp->least_saving < 0 || (sp->groups > 0 && (!sp->group_starts || !sp->prefix_lengths)) ||
       p->workspace_bytes < dsa_attn_shared_workspace_size(p->batch, p->s1, p->n1, p->d, sp->groups))
     return DSA_ERR_INVALID_ARG;
   if (sp->groups > 0) {
@@ -569,9 +571,10 @@ extern "C" int dsa_attn_shared(const DsaAttnSharedParams* sp, void* stream_) {
     // with 8192 shared keys: 34 us against 37; 8 rows: 32 against 27), 64 heads at 1.5 to 3 M.
     const Kind own = kind_of(l.own_nh, p->d);
     const double all = (double)l.rest * ((p->max_blocks * p->page_size >> own.shift) + 1) * own.cost * own.sms;
-    // (places and units are counted in 32 bits)
+    // (places, units and the keys of a tile of 128 are counted in 32 bits)
     const int64_t tiles = (p->max_blocks * p->page_size + kTile - 1) / kTile + 8;
-    if (can_share(l) && all > 2.5 * (double)sp->least_saving && l.most * l.nh <= kMax && l.most + l.rest <= kMax / tiles) {
+    if (can_share(l) && all > 2.5 * (double)sp->least_saving && l.most * l.nh <= kMax && l.most + l.rest <= kMax / tiles &&
+        p->max_blocks * p->page_size <= kMax - pair::kTile) {
       if (!one_matrix(p, p->q_head_stride, p->q_token_stride, p->q_batch_stride) ||
           !one_matrix(p, p->qr_head_stride, p->qr_token_stride, p->qr_batch_stride) || l.shares < 1)
         return DSA_ERR_INVALID_ARG;

@@ -135,6 +135,16 @@ def test_prefixes_of_any_length():
         c.run()
 
 
+@pytest.mark.parametrize("page", [8, 32, 1000])
+def test_idle_groups_and_empty_ones_with_endless_prefixes(page):
+    """Nothing bounds the prefix of a group without a row that sees keys: it shares nothing."""
+    c = Shared([(2000, [None, None, None, None]), (2000, [20, 30, None]), (64, [None])], [5], 16, 128, page, seed=4)
+    c.starts = i32([0, 4, 4, 7, 8])
+    for now in ((1 << 31) - 1, (1 << 31) - 64, (1 << 31) - 65, 1 << 30, 1 << 21):
+        c.prefixes = i32([now, now, 2000, now])
+        c.run()
+
+
 def test_rows_outside_all_groups_and_empty_groups():
     c = Shared([(200, [20, 30, 40, 50, 60])], (), 16, 128, 32, seed=2)
     for starts in ([2, 4], [0, 0, 0, 5, 5], [1, 1, 5, 5], [5, 5], [0, 2, 5]):

@@ -175,7 +175,7 @@ def test_c_entries_refuse_what_the_kernels_cannot_take():
             setattr(p if k in ("groups", "group_starts", "prefix_lengths") else a, k, v)
         return lib.dsa_attn_shared(p, None)
 
-    for kw in (dict(groups=-1), dict(groups=1 << 31), dict(group_starts=0), dict(prefix_lengths=0), dict(batch=-1), dict(s1=-1),
+    for kw in (dict(groups=-1), dict(groups=1 << 31), dict(groups=(1 << 30) + 1), dict(group_starts=0), dict(prefix_lengths=0), dict(batch=-1), dict(s1=-1),
                dict(page_size=12), dict(n1=0), dict(n1=129), dict(scale=float("inf")), dict(out=1025), dict(workspace=0),
                dict(act_k=0), dict(q_head_stride=4), dict(num_pages=0)):
         assert shared(**kw) == bad, kw
