@@ -37,7 +37,7 @@ struct Args {
 };
 
 struct Request {
-  int32_t slot, tokens, count;   // an empty one where it asks for what cannot be
+  int32_t slot, tokens, count;   // one that asks for what cannot be: 0, 0, and places for its tokens
 };
 __device__ __forceinline__ Request request_of(const DsaBatchPlanParams& p, int64_t b, bool* bad) {
   Request r{p.rows[b], 0, 0};
@@ -45,7 +45,7 @@ __device__ __forceinline__ Request request_of(const DsaBatchPlanParams& p, int64
   const int64_t n = there ? p.seq_lengths[r.slot] : 0, c = p.counts[b];
   if (!there || c < 0 || c > n || n > p.max_blocks * p.page_size) {
     *bad = true;
-    return Request{0, 0, 0};
+    return Request{0, 0, c > 0 ? (int32_t)c : 0};
   }
   r.tokens = (int32_t)n;
   r.count = (int32_t)c;
@@ -108,10 +108,11 @@ __device__ __forceinline__ void plan_tokens(const Args& a, int64_t block) {
         if (ends[mid] > t) hi = mid;
         else lo = mid + 1;
       }
-      const uint32_t pos = (uint32_t)(tokens[lo] - (ends[lo] - t)), size = (uint32_t)p.page_size, block = pos / size;
-      const int32_t page = p.block_table[(int64_t)slot[lo] * p.max_blocks + block];
+      const int64_t at = tokens[lo] - (ends[lo] - t);   // below 0: of a request that cannot be
+      const uint32_t pos = (uint32_t)max(at, (int64_t)0), size = (uint32_t)p.page_size, block = pos / size;
+      const int32_t page = at < 0 ? -1 : p.block_table[(int64_t)slot[lo] * p.max_blocks + block];
       bad |= page < 0;
-      p.token_rows[t] = (int32_t)(b0 + lo);
+      p.token_rows[t] = at < 0 ? -1 : (int32_t)(b0 + lo);
       p.positions[t] = (int32_t)pos;
       p.slot_map[t] = page < 0 ? -1 : page * p.page_size + (pos - block * size);
     }
@@ -220,7 +221,7 @@ __device__ __forceinline__ void plan_groups(const Args& a, Wait wait) {
     const int64_t end = tokens + block_prefix<kBlock>(q.count, tmp, &total);
     if (b < p.batch) {
       p.key_lengths[b] = q.tokens;
-      p.query_ends[b] = (int32_t)end;
+      p.query_ends[b] = (int32_t)min(end, (int64_t)0x7fffffff);
     }
     tokens += total;
   }

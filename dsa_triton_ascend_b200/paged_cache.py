@@ -451,13 +451,13 @@ def paged_batch_plan(block_table, seq_lengths, rows, counts, page_size, num_toke
       ``flash_attention_shared_prefix``); a request that shares less with the one before it begins a
       group.  The first ``max_groups`` (default B) are listed.
 
-    A request that cannot be (a slot out of range, a count past its length) is taken as an empty one,
-    a token without a page has slot -1, and tokens past ``num_tokens`` are left out; all are reported
-    by ``check_device_errors``.
+    A request that cannot be (a slot out of range, a count past its length) has length 0, and its tokens
+    keep their places, with -1, 0 and -1 as behind the last; a token without a page has slot -1, and tokens
+    past ``num_tokens`` are left out; all are reported by ``check_device_errors``.
     """
     page_size, num_tokens, min_prefix = int(page_size), int(num_tokens), int(min_prefix)
     if max_groups is None:
-        max_groups = rows.numel()
+        max_groups = rows.numel() if torch.is_tensor(rows) else 0
     max_groups = int(max_groups)
     args = (block_table, seq_lengths, rows, counts, page_size, num_tokens, max_groups, min_prefix)
     fast = binding()

@@ -646,8 +646,8 @@ int64_t dsa_pages_workspace_size(int32_t op, int64_t n, int64_t slots, int64_t n
  *       request of its own is a group with 0.  Of more groups the first max_groups are listed;
  *       behind the last one starts are batch and lengths 0.
  * A request that asks for what cannot be (a slot out of range, a count below 0 or past the length, a
- * length past the table) is taken as an empty one, a token without a page has slot -1, tokens past
- * num_tokens are not listed; error_flag tells.
+ * length past the table) has length 0, and its tokens keep their places, with -1, 0 and -1; a
+ * token without a page has slot -1, tokens past num_tokens are not listed; error_flag tells.
  * Workspace: dsa_batch_plan_workspace_size() bytes.
  */
 typedef struct DsaBatchPlanParams {

@@ -35,12 +35,17 @@ def _expect(table, lens, rows, counts, page, T, most, least):
     for r, c in zip(rows, counts):
         n = lens[r] if 0 <= r < len(lens) else 0
         if not 0 <= r < len(lens) or c < 0 or c > n or n > width * page:
-            err, r, n, c = 4, 0, 0, 0
+            err, r, n, c = 4, 0, 0, max(c, 0)
         req.append((r, n, c))
     out = [[table[r][j] if j * page < n else -1 for j in range(width)] for r, n, _ in req]
     ends, where, pos, slots = [], [], [], []
     for b, (r, n, c) in enumerate(req):
         for p in range(n - c, n):
+            if p < 0:   # of a request that cannot be: its place is kept
+                where.append(-1)
+                pos.append(0)
+                slots.append(-1)
+                continue
             where.append(b)
             pos.append(p)
             slots.append(-1 if table[r][p // page] < 0 else table[r][p // page] * page + p % page)

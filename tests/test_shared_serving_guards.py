@@ -119,7 +119,7 @@ def test_paged_cache_store_shapes(kw, msg, monkeypatch):
 @pytest.mark.parametrize("kw,msg", [
     (dict(block_table=t(4, 3)), "block_table"), (dict(block_table=i(4)), "block_table"),
     (dict(block_table=i(0, 3), seq_lengths=i(0)), "empty"), (dict(seq_lengths=i(3)), "seq_lengths"),
-    (dict(rows=i(2, 1)), "rows"), (dict(rows=i(2).long()), "rows"), (dict(counts=i(3)), "counts"),
+    (dict(rows=i(2, 1)), "rows"), (dict(rows=[0, 1]), "rows"), (dict(rows=i(2).long()), "rows"), (dict(counts=i(3)), "counts"),
     (dict(page_size=0), "page_size"), (dict(num_tokens=-1), "num_tokens"), (dict(num_tokens=1 << 31), "num_tokens"),
     (dict(max_groups=-1), "max_groups"), (dict(min_prefix=-1), "min_prefix"), (dict(page_size=1 << 30), "32 bits"),
 ])
