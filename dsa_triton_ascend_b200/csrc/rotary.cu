@@ -9,6 +9,8 @@
 // the same tensor takes 44.6; the gradient of 2 x 4093 tokens x 64 heads x 128, half of each head
 // rotated, in 45.6 us, 5.9 TB/s (49.5 with blocks of 256 threads, 51.5 with both pieces in a
 // thread, 62 with two heads a thread).
+// With positions of several axes a pair takes its angle from its axis' row of the table (the same kernels,
+// bound by memory as well): the same two tensors in 42.3 us (three axes in blocks) and 46 (axes in turn).
 #include <cuda_runtime.h>
 
 #include <type_traits>

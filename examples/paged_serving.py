@@ -80,11 +80,14 @@ class PagedSession:
         """``counts[i]`` [n] new tokens for slot ``rows[i]``, one slot's behind another's in
         ``key`` [T, 1, ...], ``key_rope`` and ``key_index`` (T at least their sum), with ``query`` [n, S, ...] and
         ``query_rope`` padded to S tokens a slot.  Neighbouring slots that are forks of a sequence share its
-        keys.  With ``sections``, ``axes(positions)`` [A, ...] are the positions on A axes."""
+        keys.  With ``sections``, ``axes(positions)`` [A, ...] are the positions on A axes.  A slot that the pool cannot
+        serve stays as it was, gives zeros and is reported."""
+        before = self.lengths[rows]
         grow = torch.zeros_like(self.lengths).index_copy_(0, rows.long(), counts)
         self.block_table, self.lengths, self.refs = dsa.paged_cache_extend(
             self.block_table, self.lengths, self.refs, grow, self.page_size)
-        plan = dsa.paged_batch_plan(self.block_table, self.lengths, rows, counts, self.page_size, key.shape[0])
+        served = torch.where(self.lengths[rows] - before == counts, rows, -1)
+        plan = dsa.paged_batch_plan(self.block_table, self.lengths, served, counts, self.page_size, key.shape[0])
         turn = lambda x, at: dsa.rotary_embedding(x, self.table, at) if sections is None else \
             dsa.rotary_embedding_axes(x, self.table, axes(at), sections)
         key_index = dsa.rotary_embedding(key_index, self.table, plan.positions, layout="half")

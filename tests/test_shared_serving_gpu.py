@@ -107,6 +107,41 @@ def test_packed_steps_of_forks(heads, sections, share, monkeypatch):
     assert session.lengths.tolist() == [156, 155, 169, 152, 156, 44, 152, 198, 0, 0]
 
 
+@pytest.mark.parametrize("old", [0, 60])
+def test_a_packed_step_that_the_pool_cannot_serve(old):
+    """The refused slot keeps its keys (or none), the others' tokens go where they would without it."""
+    from paged_serving import PagedSession
+
+    def run(pages):
+        g = torch.Generator(device="cuda")
+        g.manual_seed(7)
+        rnd = lambda *shape: torch.randn(*shape, generator=g, device="cuda").bfloat16()
+        tokens = lambda n, S, T: (rnd(n, S, 8, 512), rnd(n, S, 8, 64), rnd(T, 1, 512), rnd(T, 1, 64), rnd(T, 1, 128))
+        session = PagedSession(slots=4, num_pages=pages, page_size=16, max_blocks=8, heads=8)
+        session.extend_packed(i32(0, 1, 2), i32(20, old, 33), *tokens(3, 60, 53 + old))
+        dsa.check_device_errors()
+        kept = [c[session.block_table[1, :old // 16].long()].clone() for c in session.caches]
+        out = session.extend_packed(i32(0, 1, 2), i32(3, 50, 4), *tokens(3, 50, 57))
+        return session, kept, out
+
+    full, kept, out = run(7 + old // 16)                # 50 tokens more take three pages or four
+    with pytest.raises(RuntimeError, match="bits 0x14"):
+        dsa.check_device_errors()
+    assert full.lengths.tolist() == [23, old, 37, 0] and not out[1].any()
+    assert all(torch.equal(c[full.block_table[1, :old // 16].long()], k) for c, k in zip(full.caches, kept))
+    roomy, _, want = run(40)
+    dsa.check_device_errors()
+    # the same keys, summed in other parts: twice the fp32 sums' 2^-12 of the values, and a rounding each
+    most = roomy.caches[0].abs().max().double()
+    for b in (0, 2):
+        x, y = out[b].double(), want[b].double()
+        assert bool(((x - y).abs() <= 2.0 ** -11 * most + 2.0 ** -8 * (x.abs() + y.abs()) * 1.01).all())
+        n = full.lengths[b].item()
+        for x, y in zip(full.caches, roomy.caches):
+            pages = [t[b, :-(-n // 16)].long() for t in (full.block_table, roomy.block_table)]
+            assert torch.equal(x[pages[0]].flatten(0, 1)[:n], y[pages[1]].flatten(0, 1)[:n])
+
+
 @pytest.fixture
 def paths(monkeypatch):
     """both(call): the results of the Python path and of the compiled one, which has to be taken."""
