@@ -17,7 +17,7 @@
 //
 // Measured (replayed from a graph, against attn_paged.cu alone): 64 rows of 16 heads, D = 512, with 32811 shared
 // and 17 to 2048 own keys, 108 us against 309; 84 rows of 20 heads in five groups, 9 of them alone, 74
-// against 98; 24 rows x 2 tokens of 32 heads, D = 256, in two groups, 49 against 53.  Of the 108: plan 4.6, the pieces'
+// against 98; 24 rows x 2 tokens of 32 heads, D = 256, in two groups, 47 against 53.  Of the 108: plan 4.6, the pieces'
 // tiles from 8 to 83 in 62 CTA pairs (3,645 cycles for 128 keys and 128 heads, 2,176 of them products)
 // beside the rests in 24 CTAs, results to 94, join 7.  In one launch, all in pieces of 128 heads, it took 123.
 #include <cuda_runtime.h>
@@ -261,7 +261,9 @@ __global__ void __launch_bounds__(kJoinThreads)
   constexpr bool kWide = kLanes == kJoinThreads;
   constexpr int kCols = D / 4;                // threads of a part, a float4 each
   constexpr int kGroups = kLanes / kCols;     // parts at a time
-  constexpr int kAhead = 4;                   // of a thread
+  // of a thread: 6 for 24 rows x 2 tokens, 32 heads, D = 256 take 47.3 us a call against 48.8 with 4 and 49.8 with 12;
+  // at D = 512 6 take 1 us more than 4, as fewer blocks of more registers run at once
+  constexpr int kAhead = D == 512 ? 4 : 6;
   __shared__ float4 part[kWide ? kGroups : 1][kWide ? D / 4 : 1];
   griddep_wait();
   griddep_launch_dependents();
