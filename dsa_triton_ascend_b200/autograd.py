@@ -193,7 +193,11 @@ class RotaryEmbeddingFunction(torch.autograd.Function):
 
 class RotaryEmbeddingAxesFunction(torch.autograd.Function):
     """out = rotary_embedding_axes(x, table, positions, sections, layout, order, offset, inverse); the
-    gradient of ``x`` turns the other way, as for :class:`RotaryEmbeddingFunction`."""
+    gradient of ``x`` turns the other way, as for :class:`RotaryEmbeddingFunction`.
+
+    To capture a backward pass into a CUDA graph, run the step on a side stream first and let no graph that
+    autograd made of the same leaves outside live on: torch's engine waits for the stream of a leaf that
+    such a graph keeps, which a capture cannot."""
 
     @staticmethod
     def forward(ctx, x, table, positions, sections, layout="interleaved", order="blocks", offset=0, inverse=False):

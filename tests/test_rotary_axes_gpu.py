@@ -231,3 +231,33 @@ def test_captured_on_another_stream_and_after(layout):
     pos.copy_(89 - pos)
     graph.replay()
     assert torch.equal(got, call()) and not torch.equal(got, ref)
+
+
+@pytest.mark.parametrize("order", ["blocks", "cycled"])
+def test_backward_captured(order):
+    """A step of forward and backward in a graph, run on a side stream before the capture; no graph of
+    autograd's own outlives its run."""
+    g = _gen(6)
+    x = torch.randn(3, 5, 8, 64, generator=g, device="cuda").half().requires_grad_()
+    w = torch.randn(3, 5, 8, 64, generator=g, device="cuda").half()
+    pos = torch.randint(0, 50, (2, 3, 5), generator=g, device="cuda", dtype=torch.int32)
+    table = dsa.rotary_table(50, 64)
+
+    def step():
+        out = dsa.RotaryEmbeddingAxesFunction.apply(x, table, pos, (17, 15), "half", order)
+        return torch.autograd.grad(out, x, w)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(2):
+        pos.copy_(49 - pos)
+        w.neg_()
+        graph.replay()
+        assert torch.equal(got, dsa.rotary_embedding_axes(w, table, pos, (17, 15), "half", order, inverse=True))
