@@ -70,10 +70,6 @@ struct Item {
 };
 struct ItemArgs : Args {
   const Item* items;      // [rows]
-  const int32_t* limit;   // CTAs (or pairs) that take part
-  // The second launch may run beside the first: that one lets it start once the plan is there, and it
-  // ends after that one, so that what follows it has both.
-  bool second;
 };
 
 __device__ __forceinline__ int row_keys(const ItemArgs& a, int row) { return a.items[row].keys; }
@@ -106,18 +102,6 @@ template <int NH>
 __device__ __forceinline__ int64_t own_place(const ItemArgs& a, int shares, int row) {
   return (int64_t)2 * shares * NH + a.items[row].place;
 }
-// The stream's kernels before this one have ended: before anything of theirs is read, and before the end.
-// The next kernel may start once that is so (where pieces wait for it, at once, else after the division).
-__device__ __forceinline__ void wait_first(const Args&) { griddep_wait(); }
-__device__ __forceinline__ void wait_first(const ItemArgs& a) {
-  if (!a.second) griddep_wait();
-  griddep_launch_dependents();
-}
-__device__ __forceinline__ void wait_last(const Args&) {}
-__device__ __forceinline__ void wait_last(const ItemArgs& a) {
-  if (a.second) griddep_wait();
-}
-
 template <int kTile, int kCost, typename A>
 __device__ __forceinline__ int row_units(const A& a, int row) {
   const int tiles = (row_keys(a, row) + kTile - 1) / kTile;
@@ -262,20 +246,6 @@ __device__ __forceinline__ Work share_of(const A& a, int cta, int ctas_max, bool
   work.row = start[0];
   work.unit = start[1];
   return work;
-}
-
-// The same, of as many CTAs as take part, and the next kernel let start.
-template <int kTile, int kCost, int kThreads>
-__device__ __forceinline__ Work take_share(const Args& a, int cta, int grid, bool first_cta, int* tmp, int32_t* start) {
-  const Work work = share_of<kTile, kCost, kThreads>(a, cta, grid, first_cta, tmp, start);
-  griddep_launch_dependents();
-  return work;
-}
-template <int kTile, int kCost, int kThreads>
-__device__ __forceinline__ Work take_share(const ItemArgs& a, int cta, int grid, bool first_cta, int* tmp, int32_t* start) {
-  const int limit = min(grid, *a.limit);
-  if (cta >= limit) return Work{0, 0, 0};
-  return share_of<kTile, kCost, kThreads>(a, cta, limit, first_cta, tmp, start);
 }
 
 // The statistics of one (row, head): raw maximum `top`, sum over the exponents' reference `ref`,

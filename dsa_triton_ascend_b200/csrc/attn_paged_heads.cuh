@@ -139,8 +139,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (base & 1023u) {
     if (threadIdx.x == 0) report_error(a.error_flag, kErrMisaligned);
-    wait_first(a);
-    wait_last(a);
+    griddep_wait();   // (this kernel's end stands for the one's before it)
     return;
   }
   if (threadIdx.x == 0) {
@@ -161,7 +160,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     fence_mbarrier_init();
   }
   if (warp == kQkWarp) tmem_alloc<1>(smem_u32(tmem_ptr), C::kTmem);
-  wait_first(a);   // what the stream's kernels before this one wrote may be read from here on
+  griddep_wait();   // what the stream's kernels before this one wrote may be read from here on
 
   if (threadIdx.x == kLoadWarp * 32) {
     tma_prefetch_desc(&maps.k);
@@ -169,9 +168,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&maps.q);
     tma_prefetch_desc(&maps.qr);
   }
-  Work work = take_share<kTile, kSegmentCost, kThreads>(a, blockIdx.x, gridDim.x, blockIdx.x == 0, tmp, start);
+  Work work = share_of<kTile, kSegmentCost, kThreads>(a, blockIdx.x, gridDim.x, blockIdx.x == 0, tmp, start);
   tc_fence_before();
   __syncthreads();
+  griddep_launch_dependents();   // with this CTA's tensor memory taken: the next kernel may take some before it waits
   tc_fence_after();
   const uint32_t tmem = *tmem_ptr;
   const uint32_t t_o = tmem + 4 * NH;
@@ -565,7 +565,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_relinquish<1>();
     tmem_dealloc<1>(tmem, C::kTmem);
   }
-  wait_last(a);
 }
 
 }  // namespace attn_paged

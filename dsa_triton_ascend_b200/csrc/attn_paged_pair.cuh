@@ -106,8 +106,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (base & 1023u) {   // the same in both CTAs
     if (threadIdx.x == 0) report_error(a.error_flag, kErrMisaligned);
-    wait_first(a);
-    wait_last(a);
+    griddep_wait();   // (this kernel's end stands for the one's before it)
     return;
   }
   const uint32_t rank = cluster_ctarank();
@@ -129,7 +128,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     fence_mbarrier_init();
   }
   if (warp == kMmaWarp) tmem_alloc<2>(smem_u32(tmem_ptr), C::kTmem);
-  wait_first(a);
+  griddep_wait();
   if (threadIdx.x == kKeyWarp * 32) {
     tma_prefetch_desc(&maps.k);
     tma_prefetch_desc(&maps.kr);
@@ -137,10 +136,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&maps.q);
     tma_prefetch_desc(&maps.qr);
   }
-  Work work = take_share<kTile, kSegmentCost, kThreads>(a, blockIdx.x >> 1, gridDim.x >> 1, blockIdx.x == 0, tmp, start);
+  Work work = share_of<kTile, kSegmentCost, kThreads>(a, blockIdx.x >> 1, gridDim.x >> 1, blockIdx.x == 0, tmp, start);
   tc_fence_before();
   __syncthreads();
   cluster_sync();
+  griddep_launch_dependents();   // with this CTA's tensor memory taken: the next kernel may take some before it waits
   tc_fence_after();
   const uint32_t tmem = *tmem_ptr;
   bool failed = false;
@@ -543,7 +543,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     tmem_relinquish<2>();
     tmem_dealloc<2>(tmem, C::kTmem);
   }
-  wait_last(a);
 }
 
 }  // namespace pair

@@ -10,16 +10,16 @@
 //
 // Four launches: shared_plan_kernel makes the pieces from the lengths, in one block, so that a captured call
 // follows them; a kernel of attn_paged.cu takes the prefixes' pieces, 64 or 128 heads each, bound by
-// products; another one, of the size that a row's own heads need, the rests, bound by memory.  The two
-// run side by side: the plan divides the multiprocessors between them by what they cost, and the
-// second starts where the first leaves some.  A group shares the whole pages of its prefix, at most as
+// products; another one, of the size that a row's own heads need, the rests, bound by memory.  Each
+// waits for the one before it, as only that is promised to show it what that one and the plan wrote: the
+// second does not run beside the first.  A group shares the whole pages of its prefix, at most as
 // many as all of its rows see, where that costs less than its rows by themselves.
 //
-// Measured (replayed from a graph, against attn_paged.cu alone): 64 rows of 16 heads, D = 512, with 32811 shared
-// and 17 to 2048 own keys, 108 us against 309; 84 rows of 20 heads in five groups, 9 of them alone, 74
-// against 98; 24 rows x 2 tokens of 32 heads, D = 256, in two groups, 47 against 53.  Of the 108: plan 4.6, the pieces'
-// tiles from 8 to 83 in 62 CTA pairs (3,645 cycles for 128 keys and 128 heads, 2,176 of them products)
-// beside the rests in 24 CTAs, results to 94, join 7.  In one launch, all in pieces of 128 heads, it took 123.
+// Measured (against attn_paged.cu alone): 64 rows of 16 heads, D = 512, with 32811 shared and 17 to 2048 own
+// keys, 119 us against 309; 84 rows of 20 heads in five groups, 9 of them alone, 82 against 98; 24 rows x 2 tokens
+// of 32 heads, D = 256, in two groups, 56 against 55.  The pair kernel's tile of 128 keys and 128 heads takes 3,645
+// cycles, 2,176 of them products.  (Beside one another, the second launch reading the plan before a wait of its
+// own, the two took 108, 72 and 47.)
 #include <cuda_runtime.h>
 
 #include <type_traits>
@@ -42,28 +42,22 @@ constexpr int kPlanGroups = 1024;
 constexpr int64_t kMaxGroups = 1 << 30;
 
 // What a launch of either kind is made of: keys of a tile (1 << shift), units of starting a piece,
-// multiprocessors of a share; and in cycles what a tile takes, a piece's start and end, and a launch's.
+// multiprocessors of a share; and in cycles what a tile takes, and a piece's start and end.
 struct Kind {
-  int32_t shift, start, sms, cost, piece, fixed;
-};
-
-// What the plan tells the join: shares of either launch, units of all pieces.
-struct Limits {
-  int32_t shares, rest_shares, units, unused;
+  int32_t shift, start, sms, cost, piece;
 };
 
 struct PlanArgs {
   Args a;            // of the rest
   Item* pieces;      // [most]
   Item* rest;        // [rows]
-  Limits* limits;
   int4* by_row;      // [batch]: shared keys (0: none), first piece, first token of the row's group, first unit
   int4* by_group;    // [groups]: shared keys, pieces, first row with keys, first piece
   int32_t* by_units; // [groups]: first unit
   const int32_t* starts;
   const int32_t* prefixes;
   int32_t groups, batch, s1, packed;   // packed: tokens of a row of the rest
-  int32_t most, per_item, nh, sms;     // pieces at most; tokens and places of each
+  int32_t most, per_item, nh;          // pieces at most; tokens and places of each
   Kind prefix, own;
   int32_t own_rows;                    // rows of the rest of a batch row
   int64_t least_saving;
@@ -89,13 +83,11 @@ __device__ __forceinline__ int units_of(const Kind& k, int keys) { return keys >
 
 // One block: what the inputs hold is fetched at once and held in shared memory where it fits, since each
 // trip to memory, each barrier and each line of code takes its time here, and nothing else does.
-// (Sums are of whole numbers, so that the division of the work does not depend on their order.)
 __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const __grid_constant__ PlanArgs p) {
   __shared__ int4 group_room[kPlanGroups];
   __shared__ int unit_room[kPlanGroups], start_room[kPlanGroups + 1];
   __shared__ int seen_room[kPlanRows], shared_room[kPlanRows];
   __shared__ unsigned long long saved;
-  __shared__ int tiles[2], count[2];   // of the pieces and of the rest
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   constexpr int kWarps = kPlanThreads / 32;
   griddep_wait();
@@ -104,10 +96,7 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const __grid_
   int4* by_group = groups_here ? group_room : p.by_group;
   int* by_units = groups_here ? unit_room : p.by_units;
   const int32_t* starts = groups_here ? start_room : p.starts;
-  if (tid == 0) {
-    saved = 0;
-    tiles[0] = tiles[1] = count[0] = count[1] = 0;
-  }
+  if (tid == 0) saved = 0;
   bool bad = false;
 #pragma unroll 1
   for (int g = tid; g <= p.groups; g += kPlanThreads) {
@@ -178,7 +167,6 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const __grid_
       pieces += __shfl_sync(0xffffffffu, n, 31);
       all += __shfl_sync(0xffffffffu, u, 31);
     }
-    if (lane == 0) count[0] = pieces, tiles[0] = all - pieces * p.prefix.start;
   }
   __syncthreads();
 #pragma unroll 1
@@ -200,42 +188,10 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const __grid_
     }
   }
   __syncthreads();
-  int rest = 0, rows = 0;
 #pragma unroll 1
   for (int r = tid; r < p.a.rows; r += kPlanThreads) {
     const int b = r / p.a.s1, n = row_keys(p.a, r), shared = n > 0 ? rows_here ? shared_room[b] : p.by_row[b].x : 0;
     p.rest[r] = Item{n - shared, shared, b, r * p.a.n1, p.a.n1, shared > 0 || p.a.diag > 0, r * p.a.n1, 0};
-    rest += tiles_of(p.own, n - shared);
-    rows += n > shared;
-  }
-  rest = __reduce_add_sync(0xffffffffu, rest);
-  rows = __reduce_add_sync(0xffffffffu, rows);
-  if (lane == 0 && rest) {
-    atomicAdd(&tiles[1], rest);
-    atomicAdd(&count[1], rows);
-  }
-  __syncthreads();
-  if (warp == 0) {
-    // so many multiprocessors for the pieces that both launches end as early as may be
-    const float a = (float)tiles[0] * p.prefix.cost + (float)count[0] * p.prefix.piece;
-    const float b = (float)tiles[1] * p.own.cost + (float)count[1] * p.own.piece;
-    const int all = p.sms / p.prefix.sms;
-    float best = INFINITY;
-    int n = 0;
-#pragma unroll 1
-    for (int k = lane + 1; k <= all && a > 0.0f; k += 32) {
-      const int m = (p.sms - k * p.prefix.sms) / p.own.sms;
-      const float t = fmaxf(p.prefix.fixed + a / k, b > 0.0f ? p.own.fixed + b / max(m, 1) + (m < 1 ? a : 0.0f) : 0.0f);
-      if (t < best) best = t, n = k;
-    }
-#pragma unroll 1
-    for (int o = 16; o > 0; o >>= 1) {
-      const float t = __shfl_xor_sync(0xffffffffu, best, o);
-      const int k = __shfl_xor_sync(0xffffffffu, n, o);
-      if (t < best || (t == best && k < n)) best = t, n = k;
-    }
-    if (lane == 0) *p.limits = Limits{max(n, 1), max((p.sms - n * p.prefix.sms) / p.own.sms, 1),
-                                        tiles[0] + count[0] * p.prefix.start, 0};
   }
 }
 
@@ -243,9 +199,9 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const __grid_
 struct SharedParts {
   const float* ws_o;
   const float4* ws_s;
-  const Limits* limits;
+  const int32_t* units;   // of all pieces
   const int4* by_row;
-  int32_t shares, nh;   // shares of the launch, heads of a piece
+  int32_t shares, nh;     // shares of the launch, heads of a piece
   Kind kind;
   rotary::FastDiv n1, s1, heads, per_item;   // heads and tokens of a row, heads of a token, tokens of a piece
 };
@@ -273,7 +229,7 @@ __global__ void __launch_bounds__(kJoinThreads)
   const int t = threadIdx.x % kLanes, grp = t / kCols, col = t % kCols, lane = threadIdx.x & 31;
   T* out = static_cast<T*>(a.out) + at * D;
   const int4 g = sp.by_row[b];
-  const Limits limits = *sp.limits;
+  const int piece_units = *sp.units;
   const int first = a.ws_prefix[row], count = a.ws_prefix[row + 1] - first, all = a.ws_prefix[a.rows];
   const int64_t cap = (int64_t)a.max_blocks * a.page_size, ak = a.act_k[b];
   const int tokens = (int)sp.heads.div(a.n1), s = (int)sp.heads.div(head);   // of a packed row, and the one of this head
@@ -286,12 +242,12 @@ __global__ void __launch_bounds__(kJoinThreads)
   // the row's own parts, then those of the piece of which it is head `head2`
   Parts p{1, 0, 0, (int64_t)2 * grid * NH + (int64_t)row * a.n1}, p2{1, 0, 0, 0};
   int head2 = 0;
-  if (count > 0) find_parts(first, count, all, kCost, min(grid, limits.rest_shares), &p);
+  if (count > 0) find_parts(first, count, all, kCost, grid, &p);
   if (g.x > 0 && seen > 0) {
     const int token = row * tokens + s - g.z, item = (int)sp.per_item.div(token), units = units_of(sp.kind, g.x);
     head2 = (token - item * (int)sp.per_item.d) * a.heads + head - s * a.heads;
     p2.own = (int64_t)(2 * sp.shares + g.y + item) * sp.nh;
-    find_parts(g.w + item * units, units, limits.units, sp.kind.start, min(sp.shares, limits.shares), &p2);
+    find_parts(g.w + item * units, units, piece_units, sp.kind.start, sp.shares, &p2);
   }
   const int n1 = p.c1 - p.c0 + 1, n = n1 + p2.c1 - p2.c0 + 1;
   if (a.diag == 0 && n == 1 && n1 == 1 && p.c0 == p.c1 && g.x == 0) return;   // written whole
@@ -385,7 +341,7 @@ struct Layout {
   int nh, own_nh, packed;
   int64_t per_item, most, rest, shares, own_shares, places, own_places;
   int64_t lists(int64_t batch, int64_t groups) const {   // bytes of what the plan makes
-    return align256((most + rest) * (int64_t)sizeof(Item)) + align256((batch + groups) * 16 + groups * 4) + 256;
+    return align256((most + rest) * (int64_t)sizeof(Item)) + align256((batch + groups) * 16 + groups * 4);
   }
   int64_t bytes(int64_t d, int64_t batch, int64_t groups) const {
     return align256((places + own_places) * (d * 4 + 16) + (most + rest + 2) * 4) + lists(batch, groups);
@@ -414,13 +370,13 @@ Layout layout_of(int64_t batch, int64_t s1, int64_t n1, int64_t d, int64_t group
 bool can_share(const Layout& l) { return l.per_item > l.packed; }
 
 // The kernel for `nh` heads, in cycles: a tile (the slope over rows of 4096 and 12288 keys, or prefixes of
-// 16384 and 49152, that lie in L2), the start and end of a piece (what rows of 400 and 1100 keys take
-// beyond their tiles) and of a launch.
+// 16384 and 49152, that lie in L2), and the start and end of a piece (what rows of 400 and 1100 keys take
+// beyond their tiles).
 Kind kind_of(int nh, int64_t d) {
-  if (nh == 128 && d == 512) return {7, pair::kSegmentCost, 2, 4350, 17000, 15000};
-  if (nh == 128) return {6, wide::kSegmentCost, 1, 1850, 12000, 13000};
+  if (nh == 128 && d == 512) return {7, pair::kSegmentCost, 2, 4350, 17000};
+  if (nh == 128) return {6, wide::kSegmentCost, 1, 1850, 12000};
   const int tile = d == 512 ? (nh == 64 ? 3000 : nh == 32 ? 2600 : 2400) : d == 256 ? (nh == 64 ? 1650 : 1450) : (nh == 64 ? 1600 : 1400);
-  return {6, kSegmentCost, 1, tile, 12000, 14000};
+  return {6, kSegmentCost, 1, tile, 12000};
 }
 static_assert(pair::kTile == 128 && wide::kTile == 64 && kTile == 64, "kind_of has the tiles' sizes");
 
@@ -490,14 +446,13 @@ int launch_shared(const DsaAttnSharedParams* sp, const Layout& l, cudaStream_t s
   own.ws_prefix = pre.ws_prefix + l.most + 1;
   uint8_t* ws = static_cast<uint8_t*>(p->workspace) + align256((l.places + l.own_places) * (D * 4 + 16) + (l.most + l.rest + 2) * 4);
   PlanArgs plan;
-  plan.limits = reinterpret_cast<Limits*>(ws);
-  plan.pieces = reinterpret_cast<Item*>(ws + 256);
+  plan.pieces = reinterpret_cast<Item*>(ws);
   plan.rest = plan.pieces + l.most;
-  plan.by_row = reinterpret_cast<int4*>(ws + 256 + align256((l.most + l.rest) * (int64_t)sizeof(Item)));
+  plan.by_row = reinterpret_cast<int4*>(ws + align256((l.most + l.rest) * (int64_t)sizeof(Item)));
   plan.by_group = plan.by_row + p->batch;
   plan.by_units = reinterpret_cast<int32_t*>(plan.by_group + sp->groups);
-  pre.items = plan.pieces, pre.limit = &plan.limits->shares, pre.second = false;
-  own.items = plan.rest, own.limit = &plan.limits->rest_shares, own.second = true;
+  pre.items = plan.pieces;
+  own.items = plan.rest;
   plan.a = own;
   plan.starts = sp->group_starts;
   plan.prefixes = sp->prefix_lengths;
@@ -509,7 +464,6 @@ int launch_shared(const DsaAttnSharedParams* sp, const Layout& l, cudaStream_t s
   plan.most = (int)l.most;
   plan.per_item = (int)l.per_item;
   plan.nh = l.nh;
-  plan.sms = sm_count();
   plan.prefix = kind_of(l.nh, D);
   plan.own = kind_of(l.own_nh, D);
   plan.least_saving = sp->least_saving;
@@ -517,7 +471,7 @@ int launch_shared(const DsaAttnSharedParams* sp, const Layout& l, cudaStream_t s
   int rc = launch_pieces<D, T>(&flat, l.nh, (int)l.shares, pre, stream);
   if (rc == DSA_OK) rc = launch_pieces<D, T>(&flat, l.own_nh, (int)l.own_shares, own, stream);
   if (rc != DSA_OK) return rc;
-  const SharedParts parts{pre.ws_o, pre.ws_s, plan.limits, plan.by_row, (int)l.shares, l.nh, plan.prefix,
+  const SharedParts parts{pre.ws_o, pre.ws_s, pre.ws_prefix + l.most, plan.by_row, (int)l.shares, l.nh, plan.prefix,
                           rotary::FastDiv((uint32_t)own.n1), rotary::FastDiv((uint32_t)own.s1),
                           rotary::FastDiv((uint32_t)own.heads), rotary::FastDiv((uint32_t)l.per_item)};
   auto join = [&](auto nh, auto cost) -> int {

@@ -199,8 +199,7 @@ __global__ void __launch_bounds__(kThreads) plan_rows_kernel(const __grid_consta
             (int64_t)(gridDim.x - a.token_blocks) * kWarps);
 }
 
-// Lengths, ends and groups, by one block of kBlock threads.  What does not hang on the comparisons is done
-// before `wait`, which returns when they are made.
+// Lengths, ends and groups, by one block of kBlock threads.  `wait` returns when the comparisons are made.
 template <int kBlock, typename Wait>
 __device__ __forceinline__ void plan_groups(const Args& a, Wait wait) {
   const DsaBatchPlanParams& p = a.p;
@@ -251,9 +250,10 @@ __device__ __forceinline__ void plan_groups(const Args& a, Wait wait) {
   }
 }
 
-// (The kernel above has let this one start after its own wait, so the inputs are there.)
+// (Nothing is read before the wait: what the kernel above has waited for is not yet this one's to see.)
 __global__ void __launch_bounds__(kGroupThreads) plan_groups_kernel(const __grid_constant__ Args a) {
-  plan_groups<kGroupThreads>(a, [] { griddep_wait(); });
+  griddep_wait();
+  plan_groups<kGroupThreads>(a, [] {});
 }
 
 // All of a small step by one cluster: the groups by its first CTA, tokens by the last ones.
