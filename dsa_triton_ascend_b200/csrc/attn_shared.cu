@@ -117,6 +117,7 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const __grid_
   const bool none = __syncthreads_or(bad);   // groups that are no division of the batch are not used
   if (none && tid == 0) report_error(p.a.error_flag, kErrBadIndex);
   const int groups = none ? 0 : p.groups;
+  const bool any = p.least_saving < 0;   // whatever sharing costs
 
 #pragma unroll 1
   for (int g = warp; g < groups; g += kWarps) {
@@ -141,12 +142,12 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const __grid_
       // shared where its pieces cost less than its keys do in its rows
       const long long less = (long long)own * tiles_of(p.own, keys) * p.own.cost -
                              (long long)items * ((long long)tiles_of(p.prefix, keys) * p.prefix.cost + p.prefix.piece) * p.prefix.sms;
-      by_group[g] = less > 0 ? make_int4(keys, items, lead, 0) : make_int4(0, 0, 0, 0);
+      by_group[g] = less > 0 || (any && keys > 0) ? make_int4(keys, items, lead, 0) : make_int4(0, 0, 0, 0);
       if (less > 0) atomicAdd(&saved, (unsigned long long)less);
     }
   }
   __syncthreads();
-  const int sharing = (long long)saved > p.least_saving ? groups : 0;
+  const int sharing = any || (long long)saved > p.least_saving ? groups : 0;
   if (warp == 0) {
     int pieces = 0, all = 0;
 #pragma unroll 1
@@ -523,7 +524,7 @@ extern "C" int dsa_attn_shared(const DsaAttnSharedParams* sp, void* stream_) {
   const DsaAttnPagedParams* p = &sp->attn;
   if (p->batch == 0 || p->s1 == 0) return DSA_OK;
   constexpr int64_t kMax = 0x7fffffff;
-  if (!valid_params(p, kTile) || sp->groups > kMaxGroups || sp->least_saving < 0 || (sp->groups > 0 && (!sp->group_starts || !sp->prefix_lengths)) ||
+  if (!valid_params(p, kTile) || sp->groups > kMaxGroups || (sp->groups > 0 && (!sp->group_starts || !sp->prefix_lengths)) ||
       p->workspace_bytes < dsa_attn_shared_workspace_size(p->batch, p->s1, p->n1, p->d, sp->groups))
     return DSA_ERR_INVALID_ARG;
   if (sp->groups > 0) {

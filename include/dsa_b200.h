@@ -465,7 +465,8 @@ int dsa_attn_paged_shares_keys(int64_t s1, int64_t n1);
  * Where a token has more than 64 heads nothing is shared; where something can be, all heads of query
  * and of query_rope lie one step apart, across tokens and rows.  A prefix is shared where that takes
  * fewer cycles than its rows by themselves, and anything only where it saves more than least_saving
- * (cycles of one multiprocessor, >= 0) altogether.
+ * (cycles of one multiprocessor) altogether; with a negative least_saving each prefix of a page or more,
+ * whatever that costs.
  * Workspace: dsa_attn_shared_workspace_size() bytes.
  */
 typedef struct DsaAttnSharedParams {
