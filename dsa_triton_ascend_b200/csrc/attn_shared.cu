@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const __grid_
       const uint32_t tokens = (uint32_t)(to - from) * p.s1, own = (uint32_t)rows * p.own_rows;
       const int items = (int)((tokens + p.per_item - 1) / (uint32_t)p.per_item);
       // shared where its pieces cost less than its keys do in its rows
-      const long long less = (long long)own * tiles_of(p.own, keys) * p.own.cost -
+      const long long less = (long long)own * tiles_of(p.own, keys) * p.own.cost * p.own.sms -
                              (long long)items * ((long long)tiles_of(p.prefix, keys) * p.prefix.cost + p.prefix.piece) * p.prefix.sms;
       by_group[g] = less > 0 || (any && keys > 0) ? make_int4(keys, items, lead, 0) : make_int4(0, 0, 0, 0);
       if (less > 0) atomicAdd(&saved, (unsigned long long)less);
