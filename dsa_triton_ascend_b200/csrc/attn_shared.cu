@@ -37,7 +37,7 @@ namespace dsa {
 namespace attn_paged {
 
 constexpr int kPlanThreads = 512;
-constexpr int kPlanRows = 2048;     // batch rows and groups whose lists fit into shared memory
+constexpr int kPlanRows = 1984;     // batch rows and groups whose lists fit into shared memory
 constexpr int kPlanGroups = 1024;
 constexpr int64_t kMaxGroups = 1 << 30;
 
@@ -51,31 +51,77 @@ struct PlanArgs {
   Args a;            // of the rest
   Item* pieces;      // [most]
   Item* rest;        // [rows]
-  int4* by_row;      // [batch]: shared keys (0: none), first piece, first token of the row's group, first unit
+  // [batch]: shared keys (0: none), first token of the row's group, and what to add to the number of a
+  // window of the group for its piece, and to that number times a piece's units for the piece's first one
+  int4* by_row;
   int4* by_group;    // [groups]: shared keys, pieces, first row with keys, first piece
   int32_t* by_units; // [groups]: first unit
   const int32_t* starts;
   const int32_t* prefixes;
   int32_t groups, batch, s1, packed;   // packed: tokens of a row of the rest
   int32_t most, per_item, nh;          // pieces at most; tokens and places of each
+  rotary::FastDiv item;                // by per_item
   Kind prefix, own;
-  int32_t own_rows;                    // rows of the rest of a batch row
   int64_t least_saving;
 };
 
-// Keys that the first token of batch row b with any sees (0: no token of the row sees one).
-__device__ __forceinline__ int least_seen(const PlanArgs& p, int b) {
-  const int ak = p.a.act_k[b], aq = p.a.act_q ? p.a.act_q[b] : p.s1;
+// Of the s1 tokens of a batch row with `ak` keys and `aq` queries those that see a key are
+// first .. first + tokens - 1; the first of them sees `keys` (0: no token sees one).
+struct Seen {
+  int first, tokens, keys;
+};
+__device__ __forceinline__ Seen seen_of(const PlanArgs& p, int ak, int aq) {
   const int cap = p.a.max_blocks * p.a.page_size;   // (below 2^31, as the host has seen to)
-  if (ak <= 0 || aq <= 0) return 0;
-  int64_t n = ak;
+  int64_t first = 0, n = ak;
   if (p.a.mode == 3) {
-    n = (int64_t)ak - aq + 1;
-    if (n - 1 + min(p.s1, aq) < 1) return 0;   // (more queries counted than there are)
-    if (n < 1) n = 1;
+    first = max((int64_t)aq - ak, (int64_t)0);      // (with more queries than keys)
+    n = max((int64_t)ak - aq + 1, (int64_t)1);
   }
-  return (int)(n < cap ? n : cap);
+  const int64_t tokens = min(p.s1, aq) - first;
+  if (ak <= 0 || tokens <= 0) return {0, 0, 0};
+  return {(int)first, (int)tokens, (int)(n < cap ? n : cap)};
 }
+
+// A group's pieces are windows of per_item of its tokens, in the order of the tokens; those without a
+// token that sees a key (of idle rows, or padding) are left out.  Of a batch row: the windows that are
+// in no row of the group before it, first .. first + count - 1, which are the pieces `index` and on, and
+// what a window's number and its piece's differ by.
+struct Windows {
+  int first, count, index, shift;
+};
+struct Counter {
+  int last, pieces;   // the last window so far (-1), how many there are
+};
+__device__ __forceinline__ int windows_up_to(const PlanArgs& p, int tokens) { return (int)p.item.div((uint32_t)tokens + p.per_item - 1); }
+// By a warp, row b of the group each; moves `c` on.
+__device__ __forceinline__ Windows windows_of(const PlanArgs& p, const Seen& seen, int b, Counter& c) {
+  const int lane = threadIdx.x & 31, token = b * p.s1 + seen.first;
+  const bool some = seen.tokens > 0;
+  const int w0 = some ? (int)p.item.div((uint32_t)token) : 0, w1 = some ? (int)p.item.div((uint32_t)(token + seen.tokens - 1)) : -1;
+  int last = max(w1, c.last);
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, last, o);
+    if (lane >= o) last = max(last, y);
+  }
+  int before = __shfl_up_sync(0xffffffffu, last, 1);
+  if (lane == 0) before = c.last;
+  Windows w;
+  w.first = max(w0, before + 1);
+  w.count = some ? w1 + 1 - w.first : 0;
+  int sum = w.count;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += y;
+  }
+  w.index = c.pieces + sum - w.count;
+  w.shift = w.index - w.first;   // (a window that the row before has, too, is the piece before)
+  c.last = __shfl_sync(0xffffffffu, last, 31);
+  c.pieces += __shfl_sync(0xffffffffu, sum, 31);
+  return w;
+}
+
 __device__ __forceinline__ int tiles_of(const Kind& k, int keys) {
   return (int)(((uint32_t)keys + (1u << k.shift) - 1) >> k.shift);
 }
@@ -86,7 +132,8 @@ __device__ __forceinline__ int units_of(const Kind& k, int keys) { return keys >
 __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const __grid_constant__ PlanArgs p) {
   __shared__ int4 group_room[kPlanGroups];
   __shared__ int unit_room[kPlanGroups], start_room[kPlanGroups + 1];
-  __shared__ int seen_room[kPlanRows], shared_room[kPlanRows];
+  __shared__ int2 length_room[kPlanRows];   // keys and queries
+  __shared__ int shared_room[kPlanRows];
   __shared__ unsigned long long saved;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   constexpr int kWarps = kPlanThreads / 32;
@@ -96,6 +143,13 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const __grid_
   int4* by_group = groups_here ? group_room : p.by_group;
   int* by_units = groups_here ? unit_room : p.by_units;
   const int32_t* starts = groups_here ? start_room : p.starts;
+  auto lengths = [&](int b) { return make_int2(p.a.act_k[b], p.a.act_q ? p.a.act_q[b] : p.s1); };
+  // of row `from` + i (none behind `to`)
+  auto seen_at = [&](int from, int i, int to) {
+    if (from + i >= to) return Seen{0, 0, 0};
+    const int2 n = rows_here ? length_room[from + i] : lengths(from + i);
+    return seen_of(p, n.x, n.y);
+  };
   if (tid == 0) saved = 0;
   bool bad = false;
 #pragma unroll 1
@@ -107,7 +161,7 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const __grid_
 #pragma unroll 1
   for (int b = tid; b < p.batch; b += kPlanThreads) {
     if (rows_here) {
-      seen_room[b] = least_seen(p, b);
+      length_room[b] = lengths(b);
       shared_room[b] = 0;
     }
     p.by_row[b] = make_int4(0, 0, 0, 0);
@@ -122,23 +176,31 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const __grid_
 #pragma unroll 1
   for (int g = warp; g < groups; g += kWarps) {
     const int from = starts[g], to = starts[g + 1], prefix = p.prefixes[g];
-    int least = 0x7fffffff, rows = 0, lead = 0x7fffffff;
+    int least = 0x7fffffff, rows = 0, some_tokens = 0, lead = 0x7fffffff;   // those with keys
 #pragma unroll 1
-    for (int b = from + lane; b < to; b += 32) {
-      const int n = rows_here ? seen_room[b] : least_seen(p, b);
-      if (n == 0) continue;
-      least = min(least, n);
-      lead = min(lead, b);
+    for (int i = lane; i < to - from; i += 32) {
+      const Seen seen = seen_at(from, i, to);
+      if (seen.tokens == 0) continue;
+      least = min(least, seen.keys);
+      lead = min(lead, from + i);
       ++rows;
+      some_tokens += seen.tokens;
     }
     least = __reduce_min_sync(0xffffffffu, least);
     lead = __reduce_min_sync(0xffffffffu, lead);
     rows = __reduce_add_sync(0xffffffffu, rows);
+    some_tokens = __reduce_add_sync(0xffffffffu, some_tokens);
+    const int tokens = (to - from) * p.s1, own = p.packed > 1 ? rows : some_tokens;   // own: rows of the rest
+    int items = windows_up_to(p, tokens);
+    if (some_tokens < tokens) {
+      Counter c{-1, 0};
+#pragma unroll 1
+      for (int b0 = 0; b0 < to - from; b0 += 32) windows_of(p, seen_at(from, b0 + lane, to), b0 + lane, c);
+      items = c.pieces;
+    }
     if (lane == 0) {
-      const uint32_t some = rows > 0 ? max(min(prefix, least), 0) : 0;   // (idle rows have no page to read)
+      const uint32_t some = own > 0 ? max(min(prefix, least), 0) : 0;   // (idle rows have no page to read)
       const int keys = (int)(some - some % (uint32_t)p.a.page_size);
-      const uint32_t tokens = (uint32_t)(to - from) * p.s1, own = (uint32_t)rows * p.own_rows;
-      const int items = (int)((tokens + p.per_item - 1) / (uint32_t)p.per_item);
       // shared where its pieces cost less than its keys do in its rows
       const long long less = (long long)own * tiles_of(p.own, keys) * p.own.cost * p.own.sms -
                              (long long)items * ((long long)tiles_of(p.prefix, keys) * p.prefix.cost + p.prefix.piece) * p.prefix.sms;
@@ -175,17 +237,40 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const __grid_
     const int4 group = by_group[g];
     const int from = starts[g], to = starts[g + 1];
     if (group.x == 0) continue;
-    const int first = from * p.s1, tokens = (to - from) * p.s1;
-#pragma unroll 1
-    for (int i = lane; i < group.y; i += 32) {
-      const int t = i * p.per_item, at = group.w + i;
+    const int first = from * p.s1, tokens = (to - from) * p.s1, units = units_of(p.prefix, group.x);
+    auto put_row = [&](int b, int shift) {
+      p.by_row[b] = make_int4(group.x, first, group.w + shift, by_units[g] + shift * units);
+      if (rows_here) shared_room[b] = group.x;
+    };
+    auto put_piece = [&](int at, int window) {
+      const int t = window * p.per_item;
       p.pieces[at] = Item{group.x, 0, group.z, (first + t) * p.a.heads, min(p.per_item, tokens - t) * p.a.heads, 1,
                           at * p.nh, 0};
-    }
+    };
+    if (group.y == windows_up_to(p, tokens)) {   // each window is a piece
 #pragma unroll 1
-    for (int b = from + lane; b < to; b += 32) {
-      p.by_row[b] = make_int4(group.x, group.w, first, by_units[g]);
-      if (rows_here) shared_room[b] = group.x;
+      for (int i = lane; i < group.y; i += 32) put_piece(group.w + i, i);
+#pragma unroll 1
+      for (int b = from + lane; b < to; b += 32) put_row(b, 0);
+      continue;
+    }
+    Counter c{-1, 0};
+#pragma unroll 1
+    for (int b0 = 0; b0 < to - from; b0 += 32) {
+      const int b = from + b0 + lane, done = c.pieces;
+      const Windows w = windows_of(p, seen_at(from, b0 + lane, to), b0 + lane, c);
+      if (b < to) put_row(b, w.shift);
+      // the new pieces of these 32 rows, a lane each: the row of one is the last that begins at it or before
+#pragma unroll 1
+      for (int j0 = done; j0 < c.pieces; j0 += 32) {
+        const int j = j0 + lane;
+        int r = 0;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+          if (__shfl_sync(0xffffffffu, w.index, r + o) <= j) r += o;
+        const int shift = __shfl_sync(0xffffffffu, w.shift, r);
+        if (j < c.pieces) put_piece(group.w + j, j - shift);
+      }
     }
   }
   __syncthreads();
@@ -245,9 +330,9 @@ __global__ void __launch_bounds__(kJoinThreads)
   int head2 = 0;
   if (count > 0) find_parts(first, count, all, kCost, grid, &p);
   if (g.x > 0 && seen > 0) {
-    const int token = row * tokens + s - g.z, item = (int)sp.per_item.div(token), units = units_of(sp.kind, g.x);
+    const int token = row * tokens + s - g.y, item = (int)sp.per_item.div(token), units = units_of(sp.kind, g.x);
     head2 = (token - item * (int)sp.per_item.d) * a.heads + head - s * a.heads;
-    p2.own = (int64_t)(2 * sp.shares + g.y + item) * sp.nh;
+    p2.own = (int64_t)(2 * sp.shares + g.z + item) * sp.nh;
     find_parts(g.w + item * units, units, piece_units, sp.kind.start, sp.shares, &p2);
   }
   const int n1 = p.c1 - p.c0 + 1, n = n1 + p2.c1 - p2.c0 + 1;
@@ -461,9 +546,9 @@ int launch_shared(const DsaAttnSharedParams* sp, const Layout& l, cudaStream_t s
   plan.batch = (int)p->batch;
   plan.s1 = (int)p->s1;
   plan.packed = l.packed;
-  plan.own_rows = (int)p->s1 / l.packed;
   plan.most = (int)l.most;
   plan.per_item = (int)l.per_item;
+  plan.item = rotary::FastDiv((uint32_t)l.per_item);
   plan.nh = l.nh;
   plan.prefix = kind_of(l.nh, D);
   plan.own = kind_of(l.own_nh, D);

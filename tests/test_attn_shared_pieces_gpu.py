@@ -143,6 +143,18 @@ def test_ragged_counts(mode, heads, d):
     c.run(mode, act_q=counts)
 
 
+@pytest.mark.parametrize("rows,s1,heads,d", [(90, 5, 8, 512), (100, 3, 50, 128), (40, 70, 16, 256), (2100, 2, 4, 128), (700, 1, 9, 128)])
+def test_ragged_counts_of_many_rows(rows, s1, heads, d):
+    """Windows of several rows, rows of several windows, gaps of whole windows; batches past what the plan
+    holds in shared memory."""
+    rng = random.Random(rows)
+    few = [rng.choice([0, 0, 1, rng.randint(0, s1), s1]) if (b // 19) % 3 else 0 for b in range(rows)]
+    own = [None if n == 0 and rng.random() < 0.5 else rng.randint(s1, s1 + 40) for n in few]
+    cut = rows // 3
+    c = Pieces([(64, own[:cut]), (40, own[cut:])], (), heads, d, 8 if d == 128 else 32, s1=s1, seed=rows)
+    c.run(rng.choice([0, 3]), act_q=few)               # (of 40 rows the first group is idle)
+
+
 def test_prefixes_of_any_length():
     """Longer than the rows, below zero, none, a part of a page, less than is shared."""
     c = Pieces([(200, [20, 30, 40]), (200, [5, 6]), (200, [7, 8]), (200, [9, 1])], (), 16, 128, 32, seed=1)
