@@ -456,11 +456,12 @@ Layout layout_of(int64_t batch, int64_t s1, int64_t n1, int64_t d, int64_t group
 bool can_share(const Layout& l) { return l.per_item > l.packed; }
 
 // The kernel for `nh` heads, in cycles: a tile (the slope over rows of 4096 and 12288 keys, or prefixes of
-// 16384 and 49152, that lie in L2), and the start and end of a piece (what rows of 400 and 1100 keys take
-// beyond their tiles).
+// 16384 and 49152, that lie in L2), and the start and end of a piece with its parts in the join (what rows of
+// 400 and 1100 keys take beyond their tiles; of 128 heads at D >= 256 what fits 350 calls of 4 to 64 rows over 1024
+// to 32768 shared keys best).
 Kind kind_of(int nh, int64_t d) {
-  if (nh == 128 && d == 512) return {7, pair::kSegmentCost, 2, 4350, 17000};
-  if (nh == 128) return {6, wide::kSegmentCost, 1, 1850, 12000};
+  if (nh == 128 && d == 512) return {7, pair::kSegmentCost, 2, 4350, 37000};
+  if (nh == 128) return {6, wide::kSegmentCost, 1, 1850, d == 256 ? 32000 : 12000};
   const int tile = d == 512 ? (nh == 64 ? 3000 : nh == 32 ? 2600 : 2400) : d == 256 ? (nh == 64 ? 1650 : 1450) : (nh == 64 ? 1600 : 1400);
   return {6, kSegmentCost, 1, tile, 12000};
 }
@@ -552,7 +553,9 @@ int launch_shared(const DsaAttnSharedParams* sp, const Layout& l, cudaStream_t s
   plan.nh = l.nh;
   plan.prefix = kind_of(l.nh, D);
   plan.own = kind_of(l.own_nh, D);
-  plan.least_saving = sp->least_saving;
+  // keys of later tokens cost this join more than the other one (64 x 5 tokens of 16 heads, D = 512: 39 us against 19)
+  const bool late = diag > 0 && D == 512 && sp->least_saving > 0;
+  plan.least_saving = sp->least_saving + (late ? 700 * p->batch * p->s1 * p->n1 : 0);
   if (!launch_early(shared_plan_kernel, 1, kPlanThreads, 0, stream, plan)) return DSA_ERR_CUDA;
   int rc = launch_pieces<D, T>(&flat, l.nh, (int)l.shares, pre, stream);
   if (rc == DSA_OK) rc = launch_pieces<D, T>(&flat, l.own_nh, (int)l.own_shares, own, stream);
@@ -614,14 +617,17 @@ extern "C" int dsa_attn_shared(const DsaAttnSharedParams* sp, void* stream_) {
     return DSA_ERR_INVALID_ARG;
   if (sp->groups > 0) {
     const Layout l = layout_of(p->batch, p->s1, p->n1, p->d, sp->groups, packs(p->s1, p->n1) && !p->act_q);
-    // Small calls are left to the other operator, by what the tables can hold: the plan and the pieces' launch
-    // take 4 us where nothing is shared, and 16 heads, D = 512, begin to gain at 3.5 M cycles saved (16 rows
-    // with 8192 shared keys: 34 us against 37; 8 rows: 32 against 27), 64 heads at 1.5 to 3 M.
-    const Kind own = kind_of(l.own_nh, p->d);
-    const double all = (double)l.rest * ((p->max_blocks * p->page_size >> own.shift) + 1) * own.cost * own.sms;
+    // Calls that cannot save enough are left to the other operator, by what the tables hold: with one prefix
+    // of all their keys and a quarter to spare, as the plan, the pieces' launch and this join take 3 to 6 us more
+    // where nothing is shared (up to 25 with later tokens' keys or 64 heads of 64 rows).
+    const Kind own = kind_of(l.own_nh, p->d), pre = kind_of(l.nh, p->d);
+    const int64_t cap = p->max_blocks * p->page_size, pieces = (p->batch * p->s1 + l.per_item - 1) / l.per_item;
+    const double most = (double)l.rest * ((cap >> own.shift) + 1) * own.cost * own.sms -
+                        (double)pieces * ((double)(cap >> pre.shift) * pre.cost + pre.piece) * pre.sms;
+    const bool worth = sp->least_saving <= 0 || most > 1.25 * (double)sp->least_saving;
     // (places, units and the keys of a tile of 128 are counted in 32 bits)
     const int64_t tiles = (p->max_blocks * p->page_size + kTile - 1) / kTile + 8;
-    if (can_share(l) && all > 2.5 * (double)sp->least_saving && l.most * l.nh <= kMax && l.most + l.rest <= kMax / tiles &&
+    if (can_share(l) && worth && l.most * l.nh <= kMax && l.most + l.rest <= kMax / tiles &&
         p->max_blocks * p->page_size <= kMax - pair::kTile) {
       if (!one_matrix(p, p->q_head_stride, p->q_token_stride, p->q_batch_stride) ||
           !one_matrix(p, p->qr_head_stride, p->qr_token_stride, p->qr_batch_stride) || l.shares < 1)

@@ -17,8 +17,12 @@ from ._lib import (BIND_ATTN, BIND_SHARED, AttnPagedParams, AttnSharedParams, bi
 
 _VALID_D = (128, 256, 512)
 _D_ROPE = 64
-# Cycles of one multiprocessor that sharing has to save, as it takes two launches more
-_LEAST_SAVING = 1500000
+# Cycles of one multiprocessor that sharing has to save, as it takes two launches more, one of them to
+# be waited for, and a larger join: times 19, 20 and 14 at D = 512, 256 and 128.  Of 300 calls of 4 to 64 rows, 8 to
+# 80 heads and 1024 to 32768 shared keys 61 save more: 57 gain up to 18 us, 4 lose, 1.8 us of 36 at most.  With
+# nothing saved sharing would cost 9 to 14 us.
+_LEAST_SAVING = 250000
+_LEAST_TIMES = {128: 14, 256: 20, 512: 19}
 _MAX_SCALE = torch.finfo(torch.float32).max
 
 
@@ -210,8 +214,8 @@ def _shared_plan(query, query_rope, key_cache, key_rope_cache, block_table, grou
                          f"got {group_starts.numel()}")
     p = AttnSharedParams()
     p.attn = AttnPagedParams.from_buffer_copy(template)
-    p.groups, p.least_saving = groups, _LEAST_SAVING
     B, S1, N1, D = query.shape
+    p.groups, p.least_saving = groups, _LEAST_SAVING * _LEAST_TIMES[D]
     # pieces of a prefix are runs of heads of neighbouring tokens; queries that lie otherwise are copied
     fits = []
     for t, name, width in ((query, "q", D), (query_rope, "qr", _D_ROPE)):

@@ -32,12 +32,14 @@ def shares(c, mode=0, act_q=None):
     return True
 
 
-@pytest.mark.parametrize("rows,s1,heads,gain", [(64, 5, 16, True), (64, 3, 32, True), (48, 4, 20, True), (32, 7, 16, False)])
-def test_packed_tokens_that_take_two_multiprocessors(rows, s1, heads, gain):
+@pytest.mark.parametrize("rows,s1,heads,shared,gain", [
+    (64, 5, 16, 8192, True), (64, 3, 32, 16384, True), (48, 4, 20, 16384, True),
+    (64, 3, 32, 8192, False), (48, 4, 20, 8192, False), (32, 7, 16, 8192, False)])
+def test_packed_tokens_that_take_two_multiprocessors(rows, s1, heads, shared, gain):
     """65 to 112 heads of packed tokens, D = 512, are taken by pairs of CTAs, and so are pieces: of
-    64 x 5 tokens 40 pieces cost 23.6 M cycles over 8192 keys, the rows 35.6 M; of 32 x 7 tokens 28 pieces
-    16.5 M, the rows 17.8 M, which is less of a difference than a launch more takes."""
-    c = Pieces([(8192, [random.Random(b).randint(s1, 90) for b in range(rows)])], (), heads, 512, 64, s1=s1, seed=s1)
+    64 x 5 tokens 40 pieces cost 25.2 M cycles over 8192 keys, the rows 35.6 M.  The last three lose: 162 us shared
+    against 155, 124 against 122, 125 against 97."""
+    c = Pieces([(shared, [random.Random(b).randint(s1, 90) for b in range(rows)])], (), heads, 512, 64, s1=s1, seed=s1)
     assert shares(c, 3) == gain
 
 
@@ -59,3 +61,15 @@ def test_tokens_before_the_first_key_are_no_work():
                                             actual_seq_lengths_key=c.lens, scale_value=c.scale, actual_seq_lengths_query=[64] * 8,
                                             sparse_mode=3, return_softmax_lse=True)
     c.check(got, 3, [64] * 8)
+
+
+@pytest.mark.parametrize("rows,heads,d,shared,gain", [
+    (8, 16, 512, 8192, False), (12, 16, 512, 8192, False), (16, 16, 512, 8192, False), (16, 16, 512, 16384, True),
+    (64, 16, 512, 4096, True), (64, 64, 512, 4096, False), (16, 64, 512, 32768, True), (16, 16, 256, 8192, False),
+    (16, 32, 256, 32768, True), (8, 32, 128, 16384, False), (64, 32, 128, 8192, True)])
+def test_wide_tables_share_where_that_gains(rows, heads, d, shared, gain):
+    """Tables of 65536 tokens, so that it is the plan that decides.  Measured, shared against not: 36.4 / 24.4, 38.4 /
+    36.3 (16 rows), 43 / 54, 44.5 / 54.8, 86 / 71, 101 / 115; 33 / 26, 49 / 59; 30.4 / 26, 41 / 58 us."""
+    c = Pieces([(shared, [random.Random(b).randint(1, 400) for b in range(rows)])], (), heads, d, 64, seed=rows)
+    c.table = torch.cat([c.table, c.table.new_full((rows, 1024 - c.table.shape[1]), -1)], 1)
+    assert shares(c) == gain
