@@ -253,6 +253,8 @@ def lib() -> ctypes.CDLL:
                 l.dsa_attn_paged_shares_keys.restype = ctypes.c_int
                 l.dsa_attn_shared.argtypes = [ctypes.POINTER(AttnSharedParams), _p]
                 l.dsa_attn_shared.restype = ctypes.c_int
+                l.dsa_attn_shared_looks.argtypes = [ctypes.POINTER(AttnSharedParams), ctypes.c_int]
+                l.dsa_attn_shared_looks.restype = ctypes.c_int
                 l.dsa_attn_shared_workspace_size.argtypes = [_i64] * 5
                 l.dsa_attn_shared_workspace_size.restype = _i64
                 l.dsa_rotary.argtypes = [ctypes.POINTER(RotaryParams), _p]

@@ -606,37 +606,46 @@ extern "C" int64_t dsa_attn_shared_workspace_size(int64_t batch, int64_t s1, int
   return most;
 }
 
+extern "C" int dsa_attn_shared_looks(const DsaAttnSharedParams* sp, int counted) {
+  using namespace dsa::attn_paged;
+  constexpr int64_t kMax = 0x7fffffff;
+  if (!sp) return 0;
+  const DsaAttnPagedParams* p = &sp->attn;
+  if (sp->groups < 1 || sp->groups > kMaxGroups || p->batch < 1 || p->s1 < 1 || p->n1 < 1 || p->n1 > 128 || p->batch > kMax ||
+      p->s1 > kMax || p->batch * p->s1 > kMax / p->n1 || p->page_size < 1 || p->max_blocks < 1 ||
+      p->max_blocks > (kMax - pair::kTile) / p->page_size)
+    return 0;
+  const Layout l = layout_of(p->batch, p->s1, p->n1, p->d, sp->groups, packs(p->s1, p->n1) && !counted);
+  // Calls that cannot save enough are left to the other operator, by what the tables hold: with one prefix
+  // of all their keys and a quarter to spare, as the plan, the pieces' launch and this join take 3 to 6 us more
+  // where nothing is shared (up to 25 with later tokens' keys or 64 heads of 64 rows).
+  const Kind own = kind_of(l.own_nh, p->d), pre = kind_of(l.nh, p->d);
+  const int64_t cap = p->max_blocks * p->page_size;
+  if (!can_share(l)) return 0;   // a token's heads fill a piece
+  const int64_t pieces = (p->batch * p->s1 + l.per_item - 1) / l.per_item;
+  const double most = (double)l.rest * ((cap >> own.shift) + 1) * own.cost * own.sms -
+                      (double)pieces * ((double)(cap >> pre.shift) * pre.cost + pre.piece) * pre.sms;
+  if (sp->least_saving > 0 && most <= 1.25 * (double)sp->least_saving) return 0;
+  // (places, units and the keys of a tile of 128 are counted in 32 bits)
+  const int64_t tiles = (cap + kTile - 1) / kTile + 8;
+  return l.most * l.nh <= kMax && l.most + l.rest <= kMax / tiles;
+}
+
 extern "C" int dsa_attn_shared(const DsaAttnSharedParams* sp, void* stream_) {
   using namespace dsa::attn_paged;
   if (!sp || sp->attn.batch < 0 || sp->attn.s1 < 0 || sp->groups < 0) return DSA_ERR_INVALID_ARG;
   const DsaAttnPagedParams* p = &sp->attn;
   if (p->batch == 0 || p->s1 == 0) return DSA_OK;
-  constexpr int64_t kMax = 0x7fffffff;
   if (!valid_params(p, kTile) || sp->groups > kMaxGroups || (sp->groups > 0 && (!sp->group_starts || !sp->prefix_lengths)) ||
       p->workspace_bytes < dsa_attn_shared_workspace_size(p->batch, p->s1, p->n1, p->d, sp->groups))
     return DSA_ERR_INVALID_ARG;
-  if (sp->groups > 0) {
-    const Layout l = layout_of(p->batch, p->s1, p->n1, p->d, sp->groups, packs(p->s1, p->n1) && !p->act_q);
-    // Calls that cannot save enough are left to the other operator, by what the tables hold: with one prefix
-    // of all their keys and a quarter to spare, as the plan, the pieces' launch and this join take 3 to 6 us more
-    // where nothing is shared (up to 25 with later tokens' keys or 64 heads of 64 rows).
-    const Kind own = kind_of(l.own_nh, p->d), pre = kind_of(l.nh, p->d);
-    const int64_t cap = p->max_blocks * p->page_size, pieces = (p->batch * p->s1 + l.per_item - 1) / l.per_item;
-    const double most = (double)l.rest * ((cap >> own.shift) + 1) * own.cost * own.sms -
-                        (double)pieces * ((double)(cap >> pre.shift) * pre.cost + pre.piece) * pre.sms;
-    const bool worth = sp->least_saving <= 0 || most > 1.25 * (double)sp->least_saving;
-    // (places, units and the keys of a tile of 128 are counted in 32 bits)
-    const int64_t tiles = (p->max_blocks * p->page_size + kTile - 1) / kTile + 8;
-    if (can_share(l) && worth && l.most * l.nh <= kMax && l.most + l.rest <= kMax / tiles &&
-        p->max_blocks * p->page_size <= kMax - pair::kTile) {
-      if (!one_matrix(p, p->q_head_stride, p->q_token_stride, p->q_batch_stride) ||
-          !one_matrix(p, p->qr_head_stride, p->qr_token_stride, p->qr_batch_stride) || l.shares < 1)
-        return DSA_ERR_INVALID_ARG;
-      if (p->dtype == DSA_DTYPE_BF16) return launch_shared_dim<__nv_bfloat16>(sp, l, static_cast<cudaStream_t>(stream_));
-      if (p->dtype == DSA_DTYPE_FP16) return launch_shared_dim<__half>(sp, l, static_cast<cudaStream_t>(stream_));
-      return DSA_ERR_INVALID_ARG;
-    }
-  }
-  // a token's heads fill a piece, there is no group, or the call is too small or too large: nothing to share
-  return dsa_attn_paged(p, stream_);
+  const int counted = p->act_q != nullptr;
+  if (!dsa_attn_shared_looks(sp, counted)) return dsa_attn_paged(p, stream_);
+  const Layout l = layout_of(p->batch, p->s1, p->n1, p->d, sp->groups, packs(p->s1, p->n1) && !counted);
+  if (!one_matrix(p, p->q_head_stride, p->q_token_stride, p->q_batch_stride) ||
+      !one_matrix(p, p->qr_head_stride, p->qr_token_stride, p->qr_batch_stride) || l.shares < 1)
+    return DSA_ERR_INVALID_ARG;
+  if (p->dtype == DSA_DTYPE_BF16) return launch_shared_dim<__nv_bfloat16>(sp, l, static_cast<cudaStream_t>(stream_));
+  if (p->dtype == DSA_DTYPE_FP16) return launch_shared_dim<__half>(sp, l, static_cast<cudaStream_t>(stream_));
+  return DSA_ERR_INVALID_ARG;
 }

@@ -198,13 +198,13 @@ def _one_matrix(t: torch.Tensor, strides):
 
 
 def _shared_plan(query, query_rope, key_cache, key_rope_cache, block_table, group_starts, prefix_lengths,
-                 scale_value, sparse_mode):
+                 scale_value, sparse_mode, counted=True):
     """As _plan, for flash_attention_shared_prefix."""
     for t, what in ((group_starts, "group_starts"), (prefix_lengths, "prefix_lengths")):
         if not torch.is_tensor(t) or t.dtype != torch.int32 or t.dim() != 1:
             raise ValueError(f"{what} must be an int32 tensor of 1 dim")
-    template, _, _, stat_shape, _ = _plan(query, query_rope, key_cache, key_rope_cache, block_table, scale_value,
-                                          sparse_mode, True)
+    template, q_fits, qr_fits, stat_shape, _ = _plan(query, query_rope, key_cache, key_rope_cache, block_table, scale_value,
+                                                     sparse_mode, counted)
     H.require_cuda(group_starts, prefix_lengths)
     if group_starts.device != query.device or prefix_lengths.device != query.device:
         raise ValueError("all tensors must be on one device")
@@ -216,17 +216,15 @@ def _shared_plan(query, query_rope, key_cache, key_rope_cache, block_table, grou
     p.attn = AttnPagedParams.from_buffer_copy(template)
     B, S1, N1, D = query.shape
     p.groups, p.least_saving = groups, _LEAST_SAVING * _LEAST_TIMES[D]
-    # pieces of a prefix are runs of heads of neighbouring tokens; queries that lie otherwise are copied
-    fits = []
-    for t, name, width in ((query, "q", D), (query_rope, "qr", _D_ROPE)):
-        st = _tma_strides(t)
-        fits.append(st is not None and (N1 > 64 or _one_matrix(t, st)))
-        if not fits[-1]:
-            p_strides = (S1 * N1 * width, N1 * width, width)
-            for dim, v in zip(("batch", "token", "head"), p_strides):
-                setattr(p.attn, f"{name}_{dim}_stride", v)
+    if lib().dsa_attn_shared_looks(p, counted):
+        # pieces of a prefix are runs of heads of neighbouring tokens; queries that lie otherwise are copied
+        qs, qrs = _tma_strides(query), _tma_strides(query_rope)
+        q_fits, qr_fits = [st is not None and _one_matrix(t, st) for t, st in ((query, qs), (query_rope, qrs))]
+        contiguous = lambda w: (S1 * N1 * w, N1 * w, w)
+        p.attn.q_batch_stride, p.attn.q_token_stride, p.attn.q_head_stride = qs if q_fits else contiguous(D)
+        p.attn.qr_batch_stride, p.attn.qr_token_stride, p.attn.qr_head_stride = qrs if qr_fits else contiguous(_D_ROPE)
     p.attn.workspace_bytes = lib().dsa_attn_shared_workspace_size(B, S1, N1, D, groups)
-    return bytes(p), fits[0], fits[1], stat_shape, max(p.attn.workspace_bytes, 16)
+    return bytes(p), q_fits, qr_fits, stat_shape, max(p.attn.workspace_bytes, 16)
 
 
 def flash_attention_shared_prefix(
@@ -275,7 +273,7 @@ def flash_attention_shared_prefix(
                                                  group_starts, prefix_lengths, actual_seq_lengths_key, scale_value,
                                                  actual_seq_lengths_query, sparse_mode, return_softmax_lse)
     plan = _shared_plan(query, query_rope, key_cache, key_rope_cache, block_table, group_starts, prefix_lengths,
-                        float(scale_value), sparse_mode)
+                        float(scale_value), sparse_mode, actual_seq_lengths_query is not None)
     template, q_fits, qr_fits, _, ws_bytes = plan
     p = AttnSharedParams.from_buffer_copy(template)
     starts, prefixes = group_starts.contiguous(), prefix_lengths.contiguous()

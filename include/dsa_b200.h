@@ -478,6 +478,9 @@ typedef struct DsaAttnSharedParams {
 } DsaAttnSharedParams;
 
 int dsa_attn_shared(const DsaAttnSharedParams* params, void* stream);
+/* 1 where a call of these sizes looks at its groups, and its queries have to lie so; 0 where it is
+ * dsa_attn_paged's whatever they are.  Reads the sizes, groups and least_saving; counted: with act_q. */
+int dsa_attn_shared_looks(const DsaAttnSharedParams* params, int counted);
 int64_t dsa_attn_shared_workspace_size(int64_t batch, int64_t s1, int64_t n1, int64_t d, int64_t groups);
 
 /*

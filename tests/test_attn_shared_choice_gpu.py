@@ -3,12 +3,14 @@
 As in test_attn_shared_pieces_gpu.py, all rows of a group but the first with keys name a page of NaN in
 the prefix: a call that shares it gives the group's result, one that does not gives NaN in those rows.
 """
+import importlib
 import random
 
 import pytest
 import torch
 
 import dsa_triton_ascend_b200 as dsa
+from test_attn_shared_gpu import Shared
 from test_attn_shared_pieces_gpu import Pieces
 
 pytestmark = pytest.mark.gpu
@@ -73,3 +75,20 @@ def test_wide_tables_share_where_that_gains(rows, heads, d, shared, gain):
     c = Pieces([(shared, [random.Random(b).randint(1, 400) for b in range(rows)])], (), heads, d, 64, seed=rows)
     c.table = torch.cat([c.table, c.table.new_full((rows, 1024 - c.table.shape[1]), -1)], 1)
     assert shares(c) == gain
+
+
+@pytest.mark.parametrize("s1,heads,act_q", [(1, 16, None), (3, 16, [3, 1, 2]), (1, 128, None), (12, 8, None)])
+def test_queries_of_a_call_that_shares_nothing_are_not_copied(s1, heads, act_q, monkeypatch):
+    """Small tables, or more heads than a piece takes: flash_attention_paged's call, whose queries may lie as TMA
+    reads them."""
+    module = importlib.import_module("dsa_triton_ascend_b200.flash_attention_paged")
+    c = Shared([(130, [64, 33, 7])], (), heads, 512, 64, s1=s1, seed=8)
+    wide = torch.zeros(3, s1 + 2, heads + 1, 640, device="cuda", dtype=torch.bfloat16)
+    q, qr = wide[:, 1:s1 + 1, 1:, :512], wide[:, 1:s1 + 1, 1:, 512:576]
+    q.copy_(c.q)
+    qr.copy_(c.qr)
+    c.q, c.qr = q, qr
+    monkeypatch.setattr(module, "_copied", lambda t: pytest.fail("copied"))
+    got = c.run(3, act_q=act_q)
+    same = dsa.flash_attention_paged(q, qr, c.kc, c.krc, c.table, c.lens, c.scale, act_q, 3, True)
+    assert all(torch.equal(x, y) for x, y in zip(got, same))
