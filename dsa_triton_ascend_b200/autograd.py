@@ -202,6 +202,7 @@ class RotaryEmbeddingAxesFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, table, positions, sections, layout="interleaved", order="blocks", offset=0, inverse=False):
         ctx.save_for_backward(table, positions)
+        sections = tuple(sections) if hasattr(sections, "__iter__") else sections   # the caller's may change
         ctx.cfg = (sections, layout, order, offset, inverse)
         return rotary_embedding_axes(x, table, positions, *ctx.cfg)
 
