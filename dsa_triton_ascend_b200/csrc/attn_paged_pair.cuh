@@ -137,10 +137,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&maps.qr);
   }
   Work work = share_of<kTile, kSegmentCost, kThreads>(a, blockIdx.x >> 1, gridDim.x >> 1, blockIdx.x == 0, tmp, start);
+  release_next<false>(a);
   tc_fence_before();
   __syncthreads();
   cluster_sync();
-  griddep_launch_dependents();   // with this CTA's tensor memory taken: the next kernel may take some before it waits
+  release_next<true>(a);
   tc_fence_after();
   const uint32_t tmem = *tmem_ptr;
   bool failed = false;

@@ -128,9 +128,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&maps.qr);
   }
   Work work = share_of<kTile, kSegmentCost, kThreads>(a, blockIdx.x, gridDim.x, blockIdx.x == 0, tmp, start);
+  release_next<false>(a);
   tc_fence_before();
   __syncthreads();
-  griddep_launch_dependents();   // with this CTA's tensor memory taken: the next kernel may take some before it waits
+  release_next<true>(a);
   tc_fence_after();
   const uint32_t tmem = *tmem_ptr;
   bool failed = false;

@@ -43,7 +43,12 @@ def test_nothing_is_read_before_the_wait(name, count):
 
 @pytest.mark.parametrize("name", ["attn_paged_heads.cuh", "attn_paged_pair.cuh", "attn_paged_wide.cuh"])
 def test_the_next_kernel_starts_behind_the_tensor_memory(name):
-    """A kernel that waits for this one with tensor memory of its own must not have taken it first."""
+    """A kernel that waits for this one with tensor memory of its own must not have taken it first.  (With
+    Args the next one is a join, which takes none.)"""
     (_, body), = kernels(name)
     alloc, barrier = body.index("tmem_alloc<"), body.index("__syncthreads();")
-    assert alloc < barrier < body.index("griddep_launch_dependents();")
+    assert alloc < barrier < body.index("release_next<true>(a);") and "griddep_launch_dependents" not in body
+    with open(os.path.join(CSRC, "attn_paged.cuh")) as f:
+        text = f.read()
+    items = re.search(r"release_next\(const ItemArgs&\) \{([^}]*)\}", text).group(1)
+    assert items.strip() == "if (kBehind) griddep_launch_dependents();"
