@@ -16,10 +16,11 @@
 // many as all of its rows see, where that costs less than its rows by themselves.
 //
 // Measured (against attn_paged.cu alone): 64 rows of 16 heads, D = 512, with 32811 shared and 17 to 2048 own
-// keys, 119 us against 309; 84 rows of 20 heads in five groups, 9 of them alone, 82 against 98; 24 rows x 2 tokens
-// of 32 heads, D = 256, in two groups, 56 against 55.  The pair kernel's tile of 128 keys and 128 heads takes 3,645
-// cycles, 2,176 of them products.  (Beside one another, the second launch reading the plan before a wait of its
-// own, the two took 108, 72 and 47.)
+// keys, 118.5 us against 309; 84 rows of 20 heads in five groups, 9 of them alone, 82 against 98; 64 rows x 5 tokens
+// of 16 heads, D = 512, with 32768 shared keys, 389 against 511; 24 rows x 2 tokens of 32 heads, D = 256, in two groups
+// save too little and go to attn_paged.cu (52).  Of the 118.5: plan 5, pieces 80, rests 24, join 10.  The pair kernel's
+// tile of 128 keys and 128 heads takes 3,645 cycles, 2,176 of them products.  (Beside one another, the second launch
+// reading the plan before a wait of its own, the two took 108 in all; 72 in the five groups, 47 for the drafted tokens.)
 #include <cuda_runtime.h>
 
 #include <type_traits>
@@ -457,7 +458,7 @@ bool can_share(const Layout& l) { return l.per_item > l.packed; }
 
 // The kernel for `nh` heads, in cycles: a tile (the slope over rows of 4096 and 12288 keys, or prefixes of
 // 16384 and 49152, that lie in L2), and the start and end of a piece with its parts in the join (what rows of
-// 400 and 1100 keys take beyond their tiles; of 128 heads at D >= 256 what fits 350 calls of 4 to 64 rows over 1024
+// 400 and 1100 keys take beyond their tiles; of 128 heads at D >= 256 what fits 400 calls of 4 to 64 rows over 1024
 // to 32768 shared keys best).
 Kind kind_of(int nh, int64_t d) {
   if (nh == 128 && d == 512) return {7, pair::kSegmentCost, 2, 4350, 37000};

@@ -9,8 +9,9 @@
 // Two launches: plan_rows_kernel, over the whole GPU, in which some blocks write the tokens' lists (each
 // finds its tokens' requests by a scan of the counts of its own, up to the last it needs), the others
 // the block table's rows and how many pages each has in common with the row before it; and
-// plan_groups_kernel, one block beside it: lengths and ends, then the groups.  A small step (up to 112
-// turns of a warp and 6144 tokens) is one launch of a cluster that does both.  Bound by latency, of a chain of
+// plan_groups_kernel, one block behind it: lengths and ends, then the groups.  A small step is one launch of a
+// cluster of eight that does both: a CTA for the groups, one for each 1024 tokens, at least one for the rows, whose
+// warps have two turns each at most (32 requests with tables of up to 256 blocks and a token each take 64 of 96 turns).  Bound by latency, of a chain of
 // dependent loads (slot, length, page), and the host: 32 requests, tables of 64 blocks, 7.6 us a call against 9.5
 // with two launches (the kernel 4.2, replayed one behind another 6.2 against 6.4); 509 requests, tables of
 // 512 blocks, 9.6 a call (10.4 replayed).

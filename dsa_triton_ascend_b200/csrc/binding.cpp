@@ -5,7 +5,7 @@
 // then kept here under that signature, and a call whose signature is known allocates its
 // outputs, puts in the addresses and calls the library: 3 us for a store, 5 for a rotation or an append, 8 to
 // 9 for a plan, 11 for upkeep, 13 for attention, 16 with a shared prefix (four launches), instead of
-// 17 to 70 (attention 39).  Any other call (a new signature,
+// 17 to 70 (attention 39).  The number of packed tokens is part of a signature, but for a plan's.  Any other call (a new signature,
 // another current device, an address that is not aligned) is answered with None and takes the
 // Python path.  Nothing is kept by address.
 #define PY_SSIZE_T_CLEAN

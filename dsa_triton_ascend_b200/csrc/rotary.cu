@@ -10,7 +10,8 @@
 // rotated, in 45.6 us, 5.9 TB/s (49.5 with blocks of 256 threads, 51.5 with both pieces in a
 // thread, 62 with two heads a thread).
 // With positions of several axes a pair takes its angle from its axis' row of the table (the same kernels,
-// bound by memory as well): the same two tensors in 42.3 us (three axes in blocks) and 46 (axes in turn).
+// bound by memory as well): the same two tensors in 42.3 us (three axes in blocks) and 46 (axes in
+// turn; 42.5 called back to back).
 #include <cuda_runtime.h>
 
 #include <type_traits>
@@ -25,7 +26,7 @@ constexpr int kThreads = 128;
 constexpr int kMaxPairs = 128;
 
 // Heads of a thread: 4, or 8 where a thread fetches the angles of several axes (8186 tokens x 64 heads x
-// 128, half layout, axes in turn: 44.0 us against 49.7 with 4; with one axis both take 45.5).
+// 128, half layout, axes in turn, called back to back: 42.5 us against 48.0 with 4; with one axis both take 45.5).
 struct Args {
   static constexpr int kHeads = 4;
   const void* x;

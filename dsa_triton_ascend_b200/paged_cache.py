@@ -453,7 +453,8 @@ def paged_batch_plan(block_table, seq_lengths, rows, counts, page_size, num_toke
 
     A request that cannot be (a slot out of range, a count past its length) has length 0, and its tokens
     keep their places, with -1, 0 and -1 as behind the last; a token without a page has slot -1, and tokens
-    past ``num_tokens`` are left out; all are reported by ``check_device_errors``.
+    past ``num_tokens`` are left out; all are reported by ``check_device_errors``.  A slot that is in ``rows``
+    twice with new tokens gives them the same places of the cache twice, which ``paged_cache_store`` does not take.
     """
     page_size, num_tokens, min_prefix = int(page_size), int(num_tokens), int(min_prefix)
     if max_groups is None:
